@@ -42,6 +42,7 @@ extern "C" {
 #define SPCONV_STATUS_TABLE_FULL 2    /* a probe sequence visited every slot */
 #define SPCONV_STATUS_DUPLICATE 4     /* a coordinate occurs twice; the highest row is kept */
 #define SPCONV_STATUS_WAIT_TIMEOUT 8  /* a kernel-internal wait hit its time limit */
+#define SPCONV_STATUS_OFFSETS 16      /* sample offsets that do not ascend from 0 to the row count */
 
 /* Feature dtypes. */
 #define SPCONV_F32 0
@@ -278,6 +279,106 @@ int spconv_submanifold_conv_weight_grad(
     int kernel_volume, const int32_t *neighbor_map, const uint32_t *masks, const int32_t *order,
     float *grad_weight, float *grad_bias, void *workspace, int64_t workspace_bytes,
     int32_t *status, void *stream);
+
+/* Pointwise (1x1x1) linear layer over voxel features:
+ *   out[i, co] = residual[i, co] + act(bias[co] + sum_ci feats[i, ci] * weight[co, ci])
+ * accumulated in fp32 and rounded once to `dtype`.
+ *   feats [M, Ci], weight [Co, Ci], bias [Co] or NULL, residual [M, Co] or NULL, out [M, Co]: in
+ *   dtype, row-major; preact [M, Co] in dtype, or NULL: also receives act's argument, which the
+ *   backward needs for every activation but SPCONV_ACT_NONE
+ *   out may be residual itself (each element is read before it is written); it may not otherwise
+ *   overlap an input
+ *   kernel_choice: SPCONV_KERNEL_*; SPCONV_KERNEL_TCGEN05 returns SPCONV_ERR_UNSUPPORTED where the
+ *   tensor-core kernel does not apply (fp32, channel counts that are no multiple of 8, pointers
+ *   not aligned to 16 bytes)
+ * No counterpart in the reference (its networks would call torch for this layer). */
+#define SPCONV_ACT_NONE 0
+#define SPCONV_ACT_RELU 1
+#define SPCONV_ACT_GELU 2             /* x * Phi(x), Phi the normal distribution function */
+#define SPCONV_ACT_SILU 3             /* x / (1 + exp(-x)) */
+int spconv_linear_forward(const void *feats, int dtype, int64_t num_rows, int Ci, const void *weight,
+                          const void *bias, const void *residual, int Co, int activation,
+                          void *out, void *preact, int kernel_choice, int32_t *status, void *stream);
+
+/* Gradients of spconv_linear_forward, with dz = grad_out * act'(preact) rounded to `dtype`:
+ *   grad_feats[i, ci] = sum_co dz[i, co] * weight[co, ci]
+ *   grad_weight[co, ci] = sum_i dz[i, co] * feats[i, ci];  grad_bias[co] = sum_i dz[i, co]
+ * (the residual's gradient is grad_out). Sums are fp32, the same in every run. Each output may be
+ * NULL; grad_feats is in dtype, grad_weight in weight_dtype and grad_bias in bias_dtype, each
+ * SPCONV_F32 or dtype. preact may be NULL for SPCONV_ACT_NONE.
+ *   workspace: 256-byte aligned, spconv_linear_backward_workspace_bytes(...) bytes. */
+int64_t spconv_linear_backward_workspace_bytes(int dtype, int64_t num_rows, int Ci, int Co, int activation);
+int spconv_linear_backward(const void *grad_out, const void *preact, const void *feats, const void *weight,
+                           int dtype, int64_t num_rows, int Ci, int Co, int activation,
+                           void *grad_feats, void *grad_weight, int weight_dtype, void *grad_bias,
+                           int bias_dtype, void *workspace, int64_t workspace_bytes, int kernel_choice,
+                           int32_t *status, void *stream);
+
+/* The gated residual step between two blocks with a norm on either side:
+ *   u = N1(feats) * weight + bias;  hidden = residual_scale * residual + gate * u
+ *   normed = N2(hidden) * next_weight + next_bias
+ * N1 = norm, N2 = next_norm: SPCONV_NORM_LAYER ((t - mean) / sqrt(var + eps)), SPCONV_NORM_RMS
+ * (t / sqrt(mean(t^2) + eps)) or SPCONV_NORM_NONE (N1: t itself; N2: no `normed`). An absent
+ * (NULL) parameter counts as 1 (gate, weights) or 0 (biases), an absent residual as 0.
+ * A parameter is one row of `channels` values, or one row per sample of the batch (per_sample);
+ * then `offsets` [num_samples + 1] int32 on the device holds each sample's first row, ascending
+ * from 0 to num_rows (anything else sets SPCONV_STATUS_OFFSETS; every row is still assigned to a
+ * sample inside the range). channels <= 8192, num_samples <= 65535, num_rows < 2^31.
+ * hidden may be residual or feats itself and normed may be feats itself (a row is read before it
+ * is written); outputs may not otherwise overlap inputs or each other.
+ * The backward takes the forward's inputs (not its outputs), grad_hidden and / or grad_normed,
+ * and writes grad_feats, grad_residual and each parameter's `grad` where not NULL, the latter in
+ * the parameter's type and shape, the same bits in every run; its outputs overlap no input.
+ *   workspace (backward, if a parameter's gradient is wanted): 16-byte aligned,
+ *   spconv_residual_norm_workspace_bytes(num_rows, channels, num_samples) bytes.
+ * No counterpart in the reference. */
+#define SPCONV_NORM_NONE 0
+#define SPCONV_NORM_LAYER 1
+#define SPCONV_NORM_RMS 2
+typedef struct {
+    const void *data;                 /* NULL: absent */
+    void *grad;                       /* backward output, NULL: not wanted */
+    int dtype;                        /* SPCONV_F32 or the features' type */
+    int per_sample;                   /* 1: [num_samples, channels], 0: [channels] */
+} spconv_channel_param;
+typedef struct {
+    int dtype;                        /* features, residual, outputs and their gradients */
+    int channels;
+    int64_t num_rows;
+    const void *feats, *residual;
+    void *hidden, *normed;
+    const void *grad_hidden, *grad_normed;
+    void *grad_feats, *grad_residual;
+    spconv_channel_param gate, weight, bias, next_weight, next_bias;
+    const int32_t *offsets;
+    int num_samples;
+    int norm, next_norm;
+    float residual_scale, eps;
+    void *workspace;
+    int64_t workspace_bytes;
+    int32_t *status;
+} spconv_residual_norm_args;
+int64_t spconv_residual_norm_workspace_bytes(int64_t num_rows, int channels, int num_samples);
+int spconv_residual_norm_forward(const spconv_residual_norm_args *args, void *stream);
+int spconv_residual_norm_backward(const spconv_residual_norm_args *args, void *stream);
+
+/* Global norm of many gradient tensors, and clipping by it:
+ *   total = sqrt(sum of all squares) (SPCONV_CLIP_P2) or the largest magnitude (SPCONV_CLIP_INF)
+ *   outs[k] = grads[k] * min(1, max_norm / (total + 1e-6))
+ * grads / outs: num_tensors device pointers (the arrays themselves are host memory, read before
+ * the call returns), numels elements of type dtypes[k] each, contiguous, of any alignment.
+ * outs[k] may be grads[k] (in place; nothing is then written while the factor is 1). An output
+ * that shares memory with another output or gradient is refused. total_norm: device float. A
+ * norm that is not finite gives the factor of the formula (0 or NaN). The squares are summed in
+ * fp64, the same bits in every run.
+ *   workspace: 8-byte aligned, spconv_clip_gradients_workspace_bytes(num_tensors) bytes.
+ * No counterpart in the reference. */
+#define SPCONV_CLIP_P2 0
+#define SPCONV_CLIP_INF 1
+int64_t spconv_clip_gradients_workspace_bytes(int num_tensors);
+int spconv_clip_gradients(const void *const *grads, void *const *outs, const int64_t *numels,
+                          const int32_t *dtypes, int num_tensors, int norm_kind, float max_norm,
+                          float *total_norm, void *workspace, int64_t workspace_bytes, void *stream);
 
 /* Stage timing, for profiling and for the benchmark's roofline figures.
  * spconv_stage_timing(max_calls > 0) creates CUDA events on the current device for

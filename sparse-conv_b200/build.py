@@ -14,6 +14,7 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -49,7 +50,7 @@ def build(force: bool = False, verbose: bool = False, extra_flags=None) -> str:
     os.makedirs(LIB_DIR, exist_ok=True)
     sources = sorted(f for f in os.listdir(CSRC) if f.endswith(".cu"))
     dep_t = _deps_mtime()
-    objs = []
+    objs, todo = [], []
     changed = force or not os.path.exists(LIB_PATH)
     flags = NVCC_FLAGS + list(extra_flags or [])
     for src in sources:
@@ -62,8 +63,10 @@ def build(force: bool = False, verbose: bool = False, extra_flags=None) -> str:
         cmd = [nvcc()] + flags + ["-I", INCLUDE, "-c", sp, "-o", op]
         if verbose:
             print(" ".join(cmd), flush=True)
-        subprocess.check_call(cmd)
+        todo.append(cmd)
         changed = True
+    with ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as pool:
+        list(pool.map(subprocess.check_call, todo))
     if changed or any(os.path.getmtime(o) > os.path.getmtime(LIB_PATH) for o in objs):
         tmp = LIB_PATH + ".tmp"
         cmd = [nvcc(), "-shared", "-gencode", "arch=compute_100a,code=sm_100a",

@@ -1,0 +1,398 @@
+// Pointwise linear layer over voxel features and its gradients:
+//
+//   out = residual + act(z),  z = feats W^T + bias          feats [M, Ci], W [Co, Ci]
+//   dz = grad_out * act'(z);  grad_feats = dz W;  grad_W = dz^T feats;  grad_bias = sum dz
+//
+// This file holds the CUDA-core product (exact fp32 FMAs; fp32 features, odd channel counts,
+// unaligned pointers), the activation's backward with the bias sums, the sum over splits, and
+// the entry points.
+#include <algorithm>
+#include <type_traits>
+
+#include "activation.cuh"
+#include "common.cuh"
+#include "linear_internal.h"
+
+namespace spconv {
+
+constexpr int kSimtThreads = 256, kSimtBK = 16;
+
+// Reads rows x BK elements of an operand (K contiguous unless T_) into registers and stores them
+// as [k][row] fp32 in shared memory.
+template <typename T, int ROWS, bool T_>
+struct SimtTile {
+    static constexpr int kPer = (ROWS * kSimtBK + kSimtThreads - 1) / kSimtThreads;
+    float v[kPer];
+    __device__ __forceinline__ static void place(int i, int &row, int &k) {
+        if constexpr (T_) { row = i % ROWS; k = i / ROWS; }       // neighbours along the rows
+        else { k = i % kSimtBK; row = i / kSimtBK; }              // neighbours along K
+    }
+    __device__ __forceinline__ void load(const T *p, int64_t rows, int64_t row0, int64_t k0, int64_t k_end, int64_t ld) {
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+            const int i = threadIdx.x + j * kSimtThreads;
+            int r, k;
+            place(i, r, k);
+            v[j] = 0.f;
+            if (i < ROWS * kSimtBK && row0 + r < rows && k0 + k < k_end)
+                v[j] = dtype_traits<T>::to_f(T_ ? p[(k0 + k) * ld + row0 + r] : p[(row0 + r) * ld + k0 + k]);
+        }
+    }
+    __device__ __forceinline__ void store(float (*s)[ROWS + 4]) const {
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+            const int i = threadIdx.x + j * kSimtThreads;
+            int r, k;
+            place(i, r, k);
+            if (i < ROWS * kSimtBK) s[k][r] = v[j];
+        }
+    }
+};
+
+// out[m, n] = epilogue(sum_k A(m, k) B(n, k)): BM x BN outputs per block, TM x TN per thread,
+// K in steps of 16 through two shared-memory buffers; the next step's global loads run under
+// the current step's FMAs. blockIdx.z is the split of K.
+template <typename T, int BM, int BN, int TM, int TN, bool AT, bool BT, int ACT>
+__global__ void __launch_bounds__(kSimtThreads)
+linear_simt_kernel(GemmArgs g) {
+    static_assert(BM * BN == TM * TN * kSimtThreads, "threads cover the tile");
+    __shared__ float sa[2][kSimtBK][BM + 4], sb[2][kSimtBK][BN + 4];
+    const T *a = (const T *)g.a, *b = (const T *)g.b;
+    const int64_t m0 = (int64_t)blockIdx.x * BM, n0 = (int64_t)blockIdx.y * BN;
+    const int64_t k_begin = g.splits > 1 ? blockIdx.z * g.k_per_split : 0;
+    const int64_t k_end = g.splits > 1 ? min(g.K, k_begin + g.k_per_split) : g.K;
+    const int64_t lda = AT ? g.M : g.K, ldb = BT ? g.N : g.K;
+    const int tn = threadIdx.x % (BN / TN), tm = threadIdx.x / (BN / TN);
+    float acc[TM][TN] = {};
+    SimtTile<T, BM, AT> ta;
+    SimtTile<T, BN, BT> tb;
+    ta.load(a, g.M, m0, k_begin, k_end, lda);
+    tb.load(b, g.N, n0, k_begin, k_end, ldb);
+    int buf = 0;
+    for (int64_t k = k_begin; k < k_end; k += kSimtBK, buf ^= 1) {
+        ta.store(sa[buf]);
+        tb.store(sb[buf]);
+        __syncthreads();
+        if (k + kSimtBK < k_end) {
+            ta.load(a, g.M, m0, k + kSimtBK, k_end, lda);
+            tb.load(b, g.N, n0, k + kSimtBK, k_end, ldb);
+        }
+#pragma unroll
+        for (int kk = 0; kk < kSimtBK; ++kk) {
+            float fa[TM], fb[TN];
+#pragma unroll
+            for (int i = 0; i < TM; ++i) fa[i] = sa[buf][kk][tm * TM + i];
+#pragma unroll
+            for (int j = 0; j < TN; ++j) fb[j] = sb[buf][kk][tn * TN + j];
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j) acc[i][j] = fmaf(fa[i], fb[j], acc[i][j]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+        const int64_t m = m0 + tm * TM + i;
+        if (m >= g.M) continue;
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+            const int64_t n = n0 + tn * TN + j;
+            if (n >= g.N) continue;
+            const int64_t at = m * g.N + n;
+            float z = acc[i][j];
+            if (g.partial) {
+                g.partial[(int64_t)blockIdx.z * g.M * g.N + at] = z;
+                continue;
+            }
+            if (g.bias) z += dtype_traits<T>::to_f(((const T *)g.bias)[n]);
+            if (g.preact) ((T *)g.preact)[at] = dtype_traits<T>::from_f(z);
+            z = act_value<ACT>(z);
+            if (g.residual) z += dtype_traits<T>::to_f(((const T *)g.residual)[at]);
+            ((T *)g.out)[at] = dtype_traits<T>::from_f(z);
+        }
+    }
+}
+
+template <typename T, bool AT, bool BT, int ACT>
+static int simt_shape(const GemmArgs &g) {
+    auto run = [&](auto kern, int bm, int bn) {
+        const int64_t gx = (g.M + bm - 1) / bm, gy = (g.N + bn - 1) / bn;
+        kern<<<dim3((unsigned)gx, (unsigned)gy, (unsigned)g.splits), kSimtThreads, 0, g.stream>>>(g);
+        return check_launch("linear_simt_kernel");
+    };
+    // narrow outputs (class scores) leave three quarters of a 64-wide tile idle
+    if (g.N <= 16) return run(linear_simt_kernel<T, 128, 16, 4, 2, AT, BT, ACT>, 128, 16);
+    if (g.M <= 16) return run(linear_simt_kernel<T, 16, 128, 2, 4, AT, BT, ACT>, 16, 128);
+    return run(linear_simt_kernel<T, 128, 64, 8, 4, AT, BT, ACT>, 128, 64);
+}
+
+template <typename T>
+static int simt_type(const GemmArgs &g) {
+    if (g.a_t) return simt_shape<T, true, true, SPCONV_ACT_NONE>(g);       // weight gradient
+    if (g.b_t) return simt_shape<T, false, true, SPCONV_ACT_NONE>(g);      // input gradient
+    return act_dispatch(g.activation, [&](auto act) { return simt_shape<T, false, false, act.value>(g); });
+}
+
+int launch_gemm_simt(const GemmArgs &g) {
+    if (g.dtype == SPCONV_F32) return simt_type<float>(g);
+    if (g.dtype == SPCONV_F16) return simt_type<__half>(g);
+    return simt_type<__nv_bfloat16>(g);
+}
+
+// ---------------------------------------------------------------------------------------
+// dz = grad_out * act'(z), and its column sums. One read of each input, one write of dz; a lane
+// owns VEC neighbouring columns of a 32 * VEC column tile and walks the chunk's rows, so the
+// sums stay in registers; partial[chunk][Co] holds them per block.
+// ---------------------------------------------------------------------------------------
+constexpr int kDactThreads = 256;
+
+template <typename T, int VEC, int ACT>
+__global__ void __launch_bounds__(kDactThreads)
+linear_dact_kernel(const T *__restrict__ gout, const T *__restrict__ z, T *__restrict__ dz, float *__restrict__ partial,
+                   int64_t M, int Co, int lpr, int64_t chunk) {
+    __shared__ float part[kDactThreads / 32][32 * VEC];
+    const int lane = threadIdx.x & (lpr - 1), group = threadIdx.x / lpr, groups = kDactThreads / lpr;
+    const int col = (blockIdx.y * 32 + lane) * VEC;
+    const bool have = col < Co;
+    const int64_t row0 = (int64_t)blockIdx.x * chunk, row1 = min(M, row0 + chunk);
+    float acc[VEC] = {};
+    if (have) {
+#pragma unroll 4
+        for (int64_t r = row0 + group; r < row1; r += groups) {
+            const int64_t at = r * Co + col;
+            alignas(16) T gv[VEC], zv[VEC];
+            if constexpr (VEC > 1) {
+                *reinterpret_cast<uint4 *>(gv) = __ldg(reinterpret_cast<const uint4 *>(gout + at));
+                if constexpr (ACT != SPCONV_ACT_NONE) *reinterpret_cast<uint4 *>(zv) = __ldcs(reinterpret_cast<const uint4 *>(z + at));
+            } else {
+                gv[0] = gout[at];
+                if constexpr (ACT != SPCONV_ACT_NONE) zv[0] = z[at];
+            }
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                float d = dtype_traits<T>::to_f(gv[i]);
+                if constexpr (ACT != SPCONV_ACT_NONE) {
+                    d *= act_slope<ACT>(dtype_traits<T>::to_f(zv[i]));
+                    gv[i] = dtype_traits<T>::from_f(d);
+                }
+                acc[i] += d;                 // the bias sums take dz before it is rounded
+            }
+            if constexpr (ACT != SPCONV_ACT_NONE) {
+                if constexpr (VEC > 1) *reinterpret_cast<uint4 *>(dz + at) = *reinterpret_cast<uint4 *>(gv);
+                else dz[at] = gv[0];
+            }
+        }
+    }
+    if (!partial) return;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i)
+        for (int o = lpr; o < 32; o <<= 1) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], o);
+    if ((threadIdx.x & 31) < lpr) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) part[threadIdx.x >> 5][lane * VEC + i] = acc[i];
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < lpr * VEC; i += kDactThreads) {
+        const int c = blockIdx.y * 32 * VEC + i;
+        if (c >= Co) continue;
+        float v = 0.f;
+#pragma unroll
+        for (int w = 0; w < kDactThreads / 32; ++w) v += part[w][i];
+        partial[(int64_t)blockIdx.x * Co + c] = v;
+    }
+}
+
+// out[i] = sum over s of partial[s][i], in the order of s within 8 lanes of splits.
+template <typename T>
+__global__ void __launch_bounds__(256)
+linear_reduce_kernel(const float *__restrict__ partial, int splits, int64_t n, T *__restrict__ out) {
+    __shared__ float part[8][33];
+    const int64_t i = (int64_t)blockIdx.x * 32 + threadIdx.x;
+    float v = 0.f;
+    if (i < n)
+        for (int s = threadIdx.y; s < splits; s += 8) v += __ldcs(partial + (int64_t)s * n + i);
+    part[threadIdx.y][threadIdx.x] = v;
+    __syncthreads();
+    if (threadIdx.y == 0 && i < n) {
+        float sum = 0.f;
+#pragma unroll
+        for (int y = 0; y < 8; ++y) sum += part[y][threadIdx.x];
+        out[i] = dtype_traits<T>::from_f(sum);
+    }
+}
+
+static int launch_reduce(const float *partial, int splits, int64_t n, int out_dtype, void *out, cudaStream_t st) {
+    const dim3 grid((unsigned)((n + 31) / 32)), block(32, 8);
+    if (out_dtype == SPCONV_F32) linear_reduce_kernel<float><<<grid, block, 0, st>>>(partial, splits, n, (float *)out);
+    else if (out_dtype == SPCONV_F16) linear_reduce_kernel<__half><<<grid, block, 0, st>>>(partial, splits, n, (__half *)out);
+    else linear_reduce_kernel<__nv_bfloat16><<<grid, block, 0, st>>>(partial, splits, n, (__nv_bfloat16 *)out);
+    return check_launch("linear_reduce_kernel");
+}
+
+// Row chunks of the dz / bias pass: about four blocks per SM, at least 32 rows each.
+static int dact_chunks(int64_t M) { return (int)std::max<int64_t>(1, std::min<int64_t>(148 * 4, (M + 31) / 32)); }
+
+template <typename T, int VEC>
+static int dact_vec(const void *gout, const void *z, void *dz, float *partial, int64_t M, int Co, int activation,
+                    cudaStream_t st) {
+    const int vecs = (Co + VEC - 1) / VEC;
+    int lpr = 1;
+    while (lpr < vecs && lpr < 32) lpr <<= 1;
+    const int chunks = dact_chunks(M);
+    const dim3 grid(chunks, (vecs + 31) / 32);
+    const int64_t chunk = (M + chunks - 1) / chunks;
+    return act_dispatch(activation, [&](auto act) {
+        linear_dact_kernel<T, VEC, act.value><<<grid, kDactThreads, 0, st>>>((const T *)gout, (const T *)z, (T *)dz,
+                                                                            partial, M, Co, lpr, chunk);
+        return check_launch("linear_dact_kernel");
+    });
+}
+
+template <typename T>
+static int dact_type(const void *gout, const void *z, void *dz, float *partial, int64_t M, int Co, int activation,
+                     cudaStream_t st) {
+    constexpr int V = 16 / (int)sizeof(T);
+    const bool vec = Co % V == 0 && (((uintptr_t)gout | (uintptr_t)z | (uintptr_t)dz) & 15) == 0;
+    return vec ? dact_vec<T, V>(gout, z, dz, partial, M, Co, activation, st)
+               : dact_vec<T, 1>(gout, z, dz, partial, M, Co, activation, st);
+}
+
+static int launch_dact(int dtype, const void *gout, const void *z, void *dz, float *partial, int64_t M, int Co,
+                       int activation, cudaStream_t st) {
+    if (dtype == SPCONV_F32) return dact_type<float>(gout, z, dz, partial, M, Co, activation, st);
+    if (dtype == SPCONV_F16) return dact_type<__half>(gout, z, dz, partial, M, Co, activation, st);
+    return dact_type<__nv_bfloat16>(gout, z, dz, partial, M, Co, activation, st);
+}
+
+// Splits of the weight gradient's sum over the rows: enough blocks for four per SM, at least 256
+// rows each.
+static int wgrad_splits(int64_t M, int Ci, int Co) {
+    const int64_t tiles = Ci <= 16 ? (Co + 127) / 128 : Co <= 16 ? (Ci + 127) / 128 : (int64_t)((Co + 127) / 128) * ((Ci + 63) / 64);
+    return (int)std::max<int64_t>(1, std::min<int64_t>((148 * 4 + tiles - 1) / tiles, (M + 255) / 256));
+}
+
+static int64_t pad256(int64_t n) { return (n + 255) & ~(int64_t)255; }
+static int64_t elt(int dtype) { return dtype == SPCONV_F32 ? 4 : 2; }
+
+static int check_linear(int dtype, int64_t M, int Ci, int Co, int activation, int kernel_choice) {
+    SPCONV_REQUIRE(dtype == SPCONV_F32 || dtype == SPCONV_F16 || dtype == SPCONV_BF16, SPCONV_ERR_ARG,
+                   "unsupported dtype code %d", dtype);
+    SPCONV_REQUIRE(M >= 0 && M < ((int64_t)1 << 31), SPCONV_ERR_ARG, "rows must be in [0, 2^31)");
+    SPCONV_REQUIRE(Ci >= 1 && Ci <= 65536 && Co >= 1 && Co <= 65536, SPCONV_ERR_ARG,
+                   "channels must be in [1, 65536], got %d and %d", Ci, Co);
+    SPCONV_REQUIRE(activation >= SPCONV_ACT_NONE && activation <= SPCONV_ACT_SILU, SPCONV_ERR_ARG,
+                   "unknown activation %d", activation);
+    SPCONV_REQUIRE(kernel_choice >= SPCONV_KERNEL_AUTO && kernel_choice <= SPCONV_KERNEL_TCGEN05, SPCONV_ERR_ARG,
+                   "unknown kernel choice %d", kernel_choice);
+    return SPCONV_OK;
+}
+
+static int launch_gemm(const GemmArgs &g, int kernel_choice) {
+    SPCONV_REQUIRE(kernel_choice != SPCONV_KERNEL_TCGEN05, SPCONV_ERR_UNSUPPORTED, "no tensor-core kernel for this call");
+    return launch_gemm_simt(g);
+}
+
+}  // namespace spconv
+
+using namespace spconv;
+
+extern "C" int spconv_linear_forward(const void *feats, int dtype, int64_t M, int Ci, const void *weight,
+                                     const void *bias, const void *residual, int Co, int activation, void *out,
+                                     void *preact, int kernel_choice, int32_t *status, void *stream) {
+    if (const int rc = check_linear(dtype, M, Ci, Co, activation, kernel_choice)) return rc;
+    if (M == 0) return SPCONV_OK;
+    SPCONV_REQUIRE(feats && weight && out, SPCONV_ERR_ARG, "null pointer argument");
+    GemmArgs g = {};
+    g.a = feats;
+    g.b = weight;
+    g.dtype = dtype;
+    g.M = M;
+    g.N = Co;
+    g.K = Ci;
+    g.bias = bias;
+    g.residual = residual;
+    g.activation = activation;
+    g.out = out;
+    g.preact = preact;
+    g.splits = 1;
+    g.status = status;
+    g.stream = (cudaStream_t)stream;
+    return launch_gemm(g, kernel_choice);
+}
+
+extern "C" int64_t spconv_linear_backward_workspace_bytes(int dtype, int64_t M, int Ci, int Co, int activation) {
+    if (check_linear(dtype, M, Ci, Co, activation, SPCONV_KERNEL_AUTO) != SPCONV_OK) return -1;
+    return pad256(activation == SPCONV_ACT_NONE ? 0 : M * Co * elt(dtype)) + pad256((int64_t)dact_chunks(M) * Co * 4) +
+           pad256((int64_t)wgrad_splits(M, Ci, Co) * Co * Ci * 4);
+}
+
+extern "C" int spconv_linear_backward(const void *grad_out, const void *preact, const void *feats, const void *weight,
+                                      int dtype, int64_t M, int Ci, int Co, int activation, void *grad_feats,
+                                      void *grad_weight, int weight_dtype, void *grad_bias, int bias_dtype,
+                                      void *workspace, int64_t workspace_bytes, int kernel_choice, int32_t *status,
+                                      void *stream) {
+    if (const int rc = check_linear(dtype, M, Ci, Co, activation, kernel_choice)) return rc;
+    SPCONV_REQUIRE(!grad_weight || weight_dtype == SPCONV_F32 || weight_dtype == dtype, SPCONV_ERR_ARG,
+                   "the weight's gradient is fp32 or of the features' type");
+    SPCONV_REQUIRE(!grad_bias || bias_dtype == SPCONV_F32 || bias_dtype == dtype, SPCONV_ERR_ARG,
+                   "the bias's gradient is fp32 or of the features' type");
+    const cudaStream_t st = (cudaStream_t)stream;
+    if (M == 0) {                            // sums over no rows
+        if (grad_weight && cudaMemsetAsync(grad_weight, 0, (size_t)Co * Ci * elt(weight_dtype), st) != cudaSuccess)
+            return check_launch("linear_backward: clear");
+        if (grad_bias && cudaMemsetAsync(grad_bias, 0, (size_t)Co * elt(bias_dtype), st) != cudaSuccess)
+            return check_launch("linear_backward: clear");
+        return SPCONV_OK;
+    }
+    SPCONV_REQUIRE(grad_out && (preact || activation == SPCONV_ACT_NONE) && (feats || !grad_weight) &&
+                       (weight || !grad_feats), SPCONV_ERR_ARG, "null pointer argument");
+    SPCONV_REQUIRE(workspace && ((uintptr_t)workspace & 255) == 0 &&
+                       workspace_bytes >= spconv_linear_backward_workspace_bytes(dtype, M, Ci, Co, activation),
+                   SPCONV_ERR_ARG, "workspace missing, misaligned or too small");
+    uint8_t *ws = (uint8_t *)workspace;
+    const void *dz = grad_out;
+    if (activation != SPCONV_ACT_NONE) {
+        dz = ws;
+        ws += pad256(M * Co * elt(dtype));
+    }
+    float *bias_part = (float *)ws;
+    ws += pad256((int64_t)dact_chunks(M) * Co * 4);
+    float *weight_part = (float *)ws;
+    if (activation != SPCONV_ACT_NONE || grad_bias) {
+        if (const int rc = launch_dact(dtype, grad_out, preact, activation != SPCONV_ACT_NONE ? (void *)dz : nullptr,
+                                       grad_bias ? bias_part : nullptr, M, Co, activation, st))
+            return rc;
+        if (grad_bias)
+            if (const int rc = launch_reduce(bias_part, dact_chunks(M), Co, bias_dtype, grad_bias, st)) return rc;
+    }
+    GemmArgs g = {};
+    g.dtype = dtype;
+    g.splits = 1;
+    g.status = status;
+    g.stream = st;
+    g.a = dz;
+    if (grad_feats) {
+        g.b = weight;
+        g.b_t = true;
+        g.M = M;
+        g.N = Ci;
+        g.K = Co;
+        g.out = grad_feats;
+        if (const int rc = launch_gemm(g, kernel_choice)) return rc;
+    }
+    if (grad_weight) {
+        g.a_t = g.b_t = true;
+        g.b = feats;
+        g.M = Co;
+        g.N = Ci;
+        g.K = M;
+        g.out = nullptr;
+        g.splits = wgrad_splits(M, Ci, Co);
+        g.k_per_split = (M + g.splits - 1) / g.splits;
+        g.splits = (int)((M + g.k_per_split - 1) / g.k_per_split);
+        g.partial = weight_part;
+        if (const int rc = launch_gemm(g, kernel_choice)) return rc;
+        if (const int rc = launch_reduce(weight_part, g.splits, (int64_t)Co * Ci, weight_dtype, grad_weight, st)) return rc;
+    }
+    return SPCONV_OK;
+}

@@ -1,0 +1,30 @@
+// Interface between the pointwise linear layer's entry points (linear.cu) and its kernels.
+#pragma once
+
+#include <cstdint>
+#include <cuda_runtime.h>
+
+namespace spconv {
+
+// One matrix product out[m, n] = epilogue(sum_k A(m, k) * B(n, k)), fp32 accumulation.
+// A is [M, K] row-major, or [K, M] if a_t; B is [N, K], or [K, N] if b_t; out [M, N].
+struct GemmArgs {
+    const void *a, *b;
+    bool a_t, b_t;
+    int dtype;                       // of a, b, bias, residual, preact and out
+    int64_t M, N, K;
+    const void *bias, *residual;     // [N], [M, N], or null
+    int activation;
+    void *out, *preact;              // preact: [M, N] or null
+    // splits > 1: K is cut into `splits` ranges of `k_per_split`; split s writes its fp32 sums to
+    // partial + s * M * N and there is no epilogue (linear_reduce adds them)
+    int splits = 1;
+    int64_t k_per_split = 0;
+    float *partial = nullptr;
+    int32_t *status = nullptr;
+    cudaStream_t stream = nullptr;
+};
+
+int launch_gemm_simt(const GemmArgs &g);
+
+}  // namespace spconv

@@ -1,0 +1,777 @@
+// The gated residual step between two blocks, with a norm on either side of it, and its
+// gradients, for row-major features [M, C] in fp32, fp16 or bf16:
+//
+//   u = N1(x) * w1 + b1            (the norm after a block; N1 may be absent: u = x)
+//   h = alpha * r + g * u          (gate and residual; either may be absent)
+//   y = N2(h) * w2 + b2            (the norm before the next block; N2 may be absent: no y)
+//
+// N is LayerNorm ((t - mean) * rstd) or RMSNorm (t * rstd), rstd = 1 / sqrt(mean square + eps).
+// Each of g, w1, b1, w2, b2 is one row of C channels or one row per sample of the batch; the
+// rows of sample s are offsets[s] .. offsets[s + 1] - 1.
+//
+// Backward, from dh and dy (either may be absent), with t = dy * w2:
+//   G  = dh + rstd2 * (t - mean(t) - hhat * mean(t * hhat))       (RMS: without mean(t))
+//   dr = alpha * G;  du = G * g;  dx = N1's gradient of du * w1, by the same formula
+//   dw2 = sum dy * hhat, db2 = sum dy, dg = sum G * u, dw1 = sum du * xhat, db1 = sum du
+// over all rows, or over a sample's rows. Nothing is kept from the forward: u, h and the
+// statistics are recomputed from x and r in fp32, so the forward's rounding of h does not enter
+// the gradients, and x and r are as many bytes as x and h would be.
+//
+// Bound: HBM. Forward reads x, r and writes h, y; backward reads x, r, dh, dy and writes dx, dr.
+// All arithmetic is fp32; each output is rounded once. A row lives in the registers of the
+// lanes that own it, so every tensor is read once.
+#include <algorithm>
+
+#include "common.cuh"
+
+namespace spconv {
+
+constexpr int kRnThreads = 256;
+constexpr int kRnWarps = kRnThreads / 32;
+constexpr int kRnMaxC = 8192;
+constexpr int kRnMaxSamples = 65535;   // a grid dimension of the gradient sums
+// parameter slots, and the order of their partial sums
+enum { kG = 0, kW1 = 1, kB1 = 2, kW2 = 3, kB2 = 4, kRnParams = 5 };
+
+struct RnArgs {
+    const void *x, *r;                   // r may be null
+    void *h, *y;                         // forward outputs (y null without N2)
+    const void *dh, *dy;                 // backward inputs (either may be null)
+    void *dx, *dr;                       // backward outputs (either may be null)
+    const void *p[kRnParams];            // parameters (null: 1 for g, w; 0 for b)
+    int p_f32[kRnParams];                // 1: fp32, 0: the features' type
+    int64_t p_stride[kRnParams];         // C if there is a row per sample, else 0
+    int slot[kRnParams];                 // backward: position among the sums wanted, or -1
+    int nslots;
+    float *partial;                      // [G + B][nslots][C]
+    const int32_t *offsets;              // [B + 1], used when a parameter has a row per sample
+    int B;
+    int64_t M;
+    int C;
+    int lpr;                             // lanes per row (BLOCK: unused)
+    int64_t chunk;                       // consecutive rows per CTA
+    int norm1, norm2;
+    float alpha, eps;
+    int32_t *status;
+};
+
+// VEC consecutive values of one row: eight (one or two 16-byte loads) or one.
+template <typename T, int VEC> struct RnPack;
+template <> struct RnPack<float, 8> { uint4 q[2]; };
+template <> struct RnPack<__half, 8> { uint4 q[1]; };
+template <> struct RnPack<__nv_bfloat16, 8> { uint4 q[1]; };
+template <typename T> struct RnPack<T, 1> { T v; };
+
+template <typename T>
+__device__ __forceinline__ void rn_load(RnPack<T, 8> &p, const T *src) {
+    const uint4 *s = reinterpret_cast<const uint4 *>(src);
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(p.q) / 16); ++i) p.q[i] = __ldcs(s + i);
+}
+template <typename T>
+__device__ __forceinline__ void rn_load(RnPack<T, 1> &p, const T *src) { p.v = *src; }
+
+__device__ __forceinline__ void rn_unpack(const RnPack<float, 8> &p, float *f) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        f[4 * i] = __uint_as_float(p.q[i].x);
+        f[4 * i + 1] = __uint_as_float(p.q[i].y);
+        f[4 * i + 2] = __uint_as_float(p.q[i].z);
+        f[4 * i + 3] = __uint_as_float(p.q[i].w);
+    }
+}
+__device__ __forceinline__ void rn_unpack(const RnPack<__half, 8> &p, float *f) {
+    const __half2 *h = reinterpret_cast<const __half2 *>(p.q);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 v = __half22float2(h[i]);
+        f[2 * i] = v.x;
+        f[2 * i + 1] = v.y;
+    }
+}
+__device__ __forceinline__ void rn_unpack(const RnPack<__nv_bfloat16, 8> &p, float *f) {
+    const uint32_t *w = reinterpret_cast<const uint32_t *>(p.q);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        f[2 * i] = __uint_as_float(w[i] << 16);
+        f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+}
+template <typename T>
+__device__ __forceinline__ void rn_unpack(const RnPack<T, 1> &p, float *f) { f[0] = dtype_traits<T>::to_f(p.v); }
+
+__device__ __forceinline__ void rn_store(float *dst, const float *f, RnPack<float, 8> *) {
+    __stcs(reinterpret_cast<float4 *>(dst), make_float4(f[0], f[1], f[2], f[3]));
+    __stcs(reinterpret_cast<float4 *>(dst) + 1, make_float4(f[4], f[5], f[6], f[7]));
+}
+template <typename T>
+__device__ __forceinline__ void rn_store(T *dst, const float *f, RnPack<T, 8> *) {
+    T v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = dtype_traits<T>::from_f(f[i]);
+    uint4 q;
+    memcpy(&q, v, 16);
+    __stcs(reinterpret_cast<uint4 *>(dst), q);
+}
+template <typename T>
+__device__ __forceinline__ void rn_store(T *dst, const float *f, RnPack<T, 1> *) { *dst = dtype_traits<T>::from_f(f[0]); }
+
+// VEC values of parameter k's row for sample s from column col (its default where it is absent).
+template <typename T, int VEC>
+__device__ __forceinline__ void rn_param(const RnArgs &a, int k, int s, int col, float *f) {
+    if (a.p[k] == nullptr) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) f[i] = (k == kB1 || k == kB2) ? 0.f : 1.f;
+        return;
+    }
+    const int64_t at = (int64_t)s * a.p_stride[k] + col;
+    if (a.p_f32[k]) {
+        const float *q = (const float *)a.p[k] + at;
+        if constexpr (VEC == 8) {
+            const float4 u = __ldg((const float4 *)q), v = __ldg((const float4 *)q + 1);
+            f[0] = u.x; f[1] = u.y; f[2] = u.z; f[3] = u.w;
+            f[4] = v.x; f[5] = v.y; f[6] = v.z; f[7] = v.w;
+        } else {
+            f[0] = __ldg(q);
+        }
+    } else {
+        RnPack<T, VEC> p;
+        if constexpr (VEC == 8) {
+#pragma unroll
+            for (int i = 0; i < (int)(sizeof(p.q) / 16); ++i) p.q[i] = __ldg((const uint4 *)((const T *)a.p[k] + at) + i);
+        } else {
+            p.v = ((const T *)a.p[k])[at];
+        }
+        rn_unpack(p, f);
+    }
+}
+
+// Sums of two values over the lanes that share a row: lpr lanes of a warp, or the whole block.
+template <bool BLOCK>
+__device__ __forceinline__ void rn_sum2(float &u, float &v, int lpr, float2 *scratch) {
+    const int top = BLOCK ? 16 : lpr >> 1;
+    for (int o = top; o > 0; o >>= 1) {
+        u += __shfl_xor_sync(0xffffffffu, u, o);
+        v += __shfl_xor_sync(0xffffffffu, v, o);
+    }
+    if constexpr (BLOCK) {
+        __syncthreads();
+        if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = make_float2(u, v);
+        __syncthreads();
+        u = v = 0.f;
+#pragma unroll
+        for (int w = 0; w < kRnWarps; ++w) {
+            u += scratch[w].x;
+            v += scratch[w].y;
+        }
+    }
+}
+template <bool BLOCK>
+__device__ __forceinline__ float rn_sum(float u, int lpr, float2 *scratch) {
+    if constexpr (BLOCK) {
+        float v = 0.f;
+        rn_sum2<true>(u, v, lpr, scratch);
+    } else {
+        for (int o = lpr >> 1; o > 0; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
+    }
+    return u;
+}
+
+// Normalises the N values a lane holds of a row in place; returns rstd. The mean is taken out
+// before the squares are summed, so a large common offset costs no digits of the variance.
+template <int N, int VEC, bool BLOCK>
+__device__ __forceinline__ float rn_normalise(float (&t)[N], const bool *have, int kind, float inv_c, float eps, int lpr,
+                                              float2 *scratch) {
+    if (kind == SPCONV_NORM_NONE) return 1.f;
+    if (kind == SPCONV_NORM_LAYER) {
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) s += t[i];
+        const float mean = rn_sum<BLOCK>(s, lpr, scratch) * inv_c;
+#pragma unroll
+        for (int i = 0; i < N; ++i) t[i] = have[i / VEC] ? t[i] - mean : 0.f;
+    }
+    float q = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) q += t[i] * t[i];
+    const float rstd = rsqrtf(rn_sum<BLOCK>(q, lpr, scratch) * inv_c + eps);
+#pragma unroll
+    for (int i = 0; i < N; ++i) t[i] *= rstd;
+    return rstd;
+}
+
+// t: gradient at the normalised values n -> gradient at the values before the norm.
+template <int N, bool BLOCK>
+__device__ __forceinline__ void rn_normalise_back(float (&t)[N], const float (&n)[N], float rstd, int kind, float inv_c,
+                                                  int lpr, float2 *scratch) {
+    if (kind == SPCONV_NORM_NONE) return;
+    float s = 0.f, q = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        s += t[i];
+        q += t[i] * n[i];
+    }
+    rn_sum2<BLOCK>(s, q, lpr, scratch);
+    const float mean = kind == SPCONV_NORM_LAYER ? s * inv_c : 0.f, along = q * inv_c;
+#pragma unroll
+    for (int i = 0; i < N; ++i) t[i] = rstd * (t[i] - mean - n[i] * along);
+}
+
+// The sample of row r (offsets ascending), always in [0, B).
+__device__ __forceinline__ int rn_sample(const RnArgs &a, int64_t r) {
+    int lo = 0, hi = a.B - 1;
+    while (lo < hi) {                        // first s with offsets[s + 1] > r
+        const int mid = (lo + hi) >> 1;
+        if ((int64_t)__ldg(a.offsets + mid + 1) > r) hi = mid;
+        else lo = mid + 1;
+    }
+    return lo;
+}
+
+// Offsets have to ascend from 0 to M; whatever they hold, rows are assigned inside [0, B).
+__device__ __forceinline__ void rn_check_offsets(const RnArgs &a) {
+    if (blockIdx.x != 0 || a.B <= 1) return;
+    bool bad = false;
+    for (int s = threadIdx.x; s < a.B; s += blockDim.x) {
+        const int lo = __ldg(a.offsets + s), hi = __ldg(a.offsets + s + 1);
+        bad |= lo > hi || (s == 0 && lo != 0) || (s == a.B - 1 && hi != a.M);
+    }
+    if (bad) raise_status(a.status, SPCONV_STATUS_OFFSETS);
+}
+
+// A CTA takes `chunk` consecutive rows, sample by sample, and its row groups (lpr lanes, or the
+// block) take the rows of a sample in turn. Parameters stay in registers for a sample's rows
+// when a lane owns at most 8 columns; wider rows read them through L1.
+template <typename T, int VEC, int VPT, bool BLOCK>
+__global__ void __launch_bounds__(kRnThreads)
+residual_norm_fwd_kernel(const __grid_constant__ RnArgs a) {
+    constexpr int N = VEC * VPT;
+    constexpr bool HOIST = N <= 8;
+    __shared__ float2 scratch[kRnWarps];
+    rn_check_offsets(a);
+    const int C = a.C, lpr = a.lpr;
+    const int lanes = BLOCK ? kRnThreads : lpr;
+    const int groups = BLOCK ? 1 : kRnThreads / lpr;
+    const int group = BLOCK ? 0 : threadIdx.x / lpr, lane = BLOCK ? threadIdx.x : threadIdx.x & (lpr - 1);
+    const float inv_c = 1.f / (float)C;
+    int col[VPT];
+    bool have[VPT];
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+        col[j] = (lane + lanes * j) * VEC;
+        have[j] = col[j] < C;
+    }
+    const int64_t row0 = (int64_t)blockIdx.x * a.chunk, row1 = min(a.M, row0 + a.chunk);
+    int s = a.B > 1 && row0 < row1 ? rn_sample(a, row0) : 0;
+    for (int64_t seg = row0; seg < row1; ++s) {
+        const int64_t end = s < a.B - 1 ? min(row1, (int64_t)__ldg(a.offsets + s + 1)) : row1;
+        if (end <= seg) continue;            // an empty sample
+        float pg[HOIST ? N : 1], pw1[HOIST ? N : 1], pb1[HOIST ? N : 1], pw2[HOIST ? N : 1], pb2[HOIST ? N : 1];
+        if constexpr (HOIST) {
+#pragma unroll
+            for (int j = 0; j < VPT; ++j) {
+                const int c = have[j] ? col[j] : 0;
+                rn_param<T, VEC>(a, kG, s, c, pg + j * VEC);
+                rn_param<T, VEC>(a, kW1, s, c, pw1 + j * VEC);
+                rn_param<T, VEC>(a, kB1, s, c, pb1 + j * VEC);
+                rn_param<T, VEC>(a, kW2, s, c, pw2 + j * VEC);
+                rn_param<T, VEC>(a, kB2, s, c, pb2 + j * VEC);
+            }
+        }
+        RnPack<T, VEC> px[VPT], pr[VPT];
+        auto fetch = [&](int64_t row) {
+#pragma unroll
+            for (int j = 0; j < VPT; ++j) {
+                px[j] = RnPack<T, VEC>{};
+                pr[j] = RnPack<T, VEC>{};
+                if (row < end && have[j]) {
+                    rn_load(px[j], (const T *)a.x + row * C + col[j]);
+                    if (a.r) rn_load(pr[j], (const T *)a.r + row * C + col[j]);
+                }
+            }
+        };
+        fetch(seg + group);
+        for (int64_t base = seg; base < end; base += groups) {
+            const int64_t row = base + group;
+            float u[N], h[N];
+#pragma unroll
+            for (int j = 0; j < VPT; ++j) {
+                rn_unpack(px[j], u + j * VEC);
+                rn_unpack(pr[j], h + j * VEC);
+            }
+            fetch(row + groups);             // the next row's loads run under this row's sums
+            rn_normalise<N, VEC, BLOCK>(u, have, a.norm1, inv_c, a.eps, lpr, scratch);
+#pragma unroll
+            for (int j = 0; j < VPT; ++j) {
+                float g[VEC], w[VEC], b[VEC];
+                if constexpr (!HOIST) {
+                    const int c = have[j] ? col[j] : 0;
+                    rn_param<T, VEC>(a, kG, s, c, g);
+                    rn_param<T, VEC>(a, kW1, s, c, w);
+                    rn_param<T, VEC>(a, kB1, s, c, b);
+                }
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    const int n = j * VEC + i;
+                    if constexpr (HOIST) { g[i] = pg[n]; w[i] = pw1[n]; b[i] = pb1[n]; }
+                    h[n] = have[j] ? a.alpha * h[n] + g[i] * (u[n] * w[i] + b[i]) : 0.f;
+                }
+                if (have[j] && row < end) rn_store((T *)a.h + row * C + col[j], h + j * VEC, (RnPack<T, VEC> *)nullptr);
+            }
+            if (a.norm2 != SPCONV_NORM_NONE) {
+                rn_normalise<N, VEC, BLOCK>(h, have, a.norm2, inv_c, a.eps, lpr, scratch);
+#pragma unroll
+                for (int j = 0; j < VPT; ++j) {
+                    float w[VEC], b[VEC];
+                    if constexpr (!HOIST) {
+                        const int c = have[j] ? col[j] : 0;
+                        rn_param<T, VEC>(a, kW2, s, c, w);
+                        rn_param<T, VEC>(a, kB2, s, c, b);
+                    }
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) {
+                        const int n = j * VEC + i;
+                        if constexpr (HOIST) { w[i] = pw2[n]; b[i] = pb2[n]; }
+                        h[n] = h[n] * w[i] + b[i];
+                    }
+                    if (have[j] && row < end) rn_store((T *)a.y + row * C + col[j], h + j * VEC, (RnPack<T, VEC> *)nullptr);
+                }
+            }
+        }
+        seg = end;
+    }
+}
+
+// As the forward's walk. The parameter sums are kept per lane (N <= 8) or per warp in shared
+// memory, added up over the block in a fixed order when a sample's rows in the chunk end, and
+// written as record blockIdx + s: along a walk through the chunks and samples that index only
+// grows, so each (chunk, sample) pair that holds rows has a record of its own and at most
+// G + B - 1 are needed.
+template <typename T, int VEC, int VPT, bool BLOCK>
+__global__ void __launch_bounds__(kRnThreads)
+residual_norm_bwd_kernel(const __grid_constant__ RnArgs a) {
+    constexpr int N = VEC * VPT;
+    constexpr bool HOIST = N <= 8;
+    constexpr int kCopies = BLOCK ? 1 : kRnWarps;
+    extern __shared__ float s_acc[];         // [kCopies][nslots][C]
+    __shared__ float2 scratch[kRnWarps];
+    rn_check_offsets(a);
+    const int C = a.C, lpr = a.lpr, warp = threadIdx.x >> 5;
+    const int lanes = BLOCK ? kRnThreads : lpr;
+    const int groups = BLOCK ? 1 : kRnThreads / lpr;
+    const int group = BLOCK ? 0 : threadIdx.x / lpr, lane = BLOCK ? threadIdx.x : threadIdx.x & (lpr - 1);
+    const float inv_c = 1.f / (float)C;
+    float *mine = s_acc + (BLOCK ? 0 : (int64_t)warp * a.nslots * C);
+    int col[VPT];
+    bool have[VPT];
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+        col[j] = (lane + lanes * j) * VEC;
+        have[j] = col[j] < C;
+    }
+    const int64_t row0 = (int64_t)blockIdx.x * a.chunk, row1 = min(a.M, row0 + a.chunk);
+    int s = a.B > 1 && row0 < row1 ? rn_sample(a, row0) : 0;
+    for (int64_t seg = row0; seg < row1; ++s) {
+        const int64_t end = s < a.B - 1 ? min(row1, (int64_t)__ldg(a.offsets + s + 1)) : row1;
+        if (end <= seg) continue;
+        float pg[HOIST ? N : 1], pw1[HOIST ? N : 1], pb1[HOIST ? N : 1], pw2[HOIST ? N : 1];
+        float acc[kRnParams][HOIST ? N : 1];
+        if constexpr (HOIST) {
+#pragma unroll
+            for (int j = 0; j < VPT; ++j) {
+                const int c = have[j] ? col[j] : 0;
+                rn_param<T, VEC>(a, kG, s, c, pg + j * VEC);
+                rn_param<T, VEC>(a, kW1, s, c, pw1 + j * VEC);
+                rn_param<T, VEC>(a, kB1, s, c, pb1 + j * VEC);
+                rn_param<T, VEC>(a, kW2, s, c, pw2 + j * VEC);
+            }
+#pragma unroll
+            for (int k = 0; k < kRnParams; ++k)
+#pragma unroll
+                for (int i = 0; i < N; ++i) acc[k][i] = 0.f;
+        } else {
+            for (int i = threadIdx.x; i < kCopies * a.nslots * C; i += kRnThreads) s_acc[i] = 0.f;
+            __syncthreads();
+        }
+        // adds VEC values into parameter k's sums (shared-memory form: a lane's own columns of
+        // its warp's copy)
+        auto add = [&](int k, int j, const float *v) {
+            if constexpr (HOIST) {
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) acc[k][j * VEC + i] += v[i];
+            } else {
+                if (a.slot[k] < 0 || !have[j]) return;
+                float *d = mine + (int64_t)a.slot[k] * C + col[j];
+                if constexpr (VEC == 8) {
+                    float4 *q = reinterpret_cast<float4 *>(d);
+                    float4 u = q[0], w = q[1];
+                    u.x += v[0]; u.y += v[1]; u.z += v[2]; u.w += v[3];
+                    w.x += v[4]; w.y += v[5]; w.z += v[6]; w.w += v[7];
+                    q[0] = u;
+                    q[1] = w;
+                } else {
+                    *d += v[0];
+                }
+            }
+        };
+        RnPack<T, VEC> px[VPT], pr[VPT], ph[VPT], py[VPT];
+        auto fetch = [&](int64_t row) {
+#pragma unroll
+            for (int j = 0; j < VPT; ++j) {
+                px[j] = RnPack<T, VEC>{};
+                pr[j] = RnPack<T, VEC>{};
+                ph[j] = RnPack<T, VEC>{};
+                py[j] = RnPack<T, VEC>{};
+                if (row < end && have[j]) {
+                    const int64_t at = row * C + col[j];
+                    rn_load(px[j], (const T *)a.x + at);
+                    if (a.r) rn_load(pr[j], (const T *)a.r + at);
+                    if (a.dh) rn_load(ph[j], (const T *)a.dh + at);
+                    if (a.dy) rn_load(py[j], (const T *)a.dy + at);
+                }
+            }
+        };
+        if constexpr (HOIST) fetch(seg + group);
+        for (int64_t base = seg; base < end; base += groups) {
+            const int64_t row = base + group;
+            if constexpr (!HOIST) fetch(row);
+            float n1[N], n2[N], t[N], gr[N];     // xhat, hhat, dy * w2, dh -> G
+            const bool live = row < end;         // a row past the end holds zeros and adds none
+#pragma unroll
+            for (int j = 0; j < VPT; ++j) {
+                rn_unpack(px[j], n1 + j * VEC);
+                rn_unpack(pr[j], n2 + j * VEC);
+                rn_unpack(ph[j], gr + j * VEC);
+                rn_unpack(py[j], t + j * VEC);
+            }
+            if constexpr (HOIST) fetch(row + groups);
+            const float rstd1 = rn_normalise<N, VEC, BLOCK>(n1, have, a.norm1, inv_c, a.eps, lpr, scratch);
+#pragma unroll
+            for (int j = 0; j < VPT; ++j) {
+                float g[VEC], w[VEC], b[VEC];
+                if constexpr (!HOIST) {
+                    const int c = have[j] ? col[j] : 0;
+                    rn_param<T, VEC>(a, kG, s, c, g);
+                    rn_param<T, VEC>(a, kW1, s, c, w);
+                    rn_param<T, VEC>(a, kB1, s, c, b);
+                }
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    const int n = j * VEC + i;
+                    if constexpr (HOIST) { g[i] = pg[n]; w[i] = pw1[n]; b[i] = pb1[n]; }
+                    n2[n] = have[j] ? a.alpha * n2[n] + g[i] * (n1[n] * w[i] + b[i]) : 0.f;
+                }
+            }
+            if (a.norm2 != SPCONV_NORM_NONE && a.dy) {
+                const float rstd2 = rn_normalise<N, VEC, BLOCK>(n2, have, a.norm2, inv_c, a.eps, lpr, scratch);
+#pragma unroll
+                for (int j = 0; j < VPT; ++j) {
+                    float w[VEC], v[VEC];
+                    if constexpr (!HOIST) rn_param<T, VEC>(a, kW2, s, have[j] ? col[j] : 0, w);
+                    if (live) add(kB2, j, t + j * VEC);
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) {
+                        const int n = j * VEC + i;
+                        if constexpr (HOIST) w[i] = pw2[n];
+                        v[i] = t[n] * n2[n];
+                        t[n] *= w[i];
+                    }
+                    if (live) add(kW2, j, v);
+                }
+                rn_normalise_back<N, BLOCK>(t, n2, rstd2, a.norm2, inv_c, lpr, scratch);
+#pragma unroll
+                for (int n = 0; n < N; ++n) gr[n] += t[n];
+            }
+#pragma unroll
+            for (int j = 0; j < VPT; ++j) {
+                float g[VEC], w[VEC], b[VEC], v[VEC], o[VEC];
+                if constexpr (!HOIST) {
+                    const int c = have[j] ? col[j] : 0;
+                    rn_param<T, VEC>(a, kG, s, c, g);
+                    rn_param<T, VEC>(a, kW1, s, c, w);
+                    rn_param<T, VEC>(a, kB1, s, c, b);
+                }
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    const int n = j * VEC + i;
+                    if constexpr (HOIST) { g[i] = pg[n]; w[i] = pw1[n]; b[i] = pb1[n]; }
+                    const float d = have[j] ? gr[n] : 0.f;
+                    o[i] = a.alpha * d;
+                    v[i] = d * (n1[n] * w[i] + b[i]);
+                    gr[n] = d * g[i];            // du
+                }
+                if (a.dr && have[j] && live) rn_store((T *)a.dr + row * C + col[j], o, (RnPack<T, VEC> *)nullptr);
+                if (live) {
+                    add(kG, j, v);
+                    add(kB1, j, gr + j * VEC);
+                }
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    const int n = j * VEC + i;
+                    v[i] = gr[n] * n1[n];
+                    gr[n] *= w[i];
+                }
+                if (live) add(kW1, j, v);
+            }
+            if (a.dx) {
+                rn_normalise_back<N, BLOCK>(gr, n1, rstd1, a.norm1, inv_c, lpr, scratch);
+#pragma unroll
+                for (int j = 0; j < VPT; ++j)
+                    if (have[j] && live) rn_store((T *)a.dx + row * C + col[j], gr + j * VEC, (RnPack<T, VEC> *)nullptr);
+            }
+        }
+        if (a.nslots > 0) {
+            if constexpr (HOIST) {
+                // lanes of a warp that own the same columns, then one copy per warp
+#pragma unroll
+                for (int k = 0; k < kRnParams; ++k) {
+                    if (a.slot[k] < 0) continue;
+#pragma unroll
+                    for (int i = 0; i < N; ++i)
+                        for (int o = lpr; o < 32; o <<= 1) acc[k][i] += __shfl_xor_sync(0xffffffffu, acc[k][i], o);
+                    if ((threadIdx.x & 31) < lpr) {
+#pragma unroll
+                        for (int j = 0; j < VPT; ++j)
+                            if (have[j])
+#pragma unroll
+                                for (int i = 0; i < VEC; ++i)
+                                    mine[(int64_t)a.slot[k] * C + col[j] + i] = acc[k][j * VEC + i];
+                    }
+                }
+            }
+            __syncthreads();
+            const int n = a.nslots * C;
+            float *rec = a.partial + ((int64_t)blockIdx.x + s) * n;
+            for (int i = threadIdx.x; i < n; i += kRnThreads) {
+                float v = 0.f;
+#pragma unroll
+                for (int w = 0; w < kCopies; ++w) v += s_acc[(int64_t)w * n + i];
+                rec[i] = v;
+            }
+            __syncthreads();
+        }
+        seg = end;
+    }
+}
+
+struct RnGradArgs {
+    void *out[kRnParams];                // by slot
+    int out_f32[kRnParams], per_sample[kRnParams];
+};
+
+// Adds the records of each parameter up: all of them, or a sample's. blockIdx.y is the slot,
+// blockIdx.z the sample (only 0 for a parameter of one row). 32 columns x 32 record lanes.
+template <typename T>
+__global__ void __launch_bounds__(1024)
+residual_norm_grad_kernel(const __grid_constant__ RnArgs a, const __grid_constant__ RnGradArgs o) {
+    __shared__ float part[32][33];
+    const int k = blockIdx.y;
+    const int c = blockIdx.x * 32 + threadIdx.x;
+    const int s_first = o.per_sample[k] ? blockIdx.z : 0, s_last = o.per_sample[k] ? blockIdx.z : a.B - 1;
+    if (!o.per_sample[k] && blockIdx.z != 0) return;
+    grid_dependency_wait();
+    float v = 0.f;
+    for (int s = s_first; s <= s_last; ++s) {
+        int64_t lo = 0, hi = a.M;
+        if (a.B > 1) {
+            // the walk gives rows before offsets[1] to sample 0 and rows from offsets[B - 1] on to the last
+            lo = s == 0 ? 0 : max((int64_t)0, min(a.M, (int64_t)__ldg(a.offsets + s)));
+            hi = s == a.B - 1 ? a.M : max((int64_t)0, min(a.M, (int64_t)__ldg(a.offsets + s + 1)));
+        }
+        if (lo >= hi) continue;
+        for (int64_t b = lo / a.chunk + threadIdx.y; b <= (hi - 1) / a.chunk; b += 32)
+            if (c < a.C) v += a.partial[((b + s) * a.nslots + k) * a.C + c];
+    }
+    part[threadIdx.y][threadIdx.x] = v;
+    __syncthreads();
+    if (threadIdx.y == 0 && c < a.C) {
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) sum += part[i][threadIdx.x];
+        const int64_t at = (o.per_sample[k] ? (int64_t)blockIdx.z * a.C : 0) + c;
+        if (o.out_f32[k]) ((float *)o.out[k])[at] = sum;
+        else ((T *)o.out[k])[at] = dtype_traits<T>::from_f(sum);
+    }
+}
+
+// ---------------------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------------------
+static int rn_pow2(int n) {
+    int p = 1;
+    while (p < n) p <<= 1;
+    return p;
+}
+
+// CTAs for M rows: enough to fill the SMs twice over, no more than there are row groups.
+static int64_t rn_grid(int64_t M, int rows_per_block) {
+    const int64_t most = 148 * 4;
+    return std::max<int64_t>(1, std::min<int64_t>(most, (M + rows_per_block - 1) / rows_per_block));
+}
+
+template <typename T, int VEC, int VPT, bool BLOCK>
+static int rn_launch(RnArgs &a, bool backward, cudaStream_t st) {
+    const int rows = BLOCK ? 1 : kRnThreads / a.lpr;
+    int64_t grid = rn_grid(a.M, rows);
+    a.chunk = (a.M + grid - 1) / grid;
+    grid = (a.M + a.chunk - 1) / a.chunk;
+    if (!backward) {
+        residual_norm_fwd_kernel<T, VEC, VPT, BLOCK><<<(unsigned)grid, kRnThreads, 0, st>>>(a);
+        return check_launch("residual_norm_fwd_kernel");
+    }
+    const size_t smem = (size_t)(BLOCK ? 1 : kRnWarps) * a.nslots * a.C * sizeof(float);
+    auto kern = residual_norm_bwd_kernel<T, VEC, VPT, BLOCK>;
+    if (smem > 48 * 1024 &&
+        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+        return check_launch("residual_norm_bwd: set max dynamic shared memory");
+    kern<<<(unsigned)grid, kRnThreads, smem, st>>>(a);
+    return check_launch("residual_norm_bwd_kernel");
+}
+
+// Columns a lane owns: eight neighbours at a time where rows and parameters allow 16-byte
+// accesses, single columns otherwise; the fewest that cover the row with one warp, and a block
+// of eight warps per row beyond 1,024 channels.
+template <typename T>
+static int rn_dispatch(RnArgs &a, bool vec, bool backward, cudaStream_t st) {
+    const int C = a.C;
+    if (vec) {
+        a.lpr = std::min(32, rn_pow2(C / 8));
+        if (C <= 256) return rn_launch<T, 8, 1, false>(a, backward, st);
+        if (C <= 512) return rn_launch<T, 8, 2, false>(a, backward, st);
+        if (C <= 1024) return rn_launch<T, 8, 4, false>(a, backward, st);
+        return rn_launch<T, 8, 4, true>(a, backward, st);
+    }
+    a.lpr = std::min(32, rn_pow2(C));
+    if (C <= 32) return rn_launch<T, 1, 1, false>(a, backward, st);
+    if (C <= 64) return rn_launch<T, 1, 2, false>(a, backward, st);
+    if (C <= 128) return rn_launch<T, 1, 4, false>(a, backward, st);
+    if (C <= 256) return rn_launch<T, 1, 8, false>(a, backward, st);
+    if (C <= 1024) return rn_launch<T, 1, 32, false>(a, backward, st);
+    return rn_launch<T, 1, 32, true>(a, backward, st);
+}
+
+static bool rn_aligned(const void *p) { return ((uintptr_t)p & 15) == 0; }
+
+// Checks the call and fills the kernels' arguments (all but lpr and chunk).
+static int rn_args(const spconv_residual_norm_args *q, RnArgs &a, bool &vec, bool backward) {
+    SPCONV_REQUIRE(q != nullptr, SPCONV_ERR_ARG, "null argument block");
+    SPCONV_REQUIRE(q->dtype == SPCONV_F32 || q->dtype == SPCONV_F16 || q->dtype == SPCONV_BF16, SPCONV_ERR_ARG,
+                   "unsupported dtype code %d", q->dtype);
+    SPCONV_REQUIRE(q->num_rows >= 0 && q->num_rows < ((int64_t)1 << 31), SPCONV_ERR_ARG, "rows must be in [0, 2^31)");
+    SPCONV_REQUIRE(q->channels >= 1 && q->channels <= kRnMaxC, SPCONV_ERR_ARG, "channels must be in [1, %d], got %d",
+                   kRnMaxC, q->channels);
+    SPCONV_REQUIRE(q->norm >= 0 && q->norm <= 2 && q->next_norm >= 0 && q->next_norm <= 2, SPCONV_ERR_ARG,
+                   "unknown norm kind %d / %d", q->norm, q->next_norm);
+    SPCONV_REQUIRE(q->num_samples >= 1 && q->num_samples <= kRnMaxSamples, SPCONV_ERR_ARG,
+                   "samples must be in [1, %d], got %d", kRnMaxSamples, q->num_samples);
+    if (q->num_rows == 0) return SPCONV_OK;
+    SPCONV_REQUIRE(q->feats != nullptr, SPCONV_ERR_ARG, "null pointer argument");
+    a.x = q->feats;
+    a.r = q->residual;
+    a.h = q->hidden;
+    a.y = q->normed;
+    a.dh = q->grad_hidden;
+    a.dy = q->grad_normed;
+    a.dx = q->grad_feats;
+    a.dr = q->grad_residual;
+    a.M = q->num_rows;
+    a.C = q->channels;
+    a.norm1 = q->norm;
+    a.norm2 = q->next_norm;
+    a.alpha = q->residual_scale;
+    a.eps = q->eps;
+    a.status = q->status;
+    a.offsets = q->offsets;
+    a.B = 1;
+    a.nslots = 0;
+    a.partial = (float *)q->workspace;
+    const spconv_channel_param *ps[kRnParams] = {&q->gate, &q->weight, &q->bias, &q->next_weight, &q->next_bias};
+    vec = q->channels % 8 == 0;
+    for (const void *p : {a.x, a.r, (const void *)a.h, (const void *)a.y, a.dh, a.dy, (const void *)a.dx, (const void *)a.dr})
+        vec = vec && rn_aligned(p);
+    for (int k = 0; k < kRnParams; ++k) {
+        const spconv_channel_param &p = *ps[k];
+        a.p[k] = p.data;
+        a.p_f32[k] = p.dtype == SPCONV_F32;
+        a.p_stride[k] = p.per_sample ? q->channels : 0;
+        a.slot[k] = -1;
+        if (!p.data) {
+            SPCONV_REQUIRE(!p.grad, SPCONV_ERR_ARG, "a gradient of an absent parameter");
+            continue;
+        }
+        SPCONV_REQUIRE(p.dtype == SPCONV_F32 || p.dtype == q->dtype, SPCONV_ERR_ARG,
+                       "parameters must be fp32 or of the features' type");
+        vec = vec && rn_aligned(p.data);
+        if (p.per_sample) a.B = q->num_samples;
+        if (backward && p.grad) a.slot[k] = a.nslots++;
+    }
+    SPCONV_REQUIRE(a.B == 1 || a.offsets, SPCONV_ERR_ARG, "a parameter per sample needs the samples' row offsets");
+    if (a.B == 1) a.offsets = nullptr;
+    return SPCONV_OK;
+}
+
+template <typename F>
+static int rn_by_type(int dtype, F f) {
+    if (dtype == SPCONV_F32) return f((float *)nullptr);
+    if (dtype == SPCONV_F16) return f((__half *)nullptr);
+    return f((__nv_bfloat16 *)nullptr);
+}
+
+}  // namespace spconv
+
+using namespace spconv;
+
+extern "C" int64_t spconv_residual_norm_workspace_bytes(int64_t num_rows, int channels, int num_samples) {
+    if (num_rows < 0 || channels < 1 || channels > kRnMaxC || num_samples < 1 || num_samples > kRnMaxSamples) return -1;
+    return (rn_grid(num_rows, 1) + num_samples) * kRnParams * channels * (int64_t)sizeof(float);
+}
+
+extern "C" int spconv_residual_norm_forward(const spconv_residual_norm_args *q, void *stream) {
+    RnArgs a = {};
+    bool vec = false;
+    const int rc = rn_args(q, a, vec, false);
+    if (rc != SPCONV_OK || q->num_rows == 0) return rc;
+    SPCONV_REQUIRE(a.h && (a.norm2 == SPCONV_NORM_NONE || a.y), SPCONV_ERR_ARG, "null output pointer");
+    return rn_by_type(q->dtype, [&](auto *t) {
+        return rn_dispatch<std::remove_pointer_t<decltype(t)>>(a, vec, false, (cudaStream_t)stream);
+    });
+}
+
+extern "C" int spconv_residual_norm_backward(const spconv_residual_norm_args *q, void *stream) {
+    RnArgs a = {};
+    bool vec = false;
+    const int rc = rn_args(q, a, vec, true);
+    if (rc != SPCONV_OK) return rc;
+    const cudaStream_t st = (cudaStream_t)stream;
+    spconv_channel_param ps[kRnParams] = {q->gate, q->weight, q->bias, q->next_weight, q->next_bias};
+    if (q->num_rows == 0) {                  // sums over no rows
+        for (const auto &p : ps)
+            if (p.grad && cudaMemsetAsync(p.grad, 0, (size_t)(p.per_sample ? q->num_samples : 1) * q->channels *
+                                                        (p.dtype == SPCONV_F32 ? 4 : 2), st) != cudaSuccess)
+                return check_launch("residual_norm_backward: clear");
+        return SPCONV_OK;
+    }
+    SPCONV_REQUIRE(a.dh || a.dy, SPCONV_ERR_ARG, "no output gradient given");
+    SPCONV_REQUIRE(a.nslots == 0 ||
+                       (a.partial && rn_aligned(a.partial) &&
+                        q->workspace_bytes >= spconv_residual_norm_workspace_bytes(q->num_rows, q->channels, a.B)),
+                   SPCONV_ERR_ARG, "workspace missing, misaligned or too small");
+    return rn_by_type(q->dtype, [&](auto *t) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        int e = rn_dispatch<T>(a, vec, true, st);
+        if (e != SPCONV_OK || a.nslots == 0) return e;
+        RnGradArgs o = {};
+        bool per_sample = false;
+        for (int k = 0; k < kRnParams; ++k) {
+            if (a.slot[k] < 0) continue;
+            o.out[a.slot[k]] = ps[k].grad;
+            o.out_f32[a.slot[k]] = a.p_f32[k];
+            o.per_sample[a.slot[k]] = a.p_stride[k] != 0;
+            per_sample |= a.p_stride[k] != 0;
+        }
+        const dim3 grid((a.C + 31) / 32, a.nslots, per_sample ? a.B : 1);
+        if (launch_pdl(residual_norm_grad_kernel<T>, grid, dim3(32, 32), 0, st, a, o) != cudaSuccess)
+            return check_launch("residual_norm_grad_kernel");
+        return check_launch("residual_norm_grad_kernel");
+    });
+}

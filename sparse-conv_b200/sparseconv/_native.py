@@ -13,7 +13,9 @@ asynchronously to pinned host memory; the next op on that device (or an explicit
 """
 from __future__ import annotations
 
+import array
 import ctypes
+import functools
 import os
 import threading
 from typing import Optional, Sequence, Tuple
@@ -24,11 +26,35 @@ LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "libs
 
 SPCONV_OK, SPCONV_ERR_ARG, SPCONV_ERR_CUDA, SPCONV_ERR_UNSUPPORTED = 0, 1, 2, 3
 STATUS_COORD_RANGE, STATUS_TABLE_FULL, STATUS_DUPLICATE, STATUS_WAIT_TIMEOUT = 1, 2, 4, 8
+STATUS_OFFSETS = 16
 DTYPE_CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 KERNEL_AUTO, KERNEL_SIMT, KERNEL_TCGEN05 = 0, 1, 2
 NOALLOC_MAX_COORDS = 262144   # SPCONV_NOALLOC_MAX_COORDS
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}   # SPCONV_ACT_*
+NORMS = {"none": 0, "layer": 1, "rms": 2}                    # SPCONV_NORM_*
+CLIP_P2, CLIP_INF = 0, 1
 
 _c_i64, _c_int, _c_void_p = ctypes.c_int64, ctypes.c_int, ctypes.c_void_p
+
+
+
+class ChannelParam(ctypes.Structure):
+    """spconv_channel_param"""
+    _fields_ = [("data", _c_void_p), ("grad", _c_void_p), ("dtype", _c_int), ("per_sample", _c_int)]
+
+
+class ResidualNormArgs(ctypes.Structure):
+    """spconv_residual_norm_args"""
+    _fields_ = [("dtype", _c_int), ("channels", _c_int), ("num_rows", _c_i64),
+                ("feats", _c_void_p), ("residual", _c_void_p), ("hidden", _c_void_p), ("normed", _c_void_p),
+                ("grad_hidden", _c_void_p), ("grad_normed", _c_void_p),
+                ("grad_feats", _c_void_p), ("grad_residual", _c_void_p),
+                ("gate", ChannelParam), ("weight", ChannelParam), ("bias", ChannelParam),
+                ("next_weight", ChannelParam), ("next_bias", ChannelParam),
+                ("offsets", _c_void_p), ("num_samples", _c_int), ("norm", _c_int), ("next_norm", _c_int),
+                ("residual_scale", ctypes.c_float), ("eps", ctypes.c_float),
+                ("workspace", _c_void_p), ("workspace_bytes", _c_i64), ("status", _c_void_p)]
+
 
 # name -> (restype, argtypes); the order mirrors include/sparseconv_b200.h
 SIGNATURES = {
@@ -79,6 +105,20 @@ SIGNATURES = {
     "spconv_submanifold_conv_weight_grad": (_c_int, [
         _c_void_p, _c_void_p, _c_int, _c_i64, _c_int, _c_int, _c_int,
         _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_i64, _c_void_p, _c_void_p]),
+    "spconv_linear_forward": (_c_int, [
+        _c_void_p, _c_int, _c_i64, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int,
+        _c_void_p, _c_void_p, _c_int, _c_void_p, _c_void_p]),
+    "spconv_linear_backward_workspace_bytes": (_c_i64, [_c_int, _c_i64, _c_int, _c_int, _c_int]),
+    "spconv_linear_backward": (_c_int, [
+        _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_i64, _c_int, _c_int, _c_int,
+        _c_void_p, _c_void_p, _c_int, _c_void_p, _c_int, _c_void_p, _c_i64, _c_int, _c_void_p, _c_void_p]),
+    "spconv_residual_norm_workspace_bytes": (_c_i64, [_c_i64, _c_int, _c_int]),
+    "spconv_residual_norm_forward": (_c_int, [ctypes.POINTER(ResidualNormArgs), _c_void_p]),
+    "spconv_residual_norm_backward": (_c_int, [ctypes.POINTER(ResidualNormArgs), _c_void_p]),
+    "spconv_clip_gradients_workspace_bytes": (_c_i64, [_c_int]),
+    "spconv_clip_gradients": (_c_int, [
+        _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, ctypes.c_float, _c_void_p,
+        _c_void_p, _c_i64, _c_void_p]),
     "spconv_set_wait_limit_ns": (ctypes.c_uint64, [ctypes.c_uint64]),
     "spconv_stage_timing": (_c_int, [_c_int]),
     "spconv_stage_times_ms": (_c_int, [_c_void_p, _c_void_p, _c_int]),
@@ -176,10 +216,12 @@ def describe_status(bits: int) -> str:
         parts.append("the coordinate hash table overflowed")
     if bits & STATUS_WAIT_TIMEOUT:
         parts.append("a kernel-internal wait reached its time limit")
+    if bits & STATUS_OFFSETS:
+        parts.append("sample offsets do not ascend from 0 to the number of rows")
     return "; ".join(parts)
 
 
-_FATAL_BITS = STATUS_COORD_RANGE | STATUS_TABLE_FULL | STATUS_WAIT_TIMEOUT
+_FATAL_BITS = STATUS_COORD_RANGE | STATUS_TABLE_FULL | STATUS_WAIT_TIMEOUT | STATUS_OFFSETS
 
 
 def _inspect(st: _DeviceStatus) -> None:
@@ -600,6 +642,245 @@ def conv_weight_grad(feats: torch.Tensor, grad_out: torch.Tensor, nbr: torch.Ten
     if rc != SPCONV_OK:
         _raise(rc, "spconv_submanifold_conv_weight_grad")
     return gw, gb
+
+
+def _on_device(fn):
+    """Runs a call with the device of its tensors current (launches go to that device's stream)."""
+    @functools.wraps(fn)
+    def call(first, *args, **kwargs):
+        t = first if isinstance(first, torch.Tensor) else (first[0] if first else None)
+        if t is None or not t.is_cuda or t.device.index == torch.cuda.current_device():
+            return fn(first, *args, **kwargs)
+        with torch.cuda.device(t.device):
+            return fn(first, *args, **kwargs)
+    return call
+
+
+def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
+
+
+def _matrix(t: torch.Tensor, shape: Tuple[int, ...], dtype: torch.dtype, what: str) -> None:
+    if t.shape != shape:
+        raise ValueError(f"{what} must have shape {list(shape)}, got {list(t.shape)}")
+    if t.dtype != dtype:
+        raise TypeError(f"{what} dtype {t.dtype} differs from the features' {dtype}")
+    if not t.is_contiguous():
+        raise ValueError(f"{what} must be contiguous")
+
+
+@_on_device
+def linear_forward(feats: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor],
+                   residual: Optional[torch.Tensor], activation: str, keep_preact: bool = False,
+                   kernel: int = KERNEL_AUTO) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """(residual + act(feats @ weight.T + bias), act's argument if ``keep_preact``)."""
+    dev = _require_cuda(feats, weight, bias, residual)
+    dtype = feats.dtype
+    if dtype not in DTYPE_CODES:
+        raise TypeError(f"unsupported feature dtype {dtype}")
+    if feats.dim() != 2 or weight.dim() != 2:
+        raise ValueError("feats must be [M, Ci] and weight [Co, Ci]")
+    if not feats.is_contiguous():
+        raise ValueError("feats must be contiguous")
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"Unsupported activation {activation}.")
+    M, Ci = feats.shape
+    Co = weight.shape[0]
+    if weight.shape[1] != Ci:
+        raise ValueError(f"weight has {weight.shape[1]} input channels, feats {Ci}")
+    weight = weight.contiguous()
+    if bias is not None:
+        _matrix(bias, (Co,), dtype, "bias")
+    if residual is not None:
+        _matrix(residual, (M, Co), dtype, "residual")
+    out = torch.empty((M, Co), dtype=dtype, device=dev)
+    preact = torch.empty_like(out) if keep_preact else None
+    if M == 0:
+        return out, preact
+    before_launch(dev)
+    rc = load_library().spconv_linear_forward(
+        feats.data_ptr(), DTYPE_CODES[dtype], M, Ci, weight.data_ptr(), _ptr(bias), _ptr(residual), Co,
+        ACTIVATIONS[activation], out.data_ptr(), _ptr(preact), kernel, status_word(dev).word.data_ptr(),
+        _stream_ptr(dev))
+    if rc != SPCONV_OK:
+        _raise(rc, "spconv_linear_forward")
+    if dtype != torch.float32:
+        after_launch(dev)
+    return out, preact
+
+
+@_on_device
+def linear_backward(grad_out: torch.Tensor, preact: Optional[torch.Tensor], feats: torch.Tensor, weight: torch.Tensor,
+                    activation: str, weight_dtype: torch.dtype, bias_dtype: Optional[torch.dtype],
+                    needs: Sequence[bool], kernel: int = KERNEL_AUTO) -> list:
+    """Gradients of feats, weight (in ``weight_dtype``) and bias (in ``bias_dtype``), None where
+    ``needs`` says so; the arguments are linear_forward's, with its kept product."""
+    lib = load_library()
+    dev = _require_cuda(grad_out, preact, feats, weight)
+    M, Ci = feats.shape
+    Co = weight.shape[0]
+    dtype = feats.dtype
+    _matrix(grad_out, (M, Co), dtype, "grad_out")
+    weight = weight.contiguous()
+    code = DTYPE_CODES[dtype]
+
+    def grad(shape, wanted):                 # in the wanted dtype where the kernels write it
+        return torch.empty(shape, dtype=wanted if wanted == dtype else torch.float32, device=dev)
+    gx = torch.empty_like(feats) if needs[0] else None
+    gw = grad((Co, Ci), weight_dtype) if needs[1] else None
+    gb = grad((Co,), bias_dtype) if needs[2] else None
+    need = lib.spconv_linear_backward_workspace_bytes(code, M, Ci, Co, ACTIVATIONS[activation])
+    ws = torch.empty((max(need, 256),), dtype=torch.uint8, device=dev)
+    before_launch(dev)
+    rc = lib.spconv_linear_backward(
+        grad_out.data_ptr(), _ptr(preact), feats.data_ptr(), weight.data_ptr(), code, M, Ci, Co,
+        ACTIVATIONS[activation], _ptr(gx), _ptr(gw), 0 if gw is None else DTYPE_CODES[gw.dtype], _ptr(gb),
+        0 if gb is None else DTYPE_CODES[gb.dtype], ws.data_ptr(), need, kernel,
+        status_word(dev).word.data_ptr(), _stream_ptr(dev))
+    if rc != SPCONV_OK:
+        _raise(rc, "spconv_linear_backward")
+    if dtype != torch.float32:
+        after_launch(dev)
+    return [gx, None if gw is None else gw.to(weight_dtype), None if gb is None else gb.to(bias_dtype)]
+
+
+def _norm_args(feats: torch.Tensor, residual, params, offsets, residual_scale: float, norm: str,
+               next_norm: str, eps: float) -> ResidualNormArgs:
+    """Checked arguments shared by the forward and the backward; ``params`` are the gate, weight,
+    bias, next_weight and next_bias (each None, [C] or [samples, C])."""
+    dev = _require_cuda(feats, residual, *params, offsets)
+    if feats.dtype not in DTYPE_CODES:
+        raise TypeError(f"unsupported feature dtype {feats.dtype}")
+    if feats.dim() != 2 or feats.shape[1] < 1:
+        raise ValueError(f"feats must be an [M, C] tensor, got shape {list(feats.shape)}")
+    if not feats.is_contiguous():
+        raise ValueError("feats must be contiguous")
+    if norm not in NORMS or next_norm not in NORMS:
+        raise ValueError(f"unsupported norm {norm if norm not in NORMS else next_norm}")
+    if not eps >= 0.0:
+        raise ValueError(f"eps must be >= 0, got {eps}")
+    M, C = feats.shape
+    a = ResidualNormArgs(dtype=DTYPE_CODES[feats.dtype], channels=C, num_rows=M, feats=feats.data_ptr(),
+                         num_samples=1, norm=NORMS[norm], next_norm=NORMS[next_norm],
+                         residual_scale=residual_scale, eps=eps)
+    if residual is not None:
+        _matrix(residual, feats.shape, feats.dtype, "residual")
+        a.residual = residual.data_ptr()
+    per_sample = False
+    for name, p in zip(("gate", "weight", "bias", "next_weight", "next_bias"), params):
+        if p is None:
+            continue
+        if (name in ("weight", "bias") and norm == "none") or (name[:5] == "next_" and next_norm == "none"):
+            raise ValueError(f"{name} given without its norm")
+        if p.dtype != torch.float32 and p.dtype != feats.dtype:
+            raise TypeError(f"{name} must be float32 or {feats.dtype}, got {p.dtype}")
+        if not p.is_contiguous():
+            raise ValueError(f"{name} must be contiguous")
+        if p.dim() == 2:
+            if offsets is None:
+                raise ValueError(f"{name} has a row per sample: batch_offsets is needed")
+            if tuple(p.shape) != (offsets.numel() - 1, C):
+                raise ValueError(f"{name} must have shape {[offsets.numel() - 1, C]}, got {list(p.shape)}")
+            per_sample = True
+        elif p.dim() != 1 or p.shape[0] != C:
+            raise ValueError(f"{name} must have shape [{C}] or [samples, {C}], got {list(p.shape)}")
+        q = getattr(a, name)
+        q.data, q.dtype, q.per_sample = p.data_ptr(), DTYPE_CODES[p.dtype], p.dim() == 2
+    if offsets is not None:
+        if offsets.dtype != torch.int32 or offsets.dim() != 1 or offsets.numel() < 2 or not offsets.is_contiguous():
+            raise ValueError("batch_offsets must be a contiguous [samples + 1] int32 tensor")
+        if per_sample:
+            a.offsets, a.num_samples = offsets.data_ptr(), offsets.numel() - 1
+            before_launch(dev)
+            a.status = status_word(dev).word.data_ptr()
+    return a
+
+
+@_on_device
+def residual_norm_forward(feats: torch.Tensor, residual: Optional[torch.Tensor], params: Sequence[Optional[torch.Tensor]],
+                          offsets: Optional[torch.Tensor], residual_scale: float, norm: str, next_norm: str,
+                          eps: float) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """(hidden, normed) of the gated residual step (normed None without ``next_norm``)."""
+    a = _norm_args(feats, residual, params, offsets, residual_scale, norm, next_norm, eps)
+    hidden = torch.empty_like(feats)
+    normed = torch.empty_like(feats) if next_norm != "none" else None
+    a.hidden, a.normed = hidden.data_ptr(), _ptr(normed)
+    rc = load_library().spconv_residual_norm_forward(a, _stream_ptr(feats.device))
+    if rc != SPCONV_OK:
+        _raise(rc, "spconv_residual_norm_forward")
+    if a.status:
+        after_launch(feats.device)
+    return hidden, normed
+
+
+@_on_device
+def residual_norm_backward(feats: torch.Tensor, residual: Optional[torch.Tensor], params: Sequence[Optional[torch.Tensor]],
+                           offsets: Optional[torch.Tensor], residual_scale: float, norm: str, next_norm: str,
+                           eps: float, grad_hidden: Optional[torch.Tensor], grad_normed: Optional[torch.Tensor],
+                           needs: Sequence[bool]) -> list:
+    """Gradients of feats, residual, gate, weight, bias, next_weight and next_bias (None where
+    ``needs`` says so), each in its tensor's shape and dtype."""
+    lib = load_library()
+    a = _norm_args(feats, residual, params, offsets, residual_scale, norm, next_norm, eps)
+    for g, what in ((grad_hidden, "grad_hidden"), (grad_normed, "grad_normed")):
+        if g is not None:
+            _require_cuda(feats, g)
+            _matrix(g, feats.shape, feats.dtype, what)
+    a.grad_hidden, a.grad_normed = _ptr(grad_hidden), _ptr(grad_normed)
+    grads = [torch.empty_like(t) if t is not None and need else None
+             for t, need in zip((feats, residual, *params), needs)]
+    a.grad_feats, a.grad_residual = _ptr(grads[0]), _ptr(grads[1])
+    a.gate.grad, a.weight.grad, a.bias.grad = _ptr(grads[2]), _ptr(grads[3]), _ptr(grads[4])
+    a.next_weight.grad, a.next_bias.grad = _ptr(grads[5]), _ptr(grads[6])
+    if any(g is not None for g in grads[2:]):
+        a.workspace_bytes = lib.spconv_residual_norm_workspace_bytes(a.num_rows, a.channels, a.num_samples)
+        ws = torch.empty((max(a.workspace_bytes, 16),), dtype=torch.uint8, device=feats.device)
+        a.workspace = ws.data_ptr()
+    rc = lib.spconv_residual_norm_backward(a, _stream_ptr(feats.device))
+    if rc != SPCONV_OK:
+        _raise(rc, "spconv_residual_norm_backward")
+    if a.status:
+        after_launch(feats.device)
+    return grads
+
+
+def _is_dense(t: torch.Tensor) -> bool:
+    """Whether the elements fill their memory without gaps or overlap, in any order of dimensions."""
+    if t.is_contiguous():
+        return True
+    order = sorted(range(t.dim()), key=lambda d: (t.stride(d), t.size(d)), reverse=True)
+    return t.permute(order).is_contiguous()
+
+
+@_on_device
+def clip_gradients(grads: Sequence[torch.Tensor], outs: Sequence[torch.Tensor], max_norm: float,
+                   norm_kind: int) -> torch.Tensor:
+    """outs[k] = grads[k] * min(1, max_norm / (norm + 1e-6)); returns the norm (0-dim float32)."""
+    lib = load_library()
+    dev = grads[0].device
+    for g, o in zip(grads, outs):
+        if not g.is_cuda or g.device != dev or o.device != dev:
+            _require_cuda(*grads, *outs)
+        if g.dtype not in DTYPE_CODES:
+            raise TypeError(f"unsupported gradient dtype {g.dtype}")
+        if o is not g and (o.dtype != g.dtype or o.shape != g.shape or o.stride() != g.stride()):
+            raise ValueError("each output must have its gradient's shape, strides and dtype")
+        if not g.is_contiguous() and not _is_dense(g):
+            raise ValueError("gradients must be dense in memory")
+    n = len(grads)
+    ptrs = array.array("Q", [g.data_ptr() for g in grads])
+    optrs = ptrs if outs is grads else array.array("Q", [o.data_ptr() for o in outs])
+    sizes = array.array("q", [g.numel() for g in grads])
+    codes = array.array("i", [DTYPE_CODES[g.dtype] for g in grads])
+    total = torch.empty((), dtype=torch.float32, device=dev)
+    need = lib.spconv_clip_gradients_workspace_bytes(n)
+    ws = torch.empty((need,), dtype=torch.uint8, device=dev)
+    rc = lib.spconv_clip_gradients(ptrs.buffer_info()[0], optrs.buffer_info()[0], sizes.buffer_info()[0],
+                                   codes.buffer_info()[0], n, norm_kind, max_norm, total.data_ptr(),
+                                   ws.data_ptr(), need, _stream_ptr(dev))
+    if rc != SPCONV_OK:
+        _raise(rc, "spconv_clip_gradients")
+    return total
 
 
 def set_wait_limit_ns(limit_ns: int) -> int:

@@ -48,6 +48,12 @@ class SparseConvTensor(metaclass=ProxyableClassMeta):
             "Use 'x = x.replace_feature(new_feature)'"
             "to generate new SparseConvTensor instead.")
 
+    def batch_offsets(self) -> torch.Tensor:
+        """[batch_size + 1] int32 first row of each sample, for indices in the order of their
+        batch column (what ``from_dense`` gives)."""
+        ends = torch.arange(self.batch_size + 1, dtype=self.indices.dtype, device=self.indices.device)
+        return torch.searchsorted(self.indices[:, 0].contiguous(), ends, out_int32=True)
+
     @classmethod
     def from_dense(cls, x: torch.Tensor) -> "SparseConvTensor":
         """Channels-last dense [B, *spatial, C] -> sparse; a voxel is active iff any of
