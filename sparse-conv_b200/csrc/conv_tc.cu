@@ -35,6 +35,7 @@
 
 #include "common.cuh"
 #include "conv_internal.h"
+#include "tensor_map.h"
 
 namespace spconv {
 
@@ -778,13 +779,11 @@ static EncodeTiledFn tensor_map_encoder() {
     return fn;
 }
 
-// 2-D row-major tensor of 16-bit elements: `cols` x `rows`, rows `row_stride` bytes apart;
-// box = box_cols x box_rows; swizzle width = box_cols * 2 bytes.
-static bool make_tmap_2d(CUtensorMap *map, const void *ptr, uint64_t cols, uint64_t rows,
+bool make_tmap_2d(CUtensorMap *map, const void *ptr, uint64_t cols, uint64_t rows,
                          uint64_t row_stride, uint32_t box_cols, uint32_t box_rows) {
     EncodeTiledFn enc = tensor_map_encoder();
     if (!enc) {
-        set_error("tcgen05 conv: cuTensorMapEncodeTiled is not available from the driver");
+        set_error("cuTensorMapEncodeTiled is not available from the driver");
         return false;
     }
     const cuuint64_t dims[2] = {cols, rows};
@@ -798,7 +797,7 @@ static bool make_tmap_2d(CUtensorMap *map, const void *ptr, uint64_t cols, uint6
                            box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, sw, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) {
-        set_error("tcgen05 conv: tensor map encoding failed (CUresult %d)", (int)r);
+        set_error("tensor map encoding failed (CUresult %d)", (int)r);
         return false;
     }
     return true;

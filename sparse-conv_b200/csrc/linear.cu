@@ -288,7 +288,9 @@ static int check_linear(int dtype, int64_t M, int Ci, int Co, int activation, in
 }
 
 static int launch_gemm(const GemmArgs &g, int kernel_choice) {
-    SPCONV_REQUIRE(kernel_choice != SPCONV_KERNEL_TCGEN05, SPCONV_ERR_UNSUPPORTED, "no tensor-core kernel for this call");
+    if (kernel_choice != SPCONV_KERNEL_SIMT && gemm_tc_supported(g)) return launch_gemm_tc(g);
+    SPCONV_REQUIRE(kernel_choice != SPCONV_KERNEL_TCGEN05, SPCONV_ERR_UNSUPPORTED,
+                   "the tensor-core kernel needs fp16 or bf16, channels in eights and 16-byte aligned tensors");
     return launch_gemm_simt(g);
 }
 
@@ -323,7 +325,7 @@ extern "C" int spconv_linear_forward(const void *feats, int dtype, int64_t M, in
 extern "C" int64_t spconv_linear_backward_workspace_bytes(int dtype, int64_t M, int Ci, int Co, int activation) {
     if (check_linear(dtype, M, Ci, Co, activation, SPCONV_KERNEL_AUTO) != SPCONV_OK) return -1;
     return pad256(activation == SPCONV_ACT_NONE ? 0 : M * Co * elt(dtype)) + pad256((int64_t)dact_chunks(M) * Co * 4) +
-           pad256((int64_t)wgrad_splits(M, Ci, Co) * Co * Ci * 4);
+           pad256((int64_t)std::max(wgrad_splits(M, Ci, Co), gemm_tc_splits(Co, Ci, M)) * Co * Ci * 4);
 }
 
 extern "C" int spconv_linear_backward(const void *grad_out, const void *preact, const void *feats, const void *weight,
@@ -387,10 +389,12 @@ extern "C" int spconv_linear_backward(const void *grad_out, const void *preact, 
         g.N = Ci;
         g.K = M;
         g.out = nullptr;
-        g.splits = wgrad_splits(M, Ci, Co);
-        g.k_per_split = (M + g.splits - 1) / g.splits;
-        g.splits = (int)((M + g.k_per_split - 1) / g.k_per_split);
         g.partial = weight_part;
+        const bool tc = kernel_choice != SPCONV_KERNEL_SIMT && gemm_tc_supported(g);
+        g.splits = tc ? gemm_tc_splits(Co, Ci, M) : wgrad_splits(M, Ci, Co);
+        const int64_t step = tc ? 64 : 1;    // the tensor-core kernel's K step
+        g.k_per_split = ((M + g.splits - 1) / g.splits + step - 1) / step * step;
+        g.splits = (int)((M + g.k_per_split - 1) / g.k_per_split);
         if (const int rc = launch_gemm(g, kernel_choice)) return rc;
         if (const int rc = launch_reduce(weight_part, g.splits, (int64_t)Co * Ci, weight_dtype, grad_weight, st)) return rc;
     }

@@ -27,4 +27,11 @@ struct GemmArgs {
 
 int launch_gemm_simt(const GemmArgs &g);
 
+// Tensor-core form (linear_tc.cu): fp16 / bf16, rows and pointers aligned for TMA. Splits need
+// a_t && b_t, and k_per_split a multiple of 64.
+bool gemm_tc_supported(const GemmArgs &g);
+int launch_gemm_tc(const GemmArgs &g);
+// Splits of K for an [M, N] sum over K.
+int gemm_tc_splits(int64_t M, int64_t N, int64_t K);
+
 }  // namespace spconv

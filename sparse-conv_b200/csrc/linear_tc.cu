@@ -1,0 +1,505 @@
+// Matrix products of the pointwise linear layer on the 5th-generation tensor cores (tcgen05 /
+// TMEM), fp16 and bf16 with fp32 accumulation:
+//
+//   forward         out[M, Co]  = residual + act(feats[M, Ci] W[Co, Ci]^T + bias)   (and its argument)
+//   input gradient  gx[M, Ci]   = dz[M, Co] W[Co, Ci]                    B read along its rows
+//   weight gradient gw[Co, Ci]  = dz[M, Co]^T feats[M, Ci]               A and B read along their rows
+//
+// One persistent CTA per SM walks 128 x BN output tiles (BN = 64, 128 or 256, the last tile of a
+// row as narrow as the matrix). Operands come by TMA as 128-byte-swizzled tiles of 64 K values:
+// a K-contiguous operand as rows of 128 bytes (K-major), the others as blocks of 64 K rows of 64
+// columns (MN-major descriptors), so no operand is ever transposed in memory. Roles, coupled by
+// mbarriers only:
+//   warp 0      loads: A and B tiles of each K step into a ring of stages. Where the whole of B's
+//               column block fits beside the ring it is loaded once and stays (few K steps: the
+//               layers over millions of voxels, whose bound is HBM);
+//   warp 1      MMA: one thread; accumulators alternate between two TMEM buffers;
+//   warps 4-7 and 8-11: two epilogue groups, one for each TMEM buffer: 64 columns at a time from
+//               TMEM to registers, + bias, act, + residual, one rounding, into swizzled shared
+//               memory and out by TMA (which clips ragged edges). The residual arrives by TMA in the
+//               slot the output leaves from, one block ahead.
+// The weight gradient's K is the voxels: K is cut into splits, each writes fp32 sums of its own,
+// and linear_reduce_kernel adds them in a fixed order.
+// Every wait is bounded (the conv kernels' limit); a timeout raises SPCONV_STATUS_WAIT_TIMEOUT and
+// the CTA waits (bounded) for its own copies and MMAs before it frees TMEM and exits.
+#include <algorithm>
+#include <mutex>
+
+#include "activation.cuh"
+#include "common.cuh"
+#include "linear_internal.h"
+#include "tensor_map.h"
+
+namespace spconv {
+
+constexpr int kLtThreads = 384;
+constexpr int kLtBM = 128, kLtBK = 64;
+constexpr int kLtABytes = kLtBM * kLtBK * 2;            // 16 KB a stage
+constexpr int kLtEpiWarps = 8;
+constexpr int kLtSlot = 32 * 128;                       // 32 rows of 64 columns
+constexpr int kLtMaxStages = 12;
+constexpr int kLtMaxSlots = 4;
+constexpr int kLtMaxSmem = 227 * 1024;
+// behind the tiles: bias (256 fp32 for each epilogue warp: no barrier among them), barriers, TMEM address and abort flag
+constexpr int kLtBars = 2 * kLtMaxStages + 1 + 4 + kLtEpiWarps * kLtMaxSlots;
+constexpr int kLtTail = kLtEpiWarps * 256 * 4 + kLtBars * 8 + 16;
+
+struct LtArgs {
+    int M, N;
+    int64_t K;
+    int nb;                                 // column blocks
+    int64_t tiles;                          // row tiles * nb
+    int64_t items;                          // tiles * splits
+    int64_t k_per_split;                    // a multiple of 64 unless splits == 1
+    int BN, stages, slots;                  // slots per epilogue warp (outputs; as many again for preact)
+    int b_resident;                         // K steps of B that stay in shared memory, or 0
+    const void *bias;
+    int has_residual, has_preact;
+    float *partial;
+    int32_t *status;
+    uint64_t wait_ns;
+};
+
+__device__ __forceinline__ void lt_wait_read(int pending) {
+    if (pending <= 0) bulk_wait_read<0>();
+    else if (pending == 1) bulk_wait_read<1>();
+    else if (pending == 2) bulk_wait_read<2>();
+    else bulk_wait_read<3>();
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t lt_pack(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t lt_pack<__half>(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t lt_pack<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+template <typename T>
+__device__ __forceinline__ float2 lt_unpack(uint32_t v);
+template <>
+__device__ __forceinline__ float2 lt_unpack<__half>(uint32_t v) {
+    return __half22float2(*reinterpret_cast<const __half2 *>(&v));
+}
+template <>
+__device__ __forceinline__ float2 lt_unpack<__nv_bfloat16>(uint32_t v) {
+    return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+}
+
+template <typename T, bool A_T, bool B_T, int ACT>
+__global__ void __launch_bounds__(kLtThreads, 1)
+linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                 const __grid_constant__ CUtensorMap map_out, const __grid_constant__ CUtensorMap map_res,
+                 const __grid_constant__ CUtensorMap map_pre, const __grid_constant__ LtArgs a) {
+    constexpr bool PARTIAL = A_T;           // the weight gradient: fp32 sums of a split
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *base = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    const int BN = a.BN, S = a.stages, NO = a.slots;
+    const int b_bytes = BN * 128;
+    const int stage_bytes = kLtABytes + (a.b_resident ? 0 : b_bytes);
+    const uint32_t s_b = smem_u32(base);                               // resident B
+    const uint32_t s_stage = s_b + a.b_resident * b_bytes;
+    const int warp_slots = NO * (a.has_preact ? 2 : 1);
+    const uint32_t s_out = s_stage + S * stage_bytes;
+    uint8_t *tail = base + a.b_resident * b_bytes + S * stage_bytes + (PARTIAL ? 0 : kLtEpiWarps * warp_slots * kLtSlot);
+    float *s_bias = reinterpret_cast<float *>(tail);                   // [kLtEpiWarps][256]
+    uint64_t *bar = reinterpret_cast<uint64_t *>(tail + kLtEpiWarps * 256 * 4);
+    uint64_t *full = bar, *empty = full + kLtMaxStages, *bfull = empty + kLtMaxStages, *accfull = bfull + 1;
+    uint64_t *accempty = accfull + 2, *rbar = accempty + 2;
+    uint32_t *s_tmem = reinterpret_cast<uint32_t *>(bar + kLtBars);
+    volatile int *s_abort = reinterpret_cast<volatile int *>(s_tmem + 1);
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int64_t G = gridDim.x;
+    const uint32_t tmem_cols = (uint32_t)(2 * BN);                     // 128, 256 or 512
+    if (tid == 0) {
+        for (int s = 0; s < S; ++s) {
+            mbar_init(smem_u32(&full[s]), 1);
+            mbar_init(smem_u32(&empty[s]), 1);
+        }
+        mbar_init(smem_u32(bfull), 1);
+        for (int g = 0; g < 2; ++g) {
+            mbar_init(smem_u32(&accfull[g]), 1);
+            mbar_init(smem_u32(&accempty[g]), 4);
+        }
+        for (int i = 0; i < kLtEpiWarps * NO; ++i) mbar_init(smem_u32(&rbar[i]), 1);
+        *s_abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    }
+    if (warp == 1) {
+        tmem_alloc(smem_u32(s_tmem), tmem_cols);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *s_tmem;
+    auto wait = [&](uint64_t *b, uint32_t parity) -> bool {
+        return mbar_wait_or_abort(smem_u32(b), parity, s_abort, a.wait_ns);
+    };
+    // item -> (m0, n0) and its range of K
+    auto place = [&](int64_t item, int &m0, int &n0, int64_t &k0, int64_t &k1, int64_t &split) {
+        split = PARTIAL ? item / a.tiles : 0;
+        const int64_t tile = item - split * a.tiles;
+        m0 = (int)(tile / a.nb) * kLtBM;
+        n0 = (int)(tile % a.nb) * BN;
+        k0 = split * a.k_per_split;
+        k1 = PARTIAL ? min(a.K, k0 + a.k_per_split) : a.K;
+    };
+
+    if (warp == 0) {
+        // ------------------------------------------------------------------ loads
+        if (lane == 0) {
+            auto load_b = [&](uint32_t dst, int k, int n0, uint32_t mbar) {
+                if constexpr (B_T) {
+                    for (int c = 0; c < BN / 64; ++c) tma_load_2d(dst + c * 8192, &map_b, n0 + c * 64, k, mbar);
+                } else {
+                    tma_load_2d(dst, &map_b, k, n0, mbar);
+                }
+            };
+            int64_t cnt = 0;
+            bool ok = true;
+            if (a.b_resident && (int64_t)blockIdx.x < a.items) {      // the grid is a multiple of nb: n0 never changes
+                int m0, n0;
+                int64_t k0, k1, split;
+                place(blockIdx.x, m0, n0, k0, k1, split);
+                mbar_arrive_expect_tx(smem_u32(bfull), (uint32_t)(a.b_resident * b_bytes));
+                for (int c = 0; c < a.b_resident; ++c) load_b(s_b + c * b_bytes, c * kLtBK, n0, smem_u32(bfull));
+            }
+            for (int64_t item = blockIdx.x; item < a.items && ok; item += G) {
+                int m0, n0;
+                int64_t k0, k1, split;
+                place(item, m0, n0, k0, k1, split);
+                for (int64_t k = k0; k < k1; k += kLtBK, ++cnt) {
+                    const int s = (int)(cnt % S);
+                    const int64_t u = cnt / S;
+                    if (u > 0 && !wait(&empty[s], (uint32_t)((u - 1) & 1))) { ok = false; break; }
+                    const uint32_t mbar = smem_u32(&full[s]), dst = s_stage + s * stage_bytes;
+                    mbar_arrive_expect_tx(mbar, (uint32_t)stage_bytes);
+                    if constexpr (A_T) {
+                        tma_load_2d(dst, &map_a, m0, (int)k, mbar);
+                        tma_load_2d(dst + 8192, &map_a, m0 + 64, (int)k, mbar);
+                    } else {
+                        tma_load_2d(dst, &map_a, (int)k, m0, mbar);
+                    }
+                    if (!a.b_resident) load_b(dst + kLtABytes, (int)k, n0, mbar);
+                }
+            }
+            // every load has landed before the CTA may exit (at once unless the MMA gave up)
+            for (int64_t j = max((int64_t)0, cnt - S); j < cnt; ++j)
+                mbar_wait_bounded(smem_u32(&full[j % S]), (uint32_t)((j / S) & 1), kTmaDrainNs);
+            if (a.b_resident && (int64_t)blockIdx.x < a.items) mbar_wait_bounded(smem_u32(bfull), 0, kTmaDrainNs);
+        }
+    } else if (warp == 1) {
+        // ------------------------------------------------------------------ MMA
+        if (lane == 0) {
+            int64_t cnt = 0, it = 0;
+            bool ok = true;
+            if (a.b_resident && (int64_t)blockIdx.x < a.items) ok = wait(bfull, 0);
+            for (int64_t item = blockIdx.x; item < a.items && ok; item += G, ++it) {
+                int m0, n0;
+                int64_t k0, k1, split;
+                place(item, m0, n0, k0, k1, split);
+                const int g = (int)(it & 1);
+                const int64_t u = it >> 1;
+                if (u > 0 && !wait(&accempty[g], (uint32_t)((u - 1) & 1))) { ok = false; break; }
+                tc_fence_after();
+                const int n_mma = (min(BN, a.N - n0) + 15) & ~15;
+                const uint32_t idesc = instr_desc_f16(dtype_traits<T>::mma_format, kLtBM, n_mma) |
+                                       (A_T ? 1u << 15 : 0u) | (B_T ? 1u << 16 : 0u);
+                const uint32_t d = tmem + (uint32_t)(g * BN);
+                for (int64_t k = k0; k < k1; k += kLtBK, ++cnt) {
+                    const int s = (int)(cnt % S);
+                    if (!wait(&full[s], (uint32_t)((cnt / S) & 1))) { ok = false; break; }
+                    tc_fence_after();
+                    const uint32_t sa = s_stage + s * stage_bytes;
+                    const uint32_t sb = a.b_resident ? s_b + (uint32_t)(k / kLtBK) * b_bytes : sa + kLtABytes;
+                    const int steps = (int)min((int64_t)4, (k1 - k + 15) / 16);   // zeros past K's end are skipped
+                    for (int kk = 0; kk < steps; ++kk) {
+                        const uint64_t ad = A_T ? smem_desc_mn_sw128(sa + kk * 2048, 8192, 1024)
+                                                : smem_desc_kmajor_swizzled(sa + kk * 32, 128);
+                        const uint64_t bd = B_T ? smem_desc_mn_sw128(sb + kk * 2048, 8192, 1024)
+                                                : smem_desc_kmajor_swizzled(sb + kk * 32, 128);
+                        tc_mma_f16(d, ad, bd, idesc, (k > k0 || kk > 0) ? 1u : 0u);
+                    }
+                    tc_commit(smem_u32(&empty[s]));
+                }
+                if (ok) tc_commit(smem_u32(&accfull[g]));
+            }
+            if (!ok && cnt > 0)              // MMAs in flight read shared memory: wait for the last commit
+                mbar_wait_bounded(smem_u32(&empty[(cnt - 1) % S]), (uint32_t)(((cnt - 1) / S) & 1));
+        }
+    } else if (warp >= 4) {
+        // ------------------------------------------------------------------ epilogue
+        const int g = (warp - 4) >> 2, quad = warp & 3, ew = warp - 4;
+        float *bias_s = s_bias + ew * 256;
+        const uint32_t t_acc = tmem + (uint32_t)(g * BN) + ((uint32_t)(quad * 32) << 16);
+        const uint32_t slot0 = s_out + (uint32_t)(ew * warp_slots * kLtSlot);
+        const uint32_t pre0 = slot0 + (uint32_t)(NO * kLtSlot);
+        uint64_t *my_rbar = rbar + ew * NO;
+        const uint32_t row_at = (uint32_t)(lane * 128);
+        // one answer for the warp: its lanes must not part before the next warp-wide instruction
+        auto all_wait = [&](uint64_t *b, uint32_t parity) { return __all_sync(0xffffffffu, wait(b, parity)) != 0; };
+        int n_bias = -1;
+        int64_t blk = 0, loads = 0;          // blocks begun; residual loads issued
+        // the residual's block into its slot; `behind`: later stores that may still be reading theirs
+        auto load_residual = [&](int m, int n, int behind) {
+            if (lane == 0) {
+                lt_wait_read(behind);
+                const int s = (int)(loads % NO);
+                mbar_arrive_expect_tx(smem_u32(&my_rbar[s]), kLtSlot);
+                tma_load_2d(slot0 + s * kLtSlot, &map_res, n, m, smem_u32(&my_rbar[s]));
+            }
+            ++loads;
+        };
+        int64_t use = 0;
+        for (int64_t item = blockIdx.x + g * G; item < a.items; item += 2 * G, ++use) {
+            int m0, n0;
+            int64_t k0, k1, split;
+            place(item, m0, n0, k0, k1, split);
+            const int n_cols = min(BN, a.N - n0), blocks = (n_cols + 63) >> 6;
+            if (!PARTIAL && a.bias && n0 != n_bias) {
+                __syncwarp();
+                for (int i = lane; i < BN; i += 32)
+                    bias_s[i] = n0 + i < a.N ? dtype_traits<T>::to_f(((const T *)a.bias)[n0 + i]) : 0.f;
+                __syncwarp();
+                n_bias = n0;
+            }
+            // the group's next tile, for the residual of its first block
+            int m_next = -1, n_next = 0;
+            if (!PARTIAL && a.has_residual) {
+                if (item + 2 * G < a.items) place(item + 2 * G, m_next, n_next, k0, k1, split);
+                if (use == 0 && NO > 1) load_residual(m0 + quad * 32, n0, 0);
+            }
+            if (!all_wait(&accfull[g], (uint32_t)(use & 1))) break;
+            tc_fence_after();
+            bool ok = true;
+            for (int j = 0; j < blocks; ++j, ++blk) {
+                const int s = (int)(blk % NO);
+                const uint32_t so = slot0 + s * kLtSlot + row_at, sp = pre0 + s * kLtSlot + row_at;
+                if constexpr (!PARTIAL) {
+                    if (a.has_residual) {
+                        if (NO == 1) load_residual(m0 + quad * 32, n0 + j * 64, 0);
+                        else if (j + 1 < blocks) load_residual(m0 + quad * 32, n0 + (j + 1) * 64, NO - 2);
+                        else if (m_next >= 0) load_residual(m_next + quad * 32, n_next, NO - 2);
+                        if (!all_wait(&my_rbar[s], (uint32_t)((blk / NO) & 1))) { ok = false; break; }
+                    } else {
+                        if (lane == 0) lt_wait_read(NO - 1);
+                    }
+                    __syncwarp();
+                }
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    uint32_t r[32];
+                    tmem_ld32(t_acc + (uint32_t)(j * 64 + c * 32), r);
+                    tc_wait_ld();
+                    if constexpr (PARTIAL) {
+                        const int row = m0 + quad * 32 + lane;
+                        float *dst = a.partial + (split * a.M + row) * (int64_t)a.N + n0 + j * 64 + c * 32;
+                        if (row < a.M) {
+#pragma unroll
+                            for (int v = 0; v < 8; ++v)
+                                if (j * 64 + c * 32 + v * 4 < n_cols)
+                                    __stcg(reinterpret_cast<float4 *>(dst) + v,
+                                           make_float4(__uint_as_float(r[4 * v]), __uint_as_float(r[4 * v + 1]),
+                                                       __uint_as_float(r[4 * v + 2]), __uint_as_float(r[4 * v + 3])));
+                        }
+                    } else {
+#pragma unroll
+                        for (int v = 0; v < 4; ++v) {
+                            const uint32_t at = (uint32_t)(((c * 4 + v) ^ (lane & 7)) << 4);
+                            float f[8];
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(r[8 * v + i]);
+                            if (a.bias) {
+                                const float4 *b4 = reinterpret_cast<const float4 *>(bias_s + j * 64 + c * 32 + v * 8);
+                                const float4 b0 = b4[0], b1 = b4[1];
+                                f[0] += b0.x; f[1] += b0.y; f[2] += b0.z; f[3] += b0.w;
+                                f[4] += b1.x; f[5] += b1.y; f[6] += b1.z; f[7] += b1.w;
+                            }
+                            if (a.has_preact)
+                                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" :: "r"(sp + at),
+                                             "r"(lt_pack<T>(f[0], f[1])), "r"(lt_pack<T>(f[2], f[3])),
+                                             "r"(lt_pack<T>(f[4], f[5])), "r"(lt_pack<T>(f[6], f[7])) : "memory");
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) f[i] = act_value<ACT>(f[i]);
+                            if (a.has_residual) {
+                                uint32_t q[4];
+                                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];\n"
+                                             : "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3]) : "r"(so + at) : "memory");
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    const float2 x = lt_unpack<T>(q[i]);
+                                    f[2 * i] += x.x;
+                                    f[2 * i + 1] += x.y;
+                                }
+                            }
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" :: "r"(so + at),
+                                         "r"(lt_pack<T>(f[0], f[1])), "r"(lt_pack<T>(f[2], f[3])),
+                                         "r"(lt_pack<T>(f[4], f[5])), "r"(lt_pack<T>(f[6], f[7])) : "memory");
+                        }
+                    }
+                }
+                if (j + 1 == blocks) {       // the accumulator is in registers: free for the MMA
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_u32(&accempty[g]));
+                }
+                if constexpr (!PARTIAL) {
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (m0 + quad * 32 < a.M) {
+                            tma_store_2d(&map_out, n0 + j * 64, m0 + quad * 32, slot0 + s * kLtSlot);
+                            if (a.has_preact) tma_store_2d(&map_pre, n0 + j * 64, m0 + quad * 32, pre0 + s * kLtSlot);
+                        }
+                        bulk_commit();       // one group a block, empty or not
+                    }
+                }
+            }
+            if (!ok) break;
+        }
+        if (!PARTIAL && lane == 0) {
+            for (int64_t j = max(blk, loads - NO); j < loads; ++j)      // residual loads nobody waited for
+                mbar_wait_bounded(smem_u32(&my_rbar[j % NO]), (uint32_t)((j / NO) & 1), kTmaDrainNs);
+            bulk_wait<0>();
+        }
+    }
+
+    __syncwarp();
+    if (*s_abort && tid == 0) raise_status(a.status, SPCONV_STATUS_WAIT_TIMEOUT);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 1) tmem_dealloc(tmem, tmem_cols);
+}
+
+// ---------------------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------------------
+static int lt_sms() {
+    static std::once_flag once;
+    static int sms = 148;
+    std::call_once(once, [] {
+        int dev = 0;
+        if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    });
+    return sms;
+}
+
+bool gemm_tc_supported(const GemmArgs &g) {
+    if (g.dtype != SPCONV_F16 && g.dtype != SPCONV_BF16) return false;
+    // TMA: rows a multiple of 16 bytes apart, 16-byte aligned tensors
+    const int64_t a_row = g.a_t ? g.M : g.K, b_row = g.b_t ? g.N : g.K;
+    if (a_row % 8 || b_row % 8 || g.N % 8) return false;
+    for (const void *p : {g.a, g.b, (const void *)g.out, g.residual, (const void *)g.preact, (const void *)g.partial})
+        if ((uintptr_t)p & 15) return false;
+    return true;
+}
+
+// Columns of a tile: the widest of 256, 128, 64 that the matrix fills to more than half (each
+// operand is then read least often), narrowed while the tiles are fewer than the SMs.
+static int lt_bn(int64_t M, int64_t N, int splits) {
+    int bn = N > 128 ? 256 : N > 64 ? 128 : 64;
+    const int64_t mt = (M + kLtBM - 1) / kLtBM * splits;
+    while (bn > 64 && mt * ((N + bn - 1) / bn) < lt_sms()) bn >>= 1;
+    return bn;
+}
+
+int gemm_tc_splits(int64_t M, int64_t N, int64_t K) {
+    // whole waves of 148 items; each split costs a write and a read of fp32 sums
+    const int64_t tiles = ((M + kLtBM - 1) / kLtBM) * ((N + 255) / 256);
+    const int64_t chunks = (K + kLtBK - 1) / kLtBK;
+    const int64_t most = std::max<int64_t>(1, std::min<int64_t>(chunks / 4, lt_sms()));
+    int64_t best = 1;
+    double best_cost = 1e30;
+    for (int64_t s = 1; s <= most; ++s) {
+        const int64_t waves = (s * tiles + lt_sms() - 1) / lt_sms();
+        const double cost = (double)waves * ((chunks + s - 1) / s + 4) + 0.02 * s * tiles;
+        if (cost < best_cost) {
+            best_cost = cost;
+            best = s;
+        }
+    }
+    return (int)best;
+}
+
+template <typename T, bool A_T, bool B_T, int ACT>
+static int lt_launch(const GemmArgs &g) {
+    LtArgs a = {};
+    a.M = (int)g.M;
+    a.N = (int)g.N;
+    a.K = g.K;
+    a.BN = A_T ? (g.N > 128 ? 256 : g.N > 64 ? 128 : 64) : lt_bn(g.M, g.N, g.splits);
+    a.nb = (int)((g.N + a.BN - 1) / a.BN);
+    a.tiles = (g.M + kLtBM - 1) / kLtBM * a.nb;
+    a.items = a.tiles * g.splits;
+    a.k_per_split = g.splits > 1 ? g.k_per_split : g.K;
+    a.bias = g.bias;
+    a.has_residual = g.residual != nullptr;
+    a.has_preact = g.preact != nullptr;
+    a.partial = g.partial;
+    a.status = g.status;
+    a.wait_ns = wait_limit_ns();
+    const int sms = lt_sms();
+    int64_t grid = std::min<int64_t>(sms, a.items);
+    const int64_t nk = (g.K + kLtBK - 1) / kLtBK;
+    const int b_bytes = a.BN * 128, room = kLtMaxSmem - 1024 - kLtTail;
+    auto fit = [&](int resident) {          // output slots and stages beside `resident` K steps of B
+        const int stage = kLtABytes + (resident ? 0 : b_bytes);
+        for (int slots = A_T ? 1 : 4; slots >= 1; slots >>= 1) {
+            const int out = A_T ? 0 : kLtEpiWarps * slots * (a.has_preact ? 2 : 1) * kLtSlot;
+            const int stages = (room - resident * b_bytes - out) / stage;
+            if (stages >= 4 || (slots == 1 && stages >= 3)) {
+                a.slots = slots;
+                a.stages = std::min(stages, kLtMaxStages);
+                a.b_resident = resident;
+                return true;
+            }
+        }
+        return false;
+    };
+    // B stays where a CTA meets it again (more than one row tile per CTA) and its block fits
+    const bool stay = !A_T && a.nb <= sms && a.items > grid && nk * b_bytes <= 96 * 1024 && fit((int)nk);
+    if (stay) grid = sms / a.nb * a.nb;
+    else if (!fit(0)) {
+        set_error("linear: no shared-memory layout for this shape");
+        return SPCONV_ERR_UNSUPPORTED;
+    }
+    const int smem = 1024 + kLtTail + a.b_resident * b_bytes + a.stages * (kLtABytes + (a.b_resident ? 0 : b_bytes)) +
+                     (A_T ? 0 : kLtEpiWarps * a.slots * (a.has_preact ? 2 : 1) * kLtSlot);
+    CUtensorMap ma, mb, mo, mr, mp;
+    // K-contiguous operands: boxes of 64 K x rows; the others: 64 columns x 64 K rows
+    const bool maps =
+        (A_T ? make_tmap_2d(&ma, g.a, g.M, g.K, g.M * 2, 64, 64) : make_tmap_2d(&ma, g.a, g.K, g.M, g.K * 2, 64, kLtBM)) &&
+        (B_T ? make_tmap_2d(&mb, g.b, g.N, g.K, g.N * 2, 64, 64) : make_tmap_2d(&mb, g.b, g.K, g.N, g.K * 2, 64, a.BN)) &&
+        (A_T || make_tmap_2d(&mo, g.out, g.N, g.M, g.N * 2, 64, 32)) &&
+        (!g.residual || make_tmap_2d(&mr, g.residual, g.N, g.M, g.N * 2, 64, 32)) &&
+        (!g.preact || make_tmap_2d(&mp, g.preact, g.N, g.M, g.N * 2, 64, 32));
+    if (!maps) return SPCONV_ERR_CUDA;
+    if (A_T) mo = ma;                       // maps that the kernel does not read
+    if (!g.residual) mr = ma;
+    if (!g.preact) mp = ma;
+    auto kern = linear_tc_kernel<T, A_T, B_T, ACT>;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kLtMaxSmem) != cudaSuccess)
+        return check_launch("linear_tc: set max dynamic shared memory");
+    kern<<<(unsigned)grid, kLtThreads, smem, g.stream>>>(ma, mb, mo, mr, mp, a);
+    return check_launch("linear_tc_kernel");
+}
+
+template <typename T>
+static int lt_type(const GemmArgs &g) {
+    if (g.a_t) return lt_launch<T, true, true, SPCONV_ACT_NONE>(g);
+    if (g.b_t) return lt_launch<T, false, true, SPCONV_ACT_NONE>(g);
+    return act_dispatch(g.activation, [&](auto act) { return lt_launch<T, false, false, act.value>(g); });
+}
+
+int launch_gemm_tc(const GemmArgs &g) {
+    return g.dtype == SPCONV_F16 ? lt_type<__half>(g) : lt_type<__nv_bfloat16>(g);
+}
+
+}  // namespace spconv

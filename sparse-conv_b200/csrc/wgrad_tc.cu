@@ -73,20 +73,6 @@ static_assert(kWtPendRing > kWtDepth + 1, "gatherer signal ring");
 constexpr uint32_t kWtEnd = 0xffffffffu;
 constexpr uint32_t kWtSegFirst = 1u << 30, kWtSegLast = 1u << 29;
 
-// Shared-memory descriptor of an MN-major operand with the 128-byte swizzle: 8 K rows of 64
-// 16-bit elements (one 128-byte row per K index, 16-byte chunks XOR-ed with the row within
-// its 8-row group) form a 1024-byte atom; `sbo` = byte distance between atoms adjacent in K,
-// `lbo` = byte distance between the 64-element blocks adjacent in M/N.
-__device__ __forceinline__ uint64_t smem_desc_mn_sw128(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
-    uint64_t d = 0;
-    d |= (uint64_t)((saddr >> 4) & 0x3FFFu);
-    d |= (uint64_t)((lbo >> 4) & 0x3FFFu) << 16;
-    d |= (uint64_t)((sbo >> 4) & 0x3FFFu) << 32;
-    d |= (uint64_t)1 << 46;
-    d |= (uint64_t)2 << 61;
-    return d;
-}
-
 template <typename T>
 __global__ void __launch_bounds__(kWtThreads, 1)
 wgrad_tc_kernel(const T *__restrict__ feats, const T *__restrict__ gout, const int32_t *__restrict__ nbr,
