@@ -25,6 +25,107 @@ __device__ __forceinline__ float act_slope(float z) {
     return 1.f;
 }
 
+// ---------------------------------------------------------------------------------------
+// Two values at a time, for 16-bit features: within 2^-20 of the argument of the functions above.
+// The epilogue of a layer over millions of voxels has about 14 issue slots per output before it,
+// not HBM, sets the time, so products run as packed fp32 pairs (one slot for two) and the only
+// special-function operations are one exponential (GELU) or an exponential and a reciprocal (SiLU).
+// ---------------------------------------------------------------------------------------
+struct f32x2 { uint64_t v; };
+__device__ __forceinline__ f32x2 pack_f32x2(float a, float b) {
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 unpack_f32x2(f32x2 x) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x.v));
+    return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ float ex2_approx(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float relu_nan(float x) {          // max(x, 0), NaN stays NaN
+    float r;
+    asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// For t = min(|z|, 16): E = exp(-t^2 / 2) and -q, q = 1 - Phi(t) = E * P(t) with P a degree-9
+// polynomial for exp(t^2 / 2) (1 - Phi(t)), fitted here on [0, 4.5] for the least weighted error:
+// |dq| <= 6.5e-7 everywhere, and within 6e-4 of q itself up to t = 4. Beyond 16, E is zero.
+__device__ __forceinline__ void normal_tail2(float2 z, f32x2 &t, float2 &e, f32x2 &minus_q) {
+    t = pack_f32x2(fminf(fabsf(z.x), 16.f), fminf(fabsf(z.y), 16.f));
+    const float2 x = unpack_f32x2(mul2(mul2(t, t), pack_f32x2(-0.72134752f, -0.72134752f)));   // -log2(e) / 2
+    e = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+    constexpr float c[10] = {-0.49999940f, 0.39890096f, -0.24953401f, 0.13094953f, -0.057988375f,
+                             0.020727100f, -0.0055298521f, 9.9795568e-4f, -1.0617938e-4f, 4.9614673e-6f};
+    f32x2 p = pack_f32x2(c[9], c[9]);
+#pragma unroll
+    for (int k = 8; k >= 0; --k) p = fma2(p, t, pack_f32x2(c[k], c[k]));
+    minus_q = mul2(p, pack_f32x2(e.x, e.y));
+}
+
+// act(z) for a pair; inf and NaN as the functions above, but GELU(-inf) = 0, its limit.
+template <int ACT>
+__device__ __forceinline__ f32x2 act_value2(f32x2 z2) {
+    if constexpr (ACT == SPCONV_ACT_NONE) return z2;
+    const float2 z = unpack_f32x2(z2);
+    if constexpr (ACT == SPCONV_ACT_RELU) return pack_f32x2(relu_nan(z.x), relu_nan(z.y));
+    if constexpr (ACT == SPCONV_ACT_GELU) {                  // max(z, 0) - |z| q
+        f32x2 t, mq;
+        float2 e;
+        normal_tail2(z, t, e, mq);
+        return fma2(t, mq, pack_f32x2(relu_nan(z.x), relu_nan(z.y)));
+    }
+    const float2 x = unpack_f32x2(mul2(z2, pack_f32x2(-1.4426950f, -1.4426950f)));
+    const f32x2 d = add2(pack_f32x2(ex2_approx(x.x), ex2_approx(x.y)), pack_f32x2(1.f, 1.f));
+    const float2 d1 = unpack_f32x2(d);
+    return mul2(z2, pack_f32x2(rcp_approx(d1.x), rcp_approx(d1.y)));
+}
+
+// act'(z) for a pair.
+template <int ACT>
+__device__ __forceinline__ float2 act_slope2(float2 z) {
+    if constexpr (ACT == SPCONV_ACT_RELU) return make_float2(z.x > 0.f ? 1.f : 0.f, z.y > 0.f ? 1.f : 0.f);
+    if constexpr (ACT == SPCONV_ACT_GELU) {                  // Phi(z) + z phi(z)
+        f32x2 t, mq;
+        float2 e;
+        normal_tail2(z, t, e, mq);
+        const float2 u = unpack_f32x2(t), m = unpack_f32x2(mq);
+        // for z > 0 the slope is 1 - (q - t phi), else q - t phi
+        const float sx = fmaf(u.x * -0.39894228f, e.x, -m.x), sy = fmaf(u.y * -0.39894228f, e.y, -m.y);
+        return make_float2(z.x > 0.f ? 1.f - sx : z.x == z.x ? sx : z.x, z.y > 0.f ? 1.f - sy : z.y == z.y ? sy : z.y);
+    }
+    if constexpr (ACT == SPCONV_ACT_SILU) {
+        const float sx = rcp_approx(1.f + ex2_approx(-1.4426950f * z.x)), sy = rcp_approx(1.f + ex2_approx(-1.4426950f * z.y));
+        return make_float2(sx * (1.f + z.x * (1.f - sx)), sy * (1.f + z.y * (1.f - sy)));
+    }
+    return make_float2(1.f, 1.f);
+}
+
 // Calls f with the activation as a compile-time constant.
 template <typename F>
 inline int act_dispatch(int activation, F f) {

@@ -169,13 +169,20 @@ linear_dact_kernel(const T *__restrict__ gout, const T *__restrict__ z, T *__res
                 if constexpr (ACT != SPCONV_ACT_NONE) zv[0] = z[at];
             }
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                float d = dtype_traits<T>::to_f(gv[i]);
+            for (int i = 0; i < VEC; i += 2) {
+                float d[2] = {dtype_traits<T>::to_f(gv[i]), VEC > 1 ? dtype_traits<T>::to_f(gv[i + (VEC > 1)]) : 0.f};
                 if constexpr (ACT != SPCONV_ACT_NONE) {
-                    d *= act_slope<ACT>(dtype_traits<T>::to_f(zv[i]));
-                    gv[i] = dtype_traits<T>::from_f(d);
+                    const float z0 = dtype_traits<T>::to_f(zv[i]), z1 = VEC > 1 ? dtype_traits<T>::to_f(zv[i + (VEC > 1)]) : 0.f;
+                    const float2 slope = sizeof(T) == 2 ? act_slope2<ACT>(make_float2(z0, z1))
+                                                        : make_float2(act_slope<ACT>(z0), act_slope<ACT>(z1));
+                    d[0] *= slope.x;
+                    d[1] *= slope.y;
                 }
-                acc[i] += d;                 // the bias sums take dz before it is rounded
+#pragma unroll
+                for (int k = 0; k < (VEC > 1 ? 2 : 1); ++k) {
+                    acc[i + k] += d[k];      // the bias sums take dz before it is rounded
+                    if constexpr (ACT != SPCONV_ACT_NONE) gv[i + k] = dtype_traits<T>::from_f(d[k]);
+                }
             }
             if constexpr (ACT != SPCONV_ACT_NONE) {
                 if constexpr (VEC > 1) *reinterpret_cast<uint4 *>(dz + at) = *reinterpret_cast<uint4 *>(gv);

@@ -90,6 +90,19 @@ __device__ __forceinline__ float2 lt_unpack<__nv_bfloat16>(uint32_t v) {
     return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
 }
 
+// Eight values, rounded, as one 16-byte store to shared memory.
+template <typename T>
+__device__ __forceinline__ void lt_store8(uint32_t dst, const f32x2 (&f)[4]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 x = unpack_f32x2(f[i]);
+        w[i] = lt_pack<T>(x.x, x.y);
+    }
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n"
+                 :: "r"(dst), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+}
+
 template <typename T, bool A_T, bool B_T, int ACT>
 __global__ void __launch_bounds__(kLtThreads, 1)
 linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
@@ -312,21 +325,21 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
 #pragma unroll
                         for (int v = 0; v < 4; ++v) {
                             const uint32_t at = (uint32_t)(((c * 4 + v) ^ (lane & 7)) << 4);
-                            float f[8];
+                            f32x2 f[4];
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(r[8 * v + i]);
+                            for (int i = 0; i < 4; ++i)
+                                f[i] = pack_f32x2(__uint_as_float(r[8 * v + 2 * i]), __uint_as_float(r[8 * v + 2 * i + 1]));
                             if (a.bias) {
-                                const float4 *b4 = reinterpret_cast<const float4 *>(bias_s + j * 64 + c * 32 + v * 8);
-                                const float4 b0 = b4[0], b1 = b4[1];
-                                f[0] += b0.x; f[1] += b0.y; f[2] += b0.z; f[3] += b0.w;
-                                f[4] += b1.x; f[5] += b1.y; f[6] += b1.z; f[7] += b1.w;
+                                const ulonglong2 *b = reinterpret_cast<const ulonglong2 *>(bias_s + j * 64 + c * 32 + v * 8);
+                                const ulonglong2 b0 = b[0], b1 = b[1];
+                                f[0] = add2(f[0], {b0.x});
+                                f[1] = add2(f[1], {b0.y});
+                                f[2] = add2(f[2], {b1.x});
+                                f[3] = add2(f[3], {b1.y});
                             }
-                            if (a.has_preact)
-                                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" :: "r"(sp + at),
-                                             "r"(lt_pack<T>(f[0], f[1])), "r"(lt_pack<T>(f[2], f[3])),
-                                             "r"(lt_pack<T>(f[4], f[5])), "r"(lt_pack<T>(f[6], f[7])) : "memory");
+                            if (a.has_preact) lt_store8<T>(sp + at, f);
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) f[i] = act_value<ACT>(f[i]);
+                            for (int i = 0; i < 4; ++i) f[i] = act_value2<ACT>(f[i]);
                             if (a.has_residual) {
                                 uint32_t q[4];
                                 asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];\n"
@@ -334,13 +347,10 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
 #pragma unroll
                                 for (int i = 0; i < 4; ++i) {
                                     const float2 x = lt_unpack<T>(q[i]);
-                                    f[2 * i] += x.x;
-                                    f[2 * i + 1] += x.y;
+                                    f[i] = add2(f[i], pack_f32x2(x.x, x.y));
                                 }
                             }
-                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" :: "r"(so + at),
-                                         "r"(lt_pack<T>(f[0], f[1])), "r"(lt_pack<T>(f[2], f[3])),
-                                         "r"(lt_pack<T>(f[4], f[5])), "r"(lt_pack<T>(f[6], f[7])) : "memory");
+                            lt_store8<T>(so + at, f);
                         }
                     }
                 }
