@@ -13,11 +13,13 @@
 //   warp 0      loads: A and B tiles of each K step into a ring of stages. Where the whole of B's
 //               column block fits beside the ring it is loaded once and stays (few K steps: the
 //               layers over millions of voxels, whose bound is HBM);
-//   warp 1      MMA: one thread; accumulators alternate between two TMEM buffers;
-//   warps 4-7 and 8-11: two epilogue groups, one for each TMEM buffer: 64 columns at a time from
-//               TMEM to registers, + bias, act, + residual, one rounding, into swizzled shared
-//               memory and out by TMA (which clips ragged edges). The residual arrives by TMA in the
-//               slot the output leaves from, one block ahead.
+//   warp 1      MMA: one thread; the accumulators take turns in two (BN = 256) or four TMEM buffers;
+//   warps 2-17  four epilogue groups of four warps (one per TMEM lane quadrant), a group per
+//               buffer, or two that share a buffer's columns: 32 columns at a time from TMEM to
+//               registers, + bias, act, + residual, one rounding, into swizzled shared memory and out
+//               by TMA (which clips ragged edges). The residual arrives by TMA, ahead of its turn, in
+//               the slot the output leaves from. Four warps per scheduler, since GELU and SiLU are
+//               dependent chains that two could not hide.
 // The weight gradient's K is the voxels: K is cut into splits, each writes fp32 sums of its own,
 // and linear_reduce_kernel adds them in a fixed order.
 // Every wait is bounded (the conv kernels' limit); a timeout raises SPCONV_STATUS_WAIT_TIMEOUT and
@@ -32,17 +34,18 @@
 
 namespace spconv {
 
-constexpr int kLtThreads = 384;
+constexpr int kLtThreads = 576;
 constexpr int kLtBM = 128, kLtBK = 64;
 constexpr int kLtABytes = kLtBM * kLtBK * 2;            // 16 KB a stage
-constexpr int kLtEpiWarps = 8;
-constexpr int kLtSlot = 32 * 128;                       // 32 rows of 64 columns
+constexpr int kLtEpiWarps = 16, kLtEpiGroups = 4;
+constexpr int kLtSlot = 32 * 64;                        // 32 rows of 32 columns
+constexpr int kLtMaxBias = 4096;                        // bias columns kept in shared memory
 constexpr int kLtMaxStages = 12;
 constexpr int kLtMaxSlots = 4;
 constexpr int kLtMaxSmem = 227 * 1024;
-// behind the tiles: bias (256 fp32 for each epilogue warp: no barrier among them), barriers, TMEM address and abort flag
-constexpr int kLtBars = 2 * kLtMaxStages + 1 + 4 + kLtEpiWarps * kLtMaxSlots;
-constexpr int kLtTail = kLtEpiWarps * 256 * 4 + kLtBars * 8 + 16;
+// behind the tiles: barriers, TMEM address and abort flag, bias (fp32, at most kLtMaxBias)
+constexpr int kLtBars = 2 * kLtMaxStages + 1 + 2 * kLtEpiGroups + kLtEpiWarps * kLtMaxSlots;
+constexpr int kLtTail = (kLtBars * 8 + 8 + 15) & ~15;
 
 struct LtArgs {
     int M, N;
@@ -52,6 +55,8 @@ struct LtArgs {
     int64_t items;                          // tiles * splits
     int64_t k_per_split;                    // a multiple of 64 unless splits == 1
     int BN, stages, slots;                  // slots per epilogue warp (outputs; as many again for preact)
+    int bufs;                               // TMEM accumulators
+    int bias_smem;                          // bias columns in shared memory (N or 0)
     int b_resident;                         // K steps of B that stay in shared memory, or 0
     const void *bias;
     int has_residual, has_preact;
@@ -119,25 +124,26 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     const int warp_slots = NO * (a.has_preact ? 2 : 1);
     const uint32_t s_out = s_stage + S * stage_bytes;
     uint8_t *tail = base + a.b_resident * b_bytes + S * stage_bytes + (PARTIAL ? 0 : kLtEpiWarps * warp_slots * kLtSlot);
-    float *s_bias = reinterpret_cast<float *>(tail);                   // [kLtEpiWarps][256]
-    uint64_t *bar = reinterpret_cast<uint64_t *>(tail + kLtEpiWarps * 256 * 4);
+    uint64_t *bar = reinterpret_cast<uint64_t *>(tail);
     uint64_t *full = bar, *empty = full + kLtMaxStages, *bfull = empty + kLtMaxStages, *accfull = bfull + 1;
-    uint64_t *accempty = accfull + 2, *rbar = accempty + 2;
+    uint64_t *accempty = accfull + kLtEpiGroups, *rbar = accempty + kLtEpiGroups;
     uint32_t *s_tmem = reinterpret_cast<uint32_t *>(bar + kLtBars);
     volatile int *s_abort = reinterpret_cast<volatile int *>(s_tmem + 1);
+    float *s_bias = reinterpret_cast<float *>(tail + kLtTail);
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int64_t G = gridDim.x;
-    const uint32_t tmem_cols = (uint32_t)(2 * BN);                     // 128, 256 or 512
+    const uint32_t tmem_cols = (uint32_t)(a.bufs * BN);                // 256 or 512
+    for (int i = tid; i < a.bias_smem; i += kLtThreads) s_bias[i] = dtype_traits<T>::to_f(((const T *)a.bias)[i]);
     if (tid == 0) {
         for (int s = 0; s < S; ++s) {
             mbar_init(smem_u32(&full[s]), 1);
             mbar_init(smem_u32(&empty[s]), 1);
         }
         mbar_init(smem_u32(bfull), 1);
-        for (int g = 0; g < 2; ++g) {
+        for (int g = 0; g < a.bufs; ++g) {
             mbar_init(smem_u32(&accfull[g]), 1);
-            mbar_init(smem_u32(&accempty[g]), 4);
+            mbar_init(smem_u32(&accempty[g]), kLtEpiWarps / a.bufs);
         }
         for (int i = 0; i < kLtEpiWarps * NO; ++i) mbar_init(smem_u32(&rbar[i]), 1);
         *s_abort = 0;
@@ -217,8 +223,8 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                 int m0, n0;
                 int64_t k0, k1, split;
                 place(item, m0, n0, k0, k1, split);
-                const int g = (int)(it & 1);
-                const int64_t u = it >> 1;
+                const int g = (int)(it % a.bufs);
+                const int64_t u = it / a.bufs;
                 if (u > 0 && !wait(&accempty[g], (uint32_t)((u - 1) & 1))) { ok = false; break; }
                 tc_fence_after();
                 const int n_mma = (min(BN, a.N - n0) + 15) & ~15;
@@ -246,135 +252,143 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
             if (!ok && cnt > 0)              // MMAs in flight read shared memory: wait for the last commit
                 mbar_wait_bounded(smem_u32(&empty[(cnt - 1) % S]), (uint32_t)(((cnt - 1) / S) & 1));
         }
-    } else if (warp >= 4) {
+    } else {
         // ------------------------------------------------------------------ epilogue
-        const int g = (warp - 4) >> 2, quad = warp & 3, ew = warp - 4;
-        float *bias_s = s_bias + ew * 256;
-        const uint32_t t_acc = tmem + (uint32_t)(g * BN) + ((uint32_t)(quad * 32) << 16);
+        const int ew = warp - 2, quad = warp & 3;
+        const int buf = (ew >> 2) % a.bufs, sub = (ew >> 2) / a.bufs, share = kLtEpiGroups / a.bufs;
+        const int64_t stride = a.bufs * G;
+        const uint32_t t_acc = tmem + (uint32_t)(buf * BN) + ((uint32_t)(quad * 32) << 16);
         const uint32_t slot0 = s_out + (uint32_t)(ew * warp_slots * kLtSlot);
         const uint32_t pre0 = slot0 + (uint32_t)(NO * kLtSlot);
         uint64_t *my_rbar = rbar + ew * NO;
-        const uint32_t row_at = (uint32_t)(lane * 128);
+        const uint32_t row_at = (uint32_t)(lane * 64), row_x = (uint32_t)((lane >> 1) & 3);
         // one answer for the warp: its lanes must not part before the next warp-wide instruction
         auto all_wait = [&](uint64_t *b, uint32_t parity) { return __all_sync(0xffffffffu, wait(b, parity)) != 0; };
-        int n_bias = -1;
-        int64_t blk = 0, loads = 0;          // blocks begun; residual loads issued
-        // the residual's block into its slot; `behind`: later stores that may still be reading theirs
-        auto load_residual = [&](int m, int n, int behind) {
+        auto chunks_of = [&](int n0) { return (min(BN, a.N - n0) + 31) >> 5; };
+        int64_t blk = 0;                     // chunks begun
+        // Residual loads run `ahead` chunks before their use. The slot of load L was last the
+        // store of chunk L - NO, and when chunk b begins, b stores have been committed: those after
+        // L - NO = b + ahead - NO may still be reading.
+        const int ahead = NO >= 3 ? NO - 2 : NO - 1;
+        int64_t loads = 0, l_item = blockIdx.x + buf * G;
+        int l_chunk = sub;
+        auto load_residual = [&](int behind) {        // the next chunk's, if there is one
+            int m0 = 0, n0 = 0;
+            int64_t k0, k1, split;
+            for (; l_item < a.items; l_item += stride, l_chunk = sub) {
+                place(l_item, m0, n0, k0, k1, split);
+                if (l_chunk < chunks_of(n0)) break;
+            }
             if (lane == 0) {
                 lt_wait_read(behind);
-                const int s = (int)(loads % NO);
-                mbar_arrive_expect_tx(smem_u32(&my_rbar[s]), kLtSlot);
-                tma_load_2d(slot0 + s * kLtSlot, &map_res, n, m, smem_u32(&my_rbar[s]));
+                if (l_item < a.items) {
+                    const int s = (int)(loads % NO);
+                    mbar_arrive_expect_tx(smem_u32(&my_rbar[s]), kLtSlot);
+                    tma_load_2d(slot0 + s * kLtSlot, &map_res, n0 + l_chunk * 32, m0 + quad * 32, smem_u32(&my_rbar[s]));
+                }
             }
-            ++loads;
+            if (l_item < a.items) {
+                ++loads;
+                l_chunk += share;
+            }
         };
+        if (!PARTIAL && a.has_residual)
+            for (int i = 0; i < ahead; ++i) load_residual(0);
         int64_t use = 0;
-        for (int64_t item = blockIdx.x + g * G; item < a.items; item += 2 * G, ++use) {
+        for (int64_t item = blockIdx.x + buf * G; item < a.items; item += stride, ++use) {
             int m0, n0;
             int64_t k0, k1, split;
             place(item, m0, n0, k0, k1, split);
-            const int n_cols = min(BN, a.N - n0), blocks = (n_cols + 63) >> 6;
-            if (!PARTIAL && a.bias && n0 != n_bias) {
-                __syncwarp();
-                for (int i = lane; i < BN; i += 32)
-                    bias_s[i] = n0 + i < a.N ? dtype_traits<T>::to_f(((const T *)a.bias)[n0 + i]) : 0.f;
-                __syncwarp();
-                n_bias = n0;
-            }
-            // the group's next tile, for the residual of its first block
-            int m_next = -1, n_next = 0;
-            if (!PARTIAL && a.has_residual) {
-                if (item + 2 * G < a.items) place(item + 2 * G, m_next, n_next, k0, k1, split);
-                if (use == 0 && NO > 1) load_residual(m0 + quad * 32, n0, 0);
-            }
-            if (!all_wait(&accfull[g], (uint32_t)(use & 1))) break;
+            const int n_cols = min(BN, a.N - n0), chunks = chunks_of(n0);
+            if (!all_wait(&accfull[buf], (uint32_t)(use & 1))) break;
             tc_fence_after();
             bool ok = true;
-            for (int j = 0; j < blocks; ++j, ++blk) {
+            for (int j = sub; j < chunks; j += share, ++blk) {
                 const int s = (int)(blk % NO);
                 const uint32_t so = slot0 + s * kLtSlot + row_at, sp = pre0 + s * kLtSlot + row_at;
+                uint32_t r[32];
+                tmem_ld32(t_acc + (uint32_t)(j * 32), r);
                 if constexpr (!PARTIAL) {
                     if (a.has_residual) {
-                        if (NO == 1) load_residual(m0 + quad * 32, n0 + j * 64, 0);
-                        else if (j + 1 < blocks) load_residual(m0 + quad * 32, n0 + (j + 1) * 64, NO - 2);
-                        else if (m_next >= 0) load_residual(m_next + quad * 32, n_next, NO - 2);
-                        if (!all_wait(&my_rbar[s], (uint32_t)((blk / NO) & 1))) { ok = false; break; }
+                        load_residual(NO - 1 - ahead);
+                        if (!all_wait(&my_rbar[s], (uint32_t)((blk / NO) & 1))) ok = false;
                     } else {
                         if (lane == 0) lt_wait_read(NO - 1);
                     }
                     __syncwarp();
                 }
+                tc_wait_ld();
+                if (!ok) break;
+                if constexpr (PARTIAL) {
+                    const int row = m0 + quad * 32 + lane;
+                    float *dst = a.partial + (split * a.M + row) * (int64_t)a.N + n0 + j * 32;
+                    if (row < a.M) {
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    uint32_t r[32];
-                    tmem_ld32(t_acc + (uint32_t)(j * 64 + c * 32), r);
-                    tc_wait_ld();
-                    if constexpr (PARTIAL) {
-                        const int row = m0 + quad * 32 + lane;
-                        float *dst = a.partial + (split * a.M + row) * (int64_t)a.N + n0 + j * 64 + c * 32;
-                        if (row < a.M) {
+                        for (int v = 0; v < 8; ++v)
+                            if (j * 32 + v * 4 < n_cols)
+                                __stcg(reinterpret_cast<float4 *>(dst) + v,
+                                       make_float4(__uint_as_float(r[4 * v]), __uint_as_float(r[4 * v + 1]),
+                                                   __uint_as_float(r[4 * v + 2]), __uint_as_float(r[4 * v + 3])));
+                    }
+                } else {
 #pragma unroll
-                            for (int v = 0; v < 8; ++v)
-                                if (j * 64 + c * 32 + v * 4 < n_cols)
-                                    __stcg(reinterpret_cast<float4 *>(dst) + v,
-                                           make_float4(__uint_as_float(r[4 * v]), __uint_as_float(r[4 * v + 1]),
-                                                       __uint_as_float(r[4 * v + 2]), __uint_as_float(r[4 * v + 3])));
-                        }
-                    } else {
+                    for (int v = 0; v < 4; ++v) {
+                        const uint32_t at = ((uint32_t)v ^ row_x) << 4;
+                        f32x2 f[4];
 #pragma unroll
-                        for (int v = 0; v < 4; ++v) {
-                            const uint32_t at = (uint32_t)(((c * 4 + v) ^ (lane & 7)) << 4);
-                            f32x2 f[4];
-#pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                f[i] = pack_f32x2(__uint_as_float(r[8 * v + 2 * i]), __uint_as_float(r[8 * v + 2 * i + 1]));
-                            if (a.bias) {
-                                const ulonglong2 *b = reinterpret_cast<const ulonglong2 *>(bias_s + j * 64 + c * 32 + v * 8);
+                        for (int i = 0; i < 4; ++i)
+                            f[i] = pack_f32x2(__uint_as_float(r[8 * v + 2 * i]), __uint_as_float(r[8 * v + 2 * i + 1]));
+                        if (a.bias_smem) {
+                            const int n = n0 + j * 32 + v * 8;
+                            if (n < a.N) {
+                                const ulonglong2 *b = reinterpret_cast<const ulonglong2 *>(s_bias + n);
                                 const ulonglong2 b0 = b[0], b1 = b[1];
                                 f[0] = add2(f[0], {b0.x});
                                 f[1] = add2(f[1], {b0.y});
                                 f[2] = add2(f[2], {b1.x});
                                 f[3] = add2(f[3], {b1.y});
                             }
-                            if (a.has_preact) lt_store8<T>(sp + at, f);
+                        } else if (a.bias) {
+                            const T *b = (const T *)a.bias + n0 + j * 32 + v * 8;
+                            if (n0 + j * 32 + v * 8 < a.N) {
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) f[i] = act_value2<ACT>(f[i]);
-                            if (a.has_residual) {
-                                uint32_t q[4];
-                                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];\n"
-                                             : "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3]) : "r"(so + at) : "memory");
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) {
-                                    const float2 x = lt_unpack<T>(q[i]);
-                                    f[i] = add2(f[i], pack_f32x2(x.x, x.y));
-                                }
+                                for (int i = 0; i < 4; ++i)
+                                    f[i] = add2(f[i], pack_f32x2(dtype_traits<T>::to_f(b[2 * i]), dtype_traits<T>::to_f(b[2 * i + 1])));
                             }
-                            lt_store8<T>(so + at, f);
                         }
+                        if (a.has_preact) lt_store8<T>(sp + at, f);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) f[i] = act_value2<ACT>(f[i]);
+                        if (a.has_residual) {
+                            uint32_t q[4];
+                            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];\n"
+                                         : "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3]) : "r"(so + at) : "memory");
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const float2 x = lt_unpack<T>(q[i]);
+                                f[i] = add2(f[i], pack_f32x2(x.x, x.y));
+                            }
+                        }
+                        lt_store8<T>(so + at, f);
                     }
-                }
-                if (j + 1 == blocks) {       // the accumulator is in registers: free for the MMA
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(smem_u32(&accempty[g]));
-                }
-                if constexpr (!PARTIAL) {
                     fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) {
                         if (m0 + quad * 32 < a.M) {
-                            tma_store_2d(&map_out, n0 + j * 64, m0 + quad * 32, slot0 + s * kLtSlot);
-                            if (a.has_preact) tma_store_2d(&map_pre, n0 + j * 64, m0 + quad * 32, pre0 + s * kLtSlot);
+                            tma_store_2d(&map_out, n0 + j * 32, m0 + quad * 32, slot0 + s * kLtSlot);
+                            if (a.has_preact) tma_store_2d(&map_pre, n0 + j * 32, m0 + quad * 32, pre0 + s * kLtSlot);
                         }
-                        bulk_commit();       // one group a block, empty or not
+                        bulk_commit();       // one group a chunk, empty or not
                     }
                 }
             }
             if (!ok) break;
+            tc_fence_before();               // the accumulator has been read: free for the MMA
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&accempty[buf]));
         }
         if (!PARTIAL && lane == 0) {
-            for (int64_t j = max(blk, loads - NO); j < loads; ++j)      // residual loads nobody waited for
+            for (int64_t j = blk; j < loads; ++j)             // residual loads nobody waited for
                 mbar_wait_bounded(smem_u32(&my_rbar[j % NO]), (uint32_t)((j / NO) & 1), kTmaDrainNs);
             bulk_wait<0>();
         }
@@ -449,7 +463,9 @@ static int lt_launch(const GemmArgs &g) {
     a.tiles = (g.M + kLtBM - 1) / kLtBM * a.nb;
     a.items = a.tiles * g.splits;
     a.k_per_split = g.splits > 1 ? g.k_per_split : g.K;
+    a.bufs = a.BN == 256 ? 2 : 4;
     a.bias = g.bias;
+    a.bias_smem = g.bias && g.N <= kLtMaxBias ? (int)g.N : 0;
     a.has_residual = g.residual != nullptr;
     a.has_preact = g.preact != nullptr;
     a.partial = g.partial;
@@ -458,7 +474,7 @@ static int lt_launch(const GemmArgs &g) {
     const int sms = lt_sms();
     int64_t grid = std::min<int64_t>(sms, a.items);
     const int64_t nk = (g.K + kLtBK - 1) / kLtBK;
-    const int b_bytes = a.BN * 128, room = kLtMaxSmem - 1024 - kLtTail;
+    const int b_bytes = a.BN * 128, room = kLtMaxSmem - 1024 - kLtTail - a.bias_smem * 4;
     auto fit = [&](int resident) {          // output slots and stages beside `resident` K steps of B
         const int stage = kLtABytes + (resident ? 0 : b_bytes);
         for (int slots = A_T ? 1 : 4; slots >= 1; slots >>= 1) {
@@ -480,16 +496,16 @@ static int lt_launch(const GemmArgs &g) {
         set_error("linear: no shared-memory layout for this shape");
         return SPCONV_ERR_UNSUPPORTED;
     }
-    const int smem = 1024 + kLtTail + a.b_resident * b_bytes + a.stages * (kLtABytes + (a.b_resident ? 0 : b_bytes)) +
+    const int smem = 1024 + kLtTail + a.bias_smem * 4 + a.b_resident * b_bytes + a.stages * (kLtABytes + (a.b_resident ? 0 : b_bytes)) +
                      (A_T ? 0 : kLtEpiWarps * a.slots * (a.has_preact ? 2 : 1) * kLtSlot);
     CUtensorMap ma, mb, mo, mr, mp;
     // K-contiguous operands: boxes of 64 K x rows; the others: 64 columns x 64 K rows
     const bool maps =
         (A_T ? make_tmap_2d(&ma, g.a, g.M, g.K, g.M * 2, 64, 64) : make_tmap_2d(&ma, g.a, g.K, g.M, g.K * 2, 64, kLtBM)) &&
         (B_T ? make_tmap_2d(&mb, g.b, g.N, g.K, g.N * 2, 64, 64) : make_tmap_2d(&mb, g.b, g.K, g.N, g.K * 2, 64, a.BN)) &&
-        (A_T || make_tmap_2d(&mo, g.out, g.N, g.M, g.N * 2, 64, 32)) &&
-        (!g.residual || make_tmap_2d(&mr, g.residual, g.N, g.M, g.N * 2, 64, 32)) &&
-        (!g.preact || make_tmap_2d(&mp, g.preact, g.N, g.M, g.N * 2, 64, 32));
+        (A_T || make_tmap_2d(&mo, g.out, g.N, g.M, g.N * 2, 32, 32)) &&
+        (!g.residual || make_tmap_2d(&mr, g.residual, g.N, g.M, g.N * 2, 32, 32)) &&
+        (!g.preact || make_tmap_2d(&mp, g.preact, g.N, g.M, g.N * 2, 32, 32));
     if (!maps) return SPCONV_ERR_CUDA;
     if (A_T) mo = ma;                       // maps that the kernel does not read
     if (!g.residual) mr = ma;
