@@ -8,7 +8,10 @@ goes to ``torch.cuda.current_stream()``.
 Device-side problems (coordinates out of range, a full table, a kernel wait limit) are
 OR-ed into a per-device int32 status word. After each op the word is copied
 asynchronously to pinned host memory; the next op on that device (or an explicit
-``check_errors()``) raises ``RuntimeError`` if a bit is set. With the environment variable
+``check_errors()``) raises ``RuntimeError`` if a bit is set. The linear, norm and clipping ops, which
+are also called on a few rows, where a copy and an event would cost more than the op, give their
+kernels a word in pinned host memory instead: a kernel writes there only on a problem, and the
+next op on the device reads it without any call to CUDA. With the environment variable
 ``SPARSECONV_SYNC_CHECK=1`` each op synchronises and checks at once.
 """
 from __future__ import annotations
@@ -166,6 +169,14 @@ def _stream_ptr(device: torch.device) -> int:
 
 
 def _require_cuda(*tensors: torch.Tensor) -> torch.device:
+    first = tensors[0]
+    if first.is_cuda:
+        index = first.get_device()
+        for t in tensors:
+            if t is not None and t.get_device() != index:      # -1 on the CPU
+                break
+        else:
+            return first.device
     dev = None
     for t in tensors:
         if t is None:
@@ -191,6 +202,10 @@ class _DeviceStatus:
         self.host = torch.zeros(1, dtype=torch.int32, pin_memory=True)
         self.event = torch.cuda.Event()
         self.pending = False
+        # written by kernels that have a problem, read here directly (mapped pinned memory)
+        self.mapped = torch.zeros(1, dtype=torch.int32, pin_memory=True)
+        self.mapped_ptr = self.mapped.data_ptr()
+        self.mapped_word = ctypes.c_int32.from_address(self.mapped_ptr)
 
 
 _status = {}
@@ -258,6 +273,30 @@ def before_launch(device: torch.device) -> None:
         _inspect(st)
 
 
+def _inspect_mapped(st: _DeviceStatus) -> None:
+    bits = st.mapped_word.value
+    if bits:
+        st.mapped_word.value = 0
+        if bits & _FATAL_BITS:
+            raise RuntimeError(f"sparseconv device error: {describe_status(bits)} (status bits {bits:#x})")
+
+
+def mapped_status(index: int) -> int:
+    """Address of the device's host status word, for an op about to launch; raises for an error
+    that an earlier op reported there."""
+    st = _status.get(index) or status_word(torch.device("cuda", index))
+    if st.mapped_word.value:
+        _inspect_mapped(st)
+    return st.mapped_ptr
+
+
+def after_mapped_launch(index: int) -> None:
+    """Check at once if SPARSECONV_SYNC_CHECK=1 (not while the stream is being captured)."""
+    if os.environ.get("SPARSECONV_SYNC_CHECK", "0") == "1" and not torch.cuda.is_current_stream_capturing():
+        torch.cuda.current_stream(index).synchronize()
+        _inspect_mapped(_status[index])
+
+
 def check_errors(device: Optional[torch.device] = None) -> int:
     """Synchronise with the device's status read-back and raise on an error.
 
@@ -270,8 +309,9 @@ def check_errors(device: Optional[torch.device] = None) -> int:
             st.event.synchronize()
         torch.cuda.synchronize(st.device)
         st.host.copy_(st.word)
-        bits |= int(st.host.item())
+        bits |= int(st.host.item()) | st.mapped_word.value
         _inspect(st)
+        _inspect_mapped(st)
     return bits
 
 
@@ -279,6 +319,7 @@ def reset_status(device: Optional[torch.device] = None) -> None:
     for st in ([status_word(device)] if device is not None else list(_status.values())):
         st.word.zero_()
         st.pending = False
+        st.mapped_word.value = 0
 
 
 # ---------------------------------------------------------------------------------------
@@ -648,12 +689,18 @@ def _on_device(fn):
     """Runs a call with the device of its tensors current (launches go to that device's stream)."""
     @functools.wraps(fn)
     def call(first, *args, **kwargs):
-        t = first if isinstance(first, torch.Tensor) else (first[0] if first else None)
-        if t is None or not t.is_cuda or t.device.index == torch.cuda.current_device():
+        t = first if isinstance(first, torch.Tensor) else first[0]
+        index = t.get_device()
+        if index < 0 or index == torch._C._cuda_getDevice():
             return fn(first, *args, **kwargs)
-        with torch.cuda.device(t.device):
+        with torch.cuda.device(index):
             return fn(first, *args, **kwargs)
     return call
+
+
+def _raw_stream(index: int) -> int:
+    """The device's current stream, without building a torch.cuda.Stream."""
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
@@ -697,15 +744,13 @@ def linear_forward(feats: torch.Tensor, weight: torch.Tensor, bias: Optional[tor
     preact = torch.empty_like(out) if keep_preact else None
     if M == 0:
         return out, preact
-    before_launch(dev)
-    rc = load_library().spconv_linear_forward(
+    index = dev.index
+    rc = (_lib or load_library()).spconv_linear_forward(
         feats.data_ptr(), DTYPE_CODES[dtype], M, Ci, weight.data_ptr(), _ptr(bias), _ptr(residual), Co,
-        ACTIVATIONS[activation], out.data_ptr(), _ptr(preact), kernel, status_word(dev).word.data_ptr(),
-        _stream_ptr(dev))
+        ACTIVATIONS[activation], out.data_ptr(), _ptr(preact), kernel, mapped_status(index), _raw_stream(index))
     if rc != SPCONV_OK:
         _raise(rc, "spconv_linear_forward")
-    if dtype != torch.float32:
-        after_launch(dev)
+    after_mapped_launch(index)
     return out, preact
 
 
@@ -731,16 +776,15 @@ def linear_backward(grad_out: torch.Tensor, preact: Optional[torch.Tensor], feat
     gb = grad((Co,), bias_dtype) if needs[2] else None
     need = lib.spconv_linear_backward_workspace_bytes(code, M, Ci, Co, ACTIVATIONS[activation])
     ws = torch.empty((max(need, 256),), dtype=torch.uint8, device=dev)
-    before_launch(dev)
+    index = dev.index
     rc = lib.spconv_linear_backward(
         grad_out.data_ptr(), _ptr(preact), feats.data_ptr(), weight.data_ptr(), code, M, Ci, Co,
         ACTIVATIONS[activation], _ptr(gx), _ptr(gw), 0 if gw is None else DTYPE_CODES[gw.dtype], _ptr(gb),
         0 if gb is None else DTYPE_CODES[gb.dtype], ws.data_ptr(), need, kernel,
-        status_word(dev).word.data_ptr(), _stream_ptr(dev))
+        mapped_status(index), _raw_stream(index))
     if rc != SPCONV_OK:
         _raise(rc, "spconv_linear_backward")
-    if dtype != torch.float32:
-        after_launch(dev)
+    after_mapped_launch(index)
     return [gx, None if gw is None else gw.to(weight_dtype), None if gb is None else gb.to(bias_dtype)]
 
 
@@ -791,8 +835,7 @@ def _norm_args(feats: torch.Tensor, residual, params, offsets, residual_scale: f
             raise ValueError("batch_offsets must be a contiguous [samples + 1] int32 tensor")
         if per_sample:
             a.offsets, a.num_samples = offsets.data_ptr(), offsets.numel() - 1
-            before_launch(dev)
-            a.status = status_word(dev).word.data_ptr()
+            a.status = mapped_status(dev.index)
     return a
 
 
@@ -805,11 +848,12 @@ def residual_norm_forward(feats: torch.Tensor, residual: Optional[torch.Tensor],
     hidden = torch.empty_like(feats)
     normed = torch.empty_like(feats) if next_norm != "none" else None
     a.hidden, a.normed = hidden.data_ptr(), _ptr(normed)
-    rc = load_library().spconv_residual_norm_forward(a, _stream_ptr(feats.device))
+    index = feats.get_device()
+    rc = (_lib or load_library()).spconv_residual_norm_forward(a, _raw_stream(index))
     if rc != SPCONV_OK:
         _raise(rc, "spconv_residual_norm_forward")
     if a.status:
-        after_launch(feats.device)
+        after_mapped_launch(index)
     return hidden, normed
 
 
@@ -836,11 +880,12 @@ def residual_norm_backward(feats: torch.Tensor, residual: Optional[torch.Tensor]
         a.workspace_bytes = lib.spconv_residual_norm_workspace_bytes(a.num_rows, a.channels, a.num_samples)
         ws = torch.empty((max(a.workspace_bytes, 16),), dtype=torch.uint8, device=feats.device)
         a.workspace = ws.data_ptr()
-    rc = lib.spconv_residual_norm_backward(a, _stream_ptr(feats.device))
+    index = feats.get_device()
+    rc = lib.spconv_residual_norm_backward(a, _raw_stream(index))
     if rc != SPCONV_OK:
         _raise(rc, "spconv_residual_norm_backward")
     if a.status:
-        after_launch(feats.device)
+        after_mapped_launch(index)
     return grads
 
 
@@ -857,27 +902,32 @@ def clip_gradients(grads: Sequence[torch.Tensor], outs: Sequence[torch.Tensor], 
                    norm_kind: int) -> torch.Tensor:
     """outs[k] = grads[k] * min(1, max_norm / (norm + 1e-6)); returns the norm (0-dim float32)."""
     lib = load_library()
-    dev = grads[0].device
+    dev, index = grads[0].device, grads[0].get_device()
+    ptrs, optrs, sizes, codes = [], [], [], []
     for g, o in zip(grads, outs):
-        if not g.is_cuda or g.device != dev or o.device != dev:
+        if g.get_device() != index or (o is not g and o.get_device() != index) or index < 0:
             _require_cuda(*grads, *outs)
-        if g.dtype not in DTYPE_CODES:
+        code = DTYPE_CODES.get(g.dtype)
+        if code is None:
             raise TypeError(f"unsupported gradient dtype {g.dtype}")
-        if o is not g and (o.dtype != g.dtype or o.shape != g.shape or o.stride() != g.stride()):
+        dense = g.is_contiguous()
+        if o is not g and (o.dtype != g.dtype or o.shape != g.shape or
+                           not (dense and o.is_contiguous() or o.stride() == g.stride())):
             raise ValueError("each output must have its gradient's shape, strides and dtype")
-        if not g.is_contiguous() and not _is_dense(g):
+        if not dense and not _is_dense(g):
             raise ValueError("gradients must be dense in memory")
-    n = len(grads)
-    ptrs = array.array("Q", [g.data_ptr() for g in grads])
-    optrs = ptrs if outs is grads else array.array("Q", [o.data_ptr() for o in outs])
-    sizes = array.array("q", [g.numel() for g in grads])
-    codes = array.array("i", [DTYPE_CODES[g.dtype] for g in grads])
+        ptrs.append(g.data_ptr())
+        optrs.append(o.data_ptr())
+        sizes.append(g.numel())
+        codes.append(code)
+    n = len(ptrs)
+    ptrs, optrs, sizes, codes = (array.array(t, v) for t, v in (("Q", ptrs), ("Q", optrs), ("q", sizes), ("i", codes)))
     total = torch.empty((), dtype=torch.float32, device=dev)
     need = lib.spconv_clip_gradients_workspace_bytes(n)
     ws = torch.empty((need,), dtype=torch.uint8, device=dev)
     rc = lib.spconv_clip_gradients(ptrs.buffer_info()[0], optrs.buffer_info()[0], sizes.buffer_info()[0],
                                    codes.buffer_info()[0], n, norm_kind, max_norm, total.data_ptr(),
-                                   ws.data_ptr(), need, _stream_ptr(dev))
+                                   ws.data_ptr(), need, _raw_stream(index))
     if rc != SPCONV_OK:
         _raise(rc, "spconv_clip_gradients")
     return total
