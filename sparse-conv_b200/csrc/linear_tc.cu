@@ -48,12 +48,11 @@ constexpr int kLtBars = 2 * kLtMaxStages + 1 + 2 * kLtEpiGroups + kLtEpiWarps * 
 constexpr int kLtTail = (kLtBars * 8 + 8 + 15) & ~15;
 
 struct LtArgs {
-    int M, N;
-    int64_t K;
+    int M, N, K;
     int nb;                                 // column blocks
-    int64_t tiles;                          // row tiles * nb
-    int64_t items;                          // tiles * splits
-    int64_t k_per_split;                    // a multiple of 64 unless splits == 1
+    int tiles;                              // row tiles * nb
+    int items;                              // tiles * splits
+    int k_per_split;                        // a multiple of 64 unless splits == 1
     int BN, stages, slots;                  // slots per epilogue warp (outputs; as many again for preact)
     int bufs;                               // TMEM accumulators
     int bias_smem;                          // bias columns in shared memory (N or 0)
@@ -132,7 +131,7 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     float *s_bias = reinterpret_cast<float *>(tail + kLtTail);
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int64_t G = gridDim.x;
+    const int G = gridDim.x;
     const uint32_t tmem_cols = (uint32_t)(a.bufs * BN);                // 256 or 512
     for (int i = tid; i < a.bias_smem; i += kLtThreads) s_bias[i] = dtype_traits<T>::to_f(((const T *)a.bias)[i]);
     if (tid == 0) {
@@ -160,14 +159,44 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     auto wait = [&](uint64_t *b, uint32_t parity) -> bool {
         return mbar_wait_or_abort(smem_u32(b), parity, s_abort, a.wait_ns);
     };
-    // item -> (m0, n0) and its range of K
-    auto place = [&](int64_t item, int &m0, int &n0, int64_t &k0, int64_t &k1, int64_t &split) {
-        split = PARTIAL ? item / a.tiles : 0;
-        const int64_t tile = item - split * a.tiles;
-        m0 = (int)(tile / a.nb) * kLtBM;
-        n0 = (int)(tile % a.nb) * BN;
-        k0 = split * a.k_per_split;
-        k1 = PARTIAL ? min(a.K, k0 + a.k_per_split) : a.K;
+    // A walk over every `step`-th item: its tile and its range of K. Divisions only at the start (the
+    // single loading and MMA threads would spend longer on them than on a tile's copies).
+    struct Walk {
+        int item, m, n, split, step, dm, dn;
+    };
+    auto begin = [&](int first, int step) {
+        Walk w;
+        w.item = first;
+        w.step = step;
+        w.split = PARTIAL ? first / a.tiles : 0;
+        const int tile = first - w.split * a.tiles;
+        w.m = tile / a.nb;
+        w.n = tile - w.m * a.nb;
+        w.dm = step / a.nb;
+        w.dn = step - w.dm * a.nb;
+        return w;
+    };
+    auto advance = [&](Walk &w) {
+        w.item += w.step;
+        if constexpr (PARTIAL) {
+            w = begin(w.item, w.step);
+        } else {
+            w.m += w.dm;
+            w.n += w.dn;
+            if (w.n >= a.nb) {
+                w.n -= a.nb;
+                ++w.m;
+            }
+        }
+    };
+    auto k_begin = [&](const Walk &w) { return PARTIAL ? w.split * a.k_per_split : 0; };
+    auto k_end = [&](int k0) { return PARTIAL && a.K - k0 > a.k_per_split ? k0 + a.k_per_split : a.K; };
+    // ring position: index and the parity of its current use
+    auto next = [](int &i, uint32_t &phase, int n) {
+        if (++i == n) {
+            i = 0;
+            phase ^= 1u;
+        }
     };
 
     if (warp == 0) {
@@ -180,64 +209,62 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                     tma_load_2d(dst, &map_b, k, n0, mbar);
                 }
             };
-            int64_t cnt = 0;
+            int st = 0;
+            uint32_t phase = 0;
+            int issued = 0;                  // stages in use, at most S
             bool ok = true;
-            if (a.b_resident && (int64_t)blockIdx.x < a.items) {      // the grid is a multiple of nb: n0 never changes
-                int m0, n0;
-                int64_t k0, k1, split;
-                place(blockIdx.x, m0, n0, k0, k1, split);
+            Walk w = begin(blockIdx.x, G);
+            if (a.b_resident && w.item < a.items) {           // the grid is a multiple of nb: n never changes
                 mbar_arrive_expect_tx(smem_u32(bfull), (uint32_t)(a.b_resident * b_bytes));
-                for (int c = 0; c < a.b_resident; ++c) load_b(s_b + c * b_bytes, c * kLtBK, n0, smem_u32(bfull));
+                for (int c = 0; c < a.b_resident; ++c) load_b(s_b + c * b_bytes, c * kLtBK, w.n * BN, smem_u32(bfull));
             }
-            for (int64_t item = blockIdx.x; item < a.items && ok; item += G) {
-                int m0, n0;
-                int64_t k0, k1, split;
-                place(item, m0, n0, k0, k1, split);
-                for (int64_t k = k0; k < k1; k += kLtBK, ++cnt) {
-                    const int s = (int)(cnt % S);
-                    const int64_t u = cnt / S;
-                    if (u > 0 && !wait(&empty[s], (uint32_t)((u - 1) & 1))) { ok = false; break; }
-                    const uint32_t mbar = smem_u32(&full[s]), dst = s_stage + s * stage_bytes;
+            for (; w.item < a.items && ok; advance(w)) {
+                const int m0 = w.m * kLtBM, n0 = w.n * BN, k0 = k_begin(w), k1 = k_end(k0);
+                for (int k = k0; k < k1; k += kLtBK) {
+                    if (issued == S && !wait(&empty[st], phase ^ 1u)) { ok = false; break; }
+                    const uint32_t mbar = smem_u32(&full[st]), dst = s_stage + st * stage_bytes;
                     mbar_arrive_expect_tx(mbar, (uint32_t)stage_bytes);
                     if constexpr (A_T) {
-                        tma_load_2d(dst, &map_a, m0, (int)k, mbar);
-                        tma_load_2d(dst + 8192, &map_a, m0 + 64, (int)k, mbar);
+                        tma_load_2d(dst, &map_a, m0, k, mbar);
+                        tma_load_2d(dst + 8192, &map_a, m0 + 64, k, mbar);
                     } else {
-                        tma_load_2d(dst, &map_a, (int)k, m0, mbar);
+                        tma_load_2d(dst, &map_a, k, m0, mbar);
                     }
-                    if (!a.b_resident) load_b(dst + kLtABytes, (int)k, n0, mbar);
+                    if (!a.b_resident) load_b(dst + kLtABytes, k, n0, mbar);
+                    if (issued < S) ++issued;
+                    next(st, phase, S);
                 }
             }
-            // every load has landed before the CTA may exit (at once unless the MMA gave up)
-            for (int64_t j = max((int64_t)0, cnt - S); j < cnt; ++j)
-                mbar_wait_bounded(smem_u32(&full[j % S]), (uint32_t)((j / S) & 1), kTmaDrainNs);
-            if (a.b_resident && (int64_t)blockIdx.x < a.items) mbar_wait_bounded(smem_u32(bfull), 0, kTmaDrainNs);
+            // every load has landed before the CTA may exit (at once unless the MMA gave up): the
+            // stages from st on were last used a phase earlier than those before it
+            for (int i = 0; i < issued; ++i)
+                mbar_wait_bounded(smem_u32(&full[i]), i < st ? phase : phase ^ 1u, kTmaDrainNs);
+            if (a.b_resident && (int)blockIdx.x < a.items) mbar_wait_bounded(smem_u32(bfull), 0, kTmaDrainNs);
         }
     } else if (warp == 1) {
         // ------------------------------------------------------------------ MMA
         if (lane == 0) {
-            int64_t cnt = 0, it = 0;
+            int st = 0, buf = 0, last = -1;
+            uint32_t phase = 0, acc_phase = 1;                // the first use of a buffer passes at once
             bool ok = true;
-            if (a.b_resident && (int64_t)blockIdx.x < a.items) ok = wait(bfull, 0);
-            for (int64_t item = blockIdx.x; item < a.items && ok; item += G, ++it) {
-                int m0, n0;
-                int64_t k0, k1, split;
-                place(item, m0, n0, k0, k1, split);
-                const int g = (int)(it % a.bufs);
-                const int64_t u = it / a.bufs;
-                if (u > 0 && !wait(&accempty[g], (uint32_t)((u - 1) & 1))) { ok = false; break; }
+            Walk w = begin(blockIdx.x, G);
+            if (a.b_resident && w.item < a.items) ok = wait(bfull, 0);
+            for (; w.item < a.items && ok; advance(w)) {
+                const int n0 = w.n * BN, k0 = k_begin(w), k1 = k_end(k0);
+                if (!wait(&accempty[buf], acc_phase)) { ok = false; break; }
                 tc_fence_after();
                 const int n_mma = (min(BN, a.N - n0) + 15) & ~15;
                 const uint32_t idesc = instr_desc_f16(dtype_traits<T>::mma_format, kLtBM, n_mma) |
                                        (A_T ? 1u << 15 : 0u) | (B_T ? 1u << 16 : 0u);
-                const uint32_t d = tmem + (uint32_t)(g * BN);
-                for (int64_t k = k0; k < k1; k += kLtBK, ++cnt) {
-                    const int s = (int)(cnt % S);
-                    if (!wait(&full[s], (uint32_t)((cnt / S) & 1))) { ok = false; break; }
+                const uint32_t d = tmem + (uint32_t)(buf * BN);
+                uint32_t s_res = s_b;
+                for (int k = k0; k < k1; k += kLtBK) {
+                    if (!wait(&full[st], phase)) { ok = false; break; }
                     tc_fence_after();
-                    const uint32_t sa = s_stage + s * stage_bytes;
-                    const uint32_t sb = a.b_resident ? s_b + (uint32_t)(k / kLtBK) * b_bytes : sa + kLtABytes;
-                    const int steps = (int)min((int64_t)4, (k1 - k + 15) / 16);   // zeros past K's end are skipped
+                    const uint32_t sa = s_stage + st * stage_bytes;
+                    const uint32_t sb = a.b_resident ? s_res : sa + kLtABytes;
+                    s_res += b_bytes;
+                    const int steps = min(4, (k1 - k + 15) >> 4);     // zeros past K's end are skipped
                     for (int kk = 0; kk < steps; ++kk) {
                         const uint64_t ad = A_T ? smem_desc_mn_sw128(sa + kk * 2048, 8192, 1024)
                                                 : smem_desc_kmajor_swizzled(sa + kk * 32, 128);
@@ -245,18 +272,23 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                                                 : smem_desc_kmajor_swizzled(sb + kk * 32, 128);
                         tc_mma_f16(d, ad, bd, idesc, (k > k0 || kk > 0) ? 1u : 0u);
                     }
-                    tc_commit(smem_u32(&empty[s]));
+                    tc_commit(smem_u32(&empty[st]));
+                    last = st;
+                    next(st, phase, S);
                 }
-                if (ok) tc_commit(smem_u32(&accfull[g]));
+                if (ok) {
+                    tc_commit(smem_u32(&accfull[buf]));
+                    next(buf, acc_phase, a.bufs);
+                }
             }
-            if (!ok && cnt > 0)              // MMAs in flight read shared memory: wait for the last commit
-                mbar_wait_bounded(smem_u32(&empty[(cnt - 1) % S]), (uint32_t)(((cnt - 1) / S) & 1));
+            // MMAs in flight read shared memory: wait for the last commit (its stage's use ended `phase`
+            // if the ring has not wrapped since, else the phase before)
+            if (!ok && last >= 0) mbar_wait_bounded(smem_u32(&empty[last]), last < st ? phase : phase ^ 1u);
         }
     } else {
         // ------------------------------------------------------------------ epilogue
         const int ew = warp - 2, quad = warp & 3;
         const int buf = (ew >> 2) % a.bufs, sub = (ew >> 2) / a.bufs, share = kLtEpiGroups / a.bufs;
-        const int64_t stride = a.bufs * G;
         const uint32_t t_acc = tmem + (uint32_t)(buf * BN) + ((uint32_t)(quad * 32) << 16);
         const uint32_t slot0 = s_out + (uint32_t)(ew * warp_slots * kLtSlot);
         const uint32_t pre0 = slot0 + (uint32_t)(NO * kLtSlot);
@@ -265,53 +297,52 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         // one answer for the warp: its lanes must not part before the next warp-wide instruction
         auto all_wait = [&](uint64_t *b, uint32_t parity) { return __all_sync(0xffffffffu, wait(b, parity)) != 0; };
         auto chunks_of = [&](int n0) { return (min(BN, a.N - n0) + 31) >> 5; };
-        int64_t blk = 0;                     // chunks begun
         // Residual loads run `ahead` chunks before their use. The slot of load L was last the
         // store of chunk L - NO, and when chunk b begins, b stores have been committed: those after
         // L - NO = b + ahead - NO may still be reading.
         const int ahead = NO >= 3 ? NO - 2 : NO - 1;
-        int64_t loads = 0, l_item = blockIdx.x + buf * G;
-        int l_chunk = sub;
+        int l_slot = 0, outstanding = 0, l_chunk = sub;
+        uint32_t l_phase = 0;
+        Walk lw = begin(blockIdx.x + buf * G, a.bufs * G);
         auto load_residual = [&](int behind) {        // the next chunk's, if there is one
-            int m0 = 0, n0 = 0;
-            int64_t k0, k1, split;
-            for (; l_item < a.items; l_item += stride, l_chunk = sub) {
-                place(l_item, m0, n0, k0, k1, split);
-                if (l_chunk < chunks_of(n0)) break;
+            while (lw.item < a.items && l_chunk >= chunks_of(lw.n * BN)) {
+                advance(lw);
+                l_chunk = sub;
             }
+            const bool more = lw.item < a.items;
             if (lane == 0) {
                 lt_wait_read(behind);
-                if (l_item < a.items) {
-                    const int s = (int)(loads % NO);
-                    mbar_arrive_expect_tx(smem_u32(&my_rbar[s]), kLtSlot);
-                    tma_load_2d(slot0 + s * kLtSlot, &map_res, n0 + l_chunk * 32, m0 + quad * 32, smem_u32(&my_rbar[s]));
+                if (more) {
+                    mbar_arrive_expect_tx(smem_u32(&my_rbar[l_slot]), kLtSlot);
+                    tma_load_2d(slot0 + l_slot * kLtSlot, &map_res, lw.n * BN + l_chunk * 32, lw.m * kLtBM + quad * 32,
+                                smem_u32(&my_rbar[l_slot]));
                 }
             }
-            if (l_item < a.items) {
-                ++loads;
+            if (more) {
+                ++outstanding;
                 l_chunk += share;
+                next(l_slot, l_phase, NO);
             }
         };
         if (!PARTIAL && a.has_residual)
             for (int i = 0; i < ahead; ++i) load_residual(0);
-        int64_t use = 0;
-        for (int64_t item = blockIdx.x + buf * G; item < a.items; item += stride, ++use) {
-            int m0, n0;
-            int64_t k0, k1, split;
-            place(item, m0, n0, k0, k1, split);
+        int s = 0;
+        uint32_t s_phase = 0, use_phase = 0;
+        for (Walk w = begin(blockIdx.x + buf * G, a.bufs * G); w.item < a.items; advance(w), use_phase ^= 1u) {
+            const int m0 = w.m * kLtBM, n0 = w.n * BN;
             const int n_cols = min(BN, a.N - n0), chunks = chunks_of(n0);
-            if (!all_wait(&accfull[buf], (uint32_t)(use & 1))) break;
+            if (!all_wait(&accfull[buf], use_phase)) break;
             tc_fence_after();
             bool ok = true;
-            for (int j = sub; j < chunks; j += share, ++blk) {
-                const int s = (int)(blk % NO);
+            for (int j = sub; j < chunks; j += share, next(s, s_phase, NO)) {
                 const uint32_t so = slot0 + s * kLtSlot + row_at, sp = pre0 + s * kLtSlot + row_at;
                 uint32_t r[32];
                 tmem_ld32(t_acc + (uint32_t)(j * 32), r);
                 if constexpr (!PARTIAL) {
                     if (a.has_residual) {
                         load_residual(NO - 1 - ahead);
-                        if (!all_wait(&my_rbar[s], (uint32_t)((blk / NO) & 1))) ok = false;
+                        if (all_wait(&my_rbar[s], s_phase)) --outstanding;
+                        else ok = false;
                     } else {
                         if (lane == 0) lt_wait_read(NO - 1);
                     }
@@ -321,7 +352,7 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                 if (!ok) break;
                 if constexpr (PARTIAL) {
                     const int row = m0 + quad * 32 + lane;
-                    float *dst = a.partial + (split * a.M + row) * (int64_t)a.N + n0 + j * 32;
+                    float *dst = a.partial + ((int64_t)w.split * a.M + row) * a.N + n0 + j * 32;
                     if (row < a.M) {
 #pragma unroll
                         for (int v = 0; v < 8; ++v)
@@ -388,8 +419,8 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
             if (lane == 0) mbar_arrive(smem_u32(&accempty[buf]));
         }
         if (!PARTIAL && lane == 0) {
-            for (int64_t j = blk; j < loads; ++j)             // residual loads nobody waited for
-                mbar_wait_bounded(smem_u32(&my_rbar[j % NO]), (uint32_t)((j / NO) & 1), kTmaDrainNs);
+            for (; outstanding > 0; --outstanding, next(s, s_phase, NO))     // residual loads nobody waited for
+                mbar_wait_bounded(smem_u32(&my_rbar[s]), s_phase, kTmaDrainNs);
             bulk_wait<0>();
         }
     }
@@ -457,12 +488,14 @@ static int lt_launch(const GemmArgs &g) {
     LtArgs a = {};
     a.M = (int)g.M;
     a.N = (int)g.N;
-    a.K = g.K;
+    a.K = (int)g.K;
     a.BN = A_T ? (g.N > 128 ? 256 : g.N > 64 ? 128 : 64) : lt_bn(g.M, g.N, g.splits);
     a.nb = (int)((g.N + a.BN - 1) / a.BN);
-    a.tiles = (g.M + kLtBM - 1) / kLtBM * a.nb;
-    a.items = a.tiles * g.splits;
-    a.k_per_split = g.splits > 1 ? g.k_per_split : g.K;
+    const int64_t items = (g.M + kLtBM - 1) / kLtBM * a.nb * g.splits;
+    SPCONV_REQUIRE(items < (int64_t)1 << 30, SPCONV_ERR_ARG, "too many output tiles");
+    a.items = (int)items;
+    a.tiles = a.items / g.splits;
+    a.k_per_split = (int)(g.splits > 1 ? g.k_per_split : g.K);
     a.bufs = a.BN == 256 ? 2 : 4;
     a.bias = g.bias;
     a.bias_smem = g.bias && g.N <= kLtMaxBias ? (int)g.N : 0;
@@ -472,7 +505,7 @@ static int lt_launch(const GemmArgs &g) {
     a.status = g.status;
     a.wait_ns = wait_limit_ns();
     const int sms = lt_sms();
-    int64_t grid = std::min<int64_t>(sms, a.items);
+    int grid = std::min(sms, a.items);
     const int64_t nk = (g.K + kLtBK - 1) / kLtBK;
     const int b_bytes = a.BN * 128, room = kLtMaxSmem - 1024 - kLtTail - a.bias_smem * 4;
     auto fit = [&](int resident) {          // output slots and stages beside `resident` K steps of B
