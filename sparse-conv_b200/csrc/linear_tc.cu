@@ -55,7 +55,7 @@ struct LtArgs {
     int k_per_split;                        // a multiple of 64 unless splits == 1
     int BN, stages, slots;                  // slots per epilogue warp (outputs; as many again for preact)
     int bufs;                               // TMEM accumulators
-    int bias_smem;                          // bias columns in shared memory (N or 0)
+    int bias_smem;                          // bias columns in shared memory (N up to whole chunks of 32, or 0)
     int b_resident;                         // K steps of B that stay in shared memory, or 0
     const void *bias;
     int has_residual, has_preact;
@@ -96,7 +96,7 @@ __device__ __forceinline__ float2 lt_unpack<__nv_bfloat16>(uint32_t v) {
 
 // Eight values, rounded, as one 16-byte store to shared memory.
 template <typename T>
-__device__ __forceinline__ void lt_store8(uint32_t dst, const f32x2 (&f)[4]) {
+__device__ __forceinline__ void lt_store8(uint32_t dst, const f32x2 *f) {
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -133,7 +133,8 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int G = gridDim.x;
     const uint32_t tmem_cols = (uint32_t)(a.bufs * BN);                // 256 or 512
-    for (int i = tid; i < a.bias_smem; i += kLtThreads) s_bias[i] = dtype_traits<T>::to_f(((const T *)a.bias)[i]);
+    for (int i = tid; i < a.bias_smem; i += kLtThreads)
+        s_bias[i] = i < a.N ? dtype_traits<T>::to_f(((const T *)a.bias)[i]) : 0.f;
     if (tid == 0) {
         for (int s = 0; s < S; ++s) {
             mbar_init(smem_u32(&full[s]), 1);
@@ -362,46 +363,46 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                                                    __uint_as_float(r[4 * v + 2]), __uint_as_float(r[4 * v + 3])));
                     }
                 } else {
+                    f32x2 f[16];
 #pragma unroll
-                    for (int v = 0; v < 4; ++v) {
-                        const uint32_t at = ((uint32_t)v ^ row_x) << 4;
-                        f32x2 f[4];
+                    for (int i = 0; i < 16; ++i) f[i] = pack_f32x2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
+                    if (a.bias_smem) {
+                        const ulonglong2 *b = reinterpret_cast<const ulonglong2 *>(s_bias + n0 + j * 32);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            f[i] = pack_f32x2(__uint_as_float(r[8 * v + 2 * i]), __uint_as_float(r[8 * v + 2 * i + 1]));
-                        if (a.bias_smem) {
-                            const int n = n0 + j * 32 + v * 8;
-                            if (n < a.N) {
-                                const ulonglong2 *b = reinterpret_cast<const ulonglong2 *>(s_bias + n);
-                                const ulonglong2 b0 = b[0], b1 = b[1];
-                                f[0] = add2(f[0], {b0.x});
-                                f[1] = add2(f[1], {b0.y});
-                                f[2] = add2(f[2], {b1.x});
-                                f[3] = add2(f[3], {b1.y});
-                            }
-                        } else if (a.bias) {
-                            const T *b = (const T *)a.bias + n0 + j * 32 + v * 8;
-                            if (n0 + j * 32 + v * 8 < a.N) {
-#pragma unroll
-                                for (int i = 0; i < 4; ++i)
-                                    f[i] = add2(f[i], pack_f32x2(dtype_traits<T>::to_f(b[2 * i]), dtype_traits<T>::to_f(b[2 * i + 1])));
-                            }
+                        for (int i = 0; i < 8; ++i) {
+                            const ulonglong2 b2 = b[i];
+                            f[2 * i] = add2(f[2 * i], {b2.x});
+                            f[2 * i + 1] = add2(f[2 * i + 1], {b2.y});
                         }
-                        if (a.has_preact) lt_store8<T>(sp + at, f);
+                    } else if (a.bias) {
+                        const T *b = (const T *)a.bias + n0 + j * 32;
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) f[i] = act_value2<ACT>(f[i]);
-                        if (a.has_residual) {
+                        for (int i = 0; i < 16; ++i)
+                            if (n0 + j * 32 + 2 * i < a.N)
+                                f[i] = add2(f[i], pack_f32x2(dtype_traits<T>::to_f(b[2 * i]), dtype_traits<T>::to_f(b[2 * i + 1])));
+                    }
+                    if (a.has_preact) {
+#pragma unroll
+                        for (int v = 0; v < 4; ++v) lt_store8<T>(sp + (((uint32_t)v ^ row_x) << 4), f + 4 * v);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) f[i] = act_value2<ACT>(f[i]);
+                    if (a.has_residual) {
+#pragma unroll
+                        for (int v = 0; v < 4; ++v) {
                             uint32_t q[4];
                             asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];\n"
-                                         : "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3]) : "r"(so + at) : "memory");
+                                         : "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3])
+                                         : "r"(so + (((uint32_t)v ^ row_x) << 4)) : "memory");
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
                                 const float2 x = lt_unpack<T>(q[i]);
-                                f[i] = add2(f[i], pack_f32x2(x.x, x.y));
+                                f[4 * v + i] = add2(f[4 * v + i], pack_f32x2(x.x, x.y));
                             }
                         }
-                        lt_store8<T>(so + at, f);
                     }
+#pragma unroll
+                    for (int v = 0; v < 4; ++v) lt_store8<T>(so + (((uint32_t)v ^ row_x) << 4), f + 4 * v);
                     fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) {
@@ -498,7 +499,7 @@ static int lt_launch(const GemmArgs &g) {
     a.k_per_split = (int)(g.splits > 1 ? g.k_per_split : g.K);
     a.bufs = a.BN == 256 ? 2 : 4;
     a.bias = g.bias;
-    a.bias_smem = g.bias && g.N <= kLtMaxBias ? (int)g.N : 0;
+    a.bias_smem = g.bias && g.N <= kLtMaxBias ? (a.N + 31) & ~31 : 0;
     a.has_residual = g.residual != nullptr;
     a.has_preact = g.preact != nullptr;
     a.partial = g.partial;
