@@ -76,15 +76,19 @@ __device__ __forceinline__ float relu_nan(float x) {          // max(x, 0), NaN 
 // For t = min(|z|, 16): E = exp(-t^2 / 2) and -q, q = 1 - Phi(t) = E * P(t) with P a degree-9
 // polynomial for exp(t^2 / 2) (1 - Phi(t)), fitted here on [0, 4.5] for the least weighted error:
 // |dq| <= 6.5e-7 everywhere, and within 6e-4 of q itself up to t = 4. Beyond 16, E is zero.
-__device__ __forceinline__ void normal_tail2(float2 z, f32x2 &t, float2 &e, f32x2 &minus_q) {
-    t = pack_f32x2(fminf(fabsf(z.x), 16.f), fminf(fabsf(z.y), 16.f));
-    const float2 x = unpack_f32x2(mul2(mul2(t, t), pack_f32x2(-0.72134752f, -0.72134752f)));   // -log2(e) / 2
-    e = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+constexpr float kTailScale = -0.72134752f;                 // -log2(e) / 2
+__host__ __device__ constexpr float tail_coef(int k) {      // of -P
     constexpr float c[10] = {-0.49999940f, 0.39890096f, -0.24953401f, 0.13094953f, -0.057988375f,
                              0.020727100f, -0.0055298521f, 9.9795568e-4f, -1.0617938e-4f, 4.9614673e-6f};
-    f32x2 p = pack_f32x2(c[9], c[9]);
+    return c[k];
+}
+__device__ __forceinline__ void normal_tail2(float2 z, f32x2 &t, float2 &e, f32x2 &minus_q) {
+    t = pack_f32x2(fminf(fabsf(z.x), 16.f), fminf(fabsf(z.y), 16.f));
+    const float2 x = unpack_f32x2(mul2(mul2(t, t), pack_f32x2(kTailScale, kTailScale)));
+    e = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+    f32x2 p = pack_f32x2(tail_coef(9), tail_coef(9));
 #pragma unroll
-    for (int k = 8; k >= 0; --k) p = fma2(p, t, pack_f32x2(c[k], c[k]));
+    for (int k = 8; k >= 0; --k) p = fma2(p, t, pack_f32x2(tail_coef(k), tail_coef(k)));
     minus_q = mul2(p, pack_f32x2(e.x, e.y));
 }
 
@@ -104,6 +108,42 @@ __device__ __forceinline__ f32x2 act_value2(f32x2 z2) {
     const f32x2 d = add2(pack_f32x2(ex2_approx(x.x), ex2_approx(x.y)), pack_f32x2(1.f, 1.f));
     const float2 d1 = unpack_f32x2(d);
     return mul2(z2, pack_f32x2(rcp_approx(d1.x), rcp_approx(d1.y)));
+}
+
+// act(z) for four pairs, step by step across them: each step's four packed operations are
+// independent, which covers one operation's latency without another warp's help.
+template <int ACT>
+__device__ __forceinline__ void act_value8(f32x2 *f) {
+    if constexpr (ACT == SPCONV_ACT_GELU) {
+        f32x2 t[4], e[4], p[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 z = unpack_f32x2(f[i]);
+            t[i] = pack_f32x2(fminf(fabsf(z.x), 16.f), fminf(fabsf(z.y), 16.f));
+            f[i] = pack_f32x2(relu_nan(z.x), relu_nan(z.y));
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) e[i] = mul2(t[i], t[i]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) e[i] = mul2(e[i], pack_f32x2(kTailScale, kTailScale));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 x = unpack_f32x2(e[i]);
+            e[i] = pack_f32x2(ex2_approx(x.x), ex2_approx(x.y));
+            p[i] = pack_f32x2(tail_coef(9), tail_coef(9));
+        }
+#pragma unroll
+        for (int k = 8; k >= 0; --k)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) p[i] = fma2(p[i], t[i], pack_f32x2(tail_coef(k), tail_coef(k)));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[i] = mul2(p[i], e[i]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] = fma2(t[i], p[i], f[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] = act_value2<ACT>(f[i]);
+    }
 }
 
 // act'(z) for a pair.

@@ -15,7 +15,7 @@
 //               layers over millions of voxels, whose bound is HBM);
 //   warp 1      MMA: one thread; the accumulators take turns in two (BN = 256) or four TMEM buffers;
 //   warps 2-17  four epilogue groups of four warps (one per TMEM lane quadrant), a group per
-//               buffer, or two that share a buffer's columns: 32 columns at a time from TMEM to
+//               buffer, or two that share a buffer's columns: 64 columns at a time from TMEM to
 //               registers, + bias, act, + residual, one rounding, into swizzled shared memory and out
 //               by TMA (which clips ragged edges). The residual arrives by TMA, ahead of its turn, in
 //               the slot the output leaves from. Four warps per scheduler, since GELU and SiLU are
@@ -38,7 +38,7 @@ constexpr int kLtThreads = 576;
 constexpr int kLtBM = 128, kLtBK = 64;
 constexpr int kLtABytes = kLtBM * kLtBK * 2;            // 16 KB a stage
 constexpr int kLtEpiWarps = 16, kLtEpiGroups = 4;
-constexpr int kLtSlot = 32 * 64;                        // 32 rows of 32 columns
+constexpr int kLtSlot = 32 * 128;                       // 32 rows of 64 columns
 constexpr int kLtMaxBias = 4096;                        // bias columns kept in shared memory
 constexpr int kLtMaxStages = 12;
 constexpr int kLtMaxSlots = 4;
@@ -294,10 +294,10 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         const uint32_t slot0 = s_out + (uint32_t)(ew * warp_slots * kLtSlot);
         const uint32_t pre0 = slot0 + (uint32_t)(NO * kLtSlot);
         uint64_t *my_rbar = rbar + ew * NO;
-        const uint32_t row_at = (uint32_t)(lane * 64), row_x = (uint32_t)((lane >> 1) & 3);
+        const uint32_t row_at = (uint32_t)(lane * 128), row_x = (uint32_t)(lane & 7);
         // one answer for the warp: its lanes must not part before the next warp-wide instruction
         auto all_wait = [&](uint64_t *b, uint32_t parity) { return __all_sync(0xffffffffu, wait(b, parity)) != 0; };
-        auto chunks_of = [&](int n0) { return (min(BN, a.N - n0) + 31) >> 5; };
+        auto chunks_of = [&](int n0) { return (min(BN, a.N - n0) + 63) >> 6; };
         // Residual loads run `ahead` chunks before their use. The slot of load L was last the
         // store of chunk L - NO, and when chunk b begins, b stores have been committed: those after
         // L - NO = b + ahead - NO may still be reading.
@@ -315,7 +315,7 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                 lt_wait_read(behind);
                 if (more) {
                     mbar_arrive_expect_tx(smem_u32(&my_rbar[l_slot]), kLtSlot);
-                    tma_load_2d(slot0 + l_slot * kLtSlot, &map_res, lw.n * BN + l_chunk * 32, lw.m * kLtBM + quad * 32,
+                    tma_load_2d(slot0 + l_slot * kLtSlot, &map_res, lw.n * BN + l_chunk * 64, lw.m * kLtBM + quad * 32,
                                 smem_u32(&my_rbar[l_slot]));
                 }
             }
@@ -337,8 +337,6 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
             bool ok = true;
             for (int j = sub; j < chunks; j += share, next(s, s_phase, NO)) {
                 const uint32_t so = slot0 + s * kLtSlot + row_at, sp = pre0 + s * kLtSlot + row_at;
-                uint32_t r[32];
-                tmem_ld32(t_acc + (uint32_t)(j * 32), r);
                 if constexpr (!PARTIAL) {
                     if (a.has_residual) {
                         load_residual(NO - 1 - ahead);
@@ -348,26 +346,33 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                         if (lane == 0) lt_wait_read(NO - 1);
                     }
                     __syncwarp();
+                    if (!ok) break;
                 }
-                tc_wait_ld();
-                if (!ok) break;
-                if constexpr (PARTIAL) {
-                    const int row = m0 + quad * 32 + lane;
-                    float *dst = a.partial + ((int64_t)w.split * a.M + row) * a.N + n0 + j * 32;
-                    if (row < a.M) {
+#pragma unroll 1
+                for (int half = 0; half < 2; ++half) {
+                    const int c0 = j * 64 + half * 32;        // columns within the tile
+                    if (c0 >= n_cols) break;
+                    uint32_t r[32];
+                    tmem_ld32(t_acc + (uint32_t)c0, r);
+                    tc_wait_ld();
+                    if constexpr (PARTIAL) {
+                        const int row = m0 + quad * 32 + lane;
+                        float *dst = a.partial + ((int64_t)w.split * a.M + row) * a.N + n0 + c0;
+                        if (row < a.M) {
 #pragma unroll
-                        for (int v = 0; v < 8; ++v)
-                            if (j * 32 + v * 4 < n_cols)
-                                __stcg(reinterpret_cast<float4 *>(dst) + v,
-                                       make_float4(__uint_as_float(r[4 * v]), __uint_as_float(r[4 * v + 1]),
-                                                   __uint_as_float(r[4 * v + 2]), __uint_as_float(r[4 * v + 3])));
+                            for (int v = 0; v < 8; ++v)
+                                if (c0 + v * 4 < n_cols)
+                                    __stcg(reinterpret_cast<float4 *>(dst) + v,
+                                           make_float4(__uint_as_float(r[4 * v]), __uint_as_float(r[4 * v + 1]),
+                                                       __uint_as_float(r[4 * v + 2]), __uint_as_float(r[4 * v + 3])));
+                        }
+                        continue;
                     }
-                } else {
                     f32x2 f[16];
 #pragma unroll
                     for (int i = 0; i < 16; ++i) f[i] = pack_f32x2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
                     if (a.bias_smem) {
-                        const ulonglong2 *b = reinterpret_cast<const ulonglong2 *>(s_bias + n0 + j * 32);
+                        const ulonglong2 *b = reinterpret_cast<const ulonglong2 *>(s_bias + n0 + c0);
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
                             const ulonglong2 b2 = b[i];
@@ -375,25 +380,26 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                             f[2 * i + 1] = add2(f[2 * i + 1], {b2.y});
                         }
                     } else if (a.bias) {
-                        const T *b = (const T *)a.bias + n0 + j * 32;
+                        const T *b = (const T *)a.bias + n0 + c0;
 #pragma unroll
                         for (int i = 0; i < 16; ++i)
-                            if (n0 + j * 32 + 2 * i < a.N)
+                            if (c0 + 2 * i < n_cols)
                                 f[i] = add2(f[i], pack_f32x2(dtype_traits<T>::to_f(b[2 * i]), dtype_traits<T>::to_f(b[2 * i + 1])));
                     }
+                    const uint32_t v0 = (uint32_t)half * 4;
                     if (a.has_preact) {
 #pragma unroll
-                        for (int v = 0; v < 4; ++v) lt_store8<T>(sp + (((uint32_t)v ^ row_x) << 4), f + 4 * v);
+                        for (int v = 0; v < 4; ++v) lt_store8<T>(sp + (((v0 + v) ^ row_x) << 4), f + 4 * v);
                     }
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) f[i] = act_value2<ACT>(f[i]);
+                    for (int i = 0; i < 16; i += 4) act_value8<ACT>(f + i);
                     if (a.has_residual) {
 #pragma unroll
                         for (int v = 0; v < 4; ++v) {
                             uint32_t q[4];
                             asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];\n"
                                          : "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3])
-                                         : "r"(so + (((uint32_t)v ^ row_x) << 4)) : "memory");
+                                         : "r"(so + (((v0 + v) ^ row_x) << 4)) : "memory");
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
                                 const float2 x = lt_unpack<T>(q[i]);
@@ -402,13 +408,15 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                         }
                     }
 #pragma unroll
-                    for (int v = 0; v < 4; ++v) lt_store8<T>(so + (((uint32_t)v ^ row_x) << 4), f + 4 * v);
+                    for (int v = 0; v < 4; ++v) lt_store8<T>(so + (((v0 + v) ^ row_x) << 4), f + 4 * v);
+                }
+                if constexpr (!PARTIAL) {
                     fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) {
                         if (m0 + quad * 32 < a.M) {
-                            tma_store_2d(&map_out, n0 + j * 32, m0 + quad * 32, slot0 + s * kLtSlot);
-                            if (a.has_preact) tma_store_2d(&map_pre, n0 + j * 32, m0 + quad * 32, pre0 + s * kLtSlot);
+                            tma_store_2d(&map_out, n0 + j * 64, m0 + quad * 32, slot0 + s * kLtSlot);
+                            if (a.has_preact) tma_store_2d(&map_pre, n0 + j * 64, m0 + quad * 32, pre0 + s * kLtSlot);
                         }
                         bulk_commit();       // one group a chunk, empty or not
                     }
@@ -537,9 +545,9 @@ static int lt_launch(const GemmArgs &g) {
     const bool maps =
         (A_T ? make_tmap_2d(&ma, g.a, g.M, g.K, g.M * 2, 64, 64) : make_tmap_2d(&ma, g.a, g.K, g.M, g.K * 2, 64, kLtBM)) &&
         (B_T ? make_tmap_2d(&mb, g.b, g.N, g.K, g.N * 2, 64, 64) : make_tmap_2d(&mb, g.b, g.K, g.N, g.K * 2, 64, a.BN)) &&
-        (A_T || make_tmap_2d(&mo, g.out, g.N, g.M, g.N * 2, 32, 32)) &&
-        (!g.residual || make_tmap_2d(&mr, g.residual, g.N, g.M, g.N * 2, 32, 32)) &&
-        (!g.preact || make_tmap_2d(&mp, g.preact, g.N, g.M, g.N * 2, 32, 32));
+        (A_T || make_tmap_2d(&mo, g.out, g.N, g.M, g.N * 2, 64, 32)) &&
+        (!g.residual || make_tmap_2d(&mr, g.residual, g.N, g.M, g.N * 2, 64, 32)) &&
+        (!g.preact || make_tmap_2d(&mp, g.preact, g.N, g.M, g.N * 2, 64, 32));
     if (!maps) return SPCONV_ERR_CUDA;
     if (A_T) mo = ma;                       // maps that the kernel does not read
     if (!g.residual) mr = ma;
