@@ -149,6 +149,17 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t addr, uint32_t parity) {
         : "=r"(ok) : "r"(addr), "r"(parity) : "memory");
     return ok != 0;
 }
+// As mbar_try_wait, with a hint of how long the hardware may suspend the thread (it wakes when the
+// phase completes): a long wait then costs no issue slots of the warps that have work.
+__device__ __forceinline__ bool mbar_try_wait_suspended(uint32_t addr, uint32_t parity, uint32_t hint_ns) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred P;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 P, [%1], %2, %3;\n\t"
+        "selp.b32 %0, 1, 0, P;\n\t}\n"
+        : "=r"(ok) : "r"(addr), "r"(parity), "r"(hint_ns) : "memory");
+    return ok != 0;
+}
 // Non-blocking test: has the phase with the given parity completed?
 __device__ __forceinline__ bool mbar_test(uint32_t addr, uint32_t parity) {
     uint32_t ok;
@@ -239,6 +250,22 @@ __device__ __forceinline__ bool mbar_wait_or_abort(uint32_t addr, uint32_t parit
     }
 }
 
+// The same with suspended waits (up to 20 us between checks of the flag and the limit).
+__device__ __forceinline__ bool mbar_wait_suspended(uint32_t addr, uint32_t parity, volatile int *abort_flag,
+                                                    uint64_t limit_ns) {
+    constexpr uint32_t kHintNs = 20000;
+    if (mbar_try_wait(addr, parity)) return true;
+    const uint64_t t0 = globaltimer_ns();
+    for (;;) {
+        if (mbar_try_wait_suspended(addr, parity, kHintNs)) return true;
+        if (*abort_flag) return false;
+        if (globaltimer_ns() - t0 > limit_ns) {
+            *abort_flag = 1;
+            return false;
+        }
+    }
+}
+
 // ---------------------------------------------------------------------------------------
 // tcgen05 (sm_100a): TMEM allocation, MMA issue/commit, TMEM -> register loads.
 // ---------------------------------------------------------------------------------------
@@ -292,19 +319,6 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]),
           "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
           "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(taddr) : "memory");
-}
-
-// 32 lanes x 32 bits, 32 consecutive columns: thread l of the warp gets lane (base+l).
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(taddr) : "memory");
 }
 

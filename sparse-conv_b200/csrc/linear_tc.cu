@@ -94,6 +94,27 @@ __device__ __forceinline__ float2 lt_unpack<__nv_bfloat16>(uint32_t v) {
     return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
 }
 
+// 32 accumulator columns of the lane's row as 16 packed pairs, complete on return. The wait and the
+// pairing stand in the same statement as the load so that no copy is needed between them.
+__device__ __forceinline__ void lt_load32(uint32_t taddr, f32x2 (&f)[16]) {
+    asm volatile(
+        "{\n\t.reg .b32 x<32>;\n\t"
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
+        "x0,x1,x2,x3,x4,x5,x6,x7,x8,x9,x10,x11,x12,x13,x14,x15,"
+        "x16,x17,x18,x19,x20,x21,x22,x23,x24,x25,x26,x27,x28,x29,x30,x31}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;\n\t"
+        "mov.b64 %0, {x0,x1}; mov.b64 %1, {x2,x3}; mov.b64 %2, {x4,x5}; mov.b64 %3, {x6,x7}; "
+        "mov.b64 %4, {x8,x9}; mov.b64 %5, {x10,x11}; mov.b64 %6, {x12,x13}; mov.b64 %7, {x14,x15}; "
+        "mov.b64 %8, {x16,x17}; mov.b64 %9, {x18,x19}; mov.b64 %10, {x20,x21}; mov.b64 %11, {x22,x23}; "
+        "mov.b64 %12, {x24,x25}; mov.b64 %13, {x26,x27}; mov.b64 %14, {x28,x29}; mov.b64 %15, {x30,x31}; "
+        "}\n"
+        : "=l"(f[0].v), "=l"(f[1].v), "=l"(f[2].v), "=l"(f[3].v),
+          "=l"(f[4].v), "=l"(f[5].v), "=l"(f[6].v), "=l"(f[7].v),
+          "=l"(f[8].v), "=l"(f[9].v), "=l"(f[10].v), "=l"(f[11].v),
+          "=l"(f[12].v), "=l"(f[13].v), "=l"(f[14].v), "=l"(f[15].v)
+        : "r"(taddr) : "memory");
+}
+
 // Eight values, rounded, as one 16-byte store to shared memory.
 template <typename T>
 __device__ __forceinline__ void lt_store8(uint32_t dst, const f32x2 *f) {
@@ -158,7 +179,7 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     tc_fence_after();
     const uint32_t tmem = *s_tmem;
     auto wait = [&](uint64_t *b, uint32_t parity) -> bool {
-        return mbar_wait_or_abort(smem_u32(b), parity, s_abort, a.wait_ns);
+        return mbar_wait_suspended(smem_u32(b), parity, s_abort, a.wait_ns);
     };
     // A walk over every `step`-th item: its tile and its range of K. Divisions only at the start (the
     // single loading and MMA threads would spend longer on them than on a tile's copies).
@@ -352,32 +373,29 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                 for (int half = 0; half < 2; ++half) {
                     const int c0 = j * 64 + half * 32;        // columns within the tile
                     if (c0 >= n_cols) break;
-                    uint32_t r[32];
-                    tmem_ld32(t_acc + (uint32_t)c0, r);
-                    tc_wait_ld();
+                    f32x2 f[16];
+                    lt_load32(t_acc + (uint32_t)c0, f);
                     if constexpr (PARTIAL) {
                         const int row = m0 + quad * 32 + lane;
                         float *dst = a.partial + ((int64_t)w.split * a.M + row) * a.N + n0 + c0;
                         if (row < a.M) {
 #pragma unroll
                             for (int v = 0; v < 8; ++v)
-                                if (c0 + v * 4 < n_cols)
-                                    __stcg(reinterpret_cast<float4 *>(dst) + v,
-                                           make_float4(__uint_as_float(r[4 * v]), __uint_as_float(r[4 * v + 1]),
-                                                       __uint_as_float(r[4 * v + 2]), __uint_as_float(r[4 * v + 3])));
+                                if (c0 + v * 4 < n_cols) {
+                                    const float2 lo = unpack_f32x2(f[2 * v]), hi = unpack_f32x2(f[2 * v + 1]);
+                                    __stcg(reinterpret_cast<float4 *>(dst) + v, make_float4(lo.x, lo.y, hi.x, hi.y));
+                                }
                         }
                         continue;
                     }
-                    f32x2 f[16];
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) f[i] = pack_f32x2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
                     if (a.bias_smem) {
-                        const ulonglong2 *b = reinterpret_cast<const ulonglong2 *>(s_bias + n0 + c0);
+                        const uint32_t b = smem_u32(s_bias + n0 + c0);
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
-                            const ulonglong2 b2 = b[i];
-                            f[2 * i] = add2(f[2 * i], {b2.x});
-                            f[2 * i + 1] = add2(f[2 * i + 1], {b2.y});
+                            f32x2 b0, b1;
+                            asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];\n" : "=l"(b0.v), "=l"(b1.v) : "r"(b + i * 16));
+                            f[2 * i] = add2(f[2 * i], b0);
+                            f[2 * i + 1] = add2(f[2 * i + 1], b1);
                         }
                     } else if (a.bias) {
                         const T *b = (const T *)a.bias + n0 + c0;
