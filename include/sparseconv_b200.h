@@ -326,8 +326,10 @@ int spconv_linear_backward(const void *grad_out, const void *preact, const void 
  * sample inside the range). channels <= 8192, num_samples <= 65535, num_rows < 2^31.
  * hidden may be residual or feats itself and normed may be feats itself (a row is read before it
  * is written); outputs may not otherwise overlap inputs or each other.
- * The backward takes the forward's inputs (not its outputs), grad_hidden and / or grad_normed,
- * and writes grad_feats, grad_residual and each parameter's `grad` where not NULL, the latter in
+ * row_stats [num_rows, 4] fp32, 16-byte aligned: mean and 1 / deviation of each row under both
+ * norms (0 and 1 where there is none); written by the forward unless NULL, read by the backward.
+ * The backward takes the forward's inputs (not its outputs), row_stats, grad_hidden and / or
+ * grad_normed, and writes grad_feats, grad_residual and each parameter's `grad` where not NULL, the latter in
  * the parameter's type and shape, the same bits in every run; its outputs overlap no input.
  *   workspace (backward, if a parameter's gradient is wanted): 16-byte aligned,
  *   spconv_residual_norm_workspace_bytes(num_rows, channels, num_samples) bytes.
@@ -349,6 +351,7 @@ typedef struct {
     void *hidden, *normed;
     const void *grad_hidden, *grad_normed;
     void *grad_feats, *grad_residual;
+    float *row_stats;                 /* [num_rows, 4] */
     spconv_channel_param gate, weight, bias, next_weight, next_bias;
     const int32_t *offsets;
     int num_samples;

@@ -13,9 +13,15 @@
 //   G  = dh + rstd2 * (t - mean(t) - hhat * mean(t * hhat))       (RMS: without mean(t))
 //   dr = alpha * G;  du = G * g;  dx = N1's gradient of du * w1, by the same formula
 //   dw2 = sum dy * hhat, db2 = sum dy, dg = sum G * u, dw1 = sum du * xhat, db1 = sum du
-// over all rows, or over a sample's rows. Nothing is kept from the forward: u, h and the
-// statistics are recomputed from x and r in fp32, so the forward's rounding of h does not enter
-// the gradients, and x and r are as many bytes as x and h would be.
+// over all rows, or over a sample's rows. The forward keeps four fp32 numbers a row (mean and rstd
+// of both norms); u and h are recomputed from x and r in fp32, so the forward's rounding of h does
+// not enter the gradients, and x and r are as many bytes as x and h would be. Recomputing the
+// statistics too would save those 16 bytes a row and cost two more reductions over the row, which
+// are what bounds the backward after HBM.
+//
+// LayerNorm's statistics take one reduction, of the sums of d and d^2, d = t - t[0]: any value of
+// the row lies within sqrt(C) deviations of its mean, so mean(d^2) - mean(d)^2 loses at most a
+// factor C of the variance's digits whatever offset the row has in common.
 //
 // Bound: HBM. Forward reads x, r and writes h, y; backward reads x, r, dh, dy and writes dx, dr.
 // All arithmetic is fp32; each output is rounded once. A row lives in the registers of the
@@ -38,6 +44,7 @@ struct RnArgs {
     void *h, *y;                         // forward outputs (y null without N2)
     const void *dh, *dy;                 // backward inputs (either may be null)
     void *dx, *dr;                       // backward outputs (either may be null)
+    float4 *stats;                       // [M] mean1, rstd1, mean2, rstd2 (forward: may be null)
     const void *p[kRnParams];            // parameters (null: 1 for g, w; 0 for b)
     int p_f32[kRnParams];                // 1: fp32, 0: the features' type
     int64_t p_stride[kRnParams];         // C if there is a row per sample, else 0
@@ -146,75 +153,121 @@ __device__ __forceinline__ void rn_param(const RnArgs &a, int k, int s, int col,
     }
 }
 
-// Sums of two values over the lanes that share a row: lpr lanes of a warp, or the whole block.
-template <bool BLOCK>
-__device__ __forceinline__ void rn_sum2(float &u, float &v, int lpr, float2 *scratch) {
+// Sums of U pairs of values over the lanes that share a row: lpr lanes of a warp, or the block.
+// Without `both` only the second of each pair is summed.
+template <int U, bool BLOCK>
+__device__ __forceinline__ void rn_sum2(float (&u)[U], float (&v)[U], bool both, int lpr, float2 *scratch) {
     const int top = BLOCK ? 16 : lpr >> 1;
-    for (int o = top; o > 0; o >>= 1) {
-        u += __shfl_xor_sync(0xffffffffu, u, o);
-        v += __shfl_xor_sync(0xffffffffu, v, o);
+    if (both) {
+        for (int o = top; o > 0; o >>= 1)
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                u[i] += __shfl_xor_sync(0xffffffffu, u[i], o);
+                v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+            }
+    } else {
+        for (int o = top; o > 0; o >>= 1)
+#pragma unroll
+            for (int i = 0; i < U; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
     }
     if constexpr (BLOCK) {
+        static_assert(U == 1, "a block takes one row at a time");
         __syncthreads();
-        if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = make_float2(u, v);
+        if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = make_float2(u[0], v[0]);
         __syncthreads();
-        u = v = 0.f;
+        u[0] = v[0] = 0.f;
 #pragma unroll
         for (int w = 0; w < kRnWarps; ++w) {
-            u += scratch[w].x;
-            v += scratch[w].y;
+            u[0] += scratch[w].x;
+            v[0] += scratch[w].y;
         }
     }
 }
-template <bool BLOCK>
-__device__ __forceinline__ float rn_sum(float u, int lpr, float2 *scratch) {
-    if constexpr (BLOCK) {
-        float v = 0.f;
-        rn_sum2<true>(u, v, lpr, scratch);
-    } else {
-        for (int o = lpr >> 1; o > 0; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
+
+// Sum of a lane's N values, and of their products with n, as trees (short chains).
+template <int N>
+__device__ __forceinline__ float rn_tree(const float (&t)[N]) {
+    float s[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) s[i] = t[i];
+#pragma unroll
+    for (int w = N / 2; w > 0; w >>= 1)
+#pragma unroll
+        for (int i = 0; i < w; ++i) s[i] += s[i + w];
+    return s[0];
+}
+template <int N>
+__device__ __forceinline__ float rn_dot(const float (&t)[N], const float (&n)[N]) {
+    float p = 0.f, q = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+        p = fmaf(t[i], n[i], p);
+        if (i + 1 < N) q = fmaf(t[i + 1], n[i + 1], q);
     }
-    return u;
+    return p + q;
 }
 
-// Normalises the N values a lane holds of a row in place; returns rstd. The mean is taken out
-// before the squares are summed, so a large common offset costs no digits of the variance.
-template <int N, int VEC, bool BLOCK>
-__device__ __forceinline__ float rn_normalise(float (&t)[N], const bool *have, int kind, float inv_c, float eps, int lpr,
-                                              float2 *scratch) {
-    if (kind == SPCONV_NORM_NONE) return 1.f;
-    if (kind == SPCONV_NORM_LAYER) {
-        float s = 0.f;
+// Normalises U rows, N values of each in a lane, in place: (mean, rstd) of each row in st. Columns
+// that a lane does not have hold zeros, before and after.
+template <int U, int N, int VEC, bool BLOCK>
+__device__ __forceinline__ void rn_normalise(float (&t)[U][N], float2 (&st)[U], const bool *have, int kind, float inv_c,
+                                             float eps, int lpr, float2 *scratch) {
+    if (kind == SPCONV_NORM_NONE) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) s += t[i];
-        const float mean = rn_sum<BLOCK>(s, lpr, scratch) * inv_c;
-#pragma unroll
-        for (int i = 0; i < N; ++i) t[i] = have[i / VEC] ? t[i] - mean : 0.f;
+        for (int u = 0; u < U; ++u) st[u] = make_float2(0.f, 1.f);
+        return;
     }
-    float q = 0.f;
+    float s[U], q[U], first[U];
+    const bool layer = kind == SPCONV_NORM_LAYER;
 #pragma unroll
-    for (int i = 0; i < N; ++i) q += t[i] * t[i];
-    const float rstd = rsqrtf(rn_sum<BLOCK>(q, lpr, scratch) * inv_c + eps);
+    for (int u = 0; u < U; ++u) {
+        first[u] = 0.f;
+        s[u] = 0.f;
+        if (layer) {
+            if constexpr (BLOCK) {
+                __syncthreads();
+                if (threadIdx.x == 0) scratch[0].x = t[u][0];
+                __syncthreads();
+                first[u] = scratch[0].x;
+            } else {
+                first[u] = __shfl_sync(0xffffffffu, t[u][0], 0, lpr);
+            }
 #pragma unroll
-    for (int i = 0; i < N; ++i) t[i] *= rstd;
-    return rstd;
+            for (int i = 0; i < N; ++i) t[u][i] = have[i / VEC] ? t[u][i] - first[u] : 0.f;
+            s[u] = rn_tree<N>(t[u]);
+        }
+        q[u] = rn_dot<N>(t[u], t[u]);
+    }
+    rn_sum2<U, BLOCK>(s, q, layer, lpr, scratch);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const float m = layer ? s[u] * inv_c : 0.f;
+        const float var = q[u] * inv_c - m * m;
+        st[u] = make_float2(first[u] + m, rsqrtf((var < 0.f ? 0.f : var) + eps));     // NaN stays NaN
+#pragma unroll
+        for (int i = 0; i < N; ++i) t[u][i] = have[i / VEC] ? (t[u][i] - m) * st[u].y : 0.f;
+    }
 }
 
 // t: gradient at the normalised values n -> gradient at the values before the norm.
-template <int N, bool BLOCK>
-__device__ __forceinline__ void rn_normalise_back(float (&t)[N], const float (&n)[N], float rstd, int kind, float inv_c,
-                                                  int lpr, float2 *scratch) {
+template <int U, int N, bool BLOCK>
+__device__ __forceinline__ void rn_normalise_back(float (&t)[U][N], const float (&n)[U][N], const float (&rstd)[U],
+                                                  int kind, float inv_c, int lpr, float2 *scratch) {
     if (kind == SPCONV_NORM_NONE) return;
-    float s = 0.f, q = 0.f;
+    float s[U], q[U];
+    const bool layer = kind == SPCONV_NORM_LAYER;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        s += t[i];
-        q += t[i] * n[i];
+    for (int u = 0; u < U; ++u) {
+        s[u] = layer ? rn_tree<N>(t[u]) : 0.f;
+        q[u] = rn_dot<N>(t[u], n[u]);
     }
-    rn_sum2<BLOCK>(s, q, lpr, scratch);
-    const float mean = kind == SPCONV_NORM_LAYER ? s * inv_c : 0.f, along = q * inv_c;
+    rn_sum2<U, BLOCK>(s, q, layer, lpr, scratch);
 #pragma unroll
-    for (int i = 0; i < N; ++i) t[i] = rstd * (t[i] - mean - n[i] * along);
+    for (int u = 0; u < U; ++u) {
+        const float mean = layer ? s[u] * inv_c * rstd[u] : 0.f, along = q[u] * inv_c * rstd[u];
+#pragma unroll
+        for (int i = 0; i < N; ++i) t[u][i] = fmaf(t[u][i], rstd[u], fmaf(-n[u][i], along, -mean));
+    }
 }
 
 // The sample of row r (offsets ascending), always in [0, B).
@@ -293,14 +346,16 @@ residual_norm_fwd_kernel(const __grid_constant__ RnArgs a) {
         fetch(seg + group);
         for (int64_t base = seg; base < end; base += groups) {
             const int64_t row = base + group;
-            float u[N], h[N];
+            float uu[1][N], hh[1][N];
+            float (&u)[N] = uu[0], (&h)[N] = hh[0];
 #pragma unroll
             for (int j = 0; j < VPT; ++j) {
                 rn_unpack(px[j], u + j * VEC);
                 rn_unpack(pr[j], h + j * VEC);
             }
             fetch(row + groups);             // the next row's loads run under this row's sums
-            rn_normalise<N, VEC, BLOCK>(u, have, a.norm1, inv_c, a.eps, lpr, scratch);
+            float2 st1[1], st2[1] = {make_float2(0.f, 1.f)};
+            rn_normalise<1, N, VEC, BLOCK>(uu, st1, have, a.norm1, inv_c, a.eps, lpr, scratch);
 #pragma unroll
             for (int j = 0; j < VPT; ++j) {
                 float g[VEC], w[VEC], b[VEC];
@@ -319,7 +374,7 @@ residual_norm_fwd_kernel(const __grid_constant__ RnArgs a) {
                 if (have[j] && row < end) rn_store((T *)a.h + row * C + col[j], h + j * VEC, (RnPack<T, VEC> *)nullptr);
             }
             if (a.norm2 != SPCONV_NORM_NONE) {
-                rn_normalise<N, VEC, BLOCK>(h, have, a.norm2, inv_c, a.eps, lpr, scratch);
+                rn_normalise<1, N, VEC, BLOCK>(hh, st2, have, a.norm2, inv_c, a.eps, lpr, scratch);
 #pragma unroll
                 for (int j = 0; j < VPT; ++j) {
                     float w[VEC], b[VEC];
@@ -337,6 +392,7 @@ residual_norm_fwd_kernel(const __grid_constant__ RnArgs a) {
                     if (have[j] && row < end) rn_store((T *)a.y + row * C + col[j], h + j * VEC, (RnPack<T, VEC> *)nullptr);
                 }
             }
+            if (a.stats && lane == 0 && row < end) a.stats[row] = make_float4(st1[0].x, st1[0].y, st2[0].x, st2[0].y);
         }
         seg = end;
     }
@@ -435,8 +491,10 @@ residual_norm_bwd_kernel(const __grid_constant__ RnArgs a) {
         for (int64_t base = seg; base < end; base += groups) {
             const int64_t row = base + group;
             if constexpr (!HOIST) fetch(row);
-            float n1[N], n2[N], t[N], gr[N];     // xhat, hhat, dy * w2, dh -> G
+            float n1_[1][N], n2_[1][N], t_[1][N], gr_[1][N];
+            float (&n1)[N] = n1_[0], (&n2)[N] = n2_[0], (&t)[N] = t_[0], (&gr)[N] = gr_[0];   // xhat, hhat, dy * w2, dh -> G
             const bool live = row < end;         // a row past the end holds zeros and adds none
+            const float4 st = live ? __ldg(a.stats + row) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int j = 0; j < VPT; ++j) {
                 rn_unpack(px[j], n1 + j * VEC);
@@ -445,7 +503,9 @@ residual_norm_bwd_kernel(const __grid_constant__ RnArgs a) {
                 rn_unpack(py[j], t + j * VEC);
             }
             if constexpr (HOIST) fetch(row + groups);
-            const float rstd1 = rn_normalise<N, VEC, BLOCK>(n1, have, a.norm1, inv_c, a.eps, lpr, scratch);
+            const float rstd1[1] = {st.y}, rstd2[1] = {st.w};
+#pragma unroll
+            for (int n = 0; n < N; ++n) n1[n] = have[n / VEC] ? (n1[n] - st.x) * st.y : 0.f;
 #pragma unroll
             for (int j = 0; j < VPT; ++j) {
                 float g[VEC], w[VEC], b[VEC];
@@ -463,7 +523,8 @@ residual_norm_bwd_kernel(const __grid_constant__ RnArgs a) {
                 }
             }
             if (a.norm2 != SPCONV_NORM_NONE && a.dy) {
-                const float rstd2 = rn_normalise<N, VEC, BLOCK>(n2, have, a.norm2, inv_c, a.eps, lpr, scratch);
+#pragma unroll
+                for (int n = 0; n < N; ++n) n2[n] = have[n / VEC] ? (n2[n] - st.z) * st.w : 0.f;
 #pragma unroll
                 for (int j = 0; j < VPT; ++j) {
                     float w[VEC], v[VEC];
@@ -478,7 +539,7 @@ residual_norm_bwd_kernel(const __grid_constant__ RnArgs a) {
                     }
                     if (live) add(kW2, j, v);
                 }
-                rn_normalise_back<N, BLOCK>(t, n2, rstd2, a.norm2, inv_c, lpr, scratch);
+                rn_normalise_back<1, N, BLOCK>(t_, n2_, rstd2, a.norm2, inv_c, lpr, scratch);
 #pragma unroll
                 for (int n = 0; n < N; ++n) gr[n] += t[n];
             }
@@ -514,7 +575,7 @@ residual_norm_bwd_kernel(const __grid_constant__ RnArgs a) {
                 if (live) add(kW1, j, v);
             }
             if (a.dx) {
-                rn_normalise_back<N, BLOCK>(gr, n1, rstd1, a.norm1, inv_c, lpr, scratch);
+                rn_normalise_back<1, N, BLOCK>(gr_, n1_, rstd1, a.norm1, inv_c, lpr, scratch);
 #pragma unroll
                 for (int j = 0; j < VPT; ++j)
                     if (have[j] && live) rn_store((T *)a.dx + row * C + col[j], gr + j * VEC, (RnPack<T, VEC> *)nullptr);
@@ -552,6 +613,423 @@ residual_norm_bwd_kernel(const __grid_constant__ RnArgs a) {
         }
         seg = end;
     }
+}
+
+// ---------------------------------------------------------------------------------------
+// Rows of at most 256 channels, many of them: the streams through shared memory.
+//
+// Rows are contiguous, so R of them are one untiled bulk copy per tensor whatever the channel
+// count. One thread keeps a ring of stages of such copies in flight; twelve warps compute in
+// place (the outputs take the inputs' slots) and the same thread stores finished stages in bulk.
+// The direct kernels above hold what is in flight in registers (two loads a lane); measured
+// there and here: 2.0 M x 64 bf16 forward 255 and 186 us, 1.34 M x 128 backward 738 and 358 us.
+// A tile that crosses a sample's end is worked off in two parts, so tiles stay aligned to 16
+// bytes for every channel count; only the last one can end in a few odd bytes, which that thread
+// copies itself.
+// Waits are bounded: a timeout raises SPCONV_STATUS_WAIT_TIMEOUT and the CTA leaves once its
+// copies have landed.
+// ---------------------------------------------------------------------------------------
+constexpr int kRbWarps = 12, kRbThreads = (kRbWarps + 1) * 32;
+constexpr int kRbMaxStages = 8;
+constexpr int kRbTileBytes = 12 * 1024;      // a tensor's share of a stage, about
+constexpr int kRbMaxSmem = 226 * 1024;
+
+struct RbArgs {
+    int rows;                                // per tile, a multiple of 8
+    int stages;
+    int tile_bytes;                          // a tensor's slot in a stage
+    int cols;                                // columns of the parameters in shared memory: every lane's
+    uint64_t wait_ns;
+};
+
+template <typename T, int VEC>
+__device__ __forceinline__ void rn_load_smem(RnPack<T, VEC> &p, const T *src) {
+    if constexpr (VEC == 8) {
+        const uint4 *s = reinterpret_cast<const uint4 *>(src);
+#pragma unroll
+        for (int i = 0; i < (int)(sizeof(p.q) / 16); ++i) p.q[i] = s[i];
+    } else {
+        p.v = *src;
+    }
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void rn_store_smem(T *dst, const float *f) {
+    if constexpr (VEC == 8) {
+        alignas(16) T v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = dtype_traits<T>::from_f(f[i]);
+#pragma unroll
+        for (int i = 0; i < (int)(sizeof(v) / 16); ++i) reinterpret_cast<uint4 *>(dst)[i] = reinterpret_cast<uint4 *>(v)[i];
+    } else {
+        *dst = dtype_traits<T>::from_f(f[0]);
+    }
+}
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t mbar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n"
+                 :: "r"(dst), "l"(src), "r"(bytes), "r"(mbar) : "memory");
+}
+__device__ __forceinline__ void bulk_store(void *dst, uint32_t src, uint32_t bytes) {
+    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;\n" :: "l"(dst), "r"(src), "r"(bytes) : "memory");
+}
+
+template <typename T, int VEC, int VPT, bool BWD>
+__global__ void __launch_bounds__(kRbThreads, 1)
+residual_norm_bulk_kernel(const __grid_constant__ RnArgs a, const __grid_constant__ RbArgs rb) {
+    constexpr int N = VEC * VPT;
+    constexpr int U = N >= 4 ? 2 : 4;        // rows a lane works on at once: their sums overlap
+    static_assert(N <= 8, "a lane's sums stay in registers");
+    constexpr int kTensors = BWD ? 4 : 2;    // slots of a stage: x (then h or dx), r (then y or dr), dh, dy
+    extern __shared__ __align__(128) uint8_t s_raw[];
+    uint64_t *full = reinterpret_cast<uint64_t *>(s_raw), *done = full + kRbMaxStages, *flush = done + kRbMaxStages;
+    volatile int *s_abort = reinterpret_cast<volatile int *>(flush + 1);
+    uint8_t *ring = s_raw + 256;
+    const int S = rb.stages, R = rb.rows, C = a.C, lpr = a.lpr;
+    const int slot = rb.tile_bytes, stage = kTensors * slot + R * 16;          // the rows' statistics last
+    float *s_par = reinterpret_cast<float *>(ring + S * stage);                // [kRnParams][rb.cols]
+    float *s_acc = s_par + kRnParams * rb.cols;                                // [kRbWarps][nslots][C]
+    const int tid = threadIdx.x, warp = tid >> 5;
+    if (tid == 0) {
+        for (int i = 0; i < S; ++i) {
+            mbar_init(smem_u32(&full[i]), 1);
+            mbar_init(smem_u32(&done[i]), kRbWarps);
+        }
+        mbar_init(smem_u32(flush), kRbWarps);
+        *s_abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    }
+    rn_check_offsets(a);
+    __syncthreads();
+    auto wait = [&](uint64_t *b, uint32_t parity) { return mbar_wait_suspended(smem_u32(b), parity, s_abort, rb.wait_ns); };
+    const int64_t row0 = (int64_t)blockIdx.x * a.chunk, row1 = min(a.M, row0 + a.chunk);
+    const int tiles = row0 < row1 ? (int)((row1 - row0 + R - 1) / R) : 0;
+
+    if (warp == kRbWarps) {
+        // ------------------------------------------------------------------ copies
+        if ((tid & 31) == 0) {
+            const T *in[4] = {(const T *)a.x, (const T *)a.r, BWD ? (const T *)a.dh : nullptr, BWD ? (const T *)a.dy : nullptr};
+            T *out[2] = {BWD ? (T *)a.dx : (T *)a.h, BWD ? (T *)a.dr : (T *)a.y};
+            auto load = [&](int t, int s) {
+                const int64_t row = row0 + (int64_t)t * R;
+                const int rows = (int)min((int64_t)R, row1 - row), elems = rows * C;
+                const uint32_t whole = (uint32_t)(elems * (int)sizeof(T)) & ~15u, mbar = smem_u32(&full[s]);
+                uint8_t *base = ring + s * stage;
+                uint32_t total = BWD ? (uint32_t)rows * 16 : 0;
+                for (int k = 0; k < kTensors; ++k)
+                    if (in[k]) {
+                        total += whole;
+                        for (int e = (int)(whole / sizeof(T)); e < elems; ++e)
+                            reinterpret_cast<T *>(base + k * slot)[e] = in[k][row * C + e];
+                    }
+                mbar_arrive_expect_tx(mbar, total);
+                if (BWD) bulk_load(smem_u32(base + kTensors * slot), a.stats + row, (uint32_t)rows * 16, mbar);
+                if (whole > 0)
+                    for (int k = 0; k < kTensors; ++k)
+                        if (in[k]) bulk_load(smem_u32(base + k * slot), in[k] + row * C, whole, mbar);
+            };
+            int loaded = 0;
+            for (; loaded < min(S, tiles); ++loaded) load(loaded, loaded);
+            int s = 0, prev = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int t = 0; t < tiles; ++t) {
+                if (!wait(&done[s], phase)) { ok = false; break; }
+                const int64_t row = row0 + (int64_t)t * R;
+                const int rows = (int)min((int64_t)R, row1 - row), elems = rows * C;
+                const uint32_t whole = (uint32_t)(elems * (int)sizeof(T)) & ~15u;
+                uint8_t *base = ring + s * stage;
+                for (int k = 0; k < 2; ++k)
+                    if (out[k]) {
+                        if (whole > 0) bulk_store(out[k] + row * C, smem_u32(base + k * slot), whole);
+                        for (int e = (int)(whole / sizeof(T)); e < elems; ++e)
+                            out[k][row * C + e] = reinterpret_cast<T *>(base + k * slot)[e];
+                    }
+                if (!BWD && a.stats) bulk_store(a.stats + row, smem_u32(base + kTensors * slot), (uint32_t)rows * 16);
+                bulk_commit();
+                // the stage before this one is free once its stores have read it
+                if (t > 0 && loaded < tiles) {
+                    bulk_wait_read<1>();
+                    load(loaded++, prev);
+                }
+                prev = s;
+                if (++s == S) {
+                    s = 0;
+                    phase ^= 1u;
+                }
+            }
+            if (!ok)                          // loads in flight write shared memory: let them land
+                for (int i = 0; i < min(S, loaded); ++i) {
+                    const int uses = (loaded - 1 - i) / S;    // completed phases of stage i before its last load
+                    mbar_wait_bounded(smem_u32(&full[i]), (uint32_t)(uses & 1), kTmaDrainNs);
+                }
+            bulk_wait<0>();
+        }
+    } else {
+        // ------------------------------------------------------------------ rows
+        const int groups = kRbWarps * 32 / lpr, group = tid / lpr, lane = tid & (lpr - 1);
+        const float inv_c = 1.f / (float)C;
+        int col[VPT];
+        bool have[VPT];
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) {
+            col[j] = (lane + lpr * j) * VEC;
+            have[j] = col[j] < C;
+        }
+        float acc[kRnParams][BWD ? N : 1] = {};
+        uint32_t flush_phase = 0;
+        // All row warps: an mbarrier rather than bar.sync, since its wait is bounded.
+        auto meet = [&]() {
+            __syncwarp();
+            if ((tid & 31) == 0) mbar_arrive(smem_u32(flush));
+            const bool ok = __all_sync(0xffffffffu, wait(flush, flush_phase)) != 0;
+            flush_phase ^= 1u;
+            return ok;
+        };
+        // Puts the sums of sample `from`'s rows (if any) into record blockIdx + from, and sample
+        // `to`'s parameters (if any) into shared memory. False: give up.
+        auto turn = [&](int from, int to) -> bool {
+            if constexpr (BWD) {
+                if (from >= 0) {
+                    float *mine = s_acc + (int64_t)warp * a.nslots * C;
+#pragma unroll
+                    for (int k = 0; k < kRnParams; ++k) {
+                        if (a.slot[k] < 0) continue;
+#pragma unroll
+                        for (int i = 0; i < N; ++i)
+                            for (int o = lpr; o < 32; o <<= 1) acc[k][i] += __shfl_xor_sync(0xffffffffu, acc[k][i], o);
+                        if ((tid & 31) < lpr) {
+#pragma unroll
+                            for (int j = 0; j < VPT; ++j)
+                                if (have[j])
+#pragma unroll
+                                    for (int i = 0; i < VEC; ++i) mine[a.slot[k] * C + col[j] + i] = acc[k][j * VEC + i];
+                        }
+                    }
+                }
+            }
+            if (!meet()) return false;       // every warp is through with `from`
+            if constexpr (BWD) {
+                if (from >= 0) {
+                    const int n = a.nslots * C;
+                    float *rec = a.partial + ((int64_t)blockIdx.x + from) * n;
+                    for (int i = tid; i < n; i += kRbWarps * 32) {
+                        float v = 0.f;
+#pragma unroll
+                        for (int w = 0; w < kRbWarps; ++w) v += s_acc[(int64_t)w * n + i];
+                        rec[i] = v;
+                    }
+#pragma unroll
+                    for (int k = 0; k < kRnParams; ++k)
+#pragma unroll
+                        for (int i = 0; i < N; ++i) acc[k][i] = 0.f;
+                }
+            }
+            if (to >= 0)
+                for (int i = tid; i < kRnParams * rb.cols; i += kRbWarps * 32) {
+                    const int k = i / rb.cols, c = i - k * rb.cols;
+                    float v[1];
+                    rn_param<T, 1>(a, k, to, c < C ? c : 0, v);
+                    s_par[i] = v[0];
+                }
+            return meet();
+        };
+        // VEC parameters of a kind from the lane's j-th columns (rb.cols covers every lane's)
+        auto par = [&](int k, int j, float *f) {
+            const float *p = s_par + k * rb.cols + col[j];
+            if constexpr (VEC == 8) {
+                const float4 u = reinterpret_cast<const float4 *>(p)[0], v = reinterpret_cast<const float4 *>(p)[1];
+                f[0] = u.x; f[1] = u.y; f[2] = u.z; f[3] = u.w;
+                f[4] = v.x; f[5] = v.y; f[6] = v.z; f[7] = v.w;
+            } else {
+                f[0] = *p;
+            }
+        };
+        auto par_all = [&](int k, float (&f)[N]) {
+#pragma unroll
+            for (int j = 0; j < VPT; ++j) par(k, j, f + j * VEC);
+        };
+        int smp = a.B > 1 && tiles > 0 ? rn_sample(a, row0) : 0;
+        auto sample_end = [&](int q) { return q < a.B - 1 ? min(row1, (int64_t)__ldg(a.offsets + q + 1)) : row1; };
+        int64_t s_end = tiles > 0 ? sample_end(smp) : 0;
+        bool ok = tiles > 0 && turn(-1, smp);
+        int s = 0;
+        uint32_t phase = 0;
+        for (int t = 0; t < tiles && ok; ++t) {
+            ok = __all_sync(0xffffffffu, wait(&full[s], phase)) != 0;
+            if (!ok) break;
+            const int64_t tile0 = row0 + (int64_t)t * R, tile1 = min(row1, tile0 + R);
+            uint8_t *base_s = ring + s * stage;
+            T *tx = reinterpret_cast<T *>(base_s), *tr = reinterpret_cast<T *>(base_s + slot);
+            const T *th = reinterpret_cast<const T *>(base_s + (BWD ? 2 * slot : 0));
+            const T *ty = reinterpret_cast<const T *>(base_s + (BWD ? 3 * slot : 0));
+            float4 *ts = reinterpret_cast<float4 *>(base_s + kTensors * slot);
+            for (int64_t part = tile0; part < tile1;) {
+                if (s_end <= part) {         // the next sample that has rows (the last one takes the rest)
+                    const int from = smp;
+                    do s_end = sample_end(++smp);
+                    while (s_end <= part);
+                    if (!turn(from, smp)) { ok = false; break; }
+                }
+                const int64_t end = min(tile1, s_end);
+                const int last = (int)(end - tile0);
+                for (int base = (int)(part - tile0); base < last; base += groups * U) {
+                    int at[U];
+                    bool live[U];
+                    float n1[U][N], n2[U][N], p[N], q[N];
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+                        const int row = base + group + u * groups;
+                        live[u] = row < last;
+                        at[u] = row * C;
+#pragma unroll
+                        for (int j = 0; j < VPT; ++j) {
+                            RnPack<T, VEC> px = {}, pr = {};
+                            if (live[u] && have[j]) {
+                                rn_load_smem<T, VEC>(px, tx + at[u] + col[j]);
+                                if (a.r) rn_load_smem<T, VEC>(pr, tr + at[u] + col[j]);
+                            }
+                            rn_unpack(px, n1[u] + j * VEC);
+                            rn_unpack(pr, n2[u] + j * VEC);
+                        }
+                    }
+                    if constexpr (!BWD) {
+                        float2 st1[U], st2[U];
+                        rn_normalise<U, N, VEC, false>(n1, st1, have, a.norm1, inv_c, a.eps, lpr, nullptr);
+                        par_all(kW1, p);
+                        par_all(kB1, q);
+#pragma unroll
+                        for (int u = 0; u < U; ++u)
+#pragma unroll
+                            for (int n = 0; n < N; ++n) n1[u][n] = n1[u][n] * p[n] + q[n];
+                        par_all(kG, p);
+#pragma unroll
+                        for (int u = 0; u < U; ++u) {
+#pragma unroll
+                            for (int n = 0; n < N; ++n)
+                                n2[u][n] = have[n / VEC] ? a.alpha * n2[u][n] + p[n] * n1[u][n] : 0.f;
+#pragma unroll
+                            for (int j = 0; j < VPT; ++j)
+                                if (live[u] && have[j]) rn_store_smem<T, VEC>(tx + at[u] + col[j], n2[u] + j * VEC);
+                        }
+                        rn_normalise<U, N, VEC, false>(n2, st2, have, a.norm2, inv_c, a.eps, lpr, nullptr);
+                        if (a.norm2 != SPCONV_NORM_NONE) {
+                            par_all(kW2, p);
+                            par_all(kB2, q);
+#pragma unroll
+                            for (int u = 0; u < U; ++u) {
+#pragma unroll
+                                for (int n = 0; n < N; ++n) n2[u][n] = n2[u][n] * p[n] + q[n];
+#pragma unroll
+                                for (int j = 0; j < VPT; ++j)
+                                    if (live[u] && have[j]) rn_store_smem<T, VEC>(tr + at[u] + col[j], n2[u] + j * VEC);
+                            }
+                        }
+                        if (a.stats && lane == 0) {
+#pragma unroll
+                            for (int u = 0; u < U; ++u)
+                                if (live[u])
+                                    ts[base + group + u * groups] = make_float4(st1[u].x, st1[u].y, st2[u].x, st2[u].y);
+                        }
+                    } else {
+                        float g[U][N], t2[U][N], rstd1[U], rstd2[U], mean2[U];
+#pragma unroll
+                        for (int u = 0; u < U; ++u) {
+                            const float4 st = live[u] ? ts[base + group + u * groups] : make_float4(0.f, 0.f, 0.f, 0.f);
+                            rstd1[u] = st.y;
+                            mean2[u] = st.z;
+                            rstd2[u] = st.w;
+#pragma unroll
+                            for (int n = 0; n < N; ++n) n1[u][n] = (n1[u][n] - st.x) * st.y;
+#pragma unroll
+                            for (int j = 0; j < VPT; ++j) {
+                                RnPack<T, VEC> ph = {}, py = {};
+                                if (live[u] && have[j]) {
+                                    if (a.dh) rn_load_smem<T, VEC>(ph, th + at[u] + col[j]);
+                                    if (a.dy) rn_load_smem<T, VEC>(py, ty + at[u] + col[j]);
+                                }
+                                rn_unpack(ph, g[u] + j * VEC);
+                                rn_unpack(py, t2[u] + j * VEC);
+                            }
+                        }
+                        // dh and dy are zero in rows past the end and in columns a lane does not have, so
+                        // those add nothing to any sum
+                        if (a.norm2 != SPCONV_NORM_NONE && a.dy) {
+                            par_all(kW1, p);
+                            par_all(kB1, q);
+                            float pg[N];
+                            par_all(kG, pg);
+#pragma unroll
+                            for (int u = 0; u < U; ++u)
+#pragma unroll
+                                for (int n = 0; n < N; ++n)
+                                    n2[u][n] = (a.alpha * n2[u][n] + pg[n] * (n1[u][n] * p[n] + q[n]) - mean2[u]) * rstd2[u];
+                            par_all(kW2, p);
+#pragma unroll
+                            for (int u = 0; u < U; ++u)
+#pragma unroll
+                                for (int n = 0; n < N; ++n) {
+                                    acc[kB2][n] += t2[u][n];
+                                    acc[kW2][n] = fmaf(t2[u][n], n2[u][n], acc[kW2][n]);
+                                    t2[u][n] *= p[n];
+                                }
+                            rn_normalise_back<U, N, false>(t2, n2, rstd2, a.norm2, inv_c, lpr, nullptr);
+#pragma unroll
+                            for (int u = 0; u < U; ++u)
+#pragma unroll
+                                for (int n = 0; n < N; ++n) g[u][n] = have[n / VEC] && live[u] ? g[u][n] + t2[u][n] : 0.f;
+                        }
+                        if (a.dr) {
+#pragma unroll
+                            for (int u = 0; u < U; ++u) {
+#pragma unroll
+                                for (int n = 0; n < N; ++n) t2[u][n] = a.alpha * g[u][n];
+#pragma unroll
+                                for (int j = 0; j < VPT; ++j)
+                                    if (live[u] && have[j]) rn_store_smem<T, VEC>(tr + at[u] + col[j], t2[u] + j * VEC);
+                            }
+                        }
+                        par_all(kW1, p);
+                        par_all(kB1, q);
+#pragma unroll
+                        for (int u = 0; u < U; ++u)
+#pragma unroll
+                            for (int n = 0; n < N; ++n)
+                                acc[kG][n] = fmaf(g[u][n], n1[u][n] * p[n] + q[n], acc[kG][n]);
+                        par_all(kG, q);
+#pragma unroll
+                        for (int u = 0; u < U; ++u)
+#pragma unroll
+                            for (int n = 0; n < N; ++n) {
+                                g[u][n] *= q[n];
+                                acc[kB1][n] += g[u][n];
+                                acc[kW1][n] = fmaf(g[u][n], n1[u][n], acc[kW1][n]);
+                                g[u][n] *= p[n];
+                            }
+                        if (a.dx) {
+                            rn_normalise_back<U, N, false>(g, n1, rstd1, a.norm1, inv_c, lpr, nullptr);
+#pragma unroll
+                            for (int u = 0; u < U; ++u)
+#pragma unroll
+                                for (int j = 0; j < VPT; ++j)
+                                    if (live[u] && have[j]) rn_store_smem<T, VEC>(tx + at[u] + col[j], g[u] + j * VEC);
+                        }
+                    }
+                }
+                part = end;
+            }
+            if (!ok) break;
+            fence_proxy_async_smem();
+            __syncwarp();
+            if ((tid & 31) == 0) mbar_arrive(smem_u32(&done[s]));
+            if (++s == S) {
+                s = 0;
+                phase ^= 1u;
+            }
+        }
+        if (BWD && ok) turn(smp, -1);
+    }
+    __syncthreads();
+    if (*s_abort && tid == 0) raise_status(a.status, SPCONV_STATUS_WAIT_TIMEOUT);
 }
 
 struct RnGradArgs {
@@ -628,20 +1106,57 @@ static int rn_launch(RnArgs &a, bool backward, cudaStream_t st) {
     return check_launch("residual_norm_bwd_kernel");
 }
 
+// The bulk form: C <= 256 (a lane's parameters and sums stay in registers), tensors on 16-byte
+// boundaries, and at least two tiles per SM, or its ring never fills: below that the direct kernel
+// spreads the rows over more blocks.
+template <typename T, int VEC, int VPT>
+static bool rb_launch(RnArgs &a, bool backward, cudaStream_t st, int &rc) {
+    const int row_bytes = a.C * (int)sizeof(T), groups = kRbWarps * 32 / a.lpr;
+    const int unit = groups % 8 == 0 ? groups : groups % 4 == 0 ? groups * 2 : groups * 8;   // whole passes, 16-byte tiles
+    RbArgs rb = {};
+    rb.rows = unit * std::max(1, kRbTileBytes / (row_bytes * unit));
+    const int64_t tiles = (a.M + rb.rows - 1) / rb.rows;
+    if (tiles < 2 * 148) return false;
+    rb.tile_bytes = (rb.rows * row_bytes + 127) & ~127;
+    rb.cols = a.lpr * VPT * VEC;
+    const int extra = 256 + (kRnParams * rb.cols + (backward ? kRbWarps * a.nslots * a.C : 0)) * (int)sizeof(float);
+    const int stage = (backward ? 4 : 2) * rb.tile_bytes + rb.rows * 16;
+    rb.stages = std::min(kRbMaxStages, (kRbMaxSmem - extra) / stage);
+    if (rb.stages < 2) return false;
+    rb.wait_ns = wait_limit_ns();
+    a.chunk = (tiles + 147) / 148 * rb.rows;
+    const int grid = (int)((a.M + a.chunk - 1) / a.chunk);
+    const int smem = extra + rb.stages * stage;
+    auto kern = backward ? residual_norm_bulk_kernel<T, VEC, VPT, true> : residual_norm_bulk_kernel<T, VEC, VPT, false>;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kRbMaxSmem) != cudaSuccess) {
+        rc = check_launch("residual_norm_bulk: set max dynamic shared memory");
+        return true;
+    }
+    kern<<<grid, kRbThreads, smem, st>>>(a, rb);
+    rc = check_launch("residual_norm_bulk_kernel");
+    return true;
+}
+
 // Columns a lane owns: eight neighbours at a time where rows and parameters allow 16-byte
 // accesses, single columns otherwise; the fewest that cover the row with one warp, and a block
 // of eight warps per row beyond 1,024 channels.
 template <typename T>
-static int rn_dispatch(RnArgs &a, bool vec, bool backward, cudaStream_t st) {
+static int rn_dispatch(RnArgs &a, bool vec, bool aligned, bool backward, cudaStream_t st) {
     const int C = a.C;
+    int rc = SPCONV_OK;
+    a.lpr = std::min(32, rn_pow2(vec ? C / 8 : C));
+    if (aligned && C <= 256 &&
+        (vec ? rb_launch<T, 8, 1>(a, backward, st, rc)
+             : C <= 32 ? rb_launch<T, 1, 1>(a, backward, st, rc)
+             : C <= 64 ? rb_launch<T, 1, 2>(a, backward, st, rc)
+             : C <= 128 ? rb_launch<T, 1, 4>(a, backward, st, rc) : rb_launch<T, 1, 8>(a, backward, st, rc)))
+        return rc;
     if (vec) {
-        a.lpr = std::min(32, rn_pow2(C / 8));
         if (C <= 256) return rn_launch<T, 8, 1, false>(a, backward, st);
         if (C <= 512) return rn_launch<T, 8, 2, false>(a, backward, st);
         if (C <= 1024) return rn_launch<T, 8, 4, false>(a, backward, st);
         return rn_launch<T, 8, 4, true>(a, backward, st);
     }
-    a.lpr = std::min(32, rn_pow2(C));
     if (C <= 32) return rn_launch<T, 1, 1, false>(a, backward, st);
     if (C <= 64) return rn_launch<T, 1, 2, false>(a, backward, st);
     if (C <= 128) return rn_launch<T, 1, 4, false>(a, backward, st);
@@ -653,7 +1168,7 @@ static int rn_dispatch(RnArgs &a, bool vec, bool backward, cudaStream_t st) {
 static bool rn_aligned(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
 // Checks the call and fills the kernels' arguments (all but lpr and chunk).
-static int rn_args(const spconv_residual_norm_args *q, RnArgs &a, bool &vec, bool backward) {
+static int rn_args(const spconv_residual_norm_args *q, RnArgs &a, bool &vec, bool &aligned, bool backward) {
     SPCONV_REQUIRE(q != nullptr, SPCONV_ERR_ARG, "null argument block");
     SPCONV_REQUIRE(q->dtype == SPCONV_F32 || q->dtype == SPCONV_F16 || q->dtype == SPCONV_BF16, SPCONV_ERR_ARG,
                    "unsupported dtype code %d", q->dtype);
@@ -681,14 +1196,18 @@ static int rn_args(const spconv_residual_norm_args *q, RnArgs &a, bool &vec, boo
     a.alpha = q->residual_scale;
     a.eps = q->eps;
     a.status = q->status;
+    a.stats = (float4 *)q->row_stats;
+    SPCONV_REQUIRE(rn_aligned(a.stats), SPCONV_ERR_ARG, "row_stats is not 16-byte aligned");
     a.offsets = q->offsets;
     a.B = 1;
     a.nslots = 0;
     a.partial = (float *)q->workspace;
     const spconv_channel_param *ps[kRnParams] = {&q->gate, &q->weight, &q->bias, &q->next_weight, &q->next_bias};
     vec = q->channels % 8 == 0;
+    aligned = true;
     for (const void *p : {a.x, a.r, (const void *)a.h, (const void *)a.y, a.dh, a.dy, (const void *)a.dx, (const void *)a.dr})
-        vec = vec && rn_aligned(p);
+        aligned = aligned && rn_aligned(p);
+    vec = vec && aligned;
     for (int k = 0; k < kRnParams; ++k) {
         const spconv_channel_param &p = *ps[k];
         a.p[k] = p.data;
@@ -728,19 +1247,19 @@ extern "C" int64_t spconv_residual_norm_workspace_bytes(int64_t num_rows, int ch
 
 extern "C" int spconv_residual_norm_forward(const spconv_residual_norm_args *q, void *stream) {
     RnArgs a = {};
-    bool vec = false;
-    const int rc = rn_args(q, a, vec, false);
+    bool vec = false, aligned = false;
+    const int rc = rn_args(q, a, vec, aligned, false);
     if (rc != SPCONV_OK || q->num_rows == 0) return rc;
     SPCONV_REQUIRE(a.h && (a.norm2 == SPCONV_NORM_NONE || a.y), SPCONV_ERR_ARG, "null output pointer");
     return rn_by_type(q->dtype, [&](auto *t) {
-        return rn_dispatch<std::remove_pointer_t<decltype(t)>>(a, vec, false, (cudaStream_t)stream);
+        return rn_dispatch<std::remove_pointer_t<decltype(t)>>(a, vec, aligned, false, (cudaStream_t)stream);
     });
 }
 
 extern "C" int spconv_residual_norm_backward(const spconv_residual_norm_args *q, void *stream) {
     RnArgs a = {};
-    bool vec = false;
-    const int rc = rn_args(q, a, vec, true);
+    bool vec = false, aligned = false;
+    const int rc = rn_args(q, a, vec, aligned, true);
     if (rc != SPCONV_OK) return rc;
     const cudaStream_t st = (cudaStream_t)stream;
     spconv_channel_param ps[kRnParams] = {q->gate, q->weight, q->bias, q->next_weight, q->next_bias};
@@ -756,9 +1275,10 @@ extern "C" int spconv_residual_norm_backward(const spconv_residual_norm_args *q,
                        (a.partial && rn_aligned(a.partial) &&
                         q->workspace_bytes >= spconv_residual_norm_workspace_bytes(q->num_rows, q->channels, a.B)),
                    SPCONV_ERR_ARG, "workspace missing, misaligned or too small");
+    SPCONV_REQUIRE(a.stats, SPCONV_ERR_ARG, "row_stats of the forward are needed");
     return rn_by_type(q->dtype, [&](auto *t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        int e = rn_dispatch<T>(a, vec, true, st);
+        int e = rn_dispatch<T>(a, vec, aligned, true, st);
         if (e != SPCONV_OK || a.nslots == 0) return e;
         RnGradArgs o = {};
         bool per_sample = false;

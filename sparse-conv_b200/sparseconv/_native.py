@@ -51,7 +51,7 @@ class ResidualNormArgs(ctypes.Structure):
     _fields_ = [("dtype", _c_int), ("channels", _c_int), ("num_rows", _c_i64),
                 ("feats", _c_void_p), ("residual", _c_void_p), ("hidden", _c_void_p), ("normed", _c_void_p),
                 ("grad_hidden", _c_void_p), ("grad_normed", _c_void_p),
-                ("grad_feats", _c_void_p), ("grad_residual", _c_void_p),
+                ("grad_feats", _c_void_p), ("grad_residual", _c_void_p), ("row_stats", _c_void_p),
                 ("gate", ChannelParam), ("weight", ChannelParam), ("bias", ChannelParam),
                 ("next_weight", ChannelParam), ("next_bias", ChannelParam),
                 ("offsets", _c_void_p), ("num_samples", _c_int), ("norm", _c_int), ("next_norm", _c_int),
@@ -835,33 +835,35 @@ def _norm_args(feats: torch.Tensor, residual, params, offsets, residual_scale: f
             raise ValueError("batch_offsets must be a contiguous [samples + 1] int32 tensor")
         if per_sample:
             a.offsets, a.num_samples = offsets.data_ptr(), offsets.numel() - 1
-            a.status = mapped_status(dev.index)
+    a.status = mapped_status(dev.index)
     return a
 
 
 @_on_device
 def residual_norm_forward(feats: torch.Tensor, residual: Optional[torch.Tensor], params: Sequence[Optional[torch.Tensor]],
                           offsets: Optional[torch.Tensor], residual_scale: float, norm: str, next_norm: str,
-                          eps: float) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
-    """(hidden, normed) of the gated residual step (normed None without ``next_norm``)."""
+                          eps: float, keep_stats: bool = False
+                          ) -> Tuple[torch.Tensor, Optional[torch.Tensor], Optional[torch.Tensor]]:
+    """(hidden, normed, row statistics if ``keep_stats``) of the gated residual step (normed None
+    without ``next_norm``)."""
     a = _norm_args(feats, residual, params, offsets, residual_scale, norm, next_norm, eps)
     hidden = torch.empty_like(feats)
     normed = torch.empty_like(feats) if next_norm != "none" else None
-    a.hidden, a.normed = hidden.data_ptr(), _ptr(normed)
+    stats = torch.empty((a.num_rows, 4), dtype=torch.float32, device=feats.device) if keep_stats else None
+    a.hidden, a.normed, a.row_stats = hidden.data_ptr(), _ptr(normed), _ptr(stats)
     index = feats.get_device()
     rc = (_lib or load_library()).spconv_residual_norm_forward(a, _raw_stream(index))
     if rc != SPCONV_OK:
         _raise(rc, "spconv_residual_norm_forward")
-    if a.status:
-        after_mapped_launch(index)
-    return hidden, normed
+    after_mapped_launch(index)
+    return hidden, normed, stats
 
 
 @_on_device
 def residual_norm_backward(feats: torch.Tensor, residual: Optional[torch.Tensor], params: Sequence[Optional[torch.Tensor]],
                            offsets: Optional[torch.Tensor], residual_scale: float, norm: str, next_norm: str,
-                           eps: float, grad_hidden: Optional[torch.Tensor], grad_normed: Optional[torch.Tensor],
-                           needs: Sequence[bool]) -> list:
+                           eps: float, stats: torch.Tensor, grad_hidden: Optional[torch.Tensor],
+                           grad_normed: Optional[torch.Tensor], needs: Sequence[bool]) -> list:
     """Gradients of feats, residual, gate, weight, bias, next_weight and next_bias (None where
     ``needs`` says so), each in its tensor's shape and dtype."""
     lib = load_library()
@@ -870,7 +872,7 @@ def residual_norm_backward(feats: torch.Tensor, residual: Optional[torch.Tensor]
         if g is not None:
             _require_cuda(feats, g)
             _matrix(g, feats.shape, feats.dtype, what)
-    a.grad_hidden, a.grad_normed = _ptr(grad_hidden), _ptr(grad_normed)
+    a.grad_hidden, a.grad_normed, a.row_stats = _ptr(grad_hidden), _ptr(grad_normed), stats.data_ptr()
     grads = [torch.empty_like(t) if t is not None and need else None
              for t, need in zip((feats, residual, *params), needs)]
     a.grad_feats, a.grad_residual = _ptr(grads[0]), _ptr(grads[1])
@@ -884,8 +886,7 @@ def residual_norm_backward(feats: torch.Tensor, residual: Optional[torch.Tensor]
     rc = lib.spconv_residual_norm_backward(a, _raw_stream(index))
     if rc != SPCONV_OK:
         _raise(rc, "spconv_residual_norm_backward")
-    if a.status:
-        after_mapped_launch(index)
+    after_mapped_launch(index)
     return grads
 
 

@@ -316,3 +316,36 @@ def test_same_bits_every_run_and_replayed():
     graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(a, c) for a, c in zip(first, held))
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("C", [1, 3, 8, 24, 35, 64, 72, 100, 129, 256])
+def test_enough_rows_for_the_ring(C, dtype):
+    """Millions of values: the streams through shared memory, samples that end inside a tile, a last
+    tile that ends in odd bytes."""
+    e = torch.finfo(DT[dtype]).bits // 8
+    M = 310 * 12288 // (C * e) + 5
+    per = ("gate", "weight", "bias", "next_weight", "next_bias") if C % 3 else ("gate",)
+    _run(M, C, 40, DT[dtype], torch.float32, True, "layer", "layer" if C != 1 else "rms", per_sample=per, seed=C)
+
+
+@pytest.mark.parametrize("norm,next_norm,use", [("none", "none", (True, False)), ("rms", "none", (True, False)),
+                                                ("none", "rms", (False, True)), ("rms", "layer", (True, True))])
+def test_ring_with_parts_absent(norm, next_norm, use):
+    M = 310 * 96 + 7
+    _run(M, 64, 3, torch.bfloat16, torch.bfloat16, False, norm, next_norm, residual=False, use=use, seed=11)
+    _run(M, 64, 3, torch.bfloat16, torch.bfloat16, True, norm, next_norm, alpha=0.5, use=use, seed=12)
+
+
+def test_only_the_wanted_gradients():
+    x, r, p, off, _, dh, dy = _case(310 * 96, 64, 3, torch.bfloat16, torch.float32, True, "layer", "layer", ("gate",), seed=13)
+    named = {"feats": x, "residual": r, **p}
+
+    def grads(wanted):
+        full = {k: t.detach().clone().requires_grad_(k in wanted) for k, t in named.items()}
+        o = sparse_residual_norm(full["feats"], full["residual"], batch_offsets=off, norm="layer", next_norm="layer",
+                                 **{k: full[k] for k in p})
+        return torch.autograd.grad(o, [full[k] for k in wanted], [dh, dy])
+    every = dict(zip(named, grads(list(named))))
+    for k in named:
+        assert torch.equal(grads([k])[0], every[k]), k
