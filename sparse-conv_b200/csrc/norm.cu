@@ -19,14 +19,11 @@
 // statistics too would save those 16 bytes a row and cost two more reductions over the row, which
 // are what bounds the backward after HBM.
 //
-// LayerNorm's statistics take one reduction, of the sums of d and d^2, d = t - t[0]: any value of
-// the row lies within sqrt(C) deviations of its mean, so mean(d^2) - mean(d)^2 loses at most a
-// factor C of the variance's digits whatever offset the row has in common.
-//
 // Bound: HBM. Forward reads x, r and writes h, y; backward reads x, r, dh, dy and writes dx, dr.
 // All arithmetic is fp32; each output is rounded once. A row lives in the registers of the
 // lanes that own it, so every tensor is read once.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -38,6 +35,8 @@ constexpr int kRnMaxC = 8192;
 constexpr int kRnMaxSamples = 65535;   // a grid dimension of the gradient sums
 // parameter slots, and the order of their partial sums
 enum { kG = 0, kW1 = 1, kB1 = 2, kW2 = 3, kB2 = 4, kRnParams = 5 };
+// products the ring kernel keeps beside them: g * w1 and g * b1
+enum { kGW = 5, kGB = 6, kRbParams = 7 };
 
 struct RnArgs {
     const void *x, *r;                   // r may be null
@@ -208,8 +207,8 @@ __device__ __forceinline__ float rn_dot(const float (&t)[N], const float (&n)[N]
 }
 
 // Normalises U rows, N values of each in a lane, in place: (mean, rstd) of each row in st. Columns
-// that a lane does not have hold zeros, before and after.
-template <int U, int N, int VEC, bool BLOCK>
+// that a lane does not have hold zeros, before and after (FULL: it has them all).
+template <int U, int N, int VEC, bool BLOCK, bool FULL>
 __device__ __forceinline__ void rn_normalise(float (&t)[U][N], float2 (&st)[U], const bool *have, int kind, float inv_c,
                                              float eps, int lpr, float2 *scratch) {
     if (kind == SPCONV_NORM_NONE) {
@@ -217,43 +216,65 @@ __device__ __forceinline__ void rn_normalise(float (&t)[U][N], float2 (&st)[U], 
         for (int u = 0; u < U; ++u) st[u] = make_float2(0.f, 1.f);
         return;
     }
-    float s[U], q[U], first[U];
+    // Eight columns a lane: one reduction, of d and d^2 for d = t - c, c the mean of the row's first
+    // eight values, which lies within sqrt(C / 8) deviations of the row's mean: mean(d^2) - mean(d)^2
+    // then costs at most the factor C / 8 + 1 in the variance's rounding, whatever offset the row has
+    // in common. Single columns a lane, or a block a row: the mean first, then the squares.
+    constexpr bool ONE = VEC == 8 && !BLOCK;
+    float s[U], q[U], shift[U];
     const bool layer = kind == SPCONV_NORM_LAYER;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        first[u] = 0.f;
-        s[u] = 0.f;
+        shift[u] = s[u] = q[u] = 0.f;
         if (layer) {
-            if constexpr (BLOCK) {
-                __syncthreads();
-                if (threadIdx.x == 0) scratch[0].x = t[u][0];
-                __syncthreads();
-                first[u] = scratch[0].x;
-            } else {
-                first[u] = __shfl_sync(0xffffffffu, t[u][0], 0, lpr);
-            }
+            if constexpr (ONE) {
+                float head[8];
 #pragma unroll
-            for (int i = 0; i < N; ++i) t[u][i] = have[i / VEC] ? t[u][i] - first[u] : 0.f;
-            s[u] = rn_tree<N>(t[u]);
+                for (int i = 0; i < 8; ++i) head[i] = t[u][i];
+                shift[u] = __shfl_sync(0xffffffffu, rn_tree<8>(head) * 0.125f, 0, lpr);
+            } else {
+                s[u] = rn_tree<N>(t[u]);
+            }
+        }
+    }
+    if (!ONE && layer) {
+        rn_sum2<U, BLOCK>(s, q, true, lpr, scratch);
+#pragma unroll
+        for (int u = 0; u < U; ++u) shift[u] = s[u] * inv_c;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        if (layer) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) t[u][i] = FULL || have[i / VEC] ? t[u][i] - shift[u] : 0.f;
+            s[u] = ONE ? rn_tree<N>(t[u]) : 0.f;
         }
         q[u] = rn_dot<N>(t[u], t[u]);
     }
-    rn_sum2<U, BLOCK>(s, q, layer, lpr, scratch);
+    rn_sum2<U, BLOCK>(s, q, layer && ONE, lpr, scratch);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        const float m = layer ? s[u] * inv_c : 0.f;
+        const float m = layer && ONE ? s[u] * inv_c : 0.f;
         const float var = q[u] * inv_c - m * m;
-        st[u] = make_float2(first[u] + m, rsqrtf((var < 0.f ? 0.f : var) + eps));     // NaN stays NaN
+        const float rstd = rsqrtf((var < 0.f ? 0.f : var) + eps);            // NaN stays NaN
+        st[u] = make_float2(shift[u] + m, rstd);
+        const float offset = -m * rstd;
 #pragma unroll
-        for (int i = 0; i < N; ++i) t[u][i] = have[i / VEC] ? (t[u][i] - m) * st[u].y : 0.f;
+        for (int i = 0; i < N; ++i) t[u][i] = FULL || have[i / VEC] ? fmaf(t[u][i], rstd, offset) : 0.f;
     }
 }
 
-// t: gradient at the normalised values n -> gradient at the values before the norm.
+// t: gradient at the normalised values n -> gradient at the values before the norm, added to g.
 template <int U, int N, bool BLOCK>
-__device__ __forceinline__ void rn_normalise_back(float (&t)[U][N], const float (&n)[U][N], const float (&rstd)[U],
-                                                  int kind, float inv_c, int lpr, float2 *scratch) {
-    if (kind == SPCONV_NORM_NONE) return;
+__device__ __forceinline__ void rn_normalise_back(float (&g)[U][N], float (&t)[U][N], const float (&n)[U][N],
+                                                  const float (&rstd)[U], int kind, float inv_c, int lpr, float2 *scratch) {
+    if (kind == SPCONV_NORM_NONE) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int i = 0; i < N; ++i) g[u][i] += t[u][i];
+        return;
+    }
     float s[U], q[U];
     const bool layer = kind == SPCONV_NORM_LAYER;
 #pragma unroll
@@ -266,7 +287,7 @@ __device__ __forceinline__ void rn_normalise_back(float (&t)[U][N], const float 
     for (int u = 0; u < U; ++u) {
         const float mean = layer ? s[u] * inv_c * rstd[u] : 0.f, along = q[u] * inv_c * rstd[u];
 #pragma unroll
-        for (int i = 0; i < N; ++i) t[u][i] = fmaf(t[u][i], rstd[u], fmaf(-n[u][i], along, -mean));
+        for (int i = 0; i < N; ++i) g[u][i] = fmaf(t[u][i], rstd[u], fmaf(-n[u][i], along, g[u][i] - mean));
     }
 }
 
@@ -355,7 +376,7 @@ residual_norm_fwd_kernel(const __grid_constant__ RnArgs a) {
             }
             fetch(row + groups);             // the next row's loads run under this row's sums
             float2 st1[1], st2[1] = {make_float2(0.f, 1.f)};
-            rn_normalise<1, N, VEC, BLOCK>(uu, st1, have, a.norm1, inv_c, a.eps, lpr, scratch);
+            rn_normalise<1, N, VEC, BLOCK, false>(uu, st1, have, a.norm1, inv_c, a.eps, lpr, scratch);
 #pragma unroll
             for (int j = 0; j < VPT; ++j) {
                 float g[VEC], w[VEC], b[VEC];
@@ -374,7 +395,7 @@ residual_norm_fwd_kernel(const __grid_constant__ RnArgs a) {
                 if (have[j] && row < end) rn_store((T *)a.h + row * C + col[j], h + j * VEC, (RnPack<T, VEC> *)nullptr);
             }
             if (a.norm2 != SPCONV_NORM_NONE) {
-                rn_normalise<1, N, VEC, BLOCK>(hh, st2, have, a.norm2, inv_c, a.eps, lpr, scratch);
+                rn_normalise<1, N, VEC, BLOCK, false>(hh, st2, have, a.norm2, inv_c, a.eps, lpr, scratch);
 #pragma unroll
                 for (int j = 0; j < VPT; ++j) {
                     float w[VEC], b[VEC];
@@ -539,9 +560,7 @@ residual_norm_bwd_kernel(const __grid_constant__ RnArgs a) {
                     }
                     if (live) add(kW2, j, v);
                 }
-                rn_normalise_back<1, N, BLOCK>(t_, n2_, rstd2, a.norm2, inv_c, lpr, scratch);
-#pragma unroll
-                for (int n = 0; n < N; ++n) gr[n] += t[n];
+                rn_normalise_back<1, N, BLOCK>(gr_, t_, n2_, rstd2, a.norm2, inv_c, lpr, scratch);
             }
 #pragma unroll
             for (int j = 0; j < VPT; ++j) {
@@ -575,10 +594,12 @@ residual_norm_bwd_kernel(const __grid_constant__ RnArgs a) {
                 if (live) add(kW1, j, v);
             }
             if (a.dx) {
-                rn_normalise_back<1, N, BLOCK>(gr_, n1_, rstd1, a.norm1, inv_c, lpr, scratch);
+#pragma unroll
+                for (int n = 0; n < N; ++n) t[n] = 0.f;
+                rn_normalise_back<1, N, BLOCK>(t_, gr_, n1_, rstd1, a.norm1, inv_c, lpr, scratch);
 #pragma unroll
                 for (int j = 0; j < VPT; ++j)
-                    if (have[j] && live) rn_store((T *)a.dx + row * C + col[j], gr + j * VEC, (RnPack<T, VEC> *)nullptr);
+                    if (have[j] && live) rn_store((T *)a.dx + row * C + col[j], t + j * VEC, (RnPack<T, VEC> *)nullptr);
             }
         }
         if (a.nslots > 0) {
@@ -673,12 +694,13 @@ __device__ __forceinline__ void bulk_store(void *dst, uint32_t src, uint32_t byt
     asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;\n" :: "l"(dst), "r"(src), "r"(bytes) : "memory");
 }
 
-template <typename T, int VEC, int VPT, bool BWD>
+template <typename T, int VEC, int VPT, bool BWD, bool FULL>
 __global__ void __launch_bounds__(kRbThreads, 1)
 residual_norm_bulk_kernel(const __grid_constant__ RnArgs a, const __grid_constant__ RbArgs rb) {
     constexpr int N = VEC * VPT;
-    constexpr int U = N >= 4 ? 2 : 4;        // rows a lane works on at once: their sums overlap
-    static_assert(N <= 8, "a lane's sums stay in registers");
+    constexpr int U = N >= 16 ? 1 : N >= 4 ? 2 : 4;           // rows a lane works on at once: their sums overlap
+    constexpr int kSums = 4;                 // of G, G * xhat, dy, dy * hhat
+    static_assert(!BWD || N <= 8, "a lane's sums stay in registers");
     constexpr int kTensors = BWD ? 4 : 2;    // slots of a stage: x (then h or dx), r (then y or dr), dh, dy
     extern __shared__ __align__(128) uint8_t s_raw[];
     uint64_t *full = reinterpret_cast<uint64_t *>(s_raw), *done = full + kRbMaxStages, *flush = done + kRbMaxStages;
@@ -686,8 +708,8 @@ residual_norm_bulk_kernel(const __grid_constant__ RnArgs a, const __grid_constan
     uint8_t *ring = s_raw + 256;
     const int S = rb.stages, R = rb.rows, C = a.C, lpr = a.lpr;
     const int slot = rb.tile_bytes, stage = kTensors * slot + R * 16;          // the rows' statistics last
-    float *s_par = reinterpret_cast<float *>(ring + S * stage);                // [kRnParams][rb.cols]
-    float *s_acc = s_par + kRnParams * rb.cols;                                // [kRbWarps][nslots][C]
+    float *s_par = reinterpret_cast<float *>(ring + S * stage);                // [kRbParams][rb.cols]
+    float *s_acc = s_par + kRbParams * rb.cols;                                // [kRbWarps][nslots][C]
     const int tid = threadIdx.x, warp = tid >> 5;
     if (tid == 0) {
         for (int i = 0; i < S; ++i) {
@@ -773,9 +795,9 @@ residual_norm_bulk_kernel(const __grid_constant__ RnArgs a, const __grid_constan
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
             col[j] = (lane + lpr * j) * VEC;
-            have[j] = col[j] < C;
+            have[j] = FULL || col[j] < C;
         }
-        float acc[kRnParams][BWD ? N : 1] = {};
+        float acc[kSums][BWD ? N : 1] = {};
         uint32_t flush_phase = 0;
         // All row warps: an mbarrier rather than bar.sync, since its wait is bounded.
         auto meet = [&]() {
@@ -790,20 +812,28 @@ residual_norm_bulk_kernel(const __grid_constant__ RnArgs a, const __grid_constan
         auto turn = [&](int from, int to) -> bool {
             if constexpr (BWD) {
                 if (from >= 0) {
+                    // G's sums give the gate's, weight's and bias's: u = xhat * w1 + b1 and du = G * g with
+                    // w1, b1 and g the same for all of a sample's rows
                     float *mine = s_acc + (int64_t)warp * a.nslots * C;
 #pragma unroll
-                    for (int k = 0; k < kRnParams; ++k) {
-                        if (a.slot[k] < 0) continue;
+                    for (int k = 0; k < kSums; ++k)
 #pragma unroll
                         for (int i = 0; i < N; ++i)
                             for (int o = lpr; o < 32; o <<= 1) acc[k][i] += __shfl_xor_sync(0xffffffffu, acc[k][i], o);
-                        if ((tid & 31) < lpr) {
+                    if ((tid & 31) < lpr) {
 #pragma unroll
-                            for (int j = 0; j < VPT; ++j)
-                                if (have[j])
+                        for (int j = 0; j < VPT; ++j)
+                            if (have[j])
 #pragma unroll
-                                    for (int i = 0; i < VEC; ++i) mine[a.slot[k] * C + col[j] + i] = acc[k][j * VEC + i];
-                        }
+                                for (int i = 0; i < VEC; ++i) {
+                                    const int c = col[j] + i, n = j * VEC + i;
+                                    const float g = s_par[kG * rb.cols + c], w = s_par[kW1 * rb.cols + c], b = s_par[kB1 * rb.cols + c];
+                                    if (a.slot[kG] >= 0) mine[a.slot[kG] * C + c] = w * acc[1][n] + b * acc[0][n];
+                                    if (a.slot[kW1] >= 0) mine[a.slot[kW1] * C + c] = g * acc[1][n];
+                                    if (a.slot[kB1] >= 0) mine[a.slot[kB1] * C + c] = g * acc[0][n];
+                                    if (a.slot[kB2] >= 0) mine[a.slot[kB2] * C + c] = acc[2][n];
+                                    if (a.slot[kW2] >= 0) mine[a.slot[kW2] * C + c] = acc[3][n];
+                                }
                     }
                 }
             }
@@ -819,17 +849,21 @@ residual_norm_bulk_kernel(const __grid_constant__ RnArgs a, const __grid_constan
                         rec[i] = v;
                     }
 #pragma unroll
-                    for (int k = 0; k < kRnParams; ++k)
+                    for (int k = 0; k < kSums; ++k)
 #pragma unroll
                         for (int i = 0; i < N; ++i) acc[k][i] = 0.f;
                 }
             }
             if (to >= 0)
-                for (int i = tid; i < kRnParams * rb.cols; i += kRbWarps * 32) {
-                    const int k = i / rb.cols, c = i - k * rb.cols;
-                    float v[1];
-                    rn_param<T, 1>(a, k, to, c < C ? c : 0, v);
-                    s_par[i] = v[0];
+                for (int c = tid; c < rb.cols; c += kRbWarps * 32) {
+                    float v[kRnParams][1];
+#pragma unroll
+                    for (int k = 0; k < kRnParams; ++k) {
+                        rn_param<T, 1>(a, k, to, c < C ? c : 0, v[k]);
+                        s_par[k * rb.cols + c] = v[k][0];
+                    }
+                    s_par[kGW * rb.cols + c] = v[kG][0] * v[kW1][0];
+                    s_par[kGB * rb.cols + c] = v[kG][0] * v[kB1][0];
                 }
             return meet();
         };
@@ -863,6 +897,138 @@ residual_norm_bulk_kernel(const __grid_constant__ RnArgs a, const __grid_constan
             const T *th = reinterpret_cast<const T *>(base_s + (BWD ? 2 * slot : 0));
             const T *ty = reinterpret_cast<const T *>(base_s + (BWD ? 3 * slot : 0));
             float4 *ts = reinterpret_cast<float4 *>(base_s + kTensors * slot);
+            // U rows a group, from `base` of the tile on; TAIL: some of them may be past `last`
+            auto rows = [&](auto tail, int base, int last) {
+                constexpr bool TAIL = decltype(tail)::value;
+                int at[U];
+                bool live[U];
+                float n1[U][N], n2[U][N], p[N], q[N];
+                auto read = [&](int u, const T *src, float *f) {
+#pragma unroll
+                    for (int j = 0; j < VPT; ++j) {
+                        RnPack<T, VEC> v;
+                        if constexpr (!TAIL && FULL) {
+                            rn_load_smem<T, VEC>(v, src + at[u] + col[j]);
+                        } else {
+                            v = RnPack<T, VEC>{};
+                            if (live[u] && have[j]) rn_load_smem<T, VEC>(v, src + at[u] + col[j]);
+                        }
+                        rn_unpack(v, f + j * VEC);
+                    }
+                };
+                auto write = [&](int u, T *dst, const float *f) {
+#pragma unroll
+                    for (int j = 0; j < VPT; ++j)
+                        if ((!TAIL || live[u]) && have[j]) rn_store_smem<T, VEC>(dst + at[u] + col[j], f + j * VEC);
+                };
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int row = base + group + u * groups;
+                    live[u] = !TAIL || row < last;
+                    at[u] = row * C;
+                    read(u, tx, n1[u]);
+                    if (a.r) read(u, tr, n2[u]);
+                    else
+#pragma unroll
+                        for (int n = 0; n < N; ++n) n2[u][n] = 0.f;
+                }
+                // xhat in n1 -> h in n2 (zero in columns a lane does not have)
+                auto hidden = [&]() {
+                    par_all(kGW, p);
+                    par_all(kGB, q);
+#pragma unroll
+                    for (int u = 0; u < U; ++u)
+#pragma unroll
+                        for (int n = 0; n < N; ++n)
+                            n2[u][n] = have[n / VEC] ? fmaf(n1[u][n], p[n], fmaf(a.alpha, n2[u][n], q[n])) : 0.f;
+                };
+                if constexpr (!BWD) {
+                    float2 st1[U], st2[U];
+                    rn_normalise<U, N, VEC, false, FULL>(n1, st1, have, a.norm1, inv_c, a.eps, lpr, nullptr);
+                    hidden();
+#pragma unroll
+                    for (int u = 0; u < U; ++u) write(u, tx, n2[u]);
+                    rn_normalise<U, N, VEC, false, FULL>(n2, st2, have, a.norm2, inv_c, a.eps, lpr, nullptr);
+                    if (a.norm2 != SPCONV_NORM_NONE) {
+                        par_all(kW2, p);
+                        par_all(kB2, q);
+#pragma unroll
+                        for (int u = 0; u < U; ++u) {
+#pragma unroll
+                            for (int n = 0; n < N; ++n) n2[u][n] = fmaf(n2[u][n], p[n], q[n]);
+                            write(u, tr, n2[u]);
+                        }
+                    }
+                    if (a.stats && lane == 0) {
+#pragma unroll
+                        for (int u = 0; u < U; ++u)
+                            if (live[u]) ts[base + group + u * groups] = make_float4(st1[u].x, st1[u].y, st2[u].x, st2[u].y);
+                    }
+                } else {
+                    float g[U][N], t2[U][N], rstd1[U], rstd2[U], shift2[U];
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+                        const float4 st = live[u] ? ts[base + group + u * groups] : make_float4(0.f, 0.f, 0.f, 0.f);
+                        rstd1[u] = st.y;
+                        rstd2[u] = st.w;
+                        shift2[u] = -st.z * st.w;
+                        const float shift1 = -st.x * st.y;
+#pragma unroll
+                        for (int n = 0; n < N; ++n) n1[u][n] = fmaf(n1[u][n], st.y, shift1);
+                        if (a.dh) read(u, th, g[u]);
+                        else
+#pragma unroll
+                            for (int n = 0; n < N; ++n) g[u][n] = 0.f;
+                    }
+                    // dh and dy are zero in rows past the end and in columns a lane does not have, so
+                    // those add nothing to any sum
+                    if (a.norm2 != SPCONV_NORM_NONE && a.dy) {
+                        hidden();
+                        par_all(kW2, p);
+#pragma unroll
+                        for (int u = 0; u < U; ++u) {
+                            read(u, ty, t2[u]);
+#pragma unroll
+                            for (int n = 0; n < N; ++n) {
+                                n2[u][n] = fmaf(n2[u][n], rstd2[u], shift2[u]);
+                                acc[2][n] += t2[u][n];
+                                acc[3][n] = fmaf(t2[u][n], n2[u][n], acc[3][n]);
+                                t2[u][n] *= p[n];
+                            }
+                        }
+                        rn_normalise_back<U, N, false>(g, t2, n2, rstd2, a.norm2, inv_c, lpr, nullptr);
+                        if constexpr (TAIL || !FULL) {
+#pragma unroll
+                            for (int u = 0; u < U; ++u)
+#pragma unroll
+                                for (int n = 0; n < N; ++n) g[u][n] = have[n / VEC] && live[u] ? g[u][n] : 0.f;
+                        }
+                    }
+                    if (a.dr) {
+#pragma unroll
+                        for (int u = 0; u < U; ++u) {
+#pragma unroll
+                            for (int n = 0; n < N; ++n) t2[u][n] = a.alpha * g[u][n];
+                            write(u, tr, t2[u]);
+                        }
+                    }
+                    par_all(kGW, p);
+#pragma unroll
+                    for (int u = 0; u < U; ++u)
+#pragma unroll
+                        for (int n = 0; n < N; ++n) {
+                            acc[0][n] += g[u][n];
+                            acc[1][n] = fmaf(g[u][n], n1[u][n], acc[1][n]);
+                            g[u][n] *= p[n];
+                            t2[u][n] = 0.f;
+                        }
+                    if (a.dx) {
+                        rn_normalise_back<U, N, false>(t2, g, n1, rstd1, a.norm1, inv_c, lpr, nullptr);
+#pragma unroll
+                        for (int u = 0; u < U; ++u) write(u, tx, t2[u]);
+                    }
+                }
+            };
             for (int64_t part = tile0; part < tile1;) {
                 if (s_end <= part) {         // the next sample that has rows (the last one takes the rest)
                     const int from = smp;
@@ -872,149 +1038,9 @@ residual_norm_bulk_kernel(const __grid_constant__ RnArgs a, const __grid_constan
                 }
                 const int64_t end = min(tile1, s_end);
                 const int last = (int)(end - tile0);
-                for (int base = (int)(part - tile0); base < last; base += groups * U) {
-                    int at[U];
-                    bool live[U];
-                    float n1[U][N], n2[U][N], p[N], q[N];
-#pragma unroll
-                    for (int u = 0; u < U; ++u) {
-                        const int row = base + group + u * groups;
-                        live[u] = row < last;
-                        at[u] = row * C;
-#pragma unroll
-                        for (int j = 0; j < VPT; ++j) {
-                            RnPack<T, VEC> px = {}, pr = {};
-                            if (live[u] && have[j]) {
-                                rn_load_smem<T, VEC>(px, tx + at[u] + col[j]);
-                                if (a.r) rn_load_smem<T, VEC>(pr, tr + at[u] + col[j]);
-                            }
-                            rn_unpack(px, n1[u] + j * VEC);
-                            rn_unpack(pr, n2[u] + j * VEC);
-                        }
-                    }
-                    if constexpr (!BWD) {
-                        float2 st1[U], st2[U];
-                        rn_normalise<U, N, VEC, false>(n1, st1, have, a.norm1, inv_c, a.eps, lpr, nullptr);
-                        par_all(kW1, p);
-                        par_all(kB1, q);
-#pragma unroll
-                        for (int u = 0; u < U; ++u)
-#pragma unroll
-                            for (int n = 0; n < N; ++n) n1[u][n] = n1[u][n] * p[n] + q[n];
-                        par_all(kG, p);
-#pragma unroll
-                        for (int u = 0; u < U; ++u) {
-#pragma unroll
-                            for (int n = 0; n < N; ++n)
-                                n2[u][n] = have[n / VEC] ? a.alpha * n2[u][n] + p[n] * n1[u][n] : 0.f;
-#pragma unroll
-                            for (int j = 0; j < VPT; ++j)
-                                if (live[u] && have[j]) rn_store_smem<T, VEC>(tx + at[u] + col[j], n2[u] + j * VEC);
-                        }
-                        rn_normalise<U, N, VEC, false>(n2, st2, have, a.norm2, inv_c, a.eps, lpr, nullptr);
-                        if (a.norm2 != SPCONV_NORM_NONE) {
-                            par_all(kW2, p);
-                            par_all(kB2, q);
-#pragma unroll
-                            for (int u = 0; u < U; ++u) {
-#pragma unroll
-                                for (int n = 0; n < N; ++n) n2[u][n] = n2[u][n] * p[n] + q[n];
-#pragma unroll
-                                for (int j = 0; j < VPT; ++j)
-                                    if (live[u] && have[j]) rn_store_smem<T, VEC>(tr + at[u] + col[j], n2[u] + j * VEC);
-                            }
-                        }
-                        if (a.stats && lane == 0) {
-#pragma unroll
-                            for (int u = 0; u < U; ++u)
-                                if (live[u])
-                                    ts[base + group + u * groups] = make_float4(st1[u].x, st1[u].y, st2[u].x, st2[u].y);
-                        }
-                    } else {
-                        float g[U][N], t2[U][N], rstd1[U], rstd2[U], mean2[U];
-#pragma unroll
-                        for (int u = 0; u < U; ++u) {
-                            const float4 st = live[u] ? ts[base + group + u * groups] : make_float4(0.f, 0.f, 0.f, 0.f);
-                            rstd1[u] = st.y;
-                            mean2[u] = st.z;
-                            rstd2[u] = st.w;
-#pragma unroll
-                            for (int n = 0; n < N; ++n) n1[u][n] = (n1[u][n] - st.x) * st.y;
-#pragma unroll
-                            for (int j = 0; j < VPT; ++j) {
-                                RnPack<T, VEC> ph = {}, py = {};
-                                if (live[u] && have[j]) {
-                                    if (a.dh) rn_load_smem<T, VEC>(ph, th + at[u] + col[j]);
-                                    if (a.dy) rn_load_smem<T, VEC>(py, ty + at[u] + col[j]);
-                                }
-                                rn_unpack(ph, g[u] + j * VEC);
-                                rn_unpack(py, t2[u] + j * VEC);
-                            }
-                        }
-                        // dh and dy are zero in rows past the end and in columns a lane does not have, so
-                        // those add nothing to any sum
-                        if (a.norm2 != SPCONV_NORM_NONE && a.dy) {
-                            par_all(kW1, p);
-                            par_all(kB1, q);
-                            float pg[N];
-                            par_all(kG, pg);
-#pragma unroll
-                            for (int u = 0; u < U; ++u)
-#pragma unroll
-                                for (int n = 0; n < N; ++n)
-                                    n2[u][n] = (a.alpha * n2[u][n] + pg[n] * (n1[u][n] * p[n] + q[n]) - mean2[u]) * rstd2[u];
-                            par_all(kW2, p);
-#pragma unroll
-                            for (int u = 0; u < U; ++u)
-#pragma unroll
-                                for (int n = 0; n < N; ++n) {
-                                    acc[kB2][n] += t2[u][n];
-                                    acc[kW2][n] = fmaf(t2[u][n], n2[u][n], acc[kW2][n]);
-                                    t2[u][n] *= p[n];
-                                }
-                            rn_normalise_back<U, N, false>(t2, n2, rstd2, a.norm2, inv_c, lpr, nullptr);
-#pragma unroll
-                            for (int u = 0; u < U; ++u)
-#pragma unroll
-                                for (int n = 0; n < N; ++n) g[u][n] = have[n / VEC] && live[u] ? g[u][n] + t2[u][n] : 0.f;
-                        }
-                        if (a.dr) {
-#pragma unroll
-                            for (int u = 0; u < U; ++u) {
-#pragma unroll
-                                for (int n = 0; n < N; ++n) t2[u][n] = a.alpha * g[u][n];
-#pragma unroll
-                                for (int j = 0; j < VPT; ++j)
-                                    if (live[u] && have[j]) rn_store_smem<T, VEC>(tr + at[u] + col[j], t2[u] + j * VEC);
-                            }
-                        }
-                        par_all(kW1, p);
-                        par_all(kB1, q);
-#pragma unroll
-                        for (int u = 0; u < U; ++u)
-#pragma unroll
-                            for (int n = 0; n < N; ++n)
-                                acc[kG][n] = fmaf(g[u][n], n1[u][n] * p[n] + q[n], acc[kG][n]);
-                        par_all(kG, q);
-#pragma unroll
-                        for (int u = 0; u < U; ++u)
-#pragma unroll
-                            for (int n = 0; n < N; ++n) {
-                                g[u][n] *= q[n];
-                                acc[kB1][n] += g[u][n];
-                                acc[kW1][n] = fmaf(g[u][n], n1[u][n], acc[kW1][n]);
-                                g[u][n] *= p[n];
-                            }
-                        if (a.dx) {
-                            rn_normalise_back<U, N, false>(g, n1, rstd1, a.norm1, inv_c, lpr, nullptr);
-#pragma unroll
-                            for (int u = 0; u < U; ++u)
-#pragma unroll
-                                for (int j = 0; j < VPT; ++j)
-                                    if (live[u] && have[j]) rn_store_smem<T, VEC>(tx + at[u] + col[j], g[u] + j * VEC);
-                        }
-                    }
-                }
+                int base = (int)(part - tile0);
+                for (; base + groups * U <= last; base += groups * U) rows(std::false_type{}, base, last);
+                if (base < last) rows(std::true_type{}, base, last);
                 part = end;
             }
             if (!ok) break;
@@ -1109,9 +1135,11 @@ static int rn_launch(RnArgs &a, bool backward, cudaStream_t st) {
 // The bulk form: C <= 256 (a lane's parameters and sums stay in registers), tensors on 16-byte
 // boundaries, and at least two tiles per SM, or its ring never fills: below that the direct kernel
 // spreads the rows over more blocks.
-template <typename T, int VEC, int VPT>
-static bool rb_launch(RnArgs &a, bool backward, cudaStream_t st, int &rc) {
-    const int row_bytes = a.C * (int)sizeof(T), groups = kRbWarps * 32 / a.lpr;
+template <typename T, int VEC, int VPT, bool BWD, bool FULL>
+static bool rb_launch(RnArgs &a, cudaStream_t st, int &rc) {
+    constexpr bool backward = BWD;
+    constexpr int U = VEC * VPT >= 16 ? 1 : VEC * VPT >= 4 ? 2 : 4;
+    const int row_bytes = a.C * (int)sizeof(T), groups = kRbWarps * 32 / a.lpr * U;
     const int unit = groups % 8 == 0 ? groups : groups % 4 == 0 ? groups * 2 : groups * 8;   // whole passes, 16-byte tiles
     RbArgs rb = {};
     rb.rows = unit * std::max(1, kRbTileBytes / (row_bytes * unit));
@@ -1119,7 +1147,7 @@ static bool rb_launch(RnArgs &a, bool backward, cudaStream_t st, int &rc) {
     if (tiles < 2 * 148) return false;
     rb.tile_bytes = (rb.rows * row_bytes + 127) & ~127;
     rb.cols = a.lpr * VPT * VEC;
-    const int extra = 256 + (kRnParams * rb.cols + (backward ? kRbWarps * a.nslots * a.C : 0)) * (int)sizeof(float);
+    const int extra = 256 + (kRbParams * rb.cols + (backward ? kRbWarps * a.nslots * a.C : 0)) * (int)sizeof(float);
     const int stage = (backward ? 4 : 2) * rb.tile_bytes + rb.rows * 16;
     rb.stages = std::min(kRbMaxStages, (kRbMaxSmem - extra) / stage);
     if (rb.stages < 2) return false;
@@ -1127,7 +1155,7 @@ static bool rb_launch(RnArgs &a, bool backward, cudaStream_t st, int &rc) {
     a.chunk = (tiles + 147) / 148 * rb.rows;
     const int grid = (int)((a.M + a.chunk - 1) / a.chunk);
     const int smem = extra + rb.stages * stage;
-    auto kern = backward ? residual_norm_bulk_kernel<T, VEC, VPT, true> : residual_norm_bulk_kernel<T, VEC, VPT, false>;
+    auto kern = residual_norm_bulk_kernel<T, VEC, VPT, BWD, FULL>;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kRbMaxSmem) != cudaSuccess) {
         rc = check_launch("residual_norm_bulk: set max dynamic shared memory");
         return true;
@@ -1144,13 +1172,29 @@ template <typename T>
 static int rn_dispatch(RnArgs &a, bool vec, bool aligned, bool backward, cudaStream_t st) {
     const int C = a.C;
     int rc = SPCONV_OK;
+    if (aligned && C <= 256) {
+        // FULL: the lanes' columns are exactly the row's (a power of two): no column is ever checked
+        bool ran = false;
+        if (vec && !backward && C % 16 == 0 && C >= 64) {    // half the shuffles of eight columns a lane
+            a.lpr = rn_pow2(C / 16);
+            ran = a.lpr * 16 == C ? rb_launch<T, 8, 2, false, true>(a, st, rc) : rb_launch<T, 8, 2, false, false>(a, st, rc);
+        } else if (vec) {
+            a.lpr = rn_pow2(C / 8);
+            const bool full = a.lpr * 8 == C;
+            ran = backward ? (full ? rb_launch<T, 8, 1, true, true>(a, st, rc) : rb_launch<T, 8, 1, true, false>(a, st, rc))
+                           : (full ? rb_launch<T, 8, 1, false, true>(a, st, rc) : rb_launch<T, 8, 1, false, false>(a, st, rc));
+        } else {
+            a.lpr = std::min(32, rn_pow2(C));
+            auto single = [&](auto per) {
+                constexpr int P = decltype(per)::value;
+                return backward ? rb_launch<T, 1, P, true, false>(a, st, rc) : rb_launch<T, 1, P, false, false>(a, st, rc);
+            };
+            ran = C <= 32 ? single(std::integral_constant<int, 1>{}) : C <= 64 ? single(std::integral_constant<int, 2>{})
+                : C <= 128 ? single(std::integral_constant<int, 4>{}) : single(std::integral_constant<int, 8>{});
+        }
+        if (ran) return rc;
+    }
     a.lpr = std::min(32, rn_pow2(vec ? C / 8 : C));
-    if (aligned && C <= 256 &&
-        (vec ? rb_launch<T, 8, 1>(a, backward, st, rc)
-             : C <= 32 ? rb_launch<T, 1, 1>(a, backward, st, rc)
-             : C <= 64 ? rb_launch<T, 1, 2>(a, backward, st, rc)
-             : C <= 128 ? rb_launch<T, 1, 4>(a, backward, st, rc) : rb_launch<T, 1, 8>(a, backward, st, rc)))
-        return rc;
     if (vec) {
         if (C <= 256) return rn_launch<T, 8, 1, false>(a, backward, st);
         if (C <= 512) return rn_launch<T, 8, 2, false>(a, backward, st);
