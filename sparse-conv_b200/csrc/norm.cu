@@ -23,6 +23,7 @@
 // All arithmetic is fp32; each output is rounded once. A row lives in the registers of the
 // lanes that own it, so every tensor is read once.
 #include <algorithm>
+#include <numeric>
 #include <type_traits>
 
 #include "common.cuh"
@@ -640,17 +641,18 @@ residual_norm_bwd_kernel(const __grid_constant__ RnArgs a) {
 // Rows of at most 256 channels, many of them: the streams through shared memory.
 //
 // Rows are contiguous, so R of them are one untiled bulk copy per tensor whatever the channel
-// count. One thread keeps a ring of stages of such copies in flight; twelve warps compute in
+// count. One thread keeps a ring of stages of such copies in flight; the other warps compute in
 // place (the outputs take the inputs' slots) and the same thread stores finished stages in bulk.
 // The direct kernels above hold what is in flight in registers (two loads a lane); measured
-// there and here: 2.0 M x 64 bf16 forward 255 and 186 us, 1.34 M x 128 backward 738 and 358 us.
+// there and here: 2.0 M x 64 bf16 forward 255 and 181 us (5.6 TB/s), 1.34 M x 128 forward 328 and
+// 246 us (5.6 TB/s), backward 738 and 438 us (4.7 TB/s). The backward issues 50 instructions a
+// value and spends most of its stalls on the row reductions' shuffles.
 // A tile that crosses a sample's end is worked off in two parts, so tiles stay aligned to 16
 // bytes for every channel count; only the last one can end in a few odd bytes, which that thread
 // copies itself.
 // Waits are bounded: a timeout raises SPCONV_STATUS_WAIT_TIMEOUT and the CTA leaves once its
 // copies have landed.
 // ---------------------------------------------------------------------------------------
-constexpr int kRbWarps = 12, kRbThreads = (kRbWarps + 1) * 32;
 constexpr int kRbMaxStages = 8;
 constexpr int kRbTileBytes = 12 * 1024;      // a tensor's share of a stage, about
 constexpr int kRbMaxSmem = 226 * 1024;
@@ -694,13 +696,11 @@ __device__ __forceinline__ void bulk_store(void *dst, uint32_t src, uint32_t byt
     asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;\n" :: "l"(dst), "r"(src), "r"(bytes) : "memory");
 }
 
-template <typename T, int VEC, int VPT, bool BWD, bool FULL>
-__global__ void __launch_bounds__(kRbThreads, 1)
+template <typename T, int VEC, int VPT, bool BWD, bool FULL, int W, int U>
+__global__ void __launch_bounds__((W + 1) * 32, 1)
 residual_norm_bulk_kernel(const __grid_constant__ RnArgs a, const __grid_constant__ RbArgs rb) {
     constexpr int N = VEC * VPT;
-    constexpr int U = N >= 16 ? 1 : N >= 4 ? 2 : 4;           // rows a lane works on at once: their sums overlap
     constexpr int kSums = 4;                 // of G, G * xhat, dy, dy * hhat
-    static_assert(!BWD || N <= 8, "a lane's sums stay in registers");
     constexpr int kTensors = BWD ? 4 : 2;    // slots of a stage: x (then h or dx), r (then y or dr), dh, dy
     extern __shared__ __align__(128) uint8_t s_raw[];
     uint64_t *full = reinterpret_cast<uint64_t *>(s_raw), *done = full + kRbMaxStages, *flush = done + kRbMaxStages;
@@ -709,14 +709,14 @@ residual_norm_bulk_kernel(const __grid_constant__ RnArgs a, const __grid_constan
     const int S = rb.stages, R = rb.rows, C = a.C, lpr = a.lpr;
     const int slot = rb.tile_bytes, stage = kTensors * slot + R * 16;          // the rows' statistics last
     float *s_par = reinterpret_cast<float *>(ring + S * stage);                // [kRbParams][rb.cols]
-    float *s_acc = s_par + kRbParams * rb.cols;                                // [kRbWarps][nslots][C]
+    float *s_acc = s_par + kRbParams * rb.cols;                                // [W][nslots][C]
     const int tid = threadIdx.x, warp = tid >> 5;
     if (tid == 0) {
         for (int i = 0; i < S; ++i) {
             mbar_init(smem_u32(&full[i]), 1);
-            mbar_init(smem_u32(&done[i]), kRbWarps);
+            mbar_init(smem_u32(&done[i]), W);
         }
-        mbar_init(smem_u32(flush), kRbWarps);
+        mbar_init(smem_u32(flush), W);
         *s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
@@ -726,7 +726,7 @@ residual_norm_bulk_kernel(const __grid_constant__ RnArgs a, const __grid_constan
     const int64_t row0 = (int64_t)blockIdx.x * a.chunk, row1 = min(a.M, row0 + a.chunk);
     const int tiles = row0 < row1 ? (int)((row1 - row0 + R - 1) / R) : 0;
 
-    if (warp == kRbWarps) {
+    if (warp == W) {
         // ------------------------------------------------------------------ copies
         if ((tid & 31) == 0) {
             const T *in[4] = {(const T *)a.x, (const T *)a.r, BWD ? (const T *)a.dh : nullptr, BWD ? (const T *)a.dy : nullptr};
@@ -788,7 +788,7 @@ residual_norm_bulk_kernel(const __grid_constant__ RnArgs a, const __grid_constan
         }
     } else {
         // ------------------------------------------------------------------ rows
-        const int groups = kRbWarps * 32 / lpr, group = tid / lpr, lane = tid & (lpr - 1);
+        const int groups = W * 32 / lpr, group = tid / lpr, lane = tid & (lpr - 1);
         const float inv_c = 1.f / (float)C;
         int col[VPT];
         bool have[VPT];
@@ -842,10 +842,10 @@ residual_norm_bulk_kernel(const __grid_constant__ RnArgs a, const __grid_constan
                 if (from >= 0) {
                     const int n = a.nslots * C;
                     float *rec = a.partial + ((int64_t)blockIdx.x + from) * n;
-                    for (int i = tid; i < n; i += kRbWarps * 32) {
+                    for (int i = tid; i < n; i += W * 32) {
                         float v = 0.f;
 #pragma unroll
-                        for (int w = 0; w < kRbWarps; ++w) v += s_acc[(int64_t)w * n + i];
+                        for (int w = 0; w < W; ++w) v += s_acc[(int64_t)w * n + i];
                         rec[i] = v;
                     }
 #pragma unroll
@@ -855,7 +855,7 @@ residual_norm_bulk_kernel(const __grid_constant__ RnArgs a, const __grid_constan
                 }
             }
             if (to >= 0)
-                for (int c = tid; c < rb.cols; c += kRbWarps * 32) {
+                for (int c = tid; c < rb.cols; c += W * 32) {
                     float v[kRnParams][1];
 #pragma unroll
                     for (int k = 0; k < kRnParams; ++k) {
@@ -882,16 +882,20 @@ residual_norm_bulk_kernel(const __grid_constant__ RnArgs a, const __grid_constan
 #pragma unroll
             for (int j = 0; j < VPT; ++j) par(k, j, f + j * VEC);
         };
+        // rows counted from the chunk's first: 32 bits
+        const int rows_here = (int)(row1 - row0);
         int smp = a.B > 1 && tiles > 0 ? rn_sample(a, row0) : 0;
-        auto sample_end = [&](int q) { return q < a.B - 1 ? min(row1, (int64_t)__ldg(a.offsets + q + 1)) : row1; };
-        int64_t s_end = tiles > 0 ? sample_end(smp) : 0;
+        auto sample_end = [&](int q) {
+            return q < a.B - 1 ? (int)max((int64_t)0, min(row1, (int64_t)__ldg(a.offsets + q + 1)) - row0) : rows_here;
+        };
+        int s_end = tiles > 0 ? sample_end(smp) : 0;
         bool ok = tiles > 0 && turn(-1, smp);
         int s = 0;
         uint32_t phase = 0;
-        for (int t = 0; t < tiles && ok; ++t) {
+        for (int tile0 = 0; tile0 < rows_here && ok; tile0 += R) {
             ok = __all_sync(0xffffffffu, wait(&full[s], phase)) != 0;
             if (!ok) break;
-            const int64_t tile0 = row0 + (int64_t)t * R, tile1 = min(row1, tile0 + R);
+            const int tile1 = min(rows_here, tile0 + R);
             uint8_t *base_s = ring + s * stage;
             T *tx = reinterpret_cast<T *>(base_s), *tr = reinterpret_cast<T *>(base_s + slot);
             const T *th = reinterpret_cast<const T *>(base_s + (BWD ? 2 * slot : 0));
@@ -1029,16 +1033,15 @@ residual_norm_bulk_kernel(const __grid_constant__ RnArgs a, const __grid_constan
                     }
                 }
             };
-            for (int64_t part = tile0; part < tile1;) {
+            for (int part = tile0; part < tile1;) {
                 if (s_end <= part) {         // the next sample that has rows (the last one takes the rest)
                     const int from = smp;
                     do s_end = sample_end(++smp);
                     while (s_end <= part);
                     if (!turn(from, smp)) { ok = false; break; }
                 }
-                const int64_t end = min(tile1, s_end);
-                const int last = (int)(end - tile0);
-                int base = (int)(part - tile0);
+                const int end = min(tile1, s_end), last = end - tile0;
+                int base = part - tile0;
                 for (; base + groups * U <= last; base += groups * U) rows(std::false_type{}, base, last);
                 if (base < last) rows(std::true_type{}, base, last);
                 part = end;
@@ -1071,20 +1074,30 @@ residual_norm_grad_kernel(const __grid_constant__ RnArgs a, const __grid_constan
     __shared__ float part[32][33];
     const int k = blockIdx.y;
     const int c = blockIdx.x * 32 + threadIdx.x;
-    const int s_first = o.per_sample[k] ? blockIdx.z : 0, s_last = o.per_sample[k] ? blockIdx.z : a.B - 1;
     if (!o.per_sample[k] && blockIdx.z != 0) return;
     grid_dependency_wait();
+    // Rows before offsets[1] belong to sample 0 and rows from offsets[B - 1] on to the last, as in the walk.
+    auto first_row = [&](int s) { return s == 0 ? (int64_t)0 : max((int64_t)0, min(a.M, (int64_t)__ldg(a.offsets + s))); };
+    auto end_row = [&](int s) { return s == a.B - 1 ? a.M : max((int64_t)0, min(a.M, (int64_t)__ldg(a.offsets + s + 1))); };
+    auto record = [&](int64_t chunk, int s) { return c < a.C ? __ldcg(a.partial + ((chunk + s) * a.nslots + k) * a.C + c) : 0.f; };
+    const int64_t chunks = (a.M + a.chunk - 1) / a.chunk;
     float v = 0.f;
-    for (int s = s_first; s <= s_last; ++s) {
-        int64_t lo = 0, hi = a.M;
-        if (a.B > 1) {
-            // the walk gives rows before offsets[1] to sample 0 and rows from offsets[B - 1] on to the last
-            lo = s == 0 ? 0 : max((int64_t)0, min(a.M, (int64_t)__ldg(a.offsets + s)));
-            hi = s == a.B - 1 ? a.M : max((int64_t)0, min(a.M, (int64_t)__ldg(a.offsets + s + 1)));
+    if (o.per_sample[k]) {
+        const int s = blockIdx.z;
+        const int64_t lo = first_row(s), hi = end_row(s);
+        if (lo < hi)
+            for (int64_t b = lo / a.chunk + threadIdx.y; b <= (hi - 1) / a.chunk; b += 32) v += record(b, s);
+    } else {
+        for (int64_t b = threadIdx.y; b < chunks; b += 32) {
+            const int64_t r0 = b * a.chunk, r1 = min(a.M, r0 + a.chunk);
+            if (a.B == 1) {
+                v += record(b, 0);
+                continue;
+            }
+            const int last = rn_sample(a, r1 - 1);
+            for (int s = rn_sample(a, r0); s <= last; ++s)
+                if (max(r0, first_row(s)) < min(r1, end_row(s))) v += record(b, s);
         }
-        if (lo >= hi) continue;
-        for (int64_t b = lo / a.chunk + threadIdx.y; b <= (hi - 1) / a.chunk; b += 32)
-            if (c < a.C) v += a.partial[((b + s) * a.nslots + k) * a.C + c];
     }
     part[threadIdx.y][threadIdx.x] = v;
     __syncthreads();
@@ -1132,35 +1145,40 @@ static int rn_launch(RnArgs &a, bool backward, cudaStream_t st) {
     return check_launch("residual_norm_bwd_kernel");
 }
 
-// The bulk form: C <= 256 (a lane's parameters and sums stay in registers), tensors on 16-byte
-// boundaries, and at least two tiles per SM, or its ring never fills: below that the direct kernel
-// spreads the rows over more blocks.
+// The ring form: C <= 256 (a lane's sums stay in registers), tensors on 16-byte boundaries, and at
+// least two tiles per SM, or the ring never fills: below that the direct kernel spreads the rows over
+// more blocks.
 template <typename T, int VEC, int VPT, bool BWD, bool FULL>
 static bool rb_launch(RnArgs &a, cudaStream_t st, int &rc) {
     constexpr bool backward = BWD;
-    constexpr int U = VEC * VPT >= 16 ? 1 : VEC * VPT >= 4 ? 2 : 4;
-    const int row_bytes = a.C * (int)sizeof(T), groups = kRbWarps * 32 / a.lpr * U;
-    const int unit = groups % 8 == 0 ? groups : groups % 4 == 0 ? groups * 2 : groups * 8;   // whole passes, 16-byte tiles
+    constexpr int N = VEC * VPT;
+    // Warps and rows in hand, measured at 1.34 M x 128 bf16: forward with 12 warps 246 us at two rows of
+    // sixteen columns a lane, 340 us at one; backward with 10 warps 438 us at two rows of eight, with
+    // 12 (128 registers) 490 us, with 8 504 us, with 20 at one row 769 us. Single columns a lane need
+    // fewer registers: 15 warps.
+    constexpr int W = VEC == 1 ? 15 : BWD ? 10 : 12, U = N >= 4 ? 2 : 4;
+    const int row_bytes = a.C * (int)sizeof(T), groups = W * 32 / a.lpr * U;
+    const int unit = std::lcm(groups, 8);    // whole passes, and tiles of whole 16 bytes
     RbArgs rb = {};
     rb.rows = unit * std::max(1, kRbTileBytes / (row_bytes * unit));
     const int64_t tiles = (a.M + rb.rows - 1) / rb.rows;
     if (tiles < 2 * 148) return false;
     rb.tile_bytes = (rb.rows * row_bytes + 127) & ~127;
     rb.cols = a.lpr * VPT * VEC;
-    const int extra = 256 + (kRbParams * rb.cols + (backward ? kRbWarps * a.nslots * a.C : 0)) * (int)sizeof(float);
+    const int extra = 256 + (kRbParams * rb.cols + (backward ? W * a.nslots * a.C : 0)) * (int)sizeof(float);
     const int stage = (backward ? 4 : 2) * rb.tile_bytes + rb.rows * 16;
     rb.stages = std::min(kRbMaxStages, (kRbMaxSmem - extra) / stage);
-    if (rb.stages < 2) return false;
+    if (rb.stages < 3) return false;         // two do not keep HBM busy: 1.34 M x 128 backward 438 -> 663 us
     rb.wait_ns = wait_limit_ns();
     a.chunk = (tiles + 147) / 148 * rb.rows;
     const int grid = (int)((a.M + a.chunk - 1) / a.chunk);
     const int smem = extra + rb.stages * stage;
-    auto kern = residual_norm_bulk_kernel<T, VEC, VPT, BWD, FULL>;
+    auto kern = residual_norm_bulk_kernel<T, VEC, VPT, BWD, FULL, W, U>;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kRbMaxSmem) != cudaSuccess) {
         rc = check_launch("residual_norm_bulk: set max dynamic shared memory");
         return true;
     }
-    kern<<<grid, kRbThreads, smem, st>>>(a, rb);
+    kern<<<grid, (W + 1) * 32, smem, st>>>(a, rb);
     rc = check_launch("residual_norm_bulk_kernel");
     return true;
 }
