@@ -793,9 +793,18 @@ bool make_tmap_2d(CUtensorMap *map, const void *ptr, uint64_t cols, uint64_t row
     const uint32_t wbytes = box_cols * 2;
     const CUtensorMapSwizzle sw = wbytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B
                                 : (wbytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B);
-    const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void *>(ptr), dims, strides,
-                           box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, sw, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
-                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    auto encode = [&]() {
+        return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void *>(ptr), dims, strides, box, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, sw, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    };
+    CUresult r = encode();
+    if (r == CUDA_ERROR_INVALID_CONTEXT) {
+        // a thread's first call (autograd's, say): the driver needs the device's context current, which
+        // any runtime call that uses the device makes it
+        cudaFree(nullptr);
+        r = encode();
+    }
     if (r != CUDA_SUCCESS) {
         set_error("tensor map encoding failed (CUresult %d)", (int)r);
         return false;

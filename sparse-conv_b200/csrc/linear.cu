@@ -209,30 +209,48 @@ linear_dact_kernel(const T *__restrict__ gout, const T *__restrict__ z, T *__res
     }
 }
 
-// out[i] = sum over s of partial[s][i], in the order of s within 8 lanes of splits.
-template <typename T>
-__global__ void __launch_bounds__(256)
-linear_reduce_kernel(const float *__restrict__ partial, int splits, int64_t n, T *__restrict__ out) {
-    __shared__ float part[8][33];
-    const int64_t i = (int64_t)blockIdx.x * 32 + threadIdx.x;
+// out[i] = sum over s of partial[s][i], in the order of s within 16 lanes of splits; two arrays in one
+// launch (a weight's and a bias's sums).
+struct ReduceSeg {
+    const float *partial;
+    int splits;
+    int64_t n;
+    void *out;
+    int dtype;
+    int blocks;
+};
+
+__global__ void __launch_bounds__(512)
+linear_reduce_kernel(const ReduceSeg a, const ReduceSeg b) {
+    __shared__ float part[16][33];
+    const bool second = (int)blockIdx.x >= a.blocks;
+    const ReduceSeg &g = second ? b : a;
+    const int64_t i = (int64_t)(blockIdx.x - (second ? a.blocks : 0)) * 32 + threadIdx.x;
+    grid_dependency_wait();
     float v = 0.f;
-    if (i < n)
-        for (int s = threadIdx.y; s < splits; s += 8) v += __ldcs(partial + (int64_t)s * n + i);
+    if (i < g.n) {
+#pragma unroll 4
+        for (int s = threadIdx.y; s < g.splits; s += 16) v += __ldcs(g.partial + (int64_t)s * g.n + i);
+    }
     part[threadIdx.y][threadIdx.x] = v;
     __syncthreads();
-    if (threadIdx.y == 0 && i < n) {
+    if (threadIdx.y == 0 && i < g.n) {
         float sum = 0.f;
 #pragma unroll
-        for (int y = 0; y < 8; ++y) sum += part[y][threadIdx.x];
-        out[i] = dtype_traits<T>::from_f(sum);
+        for (int y = 0; y < 16; ++y) sum += part[y][threadIdx.x];
+        if (g.dtype == SPCONV_F32) ((float *)g.out)[i] = sum;
+        else if (g.dtype == SPCONV_F16) ((__half *)g.out)[i] = __float2half_rn(sum);
+        else ((__nv_bfloat16 *)g.out)[i] = __float2bfloat16_rn(sum);
     }
 }
 
-static int launch_reduce(const float *partial, int splits, int64_t n, int out_dtype, void *out, cudaStream_t st) {
-    const dim3 grid((unsigned)((n + 31) / 32)), block(32, 8);
-    if (out_dtype == SPCONV_F32) linear_reduce_kernel<float><<<grid, block, 0, st>>>(partial, splits, n, (float *)out);
-    else if (out_dtype == SPCONV_F16) linear_reduce_kernel<__half><<<grid, block, 0, st>>>(partial, splits, n, (__half *)out);
-    else linear_reduce_kernel<__nv_bfloat16><<<grid, block, 0, st>>>(partial, splits, n, (__nv_bfloat16 *)out);
+static ReduceSeg reduce_seg(const float *partial, int splits, int64_t n, int dtype, void *out) {
+    return {partial, splits, n, out, dtype, out ? (int)((n + 31) / 32) : 0};
+}
+
+static int launch_reduce(const ReduceSeg &a, const ReduceSeg &b, cudaStream_t st) {
+    if (a.blocks + b.blocks == 0) return SPCONV_OK;
+    launch_pdl(linear_reduce_kernel, dim3((unsigned)(a.blocks + b.blocks)), dim3(32, 16), 0, st, a, b);
     return check_launch("linear_reduce_kernel");
 }
 
@@ -331,8 +349,10 @@ extern "C" int spconv_linear_forward(const void *feats, int dtype, int64_t M, in
 
 extern "C" int64_t spconv_linear_backward_workspace_bytes(int dtype, int64_t M, int Ci, int Co, int activation) {
     if (check_linear(dtype, M, Ci, Co, activation, SPCONV_KERNEL_AUTO) != SPCONV_OK) return -1;
-    return pad256(activation == SPCONV_ACT_NONE ? 0 : M * Co * elt(dtype)) + pad256((int64_t)dact_chunks(M) * Co * 4) +
-           pad256((int64_t)std::max(wgrad_splits(M, Ci, Co), gemm_tc_splits(Co, Ci, M)) * Co * Ci * 4);
+    const int64_t separate = pad256(activation == SPCONV_ACT_NONE ? 0 : M * Co * elt(dtype)) + pad256((int64_t)dact_chunks(M) * Co * 4) +
+                             pad256((int64_t)std::max(wgrad_splits(M, Ci, Co), gemm_tc_splits(Co, Ci, M)) * Co * Ci * 4);
+    const int64_t grid = bwd_tc_grid(M);
+    return std::max(separate, pad256(grid * 8 * Co * 4) + pad256(grid * Co * Ci * 4));
 }
 
 extern "C" int spconv_linear_backward(const void *grad_out, const void *preact, const void *feats, const void *weight,
@@ -359,6 +379,18 @@ extern "C" int spconv_linear_backward(const void *grad_out, const void *preact, 
                        workspace_bytes >= spconv_linear_backward_workspace_bytes(dtype, M, Ci, Co, activation),
                    SPCONV_ERR_ARG, "workspace missing, misaligned or too small");
     uint8_t *ws = (uint8_t *)workspace;
+    bool aligned = true;
+    for (const void *p : {grad_out, preact, feats, weight, (const void *)grad_feats})
+        aligned = aligned && ((uintptr_t)p & 15) == 0;
+    if (kernel_choice != SPCONV_KERNEL_SIMT && aligned && bwd_tc_shape(dtype, M, Ci, Co, activation)) {
+        const int grid = bwd_tc_grid(M);
+        BwdArgs q = {grad_out, preact, feats, weight, dtype, M, Ci, Co, activation, grad_feats, nullptr, nullptr, status, st};
+        if (grad_bias) q.b_partial = (float *)ws;
+        if (grad_weight) q.w_partial = (float *)(ws + pad256((int64_t)grid * 8 * Co * 4));
+        if (const int rc = launch_bwd_tc(q)) return rc;
+        return launch_reduce(reduce_seg(q.w_partial, grid, (int64_t)Co * Ci, weight_dtype, grad_weight),
+                             reduce_seg(q.b_partial, grid * 8, Co, bias_dtype, grad_bias), st);
+    }
     const void *dz = grad_out;
     if (activation != SPCONV_ACT_NONE) {
         dz = ws;
@@ -371,8 +403,6 @@ extern "C" int spconv_linear_backward(const void *grad_out, const void *preact, 
         if (const int rc = launch_dact(dtype, grad_out, preact, activation != SPCONV_ACT_NONE ? (void *)dz : nullptr,
                                        grad_bias ? bias_part : nullptr, M, Co, activation, st))
             return rc;
-        if (grad_bias)
-            if (const int rc = launch_reduce(bias_part, dact_chunks(M), Co, bias_dtype, grad_bias, st)) return rc;
     }
     GemmArgs g = {};
     g.dtype = dtype;
@@ -403,7 +433,7 @@ extern "C" int spconv_linear_backward(const void *grad_out, const void *preact, 
         g.k_per_split = ((M + g.splits - 1) / g.splits + step - 1) / step * step;
         g.splits = (int)((M + g.k_per_split - 1) / g.k_per_split);
         if (const int rc = launch_gemm(g, kernel_choice)) return rc;
-        if (const int rc = launch_reduce(weight_part, g.splits, (int64_t)Co * Ci, weight_dtype, grad_weight, st)) return rc;
     }
-    return SPCONV_OK;
+    return launch_reduce(reduce_seg(weight_part, g.splits, (int64_t)Co * Ci, weight_dtype, grad_weight),
+                         reduce_seg(bias_part, dact_chunks(M), Co, bias_dtype, grad_bias), st);
 }

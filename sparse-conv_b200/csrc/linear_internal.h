@@ -34,4 +34,20 @@ int launch_gemm_tc(const GemmArgs &g);
 // Splits of K for an [M, N] sum over K.
 int gemm_tc_splits(int64_t M, int64_t N, int64_t K);
 
+// The whole backward in one pass over the rows (linear_bwd_tc.cu): grad_feats, and partial sums
+// w_partial [bwd_tc_grid(M)][Co][Ci] and b_partial [8 * bwd_tc_grid(M)][Co]; each may be null.
+struct BwdArgs {
+    const void *grad_out, *preact, *feats, *weight;
+    int dtype;
+    int64_t M;
+    int Ci, Co, activation;
+    void *grad_feats;
+    float *w_partial, *b_partial;
+    int32_t *status;
+    cudaStream_t stream;
+};
+bool bwd_tc_shape(int dtype, int64_t M, int Ci, int Co, int activation);
+int bwd_tc_grid(int64_t M);
+int launch_bwd_tc(const BwdArgs &q);
+
 }  // namespace spconv

@@ -279,3 +279,51 @@ def test_forced_kernels_agree_with_the_definition():
     v, e, _, _ = _forward_ref(x, w, b, r, "gelu")
     out, _ = _native.linear_forward(x, w, b, r, "gelu", kernel=_native.KERNEL_SIMT)
     _check(out, v, e, torch.float16, "CUDA cores")
+
+
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("M,Ci,Co", [(37888, 64, 64), (40001, 128, 128), (38000, 8, 8), (41000, 72, 96), (50003, 64, 256),
+                                     (38001, 24, 136), (39000, 128, 16), (37900, 16, 200), (60000, 128, 64)])
+def test_backward_in_one_pass(M, Ci, Co, dtype, act):
+    x, w, b, _, g = _inputs(M, Ci, Co, DT[dtype], residual=False, seed=21)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    grads = torch.autograd.grad(sparse_linear(x, w, b, activation=act), leaves, g)
+    x, w, b = x.detach(), w.detach(), b.detach()
+    refs = _backward_ref(x, w, b, g, act, DT[dtype])
+    for got, ref, what in zip(grads, refs, ("feats", "weight", "bias")):
+        _check(got, *ref, DT[dtype], what)
+    for i in range(3):                       # one gradient at a time: the same bits
+        part = [t.clone().requires_grad_(j == i) for j, t in enumerate((x, w, b))]
+        got = torch.autograd.grad(sparse_linear(*part, activation=act), part[i], g)[0]
+        assert torch.equal(got, grads[i])
+
+
+def test_backward_in_one_pass_same_bits_every_run():
+    x, w, b, _, g = _inputs(70001, 128, 128, torch.bfloat16, residual=False, seed=22)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    once = lambda: torch.autograd.grad(sparse_linear(x, w, b, activation="gelu"), leaves, g)
+    first = once()
+    for _ in range(4):
+        assert all(torch.equal(a, c) for a, c in zip(first, once()))
+
+
+@pytest.mark.parametrize("M", [300, 40000])
+def test_first_call_of_a_thread(M):
+    """A thread that has made no CUDA call of its own (autograd runs backwards in such)."""
+    import threading
+    x, w, b, _, g = _inputs(M, 64, 64, torch.bfloat16, residual=False, seed=23)
+    out, _ = _native.linear_forward(x, w, b, None, "none")
+    want = _native.linear_backward(g, None, x, w, "none", torch.bfloat16, torch.bfloat16, (True, True, True))
+    torch.cuda.synchronize()
+    got = []
+
+    def call():
+        got.append(_native.linear_backward(g, None, x, w, "none", torch.bfloat16, torch.bfloat16, (True, True, True)))
+        got.append(_native.linear_forward(x, w, b, None, "none")[0])
+    t = threading.Thread(target=call)
+    t.start()
+    t.join()
+    assert len(got) == 2
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, c) for a, c in zip(got[0], want)) and torch.equal(got[1], out)
