@@ -20,6 +20,12 @@
 //               by TMA (which clips ragged edges). The residual arrives by TMA, ahead of its turn, in
 //               the slot the output leaves from. Four warps per scheduler, since GELU and SiLU are
 //               dependent chains that two could not hide.
+// PAIR: two CTAs of a cluster, on two SMs, share a 256 x 256 tile (cta_group::2). Each holds its 128
+// rows of A, half of B's columns and its own rows' accumulators; the first one's MMA thread drives
+// both tensor cores, and commits to barriers in both. A K step then brings 32 KB into an SM instead of
+// 48. 84,000 x 512 -> 2048 bf16: 183 us unpaired, 170 us paired (1.03 PFLOP/s; the library's product
+// alone takes 151 us). Keeping a pair's halves of B in shared memory (K <= 512) leaves one output slot a
+// warp and is slower, 192 us.
 // The weight gradient's K is the voxels: K is cut into splits, each writes fp32 sums of its own,
 // and linear_reduce_kernel adds them in a fixed order.
 // Every wait is bounded (the conv kernels' limit); a timeout raises SPCONV_STATUS_WAIT_TIMEOUT and
@@ -39,7 +45,6 @@ constexpr int kLtThreads = 576;
 constexpr int kLtBM = 128, kLtBK = 64;
 constexpr int kLtABytes = kLtBM * kLtBK * 2;            // 16 KB a stage
 constexpr int kLtEpiWarps = 16, kLtEpiGroups = 4;
-constexpr int kLtSlot = 32 * 128;                       // 32 rows of 64 columns
 constexpr int kLtMaxBias = 4096;                        // bias columns kept in shared memory
 constexpr int kLtMaxStages = 12;
 constexpr int kLtMaxSlots = 4;
@@ -72,7 +77,8 @@ __device__ __forceinline__ void lt_wait_read(int pending) {
     else bulk_wait_read<3>();
 }
 
-template <typename T, bool A_T, bool B_T, int ACT>
+// CH: columns an epilogue warp takes at a time: 64, or 32 where shared memory has no room for 64.
+template <typename T, bool A_T, bool B_T, int ACT, bool PAIR, int CH>
 __global__ void __launch_bounds__(kLtThreads, 1)
 linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                  const __grid_constant__ CUtensorMap map_out, const __grid_constant__ CUtensorMap map_res,
@@ -81,13 +87,15 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     extern __shared__ uint8_t smem_raw[];
     uint8_t *base = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     const int BN = a.BN, S = a.stages, NO = a.slots;
-    const int b_bytes = BN * 128;
+    const uint32_t rank = PAIR ? cluster_rank() : 0;
+    const int b_bytes = (PAIR ? BN / 2 : BN) * 128;
     const int stage_bytes = kLtABytes + (a.b_resident ? 0 : b_bytes);
     const uint32_t s_b = smem_u32(base);                               // resident B
     const uint32_t s_stage = s_b + a.b_resident * b_bytes;
     const int warp_slots = NO * (a.has_preact ? 2 : 1);
+    constexpr int slot_bytes = 64 * CH;                                // a slot: 32 rows of CH columns
     const uint32_t s_out = s_stage + S * stage_bytes;
-    uint8_t *tail = base + a.b_resident * b_bytes + S * stage_bytes + (PARTIAL ? 0 : kLtEpiWarps * warp_slots * kLtSlot);
+    uint8_t *tail = base + a.b_resident * b_bytes + S * stage_bytes + (PARTIAL ? 0 : kLtEpiWarps * warp_slots * slot_bytes);
     uint64_t *bar = reinterpret_cast<uint64_t *>(tail);
     uint64_t *full = bar, *empty = full + kLtMaxStages, *bfull = empty + kLtMaxStages, *accfull = bfull + 1;
     uint64_t *accempty = accfull + kLtEpiGroups, *rbar = accempty + kLtEpiGroups;
@@ -96,7 +104,8 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     float *s_bias = reinterpret_cast<float *>(tail + kLtTail);
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int G = gridDim.x;
+    // workers: CTAs, or pairs of them
+    const int G = PAIR ? gridDim.x >> 1 : gridDim.x, me = PAIR ? blockIdx.x >> 1 : blockIdx.x;
     const uint32_t tmem_cols = (uint32_t)(a.bufs * BN);                // 256 or 512
     for (int i = tid; i < a.bias_smem; i += kLtThreads)
         s_bias[i] = i < a.N ? dtype_traits<T>::to_f(((const T *)a.bias)[i]) : 0.f;
@@ -108,17 +117,23 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         mbar_init(smem_u32(bfull), 1);
         for (int g = 0; g < a.bufs; ++g) {
             mbar_init(smem_u32(&accfull[g]), 1);
-            mbar_init(smem_u32(&accempty[g]), kLtEpiWarps / a.bufs);
+            mbar_init(smem_u32(&accempty[g]), (PAIR ? 2 : 1) * kLtEpiWarps / a.bufs);
         }
         for (int i = 0; i < kLtEpiWarps * NO; ++i) mbar_init(smem_u32(&rbar[i]), 1);
         *s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
     if (warp == 1) {
-        tmem_alloc(smem_u32(s_tmem), tmem_cols);
-        tmem_relinquish();
+        if constexpr (PAIR) {
+            tmem_alloc_pair(smem_u32(s_tmem), tmem_cols);
+            tmem_relinquish_pair();
+        } else {
+            tmem_alloc(smem_u32(s_tmem), tmem_cols);
+            tmem_relinquish();
+        }
     }
     tc_fence_before();
+    if constexpr (PAIR) cluster_sync();      // the barriers of both are ready
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *s_tmem;
@@ -155,6 +170,9 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
             }
         }
     };
+    auto row_of = [&](const Walk &w) { return PAIR ? w.m * (2 * kLtBM) + (int)rank * kLtBM : w.m * kLtBM; };
+    // an MMA's N: a multiple of 16, and of 32 over a pair
+    auto mma_cols = [&](int n0) { return (min(BN, a.N - n0) + (PAIR ? 31 : 15)) & ~(PAIR ? 31 : 15); };
     auto k_begin = [&](const Walk &w) { return PARTIAL ? w.split * a.k_per_split : 0; };
     auto k_end = [&](int k0) { return PARTIAL && a.K - k0 > a.k_per_split ? k0 + a.k_per_split : a.K; };
     // ring position: index and the parity of its current use
@@ -168,33 +186,44 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     if (warp == 0) {
         // ------------------------------------------------------------------ loads
         if (lane == 0) {
+            auto load = [&](uint32_t dst, const CUtensorMap *map, int x, int y, uint32_t mbar) {
+                if constexpr (PAIR) tma_load_2d_pair(dst, map, x, y, mbar);
+                else tma_load_2d(dst, map, x, y, mbar);
+            };
             auto load_b = [&](uint32_t dst, int k, int n0, uint32_t mbar) {
+                if constexpr (PAIR) n0 += (int)rank * (mma_cols(n0) >> 1);    // this CTA's half of B's columns
                 if constexpr (B_T) {
-                    for (int c = 0; c < BN / 64; ++c) tma_load_2d(dst + c * 8192, &map_b, n0 + c * 64, k, mbar);
+                    for (int c = 0; c < b_bytes / 8192; ++c) load(dst + c * 8192, &map_b, n0 + c * 64, k, mbar);
                 } else {
-                    tma_load_2d(dst, &map_b, k, n0, mbar);
+                    load(dst, &map_b, k, n0, mbar);
                 }
             };
             int st = 0;
             uint32_t phase = 0;
             int issued = 0;                  // stages in use, at most S
             bool ok = true;
-            Walk w = begin(blockIdx.x, G);
+            Walk w = begin(me, G);
             if (a.b_resident && w.item < a.items) {           // the grid is a multiple of nb: n never changes
                 mbar_arrive_expect_tx(smem_u32(bfull), (uint32_t)(a.b_resident * b_bytes));
                 for (int c = 0; c < a.b_resident; ++c) load_b(s_b + c * b_bytes, c * kLtBK, w.n * BN, smem_u32(bfull));
             }
             for (; w.item < a.items && ok; advance(w)) {
-                const int m0 = w.m * kLtBM, n0 = w.n * BN, k0 = k_begin(w), k1 = k_end(k0);
+                const int m0 = row_of(w), n0 = w.n * BN, k0 = k_begin(w), k1 = k_end(k0);
                 for (int k = k0; k < k1; k += kLtBK) {
                     if (issued == S && !wait(&empty[st], phase ^ 1u)) { ok = false; break; }
-                    const uint32_t mbar = smem_u32(&full[st]), dst = s_stage + st * stage_bytes;
-                    mbar_arrive_expect_tx(mbar, (uint32_t)stage_bytes);
-                    if constexpr (A_T) {
-                        tma_load_2d(dst, &map_a, m0, k, mbar);
-                        tma_load_2d(dst + 8192, &map_a, m0 + 64, k, mbar);
+                    uint32_t mbar = smem_u32(&full[st]);
+                    const uint32_t dst = s_stage + st * stage_bytes;
+                    if constexpr (PAIR) {    // both CTAs' bytes count on the first one's barrier
+                        if (rank == 0) mbar_arrive_expect_tx(mbar, 2 * (uint32_t)stage_bytes);
+                        mbar = cluster_addr(mbar, 0);
                     } else {
-                        tma_load_2d(dst, &map_a, k, m0, mbar);
+                        mbar_arrive_expect_tx(mbar, (uint32_t)stage_bytes);
+                    }
+                    if constexpr (A_T) {
+                        load(dst, &map_a, m0, k, mbar);
+                        load(dst + 8192, &map_a, m0 + 64, k, mbar);
+                    } else {
+                        load(dst, &map_a, k, m0, mbar);
                     }
                     if (!a.b_resident) load_b(dst + kLtABytes, k, n0, mbar);
                     if (issued < S) ++issued;
@@ -203,24 +232,39 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
             }
             // every load has landed before the CTA may exit (at once unless the MMA gave up): the
             // stages from st on were last used a phase earlier than those before it
-            for (int i = 0; i < issued; ++i)
-                mbar_wait_bounded(smem_u32(&full[i]), i < st ? phase : phase ^ 1u, kTmaDrainNs);
-            if (a.b_resident && (int)blockIdx.x < a.items) mbar_wait_bounded(smem_u32(bfull), 0, kTmaDrainNs);
+            if constexpr (PAIR) {
+                // what landed here is counted on the first CTA's barriers, and the last empties say that it
+                // was used; after giving up, the bound of such copies is waited out
+                if (!ok) {
+                    const uint64_t t0 = globaltimer_ns();
+                    while (globaltimer_ns() - t0 < kTmaDrainNs) {}
+                } else {
+                    for (int i = 0; i < issued; ++i)
+                        mbar_wait_bounded(smem_u32(&empty[i]), i < st ? phase : phase ^ 1u, a.wait_ns + kTmaDrainNs);
+                }
+            } else {
+                for (int i = 0; i < issued; ++i)
+                    mbar_wait_bounded(smem_u32(&full[i]), i < st ? phase : phase ^ 1u, kTmaDrainNs);
+                if (a.b_resident && (int)blockIdx.x < a.items) mbar_wait_bounded(smem_u32(bfull), 0, kTmaDrainNs);
+            }
         }
     } else if (warp == 1) {
         // ------------------------------------------------------------------ MMA
-        if (lane == 0) {
+        if (lane == 0 && rank == 0) {
+            auto commit = [&](uint64_t *b) {
+                if constexpr (PAIR) tc_commit_pair(smem_u32(b));
+                else tc_commit(smem_u32(b));
+            };
             int st = 0, buf = 0, last = -1;
             uint32_t phase = 0, acc_phase = 1;                // the first use of a buffer passes at once
             bool ok = true;
-            Walk w = begin(blockIdx.x, G);
+            Walk w = begin(me, G);
             if (a.b_resident && w.item < a.items) ok = wait(bfull, 0);
             for (; w.item < a.items && ok; advance(w)) {
                 const int n0 = w.n * BN, k0 = k_begin(w), k1 = k_end(k0);
                 if (!wait(&accempty[buf], acc_phase)) { ok = false; break; }
                 tc_fence_after();
-                const int n_mma = (min(BN, a.N - n0) + 15) & ~15;
-                const uint32_t idesc = instr_desc_f16(dtype_traits<T>::mma_format, kLtBM, n_mma) |
+                const uint32_t idesc = instr_desc_f16(dtype_traits<T>::mma_format, PAIR ? 2 * kLtBM : kLtBM, mma_cols(n0)) |
                                        (A_T ? 1u << 15 : 0u) | (B_T ? 1u << 16 : 0u);
                 const uint32_t d = tmem + (uint32_t)(buf * BN);
                 uint32_t s_res = s_b;
@@ -236,14 +280,15 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                                                 : smem_desc_kmajor_swizzled(sa + kk * 32, 128);
                         const uint64_t bd = B_T ? smem_desc_mn_sw128(sb + kk * 2048, 8192, 1024)
                                                 : smem_desc_kmajor_swizzled(sb + kk * 32, 128);
-                        tc_mma_f16(d, ad, bd, idesc, (k > k0 || kk > 0) ? 1u : 0u);
+                        if constexpr (PAIR) tc_mma_f16_pair(d, ad, bd, idesc, (k > k0 || kk > 0) ? 1u : 0u);
+                        else tc_mma_f16(d, ad, bd, idesc, (k > k0 || kk > 0) ? 1u : 0u);
                     }
-                    tc_commit(smem_u32(&empty[st]));
+                    commit(&empty[st]);
                     last = st;
                     next(st, phase, S);
                 }
                 if (ok) {
-                    tc_commit(smem_u32(&accfull[buf]));
+                    commit(&accfull[buf]);
                     next(buf, acc_phase, a.bufs);
                 }
             }
@@ -256,20 +301,21 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         const int ew = warp - 2, quad = warp & 3;
         const int buf = (ew >> 2) % a.bufs, sub = (ew >> 2) / a.bufs, share = kLtEpiGroups / a.bufs;
         const uint32_t t_acc = tmem + (uint32_t)(buf * BN) + ((uint32_t)(quad * 32) << 16);
-        const uint32_t slot0 = s_out + (uint32_t)(ew * warp_slots * kLtSlot);
-        const uint32_t pre0 = slot0 + (uint32_t)(NO * kLtSlot);
+        const uint32_t slot0 = s_out + (uint32_t)(ew * warp_slots * slot_bytes);
+        const uint32_t pre0 = slot0 + (uint32_t)(NO * slot_bytes);
         uint64_t *my_rbar = rbar + ew * NO;
-        const uint32_t row_at = (uint32_t)(lane * 128), row_x = (uint32_t)(lane & 7);
+        // rows of 128 (64) bytes: the 16-byte chunk's index XOR-ed with address bits 7 and up
+        const uint32_t row_at = (uint32_t)(lane * 2 * CH), row_x = (uint32_t)(CH == 64 ? lane & 7 : (lane >> 1) & 3);
         // one answer for the warp: its lanes must not part before the next warp-wide instruction
         auto all_wait = [&](uint64_t *b, uint32_t parity) { return __all_sync(0xffffffffu, wait(b, parity)) != 0; };
-        auto chunks_of = [&](int n0) { return (min(BN, a.N - n0) + 63) >> 6; };
+        auto chunks_of = [&](int n0) { return (min(BN, a.N - n0) + CH - 1) / CH; };
         // Residual loads run `ahead` chunks before their use. The slot of load L was last the
         // store of chunk L - NO, and when chunk b begins, b stores have been committed: those after
         // L - NO = b + ahead - NO may still be reading.
         const int ahead = NO >= 3 ? NO - 2 : NO - 1;
         int l_slot = 0, outstanding = 0, l_chunk = sub;
         uint32_t l_phase = 0;
-        Walk lw = begin(blockIdx.x + buf * G, a.bufs * G);
+        Walk lw = begin(me + buf * G, a.bufs * G);
         auto load_residual = [&](int behind) {        // the next chunk's, if there is one
             while (lw.item < a.items && l_chunk >= chunks_of(lw.n * BN)) {
                 advance(lw);
@@ -279,8 +325,8 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
             if (lane == 0) {
                 lt_wait_read(behind);
                 if (more) {
-                    mbar_arrive_expect_tx(smem_u32(&my_rbar[l_slot]), kLtSlot);
-                    tma_load_2d(slot0 + l_slot * kLtSlot, &map_res, lw.n * BN + l_chunk * 64, lw.m * kLtBM + quad * 32,
+                    mbar_arrive_expect_tx(smem_u32(&my_rbar[l_slot]), slot_bytes);
+                    tma_load_2d(slot0 + l_slot * slot_bytes, &map_res, lw.n * BN + l_chunk * CH, row_of(lw) + quad * 32,
                                 smem_u32(&my_rbar[l_slot]));
                 }
             }
@@ -294,14 +340,14 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
             for (int i = 0; i < ahead; ++i) load_residual(0);
         int s = 0;
         uint32_t s_phase = 0, use_phase = 0;
-        for (Walk w = begin(blockIdx.x + buf * G, a.bufs * G); w.item < a.items; advance(w), use_phase ^= 1u) {
-            const int m0 = w.m * kLtBM, n0 = w.n * BN;
+        for (Walk w = begin(me + buf * G, a.bufs * G); w.item < a.items; advance(w), use_phase ^= 1u) {
+            const int m0 = row_of(w), n0 = w.n * BN;
             const int n_cols = min(BN, a.N - n0), chunks = chunks_of(n0);
             if (!all_wait(&accfull[buf], use_phase)) break;
             tc_fence_after();
             bool ok = true;
             for (int j = sub; j < chunks; j += share, next(s, s_phase, NO)) {
-                const uint32_t so = slot0 + s * kLtSlot + row_at, sp = pre0 + s * kLtSlot + row_at;
+                const uint32_t so = slot0 + s * slot_bytes + row_at, sp = pre0 + s * slot_bytes + row_at;
                 if constexpr (!PARTIAL) {
                     if (a.has_residual) {
                         load_residual(NO - 1 - ahead);
@@ -314,8 +360,8 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                     if (!ok) break;
                 }
 #pragma unroll 1
-                for (int half = 0; half < 2; ++half) {
-                    const int c0 = j * 64 + half * 32;        // columns within the tile
+                for (int half = 0; half < CH / 32; ++half) {
+                    const int c0 = j * CH + half * 32;        // columns within the tile
                     if (c0 >= n_cols) break;
                     f32x2 f[16];
                     lt_load32(t_acc + (uint32_t)c0, f);
@@ -377,8 +423,8 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                     __syncwarp();
                     if (lane == 0) {
                         if (m0 + quad * 32 < a.M) {
-                            tma_store_2d(&map_out, n0 + j * 64, m0 + quad * 32, slot0 + s * kLtSlot);
-                            if (a.has_preact) tma_store_2d(&map_pre, n0 + j * 64, m0 + quad * 32, pre0 + s * kLtSlot);
+                            tma_store_2d(&map_out, n0 + j * CH, m0 + quad * 32, slot0 + s * slot_bytes);
+                            if (a.has_preact) tma_store_2d(&map_pre, n0 + j * CH, m0 + quad * 32, pre0 + s * slot_bytes);
                         }
                         bulk_commit();       // one group a chunk, empty or not
                     }
@@ -387,7 +433,10 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
             if (!ok) break;
             tc_fence_before();               // the accumulator has been read: free for the MMA
             __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&accempty[buf]));
+            if (lane == 0) {
+                if constexpr (PAIR) mbar_arrive_cluster(cluster_addr(smem_u32(&accempty[buf]), 0));
+                else mbar_arrive(smem_u32(&accempty[buf]));
+            }
         }
         if (!PARTIAL && lane == 0) {
             for (; outstanding > 0; --outstanding, next(s, s_phase, NO))     // residual loads nobody waited for
@@ -399,9 +448,13 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     __syncwarp();
     if (*s_abort && tid == 0) raise_status(a.status, SPCONV_STATUS_WAIT_TIMEOUT);
     tc_fence_before();
+    if constexpr (PAIR) cluster_sync();      // neither leaves while the other's MMAs or arrivals may reach it
     __syncthreads();
     tc_fence_after();
-    if (warp == 1) tmem_dealloc(tmem, tmem_cols);
+    if (warp == 1) {
+        if constexpr (PAIR) tmem_dealloc_pair(tmem, tmem_cols);
+        else tmem_dealloc(tmem, tmem_cols);
+    }
 }
 
 // ---------------------------------------------------------------------------------------
@@ -454,15 +507,24 @@ int gemm_tc_splits(int64_t M, int64_t N, int64_t K) {
     return (int)best;
 }
 
-template <typename T, bool A_T, bool B_T, int ACT>
+// A pair of CTAs takes 256 x 256 tiles where B cannot stay in shared memory anyway and there is a tile
+// for every pair of SMs.
+static bool lt_pair(const GemmArgs &g) {
+    const int64_t nk = (g.K + kLtBK - 1) / kLtBK;
+    const int64_t tiles = (g.M + 2 * kLtBM - 1) / (2 * kLtBM) * ((g.N + 255) / 256) * g.splits;
+    return g.N >= 256 && g.M >= 256 && nk * 256 * 128 > 96 * 1024 && tiles >= lt_sms() / 2;
+}
+
+template <typename T, bool A_T, bool B_T, int ACT, bool PAIR, int CH>
 static int lt_launch(const GemmArgs &g) {
     LtArgs a = {};
     a.M = (int)g.M;
     a.N = (int)g.N;
     a.K = (int)g.K;
-    a.BN = A_T ? (g.N > 128 ? 256 : g.N > 64 ? 128 : 64) : lt_bn(g.M, g.N, g.splits);
+    a.BN = PAIR ? 256 : A_T ? (g.N > 128 ? 256 : g.N > 64 ? 128 : 64) : lt_bn(g.M, g.N, g.splits);
     a.nb = (int)((g.N + a.BN - 1) / a.BN);
-    const int64_t items = (g.M + kLtBM - 1) / kLtBM * a.nb * g.splits;
+    constexpr int rows = PAIR ? 2 * kLtBM : kLtBM;
+    const int64_t items = (g.M + rows - 1) / rows * a.nb * g.splits;
     SPCONV_REQUIRE(items < (int64_t)1 << 30, SPCONV_ERR_ARG, "too many output tiles");
     a.items = (int)items;
     a.tiles = a.items / g.splits;
@@ -476,60 +538,75 @@ static int lt_launch(const GemmArgs &g) {
     a.status = g.status;
     a.wait_ns = wait_limit_ns();
     const int sms = lt_sms();
-    int grid = std::min(sms, a.items);
+    int grid = PAIR ? 2 * std::min(sms / 2, a.items) : std::min(sms, a.items);
     const int64_t nk = (g.K + kLtBK - 1) / kLtBK;
-    const int b_bytes = a.BN * 128, room = kLtMaxSmem - 1024 - kLtTail - a.bias_smem * 4;
-    auto fit = [&](int resident) {          // output slots and stages beside `resident` K steps of B
+    const int b_bytes = (PAIR ? a.BN / 2 : a.BN) * 128, room = kLtMaxSmem - 1024 - kLtTail - a.bias_smem * 4;
+    // output slots and stages beside `resident` K steps of B: four stages at least where that is
+    // possible at all, then as many slots as fit
+    auto fit = [&](int resident) {
         const int stage = kLtABytes + (resident ? 0 : b_bytes);
-        for (int slots = A_T ? 1 : 4; slots >= 1; slots >>= 1) {
-            const int out = A_T ? 0 : kLtEpiWarps * slots * (a.has_preact ? 2 : 1) * kLtSlot;
-            const int stages = (room - resident * b_bytes - out) / stage;
-            if (stages >= 4 || (slots == 1 && stages >= 3)) {
+        for (int least = 4; least >= 3; --least)
+            for (int slots = 4; slots >= 1; slots >>= 1) {
+                const int out = A_T ? 0 : kLtEpiWarps * slots * (a.has_preact ? 2 : 1) * 64 * CH;
+                const int stages = (room - resident * b_bytes - out) / stage;
+                if (stages < least) continue;
                 a.slots = slots;
                 a.stages = std::min(stages, kLtMaxStages);
                 a.b_resident = resident;
                 return true;
             }
-        }
         return false;
     };
     // B stays where a CTA meets it again (more than one row tile per CTA) and its block fits
-    const bool stay = !A_T && a.nb <= sms && a.items > grid && nk * b_bytes <= 96 * 1024 && fit((int)nk);
+    const bool stay = !A_T && !PAIR && a.nb <= sms && a.items > grid && nk * b_bytes <= 96 * 1024 && fit((int)nk);
     if (stay) grid = sms / a.nb * a.nb;
     else if (!fit(0)) {
+        if constexpr (CH == 64 && !A_T) return lt_launch<T, A_T, B_T, ACT, PAIR, 32>(g);
         set_error("linear: no shared-memory layout for this shape");
         return SPCONV_ERR_UNSUPPORTED;
     }
     const int smem = 1024 + kLtTail + a.bias_smem * 4 + a.b_resident * b_bytes + a.stages * (kLtABytes + (a.b_resident ? 0 : b_bytes)) +
-                     (A_T ? 0 : kLtEpiWarps * a.slots * (a.has_preact ? 2 : 1) * kLtSlot);
-    auto kern = linear_tc_kernel<T, A_T, B_T, ACT>;
+                     (A_T ? 0 : kLtEpiWarps * a.slots * (a.has_preact ? 2 : 1) * 64 * CH);
+    auto kern = linear_tc_kernel<T, A_T, B_T, ACT, PAIR, CH>;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kLtMaxSmem) != cudaSuccess)
         return check_launch("linear_tc: set max dynamic shared memory");
     CUtensorMap ma, mb, mo, mr, mp;
     // K-contiguous operands: boxes of 64 K x rows; the others: 64 columns x 64 K rows
     const bool maps =
         (A_T ? make_tmap_2d(&ma, g.a, g.M, g.K, g.M * 2, 64, 64) : make_tmap_2d(&ma, g.a, g.K, g.M, g.K * 2, 64, kLtBM)) &&
-        (B_T ? make_tmap_2d(&mb, g.b, g.N, g.K, g.N * 2, 64, 64) : make_tmap_2d(&mb, g.b, g.K, g.N, g.K * 2, 64, a.BN)) &&
-        (A_T || make_tmap_2d(&mo, g.out, g.N, g.M, g.N * 2, 64, 32)) &&
-        (!g.residual || make_tmap_2d(&mr, g.residual, g.N, g.M, g.N * 2, 64, 32)) &&
-        (!g.preact || make_tmap_2d(&mp, g.preact, g.N, g.M, g.N * 2, 64, 32));
+        (B_T ? make_tmap_2d(&mb, g.b, g.N, g.K, g.N * 2, 64, 64) : make_tmap_2d(&mb, g.b, g.K, g.N, g.K * 2, 64, PAIR ? a.BN / 2 : a.BN)) &&
+        (A_T || make_tmap_2d(&mo, g.out, g.N, g.M, g.N * 2, CH, 32)) &&
+        (!g.residual || make_tmap_2d(&mr, g.residual, g.N, g.M, g.N * 2, CH, 32)) &&
+        (!g.preact || make_tmap_2d(&mp, g.preact, g.N, g.M, g.N * 2, CH, 32));
     if (!maps) return SPCONV_ERR_CUDA;
     if (A_T) mo = ma;                       // maps that the kernel does not read
     if (!g.residual) mr = ma;
     if (!g.preact) mp = ma;
-    kern<<<(unsigned)grid, kLtThreads, smem, g.stream>>>(ma, mb, mo, mr, mp, a);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3(kLtThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = g.stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim = {2, 1, 1};
+    cfg.attrs = attr;
+    cfg.numAttrs = PAIR ? 1 : 0;
+    cudaLaunchKernelEx(&cfg, kern, ma, mb, mo, mr, mp, a);
     return check_launch("linear_tc_kernel");
 }
 
-template <typename T>
+template <typename T, bool PAIR>
 static int lt_type(const GemmArgs &g) {
-    if (g.a_t) return lt_launch<T, true, true, SPCONV_ACT_NONE>(g);
-    if (g.b_t) return lt_launch<T, false, true, SPCONV_ACT_NONE>(g);
-    return act_dispatch(g.activation, [&](auto act) { return lt_launch<T, false, false, act.value>(g); });
+    constexpr int CH = PAIR ? 32 : 64;       // a pair's accumulators leave faster than they fill either way
+    if (g.a_t) return lt_launch<T, true, true, SPCONV_ACT_NONE, PAIR, CH>(g);
+    if (g.b_t) return lt_launch<T, false, true, SPCONV_ACT_NONE, PAIR, CH>(g);
+    return act_dispatch(g.activation, [&](auto act) { return lt_launch<T, false, false, act.value, PAIR, CH>(g); });
 }
 
 int launch_gemm_tc(const GemmArgs &g) {
-    return g.dtype == SPCONV_F16 ? lt_type<__half>(g) : lt_type<__nv_bfloat16>(g);
+    if (lt_pair(g)) return g.dtype == SPCONV_F16 ? lt_type<__half, true>(g) : lt_type<__nv_bfloat16, true>(g);
+    return g.dtype == SPCONV_F16 ? lt_type<__half, false>(g) : lt_type<__nv_bfloat16, false>(g);
 }
 
 }  // namespace spconv

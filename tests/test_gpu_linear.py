@@ -327,3 +327,19 @@ def test_first_call_of_a_thread(M):
     assert len(got) == 2
     torch.cuda.synchronize()
     assert all(torch.equal(a, c) for a, c in zip(got[0], want)) and torch.equal(got[1], out)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("act,residual", [("none", False), ("gelu", True)])
+@pytest.mark.parametrize("M,Ci,Co", [(20000, 512, 520), (19001, 1024, 264), (9473, 520, 1032), (10000, 648, 512)])
+def test_tiles_over_two_sms(M, Ci, Co, dtype, act, residual):
+    """Many rows and channels: pairs of CTAs, with ragged last tiles in both directions."""
+    x, w, b, r, g = _inputs(M, Ci, Co, DT[dtype], residual=residual, seed=31)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    out = sparse_linear(x, w, b, residual=r, activation=act)
+    grads = torch.autograd.grad(out, leaves, g)
+    x, w, b = x.detach(), w.detach(), b.detach()
+    v, e, _, _ = _forward_ref(x, w, b, r, act)
+    _check(out.detach(), v, e, DT[dtype], "out")
+    for got, ref, what in zip(grads, _backward_ref(x, w, b, g, act, DT[dtype]), ("feats", "weight", "bias")):
+        _check(got, *ref, DT[dtype], what)
