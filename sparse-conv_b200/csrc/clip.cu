@@ -9,9 +9,12 @@
 // is copied to the device and a captured graph needs no memory of the host's; lists longer than
 // one parameter block holds take several launches of each.
 //
-// Bound: HBM, one read for the norm and one read and write for the scaling; the second pass
-// walks the chunks in the opposite order, so what the first left in the L2 is read from there.
-// Where nothing is clipped and the output is the gradient itself, nothing is moved.
+// The elements of all tensors, in eights, are cut into one range per block, and a block walks its
+// range with four 16-byte loads a thread in flight, looking up a tensor only where one ends.
+//
+// Bound: HBM, one read for the norm and one read and write for the scaling; the second pass walks
+// each range backwards, so what the first left in the L2 is read from there. Where nothing is
+// clipped and the output is the gradient itself, nothing is moved.
 //
 // Squares are added in fp32 eight at a time and the eights in fp64. An eight whose fp32 sum
 // left the range in which squares are exact to fp32's precision (over 1e30, or under 1e-30) is
@@ -24,7 +27,6 @@
 namespace spconv {
 
 constexpr int kClThreads = 256;
-constexpr int64_t kClChunk = 8192;           // elements a block takes at a time
 constexpr int kClMaxBlocks = 148 * 6;
 
 // K tensors in one launch's parameters.
@@ -33,7 +35,7 @@ struct ClTable {
     const void *grad[K];
     void *out[K];
     int64_t numel[K];
-    int64_t first_chunk[K + 1];              // chunks of the tensors before it
+    int64_t first[K + 1];                    // eights of elements in the tensors before it
     uint8_t dtype[K];
     int n;
 };
@@ -45,15 +47,23 @@ struct ClArgs {
     float *total;
 };
 
+// The tensor that holds eight number e.
 template <int K>
-__device__ __forceinline__ int cl_find(const ClTable<K> &t, int64_t chunk) {
+__device__ __forceinline__ int cl_find(const ClTable<K> &t, int64_t e) {
     int lo = 0, hi = t.n - 1;
-    while (lo < hi) {                        // last tensor with first_chunk <= chunk
+    while (lo < hi) {                        // last tensor with first <= e
         const int mid = (lo + hi + 1) >> 1;
-        if (t.first_chunk[mid] <= chunk) lo = mid;
+        if (t.first[mid] <= e) lo = mid;
         else hi = mid - 1;
     }
     return lo;
+}
+// This block's range of eights.
+template <int K>
+__device__ __forceinline__ void cl_range(const ClTable<K> &t, int64_t &e0, int64_t &e1) {
+    const int64_t per = (t.first[t.n] + gridDim.x - 1) / gridDim.x;
+    e0 = min(t.first[t.n], blockIdx.x * per);
+    e1 = min(t.first[t.n], e0 + per);
 }
 
 template <typename T>
@@ -121,33 +131,32 @@ __device__ __forceinline__ void cl_norm_chunk(const T *g, int n, bool largest, d
     }
 }
 
+// Backwards: the end of the part was read last by the norm.
 template <typename T>
 __device__ __forceinline__ void cl_scale_chunk(const T *g, T *out, int n, float coef) {
-    constexpr int V = 16 / sizeof(T);
+    constexpr int V = 16 / sizeof(T), kBatch = 4 * kClThreads;
     int done = 0;
-    if ((((uintptr_t)g | (uintptr_t)out) & 15) == 0) {
-        const int vecs = n / V;
-        const uint4 *q = reinterpret_cast<const uint4 *>(g);
-        uint4 *o = reinterpret_cast<uint4 *>(out);
-        auto scale = [&](uint4 v) {
-            T *x = reinterpret_cast<T *>(&v);
-#pragma unroll
-            for (int i = 0; i < V; ++i) x[i] = dtype_traits<T>::from_f(dtype_traits<T>::to_f(x[i]) * coef);
-            return v;
-        };
-        int e = threadIdx.x;
-        for (; e + 3 * kClThreads < vecs; e += 4 * kClThreads) {
-            uint4 v[4];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) v[u] = q[e + u * kClThreads];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) __stcs(o + e + u * kClThreads, scale(v[u]));
-        }
-        for (; e < vecs; e += kClThreads) __stcs(o + e, scale(q[e]));
-        done = vecs * V;
-    }
+    if ((((uintptr_t)g | (uintptr_t)out) & 15) == 0) done = n / V * V;
     for (int i = done + threadIdx.x; i < n; i += kClThreads)
         out[i] = dtype_traits<T>::from_f(dtype_traits<T>::to_f(g[i]) * coef);
+    const int vecs = done / V, batches = vecs / kBatch;
+    const uint4 *q = reinterpret_cast<const uint4 *>(g);
+    uint4 *o = reinterpret_cast<uint4 *>(out);
+    auto scale = [&](uint4 v) {
+        T *x = reinterpret_cast<T *>(&v);
+#pragma unroll
+        for (int i = 0; i < V; ++i) x[i] = dtype_traits<T>::from_f(dtype_traits<T>::to_f(x[i]) * coef);
+        return v;
+    };
+    for (int e = batches * kBatch + threadIdx.x; e < vecs; e += kClThreads) __stcs(o + e, scale(__ldcs(q + e)));
+    for (int b = batches - 1; b >= 0; --b) {
+        const int e = b * kBatch + threadIdx.x;
+        uint4 v[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) v[u] = __ldcs(q + e + u * kClThreads);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) __stcs(o + e + u * kClThreads, scale(v[u]));
+    }
 }
 
 // The sum (or the largest) of one value per thread, the same bits in every run.
@@ -170,14 +179,15 @@ clip_norm_kernel(const __grid_constant__ ClTable<K> t, const __grid_constant__ C
     double sum = 0.0;
     uint32_t top = 0;
     const bool largest = a.max_norm_kind != 0;
-    const int64_t chunks = t.first_chunk[t.n];
-    for (int64_t c = blockIdx.x; c < chunks; c += gridDim.x) {
-        const int k = cl_find(t, c);
-        const int64_t at = (c - t.first_chunk[k]) * kClChunk;
-        const int n = (int)min(kClChunk, t.numel[k] - at);
+    int64_t e, end;
+    cl_range(t, e, end);
+    for (int k = e < end ? cl_find(t, e) : 0; e < end; ++k) {
+        const int64_t at = (e - t.first[k]) * 8, stop = min(end, t.first[k + 1]);
+        const int n = (int)(min(t.numel[k], (stop - t.first[k]) * 8) - at);
         if (t.dtype[k] == SPCONV_F32) cl_norm_chunk((const float *)t.grad[k] + at, n, largest, sum, top);
         else if (t.dtype[k] == SPCONV_F16) cl_norm_chunk((const __half *)t.grad[k] + at, n, largest, sum, top);
         else cl_norm_chunk((const __nv_bfloat16 *)t.grad[k] + at, n, largest, sum, top);
+        e = stop;
     }
     const double v = cl_block_reduce(largest ? (double)__uint_as_float(top) : sum, largest);
     if (threadIdx.x == 0) a.partial[a.first_partial + blockIdx.x] = v;
@@ -198,13 +208,13 @@ clip_scale_kernel(const __grid_constant__ ClTable<K> t, const __grid_constant__ 
     if (a.total && blockIdx.x == 0 && threadIdx.x == 0) *a.total = (float)total;
     const double ratio = (double)a.max_norm / (total + 1e-6);
     const float coef = ratio >= 1.0 ? 1.f : (float)ratio;     // NaN stays NaN
-    const int64_t chunks = t.first_chunk[t.n];
-    for (int64_t b = blockIdx.x; b < chunks; b += gridDim.x) {
-        const int64_t c = chunks - 1 - b;                     // what was read last comes first
-        const int k = cl_find(t, c);
+    int64_t begin, e;
+    cl_range(t, begin, e);
+    for (int k = begin < e ? cl_find(t, e - 1) : 0; e > begin; --k) {
+        const int64_t start = max(begin, t.first[k]), at = (start - t.first[k]) * 8;
+        const int n = (int)(min(t.numel[k], (e - t.first[k]) * 8) - at);
+        e = start;
         if (coef == 1.f && t.out[k] == t.grad[k]) continue;
-        const int64_t at = (c - t.first_chunk[k]) * kClChunk;
-        const int n = (int)min(kClChunk, t.numel[k] - at);
         if (t.dtype[k] == SPCONV_F32) cl_scale_chunk((const float *)t.grad[k] + at, (float *)t.out[k] + at, n, coef);
         else if (t.dtype[k] == SPCONV_F16) cl_scale_chunk((const __half *)t.grad[k] + at, (__half *)t.out[k] + at, n, coef);
         else cl_scale_chunk((const __nv_bfloat16 *)t.grad[k] + at, (__nv_bfloat16 *)t.out[k] + at, n, coef);
@@ -217,7 +227,8 @@ struct ClRange {
     bool operator<(const ClRange &o) const { return lo < o.lo; }
 };
 
-static int cl_blocks(int64_t chunks) { return (int)std::max<int64_t>(1, std::min<int64_t>(kClMaxBlocks, chunks)); }
+// A block per 512 eights, up to six blocks per SM; ranges of 2^28 eights are beyond any memory.
+static int cl_blocks(int64_t eights) { return (int)std::max<int64_t>(1, std::min<int64_t>(kClMaxBlocks, (eights + 511) / 512)); }
 
 template <int K>
 static int cl_run(const void *const *grads, void *const *outs, const int64_t *numels, const int32_t *dtypes,
@@ -227,19 +238,19 @@ static int cl_run(const void *const *grads, void *const *outs, const int64_t *nu
     for (size_t i = 0; i < live.size(); ++i) {
         ClTable<K> &t = tables[i / K];
         const int j = (int)(i % K), k = live[i];
-        if (j == 0) t.first_chunk[0] = 0;
+        if (j == 0) t.first[0] = 0;
         t.grad[j] = grads[k];
         t.out[j] = outs[k];
         t.numel[j] = numels[k];
         t.dtype[j] = (uint8_t)dtypes[k];
-        t.first_chunk[j + 1] = t.first_chunk[j] + (numels[k] + kClChunk - 1) / kClChunk;
+        t.first[j + 1] = t.first[j] + (numels[k] + 7) / 8;
         t.n = j + 1;
     }
-    for (const auto &t : tables) partials += cl_blocks(t.first_chunk[t.n]);
+    for (const auto &t : tables) partials += cl_blocks(t.first[t.n]);
     a.num_partials = partials;
     a.first_partial = 0;
     for (const auto &t : tables) {
-        const int blocks = cl_blocks(t.first_chunk[t.n]);
+        const int blocks = cl_blocks(t.first[t.n]);
         clip_norm_kernel<K><<<blocks, kClThreads, 0, st>>>(t, a);
         if (const int rc = check_launch("clip_norm_kernel")) return rc;
         a.first_partial += blocks;
@@ -248,7 +259,7 @@ static int cl_run(const void *const *grads, void *const *outs, const int64_t *nu
     // launch, which follows the last norm launch, may start under it
     bool first = true;
     for (const auto &t : tables) {
-        const int blocks = cl_blocks(t.first_chunk[t.n]);
+        const int blocks = cl_blocks(t.first[t.n]);
         if (first) launch_pdl(clip_scale_kernel<K>, dim3(blocks), dim3(kClThreads), 0, st, t, a);
         else clip_scale_kernel<K><<<blocks, kClThreads, 0, st>>>(t, a);
         if (const int rc = check_launch("clip_scale_kernel")) return rc;

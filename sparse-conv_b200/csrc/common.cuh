@@ -3,6 +3,7 @@
 // the async-proxy fence and the tcgen05 (5th-generation tensor core / TMEM) instructions.
 #pragma once
 
+#include <atomic>
 #include <cstdint>
 #include <cuda_runtime.h>
 #include <cuda_fp16.h>
@@ -27,6 +28,20 @@ void stage_mark(int stage, int which, cudaStream_t stream);
             return (code);                \
         }                                 \
     } while (0)
+
+// Allows `kern` up to `bytes` of dynamic shared memory on the current device; the attribute is set
+// once for each kernel and device (`done`: a static of the caller's, one bit a device).
+template <typename K>
+inline cudaError_t allow_smem(K kern, int bytes, std::atomic<uint64_t> &done) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = 1ull << (dev & 63);
+    if (dev < 64 && (done.load(std::memory_order_relaxed) & bit)) return cudaSuccess;
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    return e;
+}
 
 // ---------------------------------------------------------------------------------------
 // Device-side status: kernels OR bits into a caller-provided int32 word.

@@ -330,7 +330,8 @@ static int lb_launch(const BwdArgs &q) {
     const int cols = (a.co_blocks / 2 + 2) * a.ci_blocks * 64;
     a.tmem_cols = cols <= 256 ? 256 : 512;
     auto kern = linear_bwd_tc_kernel<T, ACT>;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kLbMaxSmem) != cudaSuccess)
+    static std::atomic<uint64_t> set{0};
+    if (allow_smem(kern, kLbMaxSmem, set) != cudaSuccess)
         return check_launch("linear_bwd_tc: set max dynamic shared memory");
     CUtensorMap mg, mz, mx, mw, mo;
     const bool maps = make_tmap_2d(&mg, q.grad_out, q.Co, q.M, (uint64_t)q.Co * 2, 64, kLbRows) &&

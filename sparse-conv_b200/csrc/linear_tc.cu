@@ -568,7 +568,8 @@ static int lt_launch(const GemmArgs &g) {
     const int smem = 1024 + kLtTail + a.bias_smem * 4 + a.b_resident * b_bytes + a.stages * (kLtABytes + (a.b_resident ? 0 : b_bytes)) +
                      (A_T ? 0 : kLtEpiWarps * a.slots * (a.has_preact ? 2 : 1) * 64 * CH);
     auto kern = linear_tc_kernel<T, A_T, B_T, ACT, PAIR, CH>;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kLtMaxSmem) != cudaSuccess)
+    static std::atomic<uint64_t> set{0};
+    if (allow_smem(kern, kLtMaxSmem, set) != cudaSuccess)
         return check_launch("linear_tc: set max dynamic shared memory");
     CUtensorMap ma, mb, mo, mr, mp;
     // K-contiguous operands: boxes of 64 K x rows; the others: 64 columns x 64 K rows

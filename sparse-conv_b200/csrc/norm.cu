@@ -1174,7 +1174,8 @@ static bool rb_launch(RnArgs &a, cudaStream_t st, int &rc) {
     const int grid = (int)((a.M + a.chunk - 1) / a.chunk);
     const int smem = extra + rb.stages * stage;
     auto kern = residual_norm_bulk_kernel<T, VEC, VPT, BWD, FULL, W, U>;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kRbMaxSmem) != cudaSuccess) {
+    static std::atomic<uint64_t> set{0};
+    if (allow_smem(kern, kRbMaxSmem, set) != cudaSuccess) {
         rc = check_launch("residual_norm_bulk: set max dynamic shared memory");
         return true;
     }

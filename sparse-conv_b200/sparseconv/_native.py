@@ -19,6 +19,7 @@ from __future__ import annotations
 import array
 import ctypes
 import functools
+import operator
 import os
 import threading
 from typing import Optional, Sequence, Tuple
@@ -890,6 +891,11 @@ def residual_norm_backward(feats: torch.Tensor, residual: Optional[torch.Tensor]
     return grads
 
 
+_data_ptr, _numel, _get_device, _is_contiguous = (
+    getattr(torch.Tensor, name) for name in ("data_ptr", "numel", "get_device", "is_contiguous"))
+_dtype = operator.attrgetter("dtype")
+
+
 def _is_dense(t: torch.Tensor) -> bool:
     """Whether the elements fill their memory without gaps or overlap, in any order of dimensions."""
     if t.is_contiguous():
@@ -904,24 +910,28 @@ def clip_gradients(grads: Sequence[torch.Tensor], outs: Sequence[torch.Tensor], 
     """outs[k] = grads[k] * min(1, max_norm / (norm + 1e-6)); returns the norm (0-dim float32)."""
     lib = load_library()
     dev, index = grads[0].device, grads[0].get_device()
-    ptrs, optrs, sizes, codes = [], [], [], []
-    for g, o in zip(grads, outs):
-        if g.get_device() != index or (o is not g and o.get_device() != index) or index < 0:
-            _require_cuda(*grads, *outs)
-        code = DTYPE_CODES.get(g.dtype)
-        if code is None:
-            raise TypeError(f"unsupported gradient dtype {g.dtype}")
-        dense = g.is_contiguous()
-        if o is not g and (o.dtype != g.dtype or o.shape != g.shape or
-                           not (dense and o.is_contiguous() or o.stride() == g.stride())):
-            raise ValueError("each output must have its gradient's shape, strides and dtype")
-        if not dense and not _is_dense(g):
-            raise ValueError("gradients must be dense in memory")
-        ptrs.append(g.data_ptr())
-        optrs.append(o.data_ptr())
-        sizes.append(g.numel())
-        codes.append(code)
-    n = len(ptrs)
+    n = len(grads)
+    # whole lists at a time: a network has hundreds of gradients
+    ptrs, sizes, dtypes = (list(map(f, grads)) for f in (_data_ptr, _numel, _dtype))
+    where = set(map(_get_device, grads))
+    optrs = ptrs
+    if outs is not grads:
+        optrs = list(map(_data_ptr, outs))
+        where.update(map(_get_device, outs))
+        if list(map(_numel, outs)) != sizes or list(map(_dtype, outs)) != dtypes:
+            raise ValueError("each output must have its gradient's size and dtype")
+    if where != {index} or index < 0:
+        _require_cuda(*grads, *outs)
+    if not (all(map(_is_contiguous, grads)) and (outs is grads or all(map(_is_contiguous, outs)))):
+        for g, o in zip(grads, outs):
+            if not _is_dense(g):
+                raise ValueError("gradients must be dense in memory")
+            if o.stride() != g.stride() and not (g.is_contiguous() and o.is_contiguous()):
+                raise ValueError("each output must have its gradient's strides")
+    try:
+        codes = [DTYPE_CODES[d] for d in dtypes]
+    except KeyError as e:
+        raise TypeError(f"unsupported gradient dtype {e.args[0]}") from None
     ptrs, optrs, sizes, codes = (array.array(t, v) for t, v in (("Q", ptrs), ("Q", optrs), ("q", sizes), ("i", codes)))
     total = torch.empty((), dtype=torch.float32, device=dev)
     need = lib.spconv_clip_gradients_workspace_bytes(n)

@@ -20,7 +20,6 @@ def _norm_kind(norm_type: float) -> int:
     raise ValueError(f"norm_type must be 2 or inf, got {norm_type}")
 
 
-@torch.no_grad()
 def clip_gradients(grads: Sequence[torch.Tensor], max_norm: float, norm_type: float = 2.0,
                    out: Optional[Sequence[torch.Tensor]] = None) -> torch.Tensor:
     """out[k] = grads[k] * min(1, max_norm / (total + 1e-6)), total the norm of all gradients as
@@ -31,7 +30,7 @@ def clip_gradients(grads: Sequence[torch.Tensor], max_norm: float, norm_type: fl
             list is not empty.
         max_norm: largest norm the result may have, >= 0.
         norm_type: 2.0 (square root of the sum of squares) or inf (largest magnitude).
-        out: tensors of the gradients' shapes, strides and dtypes; None clips in place. Outputs
+        out: tensors of the gradients' sizes and dtypes, laid out alike; None clips in place. Outputs
             may not share memory with one another or with other gradients, so in place a tensor
             may not be listed twice.
 
