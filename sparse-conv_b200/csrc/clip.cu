@@ -10,7 +10,7 @@
 // one parameter block holds take several launches of each.
 //
 // The elements of all tensors, in eights, are cut into one range per block, and a block walks its
-// range with four 16-byte loads a thread in flight, looking up a tensor only where one ends.
+// range with eight 16-byte loads a thread in flight, looking up a tensor only where one ends.
 //
 // Bound: HBM, one read for the norm and one read and write for the scaling; the second pass walks
 // each range backwards, so what the first left in the L2 is read from there. Where nothing is
@@ -27,7 +27,9 @@
 namespace spconv {
 
 constexpr int kClThreads = 256;
-constexpr int kClMaxBlocks = 148 * 6;
+constexpr int kClBlocksPerSm = 4;            // all resident at 64 registers: one wave
+constexpr int kClMaxBlocks = 148 * kClBlocksPerSm;
+constexpr int kClBatch = 8;                  // 16-byte loads a thread has in flight
 
 // K tensors in one launch's parameters.
 template <int K>
@@ -103,14 +105,15 @@ __device__ __forceinline__ void cl_norm_chunk(const T *g, int n, bool largest, d
         const int eights = n / 8;
         const uint4 *q = reinterpret_cast<const uint4 *>(g);
         int e = threadIdx.x;
-        for (; e + 3 * kClThreads < eights; e += 4 * kClThreads) {
-            uint4 v[4][R];
+        constexpr int B = kClBatch / R;
+        for (; e + (B - 1) * kClThreads < eights; e += B * kClThreads) {
+            uint4 v[B][R];
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
+            for (int u = 0; u < B; ++u)
 #pragma unroll
                 for (int r = 0; r < R; ++r) v[u][r] = __ldg(q + (e + u * kClThreads) * R + r);
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
+            for (int u = 0; u < B; ++u) {
                 float f[8];
 #pragma unroll
                 for (int r = 0; r < R; ++r) cl_unpack16<T>(v[u][r], f + r * V);
@@ -134,7 +137,7 @@ __device__ __forceinline__ void cl_norm_chunk(const T *g, int n, bool largest, d
 // Backwards: the end of the part was read last by the norm.
 template <typename T>
 __device__ __forceinline__ void cl_scale_chunk(const T *g, T *out, int n, float coef) {
-    constexpr int V = 16 / sizeof(T), kBatch = 4 * kClThreads;
+    constexpr int V = 16 / sizeof(T), kBatch = kClBatch * kClThreads;
     int done = 0;
     if ((((uintptr_t)g | (uintptr_t)out) & 15) == 0) done = n / V * V;
     for (int i = done + threadIdx.x; i < n; i += kClThreads)
@@ -151,11 +154,11 @@ __device__ __forceinline__ void cl_scale_chunk(const T *g, T *out, int n, float 
     for (int e = batches * kBatch + threadIdx.x; e < vecs; e += kClThreads) __stcs(o + e, scale(__ldcs(q + e)));
     for (int b = batches - 1; b >= 0; --b) {
         const int e = b * kBatch + threadIdx.x;
-        uint4 v[4];
+        uint4 v[kClBatch];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) v[u] = __ldcs(q + e + u * kClThreads);
+        for (int u = 0; u < kClBatch; ++u) v[u] = __ldcs(q + e + u * kClThreads);
 #pragma unroll
-        for (int u = 0; u < 4; ++u) __stcs(o + e + u * kClThreads, scale(v[u]));
+        for (int u = 0; u < kClBatch; ++u) __stcs(o + e + u * kClThreads, scale(v[u]));
     }
 }
 
@@ -173,7 +176,7 @@ __device__ __forceinline__ double cl_block_reduce(double v, bool largest) {
 }
 
 template <int K>
-__global__ void __launch_bounds__(kClThreads)
+__global__ void __launch_bounds__(kClThreads, kClBlocksPerSm)
 clip_norm_kernel(const __grid_constant__ ClTable<K> t, const __grid_constant__ ClArgs a) {
     grid_launch_dependents();
     double sum = 0.0;
@@ -194,7 +197,7 @@ clip_norm_kernel(const __grid_constant__ ClTable<K> t, const __grid_constant__ C
 }
 
 template <int K>
-__global__ void __launch_bounds__(kClThreads)
+__global__ void __launch_bounds__(kClThreads, kClBlocksPerSm)
 clip_scale_kernel(const __grid_constant__ ClTable<K> t, const __grid_constant__ ClArgs a) {
     grid_dependency_wait();
     const bool largest = a.max_norm_kind != 0;
@@ -227,7 +230,7 @@ struct ClRange {
     bool operator<(const ClRange &o) const { return lo < o.lo; }
 };
 
-// A block per 512 eights, up to six blocks per SM; ranges of 2^28 eights are beyond any memory.
+// A block per 512 eights, up to four blocks per SM; ranges of 2^28 eights are beyond any memory.
 static int cl_blocks(int64_t eights) { return (int)std::max<int64_t>(1, std::min<int64_t>(kClMaxBlocks, (eights + 511) / 512)); }
 
 template <int K>
