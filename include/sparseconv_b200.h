@@ -291,14 +291,20 @@ int spconv_submanifold_conv_weight_grad(
  *   kernel_choice: SPCONV_KERNEL_*; SPCONV_KERNEL_TCGEN05 returns SPCONV_ERR_UNSUPPORTED where the
  *   tensor-core kernel does not apply (fp32, channel counts that are no multiple of 8, pointers
  *   not aligned to 16 bytes)
+ *   workspace: 256-byte aligned, spconv_linear_forward_workspace_bytes(...) bytes; 0 for most shapes,
+ *   more for 16-bit channel counts that are no multiple of 8 where copies into whole rows let the
+ *   tensor cores run; with NULL the CUDA-core kernel takes those
  * No counterpart in the reference (its networks would call torch for this layer). */
 #define SPCONV_ACT_NONE 0
 #define SPCONV_ACT_RELU 1
 #define SPCONV_ACT_GELU 2             /* x * Phi(x), Phi the normal distribution function */
 #define SPCONV_ACT_SILU 3             /* x / (1 + exp(-x)) */
+int64_t spconv_linear_forward_workspace_bytes(int dtype, int64_t num_rows, int Ci, int Co, int has_residual,
+                                              int has_preact);
 int spconv_linear_forward(const void *feats, int dtype, int64_t num_rows, int Ci, const void *weight,
                           const void *bias, const void *residual, int Co, int activation,
-                          void *out, void *preact, int kernel_choice, int32_t *status, void *stream);
+                          void *out, void *preact, void *workspace, int64_t workspace_bytes,
+                          int kernel_choice, int32_t *status, void *stream);
 
 /* Gradients of spconv_linear_forward, with dz = grad_out * act'(preact) rounded to `dtype`:
  *   grad_feats[i, ci] = sum_co dz[i, co] * weight[co, ci]

@@ -319,16 +319,71 @@ static int launch_gemm(const GemmArgs &g, int kernel_choice) {
     return launch_gemm_simt(g);
 }
 
-}  // namespace spconv
+// ---------------------------------------------------------------------------------------
+// Channel counts that are no multiple of 8, 16-bit: TMA needs rows a multiple of 16 bytes apart, so the
+// operands are copied into rows of whole eights (zeros behind) and the results out of such rows,
+// where the tensor cores then save more than the copies cost: about 15 TFLOP/s of the CUDA-core kernel
+// at such widths against 4 TB/s of copying and 15 us of launches. Measured in bf16, forward and
+// backward, CUDA cores and here: 15,000 x 1001 -> 517 625 and 76, 1558 and 191 us; 20,000 x 257 -> 131 91
+// and 41, 251 and 87 us.
+// ---------------------------------------------------------------------------------------
+static int up8(int c) { return (c + 7) & ~7; }
 
-using namespace spconv;
+bool linear_padded(int dtype, int64_t M, int Ci, int Co) {
+    if ((dtype != SPCONV_F16 && dtype != SPCONV_BF16) || (Ci % 8 == 0 && Co % 8 == 0)) return false;
+    const double cuda_cores = 2.0 * Ci * Co / 15e12, copies = (4.0 * up8(Ci) + 6.0 * up8(Co)) / 4e12;
+    return M * (cuda_cores - copies) > 15e-6;
+}
 
-extern "C" int spconv_linear_forward(const void *feats, int dtype, int64_t M, int Ci, const void *weight,
-                                     const void *bias, const void *residual, int Co, int activation, void *out,
-                                     void *preact, int kernel_choice, int32_t *status, void *stream) {
-    if (const int rc = check_linear(dtype, M, Ci, Co, activation, kernel_choice)) return rc;
-    if (M == 0) return SPCONV_OK;
-    SPCONV_REQUIRE(feats && weight && out, SPCONV_ERR_ARG, "null pointer argument");
+// dst [rows, dst_cols] = src [rows, src_cols] of 16-bit (or 32-bit) values, cut off or with zeros behind.
+template <typename V>
+__global__ void __launch_bounds__(256)
+linear_repitch_kernel(const V *__restrict__ src, int src_cols, V *__restrict__ dst, int dst_cols, int64_t rows) {
+    const int64_t n = rows * dst_cols, step = (int64_t)gridDim.x * blockDim.x;
+    int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    int64_t r = i / dst_cols;
+    int c = (int)(i - r * dst_cols);
+    const int64_t dr = step / dst_cols;
+    const int dc = (int)(step - dr * dst_cols);
+    for (; i < n; i += step) {
+        dst[i] = c < src_cols ? src[r * src_cols + c] : V(0);
+        r += dr;
+        c += dc;
+        if (c >= dst_cols) {
+            c -= dst_cols;
+            ++r;
+        }
+    }
+}
+
+static int launch_repitch(const void *src, int src_cols, void *dst, int dst_cols, int64_t rows, int bytes, cudaStream_t st) {
+    const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>(148 * 16, (rows * dst_cols + 1023) / 1024));
+    if (bytes == 2) linear_repitch_kernel<uint16_t><<<grid, 256, 0, st>>>((const uint16_t *)src, src_cols, (uint16_t *)dst, dst_cols, rows);
+    else linear_repitch_kernel<uint32_t><<<grid, 256, 0, st>>>((const uint32_t *)src, src_cols, (uint32_t *)dst, dst_cols, rows);
+    return check_launch("linear_repitch_kernel");
+}
+
+static int64_t padded_forward_bytes(int64_t M, int Ci, int Co, bool residual, bool preact) {
+    const int64_t pi = up8(Ci), po = up8(Co);
+    return pad256(M * pi * 2) + pad256(po * pi * 2) + pad256(po * 2) + (1 + (residual ? 1 : 0) + (preact ? 1 : 0)) * pad256(M * po * 2);
+}
+
+static int64_t separate_backward_bytes(int dtype, int64_t M, int Ci, int Co, int activation) {
+    const int64_t separate = pad256(activation == SPCONV_ACT_NONE ? 0 : M * Co * elt(dtype)) + pad256((int64_t)dact_chunks(M) * Co * 4) +
+                             pad256((int64_t)std::max(wgrad_splits(M, Ci, Co), gemm_tc_splits(Co, Ci, M)) * Co * Ci * 4);
+    const int64_t grid = bwd_tc_grid(M);
+    return std::max(separate, pad256(grid * 8 * Co * 4) + pad256(grid * Co * Ci * 4));
+}
+
+static int64_t padded_backward_bytes(int dtype, int64_t M, int Ci, int Co, int activation) {
+    const int64_t pi = up8(Ci), po = up8(Co);
+    return 2 * pad256(M * pi * 2) + 2 * pad256(M * po * 2) + pad256(po * pi * 2) + pad256(po * pi * 4) + pad256(po * 4) +
+           separate_backward_bytes(dtype, M, (int)pi, (int)po, activation);
+}
+
+static int linear_forward(const void *feats, int dtype, int64_t M, int Ci, const void *weight, const void *bias,
+                          const void *residual, int Co, int activation, void *out, void *preact, int kernel_choice,
+                          int32_t *status, cudaStream_t st) {
     GemmArgs g = {};
     g.a = feats;
     g.b = weight;
@@ -343,41 +398,14 @@ extern "C" int spconv_linear_forward(const void *feats, int dtype, int64_t M, in
     g.preact = preact;
     g.splits = 1;
     g.status = status;
-    g.stream = (cudaStream_t)stream;
+    g.stream = st;
     return launch_gemm(g, kernel_choice);
 }
 
-extern "C" int64_t spconv_linear_backward_workspace_bytes(int dtype, int64_t M, int Ci, int Co, int activation) {
-    if (check_linear(dtype, M, Ci, Co, activation, SPCONV_KERNEL_AUTO) != SPCONV_OK) return -1;
-    const int64_t separate = pad256(activation == SPCONV_ACT_NONE ? 0 : M * Co * elt(dtype)) + pad256((int64_t)dact_chunks(M) * Co * 4) +
-                             pad256((int64_t)std::max(wgrad_splits(M, Ci, Co), gemm_tc_splits(Co, Ci, M)) * Co * Ci * 4);
-    const int64_t grid = bwd_tc_grid(M);
-    return std::max(separate, pad256(grid * 8 * Co * 4) + pad256(grid * Co * Ci * 4));
-}
-
-extern "C" int spconv_linear_backward(const void *grad_out, const void *preact, const void *feats, const void *weight,
-                                      int dtype, int64_t M, int Ci, int Co, int activation, void *grad_feats,
-                                      void *grad_weight, int weight_dtype, void *grad_bias, int bias_dtype,
-                                      void *workspace, int64_t workspace_bytes, int kernel_choice, int32_t *status,
-                                      void *stream) {
-    if (const int rc = check_linear(dtype, M, Ci, Co, activation, kernel_choice)) return rc;
-    SPCONV_REQUIRE(!grad_weight || weight_dtype == SPCONV_F32 || weight_dtype == dtype, SPCONV_ERR_ARG,
-                   "the weight's gradient is fp32 or of the features' type");
-    SPCONV_REQUIRE(!grad_bias || bias_dtype == SPCONV_F32 || bias_dtype == dtype, SPCONV_ERR_ARG,
-                   "the bias's gradient is fp32 or of the features' type");
-    const cudaStream_t st = (cudaStream_t)stream;
-    if (M == 0) {                            // sums over no rows
-        if (grad_weight && cudaMemsetAsync(grad_weight, 0, (size_t)Co * Ci * elt(weight_dtype), st) != cudaSuccess)
-            return check_launch("linear_backward: clear");
-        if (grad_bias && cudaMemsetAsync(grad_bias, 0, (size_t)Co * elt(bias_dtype), st) != cudaSuccess)
-            return check_launch("linear_backward: clear");
-        return SPCONV_OK;
-    }
-    SPCONV_REQUIRE(grad_out && (preact || activation == SPCONV_ACT_NONE) && (feats || !grad_weight) &&
-                       (weight || !grad_feats), SPCONV_ERR_ARG, "null pointer argument");
-    SPCONV_REQUIRE(workspace && ((uintptr_t)workspace & 255) == 0 &&
-                       workspace_bytes >= spconv_linear_backward_workspace_bytes(dtype, M, Ci, Co, activation),
-                   SPCONV_ERR_ARG, "workspace missing, misaligned or too small");
+static int linear_backward(const void *grad_out, const void *preact, const void *feats, const void *weight, int dtype,
+                           int64_t M, int Ci, int Co, int activation, void *grad_feats, void *grad_weight,
+                           int weight_dtype, void *grad_bias, int bias_dtype, void *workspace, int kernel_choice,
+                           int32_t *status, cudaStream_t st) {
     uint8_t *ws = (uint8_t *)workspace;
     bool aligned = true;
     for (const void *p : {grad_out, preact, feats, weight, (const void *)grad_feats})
@@ -436,4 +464,109 @@ extern "C" int spconv_linear_backward(const void *grad_out, const void *preact, 
     }
     return launch_reduce(reduce_seg(weight_part, g.splits, (int64_t)Co * Ci, weight_dtype, grad_weight),
                          reduce_seg(bias_part, dact_chunks(M), Co, bias_dtype, grad_bias), st);
+}
+
+}  // namespace spconv
+
+using namespace spconv;
+
+extern "C" int64_t spconv_linear_forward_workspace_bytes(int dtype, int64_t M, int Ci, int Co, int has_residual,
+                                                         int has_preact) {
+    if (check_linear(dtype, M, Ci, Co, SPCONV_ACT_NONE, SPCONV_KERNEL_AUTO) != SPCONV_OK) return -1;
+    return linear_padded(dtype, M, Ci, Co) ? padded_forward_bytes(M, Ci, Co, has_residual != 0, has_preact != 0) : 0;
+}
+
+extern "C" int spconv_linear_forward(const void *feats, int dtype, int64_t M, int Ci, const void *weight,
+                                     const void *bias, const void *residual, int Co, int activation, void *out,
+                                     void *preact, void *workspace, int64_t workspace_bytes, int kernel_choice,
+                                     int32_t *status, void *stream) {
+    if (const int rc = check_linear(dtype, M, Ci, Co, activation, kernel_choice)) return rc;
+    if (M == 0) return SPCONV_OK;
+    SPCONV_REQUIRE(feats && weight && out, SPCONV_ERR_ARG, "null pointer argument");
+    const cudaStream_t st = (cudaStream_t)stream;
+    // without the workspace the CUDA-core kernel takes such shapes too
+    if (kernel_choice != SPCONV_KERNEL_AUTO || !workspace || !linear_padded(dtype, M, Ci, Co))
+        return linear_forward(feats, dtype, M, Ci, weight, bias, residual, Co, activation, out, preact, kernel_choice, status, st);
+    SPCONV_REQUIRE(((uintptr_t)workspace & 255) == 0 &&
+                       workspace_bytes >= padded_forward_bytes(M, Ci, Co, residual != nullptr, preact != nullptr),
+                   SPCONV_ERR_ARG, "workspace misaligned or too small");
+    const int pi = up8(Ci), po = up8(Co);
+    uint8_t *ws = (uint8_t *)workspace;
+    auto take = [&](int64_t bytes) {
+        void *p = ws;
+        ws += pad256(bytes);
+        return p;
+    };
+    void *x = take(M * pi * 2), *w = take((int64_t)po * pi * 2), *b = take(po * 2), *y = take(M * po * 2);
+    void *r = residual ? take(M * po * 2) : nullptr, *z = preact ? take(M * po * 2) : nullptr;
+    int rc = launch_repitch(feats, Ci, x, pi, M, 2, st);
+    if (!rc) rc = launch_repitch(weight, Ci, w, pi, Co, 2, st);
+    if (!rc && po > Co && cudaMemsetAsync((uint8_t *)w + (int64_t)Co * pi * 2, 0, (size_t)(po - Co) * pi * 2, st) != cudaSuccess)
+        rc = check_launch("linear_forward: clear");
+    if (!rc && bias) rc = launch_repitch(bias, Co, b, po, 1, 2, st);
+    if (!rc && residual) rc = launch_repitch(residual, Co, r, po, M, 2, st);
+    if (!rc) rc = linear_forward(x, dtype, M, pi, w, bias ? b : nullptr, r, po, activation, y, z, kernel_choice, status, st);
+    if (!rc) rc = launch_repitch(y, po, out, Co, M, 2, st);
+    if (!rc && preact) rc = launch_repitch(z, po, preact, Co, M, 2, st);
+    return rc;
+}
+
+extern "C" int64_t spconv_linear_backward_workspace_bytes(int dtype, int64_t M, int Ci, int Co, int activation) {
+    if (check_linear(dtype, M, Ci, Co, activation, SPCONV_KERNEL_AUTO) != SPCONV_OK) return -1;
+    return linear_padded(dtype, M, Ci, Co) ? padded_backward_bytes(dtype, M, Ci, Co, activation)
+                                           : separate_backward_bytes(dtype, M, Ci, Co, activation);
+}
+
+extern "C" int spconv_linear_backward(const void *grad_out, const void *preact, const void *feats, const void *weight,
+                                      int dtype, int64_t M, int Ci, int Co, int activation, void *grad_feats,
+                                      void *grad_weight, int weight_dtype, void *grad_bias, int bias_dtype,
+                                      void *workspace, int64_t workspace_bytes, int kernel_choice, int32_t *status,
+                                      void *stream) {
+    if (const int rc = check_linear(dtype, M, Ci, Co, activation, kernel_choice)) return rc;
+    SPCONV_REQUIRE(!grad_weight || weight_dtype == SPCONV_F32 || weight_dtype == dtype, SPCONV_ERR_ARG,
+                   "the weight's gradient is fp32 or of the features' type");
+    SPCONV_REQUIRE(!grad_bias || bias_dtype == SPCONV_F32 || bias_dtype == dtype, SPCONV_ERR_ARG,
+                   "the bias's gradient is fp32 or of the features' type");
+    const cudaStream_t st = (cudaStream_t)stream;
+    if (M == 0) {                            // sums over no rows
+        if (grad_weight && cudaMemsetAsync(grad_weight, 0, (size_t)Co * Ci * elt(weight_dtype), st) != cudaSuccess)
+            return check_launch("linear_backward: clear");
+        if (grad_bias && cudaMemsetAsync(grad_bias, 0, (size_t)Co * elt(bias_dtype), st) != cudaSuccess)
+            return check_launch("linear_backward: clear");
+        return SPCONV_OK;
+    }
+    SPCONV_REQUIRE(grad_out && (preact || activation == SPCONV_ACT_NONE) && (feats || !grad_weight) &&
+                       (weight || !grad_feats), SPCONV_ERR_ARG, "null pointer argument");
+    SPCONV_REQUIRE(workspace && ((uintptr_t)workspace & 255) == 0 &&
+                       workspace_bytes >= spconv_linear_backward_workspace_bytes(dtype, M, Ci, Co, activation),
+                   SPCONV_ERR_ARG, "workspace missing, misaligned or too small");
+    if (activation == SPCONV_ACT_NONE) preact = nullptr;
+    if (kernel_choice != SPCONV_KERNEL_AUTO || !linear_padded(dtype, M, Ci, Co))
+        return linear_backward(grad_out, preact, feats, weight, dtype, M, Ci, Co, activation, grad_feats, grad_weight,
+                               weight_dtype, grad_bias, bias_dtype, workspace, kernel_choice, status, st);
+    const int pi = up8(Ci), po = up8(Co);
+    uint8_t *ws = (uint8_t *)workspace;
+    auto take = [&](int64_t bytes) {
+        void *p = ws;
+        ws += pad256(bytes);
+        return p;
+    };
+    void *x = take(M * pi * 2), *gx = take(M * pi * 2), *g = take(M * po * 2), *z = take(M * po * 2);
+    void *w = take((int64_t)po * pi * 2), *gw = take((int64_t)po * pi * 4), *gb = take(po * 4);
+    int rc = launch_repitch(grad_out, Co, g, po, M, 2, st);
+    if (!rc && preact) rc = launch_repitch(preact, Co, z, po, M, 2, st);
+    if (!rc && grad_weight) rc = launch_repitch(feats, Ci, x, pi, M, 2, st);
+    if (!rc && grad_feats) {                 // dz is zero in the columns past Co, W has to be finite there
+        rc = launch_repitch(weight, Ci, w, pi, Co, 2, st);
+        if (!rc && po > Co && cudaMemsetAsync((uint8_t *)w + (int64_t)Co * pi * 2, 0, (size_t)(po - Co) * pi * 2, st) != cudaSuccess)
+            rc = check_launch("linear_backward: clear");
+    }
+    if (!rc)
+        rc = linear_backward(g, preact ? z : nullptr, grad_weight ? x : nullptr, grad_feats ? w : nullptr, dtype, M, pi, po,
+                             activation, grad_feats ? gx : nullptr, grad_weight ? gw : nullptr, weight_dtype,
+                             grad_bias ? gb : nullptr, bias_dtype, ws, kernel_choice, status, st);
+    if (!rc && grad_feats) rc = launch_repitch(gx, pi, grad_feats, Ci, M, 2, st);
+    if (!rc && grad_weight) rc = launch_repitch(gw, pi, grad_weight, Ci, Co, (int)elt(weight_dtype), st);
+    if (!rc && grad_bias) rc = launch_repitch(gb, po, grad_bias, Co, 1, (int)elt(bias_dtype), st);
+    return rc;
 }

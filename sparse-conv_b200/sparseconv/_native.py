@@ -109,9 +109,10 @@ SIGNATURES = {
     "spconv_submanifold_conv_weight_grad": (_c_int, [
         _c_void_p, _c_void_p, _c_int, _c_i64, _c_int, _c_int, _c_int,
         _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_i64, _c_void_p, _c_void_p]),
+    "spconv_linear_forward_workspace_bytes": (_c_i64, [_c_int, _c_i64, _c_int, _c_int, _c_int, _c_int]),
     "spconv_linear_forward": (_c_int, [
         _c_void_p, _c_int, _c_i64, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int,
-        _c_void_p, _c_void_p, _c_int, _c_void_p, _c_void_p]),
+        _c_void_p, _c_void_p, _c_void_p, _c_i64, _c_int, _c_void_p, _c_void_p]),
     "spconv_linear_backward_workspace_bytes": (_c_i64, [_c_int, _c_i64, _c_int, _c_int, _c_int]),
     "spconv_linear_backward": (_c_int, [
         _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_i64, _c_int, _c_int, _c_int,
@@ -746,9 +747,15 @@ def linear_forward(feats: torch.Tensor, weight: torch.Tensor, bias: Optional[tor
     if M == 0:
         return out, preact
     index = dev.index
-    rc = (_lib or load_library()).spconv_linear_forward(
+    lib = _lib or load_library()
+    ws, need = None, 0
+    if Ci % 8 or Co % 8:
+        need = lib.spconv_linear_forward_workspace_bytes(DTYPE_CODES[dtype], M, Ci, Co, residual is not None, keep_preact)
+        ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need > 0 else None
+    rc = lib.spconv_linear_forward(
         feats.data_ptr(), DTYPE_CODES[dtype], M, Ci, weight.data_ptr(), _ptr(bias), _ptr(residual), Co,
-        ACTIVATIONS[activation], out.data_ptr(), _ptr(preact), kernel, mapped_status(index), _raw_stream(index))
+        ACTIVATIONS[activation], out.data_ptr(), _ptr(preact), _ptr(ws), need, kernel, mapped_status(index),
+        _raw_stream(index))
     if rc != SPCONV_OK:
         _raise(rc, "spconv_linear_forward")
     after_mapped_launch(index)

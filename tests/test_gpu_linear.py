@@ -343,3 +343,20 @@ def test_tiles_over_two_sms(M, Ci, Co, dtype, act, residual):
     _check(out.detach(), v, e, DT[dtype], "out")
     for got, ref, what in zip(grads, _backward_ref(x, w, b, g, act, DT[dtype]), ("feats", "weight", "bias")):
         _check(got, *ref, DT[dtype], what)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("act,residual", [("none", True), ("gelu", False), ("silu", True)])
+@pytest.mark.parametrize("M,Ci,Co", [(20000, 257, 131), (9001, 300, 203), (40001, 129, 72), (60000, 72, 93), (15000, 1001, 517),
+                                     (200001, 129, 72)])
+def test_channels_no_multiple_of_eight(M, Ci, Co, dtype, act, residual):
+    """Around the row counts from which the copies into whole rows pay, forward and backward."""
+    x, w, b, r, g = _inputs(M, Ci, Co, DT[dtype], residual=residual, bias=act != "silu", seed=41)
+    leaves = [t.requires_grad_(True) for t in (x, w, b) if t is not None]
+    out = sparse_linear(x, w, b, residual=r, activation=act)
+    grads = torch.autograd.grad(out, leaves, g)
+    x, w, b = (None if t is None else t.detach() for t in (x, w, b))
+    v, e, _, _ = _forward_ref(x, w, b, r, act)
+    _check(out.detach(), v, e, DT[dtype], "out")
+    for got, ref, what in zip(grads, _backward_ref(x, w, b, g, act, DT[dtype]), ("feats", "weight", "bias")):
+        _check(got, *ref, DT[dtype], what)

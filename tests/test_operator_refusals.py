@@ -19,17 +19,25 @@ def lib():
 
 def test_linear_forward(lib):
     f = lib.spconv_linear_forward
-    assert f(P, 7, 10, 8, P, None, None, 8, 0, P, None, 0, None, None) == 1            # dtype
-    assert f(P, 0, -1, 8, P, None, None, 8, 0, P, None, 0, None, None) == 1            # rows
-    assert f(P, 0, 1 << 31, 8, P, None, None, 8, 0, P, None, 0, None, None) == 1
-    assert f(P, 0, 10, 0, P, None, None, 8, 0, P, None, 0, None, None) == 1            # channels
+    assert f(P, 7, 10, 8, P, None, None, 8, 0, P, None, None, 0, 0, None, None) == 1            # dtype
+    assert f(P, 0, -1, 8, P, None, None, 8, 0, P, None, None, 0, 0, None, None) == 1            # rows
+    assert f(P, 0, 1 << 31, 8, P, None, None, 8, 0, P, None, None, 0, 0, None, None) == 1
+    assert f(P, 0, 10, 0, P, None, None, 8, 0, P, None, None, 0, 0, None, None) == 1            # channels
     assert b"channels" in lib.spconv_last_error()
-    assert f(P, 0, 10, 8, P, None, None, 65537, 0, P, None, 0, None, None) == 1
-    assert f(P, 0, 10, 8, P, None, None, 8, 4, P, None, 0, None, None) == 1            # activation
-    assert f(P, 0, 10, 8, P, None, None, 8, 0, P, None, 3, None, None) == 1            # kernel choice
-    assert f(None, 0, 10, 8, P, None, None, 8, 0, P, None, 0, None, None) == 1         # null
-    assert f(P, 0, 10, 8, P, None, None, 8, 0, P, None, 2, None, None) == 3            # tcgen05: no fp32
-    assert f(None, 0, 0, 8, None, None, None, 8, 0, None, None, 0, None, None) == 0    # no rows
+    assert f(P, 0, 10, 8, P, None, None, 65537, 0, P, None, None, 0, 0, None, None) == 1
+    assert f(P, 0, 10, 8, P, None, None, 8, 4, P, None, None, 0, 0, None, None) == 1            # activation
+    assert f(P, 0, 10, 8, P, None, None, 8, 0, P, None, None, 0, 3, None, None) == 1            # kernel choice
+    assert f(None, 0, 10, 8, P, None, None, 8, 0, P, None, None, 0, 0, None, None) == 1         # null
+    assert f(P, 0, 10, 8, P, None, None, 8, 0, P, None, None, 0, 2, None, None) == 3            # tcgen05: no fp32
+    assert f(None, 0, 0, 8, None, None, None, 8, 0, None, None, None, 0, 0, None, None) == 0    # no rows
+    need = lib.spconv_linear_forward_workspace_bytes(2, 50000, 257, 131, 1, 0)
+    assert need > 50000 * (264 + 2 * 136) * 2 and lib.spconv_linear_forward_workspace_bytes(2, 50000, 256, 128, 1, 1) == 0
+    for m, ci, co in ((20000, 257, 131), (15000, 1001, 517), (200001, 129, 72)):            # shapes that are copied
+        assert lib.spconv_linear_forward_workspace_bytes(1, m, ci, co, 0, 0) > 0
+    assert lib.spconv_linear_forward_workspace_bytes(0, 50000, 257, 131, 1, 0) == 0          # fp32: no tensor cores
+    assert lib.spconv_linear_forward_workspace_bytes(2, 50000, 0, 131, 1, 0) == -1
+    assert f(P, 2, 50000, 257, P, None, P, 131, 0, P, None, P, need - 1, 0, None, None) == 1
+    assert f(P, 2, 50000, 257, P, None, P, 131, 0, P, None, ctypes.c_void_p(8), need, 0, None, None) == 1
 
 
 def test_linear_backward(lib):
