@@ -265,14 +265,14 @@ __device__ __forceinline__ bool mbar_wait_or_abort(uint32_t addr, uint32_t parit
     }
 }
 
-// The same with suspended waits (up to 20 us between checks of the flag and the limit).
+// The same with suspended waits (up to 20 us, or the limit, between checks of the flag and the limit).
 __device__ __forceinline__ bool mbar_wait_suspended(uint32_t addr, uint32_t parity, volatile int *abort_flag,
                                                     uint64_t limit_ns) {
-    constexpr uint32_t kHintNs = 20000;
+    const uint32_t hint_ns = limit_ns < 20000ull ? (uint32_t)limit_ns : 20000u;
     if (mbar_try_wait(addr, parity)) return true;
     const uint64_t t0 = globaltimer_ns();
     for (;;) {
-        if (mbar_try_wait_suspended(addr, parity, kHintNs)) return true;
+        if (mbar_try_wait_suspended(addr, parity, hint_ns)) return true;
         if (*abort_flag) return false;
         if (globaltimer_ns() - t0 > limit_ns) {
             *abort_flag = 1;

@@ -159,7 +159,8 @@ linear_bwd_tc_kernel(const __grid_constant__ CUtensorMap map_g, const __grid_con
                 tc_commit(smem_u32(&accfull[s]));
             }
             if (ok) tc_commit(smem_u32(wdone));
-            else if (i > 0) mbar_wait_bounded(smem_u32(&accfull[(i - 1) & 1]), (uint32_t)(((i - 1) >> 1) & 1));
+            // MMAs in flight read shared memory and write TMEM, and the epilogue may have given up
+            if (i > 0) mbar_wait_bounded(smem_u32(&accfull[(i - 1) & 1]), (uint32_t)(((i - 1) >> 1) & 1));
         }
     } else if (warp < 6) {
         // ------------------------------------------------------------------ epilogue
@@ -286,10 +287,10 @@ linear_bwd_tc_kernel(const __grid_constant__ CUtensorMap map_g, const __grid_con
     }
 
     __syncwarp();
-    if (*s_abort && tid == 0) raise_status(a.status, SPCONV_STATUS_WAIT_TIMEOUT);
     tc_fence_before();
-    __syncthreads();
+    __syncthreads();                         // every role has set the flag by now if it gives up
     tc_fence_after();
+    if (tid == 0 && *s_abort) raise_status(a.status, SPCONV_STATUS_WAIT_TIMEOUT);
     if (warp == 1) tmem_dealloc(tmem, (uint32_t)a.tmem_cols);
 }
 

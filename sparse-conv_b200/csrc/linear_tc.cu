@@ -292,9 +292,10 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                     next(buf, acc_phase, a.bufs);
                 }
             }
-            // MMAs in flight read shared memory: wait for the last commit (its stage's use ended `phase`
-            // if the ring has not wrapped since, else the phase before)
-            if (!ok && last >= 0) mbar_wait_bounded(smem_u32(&empty[last]), last < st ? phase : phase ^ 1u);
+            // MMAs in flight read shared memory and write TMEM, and the epilogue may have given up: wait for
+            // the last commit (its stage's use ended `phase` if the ring has not wrapped since, else the
+            // phase before)
+            if (last >= 0) mbar_wait_bounded(smem_u32(&empty[last]), last < st ? phase : phase ^ 1u);
         }
     } else {
         // ------------------------------------------------------------------ epilogue
@@ -446,11 +447,11 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     }
 
     __syncwarp();
-    if (*s_abort && tid == 0) raise_status(a.status, SPCONV_STATUS_WAIT_TIMEOUT);
     tc_fence_before();
     if constexpr (PAIR) cluster_sync();      // neither leaves while the other's MMAs or arrivals may reach it
-    __syncthreads();
+    __syncthreads();                         // every role has set the flag by now if it gives up
     tc_fence_after();
+    if (tid == 0 && *s_abort) raise_status(a.status, SPCONV_STATUS_WAIT_TIMEOUT);
     if (warp == 1) {
         if constexpr (PAIR) tmem_dealloc_pair(tmem, tmem_cols);
         else tmem_dealloc(tmem, tmem_cols);

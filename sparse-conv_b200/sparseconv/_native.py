@@ -292,9 +292,13 @@ def mapped_status(index: int) -> int:
     return st.mapped_ptr
 
 
+# read once, for the ops whose host time counts
+_SYNC_CHECK = os.environ.get("SPARSECONV_SYNC_CHECK", "0") == "1"
+
+
 def after_mapped_launch(index: int) -> None:
-    """Check at once if SPARSECONV_SYNC_CHECK=1 (not while the stream is being captured)."""
-    if os.environ.get("SPARSECONV_SYNC_CHECK", "0") == "1" and not torch.cuda.is_current_stream_capturing():
+    """Check at once if SPARSECONV_SYNC_CHECK=1 at import (not while the stream is being captured)."""
+    if _SYNC_CHECK and not torch.cuda.is_current_stream_capturing():
         torch.cuda.current_stream(index).synchronize()
         _inspect_mapped(_status[index])
 
@@ -765,35 +769,50 @@ def linear_forward(feats: torch.Tensor, weight: torch.Tensor, bias: Optional[tor
 @_on_device
 def linear_backward(grad_out: torch.Tensor, preact: Optional[torch.Tensor], feats: torch.Tensor, weight: torch.Tensor,
                     activation: str, weight_dtype: torch.dtype, bias_dtype: Optional[torch.dtype],
-                    needs: Sequence[bool], kernel: int = KERNEL_AUTO) -> list:
+                    needs: Sequence[bool], kernel: int = KERNEL_AUTO) -> tuple:
     """Gradients of feats, weight (in ``weight_dtype``) and bias (in ``bias_dtype``), None where
     ``needs`` says so; the arguments are linear_forward's, with its kept product."""
-    lib = load_library()
-    dev = _require_cuda(grad_out, preact, feats, weight)
+    _require_cuda(grad_out, preact, feats, weight)
+    _matrix(grad_out, (feats.shape[0], weight.shape[0]), feats.dtype, "grad_out")
+    return linear_backward_of(grad_out, preact, feats, weight.contiguous(), ACTIVATIONS[activation], weight_dtype,
+                              bias_dtype, needs, kernel)
+
+
+def linear_backward_of(grad_out, preact, feats, weight, activation: int, weight_dtype, bias_dtype, needs,
+                       kernel: int = KERNEL_AUTO) -> tuple:
+    """linear_backward of tensors that a forward has checked (autograd's), contiguous; a network's
+    backward calls it once a layer, so it does no more than it must."""
+    lib = _lib or load_library()
     M, Ci = feats.shape
     Co = weight.shape[0]
-    dtype = feats.dtype
-    _matrix(grad_out, (M, Co), dtype, "grad_out")
-    weight = weight.contiguous()
+    dtype, dev, index = feats.dtype, feats.device, feats.get_device()
     code = DTYPE_CODES[dtype]
-
-    def grad(shape, wanted):                 # in the wanted dtype where the kernels write it
-        return torch.empty(shape, dtype=wanted if wanted == dtype else torch.float32, device=dev)
-    gx = torch.empty_like(feats) if needs[0] else None
-    gw = grad((Co, Ci), weight_dtype) if needs[1] else None
-    gb = grad((Co,), bias_dtype) if needs[2] else None
-    need = lib.spconv_linear_backward_workspace_bytes(code, M, Ci, Co, ACTIVATIONS[activation])
-    ws = torch.empty((max(need, 256),), dtype=torch.uint8, device=dev)
-    index = dev.index
+    gx = gw = gb = None
+    gx_ptr = gw_ptr = gb_ptr = None
+    gw_code = gb_code = 0
+    if needs[0]:
+        gx = torch.empty_like(feats)
+        gx_ptr = gx.data_ptr()
+    if needs[1]:                             # in the wanted dtype where the kernels write it
+        gw = torch.empty((Co, Ci), dtype=dtype if weight_dtype == dtype else torch.float32, device=dev)
+        gw_ptr, gw_code = gw.data_ptr(), code if weight_dtype == dtype else 0
+    if needs[2]:
+        gb = torch.empty((Co,), dtype=dtype if bias_dtype == dtype else torch.float32, device=dev)
+        gb_ptr, gb_code = gb.data_ptr(), code if bias_dtype == dtype else 0
+    need = lib.spconv_linear_backward_workspace_bytes(code, M, Ci, Co, activation)
+    ws = torch.empty((need if need > 0 else 256,), dtype=torch.uint8, device=dev)
     rc = lib.spconv_linear_backward(
-        grad_out.data_ptr(), _ptr(preact), feats.data_ptr(), weight.data_ptr(), code, M, Ci, Co,
-        ACTIVATIONS[activation], _ptr(gx), _ptr(gw), 0 if gw is None else DTYPE_CODES[gw.dtype], _ptr(gb),
-        0 if gb is None else DTYPE_CODES[gb.dtype], ws.data_ptr(), need, kernel,
+        grad_out.data_ptr(), None if preact is None else preact.data_ptr(), feats.data_ptr(), weight.data_ptr(), code,
+        M, Ci, Co, activation, gx_ptr, gw_ptr, gw_code, gb_ptr, gb_code, ws.data_ptr(), need, kernel,
         mapped_status(index), _raw_stream(index))
     if rc != SPCONV_OK:
         _raise(rc, "spconv_linear_backward")
     after_mapped_launch(index)
-    return [gx, None if gw is None else gw.to(weight_dtype), None if gb is None else gb.to(bias_dtype)]
+    if gw is not None and gw.dtype != weight_dtype:
+        gw = gw.to(weight_dtype)
+    if gb is not None and gb.dtype != bias_dtype:
+        gb = gb.to(bias_dtype)
+    return gx, gw, gb
 
 
 def _norm_args(feats: torch.Tensor, residual, params, offsets, residual_scale: float, norm: str,
@@ -850,21 +869,25 @@ def _norm_args(feats: torch.Tensor, residual, params, offsets, residual_scale: f
 @_on_device
 def residual_norm_forward(feats: torch.Tensor, residual: Optional[torch.Tensor], params: Sequence[Optional[torch.Tensor]],
                           offsets: Optional[torch.Tensor], residual_scale: float, norm: str, next_norm: str,
-                          eps: float, keep_stats: bool = False
-                          ) -> Tuple[torch.Tensor, Optional[torch.Tensor], Optional[torch.Tensor]]:
-    """(hidden, normed, row statistics if ``keep_stats``) of the gated residual step (normed None
-    without ``next_norm``)."""
+                          eps: float, keep_stats: bool = False) -> tuple:
+    """(hidden, normed) of the gated residual step (normed None without ``next_norm``); with
+    ``keep_stats`` also the row statistics and the call's arguments, for residual_norm_backward_of."""
     a = _norm_args(feats, residual, params, offsets, residual_scale, norm, next_norm, eps)
     hidden = torch.empty_like(feats)
-    normed = torch.empty_like(feats) if next_norm != "none" else None
-    stats = torch.empty((a.num_rows, 4), dtype=torch.float32, device=feats.device) if keep_stats else None
-    a.hidden, a.normed, a.row_stats = hidden.data_ptr(), _ptr(normed), _ptr(stats)
+    a.hidden = hidden.data_ptr()
+    normed = stats = None
+    if next_norm != "none":
+        normed = torch.empty_like(feats)
+        a.normed = normed.data_ptr()
+    if keep_stats:
+        stats = torch.empty((a.num_rows, 4), dtype=torch.float32, device=feats.device)
+        a.row_stats = stats.data_ptr()
     index = feats.get_device()
     rc = (_lib or load_library()).spconv_residual_norm_forward(a, _raw_stream(index))
     if rc != SPCONV_OK:
         _raise(rc, "spconv_residual_norm_forward")
     after_mapped_launch(index)
-    return hidden, normed, stats
+    return (hidden, normed, stats, a) if keep_stats else (hidden, normed)
 
 
 @_on_device
@@ -874,23 +897,48 @@ def residual_norm_backward(feats: torch.Tensor, residual: Optional[torch.Tensor]
                            grad_normed: Optional[torch.Tensor], needs: Sequence[bool]) -> list:
     """Gradients of feats, residual, gate, weight, bias, next_weight and next_bias (None where
     ``needs`` says so), each in its tensor's shape and dtype."""
-    lib = load_library()
     a = _norm_args(feats, residual, params, offsets, residual_scale, norm, next_norm, eps)
     for g, what in ((grad_hidden, "grad_hidden"), (grad_normed, "grad_normed")):
         if g is not None:
             _require_cuda(feats, g)
             _matrix(g, feats.shape, feats.dtype, what)
-    a.grad_hidden, a.grad_normed, a.row_stats = _ptr(grad_hidden), _ptr(grad_normed), stats.data_ptr()
-    grads = [torch.empty_like(t) if t is not None and need else None
-             for t, need in zip((feats, residual, *params), needs)]
-    a.grad_feats, a.grad_residual = _ptr(grads[0]), _ptr(grads[1])
-    a.gate.grad, a.weight.grad, a.bias.grad = _ptr(grads[2]), _ptr(grads[3]), _ptr(grads[4])
-    a.next_weight.grad, a.next_bias.grad = _ptr(grads[5]), _ptr(grads[6])
-    if any(g is not None for g in grads[2:]):
-        a.workspace_bytes = lib.spconv_residual_norm_workspace_bytes(a.num_rows, a.channels, a.num_samples)
-        ws = torch.empty((max(a.workspace_bytes, 16),), dtype=torch.uint8, device=feats.device)
+    return residual_norm_backward_of(a, feats, residual, params, offsets, stats, grad_hidden, grad_normed, needs)
+
+
+def residual_norm_backward_of(args: ResidualNormArgs, feats, residual, params, offsets, stats, grad_hidden, grad_normed,
+                              needs) -> list:
+    """residual_norm_backward with the arguments that a forward of the same tensors has checked: only
+    the addresses are taken anew (saved tensors may have been moved)."""
+    lib, index = _lib or load_library(), feats.get_device()
+    a = ResidualNormArgs.from_buffer_copy(args)
+    a.hidden = a.normed = None
+    a.feats, a.row_stats = feats.data_ptr(), stats.data_ptr()
+    a.grad_hidden = None if grad_hidden is None else grad_hidden.data_ptr()
+    a.grad_normed = None if grad_normed is None else grad_normed.data_ptr()
+    grads = [None] * 7
+    if needs[0]:
+        grads[0] = g = torch.empty_like(feats)
+        a.grad_feats = g.data_ptr()
+    if residual is not None:
+        a.residual = residual.data_ptr()
+        if needs[1]:
+            grads[1] = g = torch.empty_like(residual)
+            a.grad_residual = g.data_ptr()
+    sums = False
+    for i, (q, p) in enumerate(zip((a.gate, a.weight, a.bias, a.next_weight, a.next_bias), params), 2):
+        if p is not None:
+            q.data = p.data_ptr()
+            if needs[i]:
+                grads[i] = g = torch.empty_like(p)
+                q.grad = g.data_ptr()
+                sums = True
+    if a.offsets:
+        a.offsets = offsets.data_ptr()
+    if sums:
+        a.workspace_bytes = need = lib.spconv_residual_norm_workspace_bytes(a.num_rows, a.channels, a.num_samples)
+        ws = torch.empty((need,), dtype=torch.uint8, device=feats.device)
         a.workspace = ws.data_ptr()
-    index = feats.get_device()
+    a.status = mapped_status(index)
     rc = lib.spconv_residual_norm_backward(a, _raw_stream(index))
     if rc != SPCONV_OK:
         _raise(rc, "spconv_residual_norm_backward")

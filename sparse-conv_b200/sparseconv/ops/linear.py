@@ -23,25 +23,25 @@ class Activation:
 class SparseLinearFunction(Function):
     @staticmethod
     def forward(ctx, feats, weight, bias, residual, activation):
-        w = weight.to(feats.dtype)
+        w = weight.to(feats.dtype).contiguous()
         b = None if bias is None else bias.to(feats.dtype)
-        keep = activation != Activation.NONE and any(ctx.needs_input_grad[:3])
+        needs = ctx.needs_input_grad
+        keep = activation != Activation.NONE and (needs[0] or needs[1] or needs[2])
         out, preact = _native.linear_forward(feats, w, b, residual, activation, keep_preact=keep)
         ctx.save_for_backward(feats, w, preact)
-        ctx.dtypes = (weight.dtype, None if bias is None else bias.dtype)
-        ctx.activation = activation
+        ctx.settings = (_native.ACTIVATIONS[activation], weight.dtype, None if bias is None else bias.dtype)
         return out
 
     @staticmethod
     def backward(ctx, grad_out):
         feats, weight, preact = ctx.saved_tensors
-        weight_dtype, bias_dtype = ctx.dtypes
-        grad_out = grad_out.to(feats.dtype).contiguous()
-        grad_feats = grad_weight = grad_bias = None
-        if any(ctx.needs_input_grad[:3]):
-            grad_feats, grad_weight, grad_bias = _native.linear_backward(
-                grad_out, preact, feats, weight, ctx.activation, weight_dtype, bias_dtype, ctx.needs_input_grad[:3])
-        return grad_feats, grad_weight, grad_bias, grad_out if ctx.needs_input_grad[3] else None, None
+        needs = ctx.needs_input_grad
+        if not grad_out.is_contiguous():
+            grad_out = grad_out.contiguous()
+        grads = (None, None, None)
+        if needs[0] or needs[1] or needs[2]:
+            grads = _native.linear_backward_of(grad_out, preact, feats, weight, *ctx.settings, needs)
+        return (*grads, grad_out if needs[3] else None, None)
 
 
 def sparse_linear(
@@ -67,8 +67,9 @@ def sparse_linear(
         activation) is kept in the feature dtype; weight and bias gradients come in the
         parameters' dtypes, summed in fp32 in a fixed order.
     """
-    if not torch.is_grad_enabled() or not any(
-            t is not None and t.requires_grad for t in (feats, weight, bias, residual)):
-        return _native.linear_forward(feats, weight.to(feats.dtype), None if bias is None else bias.to(feats.dtype),
-                                      residual, activation)[0]
-    return SparseLinearFunction.apply(feats, weight, bias, residual, activation)
+    if torch.is_grad_enabled() and (feats.requires_grad or weight.requires_grad or
+                                    (bias is not None and bias.requires_grad) or
+                                    (residual is not None and residual.requires_grad)):
+        return SparseLinearFunction.apply(feats, weight, bias, residual, activation)
+    return _native.linear_forward(feats, weight.to(feats.dtype), None if bias is None else bias.to(feats.dtype),
+                                  residual, activation)[0]

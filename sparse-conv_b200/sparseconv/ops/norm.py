@@ -24,10 +24,9 @@ class ResidualNormFunction(Function):
     def forward(ctx, feats, residual, gate, weight, bias, next_weight, next_bias, batch_offsets,
                 residual_scale, norm, next_norm, eps):
         params = (gate, weight, bias, next_weight, next_bias)
-        hidden, normed, stats = _native.residual_norm_forward(
+        hidden, normed, stats, ctx.args = _native.residual_norm_forward(
             feats, residual, params, batch_offsets, residual_scale, norm, next_norm, eps, keep_stats=True)
         ctx.save_for_backward(feats, residual, *params, batch_offsets, stats)
-        ctx.settings = (residual_scale, norm, next_norm, eps)
         ctx.set_materialize_grads(False)
         return hidden, normed
 
@@ -37,9 +36,9 @@ class ResidualNormFunction(Function):
         if grad_hidden is None and grad_normed is None:
             return (None,) * 12
         feats, residual, *params, batch_offsets, stats = ctx.saved_tensors
-        gh, gn = (None if g is None else g.to(feats.dtype).contiguous() for g in (grad_hidden, grad_normed))
-        grads = _native.residual_norm_backward(
-            feats, residual, params, batch_offsets, *ctx.settings, stats, gh, gn, ctx.needs_input_grad[:7])
+        gh, gn = (g if g is None or g.is_contiguous() else g.contiguous() for g in (grad_hidden, grad_normed))
+        grads = _native.residual_norm_backward_of(
+            ctx.args, feats, residual, params, batch_offsets, stats, gh, gn, ctx.needs_input_grad)
         return (*grads, None, None, None, None, None)
 
 
@@ -83,7 +82,7 @@ def sparse_residual_norm(
     params = (feats, residual, gate, weight, bias, next_weight, next_bias)
     if not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in params):
         return _native.residual_norm_forward(feats, residual, params[2:], batch_offsets, residual_scale,
-                                             norm, next_norm, eps)[:2]
+                                             norm, next_norm, eps)
     return ResidualNormFunction.apply(*params, batch_offsets, residual_scale, norm, next_norm, eps)
 
 
