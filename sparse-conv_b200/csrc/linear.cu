@@ -63,6 +63,9 @@ linear_simt_kernel(GemmArgs g) {
     const int64_t k_end = g.splits > 1 ? min(g.K, k_begin + g.k_per_split) : g.K;
     const int64_t lda = AT ? g.M : g.K, ldb = BT ? g.N : g.K;
     const int tn = threadIdx.x % (BN / TN), tm = threadIdx.x / (BN / TN);
+    // A thread's columns: fours, BN / 2 apart where it has eight, so that a quarter-warp's 16-byte reads
+    // of B fall on different banks.
+    auto col = [&](int j) { return TN <= 4 ? tn * TN + j : (j / 4) * (BN / 2) + tn * 4 + j % 4; };
     float acc[TM][TN] = {};
     SimtTile<T, BM, AT> ta;
     SimtTile<T, BN, BT> tb;
@@ -83,7 +86,7 @@ linear_simt_kernel(GemmArgs g) {
 #pragma unroll
             for (int i = 0; i < TM; ++i) fa[i] = sa[buf][kk][tm * TM + i];
 #pragma unroll
-            for (int j = 0; j < TN; ++j) fb[j] = sb[buf][kk][tn * TN + j];
+            for (int j = 0; j < TN; ++j) fb[j] = sb[buf][kk][col(j)];
 #pragma unroll
             for (int i = 0; i < TM; ++i)
 #pragma unroll
@@ -96,7 +99,7 @@ linear_simt_kernel(GemmArgs g) {
         if (m >= g.M) continue;
 #pragma unroll
         for (int j = 0; j < TN; ++j) {
-            const int64_t n = n0 + tn * TN + j;
+            const int64_t n = n0 + col(j);
             if (n >= g.N) continue;
             const int64_t at = m * g.N + n;
             float z = acc[i][j];
@@ -123,6 +126,10 @@ static int simt_shape(const GemmArgs &g) {
     // narrow outputs (class scores) leave three quarters of a 64-wide tile idle
     if (g.N <= 16) return run(linear_simt_kernel<T, 128, 16, 4, 2, AT, BT, ACT>, 128, 16);
     if (g.M <= 16) return run(linear_simt_kernel<T, 16, 128, 2, 4, AT, BT, ACT>, 16, 128);
+    // 128 columns where there are that many and the tiles still fill the SMs: a quarter fewer reads of
+    // shared memory for each product
+    if (g.N > 64 && (g.M + 127) / 128 * ((g.N + 127) / 128) * g.splits >= 148)
+        return run(linear_simt_kernel<T, 128, 128, 8, 8, AT, BT, ACT>, 128, 128);
     return run(linear_simt_kernel<T, 128, 64, 8, 4, AT, BT, ACT>, 128, 64);
 }
 
