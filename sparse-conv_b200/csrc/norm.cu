@@ -153,11 +153,17 @@ __device__ __forceinline__ void rn_param(const RnArgs &a, int k, int s, int col,
     }
 }
 
-// Sums of U pairs of values over the lanes that share a row: lpr lanes of a warp, or the block.
-// Without `both` only the second of each pair is summed.
-template <int U, bool BLOCK>
-__device__ __forceinline__ void rn_sum2(float (&u)[U], float (&v)[U], bool both, int lpr, float2 *scratch) {
-    const int top = BLOCK ? 16 : lpr >> 1;
+// Sums of U pairs of values over the lanes that share a row: lpr lanes of a warp (WARPS == 0), or a
+// block of WARPS warps, whose sums meet in `scratch` [2][WARPS]. The halves take turns, so that one
+// barrier a sum is enough: between two uses of a half lies the other's barrier. Without `both` only the
+// second of each pair is summed.
+struct RnScratch {
+    float2 *part;
+    int half;
+};
+template <int U, int WARPS>
+__device__ __forceinline__ void rn_sum2(float (&u)[U], float (&v)[U], bool both, int lpr, RnScratch &scratch) {
+    const int top = WARPS ? 16 : lpr >> 1;
     if (both) {
         for (int o = top; o > 0; o >>= 1)
 #pragma unroll
@@ -170,16 +176,17 @@ __device__ __forceinline__ void rn_sum2(float (&u)[U], float (&v)[U], bool both,
 #pragma unroll
             for (int i = 0; i < U; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
     }
-    if constexpr (BLOCK) {
+    if constexpr (WARPS > 1) {
         static_assert(U == 1, "a block takes one row at a time");
-        __syncthreads();
-        if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = make_float2(u[0], v[0]);
+        float2 *part = scratch.part + scratch.half * WARPS;
+        scratch.half ^= 1;
+        if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = make_float2(u[0], v[0]);
         __syncthreads();
         u[0] = v[0] = 0.f;
 #pragma unroll
-        for (int w = 0; w < kRnWarps; ++w) {
-            u[0] += scratch[w].x;
-            v[0] += scratch[w].y;
+        for (int w = 0; w < WARPS; ++w) {
+            u[0] += part[w].x;
+            v[0] += part[w].y;
         }
     }
 }
@@ -209,9 +216,9 @@ __device__ __forceinline__ float rn_dot(const float (&t)[N], const float (&n)[N]
 
 // Normalises U rows, N values of each in a lane, in place: (mean, rstd) of each row in st. Columns
 // that a lane does not have hold zeros, before and after (FULL: it has them all).
-template <int U, int N, int VEC, bool BLOCK, bool FULL>
+template <int U, int N, int VEC, int WARPS, bool FULL>
 __device__ __forceinline__ void rn_normalise(float (&t)[U][N], float2 (&st)[U], const bool *have, int kind, float inv_c,
-                                             float eps, int lpr, float2 *scratch) {
+                                             float eps, int lpr, RnScratch &scratch) {
     if (kind == SPCONV_NORM_NONE) {
 #pragma unroll
         for (int u = 0; u < U; ++u) st[u] = make_float2(0.f, 1.f);
@@ -221,7 +228,7 @@ __device__ __forceinline__ void rn_normalise(float (&t)[U][N], float2 (&st)[U], 
     // eight values, which lies within sqrt(C / 8) deviations of the row's mean: mean(d^2) - mean(d)^2
     // then costs at most the factor C / 8 + 1 in the variance's rounding, whatever offset the row has
     // in common. Single columns a lane, or a block a row: the mean first, then the squares.
-    constexpr bool ONE = VEC == 8 && !BLOCK;
+    constexpr bool ONE = VEC == 8 && WARPS == 0;
     float s[U], q[U], shift[U];
     const bool layer = kind == SPCONV_NORM_LAYER;
 #pragma unroll
@@ -239,7 +246,7 @@ __device__ __forceinline__ void rn_normalise(float (&t)[U][N], float2 (&st)[U], 
         }
     }
     if (!ONE && layer) {
-        rn_sum2<U, BLOCK>(s, q, true, lpr, scratch);
+        rn_sum2<U, WARPS>(s, q, true, lpr, scratch);
 #pragma unroll
         for (int u = 0; u < U; ++u) shift[u] = s[u] * inv_c;
     }
@@ -252,7 +259,7 @@ __device__ __forceinline__ void rn_normalise(float (&t)[U][N], float2 (&st)[U], 
         }
         q[u] = rn_dot<N>(t[u], t[u]);
     }
-    rn_sum2<U, BLOCK>(s, q, layer && ONE, lpr, scratch);
+    rn_sum2<U, WARPS>(s, q, layer && ONE, lpr, scratch);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const float m = layer && ONE ? s[u] * inv_c : 0.f;
@@ -266,9 +273,9 @@ __device__ __forceinline__ void rn_normalise(float (&t)[U][N], float2 (&st)[U], 
 }
 
 // t: gradient at the normalised values n -> gradient at the values before the norm, added to g.
-template <int U, int N, bool BLOCK>
+template <int U, int N, int WARPS>
 __device__ __forceinline__ void rn_normalise_back(float (&g)[U][N], float (&t)[U][N], const float (&n)[U][N],
-                                                  const float (&rstd)[U], int kind, float inv_c, int lpr, float2 *scratch) {
+                                                  const float (&rstd)[U], int kind, float inv_c, int lpr, RnScratch &scratch) {
     if (kind == SPCONV_NORM_NONE) {
 #pragma unroll
         for (int u = 0; u < U; ++u)
@@ -283,7 +290,7 @@ __device__ __forceinline__ void rn_normalise_back(float (&g)[U][N], float (&t)[U
         s[u] = layer ? rn_tree<N>(t[u]) : 0.f;
         q[u] = rn_dot<N>(t[u], n[u]);
     }
-    rn_sum2<U, BLOCK>(s, q, layer, lpr, scratch);
+    rn_sum2<U, WARPS>(s, q, layer, lpr, scratch);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const float mean = layer ? s[u] * inv_c * rstd[u] : 0.f, along = q[u] * inv_c * rstd[u];
@@ -314,26 +321,37 @@ __device__ __forceinline__ void rn_check_offsets(const RnArgs &a) {
     if (bad) raise_status(a.status, SPCONV_STATUS_OFFSETS);
 }
 
-// A CTA takes `chunk` consecutive rows, sample by sample, and its row groups (lpr lanes, or the
-// block) take the rows of a sample in turn. Parameters stay in registers for a sample's rows
-// when a lane owns at most 8 columns; wider rows read them through L1.
-template <typename T, int VEC, int VPT, bool BLOCK>
-__global__ void __launch_bounds__(kRnThreads)
+// Direct form: rows from global memory into registers and back, the next row's loads under this one's
+// sums. For few rows (short and latency-bound: the ring would not fill), for more than 256 channels,
+// where a block of WARPS warps takes a row, and for tensors off 16-byte boundaries.
+//
+// A block takes `chunk` consecutive rows, sample by sample, and its row groups (lpr lanes, or the
+// block) take the rows of a sample in turn. A lane owns at most 8 columns, whose parameters stay in
+// registers for a sample's rows, and in the backward their sums too: a block of as many warps as that
+// takes beats a warp with more columns a lane (100,000 x 333 fp16: 3.2 ms forward with 32 single
+// columns a lane).
+template <typename T, int VEC, int VPT, int WARPS>
+struct RnDirect {
+    static constexpr int N = VEC * VPT;
+    static constexpr int kThreads = WARPS ? WARPS * 32 : kRnThreads;
+    static_assert(N <= 8, "parameters and sums stay in registers");
+};
+
+template <typename T, int VEC, int VPT, int WARPS>
+__global__ void __launch_bounds__(RnDirect<T, VEC, VPT, WARPS>::kThreads)
 residual_norm_fwd_kernel(const __grid_constant__ RnArgs a) {
-    constexpr int N = VEC * VPT;
-    constexpr bool HOIST = N <= 8;
-    __shared__ float2 scratch[kRnWarps];
+    constexpr int N = VEC * VPT, kThreads = RnDirect<T, VEC, VPT, WARPS>::kThreads;
+    __shared__ float2 part[2 * (WARPS ? WARPS : 1)];
+    RnScratch scratch{part, 0};
     rn_check_offsets(a);
-    const int C = a.C, lpr = a.lpr;
-    const int lanes = BLOCK ? kRnThreads : lpr;
-    const int groups = BLOCK ? 1 : kRnThreads / lpr;
-    const int group = BLOCK ? 0 : threadIdx.x / lpr, lane = BLOCK ? threadIdx.x : threadIdx.x & (lpr - 1);
+    const int C = a.C, lpr = WARPS ? kThreads : a.lpr;
+    const int groups = kThreads / lpr, group = threadIdx.x / lpr, lane = threadIdx.x & (lpr - 1);
     const float inv_c = 1.f / (float)C;
     int col[VPT];
     bool have[VPT];
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
-        col[j] = (lane + lanes * j) * VEC;
+        col[j] = (lane + lpr * j) * VEC;
         have[j] = col[j] < C;
     }
     const int64_t row0 = (int64_t)blockIdx.x * a.chunk, row1 = min(a.M, row0 + a.chunk);
@@ -341,17 +359,15 @@ residual_norm_fwd_kernel(const __grid_constant__ RnArgs a) {
     for (int64_t seg = row0; seg < row1; ++s) {
         const int64_t end = s < a.B - 1 ? min(row1, (int64_t)__ldg(a.offsets + s + 1)) : row1;
         if (end <= seg) continue;            // an empty sample
-        float pg[HOIST ? N : 1], pw1[HOIST ? N : 1], pb1[HOIST ? N : 1], pw2[HOIST ? N : 1], pb2[HOIST ? N : 1];
-        if constexpr (HOIST) {
+        float pg[N], pw1[N], pb1[N], pw2[N], pb2[N];
 #pragma unroll
-            for (int j = 0; j < VPT; ++j) {
-                const int c = have[j] ? col[j] : 0;
-                rn_param<T, VEC>(a, kG, s, c, pg + j * VEC);
-                rn_param<T, VEC>(a, kW1, s, c, pw1 + j * VEC);
-                rn_param<T, VEC>(a, kB1, s, c, pb1 + j * VEC);
-                rn_param<T, VEC>(a, kW2, s, c, pw2 + j * VEC);
-                rn_param<T, VEC>(a, kB2, s, c, pb2 + j * VEC);
-            }
+        for (int j = 0; j < VPT; ++j) {
+            const int c = have[j] ? col[j] : 0;
+            rn_param<T, VEC>(a, kG, s, c, pg + j * VEC);
+            rn_param<T, VEC>(a, kW1, s, c, pw1 + j * VEC);
+            rn_param<T, VEC>(a, kB1, s, c, pb1 + j * VEC);
+            rn_param<T, VEC>(a, kW2, s, c, pw2 + j * VEC);
+            rn_param<T, VEC>(a, kB2, s, c, pb2 + j * VEC);
         }
         RnPack<T, VEC> px[VPT], pr[VPT];
         auto fetch = [&](int64_t row) {
@@ -368,51 +384,28 @@ residual_norm_fwd_kernel(const __grid_constant__ RnArgs a) {
         fetch(seg + group);
         for (int64_t base = seg; base < end; base += groups) {
             const int64_t row = base + group;
-            float uu[1][N], hh[1][N];
-            float (&u)[N] = uu[0], (&h)[N] = hh[0];
+            float u[1][N], h[1][N];
 #pragma unroll
             for (int j = 0; j < VPT; ++j) {
-                rn_unpack(px[j], u + j * VEC);
-                rn_unpack(pr[j], h + j * VEC);
+                rn_unpack(px[j], u[0] + j * VEC);
+                rn_unpack(pr[j], h[0] + j * VEC);
             }
-            fetch(row + groups);             // the next row's loads run under this row's sums
-            float2 st1[1], st2[1] = {make_float2(0.f, 1.f)};
-            rn_normalise<1, N, VEC, BLOCK, false>(uu, st1, have, a.norm1, inv_c, a.eps, lpr, scratch);
+            fetch(row + groups);
+            float2 st1[1], st2[1];
+            rn_normalise<1, N, VEC, WARPS, false>(u, st1, have, a.norm1, inv_c, a.eps, lpr, scratch);
 #pragma unroll
-            for (int j = 0; j < VPT; ++j) {
-                float g[VEC], w[VEC], b[VEC];
-                if constexpr (!HOIST) {
-                    const int c = have[j] ? col[j] : 0;
-                    rn_param<T, VEC>(a, kG, s, c, g);
-                    rn_param<T, VEC>(a, kW1, s, c, w);
-                    rn_param<T, VEC>(a, kB1, s, c, b);
-                }
+            for (int n = 0; n < N; ++n)
+                h[0][n] = have[n / VEC] ? a.alpha * h[0][n] + pg[n] * (u[0][n] * pw1[n] + pb1[n]) : 0.f;
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) {
-                    const int n = j * VEC + i;
-                    if constexpr (HOIST) { g[i] = pg[n]; w[i] = pw1[n]; b[i] = pb1[n]; }
-                    h[n] = have[j] ? a.alpha * h[n] + g[i] * (u[n] * w[i] + b[i]) : 0.f;
-                }
-                if (have[j] && row < end) rn_store((T *)a.h + row * C + col[j], h + j * VEC, (RnPack<T, VEC> *)nullptr);
-            }
+            for (int j = 0; j < VPT; ++j)
+                if (have[j] && row < end) rn_store((T *)a.h + row * C + col[j], h[0] + j * VEC, (RnPack<T, VEC> *)nullptr);
+            rn_normalise<1, N, VEC, WARPS, false>(h, st2, have, a.norm2, inv_c, a.eps, lpr, scratch);
             if (a.norm2 != SPCONV_NORM_NONE) {
-                rn_normalise<1, N, VEC, BLOCK, false>(hh, st2, have, a.norm2, inv_c, a.eps, lpr, scratch);
 #pragma unroll
-                for (int j = 0; j < VPT; ++j) {
-                    float w[VEC], b[VEC];
-                    if constexpr (!HOIST) {
-                        const int c = have[j] ? col[j] : 0;
-                        rn_param<T, VEC>(a, kW2, s, c, w);
-                        rn_param<T, VEC>(a, kB2, s, c, b);
-                    }
+                for (int n = 0; n < N; ++n) h[0][n] = h[0][n] * pw2[n] + pb2[n];
 #pragma unroll
-                    for (int i = 0; i < VEC; ++i) {
-                        const int n = j * VEC + i;
-                        if constexpr (HOIST) { w[i] = pw2[n]; b[i] = pb2[n]; }
-                        h[n] = h[n] * w[i] + b[i];
-                    }
-                    if (have[j] && row < end) rn_store((T *)a.y + row * C + col[j], h + j * VEC, (RnPack<T, VEC> *)nullptr);
-                }
+                for (int j = 0; j < VPT; ++j)
+                    if (have[j] && row < end) rn_store((T *)a.y + row * C + col[j], h[0] + j * VEC, (RnPack<T, VEC> *)nullptr);
             }
             if (a.stats && lane == 0 && row < end) a.stats[row] = make_float4(st1[0].x, st1[0].y, st2[0].x, st2[0].y);
         }
@@ -420,31 +413,26 @@ residual_norm_fwd_kernel(const __grid_constant__ RnArgs a) {
     }
 }
 
-// As the forward's walk. The parameter sums are kept per lane (N <= 8) or per warp in shared
-// memory, added up over the block in a fixed order when a sample's rows in the chunk end, and
-// written as record blockIdx + s: along a walk through the chunks and samples that index only
-// grows, so each (chunk, sample) pair that holds rows has a record of its own and at most
-// G + B - 1 are needed.
-template <typename T, int VEC, int VPT, bool BLOCK>
-__global__ void __launch_bounds__(kRnThreads)
+// As the forward's walk. When a sample's rows in the chunk end, the parameter sums are written as record
+// blockIdx + s (added up over the block's warps first, in a fixed order, where those share rows' columns):
+// along a walk through the chunks and samples that index only grows, so each (chunk, sample) pair that
+// holds rows has a record of its own and at most G + B - 1 are needed.
+template <typename T, int VEC, int VPT, int WARPS>
+__global__ void __launch_bounds__(RnDirect<T, VEC, VPT, WARPS>::kThreads)
 residual_norm_bwd_kernel(const __grid_constant__ RnArgs a) {
-    constexpr int N = VEC * VPT;
-    constexpr bool HOIST = N <= 8;
-    constexpr int kCopies = BLOCK ? 1 : kRnWarps;
-    extern __shared__ float s_acc[];         // [kCopies][nslots][C]
-    __shared__ float2 scratch[kRnWarps];
+    constexpr int N = VEC * VPT, kThreads = RnDirect<T, VEC, VPT, WARPS>::kThreads;
+    extern __shared__ float s_acc[];         // WARPS == 0: [kRnWarps][nslots][C]
+    __shared__ float2 part[2 * (WARPS ? WARPS : 1)];
+    RnScratch scratch{part, 0};
     rn_check_offsets(a);
-    const int C = a.C, lpr = a.lpr, warp = threadIdx.x >> 5;
-    const int lanes = BLOCK ? kRnThreads : lpr;
-    const int groups = BLOCK ? 1 : kRnThreads / lpr;
-    const int group = BLOCK ? 0 : threadIdx.x / lpr, lane = BLOCK ? threadIdx.x : threadIdx.x & (lpr - 1);
+    const int C = a.C, lpr = WARPS ? kThreads : a.lpr, warp = threadIdx.x >> 5;
+    const int groups = kThreads / lpr, group = threadIdx.x / lpr, lane = threadIdx.x & (lpr - 1);
     const float inv_c = 1.f / (float)C;
-    float *mine = s_acc + (BLOCK ? 0 : (int64_t)warp * a.nslots * C);
     int col[VPT];
     bool have[VPT];
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
-        col[j] = (lane + lanes * j) * VEC;
+        col[j] = (lane + lpr * j) * VEC;
         have[j] = col[j] < C;
     }
     const int64_t row0 = (int64_t)blockIdx.x * a.chunk, row1 = min(a.M, row0 + a.chunk);
@@ -452,46 +440,18 @@ residual_norm_bwd_kernel(const __grid_constant__ RnArgs a) {
     for (int64_t seg = row0; seg < row1; ++s) {
         const int64_t end = s < a.B - 1 ? min(row1, (int64_t)__ldg(a.offsets + s + 1)) : row1;
         if (end <= seg) continue;
-        float pg[HOIST ? N : 1], pw1[HOIST ? N : 1], pb1[HOIST ? N : 1], pw2[HOIST ? N : 1];
-        float acc[kRnParams][HOIST ? N : 1];
-        if constexpr (HOIST) {
+        float pg[N], pw1[N], pb1[N], pw2[N];
+        float sum_g[N], sum_gn[N], sum_y[N], sum_yn[N];       // of G, G * xhat, dy, dy * hhat
 #pragma unroll
-            for (int j = 0; j < VPT; ++j) {
-                const int c = have[j] ? col[j] : 0;
-                rn_param<T, VEC>(a, kG, s, c, pg + j * VEC);
-                rn_param<T, VEC>(a, kW1, s, c, pw1 + j * VEC);
-                rn_param<T, VEC>(a, kB1, s, c, pb1 + j * VEC);
-                rn_param<T, VEC>(a, kW2, s, c, pw2 + j * VEC);
-            }
-#pragma unroll
-            for (int k = 0; k < kRnParams; ++k)
-#pragma unroll
-                for (int i = 0; i < N; ++i) acc[k][i] = 0.f;
-        } else {
-            for (int i = threadIdx.x; i < kCopies * a.nslots * C; i += kRnThreads) s_acc[i] = 0.f;
-            __syncthreads();
+        for (int j = 0; j < VPT; ++j) {
+            const int c = have[j] ? col[j] : 0;
+            rn_param<T, VEC>(a, kG, s, c, pg + j * VEC);
+            rn_param<T, VEC>(a, kW1, s, c, pw1 + j * VEC);
+            rn_param<T, VEC>(a, kB1, s, c, pb1 + j * VEC);
+            rn_param<T, VEC>(a, kW2, s, c, pw2 + j * VEC);
         }
-        // adds VEC values into parameter k's sums (shared-memory form: a lane's own columns of
-        // its warp's copy)
-        auto add = [&](int k, int j, const float *v) {
-            if constexpr (HOIST) {
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) acc[k][j * VEC + i] += v[i];
-            } else {
-                if (a.slot[k] < 0 || !have[j]) return;
-                float *d = mine + (int64_t)a.slot[k] * C + col[j];
-                if constexpr (VEC == 8) {
-                    float4 *q = reinterpret_cast<float4 *>(d);
-                    float4 u = q[0], w = q[1];
-                    u.x += v[0]; u.y += v[1]; u.z += v[2]; u.w += v[3];
-                    w.x += v[4]; w.y += v[5]; w.z += v[6]; w.w += v[7];
-                    q[0] = u;
-                    q[1] = w;
-                } else {
-                    *d += v[0];
-                }
-            }
-        };
+        for (int n = 0; n < N; ++n) sum_g[n] = sum_gn[n] = sum_y[n] = sum_yn[n] = 0.f;
         RnPack<T, VEC> px[VPT], pr[VPT], ph[VPT], py[VPT];
         auto fetch = [&](int64_t row) {
 #pragma unroll
@@ -509,129 +469,95 @@ residual_norm_bwd_kernel(const __grid_constant__ RnArgs a) {
                 }
             }
         };
-        if constexpr (HOIST) fetch(seg + group);
+        fetch(seg + group);
         for (int64_t base = seg; base < end; base += groups) {
             const int64_t row = base + group;
-            if constexpr (!HOIST) fetch(row);
-            float n1_[1][N], n2_[1][N], t_[1][N], gr_[1][N];
-            float (&n1)[N] = n1_[0], (&n2)[N] = n2_[0], (&t)[N] = t_[0], (&gr)[N] = gr_[0];   // xhat, hhat, dy * w2, dh -> G
             const bool live = row < end;         // a row past the end holds zeros and adds none
+            float n1[1][N], n2[1][N], t[1][N], g[1][N];       // xhat, hhat, dy * w2, dh -> G
             const float4 st = live ? __ldg(a.stats + row) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int j = 0; j < VPT; ++j) {
-                rn_unpack(px[j], n1 + j * VEC);
-                rn_unpack(pr[j], n2 + j * VEC);
-                rn_unpack(ph[j], gr + j * VEC);
-                rn_unpack(py[j], t + j * VEC);
+                rn_unpack(px[j], n1[0] + j * VEC);
+                rn_unpack(pr[j], n2[0] + j * VEC);
+                rn_unpack(ph[j], g[0] + j * VEC);
+                rn_unpack(py[j], t[0] + j * VEC);
             }
-            if constexpr (HOIST) fetch(row + groups);
+            fetch(row + groups);
             const float rstd1[1] = {st.y}, rstd2[1] = {st.w};
 #pragma unroll
-            for (int n = 0; n < N; ++n) n1[n] = have[n / VEC] ? (n1[n] - st.x) * st.y : 0.f;
-#pragma unroll
-            for (int j = 0; j < VPT; ++j) {
-                float g[VEC], w[VEC], b[VEC];
-                if constexpr (!HOIST) {
-                    const int c = have[j] ? col[j] : 0;
-                    rn_param<T, VEC>(a, kG, s, c, g);
-                    rn_param<T, VEC>(a, kW1, s, c, w);
-                    rn_param<T, VEC>(a, kB1, s, c, b);
-                }
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) {
-                    const int n = j * VEC + i;
-                    if constexpr (HOIST) { g[i] = pg[n]; w[i] = pw1[n]; b[i] = pb1[n]; }
-                    n2[n] = have[j] ? a.alpha * n2[n] + g[i] * (n1[n] * w[i] + b[i]) : 0.f;
-                }
-            }
+            for (int n = 0; n < N; ++n) n1[0][n] = have[n / VEC] ? (n1[0][n] - st.x) * st.y : 0.f;
             if (a.norm2 != SPCONV_NORM_NONE && a.dy) {
 #pragma unroll
-                for (int n = 0; n < N; ++n) n2[n] = have[n / VEC] ? (n2[n] - st.z) * st.w : 0.f;
-#pragma unroll
-                for (int j = 0; j < VPT; ++j) {
-                    float w[VEC], v[VEC];
-                    if constexpr (!HOIST) rn_param<T, VEC>(a, kW2, s, have[j] ? col[j] : 0, w);
-                    if (live) add(kB2, j, t + j * VEC);
-#pragma unroll
-                    for (int i = 0; i < VEC; ++i) {
-                        const int n = j * VEC + i;
-                        if constexpr (HOIST) w[i] = pw2[n];
-                        v[i] = t[n] * n2[n];
-                        t[n] *= w[i];
-                    }
-                    if (live) add(kW2, j, v);
+                for (int n = 0; n < N; ++n) {
+                    const float h = a.alpha * n2[0][n] + pg[n] * (n1[0][n] * pw1[n] + pb1[n]);
+                    n2[0][n] = have[n / VEC] ? (h - st.z) * st.w : 0.f;
+                    sum_y[n] += t[0][n];
+                    sum_yn[n] = fmaf(t[0][n], n2[0][n], sum_yn[n]);
+                    t[0][n] *= pw2[n];
                 }
-                rn_normalise_back<1, N, BLOCK>(gr_, t_, n2_, rstd2, a.norm2, inv_c, lpr, scratch);
+                rn_normalise_back<1, N, WARPS>(g, t, n2, rstd2, a.norm2, inv_c, lpr, scratch);
+#pragma unroll
+                for (int n = 0; n < N; ++n) g[0][n] = have[n / VEC] && live ? g[0][n] : 0.f;
             }
+            if (a.dr) {
 #pragma unroll
-            for (int j = 0; j < VPT; ++j) {
-                float g[VEC], w[VEC], b[VEC], v[VEC], o[VEC];
-                if constexpr (!HOIST) {
-                    const int c = have[j] ? col[j] : 0;
-                    rn_param<T, VEC>(a, kG, s, c, g);
-                    rn_param<T, VEC>(a, kW1, s, c, w);
-                    rn_param<T, VEC>(a, kB1, s, c, b);
-                }
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) {
-                    const int n = j * VEC + i;
-                    if constexpr (HOIST) { g[i] = pg[n]; w[i] = pw1[n]; b[i] = pb1[n]; }
-                    const float d = have[j] ? gr[n] : 0.f;
-                    o[i] = a.alpha * d;
-                    v[i] = d * (n1[n] * w[i] + b[i]);
-                    gr[n] = d * g[i];            // du
-                }
-                if (a.dr && have[j] && live) rn_store((T *)a.dr + row * C + col[j], o, (RnPack<T, VEC> *)nullptr);
-                if (live) {
-                    add(kG, j, v);
-                    add(kB1, j, gr + j * VEC);
-                }
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) {
-                    const int n = j * VEC + i;
-                    v[i] = gr[n] * n1[n];
-                    gr[n] *= w[i];
-                }
-                if (live) add(kW1, j, v);
-            }
-            if (a.dx) {
-#pragma unroll
-                for (int n = 0; n < N; ++n) t[n] = 0.f;
-                rn_normalise_back<1, N, BLOCK>(t_, gr_, n1_, rstd1, a.norm1, inv_c, lpr, scratch);
+                for (int n = 0; n < N; ++n) t[0][n] = a.alpha * g[0][n];
 #pragma unroll
                 for (int j = 0; j < VPT; ++j)
-                    if (have[j] && live) rn_store((T *)a.dx + row * C + col[j], t + j * VEC, (RnPack<T, VEC> *)nullptr);
+                    if (have[j] && live) rn_store((T *)a.dr + row * C + col[j], t[0] + j * VEC, (RnPack<T, VEC> *)nullptr);
+            }
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                sum_g[n] += g[0][n];
+                sum_gn[n] = fmaf(g[0][n], n1[0][n], sum_gn[n]);
+                g[0][n] *= pg[n] * pw1[n];
+                t[0][n] = 0.f;
+            }
+            if (a.dx) {
+                rn_normalise_back<1, N, WARPS>(t, g, n1, rstd1, a.norm1, inv_c, lpr, scratch);
+#pragma unroll
+                for (int j = 0; j < VPT; ++j)
+                    if (have[j] && live) rn_store((T *)a.dx + row * C + col[j], t[0] + j * VEC, (RnPack<T, VEC> *)nullptr);
             }
         }
         if (a.nslots > 0) {
-            if constexpr (HOIST) {
-                // lanes of a warp that own the same columns, then one copy per warp
+            const int n_rec = a.nslots * C;
+            float *rec = a.partial + ((int64_t)blockIdx.x + s) * n_rec;
+            float *dst = WARPS ? rec : s_acc + (int64_t)warp * n_rec;
+            if constexpr (WARPS == 0) {      // lanes of a warp that own the same columns
 #pragma unroll
-                for (int k = 0; k < kRnParams; ++k) {
-                    if (a.slot[k] < 0) continue;
-#pragma unroll
-                    for (int i = 0; i < N; ++i)
-                        for (int o = lpr; o < 32; o <<= 1) acc[k][i] += __shfl_xor_sync(0xffffffffu, acc[k][i], o);
-                    if ((threadIdx.x & 31) < lpr) {
-#pragma unroll
-                        for (int j = 0; j < VPT; ++j)
-                            if (have[j])
-#pragma unroll
-                                for (int i = 0; i < VEC; ++i)
-                                    mine[(int64_t)a.slot[k] * C + col[j] + i] = acc[k][j * VEC + i];
+                for (int n = 0; n < N; ++n)
+                    for (int o = lpr; o < 32; o <<= 1) {
+                        sum_g[n] += __shfl_xor_sync(0xffffffffu, sum_g[n], o);
+                        sum_gn[n] += __shfl_xor_sync(0xffffffffu, sum_gn[n], o);
+                        sum_y[n] += __shfl_xor_sync(0xffffffffu, sum_y[n], o);
+                        sum_yn[n] += __shfl_xor_sync(0xffffffffu, sum_yn[n], o);
                     }
+            }
+            // G's sums give the gate's, weight's and bias's: u = xhat * w1 + b1 and du = G * g with w1, b1
+            // and g the same for all of a sample's rows
+            if (WARPS || (int)(threadIdx.x & 31) < lpr) {
+#pragma unroll
+                for (int n = 0; n < N; ++n) {
+                    const int c = col[n / VEC] + n % VEC;
+                    if (!have[n / VEC]) continue;
+                    if (a.slot[kG] >= 0) dst[a.slot[kG] * C + c] = pw1[n] * sum_gn[n] + pb1[n] * sum_g[n];
+                    if (a.slot[kW1] >= 0) dst[a.slot[kW1] * C + c] = pg[n] * sum_gn[n];
+                    if (a.slot[kB1] >= 0) dst[a.slot[kB1] * C + c] = pg[n] * sum_g[n];
+                    if (a.slot[kB2] >= 0) dst[a.slot[kB2] * C + c] = sum_y[n];
+                    if (a.slot[kW2] >= 0) dst[a.slot[kW2] * C + c] = sum_yn[n];
                 }
             }
-            __syncthreads();
-            const int n = a.nslots * C;
-            float *rec = a.partial + ((int64_t)blockIdx.x + s) * n;
-            for (int i = threadIdx.x; i < n; i += kRnThreads) {
-                float v = 0.f;
+            if constexpr (WARPS == 0) {
+                __syncthreads();
+                for (int i = threadIdx.x; i < n_rec; i += kThreads) {
+                    float v = 0.f;
 #pragma unroll
-                for (int w = 0; w < kCopies; ++w) v += s_acc[(int64_t)w * n + i];
-                rec[i] = v;
+                    for (int w = 0; w < kRnWarps; ++w) v += s_acc[(int64_t)w * n_rec + i];
+                    rec[i] = v;
+                }
+                __syncthreads();
             }
-            __syncthreads();
         }
         seg = end;
     }
@@ -798,6 +724,7 @@ residual_norm_bulk_kernel(const __grid_constant__ RnArgs a, const __grid_constan
             have[j] = FULL || col[j] < C;
         }
         float acc[kSums][BWD ? N : 1] = {};
+        RnScratch scratch{nullptr, 0};       // rows stay within a warp
         uint32_t flush_phase = 0;
         // All row warps: an mbarrier rather than bar.sync, since its wait is bounded.
         auto meet = [&]() {
@@ -948,11 +875,11 @@ residual_norm_bulk_kernel(const __grid_constant__ RnArgs a, const __grid_constan
                 };
                 if constexpr (!BWD) {
                     float2 st1[U], st2[U];
-                    rn_normalise<U, N, VEC, false, FULL>(n1, st1, have, a.norm1, inv_c, a.eps, lpr, nullptr);
+                    rn_normalise<U, N, VEC, 0, FULL>(n1, st1, have, a.norm1, inv_c, a.eps, lpr, scratch);
                     hidden();
 #pragma unroll
                     for (int u = 0; u < U; ++u) write(u, tx, n2[u]);
-                    rn_normalise<U, N, VEC, false, FULL>(n2, st2, have, a.norm2, inv_c, a.eps, lpr, nullptr);
+                    rn_normalise<U, N, VEC, 0, FULL>(n2, st2, have, a.norm2, inv_c, a.eps, lpr, scratch);
                     if (a.norm2 != SPCONV_NORM_NONE) {
                         par_all(kW2, p);
                         par_all(kB2, q);
@@ -1000,7 +927,7 @@ residual_norm_bulk_kernel(const __grid_constant__ RnArgs a, const __grid_constan
                                 t2[u][n] *= p[n];
                             }
                         }
-                        rn_normalise_back<U, N, false>(g, t2, n2, rstd2, a.norm2, inv_c, lpr, nullptr);
+                        rn_normalise_back<U, N, 0>(g, t2, n2, rstd2, a.norm2, inv_c, lpr, scratch);
                         if constexpr (TAIL || !FULL) {
 #pragma unroll
                             for (int u = 0; u < U; ++u)
@@ -1027,7 +954,7 @@ residual_norm_bulk_kernel(const __grid_constant__ RnArgs a, const __grid_constan
                             t2[u][n] = 0.f;
                         }
                     if (a.dx) {
-                        rn_normalise_back<U, N, false>(t2, g, n1, rstd1, a.norm1, inv_c, lpr, nullptr);
+                        rn_normalise_back<U, N, 0>(t2, g, n1, rstd1, a.norm1, inv_c, lpr, scratch);
 #pragma unroll
                         for (int u = 0; u < U; ++u) write(u, tx, t2[u]);
                     }
@@ -1120,28 +1047,24 @@ static int rn_pow2(int n) {
     return p;
 }
 
-// CTAs for M rows: enough to fill the SMs twice over, no more than there are row groups.
-static int64_t rn_grid(int64_t M, int rows_per_block) {
-    const int64_t most = 148 * 4;
-    return std::max<int64_t>(1, std::min<int64_t>(most, (M + rows_per_block - 1) / rows_per_block));
+// Blocks for M rows: enough to fill the SMs, no more than there are row groups.
+static int64_t rn_grid(int64_t M, int C, int rows_per_block) {
+    const int64_t per_sm = C <= 256 ? 4 : C <= 512 ? 12 : C <= 1024 ? 6 : C <= 2048 ? 3 : 1;
+    return std::max<int64_t>(1, std::min<int64_t>(148 * per_sm, (M + rows_per_block - 1) / rows_per_block));
 }
 
-template <typename T, int VEC, int VPT, bool BLOCK>
+template <typename T, int VEC, int VPT, int WARPS>
 static int rn_launch(RnArgs &a, bool backward, cudaStream_t st) {
-    const int rows = BLOCK ? 1 : kRnThreads / a.lpr;
-    int64_t grid = rn_grid(a.M, rows);
+    constexpr int threads = RnDirect<T, VEC, VPT, WARPS>::kThreads;
+    int64_t grid = rn_grid(a.M, a.C, WARPS ? 1 : threads / a.lpr);
     a.chunk = (a.M + grid - 1) / grid;
     grid = (a.M + a.chunk - 1) / a.chunk;
     if (!backward) {
-        residual_norm_fwd_kernel<T, VEC, VPT, BLOCK><<<(unsigned)grid, kRnThreads, 0, st>>>(a);
+        residual_norm_fwd_kernel<T, VEC, VPT, WARPS><<<(unsigned)grid, threads, 0, st>>>(a);
         return check_launch("residual_norm_fwd_kernel");
     }
-    const size_t smem = (size_t)(BLOCK ? 1 : kRnWarps) * a.nslots * a.C * sizeof(float);
-    auto kern = residual_norm_bwd_kernel<T, VEC, VPT, BLOCK>;
-    if (smem > 48 * 1024 &&
-        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
-        return check_launch("residual_norm_bwd: set max dynamic shared memory");
-    kern<<<(unsigned)grid, kRnThreads, smem, st>>>(a);
+    const size_t smem = WARPS ? 0 : (size_t)kRnWarps * a.nslots * a.C * sizeof(float);    // at most 40 KB
+    residual_norm_bwd_kernel<T, VEC, VPT, WARPS><<<(unsigned)grid, threads, smem, st>>>(a);
     return check_launch("residual_norm_bwd_kernel");
 }
 
@@ -1185,8 +1108,8 @@ static bool rb_launch(RnArgs &a, cudaStream_t st, int &rc) {
 }
 
 // Columns a lane owns: eight neighbours at a time where rows and parameters allow 16-byte
-// accesses, single columns otherwise; the fewest that cover the row with one warp, and a block
-// of eight warps per row beyond 1,024 channels.
+// accesses, single columns otherwise; the fewest that cover the row with one warp, and eight with as
+// many warps as cover it beyond 256 channels.
 template <typename T>
 static int rn_dispatch(RnArgs &a, bool vec, bool aligned, bool backward, cudaStream_t st) {
     const int C = a.C;
@@ -1215,17 +1138,20 @@ static int rn_dispatch(RnArgs &a, bool vec, bool aligned, bool backward, cudaStr
     }
     a.lpr = std::min(32, rn_pow2(vec ? C / 8 : C));
     if (vec) {
-        if (C <= 256) return rn_launch<T, 8, 1, false>(a, backward, st);
-        if (C <= 512) return rn_launch<T, 8, 2, false>(a, backward, st);
-        if (C <= 1024) return rn_launch<T, 8, 4, false>(a, backward, st);
-        return rn_launch<T, 8, 4, true>(a, backward, st);
+        if (C <= 256) return rn_launch<T, 8, 1, 0>(a, backward, st);
+        if (C <= 512) return rn_launch<T, 8, 1, 2>(a, backward, st);
+        if (C <= 1024) return rn_launch<T, 8, 1, 4>(a, backward, st);
+        if (C <= 2048) return rn_launch<T, 8, 1, 8>(a, backward, st);
+        return rn_launch<T, 8, 1, 32>(a, backward, st);
     }
-    if (C <= 32) return rn_launch<T, 1, 1, false>(a, backward, st);
-    if (C <= 64) return rn_launch<T, 1, 2, false>(a, backward, st);
-    if (C <= 128) return rn_launch<T, 1, 4, false>(a, backward, st);
-    if (C <= 256) return rn_launch<T, 1, 8, false>(a, backward, st);
-    if (C <= 1024) return rn_launch<T, 1, 32, false>(a, backward, st);
-    return rn_launch<T, 1, 32, true>(a, backward, st);
+    if (C <= 32) return rn_launch<T, 1, 1, 0>(a, backward, st);
+    if (C <= 64) return rn_launch<T, 1, 2, 0>(a, backward, st);
+    if (C <= 128) return rn_launch<T, 1, 4, 0>(a, backward, st);
+    if (C <= 256) return rn_launch<T, 1, 8, 0>(a, backward, st);
+    if (C <= 512) return rn_launch<T, 1, 8, 2>(a, backward, st);
+    if (C <= 1024) return rn_launch<T, 1, 8, 4>(a, backward, st);
+    if (C <= 2048) return rn_launch<T, 1, 8, 8>(a, backward, st);
+    return rn_launch<T, 1, 8, 32>(a, backward, st);
 }
 
 static bool rn_aligned(const void *p) { return ((uintptr_t)p & 15) == 0; }
@@ -1305,7 +1231,7 @@ using namespace spconv;
 
 extern "C" int64_t spconv_residual_norm_workspace_bytes(int64_t num_rows, int channels, int num_samples) {
     if (num_rows < 0 || channels < 1 || channels > kRnMaxC || num_samples < 1 || num_samples > kRnMaxSamples) return -1;
-    return (rn_grid(num_rows, 1) + num_samples) * kRnParams * channels * (int64_t)sizeof(float);
+    return (rn_grid(num_rows, channels, 1) + num_samples) * kRnParams * channels * (int64_t)sizeof(float);
 }
 
 extern "C" int spconv_residual_norm_forward(const spconv_residual_norm_args *q, void *stream) {
