@@ -55,7 +55,7 @@ struct RnArgs {
     int B;
     int64_t M;
     int C;
-    int lpr;                             // lanes per row (BLOCK: unused)
+    int lpr;                             // lanes per row (unused where a block takes a row)
     int64_t chunk;                       // consecutive rows per CTA
     int norm1, norm2;
     float alpha, eps;
@@ -198,9 +198,9 @@ __device__ __forceinline__ float rn_tree(const float (&t)[N]) {
 #pragma unroll
     for (int i = 0; i < N; ++i) s[i] = t[i];
 #pragma unroll
-    for (int w = N / 2; w > 0; w >>= 1)
+    for (int n = N; n > 1; n = (n + 1) / 2)
 #pragma unroll
-        for (int i = 0; i < w; ++i) s[i] += s[i + w];
+        for (int i = 0; i < n / 2; ++i) s[i] += s[i + (n + 1) / 2];
     return s[0];
 }
 template <int N>
@@ -1077,9 +1077,8 @@ static bool rb_launch(RnArgs &a, cudaStream_t st, int &rc) {
     constexpr int N = VEC * VPT;
     // Warps and rows in hand, measured at 1.34 M x 128 bf16: forward with 12 warps 246 us at two rows of
     // sixteen columns a lane, 340 us at one; backward with 10 warps 438 us at two rows of eight, with
-    // 12 (128 registers) 490 us, with 8 504 us, with 20 at one row 769 us. Single columns a lane need
-    // fewer registers: 15 warps.
-    constexpr int W = VEC == 1 ? 15 : BWD ? 10 : 12, U = N >= 4 ? 2 : 4;
+    // 12 (128 registers) 490 us, with 8 504 us, with 20 at one row 769 us.
+    constexpr int W = BWD ? 10 : 12, U = 2;
     const int row_bytes = a.C * (int)sizeof(T), groups = W * 32 / a.lpr * U;
     const int unit = std::lcm(groups, 8);    // whole passes, and tiles of whole 16 bytes
     RbArgs rb = {};
@@ -1126,13 +1125,18 @@ static int rn_dispatch(RnArgs &a, bool vec, bool aligned, bool backward, cudaStr
             ran = backward ? (full ? rb_launch<T, 8, 1, true, true>(a, st, rc) : rb_launch<T, 8, 1, true, false>(a, st, rc))
                            : (full ? rb_launch<T, 8, 1, false, true>(a, st, rc) : rb_launch<T, 8, 1, false, false>(a, st, rc));
         } else {
-            a.lpr = std::min(32, rn_pow2(C));
+            // single columns: as few lanes a row as eight columns each allow, and no more columns each than
+            // that takes (35 channels: 8 lanes of 5)
+            a.lpr = 1;
+            while ((C + a.lpr - 1) / a.lpr > 8) a.lpr <<= 1;
             auto single = [&](auto per) {
                 constexpr int P = decltype(per)::value;
                 return backward ? rb_launch<T, 1, P, true, false>(a, st, rc) : rb_launch<T, 1, P, false, false>(a, st, rc);
             };
-            ran = C <= 32 ? single(std::integral_constant<int, 1>{}) : C <= 64 ? single(std::integral_constant<int, 2>{})
-                : C <= 128 ? single(std::integral_constant<int, 4>{}) : single(std::integral_constant<int, 8>{});
+            const int per = (C + a.lpr - 1) / a.lpr;
+            ran = per <= 4 ? single(std::integral_constant<int, 4>{}) : per == 5 ? single(std::integral_constant<int, 5>{})
+                : per == 6 ? single(std::integral_constant<int, 6>{}) : per == 7 ? single(std::integral_constant<int, 7>{})
+                : single(std::integral_constant<int, 8>{});
         }
         if (ran) return rc;
     }
