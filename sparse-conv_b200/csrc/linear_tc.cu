@@ -28,6 +28,9 @@
 // warp and is slower, 192 us.
 // The weight gradient's K is the voxels: K is cut into splits, each writes fp32 sums of its own,
 // and linear_reduce_kernel adds them in a fixed order.
+// Measured (bf16): 1.34 M x 128 -> 128 112 us (6.1 TB/s) and its input gradient 112 us; 2 M x 64 -> 256
+// 217 to 230 us (5.6 to 5.9 TB/s), 287 us with GELU, 330 us with SiLU: those two are bound by the
+// epilogue's issue slots, about 20 a value with the exponentials'.
 // Every wait is bounded (the conv kernels' limit); a timeout raises SPCONV_STATUS_WAIT_TIMEOUT and
 // the CTA waits (bounded) for its own copies and MMAs before it frees TMEM and exits.
 #include <algorithm>

@@ -570,8 +570,8 @@ residual_norm_bwd_kernel(const __grid_constant__ RnArgs a) {
 // count. One thread keeps a ring of stages of such copies in flight; the other warps compute in
 // place (the outputs take the inputs' slots) and the same thread stores finished stages in bulk.
 // The direct kernels above hold what is in flight in registers (two loads a lane); measured
-// there and here: 2.0 M x 64 bf16 forward 255 and 181 us (5.6 TB/s), 1.34 M x 128 forward 328 and
-// 246 us (5.6 TB/s), backward 738 and 438 us (4.7 TB/s). The backward issues 50 instructions a
+// there and here: 2.0 M x 64 bf16 forward 255 and 172 us (6.0 TB/s), 1.34 M x 128 forward 328 and
+// 243 us (5.7 TB/s), backward 738 and 426 us (4.9 TB/s). The backward issues 50 instructions a
 // value and spends most of its stalls on the row reductions' shuffles.
 // A tile that crosses a sample's end is worked off in two parts, so tiles stay aligned to 16
 // bytes for every channel count; only the last one can end in a few odd bytes, which that thread
