@@ -312,7 +312,7 @@ __device__ __forceinline__ int rn_sample(const RnArgs &a, int64_t r) {
 
 // Offsets have to ascend from 0 to M; whatever they hold, rows are assigned inside [0, B).
 __device__ __forceinline__ void rn_check_offsets(const RnArgs &a) {
-    if (blockIdx.x != 0 || a.B <= 1) return;
+    if (blockIdx.x != 0 || !a.offsets) return;
     bool bad = false;
     for (int s = threadIdx.x; s < a.B; s += blockDim.x) {
         const int lo = __ldg(a.offsets + s), hi = __ldg(a.offsets + s + 1);
@@ -1191,7 +1191,7 @@ static int rn_args(const spconv_residual_norm_args *q, RnArgs &a, bool &vec, boo
     a.status = q->status;
     a.stats = (float4 *)q->row_stats;
     SPCONV_REQUIRE(rn_aligned(a.stats), SPCONV_ERR_ARG, "row_stats is not 16-byte aligned");
-    a.offsets = q->offsets;
+    a.offsets = nullptr;                     // only read where a parameter has a row per sample
     a.B = 1;
     a.nslots = 0;
     a.partial = (float *)q->workspace;
@@ -1214,11 +1214,15 @@ static int rn_args(const spconv_residual_norm_args *q, RnArgs &a, bool &vec, boo
         SPCONV_REQUIRE(p.dtype == SPCONV_F32 || p.dtype == q->dtype, SPCONV_ERR_ARG,
                        "parameters must be fp32 or of the features' type");
         vec = vec && rn_aligned(p.data);
-        if (p.per_sample) a.B = q->num_samples;
+        if (p.per_sample) {
+            a.B = q->num_samples;
+            a.offsets = q->offsets;
+        }
         if (backward && p.grad) a.slot[k] = a.nslots++;
     }
-    SPCONV_REQUIRE(a.B == 1 || a.offsets, SPCONV_ERR_ARG, "a parameter per sample needs the samples' row offsets");
-    if (a.B == 1) a.offsets = nullptr;
+    for (const auto *p : ps)
+        SPCONV_REQUIRE(!p->data || !p->per_sample || a.offsets, SPCONV_ERR_ARG,
+                       "a parameter per sample needs the samples' row offsets");
     return SPCONV_OK;
 }
 

@@ -743,6 +743,7 @@ def linear_forward(feats: torch.Tensor, weight: torch.Tensor, bias: Optional[tor
         raise ValueError(f"weight has {weight.shape[1]} input channels, feats {Ci}")
     weight = weight.contiguous()
     if bias is not None:
+        bias = bias.contiguous()
         _matrix(bias, (Co,), dtype, "bias")
     if residual is not None:
         _matrix(residual, (M, Co), dtype, "residual")

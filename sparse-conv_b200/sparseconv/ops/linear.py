@@ -34,6 +34,8 @@ class SparseLinearFunction(Function):
 
     @staticmethod
     def backward(ctx, grad_out):
+        if torch.is_grad_enabled():              # create_graph=True: these gradients would be constants
+            raise NotImplementedError("sparse_linear has no second derivative")
         feats, weight, preact = ctx.saved_tensors
         needs = ctx.needs_input_grad
         if not grad_out.is_contiguous():

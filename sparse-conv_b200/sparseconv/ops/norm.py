@@ -33,6 +33,8 @@ class ResidualNormFunction(Function):
     @staticmethod
     def backward(ctx, grad_hidden, grad_normed):
         """From the inputs, recomputed in fp32, and the forward's row statistics (16 bytes a row)."""
+        if torch.is_grad_enabled():              # create_graph=True: these gradients would be constants
+            raise NotImplementedError("sparse_residual_norm has no second derivative")
         if grad_hidden is None and grad_normed is None:
             return (None,) * 12
         feats, residual, *params, batch_offsets, stats = ctx.saved_tensors

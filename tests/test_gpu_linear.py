@@ -360,3 +360,29 @@ def test_channels_no_multiple_of_eight(M, Ci, Co, dtype, act, residual):
     _check(out.detach(), v, e, DT[dtype], "out")
     for got, ref, what in zip(grads, _backward_ref(x, w, b, g, act, DT[dtype]), ("feats", "weight", "bias")):
         _check(got, *ref, DT[dtype], what)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_bias_of_more_columns_than_shared_memory_keeps(dtype):
+    x, w, b, r, _ = _inputs(200, 64, 5000, DT[dtype], residual=True, seed=51)
+    v, e, _, _ = _forward_ref(x, w, b, r, "relu")
+    _check(sparse_linear(x, w, b, residual=r, activation="relu"), v, e, DT[dtype], "out")
+
+
+def test_more_than_2_to_31_elements():
+    """The last rows of a large call equal the same rows alone (elements beyond a 32-bit index)."""
+    M, Ci, Co = 1_100_003, 8, 2048
+    x, w, b, _, _ = _inputs(M, Ci, Co, torch.bfloat16, residual=False, seed=52)
+    out = sparse_linear(x, w, b, activation="relu")
+    assert torch.equal(out[-1000:], sparse_linear(x[-1000:].clone(), w, b, activation="relu"))
+    assert torch.equal(out[:1000], sparse_linear(x[:1000].clone(), w, b, activation="relu"))
+
+
+def test_strided_parameters_and_second_derivatives():
+    x, w, b, _, g = _inputs(300, 16, 24, torch.float32, residual=False, seed=53)
+    want = sparse_linear(x, w, b)
+    wide = torch.stack([w.t(), w.t()], -1)                       # [Ci, Co, 2]
+    assert torch.equal(sparse_linear(x, wide[..., 0].t(), torch.stack([b, b], -1)[:, 0]), want)
+    x.requires_grad_(True)
+    with pytest.raises(NotImplementedError, match="second derivative"):
+        torch.autograd.grad(sparse_linear(x, w, b), x, g, create_graph=True)

@@ -349,3 +349,36 @@ def test_only_the_wanted_gradients():
     every = dict(zip(named, grads(list(named))))
     for k in named:
         assert torch.equal(grads([k])[0], every[k]), k
+
+
+def test_bad_offsets_of_one_sample_raise():
+    x = torch.randn(100, 64, device="cuda")
+    gate = torch.randn(1, 64, device="cuda")
+    with pytest.raises(RuntimeError, match="sample offsets"):
+        sparse_residual_norm(x, x, gate=gate, batch_offsets=torch.tensor([0, 99], dtype=torch.int32, device="cuda"))
+        _native.check_errors()
+    _native.reset_status()
+    hidden, _ = sparse_residual_norm(x, x, gate=gate, batch_offsets=torch.tensor([0, 100], dtype=torch.int32, device="cuda"))
+    assert torch.allclose(hidden, x * (1 + gate), rtol=1e-6, atol=1e-6)
+
+
+@pytest.mark.parametrize("M,C", [(8_500_001, 256), (1_100_003, 2048)])
+def test_more_than_2_to_31_elements(M, C):
+    """The first and last rows of a large call equal the same rows alone, forward and backward."""
+    x = torch.randn(M, C, device="cuda", dtype=torch.bfloat16)
+    for rows in (slice(0, 1000), slice(M - 1000, M)):
+        part = x[rows].clone().requires_grad_(True)
+        whole = x.detach().requires_grad_(True)
+        y, yp = sparse_norm(whole), sparse_norm(part)
+        # another lane layout may round a statistic the other way: one rounding of the output
+        assert ((y[rows].float() - yp.float()).abs() <= 2.0 ** -7 * yp.float().abs() + 1e-6).all()
+        g = torch.autograd.grad(y, whole, x)[0][rows]
+        gp = torch.autograd.grad(yp, part, x[rows])[0]
+        assert ((g.float() - gp.float()).abs() <= 2.0 ** -7 * gp.float().abs() + 1e-5).all()
+        del y, g, whole
+
+
+def test_second_derivative_is_refused():
+    x = torch.randn(10, 8, device="cuda", requires_grad=True)
+    with pytest.raises(NotImplementedError, match="second derivative"):
+        torch.autograd.grad(sparse_norm(x).sum(), x, create_graph=True)
