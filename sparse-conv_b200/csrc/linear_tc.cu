@@ -13,9 +13,12 @@
 //   warp 0      loads: A and B tiles of each K step into a ring of stages. Where the whole of B's
 //               column block fits beside the ring it is loaded once and stays (few K steps: the
 //               layers over millions of voxels, whose bound is HBM);
-//   warp 1      MMA: one thread; the accumulators take turns in two (BN = 256) or four TMEM buffers;
+//   warp 1      MMA: one thread; the accumulators take turns in two (BN = 256), four or eight (64) TMEM
+//               buffers. With one K step a tile's cost is this thread's: eight buffers in place of four, and
+//               descriptors advanced rather than built, took 883,771 x 64 -> 16 with a residual from 44.0 to
+//               41.9 us and 1.34 M x 128 -> 128 with GELU from 127.9 to 116.0;
 //   warps 2-17  four epilogue groups of four warps (one per TMEM lane quadrant), a group per
-//               buffer, or two that share a buffer's columns: 64 columns at a time from TMEM to
+//               buffer in turn, or two that share a buffer's columns: 64 columns at a time from TMEM to
 //               registers, + bias, act, + residual, one rounding, into swizzled shared memory and out
 //               by TMA (which clips ragged edges). The residual arrives by TMA, ahead of its turn, in
 //               the slot the output leaves from. Four warps per scheduler, since GELU and SiLU are
@@ -53,7 +56,8 @@ constexpr int kLtMaxStages = 12;
 constexpr int kLtMaxSlots = 4;
 constexpr int kLtMaxSmem = 227 * 1024;
 // behind the tiles: barriers, TMEM address and abort flag, bias (fp32, at most kLtMaxBias)
-constexpr int kLtBars = 2 * kLtMaxStages + 1 + 2 * kLtEpiGroups + kLtEpiWarps * kLtMaxSlots;
+constexpr int kLtMaxBufs = 8;
+constexpr int kLtBars = 2 * kLtMaxStages + 1 + 2 * kLtMaxBufs + kLtEpiWarps * kLtMaxSlots;
 constexpr int kLtTail = (kLtBars * 8 + 8 + 15) & ~15;
 
 struct LtArgs {
@@ -101,7 +105,7 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     uint8_t *tail = base + a.b_resident * b_bytes + S * stage_bytes + (PARTIAL ? 0 : kLtEpiWarps * warp_slots * slot_bytes);
     uint64_t *bar = reinterpret_cast<uint64_t *>(tail);
     uint64_t *full = bar, *empty = full + kLtMaxStages, *bfull = empty + kLtMaxStages, *accfull = bfull + 1;
-    uint64_t *accempty = accfull + kLtEpiGroups, *rbar = accempty + kLtEpiGroups;
+    uint64_t *accempty = accfull + kLtMaxBufs, *rbar = accempty + kLtMaxBufs;
     uint32_t *s_tmem = reinterpret_cast<uint32_t *>(bar + kLtBars);
     volatile int *s_abort = reinterpret_cast<volatile int *>(s_tmem + 1);
     float *s_bias = reinterpret_cast<float *>(tail + kLtTail);
@@ -109,7 +113,7 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     // workers: CTAs, or pairs of them
     const int G = PAIR ? gridDim.x >> 1 : gridDim.x, me = PAIR ? blockIdx.x >> 1 : blockIdx.x;
-    const uint32_t tmem_cols = (uint32_t)(a.bufs * BN);                // 256 or 512
+    const uint32_t tmem_cols = 512;                                    // bufs * BN: all there are
     for (int i = tid; i < a.bias_smem; i += kLtThreads)
         s_bias[i] = i < a.N ? dtype_traits<T>::to_f(((const T *)a.bias)[i]) : 0.f;
     if (tid == 0) {
@@ -120,7 +124,7 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         mbar_init(smem_u32(bfull), 1);
         for (int g = 0; g < a.bufs; ++g) {
             mbar_init(smem_u32(&accfull[g]), 1);
-            mbar_init(smem_u32(&accempty[g]), (PAIR ? 2 : 1) * kLtEpiWarps / a.bufs);
+            mbar_init(smem_u32(&accempty[g]), (PAIR ? 2 : 1) * kLtEpiWarps / min(a.bufs, kLtEpiGroups));
         }
         for (int i = 0; i < kLtEpiWarps * NO; ++i) mbar_init(smem_u32(&rbar[i]), 1);
         *s_abort = 0;
@@ -278,11 +282,12 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                     const uint32_t sb = a.b_resident ? s_res : sa + kLtABytes;
                     s_res += b_bytes;
                     const int steps = min(4, (k1 - k + 15) >> 4);     // zeros past K's end are skipped
-                    for (int kk = 0; kk < steps; ++kk) {
-                        const uint64_t ad = A_T ? smem_desc_mn_sw128(sa + kk * 2048, 8192, 1024)
-                                                : smem_desc_kmajor_swizzled(sa + kk * 32, 128);
-                        const uint64_t bd = B_T ? smem_desc_mn_sw128(sb + kk * 2048, 8192, 1024)
-                                                : smem_desc_kmajor_swizzled(sb + kk * 32, 128);
+                    // a K step of 16 moves a descriptor's address field (16-byte units, no carry: < 2^14)
+                    uint64_t ad = A_T ? smem_desc_mn_sw128(sa, 8192, 1024) : smem_desc_kmajor_swizzled(sa, 128);
+                    uint64_t bd = B_T ? smem_desc_mn_sw128(sb, 8192, 1024) : smem_desc_kmajor_swizzled(sb, 128);
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk, ad += A_T ? 128 : 2, bd += B_T ? 128 : 2) {
+                        if (kk >= steps) break;
                         if constexpr (PAIR) tc_mma_f16_pair(d, ad, bd, idesc, (k > k0 || kk > 0) ? 1u : 0u);
                         else tc_mma_f16(d, ad, bd, idesc, (k > k0 || kk > 0) ? 1u : 0u);
                     }
@@ -303,8 +308,9 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     } else {
         // ------------------------------------------------------------------ epilogue
         const int ew = warp - 2, quad = warp & 3;
-        const int buf = (ew >> 2) % a.bufs, sub = (ew >> 2) / a.bufs, share = kLtEpiGroups / a.bufs;
-        const uint32_t t_acc = tmem + (uint32_t)(buf * BN) + ((uint32_t)(quad * 32) << 16);
+        // `turn` tiles are in the groups' hands at a time; with more buffers than that a group alternates
+        // between bufs / turn of them
+        const int turn = min(a.bufs, kLtEpiGroups), mine = (ew >> 2) % turn, sub = (ew >> 2) / turn, share = kLtEpiGroups / turn;
         const uint32_t slot0 = s_out + (uint32_t)(ew * warp_slots * slot_bytes);
         const uint32_t pre0 = slot0 + (uint32_t)(NO * slot_bytes);
         uint64_t *my_rbar = rbar + ew * NO;
@@ -319,7 +325,7 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         const int ahead = NO >= 3 ? NO - 2 : NO - 1;
         int l_slot = 0, outstanding = 0, l_chunk = sub;
         uint32_t l_phase = 0;
-        Walk lw = begin(me + buf * G, a.bufs * G);
+        Walk lw = begin(me + mine * G, turn * G);
         auto load_residual = [&](int behind) {        // the next chunk's, if there is one
             while (lw.item < a.items && l_chunk >= chunks_of(lw.n * BN)) {
                 advance(lw);
@@ -343,12 +349,14 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         if (!PARTIAL && a.has_residual)
             for (int i = 0; i < ahead; ++i) load_residual(0);
         int s = 0;
+        int buf = mine;
         uint32_t s_phase = 0, use_phase = 0;
-        for (Walk w = begin(me + buf * G, a.bufs * G); w.item < a.items; advance(w), use_phase ^= 1u) {
+        for (Walk w = begin(me + mine * G, turn * G); w.item < a.items; advance(w)) {
             const int m0 = row_of(w), n0 = w.n * BN;
             const int n_cols = min(BN, a.N - n0), chunks = chunks_of(n0);
             if (!all_wait(&accfull[buf], use_phase)) break;
             tc_fence_after();
+            const uint32_t t_acc = tmem + (uint32_t)(buf * BN) + ((uint32_t)(quad * 32) << 16);
             bool ok = true;
             for (int j = sub; j < chunks; j += share, next(s, s_phase, NO)) {
                 const uint32_t so = slot0 + s * slot_bytes + row_at, sp = pre0 + s * slot_bytes + row_at;
@@ -440,6 +448,10 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
             if (lane == 0) {
                 if constexpr (PAIR) mbar_arrive_cluster(cluster_addr(smem_u32(&accempty[buf]), 0));
                 else mbar_arrive(smem_u32(&accempty[buf]));
+            }
+            if ((buf += turn) >= a.bufs) {
+                buf = mine;
+                use_phase ^= 1u;
             }
         }
         if (!PARTIAL && lane == 0) {
@@ -533,7 +545,7 @@ static int lt_launch(const GemmArgs &g) {
     a.items = (int)items;
     a.tiles = a.items / g.splits;
     a.k_per_split = (int)(g.splits > 1 ? g.k_per_split : g.K);
-    a.bufs = a.BN == 256 ? 2 : 4;
+    a.bufs = 512 / a.BN;
     a.bias = g.bias;
     a.bias_smem = g.bias && g.N <= kLtMaxBias ? (a.N + 31) & ~31 : 0;
     a.has_residual = g.residual != nullptr;
