@@ -101,7 +101,7 @@ linear_bwd_tc_kernel(const __grid_constant__ CUtensorMap map_g, const __grid_con
 
     if (warp == 0) {
         // ------------------------------------------------------------------ loads
-        if (lane == 0) {
+        if (elect_one()) {
             int i = 0;
             bool ok = true;
             if (a.want_x && (int)blockIdx.x < a.tiles) {
@@ -130,7 +130,7 @@ linear_bwd_tc_kernel(const __grid_constant__ CUtensorMap map_g, const __grid_con
         }
     } else if (warp == 1) {
         // ------------------------------------------------------------------ MMA
-        if (lane == 0) {
+        if (elect_one()) {
             const int n_mma = (a.Ci + 15) & ~15;
             const uint32_t id_x = instr_desc_f16(dtype_traits<T>::mma_format, kLbRows, n_mma) | (1u << 16);
             const uint32_t id_w = instr_desc_f16(dtype_traits<T>::mma_format, 128, n_mma) | (1u << 15) | (1u << 16);

@@ -14,9 +14,9 @@
 //               column block fits beside the ring it is loaded once and stays (few K steps: the
 //               layers over millions of voxels, whose bound is HBM);
 //   warp 1      MMA: one thread; the accumulators take turns in two (BN = 256), four or eight (64) TMEM
-//               buffers. With one K step a tile's cost is this thread's: eight buffers in place of four, and
-//               descriptors advanced rather than built, took 883,771 x 64 -> 16 with a residual from 44.0 to
-//               41.9 us and 1.34 M x 128 -> 128 with GELU from 127.9 to 116.0;
+//               buffers. With one K step a tile's cost is this thread's: eight buffers in place of four,
+//               descriptors advanced rather than built, and an elected lane took 883,771 x 64 -> 16 with a
+//               residual from 44.0 to 34.0 us and 1.34 M x 128 -> 128 with GELU from 127.9 to 114.6;
 //   warps 2-17  four epilogue groups of four warps (one per TMEM lane quadrant), a group per
 //               buffer in turn, or two that share a buffer's columns: 64 columns at a time from TMEM to
 //               registers, + bias, act, + residual, one rounding, into swizzled shared memory and out
@@ -26,7 +26,7 @@
 // PAIR: two CTAs of a cluster, on two SMs, share a 256 x 256 tile (cta_group::2). Each holds its 128
 // rows of A, half of B's columns and its own rows' accumulators; the first one's MMA thread drives
 // both tensor cores, and commits to barriers in both. A K step then brings 32 KB into an SM instead of
-// 48. 84,000 x 512 -> 2048 bf16: 183 us unpaired, 170 us paired (1.03 PFLOP/s; the library's product
+// 48. 84,000 x 512 -> 2048 bf16: 183 us unpaired, 170 us paired (163 since, 1.08 PFLOP/s; the library's product
 // alone takes 151 us). Keeping a pair's halves of B in shared memory (K <= 512) leaves one output slot a
 // warp and is slower, 192 us.
 // The weight gradient's K is the voxels: K is cut into splits, each writes fp32 sums of its own,
@@ -192,7 +192,7 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
 
     if (warp == 0) {
         // ------------------------------------------------------------------ loads
-        if (lane == 0) {
+        if (elect_one()) {
             auto load = [&](uint32_t dst, const CUtensorMap *map, int x, int y, uint32_t mbar) {
                 if constexpr (PAIR) tma_load_2d_pair(dst, map, x, y, mbar);
                 else tma_load_2d(dst, map, x, y, mbar);
@@ -257,7 +257,7 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         }
     } else if (warp == 1) {
         // ------------------------------------------------------------------ MMA
-        if (lane == 0 && rank == 0) {
+        if (rank == 0 && elect_one()) {
             auto commit = [&](uint64_t *b) {
                 if constexpr (PAIR) tc_commit_pair(smem_u32(b));
                 else tc_commit(smem_u32(b));
