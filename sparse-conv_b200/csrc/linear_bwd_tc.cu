@@ -7,8 +7,8 @@
 // HBM. It applies where W, both accumulators and two stages of 128 rows fit an SM: see
 // bwd_tc_shape.
 //
-// 1.34 M x 128 -> 128 with GELU, bf16: 262 us (5.2 TB/s) and 473 us for the separate kernels; 2 M x 64 ->
-// 256 without activation 272 and 602 us.
+// 1.34 M x 128 -> 128 with GELU, bf16: 242 us (5.7 TB/s) and 473 us for the separate kernels; 2 M x 64 ->
+// 256 without activation 259 and 602 us.
 // One CTA per SM takes every G-th tile of 128 rows. Roles, coupled by mbarriers:
 //   warp 0       TMA loads of the tile's z, grad_out and feats rows (blocks of 64 columns, 128-byte
 //                swizzle) into one of two stages; W once, at the start;
@@ -145,19 +145,28 @@ linear_bwd_tc_kernel(const __grid_constant__ CUtensorMap map_g, const __grid_con
                 if (a.want_x && u > 0 && !wait(&accempty[s], (u - 1) & 1u)) { ok = false; break; }
                 tc_fence_after();
                 const uint32_t dz = s_stage + s * stage_bytes + z_bytes, x = dz + g_bytes;
+                // a K step moves a descriptor's address field (16-byte units; shared addresses do not carry out of it)
                 if (a.want_x) {
                     const uint32_t d = tmem + (uint32_t)(s * nci * 64);
-                    for (int k = 0; k < k_steps; ++k)
-                        tc_mma_f16(d, smem_desc_kmajor_swizzled(dz + (k >> 2) * kLbBlock + (k & 3) * 32, 128),
-                                   smem_desc_mn_sw128(s_w + (k >> 2) * nci * 8192 + (k & 3) * 2048, 8192, 1024), id_x,
-                                   k > 0 ? 1u : 0u);
+                    uint64_t dd = smem_desc_kmajor_swizzled(dz, 128), dw = smem_desc_mn_sw128(s_w, 8192, 1024);
+                    for (int k = 0; k < k_steps; k += 4, dd += kLbBlock >> 4, dw += nci * 512) {
+#pragma unroll
+                        for (int kk = 0; kk < 4; ++kk) {
+                            if (k + kk >= k_steps) break;
+                            tc_mma_f16(d, dd + kk * 2, dw + kk * 128, id_x, k + kk > 0 ? 1u : 0u);
+                        }
+                    }
                 }
-                if (a.want_w)
-                    for (int m = 0; m < nco / 2; ++m)
+                if (a.want_w) {
+                    uint64_t dd = smem_desc_mn_sw128(dz, kLbBlock, 1024);
+                    const uint64_t dx = smem_desc_mn_sw128(x, kLbBlock, 1024);
+                    for (int m = 0; m < nco / 2; ++m, dd += 2 * kLbBlock >> 4) {
+#pragma unroll
                         for (int k = 0; k < kLbRows / 16; ++k)
-                            tc_mma_f16(t_w + (uint32_t)(m * nci * 64),
-                                       smem_desc_mn_sw128(dz + 2 * m * kLbBlock + k * 2048, kLbBlock, 1024),
-                                       smem_desc_mn_sw128(x + k * 2048, kLbBlock, 1024), id_w, (i > 0 || k > 0) ? 1u : 0u);
+                            tc_mma_f16(t_w + (uint32_t)(m * nci * 64), dd + k * 128, dx + k * 128, id_w,
+                                       (i > 0 || k > 0) ? 1u : 0u);
+                    }
+                }
                 tc_commit(smem_u32(&accfull[s]));
             }
             if (ok) tc_commit(smem_u32(wdone));
@@ -190,7 +199,7 @@ linear_bwd_tc_kernel(const __grid_constant__ CUtensorMap map_g, const __grid_con
                 tc_fence_before();
                 fence_proxy_async_smem();
                 __syncwarp();
-                if (lane == 0) {
+                if (elect_one()) {
                     mbar_arrive(smem_u32(&accempty[s]));
                     if (t * kLbRows + quad * 32 < a.M)
                         for (int c = 0; c < nci; ++c)
@@ -200,7 +209,7 @@ linear_bwd_tc_kernel(const __grid_constant__ CUtensorMap map_g, const __grid_con
                     bulk_wait_read<0>();
                 }
             }
-            if (lane == 0) mbar_arrive(smem_u32(&empty[s]));
+            if (elect_one()) mbar_arrive(smem_u32(&empty[s]));
             __syncwarp();
         }
         if (ok && a.want_w && all_wait(wdone, 0)) {
@@ -223,7 +232,7 @@ linear_bwd_tc_kernel(const __grid_constant__ CUtensorMap map_g, const __grid_con
             }
             tc_fence_before();
         }
-        if (lane == 0) bulk_wait<0>();
+        if (elect_one()) bulk_wait<0>();
     } else if (HAS_ACT || a.want_b) {
         // ------------------------------------------------------------------ dz and its sums
         const int ct = tid - 6 * 32;
@@ -266,7 +275,7 @@ linear_bwd_tc_kernel(const __grid_constant__ CUtensorMap map_g, const __grid_con
             }
             if constexpr (HAS_ACT) fence_proxy_async_smem();
             __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&ready[s]));
+            if (elect_one()) mbar_arrive(smem_u32(&ready[s]));
         }
         if (ok && a.want_b) {
             const int cw = warp - 6;
