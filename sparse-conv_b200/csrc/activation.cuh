@@ -13,14 +13,18 @@ __device__ __forceinline__ float act_value(float z) {
     return z;
 }
 
+// z as a factor beside an exponential of it that is zero far out: cut off there, so that an infinite z (a kept
+// product beyond fp16's range, of a finite forward) times that zero is zero. NaN comes through the exponential.
+__device__ __forceinline__ float slope_factor(float z) { return fmaxf(fminf(z, 200.f), -200.f); }
+
 template <int ACT>
 __device__ __forceinline__ float act_slope(float z) {
     if constexpr (ACT == SPCONV_ACT_RELU) return z > 0.f ? 1.f : 0.f;
     if constexpr (ACT == SPCONV_ACT_GELU)
-        return 0.5f * (1.f + erff(z * 0.70710678f)) + z * 0.39894228f * expf(-0.5f * z * z);
+        return 0.5f * (1.f + erff(z * 0.70710678f)) + slope_factor(z) * 0.39894228f * expf(-0.5f * z * z);
     if constexpr (ACT == SPCONV_ACT_SILU) {
         const float s = 1.f / (1.f + expf(-z));
-        return s * (1.f + z * (1.f - s));
+        return s * (1.f + slope_factor(z) * (1.f - s));
     }
     return 1.f;
 }
@@ -161,7 +165,7 @@ __device__ __forceinline__ float2 act_slope2(float2 z) {
     }
     if constexpr (ACT == SPCONV_ACT_SILU) {
         const float sx = rcp_approx(1.f + ex2_approx(-1.4426950f * z.x)), sy = rcp_approx(1.f + ex2_approx(-1.4426950f * z.y));
-        return make_float2(sx * (1.f + z.x * (1.f - sx)), sy * (1.f + z.y * (1.f - sy)));
+        return make_float2(sx * (1.f + slope_factor(z.x) * (1.f - sx)), sy * (1.f + slope_factor(z.y) * (1.f - sy)));
     }
     return make_float2(1.f, 1.f);
 }
