@@ -8,7 +8,7 @@ namespace spconv {
 template <int ACT>
 __device__ __forceinline__ float act_value(float z) {
     if constexpr (ACT == SPCONV_ACT_RELU) return z < 0.f ? 0.f : z;          // NaN stays NaN
-    if constexpr (ACT == SPCONV_ACT_GELU) return 0.5f * z * (1.f + erff(z * 0.70710678f));
+    if constexpr (ACT == SPCONV_ACT_GELU) return 0.5f * z * erfcf(z * -0.70710678f);   // 1 + erf would cancel below 0
     if constexpr (ACT == SPCONV_ACT_SILU) return z / (1.f + expf(-z));
     return z;
 }
@@ -21,7 +21,7 @@ template <int ACT>
 __device__ __forceinline__ float act_slope(float z) {
     if constexpr (ACT == SPCONV_ACT_RELU) return z > 0.f ? 1.f : 0.f;
     if constexpr (ACT == SPCONV_ACT_GELU)
-        return 0.5f * (1.f + erff(z * 0.70710678f)) + slope_factor(z) * 0.39894228f * expf(-0.5f * z * z);
+        return 0.5f * erfcf(z * -0.70710678f) + slope_factor(z) * 0.39894228f * expf(-0.5f * z * z);
     if constexpr (ACT == SPCONV_ACT_SILU) {
         const float s = 1.f / (1.f + expf(-z));
         return s * (1.f + slope_factor(z) * (1.f - s));

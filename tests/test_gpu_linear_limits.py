@@ -73,3 +73,30 @@ def test_products_beyond_half_precision(act, M):
     for got, want, lim in ((gx, dz @ w.detach().double(), e @ w.detach().double().abs()),
                            (gw, dz.t() @ x.detach().double(), e.t() @ x.detach().double().abs())):
         assert ((got.double() - want).abs() <= lim + 2.0 ** -11 * want.abs() + 2.0 ** -24).all()
+
+
+def _outputs(act, dtype, z, kernel=_native.KERNEL_AUTO):
+    """act at the values of a vector, through a layer that multiplies by one."""
+    w = torch.zeros(8, 8, device="cuda", dtype=dtype)
+    w[0, 0] = 1.0
+    x = torch.zeros(z.numel(), 8, device="cuda", dtype=dtype)
+    x[:, 0] = z.to(dtype)
+    return x[:, 0].double(), _native.linear_forward(x, w, None, None, act, kernel=kernel)[0][:, 0].double()
+
+
+def test_negative_tail_in_single_precision():
+    """GELU and its slope keep their digits for negative arguments. The argument of the error function is off
+    by 2^-23 of itself, its value by z^2 times that, the function by a few steps: (z^2 + 8) 2^-22 in all, for
+    the slope (Phi + z phi, which cancel to about -z phi, the second within z^2 2^-23) the same of each term."""
+    z0 = torch.linspace(-9.0, 0.0, 5001, device="cuda")
+    z, out = _outputs("gelu", torch.float32, z0)
+    cdf = 0.5 * torch.special.erfc(-z * 0.5 ** 0.5)
+    assert ((out - z * cdf).abs() <= (z * z + 8) * 2.0 ** -22 * (z * cdf).abs()).all()
+    x = torch.ones(1, 1, device="cuda")
+    w = torch.zeros(z0.numel(), 1, device="cuda")
+    d = torch.ones(1, z0.numel(), device="cuda")
+    slope = _native.linear_backward(d, z0[None].contiguous(), x, w, "gelu", torch.float32, torch.float32,
+                                    (False, False, True))[2].double()
+    z, phi = z0.double(), z0.double() * torch.exp(-0.5 * z0.double() ** 2) / (2 * torch.pi) ** 0.5
+    cdf = 0.5 * torch.special.erfc(-z * 0.5 ** 0.5)
+    assert ((slope - (cdf + phi)).abs() <= (z * z + 8) * 2.0 ** -22 * (cdf + phi.abs())).all()
