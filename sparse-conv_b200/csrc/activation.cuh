@@ -96,11 +96,12 @@ __device__ __forceinline__ void normal_tail2(float2 z, f32x2 &t, float2 &e, f32x
     minus_q = mul2(p, pack_f32x2(e.x, e.y));
 }
 
-// For t = -min(|z|, 5.75): Phi(t) = 2^R(t), R a degree-6 polynomial for log2(Phi), which is nearly
+// For t = -min(|z|, 13): Phi(t) = 2^R(t), R a degree-6 polynomial for log2(Phi), which is nearly
 // a parabola there: six products and one exponential, where exp(-t^2 / 2) P(t) takes twelve for the
-// same accuracy. Fitted here for the least weighted error: within 2.6e-7 everywhere and 2^-12.3 of
-// Phi itself down to -5.75, beyond which t Phi counts as -2.6e-8.
-constexpr float kLogTailEnd = 5.75f;
+// same accuracy. Fitted here on [-5.75, 0] for the least weighted error: within 2.6e-7 everywhere and 2^-12.3 of
+// Phi itself down to -5.75. It goes on falling to its minimum near -14 (13 % above Phi at -8, where t Phi is
+// -5e-15), so from -13 on t Phi counts as -4e-32.
+constexpr float kLogTailEnd = 13.f;
 __host__ __device__ constexpr float log_tail_coef(int k) {
     constexpr float c[7] = {-0.99999982f, 1.1511294f, -0.45898986f, 0.053147960f, 0.0079413289f, 7.3869905e-4f,
                             3.1020278e-5f};
@@ -109,7 +110,7 @@ __host__ __device__ constexpr float log_tail_coef(int k) {
 
 // act(z) for four pairs, in place, step by step across them: each step's four packed operations are
 // independent, which covers one operation's latency without another warp's help. inf and NaN as the
-// functions above, but GELU(-inf) = -2.6e-8 (its limit is 0).
+// functions above, but GELU(-inf) = -4e-32 (its limit is 0).
 template <int ACT>
 __device__ __forceinline__ void act_value8(f32x2 *f) {
     if constexpr (ACT == SPCONV_ACT_RELU) {

@@ -100,3 +100,14 @@ def test_negative_tail_in_single_precision():
     z, phi = z0.double(), z0.double() * torch.exp(-0.5 * z0.double() ** 2) / (2 * torch.pi) ** 0.5
     cdf = 0.5 * torch.special.erfc(-z * 0.5 ** 0.5)
     assert ((slope - (cdf + phi)).abs() <= (z * z + 8) * 2.0 ** -22 * (cdf + phi.abs())).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_far_tail_in_half_precision(dtype):
+    """GELU falls to zero: the fitted tail is within a quarter of the value to -8 and below 1e-17 from there
+    on, where Phi is under 7e-16."""
+    z, out = _outputs("gelu", dtype, torch.cat([torch.linspace(-9.0, -5.0, 2001, device="cuda"),
+                                                torch.tensor([-10.0, -13.0, -14.0, -20.0, -1e3, -6e4], device="cuda")]))
+    ref = z * 0.5 * torch.special.erfc(-z * 0.5 ** 0.5)
+    assert ((out - ref).abs() <= 0.25 * ref.abs() + 1e-17 + (2.0 ** -24 if dtype == torch.float16 else 0.0)).all()
+    assert (out[z < -9].abs() <= 1e-17).all() if dtype == torch.bfloat16 else not out[z < -6].any()
