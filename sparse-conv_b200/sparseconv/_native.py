@@ -25,6 +25,7 @@ import threading
 from typing import Optional, Sequence, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "libsparseconv_b200.so")
 
@@ -192,6 +193,16 @@ def _require_cuda(*tensors: torch.Tensor) -> torch.device:
         elif t.device != dev:
             raise RuntimeError(f"tensors on different devices: {dev} and {t.device}")
     return dev
+
+
+def refuse_forward_mode(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    """Raises for a tensor with a forward-mode tangent. A call that needs no gradients does not pass
+    through autograd, which would raise, and its result would count as constant."""
+    if getattr(forward_ad, "_current_level", 0) < 0:         # outside of every dual_level: one comparison
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{what} has no forward-mode derivative")
 
 
 # ---------------------------------------------------------------------------------------

@@ -45,6 +45,7 @@ def clip_gradients(grads: Sequence[torch.Tensor], max_norm: float, norm_type: fl
         raise ValueError(f"max_norm must be >= 0, got {max_norm}")
     if out is not None and len(out) != len(grads):
         raise ValueError(f"{len(out)} outputs for {len(grads)} gradients")
+    _native.refuse_forward_mode("clip_gradients", *grads, *(() if out is None else out))
     return _native.clip_gradients(grads, grads if out is None else out, max_norm, _norm_kind(norm_type))
 
 

@@ -69,6 +69,7 @@ def sparse_linear(
         activation) is kept in the feature dtype; weight and bias gradients come in the
         parameters' dtypes, summed in fp32 in a fixed order.
     """
+    _native.refuse_forward_mode("sparse_linear", feats, weight, bias, residual)
     if torch.is_grad_enabled() and (feats.requires_grad or weight.requires_grad or
                                     (bias is not None and bias.requires_grad) or
                                     (residual is not None and residual.requires_grad)):

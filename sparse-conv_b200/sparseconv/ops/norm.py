@@ -82,6 +82,7 @@ def sparse_residual_norm(
         fp32 and ``normed`` is computed from ``hidden`` before that is rounded.
     """
     params = (feats, residual, gate, weight, bias, next_weight, next_bias)
+    _native.refuse_forward_mode("sparse_residual_norm", *params)
     if not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in params):
         return _native.residual_norm_forward(feats, residual, params[2:], batch_offsets, residual_scale,
                                              norm, next_norm, eps)
