@@ -49,10 +49,14 @@ class SparseConvTensor(metaclass=ProxyableClassMeta):
             "to generate new SparseConvTensor instead.")
 
     def batch_offsets(self) -> torch.Tensor:
-        """[batch_size + 1] int32 first row of each sample, for indices in the order of their
-        batch column (what ``from_dense`` gives)."""
-        ends = torch.arange(self.batch_size + 1, dtype=self.indices.dtype, device=self.indices.device)
-        return torch.searchsorted(self.indices[:, 0].contiguous(), ends, out_int32=True)
+        """[batch_size + 1] int32 first row of each sample. The rows have to be in the order of their
+        batch column (what ``from_dense`` gives): offsets of other rows are all -1, which every
+        use refuses as it does any that do not ascend from 0 to the number of rows."""
+        column = self.indices[:, 0].contiguous()
+        ends = torch.arange(self.batch_size + 1, dtype=column.dtype, device=column.device)
+        offsets = torch.searchsorted(column, ends, out_int32=True)
+        # checked on the tensor's device, without a synchronisation
+        return torch.where((column[1:] >= column[:-1]).all(), offsets, -1)
 
     @classmethod
     def from_dense(cls, x: torch.Tensor) -> "SparseConvTensor":
