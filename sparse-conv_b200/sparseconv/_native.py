@@ -1008,6 +1008,8 @@ def clip_gradients(grads: Sequence[torch.Tensor], outs: Sequence[torch.Tensor], 
                                    ws.data_ptr(), need, _raw_stream(index))
     if rc != SPCONV_OK:
         _raise(rc, "spconv_clip_gradients")
+    # written through their addresses: a backward that saved them has to notice
+    torch.autograd.graph.increment_version(outs)
     return total
 
 
