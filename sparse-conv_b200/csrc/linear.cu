@@ -378,6 +378,8 @@ static int64_t padded_forward_bytes(int64_t M, int Ci, int Co, bool residual, bo
 static int64_t separate_backward_bytes(int dtype, int64_t M, int Ci, int Co, int activation) {
     const int64_t separate = pad256(activation == SPCONV_ACT_NONE ? 0 : M * Co * elt(dtype)) + pad256((int64_t)dact_chunks(M) * Co * 4) +
                              pad256((int64_t)std::max(wgrad_splits(M, Ci, Co), gemm_tc_splits(Co, Ci, M)) * Co * Ci * 4);
+    // the one pass over the rows keeps sums of every CTA; tensors off 16-byte boundaries take the separate kernels
+    if (!bwd_tc_shape(dtype, M, Ci, Co, activation)) return separate;
     const int64_t grid = bwd_tc_grid(M);
     return std::max(separate, pad256(grid * 8 * Co * 4) + pad256(grid * Co * Ci * 4));
 }
