@@ -8,11 +8,12 @@ goes to ``torch.cuda.current_stream()``.
 Device-side problems (coordinates out of range, a full table, a kernel wait limit) are
 OR-ed into a per-device int32 status word. After each op the word is copied
 asynchronously to pinned host memory; the next op on that device (or an explicit
-``check_errors()``) raises ``RuntimeError`` if a bit is set. The linear, norm and clipping ops, which
-are also called on a few rows, where a copy and an event would cost more than the op, give their
+``check_errors()``) raises ``RuntimeError`` if a bit is set. The linear and norm ops, which are
+also called on a few rows, where a copy and an event would cost more than the op, give their
 kernels a word in pinned host memory instead: a kernel writes there only on a problem, and the
-next op on the device reads it without any call to CUDA. With the environment variable
-``SPARSECONV_SYNC_CHECK=1`` each op synchronises and checks at once.
+next op on the device that checks (clipping, whose kernels report nothing, among them) reads it without
+any call to CUDA. With the environment variable ``SPARSECONV_SYNC_CHECK=1`` each op synchronises and
+checks at once; the linear, norm and clipping ops read the variable when this module is imported.
 """
 from __future__ import annotations
 
@@ -278,10 +279,13 @@ def after_launch(device: torch.device) -> None:
 
 
 def before_launch(device: torch.device) -> None:
-    """Raise for an error found by an earlier op on this device, if its read-back landed."""
+    """Raise for an error found by an earlier op on this device, if its read-back landed or it is in
+    the host's word."""
     if torch.cuda.is_current_stream_capturing():
         return
     st = status_word(device)
+    if st.mapped_word.value:
+        _inspect_mapped(st)
     if st.pending and st.event.query():
         _inspect(st)
 
@@ -1000,6 +1004,7 @@ def clip_gradients(grads: Sequence[torch.Tensor], outs: Sequence[torch.Tensor], 
     except KeyError as e:
         raise TypeError(f"unsupported gradient dtype {e.args[0]}") from None
     ptrs, optrs, sizes, codes = (array.array(t, v) for t, v in (("Q", ptrs), ("Q", optrs), ("q", sizes), ("i", codes)))
+    mapped_status(index)                     # a step's gradients end here: what went wrong on the way is raised
     total = torch.empty((), dtype=torch.float32, device=dev)
     need = lib.spconv_clip_gradients_workspace_bytes(n)
     ws = torch.empty((need,), dtype=torch.uint8, device=dev)
@@ -1010,6 +1015,7 @@ def clip_gradients(grads: Sequence[torch.Tensor], outs: Sequence[torch.Tensor], 
         _raise(rc, "spconv_clip_gradients")
     # written through their addresses: a backward that saved them has to notice
     torch.autograd.graph.increment_version(outs)
+    after_mapped_launch(index)
     return total
 
 
