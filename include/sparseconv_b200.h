@@ -306,6 +306,13 @@ int spconv_linear_forward(const void *feats, int dtype, int64_t num_rows, int Ci
                           void *out, void *preact, void *workspace, int64_t workspace_bytes,
                           int kernel_choice, int32_t *status, void *stream);
 
+/* As spconv_linear_forward, with the bias in bias_dtype: SPCONV_F32, added to the fp32 product as it
+ * is, or dtype. */
+int spconv_linear_forward_ex(const void *feats, int dtype, int64_t num_rows, int Ci, const void *weight,
+                             const void *bias, int bias_dtype, const void *residual, int Co, int activation,
+                             void *out, void *preact, void *workspace, int64_t workspace_bytes,
+                             int kernel_choice, int32_t *status, void *stream);
+
 /* Gradients of spconv_linear_forward, with dz = grad_out * act'(preact) rounded to `dtype`:
  *   grad_feats[i, ci] = sum_co dz[i, co] * weight[co, ci]
  *   grad_weight[co, ci] = sum_i dz[i, co] * feats[i, ci];  grad_bias[co] = sum_i dz[i, co]

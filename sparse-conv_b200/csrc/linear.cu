@@ -107,7 +107,7 @@ linear_simt_kernel(GemmArgs g) {
                 g.partial[(int64_t)blockIdx.z * g.M * g.N + at] = z;
                 continue;
             }
-            if (g.bias) z += dtype_traits<T>::to_f(((const T *)g.bias)[n]);
+            if (g.bias) z += g.bias_f32 ? ((const float *)g.bias)[n] : dtype_traits<T>::to_f(((const T *)g.bias)[n]);
             if (g.preact) ((T *)g.preact)[at] = dtype_traits<T>::from_f(z);
             z = act_value<ACT>(z);
             if (g.residual) z += dtype_traits<T>::to_f(((const T *)g.residual)[at]);
@@ -372,7 +372,7 @@ static int launch_repitch(const void *src, int src_cols, void *dst, int dst_cols
 
 static int64_t padded_forward_bytes(int64_t M, int Ci, int Co, bool residual, bool preact) {
     const int64_t pi = up8(Ci), po = up8(Co);
-    return pad256(M * pi * 2) + pad256(po * pi * 2) + pad256(po * 2) + (1 + (residual ? 1 : 0) + (preact ? 1 : 0)) * pad256(M * po * 2);
+    return pad256(M * pi * 2) + pad256(po * pi * 2) + pad256(po * 4) + (1 + (residual ? 1 : 0) + (preact ? 1 : 0)) * pad256(M * po * 2);
 }
 
 static int64_t separate_backward_bytes(int dtype, int64_t M, int Ci, int Co, int activation) {
@@ -391,7 +391,7 @@ static int64_t padded_backward_bytes(int dtype, int64_t M, int Ci, int Co, int a
 }
 
 static int linear_forward(const void *feats, int dtype, int64_t M, int Ci, const void *weight, const void *bias,
-                          const void *residual, int Co, int activation, void *out, void *preact, int kernel_choice,
+                          int bias_dtype, const void *residual, int Co, int activation, void *out, void *preact, int kernel_choice,
                           int32_t *status, cudaStream_t st) {
     GemmArgs g = {};
     g.a = feats;
@@ -401,6 +401,7 @@ static int linear_forward(const void *feats, int dtype, int64_t M, int Ci, const
     g.N = Co;
     g.K = Ci;
     g.bias = bias;
+    g.bias_f32 = bias_dtype == SPCONV_F32;
     g.residual = residual;
     g.activation = activation;
     g.out = out;
@@ -489,13 +490,23 @@ extern "C" int spconv_linear_forward(const void *feats, int dtype, int64_t M, in
                                      const void *bias, const void *residual, int Co, int activation, void *out,
                                      void *preact, void *workspace, int64_t workspace_bytes, int kernel_choice,
                                      int32_t *status, void *stream) {
+    return spconv_linear_forward_ex(feats, dtype, M, Ci, weight, bias, dtype, residual, Co, activation, out, preact,
+                                    workspace, workspace_bytes, kernel_choice, status, stream);
+}
+
+extern "C" int spconv_linear_forward_ex(const void *feats, int dtype, int64_t M, int Ci, const void *weight,
+                                        const void *bias, int bias_dtype, const void *residual, int Co, int activation,
+                                        void *out, void *preact, void *workspace, int64_t workspace_bytes,
+                                        int kernel_choice, int32_t *status, void *stream) {
     if (const int rc = check_linear(dtype, M, Ci, Co, activation, kernel_choice)) return rc;
+    SPCONV_REQUIRE(!bias || bias_dtype == SPCONV_F32 || bias_dtype == dtype, SPCONV_ERR_ARG,
+                   "the bias is fp32 or of the features' type");
     if (M == 0) return SPCONV_OK;
     SPCONV_REQUIRE(feats && weight && out, SPCONV_ERR_ARG, "null pointer argument");
     const cudaStream_t st = (cudaStream_t)stream;
     // without the workspace the CUDA-core kernel takes such shapes too
     if (kernel_choice != SPCONV_KERNEL_AUTO || !workspace || !linear_padded(dtype, M, Ci, Co))
-        return linear_forward(feats, dtype, M, Ci, weight, bias, residual, Co, activation, out, preact, kernel_choice, status, st);
+        return linear_forward(feats, dtype, M, Ci, weight, bias, bias_dtype, residual, Co, activation, out, preact, kernel_choice, status, st);
     SPCONV_REQUIRE(((uintptr_t)workspace & 255) == 0 &&
                        workspace_bytes >= padded_forward_bytes(M, Ci, Co, residual != nullptr, preact != nullptr),
                    SPCONV_ERR_ARG, "workspace misaligned or too small");
@@ -506,15 +517,15 @@ extern "C" int spconv_linear_forward(const void *feats, int dtype, int64_t M, in
         ws += pad256(bytes);
         return p;
     };
-    void *x = take(M * pi * 2), *w = take((int64_t)po * pi * 2), *b = take(po * 2), *y = take(M * po * 2);
+    void *x = take(M * pi * 2), *w = take((int64_t)po * pi * 2), *b = take(po * 4), *y = take(M * po * 2);
     void *r = residual ? take(M * po * 2) : nullptr, *z = preact ? take(M * po * 2) : nullptr;
     int rc = launch_repitch(feats, Ci, x, pi, M, 2, st);
     if (!rc) rc = launch_repitch(weight, Ci, w, pi, Co, 2, st);
     if (!rc && po > Co && cudaMemsetAsync((uint8_t *)w + (int64_t)Co * pi * 2, 0, (size_t)(po - Co) * pi * 2, st) != cudaSuccess)
         rc = check_launch("linear_forward: clear");
-    if (!rc && bias) rc = launch_repitch(bias, Co, b, po, 1, 2, st);
+    if (!rc && bias) rc = launch_repitch(bias, Co, b, po, 1, (int)elt(bias_dtype), st);
     if (!rc && residual) rc = launch_repitch(residual, Co, r, po, M, 2, st);
-    if (!rc) rc = linear_forward(x, dtype, M, pi, w, bias ? b : nullptr, r, po, activation, y, z, kernel_choice, status, st);
+    if (!rc) rc = linear_forward(x, dtype, M, pi, w, bias ? b : nullptr, bias_dtype, r, po, activation, y, z, kernel_choice, status, st);
     if (!rc) rc = launch_repitch(y, po, out, Co, M, 2, st);
     if (!rc && preact) rc = launch_repitch(z, po, preact, Co, M, 2, st);
     return rc;

@@ -115,6 +115,9 @@ SIGNATURES = {
     "spconv_linear_forward": (_c_int, [
         _c_void_p, _c_int, _c_i64, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int,
         _c_void_p, _c_void_p, _c_void_p, _c_i64, _c_int, _c_void_p, _c_void_p]),
+    "spconv_linear_forward_ex": (_c_int, [
+        _c_void_p, _c_int, _c_i64, _c_int, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_int, _c_int,
+        _c_void_p, _c_void_p, _c_void_p, _c_i64, _c_int, _c_void_p, _c_void_p]),
     "spconv_linear_backward_workspace_bytes": (_c_i64, [_c_int, _c_i64, _c_int, _c_int, _c_int]),
     "spconv_linear_backward": (_c_int, [
         _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_i64, _c_int, _c_int, _c_int,
@@ -741,7 +744,8 @@ def _matrix(t: torch.Tensor, shape: Tuple[int, ...], dtype: torch.dtype, what: s
 def linear_forward(feats: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor],
                    residual: Optional[torch.Tensor], activation: str, keep_preact: bool = False,
                    kernel: int = KERNEL_AUTO) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
-    """(residual + act(feats @ weight.T + bias), act's argument if ``keep_preact``)."""
+    """(residual + act(feats @ weight.T + bias), act's argument if ``keep_preact``); the bias in fp32 or
+    the features' dtype."""
     dev = _require_cuda(feats, weight, bias, residual)
     dtype = feats.dtype
     if dtype not in DTYPE_CODES:
@@ -759,7 +763,7 @@ def linear_forward(feats: torch.Tensor, weight: torch.Tensor, bias: Optional[tor
     weight = weight.contiguous()
     if bias is not None:
         bias = bias.contiguous()
-        _matrix(bias, (Co,), dtype, "bias")
+        _matrix(bias, (Co,), torch.float32 if bias.dtype == torch.float32 else dtype, "bias")
     if residual is not None:
         _matrix(residual, (M, Co), dtype, "residual")
     out = torch.empty((M, Co), dtype=dtype, device=dev)
@@ -772,12 +776,13 @@ def linear_forward(feats: torch.Tensor, weight: torch.Tensor, bias: Optional[tor
     if Ci % 8 or Co % 8:
         need = lib.spconv_linear_forward_workspace_bytes(DTYPE_CODES[dtype], M, Ci, Co, residual is not None, keep_preact)
         ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need > 0 else None
-    rc = lib.spconv_linear_forward(
-        feats.data_ptr(), DTYPE_CODES[dtype], M, Ci, weight.data_ptr(), _ptr(bias), _ptr(residual), Co,
+    rc = lib.spconv_linear_forward_ex(
+        feats.data_ptr(), DTYPE_CODES[dtype], M, Ci, weight.data_ptr(), _ptr(bias),
+        0 if bias is None else DTYPE_CODES[bias.dtype], _ptr(residual), Co,
         ACTIVATIONS[activation], out.data_ptr(), _ptr(preact), _ptr(ws), need, kernel, mapped_status(index),
         _raw_stream(index))
     if rc != SPCONV_OK:
-        _raise(rc, "spconv_linear_forward")
+        _raise(rc, "spconv_linear_forward_ex")
     after_mapped_launch(index)
     return out, preact
 

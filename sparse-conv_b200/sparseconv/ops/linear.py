@@ -20,11 +20,16 @@ class Activation:
     SILU = "silu"
 
 
+def _bias(bias: Optional[torch.Tensor], dtype: torch.dtype) -> Optional[torch.Tensor]:
+    """As the kernels add it: the features' dtype, or fp32 for every other."""
+    return bias if bias is None or bias.dtype == dtype else bias.to(torch.float32)
+
+
 class SparseLinearFunction(Function):
     @staticmethod
     def forward(ctx, feats, weight, bias, residual, activation):
         w = weight.to(feats.dtype).contiguous()
-        b = None if bias is None else bias.to(feats.dtype)
+        b = _bias(bias, feats.dtype)
         needs = ctx.needs_input_grad
         keep = activation != Activation.NONE and (needs[0] or needs[1] or needs[2])
         out, preact = _native.linear_forward(feats, w, b, residual, activation, keep_preact=keep)
@@ -58,7 +63,7 @@ def sparse_linear(
     Args:
         feats: [N, C] input features (fp32, fp16 or bf16), contiguous, on CUDA.
         weight: [Co, C] weights (cast to the feature dtype).
-        bias: [Co] bias or None (cast to the feature dtype).
+        bias: [Co] bias in the feature dtype or fp32, added in fp32 (others are cast to fp32), or None.
         residual: [N, Co] added after the activation, in the feature dtype, contiguous, or None.
         activation: any ``Activation`` value; GELU is the exact one (normal distribution function).
 
@@ -74,5 +79,4 @@ def sparse_linear(
                                     (bias is not None and bias.requires_grad) or
                                     (residual is not None and residual.requires_grad)):
         return SparseLinearFunction.apply(feats, weight, bias, residual, activation)
-    return _native.linear_forward(feats, weight.to(feats.dtype), None if bias is None else bias.to(feats.dtype),
-                                  residual, activation)[0]
+    return _native.linear_forward(feats, weight.to(feats.dtype), _bias(bias, feats.dtype), residual, activation)[0]
