@@ -216,7 +216,7 @@ __device__ __forceinline__ float rn_dot(const float (&t)[N], const float (&n)[N]
 
 // Normalises U rows, N values of each in a lane, in place: (mean, rstd) of each row in st. Columns
 // that a lane does not have hold zeros, before and after (FULL: it has them all).
-template <int U, int N, int VEC, int WARPS, bool FULL>
+template <typename T, int U, int N, int VEC, int WARPS, bool FULL>
 __device__ __forceinline__ void rn_normalise(float (&t)[U][N], float2 (&st)[U], const bool *have, int kind, float inv_c,
                                              float eps, int lpr, RnScratch &scratch) {
     if (kind == SPCONV_NORM_NONE) {
@@ -224,11 +224,15 @@ __device__ __forceinline__ void rn_normalise(float (&t)[U][N], float2 (&st)[U], 
         for (int u = 0; u < U; ++u) st[u] = make_float2(0.f, 1.f);
         return;
     }
-    // Eight columns a lane: one reduction, of d and d^2 for d = t - c, c the mean of the row's first
-    // eight values, which lies within sqrt(C / 8) deviations of the row's mean: mean(d^2) - mean(d)^2
+    // 16-bit features, eight columns a lane: one reduction, of d and d^2 for d = t - c, c the mean of the row's
+    // first eight values, which lies within sqrt(C / 8) deviations of the row's mean: mean(d^2) - mean(d)^2
     // then costs at most the factor C / 8 + 1 in the variance's rounding, whatever offset the row has
-    // in common. Single columns a lane, or a block a row: the mean first, then the squares.
-    constexpr bool ONE = VEC == 8 && WARPS == 0;
+    // in common; 4e-6 of 1 / deviation measured at C = 256 with the first eight a thousand times the others, under
+    // a hundredth of the outputs' rounding. Two reductions, the mean first, then the squares, cost nothing at
+    // 64 and 128 channels and 4 to 13 % at 32, 96, 200 and 256 (500,000 x 200 bf16 forward 271 -> 306 us). fp32 takes
+    // them (2e-7 for that row; 250,000 x 200 156 -> 183 us, no difference at powers of two), as do single columns a
+    // lane and a block a row.
+    constexpr bool ONE = sizeof(T) == 2 && VEC == 8 && WARPS == 0;
     float s[U], q[U], shift[U];
     const bool layer = kind == SPCONV_NORM_LAYER;
 #pragma unroll
@@ -392,14 +396,14 @@ residual_norm_fwd_kernel(const __grid_constant__ RnArgs a) {
             }
             fetch(row + groups);
             float2 st1[1], st2[1];
-            rn_normalise<1, N, VEC, WARPS, false>(u, st1, have, a.norm1, inv_c, a.eps, lpr, scratch);
+            rn_normalise<T, 1, N, VEC, WARPS, false>(u, st1, have, a.norm1, inv_c, a.eps, lpr, scratch);
 #pragma unroll
             for (int n = 0; n < N; ++n)
                 h[0][n] = have[n / VEC] ? a.alpha * h[0][n] + pg[n] * (u[0][n] * pw1[n] + pb1[n]) : 0.f;
 #pragma unroll
             for (int j = 0; j < VPT; ++j)
                 if (have[j] && row < end) rn_store((T *)a.h + row * C + col[j], h[0] + j * VEC, (RnPack<T, VEC> *)nullptr);
-            rn_normalise<1, N, VEC, WARPS, false>(h, st2, have, a.norm2, inv_c, a.eps, lpr, scratch);
+            rn_normalise<T, 1, N, VEC, WARPS, false>(h, st2, have, a.norm2, inv_c, a.eps, lpr, scratch);
             if (a.norm2 != SPCONV_NORM_NONE) {
 #pragma unroll
                 for (int n = 0; n < N; ++n) h[0][n] = h[0][n] * pw2[n] + pb2[n];
@@ -875,11 +879,11 @@ residual_norm_bulk_kernel(const __grid_constant__ RnArgs a, const __grid_constan
                 };
                 if constexpr (!BWD) {
                     float2 st1[U], st2[U];
-                    rn_normalise<U, N, VEC, 0, FULL>(n1, st1, have, a.norm1, inv_c, a.eps, lpr, scratch);
+                    rn_normalise<T, U, N, VEC, 0, FULL>(n1, st1, have, a.norm1, inv_c, a.eps, lpr, scratch);
                     hidden();
 #pragma unroll
                     for (int u = 0; u < U; ++u) write(u, tx, n2[u]);
-                    rn_normalise<U, N, VEC, 0, FULL>(n2, st2, have, a.norm2, inv_c, a.eps, lpr, scratch);
+                    rn_normalise<T, U, N, VEC, 0, FULL>(n2, st2, have, a.norm2, inv_c, a.eps, lpr, scratch);
                     if (a.norm2 != SPCONV_NORM_NONE) {
                         par_all(kW2, p);
                         par_all(kB2, q);

@@ -114,11 +114,13 @@ def test_norm_sums_of_few_rows(M, C, dtype):
 def test_first_channels_unlike_the_rest(M, C, dtype):
     """LayerNorm of rows whose first eight values are a thousand times the others.
 
-    With the squares taken around a shift s, var = mean(d^2) - mean(d)^2, and (s - mean)^2 is at most C / 8 - 1
-    variances where s is the mean of eight of the row's values: both terms are under C / 8 variances. A
-    mean of squares passes at most 14 roundings of U, a mean 10 (twice that in its square), the rest 2:
-    (C / 8 + 1) 36 U of the variance, half of it of 1 / deviation, and 4 U. The values themselves: their mean's and
-    their own roundings, 18 U of the largest."""
+    fp32 takes the mean first and squares the deviations: a mean of squares passes at most 22 roundings of U, so
+    1 / deviation is off by 11 U and a few steps, and the values by their mean's and their own, 18 U of the
+    largest; where the squares are taken around a shift s, var = mean(d^2) - mean(d)^2, and (s - mean)^2 is at
+    most C / 8 - 1 variances where s is the mean of eight of the row's values: both terms are under C / 8
+    variances, and with 14 roundings in the first, 20 in the second and 2 more (C / 8 + 1) 36 U of the variance
+    are lost, half of it of 1 / deviation. That is for 16-bit features, whose own rounding is far above it.
+    """
     gen = torch.Generator(device="cuda").manual_seed(C)
     x = torch.randn(M, C, generator=gen, device="cuda")
     x[:, :8] = x[:, :8] * 10 + 1000.0
@@ -128,5 +130,5 @@ def test_first_channels_unlike_the_rest(M, C, dtype):
     d = xd - xd.mean(1, keepdim=True)
     rstd = (d.square().mean(1, keepdim=True) + 1e-5).rsqrt()
     want = d * rstd
-    lim = ((C / 8 + 1) * 18 + 4) * U * want.abs() + 18 * U * xd.abs().amax(1, keepdim=True) * rstd
+    lim = (15 if dtype == "fp32" else (C / 8 + 1) * 18 + 4) * U * want.abs() + 18 * U * xd.abs().amax(1, keepdim=True) * rstd
     assert ((hidden.double() - want).abs() <= lim + torch.finfo(DT[dtype]).eps / 2 * (want.abs() + lim)).all()
