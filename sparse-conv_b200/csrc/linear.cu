@@ -401,7 +401,7 @@ static int linear_forward(const void *feats, int dtype, int64_t M, int Ci, const
     g.N = Co;
     g.K = Ci;
     g.bias = bias;
-    g.bias_f32 = bias_dtype == SPCONV_F32;
+    g.bias_f32 = bias && bias_dtype == SPCONV_F32;
     g.residual = residual;
     g.activation = activation;
     g.out = out;

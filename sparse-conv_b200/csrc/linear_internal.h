@@ -12,7 +12,7 @@ struct GemmArgs {
     const void *a, *b;
     bool a_t, b_t;
     int dtype;                       // of a, b, residual, preact and out
-    bool bias_f32;                   // the bias is in fp32, whatever dtype is
+    bool bias_f32;                   // there is a bias, in fp32 whatever dtype is
     int64_t M, N, K;
     const void *bias, *residual;     // [N], [M, N], or null
     int activation;

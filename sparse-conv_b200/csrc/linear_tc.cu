@@ -71,7 +71,7 @@ struct LtArgs {
     int bias_smem;                          // bias columns in shared memory (N up to whole chunks of 32, or 0)
     int b_resident;                         // K steps of B that stay in shared memory, or 0
     const void *bias;
-    int bias_f32;                           // in fp32, else in the features' type
+    int bias_f32;                           // a bias in fp32, else in the features' type (or none)
     int has_residual, has_preact;
     float *partial;
     int32_t *status;
@@ -115,9 +115,11 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
     // workers: CTAs, or pairs of them
     const int G = PAIR ? gridDim.x >> 1 : gridDim.x, me = PAIR ? blockIdx.x >> 1 : blockIdx.x;
     const uint32_t tmem_cols = 512;                                    // bufs * BN: all there are
-    auto bias_at = [&](int n) { return a.bias_f32 ? ((const float *)a.bias)[n] : dtype_traits<T>::to_f(((const T *)a.bias)[n]); };
-    for (int i = tid; i < a.bias_smem; i += kLtThreads)
-        s_bias[i] = i < a.N ? bias_at(i) : 0.f;
+    if (a.bias_f32)
+        for (int i = tid; i < a.bias_smem; i += kLtThreads) s_bias[i] = i < a.N ? ((const float *)a.bias)[i] : 0.f;
+    else
+        for (int i = tid; i < a.bias_smem; i += kLtThreads)
+            s_bias[i] = i < a.N ? dtype_traits<T>::to_f(((const T *)a.bias)[i]) : 0.f;
     if (tid == 0) {
         for (int s = 0; s < S; ++s) {
             mbar_init(smem_u32(&full[s]), 1);
@@ -401,11 +403,17 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
                             f[2 * i] = add2(f[2 * i], b0);
                             f[2 * i + 1] = add2(f[2 * i + 1], b1);
                         }
+                    } else if (a.bias_f32) {
+                        const float *b = (const float *)a.bias + n0 + c0;
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            if (c0 + 2 * i < n_cols) f[i] = add2(f[i], pack_f32x2(b[2 * i], b[2 * i + 1]));
                     } else if (a.bias) {
+                        const T *b = (const T *)a.bias + n0 + c0;
 #pragma unroll
                         for (int i = 0; i < 16; ++i)
                             if (c0 + 2 * i < n_cols)
-                                f[i] = add2(f[i], pack_f32x2(bias_at(n0 + c0 + 2 * i), bias_at(n0 + c0 + 2 * i + 1)));
+                                f[i] = add2(f[i], pack_f32x2(dtype_traits<T>::to_f(b[2 * i]), dtype_traits<T>::to_f(b[2 * i + 1])));
                     }
                     const uint32_t v0 = (uint32_t)half * 4;
                     if (a.has_preact) {
