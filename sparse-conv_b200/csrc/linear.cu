@@ -107,7 +107,7 @@ linear_simt_kernel(GemmArgs g) {
                 g.partial[(int64_t)blockIdx.z * g.M * g.N + at] = z;
                 continue;
             }
-            if (g.bias) z += g.bias_f32 ? ((const float *)g.bias)[n] : dtype_traits<T>::to_f(((const T *)g.bias)[n]);
+            if (g.bias) z += sizeof(T) == 2 && g.bias_f32 ? ((const float *)g.bias)[n] : dtype_traits<T>::to_f(((const T *)g.bias)[n]);
             if (g.preact) ((T *)g.preact)[at] = dtype_traits<T>::from_f(z);
             z = act_value<ACT>(z);
             if (g.residual) z += dtype_traits<T>::to_f(((const T *)g.residual)[at]);

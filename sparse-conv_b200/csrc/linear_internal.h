@@ -11,8 +11,10 @@ namespace spconv {
 struct GemmArgs {
     const void *a, *b;
     bool a_t, b_t;
+    // There is a bias, in fp32 whatever dtype is. It stands in padding: with M, N and K eight bytes on, the CUDA-core
+    // kernel was given 134 registers in place of 212 (20,000 x 512 -> 512 fp32 449 us in place of 367).
+    bool bias_f32;
     int dtype;                       // of a, b, residual, preact and out
-    bool bias_f32;                   // there is a bias, in fp32 whatever dtype is
     int64_t M, N, K;
     const void *bias, *residual;     // [N], [M, N], or null
     int activation;
