@@ -313,7 +313,8 @@ int spconv_linear_forward_ex(const void *feats, int dtype, int64_t num_rows, int
                              void *out, void *preact, void *workspace, int64_t workspace_bytes,
                              int kernel_choice, int32_t *status, void *stream);
 
-/* Gradients of spconv_linear_forward, with dz = grad_out * act'(preact) rounded to `dtype`:
+/* Gradients of spconv_linear_forward, with dz = grad_out * act'(preact), which enters the products
+ * rounded to `dtype` and grad_bias as it is:
  *   grad_feats[i, ci] = sum_co dz[i, co] * weight[co, ci]
  *   grad_weight[co, ci] = sum_i dz[i, co] * feats[i, ci];  grad_bias[co] = sum_i dz[i, co]
  * (the residual's gradient is grad_out). Sums are fp32, the same in every run. Each output may be

@@ -147,9 +147,11 @@ int launch_gemm_simt(const GemmArgs &g) {
 }
 
 // ---------------------------------------------------------------------------------------
-// dz = grad_out * act'(z), and its column sums. One read of each input, one write of dz; a lane
-// owns VEC neighbouring columns of a 32 * VEC column tile and walks the chunk's rows, so the
-// sums stay in registers; partial[chunk][Co] holds them per block.
+// dz = grad_out * act'(z), rounded to the features' type as the products' operand (half the bytes of
+// fp32, and what the tensor cores take; see linear_bwd_tc.cu for what it costs), and its column sums,
+// of dz before the rounding. One read of each input, one write of dz; a lane owns VEC neighbouring
+// columns of a 32 * VEC column tile and walks the chunk's rows, so the sums stay in registers;
+// partial[chunk][Co] holds them per block.
 // ---------------------------------------------------------------------------------------
 constexpr int kDactThreads = 256;
 

@@ -7,8 +7,14 @@
 // HBM. It applies where W, both accumulators and two stages of 128 rows fit an SM: see
 // bwd_tc_shape.
 //
-// 1.34 M x 128 -> 128 with GELU, bf16: 242 us (5.7 TB/s) and 473 us for the separate kernels; 2 M x 64 ->
+// 1.34 M x 128 -> 128 with GELU, bf16: 242 to 247 us (5.6 TB/s) and 473 us for the separate kernels; 2 M x 64 ->
 // 256 without activation 259 and 602 us.
+// Bits: dz is formed in fp32 and rounded to the features' type to be an operand of the tensor cores, as grad_out is when
+// there is no activation; the bias sums take it before. For bf16 with GELU that rounding, the rounded argument's (see
+// linear_tc.cu) and the output's own, 1.7e-3 of the norm each but the argument's 5.5e-4, make 2.4e-3 of the
+// gradient's. Handing the remainder of dz to the tensor cores as a second operand gave 1.75e-3 and took 1.34 M x 128 ->
+// 128 from 245 to 280 us and 883,771 x 64 -> 64 from 122 to 144: not kept.
+//
 // One CTA per SM takes every G-th tile of 128 rows. Roles, coupled by mbarriers:
 //   warp 0       TMA loads of the tile's z, grad_out and feats rows (blocks of 64 columns, 128-byte
 //                swizzle) into one of two stages; W once, at the start;

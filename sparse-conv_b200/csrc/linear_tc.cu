@@ -26,14 +26,19 @@
 // PAIR: two CTAs of a cluster, on two SMs, share a 256 x 256 tile (cta_group::2). Each holds its 128
 // rows of A, half of B's columns and its own rows' accumulators; the first one's MMA thread drives
 // both tensor cores, and commits to barriers in both. A K step then brings 32 KB into an SM instead of
-// 48. 84,000 x 512 -> 2048 bf16: 183 us unpaired, 170 us paired (163 since, 1.08 PFLOP/s; the library's product
-// alone takes 151 us). Keeping a pair's halves of B in shared memory (K <= 512) leaves one output slot a
+// 48. 84,000 x 512 -> 2048 bf16: 183 us unpaired, 170 us paired (152 to 163 since, up to 1.16 PFLOP/s; the library's
+// product alone takes 151 us). Keeping a pair's halves of B in shared memory (K <= 512) leaves one output slot a
 // warp and is slower, 192 us.
 // The weight gradient's K is the voxels: K is cut into splits, each writes fp32 sums of its own,
 // and linear_reduce_kernel adds them in a fixed order.
 // Measured (bf16): 1.34 M x 128 -> 128 112 us (6.1 TB/s) and its input gradient 112 us; 2 M x 64 -> 256
-// 217 to 230 us (5.6 to 5.9 TB/s), 287 us with GELU, 330 us with SiLU: those two are bound by the
-// epilogue's issue slots, about 20 a value with the exponentials'.
+// 217 to 230 us (5.6 to 5.9 TB/s), 287 to 294 us with GELU, 322 to 330 us with SiLU. Nothing is full in those two: at
+// 12.4 instructions a value the issue slots are 59 % in use, the special functions 38 %, the tensor pipe 9 % and HBM
+// 42 %; the warps wait for fixed latencies, for their loads from TMEM, each complete before its arithmetic
+// begins, and for the roles' barriers.
+// Bits: the output is rounded once, from fp32. The activation's argument is kept for the backward in the features'
+// type, as many bytes as the output; taking the slope at the rounded argument costs bf16 gradients 5.5e-4 of their norm
+// (one rounding of a bf16 result costs 1.7e-3), and in fp32 it would be twice the bytes each way where HBM is the bound.
 // Every wait is bounded (the conv kernels' limit); a timeout raises SPCONV_STATUS_WAIT_TIMEOUT and
 // the CTA waits (bounded) for its own copies and MMAs before it frees TMEM and exits.
 #include <algorithm>

@@ -575,8 +575,9 @@ residual_norm_bwd_kernel(const __grid_constant__ RnArgs a) {
 // place (the outputs take the inputs' slots) and the same thread stores finished stages in bulk.
 // The direct kernels above hold what is in flight in registers (two loads a lane); measured
 // there and here: 2.0 M x 64 bf16 forward 255 and 172 us (6.0 TB/s), 1.34 M x 128 forward 328 and
-// 243 us (5.7 TB/s), backward 738 and 426 us (4.9 TB/s). The backward issues 50 instructions a
-// value and spends most of its stalls on the row reductions' shuffles.
+// 243 us (5.7 TB/s), backward 738 and 426 us (4.9 TB/s). Nothing is full in the backward: 47 instructions a
+// value take 51 % of the issue slots, the bytes 75 % of HBM's copy rate; the 10 warps an SM that its registers
+// leave wait for fixed latencies, shared memory and the row reductions' shuffles.
 // A tile that crosses a sample's end is worked off in two parts, so tiles stay aligned to 16
 // bytes for every channel count; only the last one can end in a few odd bytes, which that thread
 // copies itself.
@@ -1051,7 +1052,15 @@ static int rn_pow2(int n) {
     return p;
 }
 
-// Blocks for M rows: enough to fill the SMs, no more than there are row groups.
+// Blocks for M rows: enough to fill the SMs, no more than there are row groups. Beyond 256 channels a block takes a row
+// at a time, so it is the blocks an SM has room for that keep rows in flight. Forward, LayerNorm on both sides,
+// bf16, by blocks per SM: 100,000 x 512 154 us at four, 117 at six, 92 at twelve, no less at more; 50,000 x 1024 160, 106
+// and 96 us at two, four and six; 50,000 x 2048 375, 240 and 213 us at one, two and three; 20,000 x 4096 571 us
+// at one and at two. The backward, which keeps more registers a thread, is up to 9 % faster with fewer (155 us at
+// six and 171 at twelve for 512 channels, 157 at three and 171 at six for 1024, 394 at one and 415 at three for
+// 2048), but the workspace is sized for one number. Up to 256 channels few rows come here, and the number hardly
+// matters forward (20,000 x 64 10 to 12 us, 40,000 x 256 29 us at one to 24); backward 40,000 x 256 takes 65, 48, 56 and
+// 73 us at one, two, four and eight, 20,000 x 64 19, 19, 28 and 30 us.
 static int64_t rn_grid(int64_t M, int C, int rows_per_block) {
     const int64_t per_sm = C <= 256 ? 4 : C <= 512 ? 12 : C <= 1024 ? 6 : C <= 2048 ? 3 : 1;
     return std::max<int64_t>(1, std::min<int64_t>(148 * per_sm, (M + rows_per_block - 1) / rows_per_block));
