@@ -397,6 +397,75 @@ int spconv_clip_gradients(const void *const *grads, void *const *outs, const int
                           const int32_t *dtypes, int num_tensors, int norm_kind, float max_norm,
                           float *total_norm, void *workspace, int64_t workspace_bytes, void *stream);
 
+/* Rotary positions of queries and keys [num_rows, heads, head_size]: pairs (u, w) of a head's values become
+ *   amplitude * (u cos - w sin, u sin + w cos),  angle = position[row, axis] * step
+ * The first rotary_dim columns hold rotary_dim / 2 pairs: columns (i, i + rotary_dim / 2)
+ * (SPCONV_ROTARY_HALF) or (2 i, 2 i + 1) (SPCONV_ROTARY_INTERLEAVED). Each axis turns n = rotary_dim / 2 / axes
+ * of them: pair i is turned by axis i / n with steps[i % n]; pairs from n * axes on and columns from rotary_dim on
+ * are copied. A step is the angle of one unit of position in 2^-64ths of a full turn, modulo 2^64 (negative
+ * steps wrap), so no position loses precision. inverse != 0 turns backwards: the gradient of the call.
+ *   query [num_rows, heads, head_size], key [num_rows, key_heads, head_size]: in dtype, strides in elements, a
+ *   head's values contiguous; either may have no heads. positions: int32, strides in elements
+ *   query_out, key_out: contiguous; each may be its input itself where that is contiguous, and overlaps nothing else
+ *   head_size <= 256, num_rows < 2^31
+ * No counterpart in the reference. */
+#define SPCONV_ROTARY_HALF 0
+#define SPCONV_ROTARY_INTERLEAVED 1
+#define SPCONV_ROTARY_MAX_PAIRS 128
+typedef struct {
+    int dtype, layout;
+    int64_t num_rows;
+    int heads, key_heads, head_size, rotary_dim, axes, inverse;
+    float amplitude;
+    const void *query, *key;
+    int64_t query_row, query_head, key_row, key_head;
+    void *query_out, *key_out;
+    const int32_t *positions;         /* [num_rows, axes] */
+    int64_t position_row, position_col;
+    uint64_t steps[SPCONV_ROTARY_MAX_PAIRS];
+} spconv_rotary_args;
+int spconv_rotary(const spconv_rotary_args *args, void *stream);
+
+/* Attention within the samples of a batch: of query i, sample b, head h (key head h / (heads / key_heads)),
+ *   out[i, h] = sum_j p_ij value[j],  p_ij = exp(s_ij) / sum_j exp(s_ij),  s_ij = scale * query[i, h] . key[j]
+ * over the sample's keys j; with `causal` those up to j - key0 <= (i - query0) + keys - queries (the last query
+ * sees the last key). A query that sees no key gets zeros.
+ *   query, grad_out [num_queries, heads, head_size], key, value [num_keys, key_heads, head_size]: in dtype, strides in
+ *   elements, a head's values contiguous; out and the gradients contiguous, overlapping no input or one another
+ *   offsets, key_offsets [num_samples + 1] int32 on the device: each sample's first query and key, ascending from 0
+ *   to the number of rows (anything else sets SPCONV_STATUS_OFFSETS, and rows may be left unwritten); both may be NULL for one
+ *   sample of all rows. Samples without queries or keys are allowed.
+ *   row_stats [num_queries, heads] fp32: written by the forward unless NULL, read by the backward
+ *   scale: positive. head_size <= 256. kernel: SPCONV_KERNEL_*; the tensor-core kernels take fp16 and bf16 heads of up
+ *   to 128 values and return SPCONV_ERR_UNSUPPORTED for others
+ * Products accumulate in fp32, as softmax statistics and row sums; outputs are rounded once. On the tensor cores p and its
+ * gradient are rounded to dtype, as their operands.
+ * The backward takes the forward's inputs, out, row_stats and grad_out, and writes grad_query, grad_key and
+ * grad_value where not NULL, the same bits in every run.
+ *   workspace: 256-byte aligned, spconv_attention_workspace_bytes(args, backward) bytes for these arguments
+ * No counterpart in the reference. */
+#define SPCONV_ATTENTION_MAX_SIZE 256
+typedef struct {
+    int dtype, kernel;
+    int64_t num_queries, num_keys;
+    int num_samples, heads, key_heads, head_size, causal;
+    float scale;
+    const int32_t *offsets, *key_offsets;
+    const void *query, *key, *value;
+    int64_t query_row, query_head, key_row, key_head, value_row, value_head;
+    void *out;
+    float *row_stats;
+    const void *grad_out;
+    int64_t grad_row, grad_head;
+    void *grad_query, *grad_key, *grad_value;
+    void *workspace;
+    int64_t workspace_bytes;
+    int32_t *status;
+} spconv_attention_args;
+int64_t spconv_attention_workspace_bytes(const spconv_attention_args *args, int backward);
+int spconv_attention_forward(const spconv_attention_args *args, void *stream);
+int spconv_attention_backward(const spconv_attention_args *args, void *stream);
+
 /* Stage timing, for profiling and for the benchmark's roofline figures.
  * spconv_stage_timing(max_calls > 0) creates CUDA events on the current device for
  * max_calls calls of each stage and starts recording, on the launch stream, the device

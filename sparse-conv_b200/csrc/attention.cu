@@ -1,0 +1,321 @@
+// Attention's entry points: checks, the choice of kernels and splits, and the small kernels around the products: copies
+// of rows that TMA cannot read, delta = grad . out, and the joining of splits.
+//
+// Splits. A sample whose rows make few tiles (pooling queries, single tokens; for the keys' gradients, few
+// conditioning tokens) leaves most SMs idle, so its keys (or queries) are cut into `splits` ranges, each
+// with fp32 results of its own, joined in order by a second kernel: the same bits every run.
+#include <algorithm>
+
+#include "attention_common.cuh"
+
+namespace spconv {
+
+constexpr int kAtThreads = 256;
+
+// Rows [rows, heads, D] with any strides into rows of `to` values, a multiple of 8, zeros behind the head's end.
+template <typename T>
+__global__ void __launch_bounds__(kAtThreads)
+attention_pack_kernel(AtTensor t, T *out, int64_t rows, int heads, int D, int to) {
+    const int64_t total = rows * heads * to;
+    for (int64_t i = (int64_t)blockIdx.x * kAtThreads + threadIdx.x; i < total; i += (int64_t)gridDim.x * kAtThreads) {
+        const int64_t rh = i / to, r = rh / heads;
+        const int d = (int)(i - rh * to), h = (int)(rh - r * heads);
+        out[i] = d < D ? ((const T *)t.p)[r * t.row + h * t.head + d] : dtype_traits<T>::from_f(0.f);
+    }
+}
+
+// delta[row, head] = grad . out, eight lanes each. Bound: HBM.
+template <typename T, bool WIDE>
+__global__ void __launch_bounds__(kAtThreads)
+attention_delta_kernel(const __grid_constant__ AtArgs a) {
+    const int64_t rh = ((int64_t)blockIdx.x * kAtThreads + threadIdx.x) >> 3;
+    const int lane = threadIdx.x & 7;
+    const bool in = rh < (int64_t)a.M * a.H;
+    float s = 0.f;
+    if (in) {
+        const int64_t r = rh / a.H;
+        const T *g = (const T *)a.grad.p + r * a.grad.row + (rh - r * a.H) * a.grad.head;
+        const T *o = (const T *)a.out_in + rh * a.D;
+        if constexpr (WIDE) {
+            constexpr int V = 16 / sizeof(T);
+            for (int d = lane * V; d < a.D; d += 8 * V) {
+                const uint4 x = *(const uint4 *)(g + d), y = *(const uint4 *)(o + d);
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    s = fmaf(dtype_traits<T>::to_f(((const T *)&x)[i]), dtype_traits<T>::to_f(((const T *)&y)[i]), s);
+            }
+        } else {
+            for (int d = lane; d < a.D; d += 8) s = fmaf(dtype_traits<T>::to_f(g[d]), dtype_traits<T>::to_f(o[d]), s);
+        }
+    }
+#pragma unroll
+    for (int o = 4; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (in && lane == 0) a.delta[rh] = s;
+}
+
+// A row's splits: out = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s, a warp each.
+template <typename T>
+__global__ void __launch_bounds__(kAtThreads)
+attention_join_kernel(const __grid_constant__ AtArgs a) {
+    const int64_t all = (int64_t)a.M * a.H, rh = ((int64_t)blockIdx.x * kAtThreads + threadIdx.x) >> 5;
+    const int lane = threadIdx.x & 31;
+    if (rh >= all) return;
+    float m = -INFINITY;
+    bool nan = false;
+    for (int s = lane; s < a.splits; s += 32) {
+        const float x = a.part_ml[s * all + rh].x;
+        m = fmaxf(m, x);
+        nan |= isnan(x);
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (__any_sync(0xffffffffu, nan)) m = NAN;
+    float acc[8] = {}, sum = 0.f;
+    bool some = false;
+    for (int s = 0; s < a.splits; ++s) {
+        const float2 ml = a.part_ml[s * all + rh];
+        if (ml.x == -INFINITY && ml.y == 0.f) continue;         // saw no key: there may be nothing written
+        some = true;
+        const float w = exp2f(ml.x - m);
+        sum = fmaf(w, ml.y, sum);
+        const float *p = a.partial + (s * all + rh) * a.D;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (lane + 32 * j < a.D) acc[j] = fmaf(w, p[lane + 32 * j], acc[j]);
+    }
+    const float inv = some ? 1.f / sum : 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+        if (lane + 32 * j < a.D) ((T *)a.out)[rh * a.D + lane + 32 * j] = dtype_traits<T>::from_f(acc[j] * inv);
+    if (lane == 0 && a.lse) a.lse[rh] = some ? m + log2f(sum) : INFINITY;
+}
+
+// out[i] = sum of the splits' partial[s * stride + i], in order.
+template <typename T>
+__global__ void __launch_bounds__(kAtThreads)
+attention_sum_kernel(const float *partial, int64_t stride, int splits, T *out, int64_t n) {
+    const int64_t i = (int64_t)blockIdx.x * kAtThreads + threadIdx.x;
+    if (i >= n) return;
+    float s = 0.f;
+    for (int k = 0; k < splits; ++k) s += partial[k * stride + i];
+    out[i] = dtype_traits<T>::from_f(s);
+}
+
+static unsigned at_blocks(int64_t threads) { return (unsigned)((threads + kAtThreads - 1) / kAtThreads); }
+
+template <typename F>
+static int at_by_type(int dtype, F f) {
+    if (dtype == SPCONV_F32) return f((float *)nullptr);
+    if (dtype == SPCONV_F16) return f((__half *)nullptr);
+    return f((__nv_bfloat16 *)nullptr);
+}
+
+// Whether TMA can read the tensor as it is: 16-byte strides (none of zero) and address, whole 16-byte heads.
+static bool at_tma(const AtTensor &t, int64_t rows, int heads, int D) {
+    return D % 8 == 0 && ((uintptr_t)t.p & 15) == 0 && (rows == 1 || (t.row % 8 == 0 && t.row > 0 && t.row < (int64_t)1 << 38)) &&
+           (heads == 1 || (t.head % 8 == 0 && t.head > 0 && t.head < (int64_t)1 << 38));
+}
+
+// Where things lie in the workspace, and how the work is cut.
+struct AtPlan {
+    bool tc;
+    int tiles2;                          // forward: two tiles a CTA
+    int splits[3];                       // forward (or queries' gradients), and keys' gradients
+    bool pack[4];                        // q, k, v, grad
+    int64_t pack_at[4], delta_at, ml_at, partial_at, bytes;
+};
+
+static int at_cut(int64_t ctas, int64_t slots, int64_t tiles, int least) {
+    if (ctas == 0 || ctas >= slots) return 1;
+    return (int)std::max<int64_t>(1, std::min<int64_t>({slots / ctas, tiles / least, 256}));
+}
+
+static AtPlan at_plan(const spconv_attention_args *q, bool backward) {
+    AtPlan p = {};
+    const int64_t M = q->num_queries, N = q->num_keys, B = q->num_samples;
+    p.tc = q->kernel != SPCONV_KERNEL_SIMT && q->dtype != SPCONV_F32 && q->head_size <= 128 && M > 0 && N > 0;
+    const int G = q->heads / q->key_heads;
+    int P = 1;
+    while (P < 128 && G % (2 * P) == 0) P *= 2;
+    const int64_t mean_q = (M + B - 1) / B, mean_k = (N + B - 1) / B;
+    auto up = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
+    if (p.tc) {
+        const int64_t rows = mean_q * P, heads = q->heads / P;
+        p.tiles2 = 0;
+        p.splits[0] = at_cut(B * up(rows, 128) * heads, 148 * (backward ? 1 : 2), up(mean_k, 128), 2);
+        p.splits[1] = at_cut(B * up(mean_k, 128) * q->key_heads, 148, up(rows, 128) * (G / P), 2);
+    } else {
+        const int64_t R = at_simt_rows(q->head_size);
+        p.splits[0] = at_cut(B * up(mean_q, R) * q->heads, 296, up(mean_k, R), 2);
+        p.splits[1] = at_cut(B * up(mean_k, R) * q->key_heads, 296, up(mean_q, R) * G, 2);
+    }
+    int64_t at = 0;
+    auto take = [&](int64_t bytes) {
+        const int64_t here = at;
+        at += (bytes + 255) / 256 * 256;
+        return here;
+    };
+    const AtTensor t[4] = {{q->query, q->query_row, q->query_head}, {q->key, q->key_row, q->key_head},
+                           {q->value, q->value_row, q->value_head}, {q->grad_out, q->grad_row, q->grad_head}};
+    for (int i = 0; i < (backward ? 4 : 3); ++i) {
+        const bool keys = i == 1 || i == 2;
+        p.pack[i] = p.tc && !at_tma(t[i], keys ? N : M, keys ? q->key_heads : q->heads, q->head_size);
+        if (p.pack[i]) p.pack_at[i] = take((keys ? N * q->key_heads : M * q->heads) * (int64_t)((q->head_size + 7) / 8 * 16));
+    }
+    const int64_t rows = M * q->heads, krows = N * q->key_heads;
+    if (backward) {
+        p.delta_at = take(rows * 4);
+        p.partial_at = take(std::max(p.splits[0] > 1 ? p.splits[0] * rows * q->head_size * 4 : 0,
+                                     p.splits[1] > 1 ? 2 * p.splits[1] * krows * q->head_size * 4 : 0));
+    } else if (p.splits[0] > 1) {
+        p.ml_at = take(p.splits[0] * rows * 8);
+        p.partial_at = take(p.splits[0] * rows * q->head_size * 4);
+    }
+    p.bytes = at;
+    return p;
+}
+
+static int at_check(const spconv_attention_args *q, bool backward) {
+    SPCONV_REQUIRE(q != nullptr, SPCONV_ERR_ARG, "null pointer argument");
+    SPCONV_REQUIRE(q->dtype == SPCONV_F32 || q->dtype == SPCONV_F16 || q->dtype == SPCONV_BF16, SPCONV_ERR_ARG,
+                   "unsupported dtype code %d", q->dtype);
+    SPCONV_REQUIRE(q->kernel >= SPCONV_KERNEL_AUTO && q->kernel <= SPCONV_KERNEL_TCGEN05, SPCONV_ERR_ARG,
+                   "unknown kernel choice %d", q->kernel);
+    SPCONV_REQUIRE(q->num_queries >= 0 && q->num_queries < (int64_t)1 << 31 && q->num_keys >= 0 && q->num_keys < (int64_t)1 << 31,
+                   SPCONV_ERR_ARG, "row counts must be in [0, 2^31)");
+    SPCONV_REQUIRE(q->num_samples >= 1 && q->num_samples < 1 << 24, SPCONV_ERR_ARG, "num_samples must be in [1, 2^24)");
+    SPCONV_REQUIRE(q->key_heads >= 1 && q->heads >= q->key_heads && q->heads <= 65535 && q->heads % q->key_heads == 0, SPCONV_ERR_ARG,
+                   "heads must be a multiple of key_heads, at most 65535");
+    SPCONV_REQUIRE(q->head_size >= 1 && q->head_size <= SPCONV_ATTENTION_MAX_SIZE, SPCONV_ERR_ARG, "head size must be in [1, %d]",
+                   SPCONV_ATTENTION_MAX_SIZE);
+    SPCONV_REQUIRE(q->scale > 0.f && q->scale < INFINITY, SPCONV_ERR_ARG, "scale must be positive and finite");
+    SPCONV_REQUIRE((q->offsets && q->key_offsets) || q->num_samples == 1, SPCONV_ERR_ARG, "several samples need the row offsets of both sides");
+    SPCONV_REQUIRE(q->kernel != SPCONV_KERNEL_TCGEN05 || (q->dtype != SPCONV_F32 && q->head_size <= 128), SPCONV_ERR_UNSUPPORTED,
+                   "the tensor-core kernels take fp16 and bf16 heads of at most 128 values");
+    SPCONV_REQUIRE((q->num_queries == 0 || (q->query && q->out)) && (q->num_keys == 0 || (q->key && q->value)), SPCONV_ERR_ARG,
+                   "null pointer argument");
+    if (backward)
+        SPCONV_REQUIRE((q->num_queries == 0 || (q->grad_out && q->row_stats)), SPCONV_ERR_ARG, "null pointer argument");
+    const int64_t need = at_plan(q, backward).bytes;
+    SPCONV_REQUIRE(need == 0 || (q->workspace && ((uintptr_t)q->workspace & 255) == 0 && q->workspace_bytes >= need), SPCONV_ERR_ARG,
+                   "workspace missing, misaligned or too small");
+    return SPCONV_OK;
+}
+
+static int at_prepare(const spconv_attention_args *q, const AtPlan &p, bool backward, cudaStream_t st, AtArgs &a) {
+    a = {};
+    a.q = {q->query, q->query_row, q->query_head};
+    a.k = {q->key, q->key_row, q->key_head};
+    a.v = {q->value, q->value_row, q->value_head};
+    a.grad = {q->grad_out, q->grad_row, q->grad_head};
+    a.out = q->out;
+    a.out_in = q->out;
+    a.lse = q->row_stats;
+    a.gq = q->grad_query;
+    a.gk = q->grad_key;
+    a.gv = q->grad_value;
+    a.offsets = q->offsets;
+    a.key_offsets = q->key_offsets;
+    a.B = q->num_samples;
+    a.M = (int)q->num_queries;
+    a.N = (int)q->num_keys;
+    a.H = q->heads;
+    a.K = q->key_heads;
+    a.D = q->head_size;
+    a.causal = q->causal != 0;
+    a.scale = q->scale;
+    a.c = (float)((double)q->scale * 1.4426950408889634);
+    a.status = q->status;
+    a.wait_ns = wait_limit_ns();
+    a.dtype = q->dtype;
+    a.stream = st;
+    uint8_t *ws = (uint8_t *)q->workspace;
+    a.delta = (float *)(ws + p.delta_at);
+    a.part_ml = (float2 *)(ws + p.ml_at);
+    a.partial = (float *)(ws + p.partial_at);
+    AtTensor *t[4] = {&a.q, &a.k, &a.v, &a.grad};
+    for (int i = 0; i < (backward ? 4 : 3); ++i) {
+        if (!p.pack[i]) continue;
+        const bool keys = i == 1 || i == 2;
+        const int64_t rows = keys ? a.N : a.M;
+        const int heads = keys ? a.K : a.H, to = (a.D + 7) / 8 * 8;
+        const unsigned blocks = (unsigned)std::min<int64_t>(at_blocks(rows * heads * to), 148 * 16);
+        uint16_t *dst = (uint16_t *)(ws + p.pack_at[i]);
+        if (a.dtype == SPCONV_F16) attention_pack_kernel<<<blocks, kAtThreads, 0, st>>>(*t[i], (__half *)dst, rows, heads, a.D, to);
+        else attention_pack_kernel<<<blocks, kAtThreads, 0, st>>>(*t[i], (__nv_bfloat16 *)dst, rows, heads, a.D, to);
+        if (const int rc = check_launch("attention_pack_kernel")) return rc;
+        *t[i] = {dst, (int64_t)heads * to, to};
+    }
+    return SPCONV_OK;
+}
+
+}  // namespace spconv
+
+using namespace spconv;
+
+extern "C" int64_t spconv_attention_workspace_bytes(const spconv_attention_args *q, int backward) {
+    if (!q || q->num_queries < 0 || q->num_keys < 0 || q->num_samples < 1 || q->key_heads < 1 || q->heads < q->key_heads ||
+        q->heads % q->key_heads || q->head_size < 1 || q->head_size > SPCONV_ATTENTION_MAX_SIZE)
+        return -1;
+    return at_plan(q, backward != 0).bytes;
+}
+
+extern "C" int spconv_attention_forward(const spconv_attention_args *q, void *stream) {
+    if (const int rc = at_check(q, false)) return rc;
+    if (q->num_queries == 0) return SPCONV_OK;
+    const AtPlan p = at_plan(q, false);
+    AtArgs a;
+    if (const int rc = at_prepare(q, p, false, (cudaStream_t)stream, a)) return rc;
+    a.splits = p.splits[0];
+    if (const int rc = launch_at_simt_forward(a)) return rc;
+    if (a.splits == 1) return SPCONV_OK;
+    return at_by_type(a.dtype, [&](auto *t) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        attention_join_kernel<T><<<at_blocks((int64_t)a.M * a.H * 32), kAtThreads, 0, a.stream>>>(a);
+        return check_launch("attention_join_kernel");
+    });
+}
+
+extern "C" int spconv_attention_backward(const spconv_attention_args *q, void *stream) {
+    if (const int rc = at_check(q, true)) return rc;
+    const AtPlan p = at_plan(q, true);
+    AtArgs a;
+    if (const int rc = at_prepare(q, p, true, (cudaStream_t)stream, a)) return rc;
+    if (a.M > 0) {
+        const bool wide = a.D % 8 == 0 && (((uintptr_t)q->grad_out | (uintptr_t)q->out) & 15) == 0 && q->grad_row % 8 == 0 && q->grad_head % 8 == 0;
+        AtArgs d = a;
+        d.grad = {q->grad_out, q->grad_row, q->grad_head};
+        const int rc = at_by_type(a.dtype, [&](auto *t) {
+            using T = std::remove_pointer_t<decltype(t)>;
+            auto kern = wide ? attention_delta_kernel<T, true> : attention_delta_kernel<T, false>;
+            kern<<<at_blocks((int64_t)a.M * a.H * 8), kAtThreads, 0, a.stream>>>(d);
+            return check_launch("attention_delta_kernel");
+        });
+        if (rc) return rc;
+    }
+    auto join = [&](const float *from, int64_t stride, void *to, int64_t n) {
+        if (!to || n == 0) return (int)SPCONV_OK;
+        return at_by_type(a.dtype, [&](auto *t) {
+            using T = std::remove_pointer_t<decltype(t)>;
+            attention_sum_kernel<T><<<at_blocks(n), kAtThreads, 0, a.stream>>>(from, stride, a.splits, (T *)to, n);
+            return check_launch("attention_sum_kernel");
+        });
+    };
+    if (a.gq && a.M > 0) {
+        a.splits = p.splits[0];
+        if (const int rc = launch_at_simt_grad_query(a)) return rc;
+        const int64_t n = (int64_t)a.M * a.H * a.D;
+        if (a.splits > 1)
+            if (const int rc = join(a.partial, n, a.gq, n)) return rc;
+    }
+    if ((a.gk || a.gv) && a.N > 0) {
+        a.splits = p.splits[1];
+        if (const int rc = launch_at_simt_grad_key(a)) return rc;
+        const int64_t n = (int64_t)a.N * a.K * a.D;
+        if (a.splits > 1) {
+            if (const int rc = join(a.partial, 2 * n, a.gk, n)) return rc;
+            if (const int rc = join(a.partial + n, 2 * n, a.gv, n)) return rc;
+        }
+    }
+    return SPCONV_OK;
+}

@@ -1,0 +1,69 @@
+// What every attention kernel does with the samples' offsets.
+#pragma once
+
+#include "attention_internal.h"
+#include "common.cuh"
+
+namespace spconv {
+
+__device__ __forceinline__ int at_offset(const int32_t *offsets, int b, int rows) {
+    return offsets ? max(0, min(rows, __ldg(offsets + b))) : (b ? rows : 0);
+}
+
+struct AtSample {
+    int b, tile;                         // the sample and the tile's number in it
+    int q0, q1, k0, k1;                  // its query and key rows
+};
+
+// The sample that tile `t` belongs to, where sample b's tiles are numbered from rows(b) / per_tile + b (its rows
+// never need more than the next one's number; a tile past a sample's end has nothing to do). By a converged warp, 32 samples
+// a step; ends inside [0, B) whatever the offsets hold.
+__device__ __forceinline__ AtSample at_find(const int32_t *by, int rows, const AtArgs &a, int t, int per_tile) {
+    const int lane = threadIdx.x & 31;
+    int lo = 0, hi = a.B;
+    while (hi - lo > 1) {
+        const int step = (hi - lo + 31) >> 5, at = lo + lane * step;
+        const bool in = lane == 0 || (at < hi && at_offset(by, at, rows) / per_tile + at <= t);
+        const int last = 31 - __clz((int)__ballot_sync(0xffffffffu, in));
+        lo += last * step;
+        hi = min(hi, lo + step);
+    }
+    AtSample s;
+    s.b = lo;
+    s.tile = t - (at_offset(by, lo, rows) / per_tile + lo);
+    s.q0 = at_offset(a.offsets, lo, a.M);
+    s.q1 = max(s.q0, at_offset(a.offsets, lo + 1, a.M));
+    s.k0 = at_offset(a.key_offsets, lo, a.N);
+    s.k1 = max(s.k0, at_offset(a.key_offsets, lo + 1, a.N));
+    return s;
+}
+
+// Offsets have to ascend from 0 to the rows; by the first block.
+__device__ __forceinline__ void at_check_offsets(const AtArgs &a) {
+    if (blockIdx.x | blockIdx.y | blockIdx.z) return;
+    bool bad = false;
+    for (int which = 0; which < 2; ++which) {
+        const int32_t *o = which ? a.key_offsets : a.offsets;
+        const int rows = which ? a.N : a.M;
+        if (!o) continue;
+        for (int s = threadIdx.x; s < a.B; s += blockDim.x) {
+            const int lo = __ldg(o + s), hi = __ldg(o + s + 1);
+            bad |= lo > hi || (s == 0 && lo != 0) || (s == a.B - 1 && hi != rows);
+        }
+    }
+    if (bad) raise_status(a.status, SPCONV_STATUS_OFFSETS);
+}
+
+// Keys that query i of a sample of n queries and m keys sees: the last query sees the last key.
+__device__ __forceinline__ int at_seen(const AtArgs &a, int i, int n, int m) {
+    return a.causal ? (int)max((int64_t)0, min((int64_t)m, (int64_t)i + 1 + m - n)) : m;
+}
+
+// Split `s` of `count` tiles: [first, last).
+__device__ __forceinline__ void at_split(int splits, int s, int count, int &first, int &last) {
+    const int per = (count + splits - 1) / splits;
+    first = min(count, s * per);
+    last = min(count, first + per);
+}
+
+}  // namespace spconv

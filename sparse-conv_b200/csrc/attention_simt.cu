@@ -1,0 +1,373 @@
+// Attention on the CUDA cores, in exact fp32 products and sums: fp32 tensors, and 16-bit ones that the tensor-core kernels
+// do not take. Forward, gradient of the queries and gradients of keys and values, each one sweep over tiles of the
+// other side with everything between the inputs and the results in registers and shared memory:
+//
+//   s = q k scale;  p = exp2(s log2(e) - lse);  out = p v;   dp = grad v;  ds = p (dp - delta)
+//   grad_query = scale ds k;  grad_key = scale ds^T q;  grad_value = p^T grad
+//
+// A block of 256 threads takes BM = 64 rows (32 of heads beyond 128 values) of one head and the opposite side's tiles of as many:
+// products of [rows][head] tiles by 16 x 16 threads, 4 x 4 results each (rows 4 ty.., columns tx + 16 j), operands as
+// float4 along the head from rows padded by four floats (no bank conflicts), so that 64 FMAs go with 8 loads of 16 bytes;
+// products along the tile (p v and the like) take single columns tx + 16 j, which spans any head size in sixteens.
+// Bound: the FMA pipe.
+#include <algorithm>
+
+#include "attention_common.cuh"
+
+namespace spconv {
+
+constexpr int kAsThreads = 256;
+
+template <int DP>
+struct AsShape {
+    static constexpr int BM = DP > 128 ? 32 : 64;        // rows of a tile, both sides
+    static constexpr int R = BM / 16;                    // rows, and columns, of a thread
+    static constexpr int C = DP / 16;                    // head columns of a thread
+    static constexpr int LD = DP + 4, LP = BM + 4;
+    static constexpr int kTile = BM * LD, kScores = BM * LP;
+};
+
+// Rows [row0, row0 + valid) of a head into a tile, zeros behind them and behind the head's end.
+template <typename T, int DP>
+__device__ __forceinline__ void as_load(float *dst, const AtTensor &t, int64_t row0, int valid, int head, int D) {
+    using S = AsShape<DP>;
+    const T *src = (const T *)t.p + row0 * t.row + head * t.head;
+    for (int i = threadIdx.x; i < S::BM * DP; i += kAsThreads) {
+        const int r = i / DP, d = i - r * DP;
+        dst[r * S::LD + d] = r < valid && d < D ? dtype_traits<T>::to_f(src[r * t.row + d]) : 0.f;
+    }
+}
+
+// acc[i][j] += a[4 ty + i][.] . b[tx + 16 j][.]
+template <int DP>
+__device__ __forceinline__ void as_dot(const float *a, const float *b, float (&acc)[AsShape<DP>::R][AsShape<DP>::R]) {
+    using S = AsShape<DP>;
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    const float *pa = a + ty * S::R * S::LD, *pb = b + tx * S::LD;
+#pragma unroll 4
+    for (int d = 0; d < DP; d += 4) {
+        float4 x[S::R], y[S::R];
+#pragma unroll
+        for (int i = 0; i < S::R; ++i) x[i] = *(const float4 *)(pa + i * S::LD + d);
+#pragma unroll
+        for (int j = 0; j < S::R; ++j) y[j] = *(const float4 *)(pb + j * 16 * S::LD + d);
+#pragma unroll
+        for (int i = 0; i < S::R; ++i)
+#pragma unroll
+            for (int j = 0; j < S::R; ++j)
+                acc[i][j] = fmaf(x[i].x, y[j].x, fmaf(x[i].y, y[j].y, fmaf(x[i].z, y[j].z, fmaf(x[i].w, y[j].w, acc[i][j]))));
+    }
+}
+
+// acc[i][j] += sum_k p[4 ty + i][k] b[k][tx + 16 j], k < BM
+template <int DP>
+__device__ __forceinline__ void as_rows(const float *p, const float *b, float (&acc)[AsShape<DP>::R][AsShape<DP>::C]) {
+    using S = AsShape<DP>;
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    const float *pp = p + ty * S::R * S::LP, *pb = b + tx;
+#pragma unroll 2
+    for (int k = 0; k < S::BM; k += 4) {
+        float x[S::R][4];
+#pragma unroll
+        for (int i = 0; i < S::R; ++i) *(float4 *)x[i] = *(const float4 *)(pp + i * S::LP + k);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int j = 0; j < S::C; ++j) {
+                const float y = pb[(k + e) * S::LD + 16 * j];
+#pragma unroll
+                for (int i = 0; i < S::R; ++i) acc[i][j] = fmaf(x[i][e], y, acc[i][j]);
+            }
+    }
+}
+
+// acc[i][j] += sum_q p[q][4 ty + i] b[q][tx + 16 j], q < BM
+template <int DP>
+__device__ __forceinline__ void as_cols(const float *p, const float *b, float (&acc)[AsShape<DP>::R][AsShape<DP>::C]) {
+    using S = AsShape<DP>;
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    const float *pp = p + ty * S::R, *pb = b + tx;
+#pragma unroll 4
+    for (int q = 0; q < S::BM; ++q) {
+        float x[S::R];
+#pragma unroll
+        for (int i = 0; i < S::R; ++i) x[i] = pp[q * S::LP + i];
+#pragma unroll
+        for (int j = 0; j < S::C; ++j) {
+            const float y = pb[q * S::LD + 16 * j];
+#pragma unroll
+            for (int i = 0; i < S::R; ++i) acc[i][j] = fmaf(x[i], y, acc[i][j]);
+        }
+    }
+}
+
+// This block's sample, found by its first warp.
+__device__ __forceinline__ AtSample as_sample(const AtArgs &a, const int32_t *by, int rows, int per_tile, AtSample *shared) {
+    at_check_offsets(a);
+    if (threadIdx.x < 32) {
+        const AtSample s = at_find(by, rows, a, blockIdx.x, per_tile);
+        if (threadIdx.x == 0) *shared = s;
+    }
+    __syncthreads();
+    return *shared;
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kAsThreads)
+attention_simt_kernel(const __grid_constant__ AtArgs a) {
+    using S = AsShape<DP>;
+    extern __shared__ __align__(16) float smem[];
+    __shared__ AtSample shared;
+    const AtSample s = as_sample(a, a.offsets, a.M, S::BM, &shared);
+    const int row0 = s.q0 + s.tile * S::BM, rows = min(S::BM, s.q1 - row0);
+    if (s.tile < 0 || rows <= 0) return;
+    float *sq = smem, *sk = sq + S::kTile, *sv = sk + S::kTile, *sp = sv + S::kTile;
+    const int h = blockIdx.y, kh = h / (a.H / a.K), n = s.q1 - s.q0, m = s.k1 - s.k0;
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, i0 = s.tile * S::BM + ty * S::R;
+    int first, last;
+    at_split(a.splits, blockIdx.z, (at_seen(a, s.tile * S::BM + rows - 1, n, m) + S::BM - 1) / S::BM, first, last);
+    as_load<T, DP>(sq, a.q, row0, rows, h, a.D);
+    float acc[S::R][S::C] = {}, top[S::R], sum[S::R] = {};
+#pragma unroll
+    for (int i = 0; i < S::R; ++i) top[i] = -INFINITY;
+    for (int t = first; t < last; ++t) {
+        const int key0 = t * S::BM, valid = min(S::BM, m - key0);
+        __syncthreads();
+        as_load<T, DP>(sk, a.k, s.k0 + key0, valid, kh, a.D);
+        as_load<T, DP>(sv, a.v, s.k0 + key0, valid, kh, a.D);
+        __syncthreads();
+        float x[S::R][S::R] = {};
+        as_dot<DP>(sq, sk, x);
+#pragma unroll
+        for (int i = 0; i < S::R; ++i) {
+            const int seen = at_seen(a, i0 + i, n, m) - key0;
+            float big = top[i];
+#pragma unroll
+            for (int j = 0; j < S::R; ++j) {
+                x[i][j] = tx + 16 * j < seen ? x[i][j] * a.c : -INFINITY;
+                big = fmaxf(big, x[i][j]);
+            }
+#pragma unroll
+            for (int o = 8; o; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+            const float base = big == -INFINITY ? 0.f : big;
+            const float down = exp2f(top[i] - base);           // top -inf: 0
+            top[i] = big;
+            float add = 0.f;
+#pragma unroll
+            for (int j = 0; j < S::R; ++j) {
+                const float p = exp2f(x[i][j] - base);
+                add += p;
+                sp[(ty * S::R + i) * S::LP + tx + 16 * j] = p;
+            }
+            sum[i] = sum[i] * down + add;
+#pragma unroll
+            for (int j = 0; j < S::C; ++j) acc[i][j] *= down;
+        }
+        __syncwarp();                                          // a row's p are of its own 16 lanes
+        as_rows<DP>(sp, sv, acc);
+    }
+#pragma unroll
+    for (int i = 0; i < S::R; ++i) {
+#pragma unroll
+        for (int o = 8; o; o >>= 1) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], o);
+        const int r = ty * S::R + i;
+        if (r >= rows) continue;
+        const int64_t at = (int64_t)(row0 + r) * a.H + h;
+        const bool none = at_seen(a, i0 + i, n, m) == 0;
+        if (a.splits > 1) {
+            const int64_t all = (int64_t)a.M * a.H;
+            if (tx == 0) a.part_ml[blockIdx.z * all + at] = make_float2(top[i], sum[i]);
+#pragma unroll
+            for (int j = 0; j < S::C; ++j)
+                if (tx + 16 * j < a.D) a.partial[(blockIdx.z * all + at) * a.D + tx + 16 * j] = acc[i][j];
+            continue;
+        }
+        if (tx == 0 && a.lse) a.lse[at] = none ? INFINITY : top[i] + log2f(sum[i]);
+        const float inv = 1.f / sum[i];
+#pragma unroll
+        for (int j = 0; j < S::C; ++j)
+            if (tx + 16 * j < a.D) ((T *)a.out)[at * a.D + tx + 16 * j] = dtype_traits<T>::from_f(none ? 0.f : acc[i][j] * inv);
+    }
+}
+
+// p and ds of a tile of queries (rows) and keys (columns) from tiles of q, grad, k and v. The probability of a row that
+// sees a single key is 1 whatever its score: ds is zero, not the difference of two roundings of grad . v.
+template <int DP>
+__device__ __forceinline__ void as_grads(const AtArgs &a, const float *sq, const float *sg, const float *sk, const float *sv,
+                                         float *sp, float *sd, const float (&lse)[AsShape<DP>::R],
+                                         const float (&delta)[AsShape<DP>::R], const int (&seen)[AsShape<DP>::R],
+                                         const bool (&single)[AsShape<DP>::R]) {
+    using S = AsShape<DP>;
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    float x[S::R][S::R] = {}, y[S::R][S::R] = {};
+    as_dot<DP>(sq, sk, x);
+    as_dot<DP>(sg, sv, y);
+#pragma unroll
+    for (int i = 0; i < S::R; ++i)
+#pragma unroll
+        for (int j = 0; j < S::R; ++j) {
+            const bool in = tx + 16 * j < seen[i];
+            const float p = in ? exp2f(fmaf(x[i][j], a.c, -lse[i])) : 0.f;
+            const int at = (ty * S::R + i) * S::LP + tx + 16 * j;
+            if (sp) sp[at] = p;
+            sd[at] = in && !single[i] ? p * (y[i][j] - delta[i]) : 0.f;
+        }
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kAsThreads)
+attention_simt_grad_query_kernel(const __grid_constant__ AtArgs a) {
+    using S = AsShape<DP>;
+    extern __shared__ __align__(16) float smem[];
+    __shared__ AtSample shared;
+    const AtSample s = as_sample(a, a.offsets, a.M, S::BM, &shared);
+    const int row0 = s.q0 + s.tile * S::BM, rows = min(S::BM, s.q1 - row0);
+    if (s.tile < 0 || rows <= 0) return;
+    float *sq = smem, *sg = sq + S::kTile, *sk = sg + S::kTile, *sv = sk + S::kTile, *sd = sv + S::kTile;
+    const int h = blockIdx.y, kh = h / (a.H / a.K), n = s.q1 - s.q0, m = s.k1 - s.k0;
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, i0 = s.tile * S::BM + ty * S::R;
+    int first, last;
+    at_split(a.splits, blockIdx.z, (at_seen(a, s.tile * S::BM + rows - 1, n, m) + S::BM - 1) / S::BM, first, last);
+    as_load<T, DP>(sq, a.q, row0, rows, h, a.D);
+    as_load<T, DP>(sg, a.grad, row0, rows, h, a.D);
+    float acc[S::R][S::C] = {}, lse[S::R], delta[S::R];
+#pragma unroll
+    for (int i = 0; i < S::R; ++i) {
+        const int r = ty * S::R + i;
+        const int64_t at = (int64_t)(row0 + r) * a.H + h;
+        lse[i] = r < rows ? a.lse[at] : INFINITY;
+        delta[i] = r < rows ? a.delta[at] : 0.f;
+    }
+    for (int t = first; t < last; ++t) {
+        const int key0 = t * S::BM, valid = min(S::BM, m - key0);
+        __syncthreads();
+        as_load<T, DP>(sk, a.k, s.k0 + key0, valid, kh, a.D);
+        as_load<T, DP>(sv, a.v, s.k0 + key0, valid, kh, a.D);
+        __syncthreads();
+        int seen[S::R];
+        bool single[S::R];
+#pragma unroll
+        for (int i = 0; i < S::R; ++i) {
+            const int all = at_seen(a, i0 + i, n, m);
+            seen[i] = all - key0;
+            single[i] = all == 1;
+        }
+        as_grads<DP>(a, sq, sg, sk, sv, nullptr, sd, lse, delta, seen, single);
+        __syncwarp();
+        as_rows<DP>(sd, sk, acc);
+    }
+#pragma unroll
+    for (int i = 0; i < S::R; ++i) {
+        const int r = ty * S::R + i;
+        if (r >= rows) continue;
+        const int64_t at = (int64_t)(row0 + r) * a.H + h;
+#pragma unroll
+        for (int j = 0; j < S::C; ++j) {
+            if (tx + 16 * j >= a.D) continue;
+            const float g = acc[i][j] * a.scale;
+            if (a.splits > 1) a.partial[(blockIdx.z * (int64_t)a.M * a.H + at) * a.D + tx + 16 * j] = g;
+            else ((T *)a.gq)[at * a.D + tx + 16 * j] = dtype_traits<T>::from_f(g);
+        }
+    }
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kAsThreads)
+attention_simt_grad_key_kernel(const __grid_constant__ AtArgs a) {
+    using S = AsShape<DP>;
+    extern __shared__ __align__(16) float smem[];
+    __shared__ AtSample shared;
+    const AtSample s = as_sample(a, a.key_offsets, a.N, S::BM, &shared);
+    const int key0 = s.tile * S::BM, row0 = s.k0 + key0, rows = min(S::BM, s.k1 - row0);
+    if (s.tile < 0 || rows <= 0) return;
+    float *sk = smem, *sv = sk + S::kTile, *sq = sv + S::kTile, *sg = sq + S::kTile, *sp = sg + S::kTile, *sd = sp + S::kScores;
+    const int kh = blockIdx.y, G = a.H / a.K, n = s.q1 - s.q0, m = s.k1 - s.k0;
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    // tiles of queries that see a key of this tile, of each of the group's heads
+    const int from = a.causal ? (int)max((int64_t)0, (int64_t)key0 - m + n) / S::BM : 0;
+    const int tiles = max(0, (n + S::BM - 1) / S::BM - from);
+    int first, last;
+    at_split(a.splits, blockIdx.z, tiles * G, first, last);
+    as_load<T, DP>(sk, a.k, row0, rows, kh, a.D);
+    as_load<T, DP>(sv, a.v, row0, rows, kh, a.D);
+    float gk[S::R][S::C] = {}, gv[S::R][S::C] = {};
+    for (int it = first; it < last; ++it) {
+        const int g = it / tiles, t = from + it - g * tiles, h = kh * G + g;
+        const int i0 = t * S::BM, valid = min(S::BM, n - i0);
+        __syncthreads();
+        as_load<T, DP>(sq, a.q, s.q0 + i0, valid, h, a.D);
+        as_load<T, DP>(sg, a.grad, s.q0 + i0, valid, h, a.D);
+        float lse[S::R], delta[S::R];
+        int seen[S::R];
+        bool single[S::R];
+#pragma unroll
+        for (int i = 0; i < S::R; ++i) {
+            const int r = ty * S::R + i;
+            const int64_t at = (int64_t)(s.q0 + i0 + r) * a.H + h;
+            lse[i] = r < valid ? a.lse[at] : INFINITY;
+            delta[i] = r < valid ? a.delta[at] : 0.f;
+            const int all = at_seen(a, i0 + r, n, m);
+            seen[i] = r < valid ? min(rows, all - key0) : 0;
+            single[i] = all == 1;
+        }
+        __syncthreads();
+        as_grads<DP>(a, sq, sg, sk, sv, sp, sd, lse, delta, seen, single);
+        __syncthreads();
+        as_cols<DP>(sp, sg, gv);
+        as_cols<DP>(sd, sq, gk);
+    }
+#pragma unroll
+    for (int i = 0; i < S::R; ++i) {
+        const int r = ty * S::R + i;
+        if (r >= rows) continue;
+        const int64_t all = (int64_t)a.N * a.K, at = (int64_t)(row0 + r) * a.K + kh;
+#pragma unroll
+        for (int j = 0; j < S::C; ++j) {
+            const int d = tx + 16 * j;
+            if (d >= a.D) continue;
+            if (a.splits > 1) {
+                a.partial[((2 * blockIdx.z) * all + at) * a.D + d] = gk[i][j] * a.scale;
+                a.partial[((2 * blockIdx.z + 1) * all + at) * a.D + d] = gv[i][j];
+            } else {
+                if (a.gk) ((T *)a.gk)[at * a.D + d] = dtype_traits<T>::from_f(gk[i][j] * a.scale);
+                if (a.gv) ((T *)a.gv)[at * a.D + d] = dtype_traits<T>::from_f(gv[i][j]);
+            }
+        }
+    }
+}
+
+int at_simt_rows(int D) { return D > 128 ? 32 : 64; }
+
+template <typename T, int DP>
+static int as_run(const AtArgs &a, int what) {
+    using S = AsShape<DP>;
+    static std::atomic<uint64_t> done[3];
+    auto kern = what == 0 ? attention_simt_kernel<T, DP> : what == 1 ? attention_simt_grad_query_kernel<T, DP> : attention_simt_grad_key_kernel<T, DP>;
+    const int smem = 4 * (what == 0 ? 3 * S::kTile + S::kScores : what == 1 ? 4 * S::kTile + S::kScores : 4 * S::kTile + 2 * S::kScores);
+    if (allow_smem(kern, smem, done[what]) != cudaSuccess) return check_launch("attention: shared memory");
+    const int64_t tiles = at_tiles(what == 2 ? a.N : a.M, a.B, S::BM);
+    kern<<<dim3((unsigned)tiles, what == 2 ? a.K : a.H, a.splits), kAsThreads, smem, a.stream>>>(a);
+    return check_launch("attention_simt_kernel");
+}
+
+template <typename T>
+static int as_size(const AtArgs &a, int what) {
+    if (a.D <= 32) return as_run<T, 32>(a, what);
+    if (a.D <= 48) return as_run<T, 48>(a, what);
+    if (a.D <= 64) return as_run<T, 64>(a, what);
+    if (a.D <= 96) return as_run<T, 96>(a, what);
+    if (a.D <= 128) return as_run<T, 128>(a, what);
+    return as_run<T, 256>(a, what);
+}
+
+static int as_type(const AtArgs &a, int what) {
+    if (a.dtype == SPCONV_F32) return as_size<float>(a, what);
+    if (a.dtype == SPCONV_F16) return as_size<__half>(a, what);
+    return as_size<__nv_bfloat16>(a, what);
+}
+
+int launch_at_simt_forward(const AtArgs &a) { return as_type(a, 0); }
+int launch_at_simt_grad_query(const AtArgs &a) { return as_type(a, 1); }
+int launch_at_simt_grad_key(const AtArgs &a) { return as_type(a, 2); }
+
+}  // namespace spconv

@@ -20,6 +20,7 @@ from __future__ import annotations
 import array
 import ctypes
 import functools
+import math
 import operator
 import os
 import threading
@@ -37,6 +38,8 @@ DTYPE_CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 KERNEL_AUTO, KERNEL_SIMT, KERNEL_TCGEN05 = 0, 1, 2
 NOALLOC_MAX_COORDS = 262144   # SPCONV_NOALLOC_MAX_COORDS
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}   # SPCONV_ACT_*
+ROTARY_LAYOUTS = {"half": 0, "interleaved": 1}               # SPCONV_ROTARY_*
+ROTARY_MAX_PAIRS = 128
 NORMS = {"none": 0, "layer": 1, "rms": 2}                    # SPCONV_NORM_*
 CLIP_P2, CLIP_INF = 0, 1
 
@@ -59,6 +62,31 @@ class ResidualNormArgs(ctypes.Structure):
                 ("next_weight", ChannelParam), ("next_bias", ChannelParam),
                 ("offsets", _c_void_p), ("num_samples", _c_int), ("norm", _c_int), ("next_norm", _c_int),
                 ("residual_scale", ctypes.c_float), ("eps", ctypes.c_float),
+                ("workspace", _c_void_p), ("workspace_bytes", _c_i64), ("status", _c_void_p)]
+
+
+class RotaryArgs(ctypes.Structure):
+    """spconv_rotary_args"""
+    _fields_ = [("dtype", _c_int), ("layout", _c_int), ("num_rows", _c_i64),
+                ("heads", _c_int), ("key_heads", _c_int), ("head_size", _c_int), ("rotary_dim", _c_int),
+                ("axes", _c_int), ("inverse", _c_int), ("amplitude", ctypes.c_float),
+                ("query", _c_void_p), ("key", _c_void_p),
+                ("query_row", _c_i64), ("query_head", _c_i64), ("key_row", _c_i64), ("key_head", _c_i64),
+                ("query_out", _c_void_p), ("key_out", _c_void_p),
+                ("positions", _c_void_p), ("position_row", _c_i64), ("position_col", _c_i64),
+                ("steps", ctypes.c_uint64 * ROTARY_MAX_PAIRS)]
+
+
+class AttentionArgs(ctypes.Structure):
+    """spconv_attention_args"""
+    _fields_ = [("dtype", _c_int), ("kernel", _c_int), ("num_queries", _c_i64), ("num_keys", _c_i64),
+                ("num_samples", _c_int), ("heads", _c_int), ("key_heads", _c_int), ("head_size", _c_int),
+                ("causal", _c_int), ("scale", ctypes.c_float), ("offsets", _c_void_p), ("key_offsets", _c_void_p),
+                ("query", _c_void_p), ("key", _c_void_p), ("value", _c_void_p),
+                ("query_row", _c_i64), ("query_head", _c_i64), ("key_row", _c_i64), ("key_head", _c_i64),
+                ("value_row", _c_i64), ("value_head", _c_i64), ("out", _c_void_p), ("row_stats", _c_void_p),
+                ("grad_out", _c_void_p), ("grad_row", _c_i64), ("grad_head", _c_i64),
+                ("grad_query", _c_void_p), ("grad_key", _c_void_p), ("grad_value", _c_void_p),
                 ("workspace", _c_void_p), ("workspace_bytes", _c_i64), ("status", _c_void_p)]
 
 
@@ -129,6 +157,10 @@ SIGNATURES = {
     "spconv_clip_gradients": (_c_int, [
         _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, ctypes.c_float, _c_void_p,
         _c_void_p, _c_i64, _c_void_p]),
+    "spconv_rotary": (_c_int, [ctypes.POINTER(RotaryArgs), _c_void_p]),
+    "spconv_attention_workspace_bytes": (_c_i64, [ctypes.POINTER(AttentionArgs), _c_int]),
+    "spconv_attention_forward": (_c_int, [ctypes.POINTER(AttentionArgs), _c_void_p]),
+    "spconv_attention_backward": (_c_int, [ctypes.POINTER(AttentionArgs), _c_void_p]),
     "spconv_set_wait_limit_ns": (ctypes.c_uint64, [ctypes.c_uint64]),
     "spconv_stage_timing": (_c_int, [_c_int]),
     "spconv_stage_times_ms": (_c_int, [_c_void_p, _c_void_p, _c_int]),
@@ -1022,6 +1054,166 @@ def clip_gradients(grads: Sequence[torch.Tensor], outs: Sequence[torch.Tensor], 
     torch.autograd.graph.increment_version(outs)
     after_mapped_launch(index)
     return total
+
+
+@functools.lru_cache(maxsize=64)
+def _turn_steps(steps: Tuple[float, ...]) -> bytes:
+    """Angles in 2^-64ths of a full turn, modulo a turn, as the kernel's table holds them."""
+    turns = [int(round(s / (2.0 * math.pi) % 1.0 * 2.0 ** 64)) & (2 ** 64 - 1) for s in steps]
+    return bytes((ctypes.c_uint64 * ROTARY_MAX_PAIRS)(*turns))
+
+
+def _heads(t: torch.Tensor, what: str) -> torch.Tensor:
+    """[rows, heads, size] with a head's values next to one another."""
+    if t.dim() != 3:
+        raise ValueError(f"{what} must be [N, heads, D], got shape {list(t.shape)}")
+    return t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous()
+
+
+@_on_device
+def _rotary_on(first: torch.Tensor, query, key, positions: torch.Tensor, layout: str, rotary_dim: int,
+               steps: Tuple[float, ...], amplitude: float, inverse: bool) -> tuple:
+    dev = _require_cuda(first, query, key, positions)
+    if first.dtype not in DTYPE_CODES:
+        raise TypeError(f"unsupported dtype {first.dtype}")
+    if layout not in ROTARY_LAYOUTS:
+        raise ValueError(f"unsupported layout {layout}")
+    if positions.dtype != torch.int32:
+        raise TypeError(f"positions must be int32, got {positions.dtype}")
+    rows, size = first.shape[0], first.shape[2]
+    if positions.dim() == 1:
+        positions = positions[:, None]
+    if positions.dim() != 2 or positions.shape[0] != rows:
+        raise ValueError(f"positions must have shape [{rows}] or [{rows}, axes], got {list(positions.shape)}")
+    if not 2 <= size <= 2 * ROTARY_MAX_PAIRS:
+        raise ValueError(f"head size must be in [2, {2 * ROTARY_MAX_PAIRS}], got {size}")
+    a = RotaryArgs(dtype=DTYPE_CODES[first.dtype], layout=ROTARY_LAYOUTS[layout], num_rows=rows, head_size=size,
+                   rotary_dim=rotary_dim, axes=positions.shape[1], inverse=inverse, amplitude=amplitude,
+                   positions=positions.data_ptr(), position_row=positions.stride(0), position_col=positions.stride(1))
+    ctypes.memmove(ctypes.addressof(a) + RotaryArgs.steps.offset, _turn_steps(steps), RotaryArgs.steps.size)
+    out = [None, None]
+    kept = []                                 # copies live until the launch
+    for i, (t, what) in enumerate(((query, "query"), (key, "key"))):
+        if t is None:
+            continue
+        if t.dtype != first.dtype:
+            raise TypeError(f"{what} dtype {t.dtype} differs from {first.dtype}")
+        t = _heads(t, what)
+        if t.shape[0] != rows or t.shape[2] != size:
+            raise ValueError(f"{what} must have shape [{rows}, heads, {size}], got {list(t.shape)}")
+        kept.append(t)
+        out[i] = torch.empty(t.shape, dtype=t.dtype, device=dev)
+        if i == 0:
+            a.heads, a.query, a.query_out = t.shape[1], t.data_ptr(), out[0].data_ptr()
+            a.query_row, a.query_head = t.stride(0), t.stride(1)
+        else:
+            a.key_heads, a.key, a.key_out = t.shape[1], t.data_ptr(), out[1].data_ptr()
+            a.key_row, a.key_head = t.stride(0), t.stride(1)
+    if rows == 0 or a.heads + a.key_heads == 0:
+        return tuple(out)
+    index = dev.index
+    mapped_status(index)
+    rc = (_lib or load_library()).spconv_rotary(a, _raw_stream(index))
+    if rc != SPCONV_OK:
+        _raise(rc, "spconv_rotary")
+    after_mapped_launch(index)
+    return tuple(out)
+
+
+def rotary(query: Optional[torch.Tensor], key: Optional[torch.Tensor], positions: torch.Tensor, layout: str,
+           rotary_dim: int, steps: Tuple[float, ...], amplitude: float, inverse: bool = False) -> tuple:
+    """(query, key) with their pairs turned by positions * steps (an axis's pairs), or backwards; None for None."""
+    return _rotary_on(query if query is not None else key, query, key, positions, layout, rotary_dim, steps,
+                      amplitude, inverse)
+
+
+def _offsets(t: torch.Tensor, what: str) -> int:
+    if t.dtype != torch.int32 or t.dim() != 1 or t.numel() < 2 or not t.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous [samples + 1] int32 tensor")
+    return t.numel() - 1
+
+
+def _attention_workspace(a: AttentionArgs, backward: bool, device: torch.device) -> Optional[torch.Tensor]:
+    a.workspace_bytes = need = (_lib or load_library()).spconv_attention_workspace_bytes(a, backward)
+    if need <= 0:
+        return None
+    ws = torch.empty((need,), dtype=torch.uint8, device=device)
+    a.workspace = ws.data_ptr()
+    return ws
+
+
+@_on_device
+def attention_forward(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, offsets: Optional[torch.Tensor],
+                      key_offsets: Optional[torch.Tensor], causal: bool, scale: float, keep_stats: bool = False,
+                      kernel: int = KERNEL_AUTO) -> tuple:
+    """(out, row statistics if ``keep_stats`` else None, the call's arguments for attention_backward_of)."""
+    dev = _require_cuda(query, key, value, offsets, key_offsets)
+    if query.dtype not in DTYPE_CODES:
+        raise TypeError(f"unsupported dtype {query.dtype}")
+    for t, what in ((key, "key"), (value, "value")):
+        if t.dtype != query.dtype:
+            raise TypeError(f"{what} dtype {t.dtype} differs from the query's {query.dtype}")
+    query, key, value = _heads(query, "query"), _heads(key, "key"), _heads(value, "value")
+    M, H, D = query.shape
+    N, K, _ = key.shape
+    if key.shape != value.shape or key.shape[2] != D:
+        raise ValueError(f"key and value must have shape [keys, key heads, {D}], got {list(key.shape)} and {list(value.shape)}")
+    if K < 1 or H < K or H % K:
+        raise ValueError(f"{H} query heads are no multiple of {K} key heads")
+    if not 1 <= D <= 256:
+        raise ValueError(f"head size must be in [1, 256], got {D}")
+    if not (scale > 0.0 and scale < float("inf")):
+        raise ValueError(f"scale must be positive and finite, got {scale}")
+    samples = 1 if offsets is None else _offsets(offsets, "batch_offsets")
+    if key_offsets is not None and _offsets(key_offsets, "key_offsets") != samples:
+        raise ValueError("batch_offsets and key_offsets must have the same number of samples")
+    index = dev.index
+    a = AttentionArgs(dtype=DTYPE_CODES[query.dtype], kernel=kernel, num_queries=M, num_keys=N, num_samples=samples,
+                      heads=H, key_heads=K, head_size=D, causal=bool(causal), scale=scale,
+                      offsets=_ptr(offsets), key_offsets=_ptr(key_offsets),
+                      query=query.data_ptr(), key=key.data_ptr(), value=value.data_ptr(),
+                      query_row=query.stride(0), query_head=query.stride(1), key_row=key.stride(0),
+                      key_head=key.stride(1), value_row=value.stride(0), value_head=value.stride(1))
+    out = torch.empty((M, H, D), dtype=query.dtype, device=dev)
+    a.out = out.data_ptr()
+    stats = None
+    if keep_stats:
+        stats = torch.empty((M, H), dtype=torch.float32, device=dev)
+        a.row_stats = stats.data_ptr()
+    if M == 0:
+        return out, stats, a
+    ws = _attention_workspace(a, False, dev)
+    a.status = mapped_status(index)
+    rc = _lib.spconv_attention_forward(a, _raw_stream(index))
+    if rc != SPCONV_OK:
+        _raise(rc, "spconv_attention_forward")
+    after_mapped_launch(index)
+    return out, stats, a
+
+
+def attention_backward_of(args: AttentionArgs, query, key, value, offsets, key_offsets, out, stats, grad_out, needs) -> list:
+    """Gradients of query, key and value (None where ``needs`` says so), contiguous, with the arguments that a
+    forward of the same tensors has checked: addresses and strides are taken anew (saved tensors may have been moved)."""
+    index = query.get_device()
+    query, key, value, grad_out = (_heads(t, "grad_out") for t in (query, key, value, grad_out))
+    out = out.contiguous()
+    a = AttentionArgs.from_buffer_copy(args)
+    a.workspace = None
+    a.query, a.key, a.value = query.data_ptr(), key.data_ptr(), value.data_ptr()
+    (a.query_row, a.query_head, _), (a.key_row, a.key_head, _), (a.value_row, a.value_head, _) = (
+        query.stride(), key.stride(), value.stride())
+    a.offsets, a.key_offsets = _ptr(offsets), _ptr(key_offsets)
+    a.out, a.row_stats = out.data_ptr(), stats.data_ptr()
+    a.grad_out, a.grad_row, a.grad_head = grad_out.data_ptr(), grad_out.stride(0), grad_out.stride(1)
+    grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if n else None for t, n in zip((query, key, value), needs)]
+    a.grad_query, a.grad_key, a.grad_value = map(_ptr, grads)
+    ws = _attention_workspace(a, True, query.device)
+    a.status = mapped_status(index)
+    rc = _lib.spconv_attention_backward(a, _raw_stream(index))
+    if rc != SPCONV_OK:
+        _raise(rc, "spconv_attention_backward")
+    after_mapped_launch(index)
+    return grads
 
 
 def set_wait_limit_ns(limit_ns: int) -> int:
