@@ -141,7 +141,7 @@ static AtPlan at_plan(const spconv_attention_args *q, bool backward) {
     auto up = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
     if (p.tc) {
         const int64_t rows = mean_q * P, heads = q->heads / P;
-        p.tiles2 = 0;
+        p.tiles2 = !backward && rows > 192 && mean_k > 512 && B * up(rows, 256) * heads >= 148;
         p.splits[0] = at_cut(B * up(rows, 128) * heads, 148 * (backward ? 1 : 2), up(mean_k, 128), 2);
         p.splits[1] = at_cut(B * up(mean_k, 128) * q->key_heads, 148, up(rows, 128) * (G / P), 2);
     } else {
@@ -267,7 +267,7 @@ extern "C" int spconv_attention_forward(const spconv_attention_args *q, void *st
     AtArgs a;
     if (const int rc = at_prepare(q, p, false, (cudaStream_t)stream, a)) return rc;
     a.splits = p.splits[0];
-    if (const int rc = launch_at_simt_forward(a)) return rc;
+    if (const int rc = p.tc ? launch_at_tc_forward(a, p.tiles2) : launch_at_simt_forward(a)) return rc;
     if (a.splits == 1) return SPCONV_OK;
     return at_by_type(a.dtype, [&](auto *t) {
         using T = std::remove_pointer_t<decltype(t)>;

@@ -779,22 +779,19 @@ static EncodeTiledFn tensor_map_encoder() {
     return fn;
 }
 
-bool make_tmap_2d(CUtensorMap *map, const void *ptr, uint64_t cols, uint64_t rows,
-                         uint64_t row_stride, uint32_t box_cols, uint32_t box_rows) {
+static bool encode_tmap(CUtensorMap *map, const void *ptr, cuuint32_t rank, const cuuint64_t *dims, const cuuint64_t *strides,
+                        const cuuint32_t *box) {
     EncodeTiledFn enc = tensor_map_encoder();
     if (!enc) {
         set_error("cuTensorMapEncodeTiled is not available from the driver");
         return false;
     }
-    const cuuint64_t dims[2] = {cols, rows};
-    const cuuint64_t strides[1] = {row_stride};
-    const cuuint32_t box[2] = {box_cols, box_rows};
-    const cuuint32_t estr[2] = {1, 1};
-    const uint32_t wbytes = box_cols * 2;
+    const cuuint32_t estr[3] = {1, 1, 1};
+    const uint32_t wbytes = box[0] * 2;
     const CUtensorMapSwizzle sw = wbytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B
                                 : (wbytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B);
     auto encode = [&]() {
-        return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void *>(ptr), dims, strides, box, estr,
+        return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, rank, const_cast<void *>(ptr), dims, strides, box, estr,
                    CU_TENSOR_MAP_INTERLEAVE_NONE, sw, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     };
@@ -810,6 +807,22 @@ bool make_tmap_2d(CUtensorMap *map, const void *ptr, uint64_t cols, uint64_t row
         return false;
     }
     return true;
+}
+
+bool make_tmap_2d(CUtensorMap *map, const void *ptr, uint64_t cols, uint64_t rows,
+                         uint64_t row_stride, uint32_t box_cols, uint32_t box_rows) {
+    const cuuint64_t dims[2] = {cols, rows};
+    const cuuint64_t strides[1] = {row_stride};
+    const cuuint32_t box[2] = {box_cols, box_rows};
+    return encode_tmap(map, ptr, 2, dims, strides, box);
+}
+
+bool make_tmap_3d(CUtensorMap *map, const void *ptr, uint64_t x, uint64_t y, uint64_t z, uint64_t y_stride, uint64_t z_stride,
+                  uint32_t box_x, uint32_t box_y, uint32_t box_z) {
+    const cuuint64_t dims[3] = {x, y, z};
+    const cuuint64_t strides[2] = {y_stride, z_stride};
+    const cuuint32_t box[3] = {box_x, box_y, box_z};
+    return encode_tmap(map, ptr, 3, dims, strides, box);
 }
 
 // Gatherer warps: four, whether a CTA has an SM to itself (large stages) or two CTAs share
