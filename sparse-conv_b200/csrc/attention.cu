@@ -303,14 +303,14 @@ extern "C" int spconv_attention_backward(const spconv_attention_args *q, void *s
     };
     if (a.gq && a.M > 0) {
         a.splits = p.splits[0];
-        if (const int rc = launch_at_simt_grad_query(a)) return rc;
+        if (const int rc = p.tc ? launch_at_tc_grad_query(a) : launch_at_simt_grad_query(a)) return rc;
         const int64_t n = (int64_t)a.M * a.H * a.D;
         if (a.splits > 1)
             if (const int rc = join(a.partial, n, a.gq, n)) return rc;
     }
     if ((a.gk || a.gv) && a.N > 0) {
         a.splits = p.splits[1];
-        if (const int rc = launch_at_simt_grad_key(a)) return rc;
+        if (const int rc = p.tc ? launch_at_tc_grad_key(a) : launch_at_simt_grad_key(a)) return rc;
         const int64_t n = (int64_t)a.N * a.K * a.D;
         if (a.splits > 1) {
             if (const int rc = join(a.partial, 2 * n, a.gk, n)) return rc;

@@ -1,0 +1,603 @@
+// Attention's gradients on the 5th-generation tensor cores (tcgen05 / TMEM), fp16 and bf16, heads of up to 128 values:
+//
+//   p = 2^(s c - lse);  dp = grad v^T;  ds = p (dp - delta);  delta = grad . out
+//   grad_query = scale ds k;   grad_key = scale ds^T q;   grad_value = p^T grad
+//
+// Two sweeps, each recomputing s and dp: one owns 128 query rows and walks the keys, one owns 128 keys and walks the rows of
+// every query head that reads them (so the gradients of shared keys add up in the accumulators). That is seven products
+// a tile where one sweep with atomic sums of grad_query would have five, but every sum has one owner and one order: the
+// same bits every run, no fp32 copy of a gradient in memory.
+//
+// A CTA an SM: eight warps compute, a thread a row and half of the 128 columns; one loads (TMA), one issues the
+// products. ds (and p) go back to TMEM in 16 bits, over s and dp, and are the A operand of the second products
+// from there; B is the tile that s or dp was made of, read along its rows (MN-major). While the threads work on one
+// of s and dp, the products that make the other run.
+//
+// p of the keys' sweep is scaled by 2^15 in fp16, whose smallest values would else lose bits where a row sees
+// thousands of keys; grad_value is scaled back in fp32. A row that sees a single key has ds = 0 exactly.
+// Rows behind a sample's end are treated as in the forward: zeroed in shared memory where a product sums over rows.
+#include <algorithm>
+
+#include "attention_tc.cuh"
+
+namespace spconv {
+
+constexpr int kAbThreads = 320;
+constexpr int kAbWarpLoad = 8, kAbWarpMma = 9;
+
+// The lane's 64 columns of a half tile.
+__device__ __forceinline__ void ab_load64(uint32_t taddr, f32x2 (&x)[32]) {
+    lt_load32(taddr, *reinterpret_cast<f32x2(*)[16]>(x));
+    lt_load32(taddr + 32, *reinterpret_cast<f32x2(*)[16]>(x + 16));
+}
+
+// A row of accumulators [from, to) times `factor`, to a row of D values: rounded, or fp32 where `part` is given.
+template <typename T>
+__device__ __forceinline__ void ab_store_row(uint32_t taddr, int from, int to, int D, bool zero, float factor, bool mine, T *out, float *part) {
+    const bool wide = (D & 7) == 0 && ((uintptr_t)out & 15) == 0;
+#pragma unroll 1
+    for (int c = from; c < to && c < D; c += 32) {
+        f32x2 o[16];
+        if (!zero) lt_load32(taddr + c, o);
+        if (!mine) continue;
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+            const int d = c + v * 8;
+            if (d >= D) break;
+            float f[8];
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 u = unpack_f32x2(o[v * 4 + i]);
+                f[2 * i] = zero ? 0.f : u.x * factor;
+                f[2 * i + 1] = zero ? 0.f : u.y * factor;
+                w[i] = lt_pack<T>(f[2 * i], f[2 * i + 1]);
+            }
+            if (part) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (d + i < D) part[d + i] = f[i];
+            } else if (wide) {
+                *(uint4 *)(out + d) = make_uint4(w[0], w[1], w[2], w[3]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (d + i < D) out[d + i] = dtype_traits<T>::from_f(f[i]);
+            }
+        }
+    }
+}
+
+template <int DP>
+struct AqShape {
+    static constexpr int kTile = DP / 64 * kAtBlock;
+    static constexpr int kK = DP == 64 ? 4 : 3, kV = DP == 64 ? 4 : 2;          // stages
+    static constexpr int kSmem = 1024 + (2 + kK + kV) * kTile + 512;
+};
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kAbThreads, 1)
+attention_tc_grad_query_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                               const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_g,
+                               const __grid_constant__ AtArgs a, const int log_p) {
+    using S = AqShape<DP>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *base = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    const uint32_t s_q = smem_u32(base), s_g = s_q + S::kTile, s_k = s_g + S::kTile, s_v = s_k + S::kK * S::kTile;
+    uint64_t *bar = reinterpret_cast<uint64_t *>(base + (2 + S::kK + S::kV) * S::kTile);
+    uint64_t *kfull = bar, *kempty = kfull + S::kK, *vfull = kempty + S::kK, *vempty = vfull + S::kV;
+    uint64_t *qfull = vempty + S::kV, *tail = qfull + 1, *sfull = tail + 1, *dpfull = sfull + 2, *dsready = dpfull + 1, *finished = dsready + 1;
+    uint32_t *s_tmem = reinterpret_cast<uint32_t *>(finished + 1);
+    volatile int *s_abort = reinterpret_cast<volatile int *>(s_tmem + 1);
+    AtSample *s_sample = reinterpret_cast<AtSample *>(s_tmem + 2);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int P = 1 << log_p, tokens = kAtRows >> log_p;
+
+    at_check_offsets(a);
+    if (warp == kAbWarpLoad) {
+        const AtSample s = at_find(a.offsets, a.M, a, a.causal ? gridDim.x - 1 - blockIdx.x : blockIdx.x, tokens);
+        if (lane == 0) *s_sample = s;
+    }
+    if (tid == 0) {
+        for (int i = 0; i < S::kK; ++i) {
+            mbar_init(smem_u32(&kfull[i]), 1);
+            mbar_init(smem_u32(&kempty[i]), 1);
+        }
+        for (int i = 0; i < S::kV; ++i) {
+            mbar_init(smem_u32(&vfull[i]), 1);
+            mbar_init(smem_u32(&vempty[i]), 1);
+        }
+        for (uint64_t *b : {qfull, tail, sfull, sfull + 1, dpfull, finished}) mbar_init(smem_u32(b), 1);
+        mbar_init(smem_u32(dsready), 8);
+        *s_abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    }
+    __syncthreads();
+    const AtSample s = *s_sample;
+    const int n = s.q1 - s.q0, m = s.k1 - s.k0, t0 = s.tile * tokens;
+    if (s.tile < 0 || t0 >= n) return;
+    if (warp == kAbWarpMma) {
+        tmem_alloc(smem_u32(s_tmem), 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *s_tmem, t_dp = tmem + 256, t_dq = tmem + 384;
+    const int head0 = blockIdx.y << log_p, kh = head0 / (a.H / a.K);
+    const int seen_last = at_seen(a, min(n, t0 + tokens) - 1, n, m);
+    int first, last;
+    at_split(a.splits, blockIdx.z, (seen_last + kAtRows - 1) / kAtRows, first, last);
+    const int tiles = last - first;
+    const int end_valid = min(kAtRows, seen_last - (last - 1) * kAtRows);
+    auto wait = [&](uint64_t *b, uint32_t parity) { return mbar_wait_suspended(smem_u32(b), parity, s_abort, a.wait_ns); };
+    auto next = [](int &i, uint32_t &phase, int stages) {
+        if (++i == stages) {
+            i = 0;
+            phase ^= 1u;
+        }
+    };
+
+    if (warp == kAbWarpLoad) {
+        // ------------------------------------------------------------------ loads: q, grad; then k, v of each tile in turn
+        if (tiles > 0) {
+            auto load = [&](uint32_t dst, const CUtensorMap *map, int head, int row, uint32_t mbar) {
+                for (int c = 0; c < DP / 64; ++c) tma_load_3d(dst + c * kAtBlock, map, c * 64, head, row, mbar);
+            };
+            if (elect_one()) {
+                mbar_arrive_expect_tx(smem_u32(qfull), 2 * S::kTile);
+                load(s_q, &map_q, head0, s.q0 + t0, smem_u32(qfull));
+                load(s_g, &map_g, head0, s.q0 + t0, smem_u32(qfull));
+            }
+            __syncwarp();
+            int ks = 0, vs = 0;
+            uint32_t kp = 1, vp = 1;
+            bool ok = true;
+            for (int j = 0; j < tiles && ok; ++j) {
+                const bool cut = j + 1 == tiles && (end_valid & 15);
+                const int row = s.k0 + (first + j) * kAtRows;
+                if (!(ok = __all_sync(0xffffffffu, wait(&kempty[ks], kp)) != 0)) break;
+                const uint32_t dst = s_k + ks * S::kTile, mbar = smem_u32(cut ? tail : &kfull[ks]);
+                if (elect_one()) {
+                    mbar_arrive_expect_tx(mbar, S::kTile);
+                    load(dst, &map_k, kh, row, mbar);
+                }
+                __syncwarp();
+                if (!(ok = __all_sync(0xffffffffu, wait(&vempty[vs], vp)) != 0)) break;
+                if (elect_one()) {
+                    mbar_arrive_expect_tx(smem_u32(&vfull[vs]), S::kTile);
+                    load(s_v + vs * S::kTile, &map_v, kh, row, smem_u32(&vfull[vs]));
+                }
+                __syncwarp();
+                if (cut) {
+                    ok = __all_sync(0xffffffffu, wait(tail, 0)) != 0;
+                    at_zero_rows<DP>(dst, end_valid, (end_valid + 15) & ~15);
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_u32(&kfull[ks]));
+                }
+                next(ks, kp, S::kK);
+                next(vs, vp, S::kV);
+            }
+        }
+    } else if (warp == kAbWarpMma) {
+        // ------------------------------------------------------------------ products
+        if (tiles > 0 && elect_one()) {
+            const uint32_t id_s = instr_desc_f16(dtype_traits<T>::mma_format, 128, 128);
+            const uint32_t id_o = instr_desc_f16(dtype_traits<T>::mma_format, 128, (a.D + 15) & ~15) | 1u << 16;
+            const int steps = (a.D + 15) >> 4;
+            int ks = 0, vs = 0, done = 0;                            // next k and v stage; the k stage of ds k
+            uint32_t kp = 0, vp = 0, ds_phase = 0;
+            bool ok = wait(qfull, 0);
+            auto scores = [&](int j) {                               // s of tile j
+                if (!(ok = ok && wait(&kfull[ks], kp))) return;
+                tc_fence_after();
+                at_mma_head<DP>(tmem + (j & 1) * 128, s_q, s_k + ks * S::kTile, id_s, steps);
+                tc_commit(smem_u32(&sfull[j & 1]));
+                next(ks, kp, S::kK);
+            };
+            auto products = [&] {                                    // dp of the next tile
+                if (!(ok = ok && wait(&vfull[vs], vp))) return;
+                tc_fence_after();
+                at_mma_head<DP>(t_dp, s_g, s_v + vs * S::kTile, id_s, steps);
+                tc_commit(smem_u32(dpfull));
+                tc_commit(smem_u32(&vempty[vs]));
+                next(vs, vp, S::kV);
+            };
+            scores(0);
+            products();
+            if (tiles > 1) scores(1);
+            for (int j = 0; j < tiles && ok; ++j, ds_phase ^= 1u) {
+                if (!(ok = wait(dsready, ds_phase))) break;
+                tc_fence_after();
+                at_mma_rows(t_dq, tmem + (j & 1) * 128, 32, s_k + done * S::kTile, id_o, j + 1 < tiles ? 8 : (end_valid + 15) >> 4, j > 0);
+                tc_commit(smem_u32(j + 1 < tiles ? &kempty[done] : finished));
+                if (++done == S::kK) done = 0;
+                if (j + 1 < tiles) products();
+                if (j + 2 < tiles) scores(j + 2);
+            }
+        }
+    } else {
+        // ------------------------------------------------------------------ a thread a row and 64 columns
+        const int half = warp >> 2, row = tid & 127;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const int token = t0 + (row >> log_p);
+        const bool mine = token < n;
+        const int seen = mine ? at_seen(a, token, n, m) : 0;
+        const bool some = __any_sync(0xffffffffu, mine);
+        const int seen_all = __reduce_min_sync(0xffffffffu, mine ? seen : m);
+        const int64_t at = (int64_t)(s.q0 + token) * a.H + head0 + (row & (P - 1));
+        const float lse = mine ? a.lse[at] : INFINITY, delta = mine ? a.delta[at] : 0.f;
+        const f32x2 c2 = pack_f32x2(a.c, a.c), l2 = pack_f32x2(-lse, -lse), d2 = pack_f32x2(-delta, -delta);
+        bool ok = true;
+        for (int j = 0; j < tiles; ++j) {
+            const uint32_t t_s = tmem + (j & 1) * 128 + half * 64 + lanes;
+            if (!(ok = __all_sync(0xffffffffu, wait(&sfull[j & 1], (j >> 1) & 1)) != 0)) break;
+            tc_fence_after();
+            f32x2 x[32];
+            const int left = seen - (first + j) * kAtRows - half * 64;
+            const bool masked = (first + j + 1) * kAtRows > seen_all;
+            if (some) {
+                ab_load64(t_s, x);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    const float2 f = unpack_f32x2(fma2(x[i], c2, l2));
+                    x[i] = pack_f32x2(ex2_approx(f.x), ex2_approx(f.y));
+                }
+            }
+            if (!(ok = __all_sync(0xffffffffu, wait(dpfull, j & 1)) != 0)) break;
+            tc_fence_after();
+            if (some) {
+                uint32_t w[32];
+#pragma unroll
+                for (int g = 0; g < 2; ++g) {
+                    f32x2 y[16];
+                    lt_load32(t_dp + half * 64 + g * 32 + lanes, y);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float2 f = unpack_f32x2(mul2(x[g * 16 + i], add2(y[i], d2)));
+                        w[g * 16 + i] = lt_pack<T>(f.x, f.y);
+                    }
+                }
+                if (masked) {                                        // behind the row's keys; all of a single one
+                    const int keep = seen == 1 ? 0 : left;
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) w[i] &= (2 * i < keep ? 0xffffu : 0u) | (2 * i + 1 < keep ? 0xffff0000u : 0u);
+                }
+                tmem_st32(t_s, w);
+                tc_wait_st();
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(dsready));
+        }
+        if (tiles > 0 && ok) ok = __all_sync(0xffffffffu, wait(finished, 0)) != 0;
+        tc_fence_after();
+        if (ok && some) {
+            float *part = a.splits > 1 ? a.partial + (blockIdx.z * (int64_t)a.M * a.H + at) * a.D : nullptr;
+            ab_store_row<T>(t_dq + lanes, half * (DP / 2), (half + 1) * (DP / 2), a.D, tiles == 0, a.scale, mine, (T *)a.gq + at * a.D, part);
+        }
+    }
+
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();                                                 // every role has set the flag by now if it gives up
+    if (*s_abort) {                                                  // copies and products in flight end within this
+        if (tid == 0) raise_status(a.status, SPCONV_STATUS_WAIT_TIMEOUT);
+        const uint64_t begin = globaltimer_ns();
+        while (globaltimer_ns() - begin < kTmaDrainNs) {}
+        __syncthreads();
+    }
+    tc_fence_after();
+    if (warp == kAbWarpMma) tmem_dealloc(tmem, 512);
+}
+
+template <int DP>
+struct AkShape {
+    static constexpr int kTile = DP / 64 * kAtBlock;
+    static constexpr int kStages = DP == 64 ? 4 : 2;                 // of q and grad
+    static constexpr int kSmem = 1024 + (2 + 2 * kStages) * kTile + kStages * 1024 + 512;
+};
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kAbThreads, 1)
+attention_tc_grad_key_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                             const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_g,
+                             const __grid_constant__ AtArgs a, const int log_p) {
+    using S = AkShape<DP>;
+    constexpr float kUp = dtype_traits<T>::mma_format == 0 ? 15.f : 0.f;         // powers of two on p
+    constexpr float kDown = dtype_traits<T>::mma_format == 0 ? 0x1p-15f : 1.f;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *base = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    const uint32_t s_k = smem_u32(base), s_v = s_k + S::kTile, s_q = s_v + S::kTile;      // stages of q, grad
+    float *s_rows = reinterpret_cast<float *>(base + (2 + 2 * S::kStages) * S::kTile);    // stages of 128 x -lse, 128 x -delta
+    uint64_t *bar = reinterpret_cast<uint64_t *>(s_rows + S::kStages * 256);
+    uint64_t *full = bar, *empty = full + S::kStages, *kvfull = empty + S::kStages, *tail = kvfull + 1, *sfull = tail + 1;
+    uint64_t *dpfull = sfull + 1, *pready = dpfull + 1, *dsready = pready + 1, *finished = dsready + 1;
+    uint32_t *s_tmem = reinterpret_cast<uint32_t *>(finished + 1);
+    volatile int *s_abort = reinterpret_cast<volatile int *>(s_tmem + 1);
+    AtSample *s_sample = reinterpret_cast<AtSample *>(s_tmem + 2);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int P = 1 << log_p, tokens = kAtRows >> log_p;
+
+    at_check_offsets(a);
+    if (warp == kAbWarpLoad) {
+        const AtSample s = at_find(a.key_offsets, a.N, a, blockIdx.x, kAtRows);
+        if (lane == 0) *s_sample = s;
+    }
+    if (tid == 0) {
+        for (int i = 0; i < S::kStages; ++i) {
+            mbar_init(smem_u32(&full[i]), 2);                        // the copies' bytes, and the rows' numbers
+            mbar_init(smem_u32(&empty[i]), 1);
+        }
+        for (uint64_t *b : {kvfull, tail, sfull, dpfull, finished}) mbar_init(smem_u32(b), 1);
+        mbar_init(smem_u32(pready), 8);
+        mbar_init(smem_u32(dsready), 8);
+        *s_abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    }
+    __syncthreads();
+    const AtSample s = *s_sample;
+    const int n = s.q1 - s.q0, m = s.k1 - s.k0, key0 = s.tile * kAtRows;
+    if (s.tile < 0 || key0 >= m) return;
+    if (warp == kAbWarpMma) {
+        tmem_alloc(smem_u32(s_tmem), 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *s_tmem, t_dp = tmem + 128, t_dv = tmem + 256, t_dk = t_dv + DP;
+    const int kh = blockIdx.y, G = a.H / a.K;
+    // tiles of queries that see a key of this tile, of each block of P heads of the group
+    const int from = a.causal ? (int)max((int64_t)0, (int64_t)key0 - m + n) / tokens : 0;
+    const int per_head = max(0, (n + tokens - 1) / tokens - from);
+    int first, last;
+    at_split(a.splits, blockIdx.z, per_head * (G >> log_p), first, last);
+    const int tiles = last - first;
+    struct Walk {
+        int head, t;                                                 // the tile's first head, and its number
+    };
+    auto begin = [&] { return Walk{kh * G + (per_head ? first / per_head : 0) * P, from + (per_head ? first % per_head : 0)}; };
+    auto advance = [&](Walk &w) {
+        if (++w.t == from + per_head) {
+            w.t = from;
+            w.head += P;
+        }
+    };
+    auto rows_of = [&](const Walk &w) { return min(tokens, n - w.t * tokens) << log_p; };
+    auto wait = [&](uint64_t *b, uint32_t parity) { return mbar_wait_suspended(smem_u32(b), parity, s_abort, a.wait_ns); };
+    auto next = [](int &i, uint32_t &phase) {
+        if (++i == S::kStages) {
+            i = 0;
+            phase ^= 1u;
+        }
+    };
+
+    if (warp == kAbWarpLoad) {
+        // ------------------------------------------------------------------ loads: k, v; then q, grad and the rows' numbers
+        if (tiles > 0) {
+            auto load = [&](uint32_t dst, const CUtensorMap *map, int head, int row, uint32_t mbar) {
+                for (int c = 0; c < DP / 64; ++c) tma_load_3d(dst + c * kAtBlock, map, c * 64, head, row, mbar);
+            };
+            if (elect_one()) {
+                mbar_arrive_expect_tx(smem_u32(kvfull), 2 * S::kTile);
+                load(s_k, &map_k, kh, s.k0 + key0, smem_u32(kvfull));
+                load(s_v, &map_v, kh, s.k0 + key0, smem_u32(kvfull));
+            }
+            __syncwarp();
+            int st = 0;
+            uint32_t phase = 1, tail_phase = 0;
+            bool ok = true;
+            Walk w = begin();
+            for (int j = 0; j < tiles; ++j, advance(w), next(st, phase)) {
+                const int rows = rows_of(w);
+                const bool cut = rows & 15;
+                float lse[4], delta[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {                        // on their way while the stage is waited for
+                    const int r = lane + 32 * i;
+                    const int64_t at = (int64_t)(s.q0 + w.t * tokens + (r >> log_p)) * a.H + w.head + (r & (P - 1));
+                    lse[i] = r < rows ? kUp - __ldg(a.lse + at) : -INFINITY;
+                    delta[i] = r < rows ? -kDown * __ldg(a.delta + at) : 0.f;
+                }
+                if (!(ok = __all_sync(0xffffffffu, wait(&empty[st], phase)) != 0)) break;
+                const uint32_t dst = s_q + st * 2 * S::kTile, mbar = smem_u32(cut ? tail : &full[st]);
+                if (elect_one()) {
+                    mbar_arrive_expect_tx(mbar, 2 * S::kTile);
+                    load(dst, &map_q, w.head, s.q0 + w.t * tokens, mbar);
+                    load(dst + S::kTile, &map_g, w.head, s.q0 + w.t * tokens, mbar);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    s_rows[st * 256 + lane + 32 * i] = lse[i];
+                    s_rows[st * 256 + 128 + lane + 32 * i] = delta[i];
+                }
+                __syncwarp();
+                if (cut) {
+                    if (!(ok = __all_sync(0xffffffffu, wait(tail, tail_phase)) != 0)) break;
+                    tail_phase ^= 1u;
+                    at_zero_rows<DP>(dst, rows, (rows + 15) & ~15);
+                    at_zero_rows<DP>(dst + S::kTile, rows, (rows + 15) & ~15);
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_u32(&full[st]));
+                }
+                if (lane == 0) mbar_arrive(smem_u32(&full[st]));
+            }
+        }
+    } else if (warp == kAbWarpMma) {
+        // ------------------------------------------------------------------ products
+        if (tiles > 0 && elect_one()) {
+            const uint32_t id_s = instr_desc_f16(dtype_traits<T>::mma_format, 128, 128);
+            const uint32_t id_o = instr_desc_f16(dtype_traits<T>::mma_format, 128, (a.D + 15) & ~15) | 1u << 16;
+            const int steps = (a.D + 15) >> 4;
+            int st = 0;
+            uint32_t phase = 0, t_phase = 0;
+            bool ok = wait(kvfull, 0) && wait(&full[0], 0);
+            if (ok) {
+                tc_fence_after();
+                at_mma_head<DP>(tmem, s_k, s_q, id_s, steps);
+                tc_commit(smem_u32(sfull));
+                at_mma_head<DP>(t_dp, s_v, s_q + S::kTile, id_s, steps);
+                tc_commit(smem_u32(dpfull));
+            }
+            Walk w = begin();
+            for (int j = 0; j < tiles && ok; ++j, t_phase ^= 1u, advance(w)) {
+                const int here = st, sum_steps = (rows_of(w) + 15) >> 4;
+                const uint32_t s_here = s_q + here * 2 * S::kTile;
+                const bool more = j + 1 < tiles;
+                next(st, phase);
+                const uint32_t s_next = s_q + st * 2 * S::kTile;
+                if (!(ok = wait(pready, t_phase))) break;
+                tc_fence_after();
+                at_mma_rows(t_dv, tmem, 32, s_here + S::kTile, id_o, sum_steps, j > 0);
+                if (more) {
+                    if (!(ok = wait(&full[st], phase))) break;
+                    tc_fence_after();
+                    at_mma_head<DP>(tmem, s_k, s_next, id_s, steps);
+                    tc_commit(smem_u32(sfull));
+                }
+                if (!(ok = wait(dsready, t_phase))) break;
+                tc_fence_after();
+                at_mma_rows(t_dk, t_dp, 32, s_here, id_o, sum_steps, j > 0);
+                tc_commit(smem_u32(more ? &empty[here] : finished));
+                if (more) {
+                    at_mma_head<DP>(t_dp, s_v, s_next + S::kTile, id_s, steps);
+                    tc_commit(smem_u32(dpfull));
+                }
+            }
+        }
+    } else {
+        // ------------------------------------------------------------------ a thread a key and 64 query rows
+        const int half = warp >> 2, row = tid & 127, key = key0 + row;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const bool mine = key < m;
+        const f32x2 c2 = pack_f32x2(a.c, a.c), k2 = pack_f32x2(kDown, kDown);
+        bool ok = true;
+        int st = 0;
+        uint32_t phase = 0, t_phase = 0;
+        Walk w = begin();
+        for (int j = 0; j < tiles; ++j, t_phase ^= 1u, next(st, phase), advance(w)) {
+            const uint32_t t_s = tmem + half * 64 + lanes, t_d = t_dp + half * 64 + lanes;
+            const uint32_t s_lse = smem_u32(s_rows + st * 256 + half * 64), s_delta = s_lse + 512;
+            // columns from `see` on see this key; from `use` on with a gradient of their score
+            int see = 0, use = 0;
+            bool masked = m == 1;
+            if (a.causal) {
+                const int64_t before = (int64_t)n - m - (int64_t)w.t * tokens;   // the query that sees key 0 last, in the tile
+                masked |= before + key0 + kAtRows - 1 > 0;
+                const int64_t at = max((int64_t)-kAtRows, min((int64_t)kAtRows, before + key)) * P - half * 64;
+                see = (int)at;
+                use = see + (key == 0 ? P : 0);
+            }
+            if (m == 1) use = kAtRows;
+            if (!(ok = __all_sync(0xffffffffu, wait(&full[st], phase) && wait(sfull, t_phase)) != 0)) break;
+            tc_fence_after();
+            f32x2 x[32];
+            uint32_t u[32];
+            ab_load64(t_s, x);
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+                f32x2 l0, l1;
+                asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];\n" : "=l"(l0.v), "=l"(l1.v) : "r"(s_lse + i * 8));
+                const float2 f0 = unpack_f32x2(fma2(x[i], c2, l0)), f1 = unpack_f32x2(fma2(x[i + 1], c2, l1));
+                x[i] = pack_f32x2(ex2_approx(f0.x), ex2_approx(f0.y));
+                x[i + 1] = pack_f32x2(ex2_approx(f1.x), ex2_approx(f1.y));
+            }
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+                const float2 f = unpack_f32x2(x[i]);
+                u[i] = lt_pack<T>(f.x, f.y);
+            }
+            if (masked) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) u[i] &= (2 * i >= see ? 0xffffu : 0u) | (2 * i + 1 >= see ? 0xffff0000u : 0u);
+            }
+            tmem_st32(t_s, u);
+            tc_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(pready));
+            if (!(ok = __all_sync(0xffffffffu, wait(dpfull, t_phase)) != 0)) break;
+            tc_fence_after();
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                f32x2 y[16];
+                lt_load32(t_d + g * 32, y);
+#pragma unroll
+                for (int i = 0; i < 16; i += 2) {
+                    f32x2 d0, d1;
+                    asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];\n" : "=l"(d0.v), "=l"(d1.v) : "r"(s_delta + (g * 16 + i) * 8));
+                    const float2 f0 = unpack_f32x2(mul2(x[g * 16 + i], fma2(y[i], k2, d0)));
+                    const float2 f1 = unpack_f32x2(mul2(x[g * 16 + i + 1], fma2(y[i + 1], k2, d1)));
+                    u[g * 16 + i] = lt_pack<T>(f0.x, f0.y);
+                    u[g * 16 + i + 1] = lt_pack<T>(f1.x, f1.y);
+                }
+            }
+            if (masked) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) u[i] &= (2 * i >= use ? 0xffffu : 0u) | (2 * i + 1 >= use ? 0xffff0000u : 0u);
+            }
+            tmem_st32(t_d, u);
+            tc_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(dsready));
+        }
+        if (tiles > 0 && ok) ok = __all_sync(0xffffffffu, wait(finished, 0)) != 0;
+        tc_fence_after();
+        if (ok) {                                                    // half 0 stores grad_value, half 1 grad_key
+            const int64_t all = (int64_t)a.N * a.K, at = (int64_t)(s.k0 + key) * a.K + kh;
+            float *part = a.splits > 1 ? a.partial + ((2 * blockIdx.z + 1 - half) * all + at) * a.D : nullptr;
+            T *out = (T *)(half ? a.gk : a.gv);
+            ab_store_row<T>((half ? t_dk : t_dv) + lanes, 0, DP, a.D, tiles == 0, half ? a.scale : kDown, mine && (out || part),
+                            out ? out + at * a.D : nullptr, part);
+        }
+    }
+
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();                                                 // every role has set the flag by now if it gives up
+    if (*s_abort) {                                                  // copies and products in flight end within this
+        if (tid == 0) raise_status(a.status, SPCONV_STATUS_WAIT_TIMEOUT);
+        const uint64_t begin_ns = globaltimer_ns();
+        while (globaltimer_ns() - begin_ns < kTmaDrainNs) {}
+        __syncthreads();
+    }
+    tc_fence_after();
+    if (warp == kAbWarpMma) tmem_dealloc(tmem, 512);
+}
+
+template <typename T, int DP, bool KEYS>
+static int ab_run(const AtArgs &a) {
+    const int G = a.H / a.K;
+    int log_p = 0;
+    while (log_p < 7 && G % (2 << log_p) == 0) ++log_p;
+    const int P = 1 << log_p, tokens = kAtRows >> log_p;
+    CUtensorMap mq, mk, mv, mg;
+    if (!at_map(&mq, a.q, a.M, a.H, a.D, P, tokens) || !at_map(&mk, a.k, a.N, a.K, a.D, 1, kAtRows) ||
+        !at_map(&mv, a.v, a.N, a.K, a.D, 1, kAtRows) || !at_map(&mg, a.grad, a.M, a.H, a.D, P, tokens))
+        return SPCONV_ERR_CUDA;
+    static std::atomic<uint64_t> done;
+    auto kern = KEYS ? attention_tc_grad_key_kernel<T, DP> : attention_tc_grad_query_kernel<T, DP>;
+    constexpr int smem = KEYS ? AkShape<DP>::kSmem : AqShape<DP>::kSmem;
+    if (allow_smem(kern, smem, done) != cudaSuccess) return check_launch("attention: shared memory");
+    const dim3 grid(KEYS ? (unsigned)at_tiles(a.N, a.B, kAtRows) : (unsigned)at_tiles(a.M, a.B, tokens), KEYS ? a.K : a.H / P, a.splits);
+    kern<<<grid, kAbThreads, smem, a.stream>>>(mq, mk, mv, mg, a, log_p);
+    return check_launch(KEYS ? "attention_tc_grad_key_kernel" : "attention_tc_grad_query_kernel");
+}
+
+template <typename T, bool KEYS>
+static int ab_size(const AtArgs &a) {
+    return a.D <= 64 ? ab_run<T, 64, KEYS>(a) : ab_run<T, 128, KEYS>(a);
+}
+
+int launch_at_tc_grad_query(const AtArgs &a) {
+    return a.dtype == SPCONV_F16 ? ab_size<__half, false>(a) : ab_size<__nv_bfloat16, false>(a);
+}
+int launch_at_tc_grad_key(const AtArgs &a) {
+    return a.dtype == SPCONV_F16 ? ab_size<__half, true>(a) : ab_size<__nv_bfloat16, true>(a);
+}
+
+}  // namespace spconv

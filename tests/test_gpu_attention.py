@@ -121,6 +121,15 @@ def test_many_short_samples(dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("causal", [False, True])
+def test_long_samples(dtype, D, causal):
+    """Enough rows for two tiles of 128 queries a block, the last one with one tile or a part of it."""
+    run([1500, 0, 1100, 1291], [1500, 0, 1100, 1291], 24, 12, D, dtype, causal=causal)
+    run([1025, 1153], [700, 2000], 24, 24, D, dtype, causal=causal)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_few_queries_many_keys(dtype):
     """Keys in splits, joined."""
     run([1, 2, 1], [5000, 17, 9001], 8, 1, 64, dtype)
