@@ -53,36 +53,53 @@ attention_delta_kernel(const __grid_constant__ AtArgs a) {
     if (in && lane == 0) a.delta[rh] = s;
 }
 
-// A row's splits: out = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s, a warp each.
+// A row's splits: out = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s. `share` warps take a row's splits in turn and add up in
+// order: all eight of a block where rows are few (eight rows of 74 splits: 75 us by a warp each), one where they are many.
 template <typename T>
 __global__ void __launch_bounds__(kAtThreads)
-attention_join_kernel(const __grid_constant__ AtArgs a) {
-    const int64_t all = (int64_t)a.M * a.H, rh = ((int64_t)blockIdx.x * kAtThreads + threadIdx.x) >> 5;
-    const int lane = threadIdx.x & 31;
-    if (rh >= all) return;
-    float m = -INFINITY;
-    bool nan = false;
-    for (int s = lane; s < a.splits; s += 32) {
-        const float x = a.part_ml[s * all + rh].x;
-        m = fmaxf(m, x);
-        nan |= isnan(x);
-    }
+attention_join_kernel(const __grid_constant__ AtArgs a, const int share) {
+    __shared__ float parts[kAtThreads / 32][256], sums[kAtThreads / 32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, w = warp % share;
+    const int64_t all = (int64_t)a.M * a.H, rh = (int64_t)blockIdx.x * (kAtThreads / 32 / share) + warp / share;
+    const bool in = rh < all;
+    float m = -INFINITY, acc[8] = {}, sum = 0.f;
+    bool nan = false, some = false;
+    if (in) {
+        for (int s = lane; s < a.splits; s += 32) {
+            const float2 ml = a.part_ml[s * all + rh];
+            m = fmaxf(m, ml.x);
+            nan |= isnan(ml.x);
+            some |= !(ml.x == -INFINITY && ml.y == 0.f);        // else it saw no key, and nothing may be written there
+        }
 #pragma unroll
-    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if (__any_sync(0xffffffffu, nan)) m = NAN;
-    float acc[8] = {}, sum = 0.f;
-    bool some = false;
-    for (int s = 0; s < a.splits; ++s) {
-        const float2 ml = a.part_ml[s * all + rh];
-        if (ml.x == -INFINITY && ml.y == 0.f) continue;         // saw no key: there may be nothing written
-        some = true;
-        const float w = exp2f(ml.x - m);
-        sum = fmaf(w, ml.y, sum);
-        const float *p = a.partial + (s * all + rh) * a.D;
+        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        if (__any_sync(0xffffffffu, nan)) m = NAN;
+        some = __any_sync(0xffffffffu, some);
+#pragma unroll 4
+        for (int s = w; s < a.splits; s += share) {
+            const float2 ml = a.part_ml[s * all + rh];
+            const bool there = !(ml.x == -INFINITY && ml.y == 0.f);
+            const float weight = there ? exp2f(ml.x - m) : 0.f;
+            const float *p = a.partial + (s * all + rh) * a.D;
+            sum = fmaf(weight, ml.y, sum);
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (lane + 32 * j < a.D) acc[j] = fmaf(w, p[lane + 32 * j], acc[j]);
+            for (int j = 0; j < 8; ++j)
+                if (lane + 32 * j < a.D) acc[j] = fmaf(weight, there ? p[lane + 32 * j] : 0.f, acc[j]);
+        }
     }
+    if (share > 1) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) parts[warp][lane + 32 * j] = acc[j];
+        if (lane == 0) sums[warp] = sum;
+        __syncthreads();
+        if (w != 0) return;
+        for (int k = 1; k < share; ++k) {
+            sum += sums[warp + k];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) acc[j] += parts[warp + k][lane + 32 * j];
+        }
+    }
+    if (!in) return;
     const float inv = some ? 1.f / sum : 0.f;
 #pragma unroll
     for (int j = 0; j < 8; ++j)
@@ -97,6 +114,7 @@ attention_sum_kernel(const float *partial, int64_t stride, int splits, T *out, i
     const int64_t i = (int64_t)blockIdx.x * kAtThreads + threadIdx.x;
     if (i >= n) return;
     float s = 0.f;
+#pragma unroll 8
     for (int k = 0; k < splits; ++k) s += partial[k * stride + i];
     out[i] = dtype_traits<T>::from_f(s);
 }
@@ -119,7 +137,7 @@ static bool at_tma(const AtTensor &t, int64_t rows, int heads, int D) {
 // Where things lie in the workspace, and how the work is cut.
 struct AtPlan {
     bool tc;
-    int tiles2;                          // forward: two tiles a CTA
+    bool pair;                           // forward: two tiles a CTA
     int splits[3];                       // forward (or queries' gradients), and keys' gradients
     bool pack[4];                        // q, k, v, grad
     int64_t pack_at[4], delta_at, ml_at, partial_at, bytes;
@@ -141,9 +159,11 @@ static AtPlan at_plan(const spconv_attention_args *q, bool backward) {
     auto up = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
     if (p.tc) {
         const int64_t rows = mean_q * P, heads = q->heads / P;
-        p.tiles2 = !backward && rows > 192 && mean_k > 512 && B * up(rows, 256) * heads >= 148;
-        p.splits[0] = at_cut(B * up(rows, 128) * heads, 148 * (backward ? 1 : 2), up(mean_k, 128), 2);
-        p.splits[1] = at_cut(B * up(mean_k, 128) * q->key_heads, 148, up(rows, 128) * (G / P), 2);
+        p.pair = !backward && q->head_size > 64 && rows > 192 && mean_k > 512 && B * up(rows, 256) * heads >= 148;
+        // CTAs that run at a time, and what each has to have for itself: 512 keys (a split's rows are written and read once more)
+        const int64_t per_sm = q->head_size > 64 ? 1 : 2;
+        p.splits[0] = at_cut(B * up(rows, 128) * heads, 148 * (backward ? per_sm : 2 * per_sm), up(mean_k, 128), 8);
+        p.splits[1] = at_cut(B * up(mean_k, 128) * q->key_heads, 148 * per_sm, up(rows, 128) * (G / P), 8);
     } else {
         const int64_t R = at_simt_rows(q->head_size);
         p.splits[0] = at_cut(B * up(mean_q, R) * q->heads, 296, up(mean_k, R), 2);
@@ -267,11 +287,12 @@ extern "C" int spconv_attention_forward(const spconv_attention_args *q, void *st
     AtArgs a;
     if (const int rc = at_prepare(q, p, false, (cudaStream_t)stream, a)) return rc;
     a.splits = p.splits[0];
-    if (const int rc = p.tc ? launch_at_tc_forward(a, p.tiles2) : launch_at_simt_forward(a)) return rc;
+    if (const int rc = p.tc ? launch_at_tc_forward(a, p.pair) : launch_at_simt_forward(a)) return rc;
     if (a.splits == 1) return SPCONV_OK;
     return at_by_type(a.dtype, [&](auto *t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        attention_join_kernel<T><<<at_blocks((int64_t)a.M * a.H * 32), kAtThreads, 0, a.stream>>>(a);
+        const int share = (int64_t)a.M * a.H <= 4096 ? kAtThreads / 32 : 1;
+        attention_join_kernel<T><<<at_blocks((int64_t)a.M * a.H * share * 32), kAtThreads, 0, a.stream>>>(a, share);
         return check_launch("attention_join_kernel");
     });
 }

@@ -30,18 +30,7 @@ __device__ __forceinline__ void tc_mma_f16_ta(uint32_t tmem_d, uint32_t tmem_a, 
         "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n"
         :: "r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
 }
-// 32 consecutive columns of the lane's row; tc_wait_st before others rely on it.
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {"
-        "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};\n"
-        :: "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-           "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
-           "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
-           "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
-        : "memory");
-}
+// 16 consecutive columns of the lane's row; tc_wait_st before others rely on it.
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *r) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {"
@@ -54,13 +43,73 @@ __device__ __forceinline__ void tc_wait_st() {
     asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
 }
 
-// A tile in shared memory: DP / 64 blocks of 128 rows x 64 values. As an operand along the head (K-major) ...
+// 2 N columns of the lane's row, all loads in flight before the first is waited for.
+template <int N>
+__device__ __forceinline__ void at_load(uint32_t taddr, f32x2 (&x)[N]) {
+    uint32_t r[2 * N];
+#pragma unroll
+    for (int g = 0; g < N / 16; ++g) {
+        uint32_t *q = r + 32 * g;
+        asm volatile(
+            "tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
+            "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+            "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
+            : "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3]), "=r"(q[4]), "=r"(q[5]), "=r"(q[6]), "=r"(q[7]),
+              "=r"(q[8]), "=r"(q[9]), "=r"(q[10]), "=r"(q[11]), "=r"(q[12]), "=r"(q[13]), "=r"(q[14]), "=r"(q[15]),
+              "=r"(q[16]), "=r"(q[17]), "=r"(q[18]), "=r"(q[19]), "=r"(q[20]), "=r"(q[21]), "=r"(q[22]), "=r"(q[23]),
+              "=r"(q[24]), "=r"(q[25]), "=r"(q[26]), "=r"(q[27]), "=r"(q[28]), "=r"(q[29]), "=r"(q[30]), "=r"(q[31])
+            : "r"(taddr + 32 * g) : "memory");
+    }
+    tc_wait_ld();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {                   // nothing that uses them moves before the wait
+        asm volatile("mov.b64 %0, {%1, %2};" : "=l"(x[i].v) : "r"(r[2 * i]), "r"(r[2 * i + 1]));
+    }
+}
+
+// 2^x of two values on the FMA pipe: x = n + f, |f| <= 1/2, 2^f by a polynomial (degree 4, exact at 0, the smallest
+// largest relative error on the interval: 2.9e-6, under a rounding of either 16-bit type) and 2^n from n's bits. Exactly
+// 0 from -127 on; NaN stays NaN. The special-function unit gives 16 exponentials a clock and SM, a quarter of
+// what the FMA pipe gives products, and is what a tile waits for: a share of the columns goes here.
+__device__ __forceinline__ f32x2 at_exp2_fma(f32x2 x) {
+    const float2 u = unpack_f32x2(x);
+    float a, b;
+    asm("max.NaN.f32 %0, %1, 0fC2FE0000;" : "=f"(a) : "f"(u.x));
+    asm("max.NaN.f32 %0, %1, 0fC2FE0000;" : "=f"(b) : "f"(u.y));
+    x = pack_f32x2(a, b);
+    const f32x2 magic = pack_f32x2(12582912.f, 12582912.f), unmagic = pack_f32x2(-12582912.f, -12582912.f);
+    const f32x2 t = add2(x, magic);
+    const f32x2 n = add2(t, unmagic), one = pack_f32x2(1.f, 1.f);
+    const f32x2 f = fma2(n, pack_f32x2(-1.f, -1.f), x);
+    f32x2 p = fma2(f, pack_f32x2(0.00958285294f, 0.00958285294f), pack_f32x2(0.0559064262f, 0.0559064262f));
+    p = fma2(p, f, pack_f32x2(0.240240991f, 0.240240991f));
+    p = fma2(p, f, pack_f32x2(0.693124175f, 0.693124175f));
+    p = fma2(p, f, one);
+    const float2 tt = unpack_f32x2(t);
+    return mul2(p, pack_f32x2(__int_as_float((__float_as_int(tt.x) << 23) + 0x3f800000),
+                              __int_as_float((__float_as_int(tt.y) << 23) + 0x3f800000)));
+}
+// 2^x of two values.
+__device__ __forceinline__ f32x2 at_exp2(f32x2 x) {
+    const float2 f = unpack_f32x2(x);
+    return pack_f32x2(ex2_approx(f.x), ex2_approx(f.y));
+}
+template <int EMU>
+__device__ __forceinline__ f32x2 at_exp2_mix(f32x2 x, int i) { return i * EMU % 8 < EMU ? at_exp2_fma(x) : at_exp2(x); }
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+// A tile in shared memory: DP / 64 blocks of ROWS rows x 64 values. As an operand along the head (K-major) ...
 __device__ __forceinline__ uint64_t at_desc_k(uint32_t saddr) { return smem_desc_kmajor_swizzled(saddr, 128); }
 // ... and along the rows (MN-major): a step of 16 rows is 2048 bytes on.
-__device__ __forceinline__ uint64_t at_desc_mn(uint32_t saddr) { return smem_desc_mn_sw128(saddr, kAtBlock, 1024); }
+template <int ROWS>
+__device__ __forceinline__ uint64_t at_desc_mn(uint32_t saddr) { return smem_desc_mn_sw128(saddr, ROWS * 128, 1024); }
 
-// D = A B^T over the head, A and B tiles of 128 rows.
-template <int DP>
+// D = A B^T over the head: A a tile of 128 rows, B one of ROWS.
+template <int DP, int ROWS>
 __device__ __forceinline__ void at_mma_head(uint32_t d, uint32_t sa, uint32_t sb, uint32_t idesc, int steps) {
     uint64_t ad = at_desc_k(sa), bd = at_desc_k(sb);
 #pragma unroll
@@ -68,31 +117,34 @@ __device__ __forceinline__ void at_mma_head(uint32_t d, uint32_t sa, uint32_t sb
         if (kk >= steps) break;
         if (kk == 4) {                               // the second block of 64 values
             ad = at_desc_k(sa + kAtBlock);
-            bd = at_desc_k(sb + kAtBlock);
+            bd = at_desc_k(sb + ROWS * 128);
         }
         tc_mma_f16(d, ad, bd, idesc, kk > 0);
         ad += 2;
         bd += 2;
     }
 }
-// D (+)= A B over the rows: A 128 x 128 in TMEM (the second half of its columns `skip` columns further on), B a tile.
-__device__ __forceinline__ void at_mma_rows(uint32_t d, uint32_t ta, int skip, uint32_t sb, uint32_t idesc, int steps, bool accumulate) {
-    uint64_t bd = at_desc_mn(sb);
+// D (+)= A B over B's ROWS rows: A 128 x ROWS in TMEM, in parts of PART columns' values (16 bits each) that begin PART
+// TMEM columns apart, where the fp32 values were that they are made of.
+template <int PART, int ROWS>
+__device__ __forceinline__ void at_mma_rows(uint32_t d, uint32_t ta, uint32_t sb, uint32_t idesc, int steps, bool accumulate) {
+    constexpr int kSteps = PART / 16;
+    uint64_t bd = at_desc_mn<ROWS>(sb);
 #pragma unroll
-    for (int kk = 0; kk < 8; ++kk, bd += 128) {
+    for (int kk = 0; kk < ROWS / 16; ++kk, bd += 128) {
         if (kk >= steps) break;
-        tc_mma_f16_ta(d, ta + kk * 8 + (kk >= 4 ? skip : 0), bd, idesc, accumulate || kk > 0);
+        tc_mma_f16_ta(d, ta + kk / kSteps * PART + kk % kSteps * 8, bd, idesc, accumulate || kk > 0);
     }
 }
 
-// Zeros rows [from, to) of a tile: by a converged warp.
-template <int DP>
+// Zeros rows [from, to) of a tile of ROWS: by a converged warp.
+template <int DP, int ROWS>
 __device__ __forceinline__ void at_zero_rows(uint32_t saddr, int from, int to) {
     const int lane = threadIdx.x & 31;
     for (int i = lane; i < (to - from) * 8 * (DP / 64); i += 32) {
         const int block = i / ((to - from) * 8), j = i - block * (to - from) * 8;
         asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};\n"
-                     :: "r"(saddr + block * kAtBlock + from * 128 + j * 16), "r"(0) : "memory");
+                     :: "r"(saddr + block * ROWS * 128 + from * 128 + j * 16), "r"(0) : "memory");
     }
 }
 

@@ -8,7 +8,7 @@
 // a tile where one sweep with atomic sums of grad_query would have five, but every sum has one owner and one order: the
 // same bits every run, no fp32 copy of a gradient in memory.
 //
-// A CTA an SM: eight warps compute, a thread a row and half of the 128 columns; one loads (TMA), one issues the
+// A CTA an SM: sixteen warps compute, a thread a row and a quarter of the 128 columns; one loads (TMA), one issues the
 // products. ds (and p) go back to TMEM in 16 bits, over s and dp, and are the A operand of the second products
 // from there; B is the tile that s or dp was made of, read along its rows (MN-major). While the threads work on one
 // of s and dp, the products that make the other run.
@@ -22,14 +22,20 @@
 
 namespace spconv {
 
-constexpr int kAbThreads = 320;
-constexpr int kAbWarpLoad = 8, kAbWarpMma = 9;
-
-// The lane's 64 columns of a half tile.
-__device__ __forceinline__ void ab_load64(uint32_t taddr, f32x2 (&x)[32]) {
-    lt_load32(taddr, *reinterpret_cast<f32x2(*)[16]>(x));
-    lt_load32(taddr + 32, *reinterpret_cast<f32x2(*)[16]>(x + 16));
-}
+// W columns (of the side that is walked) a tile: four warps compute 32 of them.
+template <int DP, int W>
+struct AbShape {
+    static constexpr int kWarps = W / 8, kThreads = kWarps * 32 + 64;
+    static constexpr int kWarpLoad = kWarps, kWarpMma = kWarps + 1;
+    static constexpr int kPerSm = DP == 64 && W == 64 ? 2 : 1, kColumns = 512 / kPerSm;
+    static constexpr int kOwn = DP / 64 * kAtBlock, kTile = DP / 64 * W * 128;      // bytes of an own tile, and of a walked one
+};
+#ifndef AB_EMUQ
+#define AB_EMUQ 0
+#endif
+#ifndef AB_EMUK
+#define AB_EMUK 0
+#endif
 
 // A row of accumulators [from, to) times `factor`, to a row of D values: rounded, or fp32 where `part` is given.
 template <typename T>
@@ -68,23 +74,22 @@ __device__ __forceinline__ void ab_store_row(uint32_t taddr, int from, int to, i
     }
 }
 
-template <int DP>
-struct AqShape {
-    static constexpr int kTile = DP / 64 * kAtBlock;
-    static constexpr int kK = DP == 64 ? 4 : 3, kV = DP == 64 ? 4 : 2;          // stages
-    static constexpr int kSmem = 1024 + (2 + kK + kV) * kTile + 512;
+template <int DP, int W>
+struct AqShape : AbShape<DP, W> {
+    static constexpr int kK = DP == 64 ? 4 : 3, kV = DP == 64 ? 4 : 2;              // stages
+    static constexpr int kSmem = 1024 + 2 * AbShape<DP, W>::kOwn + (kK + kV) * AbShape<DP, W>::kTile + 512;
 };
 
-template <typename T, int DP>
-__global__ void __launch_bounds__(kAbThreads, 1)
+template <typename T, int DP, int W>
+__global__ void __launch_bounds__(AbShape<DP, W>::kThreads, AbShape<DP, W>::kPerSm)
 attention_tc_grad_query_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                                const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_g,
                                const __grid_constant__ AtArgs a, const int log_p) {
-    using S = AqShape<DP>;
+    using S = AqShape<DP, W>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *base = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    const uint32_t s_q = smem_u32(base), s_g = s_q + S::kTile, s_k = s_g + S::kTile, s_v = s_k + S::kK * S::kTile;
-    uint64_t *bar = reinterpret_cast<uint64_t *>(base + (2 + S::kK + S::kV) * S::kTile);
+    const uint32_t s_q = smem_u32(base), s_g = s_q + S::kOwn, s_k = s_g + S::kOwn, s_v = s_k + S::kK * S::kTile;
+    uint64_t *bar = reinterpret_cast<uint64_t *>(base + 2 * S::kOwn + (S::kK + S::kV) * S::kTile);
     uint64_t *kfull = bar, *kempty = kfull + S::kK, *vfull = kempty + S::kK, *vempty = vfull + S::kV;
     uint64_t *qfull = vempty + S::kV, *tail = qfull + 1, *sfull = tail + 1, *dpfull = sfull + 2, *dsready = dpfull + 1, *finished = dsready + 1;
     uint32_t *s_tmem = reinterpret_cast<uint32_t *>(finished + 1);
@@ -94,7 +99,7 @@ attention_tc_grad_query_kernel(const __grid_constant__ CUtensorMap map_q, const 
     const int P = 1 << log_p, tokens = kAtRows >> log_p;
 
     at_check_offsets(a);
-    if (warp == kAbWarpLoad) {
+    if (warp == S::kWarpLoad) {
         const AtSample s = at_find(a.offsets, a.M, a, a.causal ? gridDim.x - 1 - blockIdx.x : blockIdx.x, tokens);
         if (lane == 0) *s_sample = s;
     }
@@ -108,7 +113,7 @@ attention_tc_grad_query_kernel(const __grid_constant__ CUtensorMap map_q, const 
             mbar_init(smem_u32(&vempty[i]), 1);
         }
         for (uint64_t *b : {qfull, tail, sfull, sfull + 1, dpfull, finished}) mbar_init(smem_u32(b), 1);
-        mbar_init(smem_u32(dsready), 8);
+        mbar_init(smem_u32(dsready), S::kWarps);
         *s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
@@ -116,20 +121,20 @@ attention_tc_grad_query_kernel(const __grid_constant__ CUtensorMap map_q, const 
     const AtSample s = *s_sample;
     const int n = s.q1 - s.q0, m = s.k1 - s.k0, t0 = s.tile * tokens;
     if (s.tile < 0 || t0 >= n) return;
-    if (warp == kAbWarpMma) {
-        tmem_alloc(smem_u32(s_tmem), 512);
+    if (warp == S::kWarpMma) {
+        tmem_alloc(smem_u32(s_tmem), S::kColumns);
         tmem_relinquish();
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *s_tmem, t_dp = tmem + 256, t_dq = tmem + 384;
+    const uint32_t tmem = *s_tmem, t_dp = tmem + 2 * W, t_dq = tmem + 3 * W;
     const int head0 = blockIdx.y << log_p, kh = head0 / (a.H / a.K);
     const int seen_last = at_seen(a, min(n, t0 + tokens) - 1, n, m);
     int first, last;
-    at_split(a.splits, blockIdx.z, (seen_last + kAtRows - 1) / kAtRows, first, last);
+    at_split(a.splits, blockIdx.z, (seen_last + W - 1) / W, first, last);
     const int tiles = last - first;
-    const int end_valid = min(kAtRows, seen_last - (last - 1) * kAtRows);
+    const int end_valid = min(W, seen_last - (last - 1) * W);
     auto wait = [&](uint64_t *b, uint32_t parity) { return mbar_wait_suspended(smem_u32(b), parity, s_abort, a.wait_ns); };
     auto next = [](int &i, uint32_t &phase, int stages) {
         if (++i == stages) {
@@ -138,16 +143,16 @@ attention_tc_grad_query_kernel(const __grid_constant__ CUtensorMap map_q, const 
         }
     };
 
-    if (warp == kAbWarpLoad) {
+    if (warp == S::kWarpLoad) {
         // ------------------------------------------------------------------ loads: q, grad; then k, v of each tile in turn
         if (tiles > 0) {
-            auto load = [&](uint32_t dst, const CUtensorMap *map, int head, int row, uint32_t mbar) {
-                for (int c = 0; c < DP / 64; ++c) tma_load_3d(dst + c * kAtBlock, map, c * 64, head, row, mbar);
+            auto load = [&](uint32_t dst, int rows, const CUtensorMap *map, int head, int row, uint32_t mbar) {
+                for (int c = 0; c < DP / 64; ++c) tma_load_3d(dst + c * rows * 128, map, c * 64, head, row, mbar);
             };
             if (elect_one()) {
-                mbar_arrive_expect_tx(smem_u32(qfull), 2 * S::kTile);
-                load(s_q, &map_q, head0, s.q0 + t0, smem_u32(qfull));
-                load(s_g, &map_g, head0, s.q0 + t0, smem_u32(qfull));
+                mbar_arrive_expect_tx(smem_u32(qfull), 2 * S::kOwn);
+                load(s_q, kAtRows, &map_q, head0, s.q0 + t0, smem_u32(qfull));
+                load(s_g, kAtRows, &map_g, head0, s.q0 + t0, smem_u32(qfull));
             }
             __syncwarp();
             int ks = 0, vs = 0;
@@ -155,23 +160,23 @@ attention_tc_grad_query_kernel(const __grid_constant__ CUtensorMap map_q, const 
             bool ok = true;
             for (int j = 0; j < tiles && ok; ++j) {
                 const bool cut = j + 1 == tiles && (end_valid & 15);
-                const int row = s.k0 + (first + j) * kAtRows;
+                const int row = s.k0 + (first + j) * W;
                 if (!(ok = __all_sync(0xffffffffu, wait(&kempty[ks], kp)) != 0)) break;
                 const uint32_t dst = s_k + ks * S::kTile, mbar = smem_u32(cut ? tail : &kfull[ks]);
                 if (elect_one()) {
                     mbar_arrive_expect_tx(mbar, S::kTile);
-                    load(dst, &map_k, kh, row, mbar);
+                    load(dst, W, &map_k, kh, row, mbar);
                 }
                 __syncwarp();
                 if (!(ok = __all_sync(0xffffffffu, wait(&vempty[vs], vp)) != 0)) break;
                 if (elect_one()) {
                     mbar_arrive_expect_tx(smem_u32(&vfull[vs]), S::kTile);
-                    load(s_v + vs * S::kTile, &map_v, kh, row, smem_u32(&vfull[vs]));
+                    load(s_v + vs * S::kTile, W, &map_v, kh, row, smem_u32(&vfull[vs]));
                 }
                 __syncwarp();
                 if (cut) {
                     ok = __all_sync(0xffffffffu, wait(tail, 0)) != 0;
-                    at_zero_rows<DP>(dst, end_valid, (end_valid + 15) & ~15);
+                    at_zero_rows<DP, W>(dst, end_valid, (end_valid + 15) & ~15);
                     fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(smem_u32(&kfull[ks]));
@@ -180,10 +185,10 @@ attention_tc_grad_query_kernel(const __grid_constant__ CUtensorMap map_q, const 
                 next(vs, vp, S::kV);
             }
         }
-    } else if (warp == kAbWarpMma) {
+    } else if (warp == S::kWarpMma) {
         // ------------------------------------------------------------------ products
         if (tiles > 0 && elect_one()) {
-            const uint32_t id_s = instr_desc_f16(dtype_traits<T>::mma_format, 128, 128);
+            const uint32_t id_s = instr_desc_f16(dtype_traits<T>::mma_format, 128, W);
             const uint32_t id_o = instr_desc_f16(dtype_traits<T>::mma_format, 128, (a.D + 15) & ~15) | 1u << 16;
             const int steps = (a.D + 15) >> 4;
             int ks = 0, vs = 0, done = 0;                            // next k and v stage; the k stage of ds k
@@ -192,14 +197,14 @@ attention_tc_grad_query_kernel(const __grid_constant__ CUtensorMap map_q, const 
             auto scores = [&](int j) {                               // s of tile j
                 if (!(ok = ok && wait(&kfull[ks], kp))) return;
                 tc_fence_after();
-                at_mma_head<DP>(tmem + (j & 1) * 128, s_q, s_k + ks * S::kTile, id_s, steps);
+                at_mma_head<DP, W>(tmem + (j & 1) * W, s_q, s_k + ks * S::kTile, id_s, steps);
                 tc_commit(smem_u32(&sfull[j & 1]));
                 next(ks, kp, S::kK);
             };
             auto products = [&] {                                    // dp of the next tile
                 if (!(ok = ok && wait(&vfull[vs], vp))) return;
                 tc_fence_after();
-                at_mma_head<DP>(t_dp, s_g, s_v + vs * S::kTile, id_s, steps);
+                at_mma_head<DP, W>(t_dp, s_g, s_v + vs * S::kTile, id_s, steps);
                 tc_commit(smem_u32(dpfull));
                 tc_commit(smem_u32(&vempty[vs]));
                 next(vs, vp, S::kV);
@@ -210,7 +215,7 @@ attention_tc_grad_query_kernel(const __grid_constant__ CUtensorMap map_q, const 
             for (int j = 0; j < tiles && ok; ++j, ds_phase ^= 1u) {
                 if (!(ok = wait(dsready, ds_phase))) break;
                 tc_fence_after();
-                at_mma_rows(t_dq, tmem + (j & 1) * 128, 32, s_k + done * S::kTile, id_o, j + 1 < tiles ? 8 : (end_valid + 15) >> 4, j > 0);
+                at_mma_rows<32, W>(t_dq, tmem + (j & 1) * W, s_k + done * S::kTile, id_o, j + 1 < tiles ? W / 16 : (end_valid + 15) >> 4, j > 0);
                 tc_commit(smem_u32(j + 1 < tiles ? &kempty[done] : finished));
                 if (++done == S::kK) done = 0;
                 if (j + 1 < tiles) products();
@@ -218,8 +223,8 @@ attention_tc_grad_query_kernel(const __grid_constant__ CUtensorMap map_q, const 
             }
         }
     } else {
-        // ------------------------------------------------------------------ a thread a row and 64 columns
-        const int half = warp >> 2, row = tid & 127;
+        // ------------------------------------------------------------------ a thread a row and 32 columns
+        const int part = warp >> 2, row = tid & 127;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const int token = t0 + (row >> log_p);
         const bool mine = token < n;
@@ -231,40 +236,32 @@ attention_tc_grad_query_kernel(const __grid_constant__ CUtensorMap map_q, const 
         const f32x2 c2 = pack_f32x2(a.c, a.c), l2 = pack_f32x2(-lse, -lse), d2 = pack_f32x2(-delta, -delta);
         bool ok = true;
         for (int j = 0; j < tiles; ++j) {
-            const uint32_t t_s = tmem + (j & 1) * 128 + half * 64 + lanes;
+            const uint32_t t_s = tmem + (j & 1) * W + part * 32 + lanes;
             if (!(ok = __all_sync(0xffffffffu, wait(&sfull[j & 1], (j >> 1) & 1)) != 0)) break;
             tc_fence_after();
-            f32x2 x[32];
-            const int left = seen - (first + j) * kAtRows - half * 64;
-            const bool masked = (first + j + 1) * kAtRows > seen_all;
+            f32x2 x[16];
             if (some) {
-                ab_load64(t_s, x);
+                lt_load32(t_s, x);
 #pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    const float2 f = unpack_f32x2(fma2(x[i], c2, l2));
-                    x[i] = pack_f32x2(ex2_approx(f.x), ex2_approx(f.y));
-                }
+                for (int i = 0; i < 16; ++i) x[i] = at_exp2_mix<AB_EMUQ>(fma2(x[i], c2, l2), i);
             }
             if (!(ok = __all_sync(0xffffffffu, wait(dpfull, j & 1)) != 0)) break;
             tc_fence_after();
             if (some) {
-                uint32_t w[32];
+                uint32_t w[16];
+                f32x2 y[16];
+                lt_load32(t_dp + part * 32 + lanes, y);
 #pragma unroll
-                for (int g = 0; g < 2; ++g) {
-                    f32x2 y[16];
-                    lt_load32(t_dp + half * 64 + g * 32 + lanes, y);
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const float2 f = unpack_f32x2(mul2(x[g * 16 + i], add2(y[i], d2)));
-                        w[g * 16 + i] = lt_pack<T>(f.x, f.y);
-                    }
+                for (int i = 0; i < 16; ++i) {
+                    const float2 f = unpack_f32x2(mul2(x[i], add2(y[i], d2)));
+                    w[i] = lt_pack<T>(f.x, f.y);
                 }
-                if (masked) {                                        // behind the row's keys; all of a single one
-                    const int keep = seen == 1 ? 0 : left;
+                if ((first + j + 1) * W > seen_all) {          // behind the row's keys; all of a single one
+                    const int keep = seen == 1 ? 0 : seen - (first + j) * W - part * 32;
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) w[i] &= (2 * i < keep ? 0xffffu : 0u) | (2 * i + 1 < keep ? 0xffff0000u : 0u);
+                    for (int i = 0; i < 16; ++i) w[i] &= (2 * i < keep ? 0xffffu : 0u) | (2 * i + 1 < keep ? 0xffff0000u : 0u);
                 }
-                tmem_st32(t_s, w);
+                tmem_st16(t_s, w);
                 tc_wait_st();
             }
             tc_fence_before();
@@ -274,8 +271,9 @@ attention_tc_grad_query_kernel(const __grid_constant__ CUtensorMap map_q, const 
         if (tiles > 0 && ok) ok = __all_sync(0xffffffffu, wait(finished, 0)) != 0;
         tc_fence_after();
         if (ok && some) {
-            float *part = a.splits > 1 ? a.partial + (blockIdx.z * (int64_t)a.M * a.H + at) * a.D : nullptr;
-            ab_store_row<T>(t_dq + lanes, half * (DP / 2), (half + 1) * (DP / 2), a.D, tiles == 0, a.scale, mine, (T *)a.gq + at * a.D, part);
+            constexpr int kCols = DP * 32 / W > 32 ? DP * 32 / W : 32;               // a part's (with more parts than 32s: none)
+            float *to = a.splits > 1 ? a.partial + (blockIdx.z * (int64_t)a.M * a.H + at) * a.D : nullptr;
+            ab_store_row<T>(t_dq + lanes, part * kCols, part * kCols + kCols, a.D, tiles == 0, a.scale, mine, (T *)a.gq + at * a.D, to);
         }
     }
 
@@ -289,39 +287,38 @@ attention_tc_grad_query_kernel(const __grid_constant__ CUtensorMap map_q, const 
         __syncthreads();
     }
     tc_fence_after();
-    if (warp == kAbWarpMma) tmem_dealloc(tmem, 512);
+    if (warp == S::kWarpMma) tmem_dealloc(tmem, S::kColumns);
 }
 
-template <int DP>
-struct AkShape {
-    static constexpr int kTile = DP / 64 * kAtBlock;
-    static constexpr int kStages = DP == 64 ? 4 : 2;                 // of q and grad
-    static constexpr int kSmem = 1024 + (2 + 2 * kStages) * kTile + kStages * 1024 + 512;
+template <int DP, int W>
+struct AkShape : AbShape<DP, W> {
+    static constexpr int kStages = DP == 64 ? (W == 64 ? 3 : 4) : 2;                // of q and grad
+    static constexpr int kSmem = 1024 + 2 * AbShape<DP, W>::kOwn + 2 * kStages * AbShape<DP, W>::kTile + kStages * W * 8 + 512;
 };
 
-template <typename T, int DP>
-__global__ void __launch_bounds__(kAbThreads, 1)
+template <typename T, int DP, int W>
+__global__ void __launch_bounds__(AbShape<DP, W>::kThreads, AbShape<DP, W>::kPerSm)
 attention_tc_grad_key_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                              const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_g,
                              const __grid_constant__ AtArgs a, const int log_p) {
-    using S = AkShape<DP>;
+    using S = AkShape<DP, W>;
     constexpr float kUp = dtype_traits<T>::mma_format == 0 ? 15.f : 0.f;         // powers of two on p
     constexpr float kDown = dtype_traits<T>::mma_format == 0 ? 0x1p-15f : 1.f;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *base = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    const uint32_t s_k = smem_u32(base), s_v = s_k + S::kTile, s_q = s_v + S::kTile;      // stages of q, grad
-    float *s_rows = reinterpret_cast<float *>(base + (2 + 2 * S::kStages) * S::kTile);    // stages of 128 x -lse, 128 x -delta
-    uint64_t *bar = reinterpret_cast<uint64_t *>(s_rows + S::kStages * 256);
+    const uint32_t s_k = smem_u32(base), s_v = s_k + S::kOwn, s_q = s_v + S::kOwn;      // stages of q, grad
+    float *s_rows = reinterpret_cast<float *>(base + 2 * S::kOwn + 2 * S::kStages * S::kTile);    // stages of W x -lse, W x -delta
+    uint64_t *bar = reinterpret_cast<uint64_t *>(s_rows + S::kStages * 2 * W);
     uint64_t *full = bar, *empty = full + S::kStages, *kvfull = empty + S::kStages, *tail = kvfull + 1, *sfull = tail + 1;
     uint64_t *dpfull = sfull + 1, *pready = dpfull + 1, *dsready = pready + 1, *finished = dsready + 1;
     uint32_t *s_tmem = reinterpret_cast<uint32_t *>(finished + 1);
     volatile int *s_abort = reinterpret_cast<volatile int *>(s_tmem + 1);
     AtSample *s_sample = reinterpret_cast<AtSample *>(s_tmem + 2);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int P = 1 << log_p, tokens = kAtRows >> log_p;
+    const int P = 1 << log_p, tokens = W >> log_p;
 
     at_check_offsets(a);
-    if (warp == kAbWarpLoad) {
+    if (warp == S::kWarpLoad) {
         const AtSample s = at_find(a.key_offsets, a.N, a, blockIdx.x, kAtRows);
         if (lane == 0) *s_sample = s;
     }
@@ -331,8 +328,8 @@ attention_tc_grad_key_kernel(const __grid_constant__ CUtensorMap map_q, const __
             mbar_init(smem_u32(&empty[i]), 1);
         }
         for (uint64_t *b : {kvfull, tail, sfull, dpfull, finished}) mbar_init(smem_u32(b), 1);
-        mbar_init(smem_u32(pready), 8);
-        mbar_init(smem_u32(dsready), 8);
+        mbar_init(smem_u32(pready), S::kWarps);
+        mbar_init(smem_u32(dsready), S::kWarps);
         *s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
@@ -340,14 +337,14 @@ attention_tc_grad_key_kernel(const __grid_constant__ CUtensorMap map_q, const __
     const AtSample s = *s_sample;
     const int n = s.q1 - s.q0, m = s.k1 - s.k0, key0 = s.tile * kAtRows;
     if (s.tile < 0 || key0 >= m) return;
-    if (warp == kAbWarpMma) {
-        tmem_alloc(smem_u32(s_tmem), 512);
+    if (warp == S::kWarpMma) {
+        tmem_alloc(smem_u32(s_tmem), S::kColumns);
         tmem_relinquish();
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *s_tmem, t_dp = tmem + 128, t_dv = tmem + 256, t_dk = t_dv + DP;
+    const uint32_t tmem = *s_tmem, t_dp = tmem + W, t_dv = tmem + 2 * W, t_dk = t_dv + DP;
     const int kh = blockIdx.y, G = a.H / a.K;
     // tiles of queries that see a key of this tile, of each block of P heads of the group
     const int from = a.causal ? (int)max((int64_t)0, (int64_t)key0 - m + n) / tokens : 0;
@@ -374,16 +371,16 @@ attention_tc_grad_key_kernel(const __grid_constant__ CUtensorMap map_q, const __
         }
     };
 
-    if (warp == kAbWarpLoad) {
+    if (warp == S::kWarpLoad) {
         // ------------------------------------------------------------------ loads: k, v; then q, grad and the rows' numbers
         if (tiles > 0) {
-            auto load = [&](uint32_t dst, const CUtensorMap *map, int head, int row, uint32_t mbar) {
-                for (int c = 0; c < DP / 64; ++c) tma_load_3d(dst + c * kAtBlock, map, c * 64, head, row, mbar);
+            auto load = [&](uint32_t dst, int rows, const CUtensorMap *map, int head, int row, uint32_t mbar) {
+                for (int c = 0; c < DP / 64; ++c) tma_load_3d(dst + c * rows * 128, map, c * 64, head, row, mbar);
             };
             if (elect_one()) {
-                mbar_arrive_expect_tx(smem_u32(kvfull), 2 * S::kTile);
-                load(s_k, &map_k, kh, s.k0 + key0, smem_u32(kvfull));
-                load(s_v, &map_v, kh, s.k0 + key0, smem_u32(kvfull));
+                mbar_arrive_expect_tx(smem_u32(kvfull), 2 * S::kOwn);
+                load(s_k, kAtRows, &map_k, kh, s.k0 + key0, smem_u32(kvfull));
+                load(s_v, kAtRows, &map_v, kh, s.k0 + key0, smem_u32(kvfull));
             }
             __syncwarp();
             int st = 0;
@@ -393,9 +390,9 @@ attention_tc_grad_key_kernel(const __grid_constant__ CUtensorMap map_q, const __
             for (int j = 0; j < tiles; ++j, advance(w), next(st, phase)) {
                 const int rows = rows_of(w);
                 const bool cut = rows & 15;
-                float lse[4], delta[4];
+                float lse[W / 32], delta[W / 32];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {                        // on their way while the stage is waited for
+                for (int i = 0; i < W / 32; ++i) {                        // on their way while the stage is waited for
                     const int r = lane + 32 * i;
                     const int64_t at = (int64_t)(s.q0 + w.t * tokens + (r >> log_p)) * a.H + w.head + (r & (P - 1));
                     lse[i] = r < rows ? kUp - __ldg(a.lse + at) : -INFINITY;
@@ -405,20 +402,20 @@ attention_tc_grad_key_kernel(const __grid_constant__ CUtensorMap map_q, const __
                 const uint32_t dst = s_q + st * 2 * S::kTile, mbar = smem_u32(cut ? tail : &full[st]);
                 if (elect_one()) {
                     mbar_arrive_expect_tx(mbar, 2 * S::kTile);
-                    load(dst, &map_q, w.head, s.q0 + w.t * tokens, mbar);
-                    load(dst + S::kTile, &map_g, w.head, s.q0 + w.t * tokens, mbar);
+                    load(dst, W, &map_q, w.head, s.q0 + w.t * tokens, mbar);
+                    load(dst + S::kTile, W, &map_g, w.head, s.q0 + w.t * tokens, mbar);
                 }
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    s_rows[st * 256 + lane + 32 * i] = lse[i];
-                    s_rows[st * 256 + 128 + lane + 32 * i] = delta[i];
+                for (int i = 0; i < W / 32; ++i) {
+                    s_rows[st * 2 * W + lane + 32 * i] = lse[i];
+                    s_rows[st * 2 * W + W + lane + 32 * i] = delta[i];
                 }
                 __syncwarp();
                 if (cut) {
                     if (!(ok = __all_sync(0xffffffffu, wait(tail, tail_phase)) != 0)) break;
                     tail_phase ^= 1u;
-                    at_zero_rows<DP>(dst, rows, (rows + 15) & ~15);
-                    at_zero_rows<DP>(dst + S::kTile, rows, (rows + 15) & ~15);
+                    at_zero_rows<DP, W>(dst, rows, (rows + 15) & ~15);
+                    at_zero_rows<DP, W>(dst + S::kTile, rows, (rows + 15) & ~15);
                     fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(smem_u32(&full[st]));
@@ -426,10 +423,10 @@ attention_tc_grad_key_kernel(const __grid_constant__ CUtensorMap map_q, const __
                 if (lane == 0) mbar_arrive(smem_u32(&full[st]));
             }
         }
-    } else if (warp == kAbWarpMma) {
+    } else if (warp == S::kWarpMma) {
         // ------------------------------------------------------------------ products
         if (tiles > 0 && elect_one()) {
-            const uint32_t id_s = instr_desc_f16(dtype_traits<T>::mma_format, 128, 128);
+            const uint32_t id_s = instr_desc_f16(dtype_traits<T>::mma_format, 128, W);
             const uint32_t id_o = instr_desc_f16(dtype_traits<T>::mma_format, 128, (a.D + 15) & ~15) | 1u << 16;
             const int steps = (a.D + 15) >> 4;
             int st = 0;
@@ -437,9 +434,9 @@ attention_tc_grad_key_kernel(const __grid_constant__ CUtensorMap map_q, const __
             bool ok = wait(kvfull, 0) && wait(&full[0], 0);
             if (ok) {
                 tc_fence_after();
-                at_mma_head<DP>(tmem, s_k, s_q, id_s, steps);
+                at_mma_head<DP, W>(tmem, s_k, s_q, id_s, steps);
                 tc_commit(smem_u32(sfull));
-                at_mma_head<DP>(t_dp, s_v, s_q + S::kTile, id_s, steps);
+                at_mma_head<DP, W>(t_dp, s_v, s_q + S::kTile, id_s, steps);
                 tc_commit(smem_u32(dpfull));
             }
             Walk w = begin();
@@ -451,27 +448,28 @@ attention_tc_grad_key_kernel(const __grid_constant__ CUtensorMap map_q, const __
                 const uint32_t s_next = s_q + st * 2 * S::kTile;
                 if (!(ok = wait(pready, t_phase))) break;
                 tc_fence_after();
-                at_mma_rows(t_dv, tmem, 32, s_here + S::kTile, id_o, sum_steps, j > 0);
+                at_mma_rows<32, W>(t_dv, tmem, s_here + S::kTile, id_o, sum_steps, j > 0);
                 if (more) {
                     if (!(ok = wait(&full[st], phase))) break;
                     tc_fence_after();
-                    at_mma_head<DP>(tmem, s_k, s_next, id_s, steps);
+                    at_mma_head<DP, W>(tmem, s_k, s_next, id_s, steps);
                     tc_commit(smem_u32(sfull));
                 }
                 if (!(ok = wait(dsready, t_phase))) break;
                 tc_fence_after();
-                at_mma_rows(t_dk, t_dp, 32, s_here, id_o, sum_steps, j > 0);
+                at_mma_rows<32, W>(t_dk, t_dp, s_here, id_o, sum_steps, j > 0);
                 tc_commit(smem_u32(more ? &empty[here] : finished));
                 if (more) {
-                    at_mma_head<DP>(t_dp, s_v, s_next + S::kTile, id_s, steps);
+                    at_mma_head<DP, W>(t_dp, s_v, s_next + S::kTile, id_s, steps);
                     tc_commit(smem_u32(dpfull));
                 }
             }
         }
     } else {
-        // ------------------------------------------------------------------ a thread a key and 64 query rows
-        const int half = warp >> 2, row = tid & 127, key = key0 + row;
+        // ------------------------------------------------------------------ a thread a key and 32 query rows
+        const int part = warp >> 2, row = tid & 127, key = key0 + row;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t t_s = tmem + part * 32 + lanes, t_d = t_dp + part * 32 + lanes;
         const bool mine = key < m;
         const f32x2 c2 = pack_f32x2(a.c, a.c), k2 = pack_f32x2(kDown, kDown);
         bool ok = true;
@@ -479,67 +477,61 @@ attention_tc_grad_key_kernel(const __grid_constant__ CUtensorMap map_q, const __
         uint32_t phase = 0, t_phase = 0;
         Walk w = begin();
         for (int j = 0; j < tiles; ++j, t_phase ^= 1u, next(st, phase), advance(w)) {
-            const uint32_t t_s = tmem + half * 64 + lanes, t_d = t_dp + half * 64 + lanes;
-            const uint32_t s_lse = smem_u32(s_rows + st * 256 + half * 64), s_delta = s_lse + 512;
+            const uint32_t s_lse = smem_u32(s_rows + st * 2 * W + part * 32), s_delta = s_lse + W * 4;
             // columns from `see` on see this key; from `use` on with a gradient of their score
             int see = 0, use = 0;
             bool masked = m == 1;
             if (a.causal) {
                 const int64_t before = (int64_t)n - m - (int64_t)w.t * tokens;   // the query that sees key 0 last, in the tile
                 masked |= before + key0 + kAtRows - 1 > 0;
-                const int64_t at = max((int64_t)-kAtRows, min((int64_t)kAtRows, before + key)) * P - half * 64;
-                see = (int)at;
+                see = (int)max((int64_t)-kAtRows, min((int64_t)kAtRows, before + key)) * P - part * 32;
                 use = see + (key == 0 ? P : 0);
             }
             if (m == 1) use = kAtRows;
             if (!(ok = __all_sync(0xffffffffu, wait(&full[st], phase) && wait(sfull, t_phase)) != 0)) break;
             tc_fence_after();
-            f32x2 x[32];
-            uint32_t u[32];
-            ab_load64(t_s, x);
+            f32x2 x[16];
+            uint32_t u[16];
+            lt_load32(t_s, x);
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) {
+            for (int i = 0; i < 16; i += 2) {
                 f32x2 l0, l1;
                 asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];\n" : "=l"(l0.v), "=l"(l1.v) : "r"(s_lse + i * 8));
-                const float2 f0 = unpack_f32x2(fma2(x[i], c2, l0)), f1 = unpack_f32x2(fma2(x[i + 1], c2, l1));
-                x[i] = pack_f32x2(ex2_approx(f0.x), ex2_approx(f0.y));
-                x[i + 1] = pack_f32x2(ex2_approx(f1.x), ex2_approx(f1.y));
+                x[i] = at_exp2_mix<AB_EMUK>(fma2(x[i], c2, l0), i);
+                x[i + 1] = at_exp2_mix<AB_EMUK>(fma2(x[i + 1], c2, l1), i + 1);
             }
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
+            for (int i = 0; i < 16; ++i) {
                 const float2 f = unpack_f32x2(x[i]);
                 u[i] = lt_pack<T>(f.x, f.y);
             }
             if (masked) {
 #pragma unroll
-                for (int i = 0; i < 32; ++i) u[i] &= (2 * i >= see ? 0xffffu : 0u) | (2 * i + 1 >= see ? 0xffff0000u : 0u);
+                for (int i = 0; i < 16; ++i) u[i] &= (2 * i >= see ? 0xffffu : 0u) | (2 * i + 1 >= see ? 0xffff0000u : 0u);
             }
-            tmem_st32(t_s, u);
+            tmem_st16(t_s, u);
             tc_wait_st();
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(pready));
             if (!(ok = __all_sync(0xffffffffu, wait(dpfull, t_phase)) != 0)) break;
             tc_fence_after();
+            f32x2 y[16];
+            lt_load32(t_d, y);
 #pragma unroll
-            for (int g = 0; g < 2; ++g) {
-                f32x2 y[16];
-                lt_load32(t_d + g * 32, y);
-#pragma unroll
-                for (int i = 0; i < 16; i += 2) {
-                    f32x2 d0, d1;
-                    asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];\n" : "=l"(d0.v), "=l"(d1.v) : "r"(s_delta + (g * 16 + i) * 8));
-                    const float2 f0 = unpack_f32x2(mul2(x[g * 16 + i], fma2(y[i], k2, d0)));
-                    const float2 f1 = unpack_f32x2(mul2(x[g * 16 + i + 1], fma2(y[i + 1], k2, d1)));
-                    u[g * 16 + i] = lt_pack<T>(f0.x, f0.y);
-                    u[g * 16 + i + 1] = lt_pack<T>(f1.x, f1.y);
-                }
+            for (int i = 0; i < 16; i += 2) {
+                f32x2 d0, d1;
+                asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];\n" : "=l"(d0.v), "=l"(d1.v) : "r"(s_delta + i * 8));
+                const float2 f0 = unpack_f32x2(mul2(x[i], fma2(y[i], k2, d0)));
+                const float2 f1 = unpack_f32x2(mul2(x[i + 1], fma2(y[i + 1], k2, d1)));
+                u[i] = lt_pack<T>(f0.x, f0.y);
+                u[i + 1] = lt_pack<T>(f1.x, f1.y);
             }
             if (masked) {
 #pragma unroll
-                for (int i = 0; i < 32; ++i) u[i] &= (2 * i >= use ? 0xffffu : 0u) | (2 * i + 1 >= use ? 0xffff0000u : 0u);
+                for (int i = 0; i < 16; ++i) u[i] &= (2 * i >= use ? 0xffffu : 0u) | (2 * i + 1 >= use ? 0xffff0000u : 0u);
             }
-            tmem_st32(t_d, u);
+            tmem_st16(t_d, u);
             tc_wait_st();
             tc_fence_before();
             __syncwarp();
@@ -547,12 +539,15 @@ attention_tc_grad_key_kernel(const __grid_constant__ CUtensorMap map_q, const __
         }
         if (tiles > 0 && ok) ok = __all_sync(0xffffffffu, wait(finished, 0)) != 0;
         tc_fence_after();
-        if (ok) {                                                    // half 0 stores grad_value, half 1 grad_key
+        if (ok) {                                                    // half of the parts stores grad_value, half grad_key
+            constexpr int kParts = W / 64, kCols = DP / kParts;
+            const bool keys = part >= kParts;
             const int64_t all = (int64_t)a.N * a.K, at = (int64_t)(s.k0 + key) * a.K + kh;
-            float *part = a.splits > 1 ? a.partial + ((2 * blockIdx.z + 1 - half) * all + at) * a.D : nullptr;
-            T *out = (T *)(half ? a.gk : a.gv);
-            ab_store_row<T>((half ? t_dk : t_dv) + lanes, 0, DP, a.D, tiles == 0, half ? a.scale : kDown, mine && (out || part),
-                            out ? out + at * a.D : nullptr, part);
+            float *to = a.splits > 1 ? a.partial + ((2 * blockIdx.z + !keys) * all + at) * a.D : nullptr;
+            T *out = (T *)(keys ? a.gk : a.gv);
+            const int c0 = (part & (kParts - 1)) * kCols;
+            ab_store_row<T>((keys ? t_dk : t_dv) + lanes, c0, c0 + kCols, a.D, tiles == 0, keys ? a.scale : kDown, mine && (out || to),
+                            out ? out + at * a.D : nullptr, to);
         }
     }
 
@@ -566,31 +561,41 @@ attention_tc_grad_key_kernel(const __grid_constant__ CUtensorMap map_q, const __
         __syncthreads();
     }
     tc_fence_after();
-    if (warp == kAbWarpMma) tmem_dealloc(tmem, 512);
+    if (warp == S::kWarpMma) tmem_dealloc(tmem, S::kColumns);
 }
 
-template <typename T, int DP, bool KEYS>
+template <typename T, int DP, int W, bool KEYS>
 static int ab_run(const AtArgs &a) {
+    using S = AbShape<DP, W>;
     const int G = a.H / a.K;
+    constexpr int rows = KEYS ? W : kAtRows;                         // query rows of a tile
     int log_p = 0;
-    while (log_p < 7 && G % (2 << log_p) == 0) ++log_p;
-    const int P = 1 << log_p, tokens = kAtRows >> log_p;
+    while ((2 << log_p) <= rows && G % (2 << log_p) == 0) ++log_p;
+    const int P = 1 << log_p, tokens = rows >> log_p, keys = KEYS ? kAtRows : W;
     CUtensorMap mq, mk, mv, mg;
-    if (!at_map(&mq, a.q, a.M, a.H, a.D, P, tokens) || !at_map(&mk, a.k, a.N, a.K, a.D, 1, kAtRows) ||
-        !at_map(&mv, a.v, a.N, a.K, a.D, 1, kAtRows) || !at_map(&mg, a.grad, a.M, a.H, a.D, P, tokens))
+    if (!at_map(&mq, a.q, a.M, a.H, a.D, P, tokens) || !at_map(&mk, a.k, a.N, a.K, a.D, 1, keys) ||
+        !at_map(&mv, a.v, a.N, a.K, a.D, 1, keys) || !at_map(&mg, a.grad, a.M, a.H, a.D, P, tokens))
         return SPCONV_ERR_CUDA;
     static std::atomic<uint64_t> done;
-    auto kern = KEYS ? attention_tc_grad_key_kernel<T, DP> : attention_tc_grad_query_kernel<T, DP>;
-    constexpr int smem = KEYS ? AkShape<DP>::kSmem : AqShape<DP>::kSmem;
+    auto kern = KEYS ? attention_tc_grad_key_kernel<T, DP, W> : attention_tc_grad_query_kernel<T, DP, W>;
+    // padded so that no more CTAs share an SM than its TMEM columns serve
+    constexpr int need = KEYS ? AkShape<DP, W>::kSmem : AqShape<DP, W>::kSmem, least = S::kPerSm == 2 ? 80 * 1024 : 120 * 1024;
+    constexpr int smem = need > least ? need : least;
     if (allow_smem(kern, smem, done) != cudaSuccess) return check_launch("attention: shared memory");
     const dim3 grid(KEYS ? (unsigned)at_tiles(a.N, a.B, kAtRows) : (unsigned)at_tiles(a.M, a.B, tokens), KEYS ? a.K : a.H / P, a.splits);
-    kern<<<grid, kAbThreads, smem, a.stream>>>(mq, mk, mv, mg, a, log_p);
+    kern<<<grid, S::kThreads, smem, a.stream>>>(mq, mk, mv, mg, a, log_p);
     return check_launch(KEYS ? "attention_tc_grad_key_kernel" : "attention_tc_grad_query_kernel");
 }
 
+#ifndef AB_WQ
+#define AB_WQ 64
+#endif
+#ifndef AB_WK
+#define AB_WK 64
+#endif
 template <typename T, bool KEYS>
 static int ab_size(const AtArgs &a) {
-    return a.D <= 64 ? ab_run<T, 64, KEYS>(a) : ab_run<T, 128, KEYS>(a);
+    return a.D <= 64 ? ab_run<T, 64, KEYS ? AB_WK : AB_WQ, KEYS>(a) : ab_run<T, 128, 128, KEYS>(a);
 }
 
 int launch_at_tc_grad_query(const AtArgs &a) {

@@ -27,39 +27,298 @@ namespace spconv {
 
 constexpr float kAfSlack = 8.f;                      // by how much the maximum in use may be exceeded, in powers of two
 
-template <int NQ, int DP>
+// A row's result: its accumulators over its sum; or, where keys are split, the accumulators as they
+// are. A warp's lanes together.
+template <typename T>
+__device__ __forceinline__ void af_store(const AtArgs &a, uint32_t t_o, int size, int64_t at, bool mine, bool none, bool nothing, float top,
+                                         float sum) {
+    const int64_t all = (int64_t)a.M * a.H;
+    float *part = a.splits > 1 ? a.partial + (blockIdx.z * all + at) * a.D : nullptr;
+    const float inv = part ? 1.f : none ? 0.f : 1.f / sum;
+    if (mine) {
+        if (part) a.part_ml[blockIdx.z * all + at] = make_float2(top * a.c, sum);
+        else if (a.lse) a.lse[at] = none ? INFINITY : fmaf(top, a.c, log2f(sum));
+    }
+    T *out = (T *)a.out + at * a.D;
+    const bool wide = (a.D & 7) == 0 && ((uintptr_t)a.out & 15) == 0;
+#pragma unroll 1
+    for (int c = 0; c < size && c < a.D; c += 16) {
+        uint32_t o[16];
+        if (!nothing) {                                              // there were keys, the same for every lane
+            tmem_ld16(t_o + c, o);
+            tc_wait_ld();
+        }
+        if (!mine || (part && nothing)) continue;
+        none |= nothing;
+#pragma unroll
+        for (int v = 0; v < 2; ++v) {
+            const int d = c + v * 8;
+            if (d >= a.D) break;
+            float f[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = none ? 0.f : __uint_as_float(o[v * 8 + i]) * inv;
+            if (part) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (d + i < a.D) part[d + i] = f[i];
+            } else if (wide) {
+                *(uint4 *)(out + d) = make_uint4(lt_pack<T>(f[0], f[1]), lt_pack<T>(f[2], f[3]), lt_pack<T>(f[4], f[5]), lt_pack<T>(f[6], f[7]));
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (d + i < a.D) out[d + i] = dtype_traits<T>::from_f(f[i]);
+            }
+        }
+    }
+}
+
+// A CTA a tile of queries.
+template <int DP>
 struct AfShape {
-    static constexpr int kThreads = NQ * 128 + 64;
-    static constexpr int kTile = DP / 64 * kAtBlock;
-    static constexpr int kStages = NQ == 2 ? (DP == 64 ? 8 : 4) : (DP == 64 ? 5 : 2);
-    static constexpr int kSmem = 1024 + (NQ + kStages) * kTile + 512;
-    // no more CTAs than the SM's 512 columns serve
-    static constexpr int kSmemLeast = NQ == 2 ? 120 * 1024 : 80 * 1024;
-    static constexpr int kColumns = NQ == 2 ? 512 : 256;
-    static constexpr int kAcc = NQ * 128;            // first column of the accumulators
+    static constexpr int kKeys = 64, kStages = 2, kPerSm = DP == 64 ? 4 : 2;
+    static constexpr int kOwn = DP / 64 * kAtBlock, kTile = kOwn / 2;            // bytes of a tile of queries, and of keys or values
+    static constexpr int kSmem = 1024 + kOwn + 2 * kStages * kTile + 256, kSmemLeast = 228 * 1024 / (kPerSm + 1);
+    static constexpr int kColumns = 512 / kPerSm;    // scores, p over them; accumulators
+    static constexpr int kThreads = 160, kControl = 4;
 };
 
-template <typename T, int NQ, int DP>
-__global__ void __launch_bounds__(NQ * 128 + 64, NQ == 2 ? 1 : 2)
+template <typename T, int DP>
+__global__ void __launch_bounds__(AfShape<DP>::kThreads, AfShape<DP>::kPerSm)
 attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                    const __grid_constant__ CUtensorMap map_v, const __grid_constant__ AtArgs a, const int log_p) {
-    using S = AfShape<NQ, DP>;
+                      const __grid_constant__ CUtensorMap map_v, const __grid_constant__ AtArgs a, const int log_p) {
+    using S = AfShape<DP>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *base = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    const uint32_t s_q = smem_u32(base), s_ring = s_q + NQ * S::kTile;
-    uint64_t *bar = reinterpret_cast<uint64_t *>(base + (NQ + S::kStages) * S::kTile);
-    uint64_t *full = bar, *empty = full + S::kStages, *qfull = empty + S::kStages, *tail = qfull + 1, *sfull = tail + 1, *pready = sfull + NQ;
-    uint32_t *s_tmem = reinterpret_cast<uint32_t *>(pready + NQ);
+    const uint32_t s_q = smem_u32(base), s_k = s_q + S::kOwn, s_v = s_k + S::kStages * S::kTile;
+    uint64_t *bar = reinterpret_cast<uint64_t *>(base + S::kOwn + 2 * S::kStages * S::kTile);
+    uint64_t *kfull = bar, *vfull = kfull + S::kStages, *qfull = vfull + S::kStages, *sfull = qfull + 1, *pready = sfull + 1;
+    uint32_t *s_tmem = reinterpret_cast<uint32_t *>(pready + 1);
     volatile int *s_abort = reinterpret_cast<volatile int *>(s_tmem + 1);
     AtSample *s_sample = reinterpret_cast<AtSample *>(s_tmem + 2);
-    constexpr int kWarpLoad = NQ * 4, kWarpMma = NQ * 4 + 1;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int P = 1 << log_p, tokens = kAtRows >> log_p;             // tokens of a tile
 
     at_check_offsets(a);
-    if (warp == kWarpLoad) {
+    if (warp == S::kControl) {
         // the last tiles of a causal sample see most: they go first
-        const AtSample s = at_find(a.offsets, a.M, a, a.causal ? gridDim.x - 1 - blockIdx.x : blockIdx.x, NQ * tokens);
+        const AtSample s = at_find(a.offsets, a.M, a, a.causal ? gridDim.x - 1 - blockIdx.x : blockIdx.x, tokens);
+        if (lane == 0) *s_sample = s;
+    }
+    if (tid == 0) {
+        for (int i = 0; i < S::kStages; ++i) {
+            mbar_init(smem_u32(&kfull[i]), 1);
+            mbar_init(smem_u32(&vfull[i]), 1);
+        }
+        mbar_init(smem_u32(qfull), 1);
+        mbar_init(smem_u32(sfull), 1);
+        mbar_init(smem_u32(pready), 4);
+        *s_abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    }
+    __syncthreads();
+    const AtSample s = *s_sample;
+    const int n = s.q1 - s.q0, m = s.k1 - s.k0, t0 = s.tile * tokens;            // the CTA's first token in the sample
+    if (s.tile < 0 || t0 >= n) return;                                           // uniform over the CTA
+    if (warp == S::kControl) {
+        tmem_alloc(smem_u32(s_tmem), S::kColumns);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *s_tmem;
+    const int head0 = blockIdx.y << log_p, kh = head0 / (a.H / a.K);
+    const int seen_last = at_seen(a, min(n, t0 + tokens) - 1, n, m);
+    int first, last;
+    at_split(a.splits, blockIdx.z, (seen_last + S::kKeys - 1) / S::kKeys, first, last);
+    const int tiles = last - first;
+    const int end_valid = min(S::kKeys, seen_last - (last - 1) * S::kKeys);      // keys of the last tile (of this split)
+    auto wait = [&](uint64_t *b, uint32_t parity) {
+        return __all_sync(0xffffffffu, mbar_wait_suspended(smem_u32(b), parity, s_abort, a.wait_ns)) != 0;
+    };
+
+    if (warp == S::kControl) {
+        // ------------------------------------------------------------------ loads and products
+        if (tiles > 0) {
+            const uint32_t id_s = instr_desc_f16(dtype_traits<T>::mma_format, 128, S::kKeys);
+            const uint32_t id_o = instr_desc_f16(dtype_traits<T>::mma_format, 128, (a.D + 15) & ~15) | 1u << 16;
+            const int steps = (a.D + 15) >> 4;
+            auto load = [&](uint32_t dst, const CUtensorMap *map, int head, int row, int bytes, uint64_t *b) {
+                mbar_arrive_expect_tx(smem_u32(b), bytes);
+                for (int c = 0; c < DP / 64; ++c) tma_load_3d(dst + c * (bytes / (DP / 64)), map, c * 64, head, row, smem_u32(b));
+            };
+            auto load_tile = [&](int j) {
+                const int row = s.k0 + (first + j) * S::kKeys, st = j & 1;
+                load(s_k + st * S::kTile, &map_k, kh, row, S::kTile, &kfull[st]);
+                load(s_v + st * S::kTile, &map_v, kh, row, S::kTile, &vfull[st]);
+            };
+            if (elect_one()) {
+                load(s_q, &map_q, head0, s.q0 + t0, S::kOwn, qfull);
+                load_tile(0);
+                if (tiles > 1) load_tile(1);
+            }
+            __syncwarp();
+            bool ok = wait(qfull, 0);
+            for (int j = 0; j <= tiles && ok; ++j) {
+                const int st = j & 1;
+                if (j > 0) {                                         // p v of the tile before
+                    const int v = st ^ 1;
+                    const bool end = j == tiles;
+                    if (!(ok = wait(&vfull[v], ((j - 1) >> 1) & 1))) break;
+                    if (end && (end_valid & 15)) {
+                        at_zero_rows<DP, S::kKeys>(s_v + v * S::kTile, end_valid, (end_valid + 15) & ~15);
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                    }
+                    if (!(ok = wait(pready, (j - 1) & 1))) break;
+                    tc_fence_after();
+                    if (elect_one()) {
+                        at_mma_rows<S::kKeys, S::kKeys>(tmem + S::kKeys, tmem, s_v + v * S::kTile, id_o, end ? (end_valid + 15) >> 4 : S::kKeys / 16, j > 1);
+                        if (end) tc_commit(smem_u32(sfull));
+                    }
+                    __syncwarp();
+                }
+                if (j < tiles) {
+                    if (!(ok = wait(&kfull[st], (j >> 1) & 1))) break;
+                    tc_fence_after();
+                    if (elect_one()) {
+                        at_mma_head<DP, S::kKeys>(tmem, s_q, s_k + st * S::kTile, id_s, steps);
+                        tc_commit(smem_u32(sfull));
+                    }
+                    __syncwarp();
+                    if (j > 0 && j + 1 < tiles) {                    // the tile before is done with: its stage takes the next
+                        if (!(ok = wait(sfull, j & 1))) break;
+                        if (elect_one()) load_tile(j + 1);
+                        __syncwarp();
+                    }
+                }
+            }
+        }
+    } else {
+        // ------------------------------------------------------------------ softmax: a thread a row
+        const uint32_t t_s = tmem + ((uint32_t)(warp * 32) << 16), t_o = t_s + S::kKeys;
+        const int token = t0 + (tid >> log_p);                       // in the sample
+        const bool mine = token < n;
+        const int seen = mine ? at_seen(a, token, n, m) : 0;
+        const bool some = __any_sync(0xffffffffu, mine);
+        // keys that every row of the warp sees: tiles up to there need no mask
+        const int seen_all = __reduce_min_sync(0xffffffffu, mine ? seen : m);
+        float top = -INFINITY, sum = 0.f;                            // of s; of p
+        bool ok = true;
+        for (int j = 0; j < tiles; ++j) {
+            if (!(ok = wait(sfull, j & 1))) break;
+            tc_fence_after();
+            if (some) {
+                f32x2 x[32];
+                at_load(t_s, x);
+                const int key0 = (first + j) * S::kKeys;
+                if (key0 + S::kKeys > seen_all) {
+                    const int left = seen - key0;
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        const float2 f = unpack_f32x2(x[i]);
+                        x[i] = pack_f32x2(2 * i < left ? f.x : -INFINITY, 2 * i + 1 < left ? f.y : -INFINITY);
+                    }
+                }
+                float big[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    const float2 f = unpack_f32x2(x[i]);
+                    big[i & 3] = max3_nan(big[i & 3], f.x, f.y);
+                }
+                const float now = max3_nan(max3_nan(big[0], big[1], big[2]), big[3], big[3]);
+                // a maximum that has grown by more than the slack (from -inf: by any amount), or is NaN, is taken over
+                const bool grown = !((now - top) * a.c <= kAfSlack) && now != -INFINITY;
+                if (__any_sync(0xffffffffu, grown)) {
+                    const float down = grown ? ex2_approx((top - now) * a.c) : 1.f;
+                    if (grown) top = now;
+                    sum *= down;
+                    if (j > 0) {                                     // the products before are done: s came after them
+#pragma unroll 1
+                        for (int c = 0; c < DP; c += 16) {
+                            uint32_t o[16];
+                            tmem_ld16(t_o + c, o);
+                            tc_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * down);
+                            tmem_st16(t_o + c, o);
+                        }
+                    }
+                }
+                const float shift = top == -INFINITY ? 0.f : -top * a.c;
+                const f32x2 c2 = pack_f32x2(a.c, a.c), s2 = pack_f32x2(shift, shift);
+                f32x2 add[2] = {pack_f32x2(0.f, 0.f), pack_f32x2(0.f, 0.f)};
+#pragma unroll
+                for (int g = 0; g < 2; ++g) {
+                    uint32_t w[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const f32x2 e = at_exp2(fma2(x[g * 16 + i], c2, s2));
+                        const float2 f = unpack_f32x2(e);
+                        add[i & 1] = add2(add[i & 1], e);
+                        w[i] = lt_pack<T>(f.x, f.y);
+                    }
+                    tmem_st16(t_s + g * 16, w);
+                }
+                const float2 f = unpack_f32x2(add2(add[0], add[1]));
+                sum += f.x + f.y;
+                tc_wait_st();
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(pready));
+        }
+        if (tiles > 0 && ok) ok = wait(sfull, tiles & 1);            // the last p v
+        tc_fence_after();
+        if (ok && some)
+            af_store<T>(a, t_o, DP, (int64_t)(s.q0 + token) * a.H + head0 + (tid & (P - 1)), mine, seen == 0, tiles == 0, top, sum);
+    }
+
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();                                                 // every role has set the flag by now if it gives up
+    if (*s_abort) {                                                  // copies and products in flight end within this
+        if (tid == 0) raise_status(a.status, SPCONV_STATUS_WAIT_TIMEOUT);
+        const uint64_t begin = globaltimer_ns();
+        while (globaltimer_ns() - begin < kTmaDrainNs) {}
+        __syncthreads();
+    }
+    tc_fence_after();
+    if (warp == S::kControl) tmem_dealloc(tmem, S::kColumns);
+}
+
+// Heads of more than 64 values: two tiles of queries a CTA, keys 128 at a time.
+struct ApShape {
+    static constexpr int kThreads = 384, kWarpLoad = 8, kWarpMma = 9;
+    // registers: launched with 168 a thread, dealt out anew: 224 x 256 + 56 x 128 = 168 x 384
+    static constexpr int kRegs = 224, kRegsOther = 56;
+    static constexpr int kTile = 2 * kAtBlock, kStages = 4;
+    static constexpr int kSmem = 1024 + (2 + kStages) * kTile + 256, kSmemLeast = 120 * 1024;
+    static constexpr int kAcc = 256;                 // first column of the accumulators, behind two tiles' scores
+};
+
+template <typename T>
+__global__ void __launch_bounds__(ApShape::kThreads, 1)
+attention_tc_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                    const __grid_constant__ CUtensorMap map_v, const __grid_constant__ AtArgs a, const int log_p) {
+    using S = ApShape;
+    constexpr int DP = 128;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *base = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    const uint32_t s_q = smem_u32(base), s_ring = s_q + 2 * S::kTile;
+    uint64_t *bar = reinterpret_cast<uint64_t *>(base + (2 + S::kStages) * S::kTile);
+    uint64_t *full = bar, *empty = full + S::kStages, *qfull = empty + S::kStages, *tail = qfull + 1, *sfull = tail + 1;
+    uint64_t *pready = sfull + 2, *odone = pready + 2;
+    uint32_t *s_tmem = reinterpret_cast<uint32_t *>(odone + 2);
+    volatile int *s_abort = reinterpret_cast<volatile int *>(s_tmem + 1);
+    AtSample *s_sample = reinterpret_cast<AtSample *>(s_tmem + 2);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int P = 1 << log_p, tokens = kAtRows >> log_p;             // tokens of a tile
+
+    at_check_offsets(a);
+    if (warp == S::kWarpLoad) {
+        // the last tiles of a causal sample see most: they go first
+        const AtSample s = at_find(a.offsets, a.M, a, a.causal ? gridDim.x - 1 - blockIdx.x : blockIdx.x, 2 * tokens);
         if (lane == 0) *s_sample = s;
     }
     if (tid == 0) {
@@ -69,19 +328,20 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         }
         mbar_init(smem_u32(qfull), 1);
         mbar_init(smem_u32(tail), 1);
-        for (int q = 0; q < NQ; ++q) {
+        for (int q = 0; q < 2; ++q) {
             mbar_init(smem_u32(&sfull[q]), 1);
             mbar_init(smem_u32(&pready[q]), 4);
+            mbar_init(smem_u32(&odone[q]), 1);
         }
         *s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
     __syncthreads();
     const AtSample s = *s_sample;
-    const int n = s.q1 - s.q0, m = s.k1 - s.k0, t0 = s.tile * NQ * tokens;        // the CTA's first token in the sample
+    const int n = s.q1 - s.q0, m = s.k1 - s.k0, t0 = s.tile * 2 * tokens;        // the CTA's first token in the sample
     if (s.tile < 0 || t0 >= n) return;                                           // uniform over the CTA
-    if (warp == kWarpMma) {
-        tmem_alloc(smem_u32(s_tmem), S::kColumns);
+    if (warp == S::kWarpMma) {
+        tmem_alloc(smem_u32(s_tmem), 512);
         tmem_relinquish();
     }
     tc_fence_before();
@@ -89,7 +349,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     tc_fence_after();
     const uint32_t tmem = *s_tmem;
     const int head0 = blockIdx.y << log_p, kh = head0 / (a.H / a.K);
-    const int nq = NQ == 2 && t0 + tokens < n ? 2 : 1;               // tiles with a row in them
+    const int nq = t0 + tokens < n ? 2 : 1;               // tiles with a row in them
     const int seen_last = at_seen(a, min(n, t0 + nq * tokens) - 1, n, m);
     int first, last;
     at_split(a.splits, blockIdx.z, (seen_last + kAtRows - 1) / kAtRows, first, last);
@@ -103,7 +363,9 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         }
     };
 
-    if (warp == kWarpLoad) {
+    if (warp >= S::kWarpLoad) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" :: "n"(S::kRegsOther));
+    if (warp == S::kWarpLoad) {
         // ------------------------------------------------------------------ loads: q; then k, v of each tile in turn
         if (tiles > 0) {
             if (elect_one()) {
@@ -117,7 +379,9 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             uint32_t phase = 1;                                      // the first use of a stage passes at once
             bool ok = true;
             for (int i = 0; i < 2 * tiles && ok; ++i, next(st, phase)) {
-                const bool is_v = i & 1, cut = is_v && i + 1 == 2 * tiles && (end_valid & 15);
+                const bool is_v = i & 1;
+                const int tile = i >> 1;
+                const bool cut = is_v && tile + 1 == tiles && (end_valid & 15);
                 ok = __all_sync(0xffffffffu, wait(&empty[st], phase)) != 0;
                 if (!ok) break;
                 const uint32_t dst = s_ring + st * S::kTile;
@@ -125,60 +389,51 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     const uint32_t mbar = smem_u32(cut ? tail : &full[st]);
                     mbar_arrive_expect_tx(mbar, S::kTile);
                     for (int c = 0; c < DP / 64; ++c)
-                        tma_load_3d(dst + c * kAtBlock, is_v ? &map_v : &map_k, c * 64, kh, s.k0 + (first + (i >> 1)) * kAtRows, mbar);
+                        tma_load_3d(dst + c * kAtBlock, is_v ? &map_v : &map_k, c * 64, kh, s.k0 + (first + tile) * kAtRows, mbar);
                 }
                 __syncwarp();
                 if (cut) {
                     ok = __all_sync(0xffffffffu, wait(tail, 0)) != 0;
-                    at_zero_rows<DP>(dst, end_valid, (end_valid + 15) & ~15);
+                    at_zero_rows<DP, kAtRows>(dst, end_valid, (end_valid + 15) & ~15);
                     fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(smem_u32(&full[st]));
                 }
             }
         }
-    } else if (warp == kWarpMma) {
+    } else if (warp == S::kWarpMma) {
         // ------------------------------------------------------------------ products
         if (tiles > 0 && elect_one()) {
             const uint32_t id_s = instr_desc_f16(dtype_traits<T>::mma_format, 128, 128);
             const uint32_t id_o = instr_desc_f16(dtype_traits<T>::mma_format, 128, (a.D + 15) & ~15) | 1u << 16;
             const int steps = (a.D + 15) >> 4;
-            int st = 0;
-            uint32_t phase = 0, p_phase = 0;
-            bool ok = wait(qfull, 0) && wait(&full[0], 0);
-            if (ok) {
+            // the ring holds k0, v0, k1, v1, ..
+            auto landed = [&](int at) { return wait(&full[at % S::kStages], (at / S::kStages) & 1); };
+            auto release = [&](int at) { tc_commit(smem_u32(&empty[at % S::kStages])); };
+            auto stage = [&](int at) { return s_ring + at % S::kStages * S::kTile; };
+            bool ok = wait(qfull, 0);
+            auto scores = [&](int q, int i) {                        // s of tile i
+                if (!(ok = ok && landed(2 * i))) return;
                 tc_fence_after();
-                for (int q = 0; q < nq; ++q) {
-                    at_mma_head<DP>(tmem + q * 128, s_q + q * S::kTile, s_ring, id_s, steps);
-                    tc_commit(smem_u32(&sfull[q]));
-                }
-                tc_commit(smem_u32(&empty[0]));
-                next(st, phase);
-            }
-            for (int j = 0; j < tiles && ok; ++j, p_phase ^= 1u) {
-                const int v_st = st;
-                const uint32_t v_phase = phase;
-                next(st, phase);
-                const bool more = j + 1 < tiles;
-                const int rows = more ? 8 : (end_valid + 15) >> 4;
-                if (!(ok = wait(&full[v_st], v_phase))) break;
-                for (int q = 0; q < nq; ++q) {
-                    if (!(ok = wait(&pready[q], p_phase))) break;
-                    if (more && q == 0 && !(ok = wait(&full[st], phase))) break;
+                at_mma_head<DP, kAtRows>(tmem + q * 128, s_q + q * S::kTile, stage(2 * i), id_s, steps);
+                tc_commit(smem_u32(&sfull[q]));
+                if (q + 1 == nq) release(2 * i);
+            };
+            for (int q = 0; q < nq; ++q) scores(q, 0);
+            for (int i = 0; i < tiles && ok; ++i)
+                for (int q = 0; q < nq && ok; ++q) {                 // p v of tile i, then the next scores over p
+                    if (!(ok = wait(&pready[q], i & 1) && landed(2 * i + 1))) break;
                     tc_fence_after();
-                    at_mma_rows(tmem + S::kAcc + q * DP, tmem + q * 128, 0, s_ring + v_st * S::kTile, id_o, rows, j > 0);
-                    if (more) at_mma_head<DP>(tmem + q * 128, s_q + q * S::kTile, s_ring + st * S::kTile, id_s, steps);
-                    tc_commit(smem_u32(&sfull[q]));
+                    at_mma_rows<128, kAtRows>(tmem + S::kAcc + q * DP, tmem + q * 128, stage(2 * i + 1), id_o,
+                                              i + 1 < tiles ? 8 : (end_valid + 15) >> 4, i > 0);
+                    tc_commit(smem_u32(&odone[q]));
+                    if (q + 1 == nq) release(2 * i + 1);
+                    if (i + 1 < tiles) scores(q, i + 1);
                 }
-                if (!ok) break;
-                tc_commit(smem_u32(&empty[v_st]));
-                if (more) {
-                    tc_commit(smem_u32(&empty[st]));
-                    next(st, phase);
-                }
-            }
         }
+    }
     } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" :: "n"(S::kRegs));
         // ------------------------------------------------------------------ softmax: a thread a row
         const int q = warp >> 2, row = tid & 127;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
@@ -198,8 +453,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 tc_fence_after();
                 if (some) {
                     f32x2 x[64];
-#pragma unroll
-                    for (int g = 0; g < 4; ++g) lt_load32(t_s + g * 32, *reinterpret_cast<f32x2(*)[16]>(x + g * 16));
+                    at_load(t_s, x);
                     const int key0 = (first + j) * kAtRows;
                     if (key0 + kAtRows > seen_all) {
                         const int left = seen - key0;
@@ -213,16 +467,16 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
 #pragma unroll
                     for (int i = 0; i < 64; ++i) {
                         const float2 f = unpack_f32x2(x[i]);
-                        big[i & 3] = fmaxf(big[i & 3], fmaxf(f.x, f.y));
+                        big[i & 3] = max3_nan(big[i & 3], f.x, f.y);
                     }
-                    const float now = fmaxf(fmaxf(big[0], big[1]), fmaxf(big[2], big[3]));
-                    // a maximum that has grown by more than the slack (from -inf: by any amount) is taken over
-                    const bool grown = (now - top) * a.c > kAfSlack;
+                    const float now = max3_nan(max3_nan(big[0], big[1], big[2]), big[3], big[3]);
+                    // a maximum that has grown by more than the slack (from -inf: by any amount), or is NaN, is taken over
+                    const bool grown = !((now - top) * a.c <= kAfSlack) && now != -INFINITY;
                     if (__any_sync(0xffffffffu, grown)) {
                         const float down = grown ? ex2_approx((top - now) * a.c) : 1.f;
                         if (grown) top = now;
                         sum *= down;
-                        if (j > 0) {                                 // every product that wrote out is done: s came after it
+                        if (j > 0) {                                 // the products before are done: s came after them
                             const f32x2 d2 = pack_f32x2(down, down);
 #pragma unroll 1
                             for (int c = 0; c < DP; c += 32) {
@@ -230,7 +484,8 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                                 lt_load32(t_o + c, o);
 #pragma unroll
                                 for (int i = 0; i < 16; ++i) o[i] = mul2(o[i], d2);
-                                tmem_st32(t_o + c, *reinterpret_cast<const uint32_t(*)[32]>(o));
+                                tmem_st16(t_o + c, reinterpret_cast<const uint32_t *>(o));
+                                tmem_st16(t_o + c + 16, reinterpret_cast<const uint32_t *>(o + 8));
                             }
                         }
                     }
@@ -238,16 +493,16 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     const f32x2 c2 = pack_f32x2(a.c, a.c), s2 = pack_f32x2(shift, shift);
                     f32x2 add[2] = {pack_f32x2(0.f, 0.f), pack_f32x2(0.f, 0.f)};
 #pragma unroll
-                    for (int g = 0; g < 2; ++g) {
-                        uint32_t w[32];
+                    for (int g = 0; g < 4; ++g) {
+                        uint32_t w[16];
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            const float2 f = unpack_f32x2(fma2(x[g * 32 + i], c2, s2));
-                            const float p0 = ex2_approx(f.x), p1 = ex2_approx(f.y);
-                            add[i & 1] = add2(add[i & 1], pack_f32x2(p0, p1));
-                            w[i] = lt_pack<T>(p0, p1);
+                        for (int i = 0; i < 16; ++i) {
+                            const f32x2 e = at_exp2(fma2(x[g * 16 + i], c2, s2));
+                            const float2 f = unpack_f32x2(e);
+                            add[i & 1] = add2(add[i & 1], e);
+                            w[i] = lt_pack<T>(f.x, f.y);
                         }
-                        tmem_st32(t_s + g * 32, w);
+                        tmem_st16(t_s + g * 16, w);
                     }
                     const float2 f = unpack_f32x2(add2(add[0], add[1]));
                     sum += f.x + f.y;
@@ -257,59 +512,10 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&pready[q]));
             }
-            if (tiles > 0 && ok) ok = __all_sync(0xffffffffu, wait(&sfull[q], phase)) != 0;    // the last p v
+            if (tiles > 0 && ok) ok = __all_sync(0xffffffffu, wait(&odone[q], (tiles - 1) & 1)) != 0;     // the last p v
             tc_fence_after();
-            if (ok && some) {
-                const int64_t all = (int64_t)a.M * a.H, at = (int64_t)(s.q0 + token) * a.H + head0 + (row & (P - 1));
-                const bool none = seen == 0;
-                float *part = nullptr;
-                float inv = none ? 0.f : 1.f / sum;
-                if (a.splits > 1) {
-                    part = a.partial + (blockIdx.z * all + at) * a.D;
-                    inv = 1.f;
-                    if (mine) a.part_ml[blockIdx.z * all + at] = make_float2(top * a.c, sum);
-                } else if (mine && a.lse) {
-                    a.lse[at] = none ? INFINITY : fmaf(top, a.c, log2f(sum));
-                }
-                T *out = (T *)a.out + at * a.D;
-                const bool wide = (a.D & 7) == 0 && ((uintptr_t)a.out & 15) == 0;
-#pragma unroll 1
-                for (int c = 0; c < a.D; c += 32) {
-                    f32x2 o[16];
-                    if (tiles > 0) {
-                        lt_load32(t_o + c, o);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) o[i] = pack_f32x2(0.f, 0.f);
-                    }
-                    if (!mine || (part && tiles == 0)) continue;
-#pragma unroll
-                    for (int v = 0; v < 4; ++v) {
-                        if (c + v * 8 >= a.D) break;
-                        uint32_t w[4];
-                        float f[8];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float2 u = unpack_f32x2(o[v * 4 + i]);
-                            f[2 * i] = none ? 0.f : u.x * inv;
-                            f[2 * i + 1] = none ? 0.f : u.y * inv;
-                            w[i] = lt_pack<T>(f[2 * i], f[2 * i + 1]);
-                        }
-                        const int d = c + v * 8;
-                        if (part) {
-#pragma unroll
-                            for (int i = 0; i < 8; ++i)
-                                if (d + i < a.D) part[d + i] = f[i];
-                        } else if (wide) {
-                            *(uint4 *)(out + d) = make_uint4(w[0], w[1], w[2], w[3]);
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < 8; ++i)
-                                if (d + i < a.D) out[d + i] = dtype_traits<T>::from_f(f[i]);
-                        }
-                    }
-                }
-            }
+            if (ok && some)
+                af_store<T>(a, t_o, DP, (int64_t)(s.q0 + token) * a.H + head0 + (row & (P - 1)), mine, seen == 0, tiles == 0, top, sum);
         }
     }
 
@@ -323,36 +529,37 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         __syncthreads();
     }
     tc_fence_after();
-    if (warp == kWarpMma) tmem_dealloc(tmem, S::kColumns);
+    if (warp == S::kWarpMma) tmem_dealloc(tmem, 512);
 }
 
-template <typename T, int NQ, int DP>
-static int af_run(const AtArgs &a) {
-    using S = AfShape<NQ, DP>;
+template <typename T, typename S, bool PAIR, typename K>
+static int af_run(const AtArgs &a, K kern, int keys, std::atomic<uint64_t> &done) {
     const int G = a.H / a.K;
     int log_p = 0;
     while (log_p < 7 && G % (2 << log_p) == 0) ++log_p;
     const int P = 1 << log_p, tokens = kAtRows >> log_p;
     CUtensorMap mq, mk, mv;
-    if (!at_map(&mq, a.q, a.M, a.H, a.D, P, tokens) || !at_map(&mk, a.k, a.N, a.K, a.D, 1, kAtRows) ||
-        !at_map(&mv, a.v, a.N, a.K, a.D, 1, kAtRows))
+    if (!at_map(&mq, a.q, a.M, a.H, a.D, P, tokens) || !at_map(&mk, a.k, a.N, a.K, a.D, 1, keys) ||
+        !at_map(&mv, a.v, a.N, a.K, a.D, 1, keys))
         return SPCONV_ERR_CUDA;
-    static std::atomic<uint64_t> done;
-    auto kern = attention_tc_kernel<T, NQ, DP>;
-    constexpr int smem = S::kSmem > S::kSmemLeast ? S::kSmem : S::kSmemLeast;
+    // no more CTAs than the SM's 512 columns serve
+    constexpr int least = S::kSmemLeast, smem = S::kSmem > least ? S::kSmem : least;
     if (allow_smem(kern, smem, done) != cudaSuccess) return check_launch("attention: shared memory");
-    kern<<<dim3((unsigned)at_tiles(a.M, a.B, NQ * tokens), a.H / P, a.splits), S::kThreads, smem, a.stream>>>(mq, mk, mv, a, log_p);
+    const dim3 grid((unsigned)at_tiles(a.M, a.B, (PAIR ? 2 : 1) * tokens), a.H / P, a.splits);
+    kern<<<grid, S::kThreads, smem, a.stream>>>(mq, mk, mv, a, log_p);
     return check_launch("attention_tc_kernel");
 }
 
 template <typename T>
-static int af_shape(const AtArgs &a, int tiles2) {
-    if (a.D <= 64) return tiles2 ? af_run<T, 2, 64>(a) : af_run<T, 1, 64>(a);
-    return tiles2 ? af_run<T, 2, 128>(a) : af_run<T, 1, 128>(a);
+static int af_type(const AtArgs &a, bool pair) {
+    static std::atomic<uint64_t> done[3];
+    if (a.D <= 64) return af_run<T, AfShape<64>, false>(a, attention_tc_kernel<T, 64>, AfShape<64>::kKeys, done[0]);
+    if (!pair) return af_run<T, AfShape<128>, false>(a, attention_tc_kernel<T, 128>, AfShape<128>::kKeys, done[1]);
+    return af_run<T, ApShape, true>(a, attention_tc_pair_kernel<T>, kAtRows, done[2]);
 }
 
-int launch_at_tc_forward(const AtArgs &a, int tiles2) {
-    return a.dtype == SPCONV_F16 ? af_shape<__half>(a, tiles2) : af_shape<__nv_bfloat16>(a, tiles2);
+int launch_at_tc_forward(const AtArgs &a, bool pair) {
+    return a.dtype == SPCONV_F16 ? af_type<__half>(a, pair) : af_type<__nv_bfloat16>(a, pair);
 }
 
 }  // namespace spconv
