@@ -1070,54 +1070,66 @@ def _heads(t: torch.Tensor, what: str) -> torch.Tensor:
     return t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous()
 
 
+@functools.lru_cache(maxsize=256)
+def _rotary_args(dtype: torch.dtype, layout: str, heads: int, key_heads: int, size: int, rotary_dim: int, axes: int,
+                 steps: Tuple[float, ...], amplitude: float, inverse: bool) -> RotaryArgs:
+    """The checked arguments of a call but for its rows and tensors; calls take copies."""
+    if dtype not in DTYPE_CODES:
+        raise TypeError(f"unsupported dtype {dtype}")
+    if layout not in ROTARY_LAYOUTS:
+        raise ValueError(f"unsupported layout {layout}")
+    if not 2 <= size <= 2 * ROTARY_MAX_PAIRS:
+        raise ValueError(f"head size must be in [2, {2 * ROTARY_MAX_PAIRS}], got {size}")
+    a = RotaryArgs(dtype=DTYPE_CODES[dtype], layout=ROTARY_LAYOUTS[layout], heads=heads, key_heads=key_heads, head_size=size,
+                   rotary_dim=rotary_dim, axes=axes, inverse=inverse, amplitude=amplitude)
+    ctypes.memmove(ctypes.addressof(a) + RotaryArgs.steps.offset, _turn_steps(steps), RotaryArgs.steps.size)
+    return a
+
+
 @_on_device
 def _rotary_on(first: torch.Tensor, query, key, positions: torch.Tensor, layout: str, rotary_dim: int,
                steps: Tuple[float, ...], amplitude: float, inverse: bool) -> tuple:
     dev = _require_cuda(first, query, key, positions)
-    if first.dtype not in DTYPE_CODES:
-        raise TypeError(f"unsupported dtype {first.dtype}")
-    if layout not in ROTARY_LAYOUTS:
-        raise ValueError(f"unsupported layout {layout}")
+    dtype, (rows, _, size) = first.dtype, first.shape
     if positions.dtype != torch.int32:
         raise TypeError(f"positions must be int32, got {positions.dtype}")
-    rows, size = first.shape[0], first.shape[2]
     if positions.dim() == 1:
         positions = positions[:, None]
     if positions.dim() != 2 or positions.shape[0] != rows:
         raise ValueError(f"positions must have shape [{rows}] or [{rows}, axes], got {list(positions.shape)}")
-    if not 2 <= size <= 2 * ROTARY_MAX_PAIRS:
-        raise ValueError(f"head size must be in [2, {2 * ROTARY_MAX_PAIRS}], got {size}")
-    a = RotaryArgs(dtype=DTYPE_CODES[first.dtype], layout=ROTARY_LAYOUTS[layout], num_rows=rows, head_size=size,
-                   rotary_dim=rotary_dim, axes=positions.shape[1], inverse=inverse, amplitude=amplitude,
-                   positions=positions.data_ptr(), position_row=positions.stride(0), position_col=positions.stride(1))
-    ctypes.memmove(ctypes.addressof(a) + RotaryArgs.steps.offset, _turn_steps(steps), RotaryArgs.steps.size)
-    out = [None, None]
-    kept = []                                 # copies live until the launch
-    for i, (t, what) in enumerate(((query, "query"), (key, "key"))):
-        if t is None:
-            continue
-        if t.dtype != first.dtype:
-            raise TypeError(f"{what} dtype {t.dtype} differs from {first.dtype}")
-        t = _heads(t, what)
-        if t.shape[0] != rows or t.shape[2] != size:
-            raise ValueError(f"{what} must have shape [{rows}, heads, {size}], got {list(t.shape)}")
-        kept.append(t)
-        out[i] = torch.empty(t.shape, dtype=t.dtype, device=dev)
-        if i == 0:
-            a.heads, a.query, a.query_out = t.shape[1], t.data_ptr(), out[0].data_ptr()
-            a.query_row, a.query_head = t.stride(0), t.stride(1)
-        else:
-            a.key_heads, a.key, a.key_out = t.shape[1], t.data_ptr(), out[1].data_ptr()
-            a.key_row, a.key_head = t.stride(0), t.stride(1)
-    if rows == 0 or a.heads + a.key_heads == 0:
-        return tuple(out)
-    index = dev.index
+    heads = key_heads = 0
+    query_out = key_out = None
+    if query is not None:                    # copies live until the launch
+        query = _heads(query, "query")
+        heads = query.shape[1]
+        query_out = torch.empty(query.shape, dtype=dtype, device=dev)
+    if key is not None:
+        key = _heads(key, "key")
+        if key.dtype != dtype:
+            raise TypeError(f"key dtype {key.dtype} differs from {dtype}")
+        if key.shape[0] != rows or key.shape[2] != size:
+            raise ValueError(f"key must have shape [{rows}, heads, {size}], got {list(key.shape)}")
+        key_heads = key.shape[1]
+        key_out = torch.empty(key.shape, dtype=dtype, device=dev)
+    a = RotaryArgs.from_buffer_copy(_rotary_args(dtype, layout, heads, key_heads, size, rotary_dim, positions.shape[1], steps,
+                                                 amplitude, inverse))
+    if rows == 0 or heads + key_heads == 0:
+        return query_out, key_out
+    a.num_rows, a.positions = rows, positions.data_ptr()
+    a.position_row, a.position_col = positions.stride()
+    if heads:
+        a.query, a.query_out = query.data_ptr(), query_out.data_ptr()
+        a.query_row, a.query_head, _ = query.stride()
+    if key_heads:
+        a.key, a.key_out = key.data_ptr(), key_out.data_ptr()
+        a.key_row, a.key_head, _ = key.stride()
+    index = first.get_device()
     mapped_status(index)
     rc = (_lib or load_library()).spconv_rotary(a, _raw_stream(index))
     if rc != SPCONV_OK:
         _raise(rc, "spconv_rotary")
     after_mapped_launch(index)
-    return tuple(out)
+    return query_out, key_out
 
 
 def rotary(query: Optional[torch.Tensor], key: Optional[torch.Tensor], positions: torch.Tensor, layout: str,
@@ -1128,9 +1140,9 @@ def rotary(query: Optional[torch.Tensor], key: Optional[torch.Tensor], positions
 
 
 def _offsets(t: torch.Tensor, what: str) -> int:
-    if t.dtype != torch.int32 or t.dim() != 1 or t.numel() < 2 or not t.is_contiguous():
+    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] < 2 or not t.is_contiguous():
         raise ValueError(f"{what} must be a contiguous [samples + 1] int32 tensor")
-    return t.numel() - 1
+    return t.shape[0] - 1
 
 
 def _attention_workspace(a: AttentionArgs, backward: bool, device: torch.device) -> Optional[torch.Tensor]:
@@ -1142,38 +1154,47 @@ def _attention_workspace(a: AttentionArgs, backward: bool, device: torch.device)
     return ws
 
 
+@functools.lru_cache(maxsize=256)
+def _attention_args(dtype: torch.dtype, heads: int, key_heads: int, size: int, causal: bool, scale: float, kernel: int) -> AttentionArgs:
+    """The checked arguments of a call but for its rows and tensors; calls take copies."""
+    if dtype not in DTYPE_CODES:
+        raise TypeError(f"unsupported dtype {dtype}")
+    if key_heads < 1 or heads < key_heads or heads % key_heads:
+        raise ValueError(f"{heads} query heads are no multiple of {key_heads} key heads")
+    if not 1 <= size <= 256:
+        raise ValueError(f"head size must be in [1, 256], got {size}")
+    if not (scale > 0.0 and scale < float("inf")):
+        raise ValueError(f"scale must be positive and finite, got {scale}")
+    return AttentionArgs(dtype=DTYPE_CODES[dtype], kernel=kernel, num_samples=1, heads=heads, key_heads=key_heads, head_size=size,
+                         causal=causal, scale=scale)
+
+
 @_on_device
 def attention_forward(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, offsets: Optional[torch.Tensor],
                       key_offsets: Optional[torch.Tensor], causal: bool, scale: float, keep_stats: bool = False,
                       kernel: int = KERNEL_AUTO) -> tuple:
     """(out, row statistics if ``keep_stats`` else None, the call's arguments for attention_backward_of)."""
     dev = _require_cuda(query, key, value, offsets, key_offsets)
-    if query.dtype not in DTYPE_CODES:
-        raise TypeError(f"unsupported dtype {query.dtype}")
-    for t, what in ((key, "key"), (value, "value")):
-        if t.dtype != query.dtype:
-            raise TypeError(f"{what} dtype {t.dtype} differs from the query's {query.dtype}")
+    dtype = query.dtype
+    if key.dtype != dtype or value.dtype != dtype:
+        raise TypeError(f"key and value dtypes {key.dtype} and {value.dtype} differ from the query's {dtype}")
     query, key, value = _heads(query, "query"), _heads(key, "key"), _heads(value, "value")
     M, H, D = query.shape
-    N, K, _ = key.shape
-    if key.shape != value.shape or key.shape[2] != D:
+    N, K, size = key.shape
+    if key.shape != value.shape or size != D:
         raise ValueError(f"key and value must have shape [keys, key heads, {D}], got {list(key.shape)} and {list(value.shape)}")
-    if K < 1 or H < K or H % K:
-        raise ValueError(f"{H} query heads are no multiple of {K} key heads")
-    if not 1 <= D <= 256:
-        raise ValueError(f"head size must be in [1, 256], got {D}")
-    if not (scale > 0.0 and scale < float("inf")):
-        raise ValueError(f"scale must be positive and finite, got {scale}")
-    samples = 1 if offsets is None else _offsets(offsets, "batch_offsets")
-    if key_offsets is not None and _offsets(key_offsets, "key_offsets") != samples:
-        raise ValueError("batch_offsets and key_offsets must have the same number of samples")
+    a = AttentionArgs.from_buffer_copy(_attention_args(dtype, H, K, D, bool(causal), float(scale), kernel))
+    a.num_queries, a.num_keys = M, N
+    if offsets is not None:
+        a.num_samples, a.offsets = _offsets(offsets, "batch_offsets"), offsets.data_ptr()
+    if key_offsets is not None:
+        if key_offsets is not offsets and _offsets(key_offsets, "key_offsets") != a.num_samples:
+            raise ValueError("batch_offsets and key_offsets must have the same number of samples")
+        a.key_offsets = key_offsets.data_ptr()
+    a.query, a.key, a.value = query.data_ptr(), key.data_ptr(), value.data_ptr()
+    (a.query_row, a.query_head, _), (a.key_row, a.key_head, _), (a.value_row, a.value_head, _) = (
+        query.stride(), key.stride(), value.stride())
     index = dev.index
-    a = AttentionArgs(dtype=DTYPE_CODES[query.dtype], kernel=kernel, num_queries=M, num_keys=N, num_samples=samples,
-                      heads=H, key_heads=K, head_size=D, causal=bool(causal), scale=scale,
-                      offsets=_ptr(offsets), key_offsets=_ptr(key_offsets),
-                      query=query.data_ptr(), key=key.data_ptr(), value=value.data_ptr(),
-                      query_row=query.stride(0), query_head=query.stride(1), key_row=key.stride(0),
-                      key_head=key.stride(1), value_row=value.stride(0), value_head=value.stride(1))
     out = torch.empty((M, H, D), dtype=query.dtype, device=dev)
     a.out = out.data_ptr()
     stats = None
