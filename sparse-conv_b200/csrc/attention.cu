@@ -143,9 +143,23 @@ struct AtPlan {
     int64_t pack_at[4], delta_at, ml_at, partial_at, bytes;
 };
 
-static int at_cut(int64_t ctas, int64_t slots, int64_t tiles, int least) {
-    if (ctas == 0 || ctas >= slots) return 1;
-    return (int)std::max<int64_t>(1, std::min<int64_t>({slots / ctas, tiles / least, 256}));
+// Splits of `tiles` steps each of `ctas` CTAs, of which `slots` run at a time, none of fewer than `least` steps. The
+// tensor-core kernels are cut only where CTAs do not fill the slots (a split's rows are written and read once more in fp32:
+// 4,096 tokens x 8 heads in 256 CTAs for 592 slots: 94 us whole, 126 us in two), the CUDA-core kernels, whose steps take as long as
+// a row's joining, also into whole waves.
+static int at_cut(int64_t ctas, int64_t slots, int64_t tiles, int least, bool waves) {
+    if (ctas == 0 || ctas >= (waves ? 4 : 1) * slots) return 1;
+    const int64_t most = std::max<int64_t>(1, std::min<int64_t>({tiles / least, (waves ? 4 : 1) * slots / ctas, 256}));
+    if (!waves) return (int)most;
+    int64_t best = 1, best_cost = INT64_MAX;
+    for (int64_t s = 1; s <= most; ++s) {
+        const int64_t cost = ((ctas * s + slots - 1) / slots) * ((tiles + s - 1) / s + (s > 1 ? 6 : 2));
+        if (cost < best_cost) {
+            best_cost = cost;
+            best = s;
+        }
+    }
+    return (int)best;
 }
 
 static AtPlan at_plan(const spconv_attention_args *q, bool backward) {
@@ -162,12 +176,12 @@ static AtPlan at_plan(const spconv_attention_args *q, bool backward) {
         p.pair = !backward && q->head_size > 64 && rows > 192 && mean_k > 512 && B * up(rows, 256) * heads >= 148;
         // CTAs that run at a time, and what each has to have for itself: 512 keys (a split's rows are written and read once more)
         const int64_t per_sm = q->head_size > 64 ? 1 : 2;
-        p.splits[0] = at_cut(B * up(rows, 128) * heads, 148 * (backward ? per_sm : 2 * per_sm), up(mean_k, 128), 8);
-        p.splits[1] = at_cut(B * up(mean_k, 128) * q->key_heads, 148 * per_sm, up(rows, 128) * (G / P), 8);
+        p.splits[0] = at_cut(B * up(rows, 128) * heads, 148 * (backward ? per_sm : 2 * per_sm), up(mean_k, 128), 8, false);
+        p.splits[1] = at_cut(B * up(mean_k, 128) * q->key_heads, 148 * per_sm, up(rows, 128) * (G / P), 8, false);
     } else {
         const int64_t R = at_simt_rows(q->head_size);
-        p.splits[0] = at_cut(B * up(mean_q, R) * q->heads, 296, up(mean_k, R), 2);
-        p.splits[1] = at_cut(B * up(mean_k, R) * q->key_heads, 296, up(mean_q, R) * G, 2);
+        p.splits[0] = at_cut(B * up(mean_q, R) * q->heads, 296, up(mean_k, R), 4, true);
+        p.splits[1] = at_cut(B * up(mean_k, R) * q->key_heads, 296, up(mean_q, R) * G, 4, true);
     }
     int64_t at = 0;
     auto take = [&](int64_t bytes) {

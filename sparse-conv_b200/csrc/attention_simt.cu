@@ -12,6 +12,7 @@
 // Bound: the FMA pipe.
 #include <algorithm>
 
+#include "activation.cuh"
 #include "attention_common.cuh"
 
 namespace spconv {
@@ -25,6 +26,7 @@ struct AsShape {
     static constexpr int C = DP / 16;                    // head columns of a thread
     static constexpr int LD = DP + 4, LP = BM + 4;
     static constexpr int kTile = BM * LD, kScores = BM * LP;
+    static constexpr int kPerSm = DP <= 64 ? 2 : 1;      // blocks, by shared memory
 };
 
 // Rows [row0, row0 + valid) of a head into a tile, zeros behind them and behind the head's end.
@@ -38,12 +40,24 @@ __device__ __forceinline__ void as_load(float *dst, const AtTensor &t, int64_t r
     }
 }
 
-// acc[i][j] += a[4 ty + i][.] . b[tx + 16 j][.]
+// Two products a slot (fma.rn.f32x2): the pipe's rate is the same, but the loads between them find slots.
+__device__ __forceinline__ f32x2 as_pair(const float *p) { return *reinterpret_cast<const f32x2 *>(p); }
+__device__ __forceinline__ float as_sum(f32x2 x) {
+    const float2 f = unpack_f32x2(x);
+    return f.x + f.y;
+}
+
+// acc[i][j] = a[4 ty + i][.] . b[tx + 16 j][.]
 template <int DP>
 __device__ __forceinline__ void as_dot(const float *a, const float *b, float (&acc)[AsShape<DP>::R][AsShape<DP>::R]) {
     using S = AsShape<DP>;
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
     const float *pa = a + ty * S::R * S::LD, *pb = b + tx * S::LD;
+    f32x2 sum[S::R][S::R];
+#pragma unroll
+    for (int i = 0; i < S::R; ++i)
+#pragma unroll
+        for (int j = 0; j < S::R; ++j) sum[i][j] = pack_f32x2(0.f, 0.f);
 #pragma unroll 4
     for (int d = 0; d < DP; d += 4) {
         float4 x[S::R], y[S::R];
@@ -54,51 +68,64 @@ __device__ __forceinline__ void as_dot(const float *a, const float *b, float (&a
 #pragma unroll
         for (int i = 0; i < S::R; ++i)
 #pragma unroll
-            for (int j = 0; j < S::R; ++j)
-                acc[i][j] = fmaf(x[i].x, y[j].x, fmaf(x[i].y, y[j].y, fmaf(x[i].z, y[j].z, fmaf(x[i].w, y[j].w, acc[i][j]))));
+            for (int j = 0; j < S::R; ++j) {
+                sum[i][j] = fma2(as_pair(&x[i].x), as_pair(&y[j].x), sum[i][j]);
+                sum[i][j] = fma2(as_pair(&x[i].z), as_pair(&y[j].z), sum[i][j]);
+            }
     }
+#pragma unroll
+    for (int i = 0; i < S::R; ++i)
+#pragma unroll
+        for (int j = 0; j < S::R; ++j) acc[i][j] = as_sum(sum[i][j]);
 }
 
-// acc[i][j] += sum_k p[4 ty + i][k] b[k][tx + 16 j], k < BM
+// acc[i][j] += sum_k p[4 ty + i][k] b[k][tx + 16 j], k < BM, the even and the odd k apart
 template <int DP>
-__device__ __forceinline__ void as_rows(const float *p, const float *b, float (&acc)[AsShape<DP>::R][AsShape<DP>::C]) {
+__device__ __forceinline__ void as_rows(const float *p, const float *b, f32x2 (&acc)[AsShape<DP>::R][AsShape<DP>::C]) {
     using S = AsShape<DP>;
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
     const float *pp = p + ty * S::R * S::LP, *pb = b + tx;
 #pragma unroll 2
     for (int k = 0; k < S::BM; k += 4) {
-        float x[S::R][4];
+        float4 x[S::R];
 #pragma unroll
-        for (int i = 0; i < S::R; ++i) *(float4 *)x[i] = *(const float4 *)(pp + i * S::LP + k);
+        for (int i = 0; i < S::R; ++i) x[i] = *(const float4 *)(pp + i * S::LP + k);
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
+        for (int j = 0; j < S::C; ++j) {
+            const float *q = pb + k * S::LD + 16 * j;
+            const f32x2 y0 = pack_f32x2(q[0], q[S::LD]), y1 = pack_f32x2(q[2 * S::LD], q[3 * S::LD]);
 #pragma unroll
-            for (int j = 0; j < S::C; ++j) {
-                const float y = pb[(k + e) * S::LD + 16 * j];
-#pragma unroll
-                for (int i = 0; i < S::R; ++i) acc[i][j] = fmaf(x[i][e], y, acc[i][j]);
-            }
+            for (int i = 0; i < S::R; ++i) acc[i][j] = fma2(as_pair(&x[i].z), y1, fma2(as_pair(&x[i].x), y0, acc[i][j]));
+        }
     }
 }
 
-// acc[i][j] += sum_q p[q][4 ty + i] b[q][tx + 16 j], q < BM
+// acc[i][j] += sum_q p[q][4 ty + i] b[q][tx + 16 j], q < BM: the even and the odd q apart
 template <int DP>
-__device__ __forceinline__ void as_cols(const float *p, const float *b, float (&acc)[AsShape<DP>::R][AsShape<DP>::C]) {
+__device__ __forceinline__ void as_cols(const float *p, const float *b, f32x2 (&acc)[AsShape<DP>::R][AsShape<DP>::C]) {
     using S = AsShape<DP>;
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
     const float *pp = p + ty * S::R, *pb = b + tx;
 #pragma unroll 4
-    for (int q = 0; q < S::BM; ++q) {
-        float x[S::R];
+    for (int q = 0; q < S::BM; q += 2) {
+        f32x2 x[S::R];
 #pragma unroll
-        for (int i = 0; i < S::R; ++i) x[i] = pp[q * S::LP + i];
+        for (int i = 0; i < S::R; ++i) x[i] = pack_f32x2(pp[q * S::LP + i], pp[(q + 1) * S::LP + i]);
 #pragma unroll
         for (int j = 0; j < S::C; ++j) {
-            const float y = pb[q * S::LD + 16 * j];
+            const f32x2 y = pack_f32x2(pb[q * S::LD + 16 * j], pb[(q + 1) * S::LD + 16 * j]);
 #pragma unroll
-            for (int i = 0; i < S::R; ++i) acc[i][j] = fmaf(x[i], y, acc[i][j]);
+            for (int i = 0; i < S::R; ++i) acc[i][j] = fma2(x[i], y, acc[i][j]);
         }
     }
+}
+
+template <int R, int C>
+__device__ __forceinline__ void as_clear(f32x2 (&acc)[R][C]) {
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+        for (int j = 0; j < C; ++j) acc[i][j] = pack_f32x2(0.f, 0.f);
 }
 
 // This block's sample, found by its first warp.
@@ -113,7 +140,7 @@ __device__ __forceinline__ AtSample as_sample(const AtArgs &a, const int32_t *by
 }
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(kAsThreads)
+__global__ void __launch_bounds__(kAsThreads, AsShape<DP>::kPerSm)
 attention_simt_kernel(const __grid_constant__ AtArgs a) {
     using S = AsShape<DP>;
     extern __shared__ __align__(16) float smem[];
@@ -127,7 +154,9 @@ attention_simt_kernel(const __grid_constant__ AtArgs a) {
     int first, last;
     at_split(a.splits, blockIdx.z, (at_seen(a, s.tile * S::BM + rows - 1, n, m) + S::BM - 1) / S::BM, first, last);
     as_load<T, DP>(sq, a.q, row0, rows, h, a.D);
-    float acc[S::R][S::C] = {}, top[S::R], sum[S::R] = {};
+    f32x2 acc[S::R][S::C];
+    float top[S::R], sum[S::R] = {};
+    as_clear(acc);
 #pragma unroll
     for (int i = 0; i < S::R; ++i) top[i] = -INFINITY;
     for (int t = first; t < last; ++t) {
@@ -136,7 +165,7 @@ attention_simt_kernel(const __grid_constant__ AtArgs a) {
         as_load<T, DP>(sk, a.k, s.k0 + key0, valid, kh, a.D);
         as_load<T, DP>(sv, a.v, s.k0 + key0, valid, kh, a.D);
         __syncthreads();
-        float x[S::R][S::R] = {};
+        float x[S::R][S::R];
         as_dot<DP>(sq, sk, x);
 #pragma unroll
         for (int i = 0; i < S::R; ++i) {
@@ -161,7 +190,7 @@ attention_simt_kernel(const __grid_constant__ AtArgs a) {
             }
             sum[i] = sum[i] * down + add;
 #pragma unroll
-            for (int j = 0; j < S::C; ++j) acc[i][j] *= down;
+            for (int j = 0; j < S::C; ++j) acc[i][j] = mul2(acc[i][j], pack_f32x2(down, down));
         }
         __syncwarp();                                          // a row's p are of its own 16 lanes
         as_rows<DP>(sp, sv, acc);
@@ -179,14 +208,14 @@ attention_simt_kernel(const __grid_constant__ AtArgs a) {
             if (tx == 0) a.part_ml[blockIdx.z * all + at] = make_float2(top[i], sum[i]);
 #pragma unroll
             for (int j = 0; j < S::C; ++j)
-                if (tx + 16 * j < a.D) a.partial[(blockIdx.z * all + at) * a.D + tx + 16 * j] = acc[i][j];
+                if (tx + 16 * j < a.D) a.partial[(blockIdx.z * all + at) * a.D + tx + 16 * j] = as_sum(acc[i][j]);
             continue;
         }
         if (tx == 0 && a.lse) a.lse[at] = none ? INFINITY : top[i] + log2f(sum[i]);
         const float inv = 1.f / sum[i];
 #pragma unroll
         for (int j = 0; j < S::C; ++j)
-            if (tx + 16 * j < a.D) ((T *)a.out)[at * a.D + tx + 16 * j] = dtype_traits<T>::from_f(none ? 0.f : acc[i][j] * inv);
+            if (tx + 16 * j < a.D) ((T *)a.out)[at * a.D + tx + 16 * j] = dtype_traits<T>::from_f(none ? 0.f : as_sum(acc[i][j]) * inv);
     }
 }
 
@@ -199,7 +228,7 @@ __device__ __forceinline__ void as_grads(const AtArgs &a, const float *sq, const
                                          const bool (&single)[AsShape<DP>::R]) {
     using S = AsShape<DP>;
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    float x[S::R][S::R] = {}, y[S::R][S::R] = {};
+    float x[S::R][S::R], y[S::R][S::R];
     as_dot<DP>(sq, sk, x);
     as_dot<DP>(sg, sv, y);
 #pragma unroll
@@ -215,7 +244,7 @@ __device__ __forceinline__ void as_grads(const AtArgs &a, const float *sq, const
 }
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(kAsThreads)
+__global__ void __launch_bounds__(kAsThreads, AsShape<DP>::kPerSm)
 attention_simt_grad_query_kernel(const __grid_constant__ AtArgs a) {
     using S = AsShape<DP>;
     extern __shared__ __align__(16) float smem[];
@@ -230,7 +259,9 @@ attention_simt_grad_query_kernel(const __grid_constant__ AtArgs a) {
     at_split(a.splits, blockIdx.z, (at_seen(a, s.tile * S::BM + rows - 1, n, m) + S::BM - 1) / S::BM, first, last);
     as_load<T, DP>(sq, a.q, row0, rows, h, a.D);
     as_load<T, DP>(sg, a.grad, row0, rows, h, a.D);
-    float acc[S::R][S::C] = {}, lse[S::R], delta[S::R];
+    f32x2 acc[S::R][S::C];
+    float lse[S::R], delta[S::R];
+    as_clear(acc);
 #pragma unroll
     for (int i = 0; i < S::R; ++i) {
         const int r = ty * S::R + i;
@@ -264,7 +295,7 @@ attention_simt_grad_query_kernel(const __grid_constant__ AtArgs a) {
 #pragma unroll
         for (int j = 0; j < S::C; ++j) {
             if (tx + 16 * j >= a.D) continue;
-            const float g = acc[i][j] * a.scale;
+            const float g = as_sum(acc[i][j]) * a.scale;
             if (a.splits > 1) a.partial[(blockIdx.z * (int64_t)a.M * a.H + at) * a.D + tx + 16 * j] = g;
             else ((T *)a.gq)[at * a.D + tx + 16 * j] = dtype_traits<T>::from_f(g);
         }
@@ -272,7 +303,7 @@ attention_simt_grad_query_kernel(const __grid_constant__ AtArgs a) {
 }
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(kAsThreads)
+__global__ void __launch_bounds__(kAsThreads, AsShape<DP>::kPerSm)
 attention_simt_grad_key_kernel(const __grid_constant__ AtArgs a) {
     using S = AsShape<DP>;
     extern __shared__ __align__(16) float smem[];
@@ -290,7 +321,9 @@ attention_simt_grad_key_kernel(const __grid_constant__ AtArgs a) {
     at_split(a.splits, blockIdx.z, tiles * G, first, last);
     as_load<T, DP>(sk, a.k, row0, rows, kh, a.D);
     as_load<T, DP>(sv, a.v, row0, rows, kh, a.D);
-    float gk[S::R][S::C] = {}, gv[S::R][S::C] = {};
+    f32x2 gk[S::R][S::C], gv[S::R][S::C];
+    as_clear(gk);
+    as_clear(gv);
     for (int it = first; it < last; ++it) {
         const int g = it / tiles, t = from + it - g * tiles, h = kh * G + g;
         const int i0 = t * S::BM, valid = min(S::BM, n - i0);
@@ -326,11 +359,11 @@ attention_simt_grad_key_kernel(const __grid_constant__ AtArgs a) {
             const int d = tx + 16 * j;
             if (d >= a.D) continue;
             if (a.splits > 1) {
-                a.partial[((2 * blockIdx.z) * all + at) * a.D + d] = gk[i][j] * a.scale;
-                a.partial[((2 * blockIdx.z + 1) * all + at) * a.D + d] = gv[i][j];
+                a.partial[((2 * blockIdx.z) * all + at) * a.D + d] = as_sum(gk[i][j]) * a.scale;
+                a.partial[((2 * blockIdx.z + 1) * all + at) * a.D + d] = as_sum(gv[i][j]);
             } else {
-                if (a.gk) ((T *)a.gk)[at * a.D + d] = dtype_traits<T>::from_f(gk[i][j] * a.scale);
-                if (a.gv) ((T *)a.gv)[at * a.D + d] = dtype_traits<T>::from_f(gv[i][j]);
+                if (a.gk) ((T *)a.gk)[at * a.D + d] = dtype_traits<T>::from_f(as_sum(gk[i][j]) * a.scale);
+                if (a.gv) ((T *)a.gv)[at * a.D + d] = dtype_traits<T>::from_f(as_sum(gv[i][j]));
             }
         }
     }
