@@ -98,43 +98,62 @@ attention_tc_grad_query_kernel(const __grid_constant__ CUtensorMap map_q, const 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int P = 1 << log_p, tokens = kAtRows >> log_p;
 
+    const int head0 = blockIdx.y << log_p, kh = head0 / (a.H / a.K);
+    auto load = [&](uint32_t dst, int rows, const CUtensorMap *map, int head, int row, uint32_t mbar) {
+        for (int c = 0; c < DP / 64; ++c) tma_load_3d(dst + c * rows * 128, map, c * 64, head, row, mbar);
+    };
+    // what a sample gives the CTA
+    AtSample s;
+    int n, m, t0, first, last, tiles, end_valid;
+    auto share = [&] {
+        n = s.q1 - s.q0;
+        m = s.k1 - s.k0;
+        t0 = s.tile * tokens;
+        const int seen_last = at_seen(a, min(n, t0 + tokens) - 1, n, m);
+        at_split(a.splits, blockIdx.z, (seen_last + W - 1) / W, first, last);
+        tiles = s.tile < 0 || t0 >= n ? -1 : last - first;           // -1: nothing to do at all
+        end_valid = min(W, seen_last - (last - 1) * W);
+    };
+
     at_check_offsets(a);
-    if (warp == S::kWarpLoad) {
-        const AtSample s = at_find(a.offsets, a.M, a, a.causal ? gridDim.x - 1 - blockIdx.x : blockIdx.x, tokens);
+    if (warp == S::kWarpLoad) {                                      // up to the first loads by this warp alone
+        if (elect_one()) {
+            for (const CUtensorMap *map : {&map_q, &map_k, &map_v, &map_g}) tma_prefetch_desc(map);
+            for (int i = 0; i < S::kK; ++i) {
+                mbar_init(smem_u32(&kfull[i]), 1);
+                mbar_init(smem_u32(&kempty[i]), 1);
+            }
+            for (int i = 0; i < S::kV; ++i) {
+                mbar_init(smem_u32(&vfull[i]), 1);
+                mbar_init(smem_u32(&vempty[i]), 1);
+            }
+            for (uint64_t *b : {qfull, tail, sfull, sfull + 1, dpfull, finished}) mbar_init(smem_u32(b), 1);
+            mbar_init(smem_u32(dsready), S::kWarps);
+            *s_abort = 0;
+            asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+        }
+        __syncwarp();
+        s = at_find(a.offsets, a.M, a, a.causal ? gridDim.x - 1 - blockIdx.x : blockIdx.x, tokens);
+        share();
         if (lane == 0) *s_sample = s;
-    }
-    if (tid == 0) {
-        for (int i = 0; i < S::kK; ++i) {
-            mbar_init(smem_u32(&kfull[i]), 1);
-            mbar_init(smem_u32(&kempty[i]), 1);
+        if (tiles > 0 && elect_one()) {
+            mbar_arrive_expect_tx(smem_u32(qfull), 2 * S::kOwn);
+            load(s_q, kAtRows, &map_q, head0, s.q0 + t0, smem_u32(qfull));
+            load(s_g, kAtRows, &map_g, head0, s.q0 + t0, smem_u32(qfull));
         }
-        for (int i = 0; i < S::kV; ++i) {
-            mbar_init(smem_u32(&vfull[i]), 1);
-            mbar_init(smem_u32(&vempty[i]), 1);
-        }
-        for (uint64_t *b : {qfull, tail, sfull, sfull + 1, dpfull, finished}) mbar_init(smem_u32(b), 1);
-        mbar_init(smem_u32(dsready), S::kWarps);
-        *s_abort = 0;
-        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
-    }
-    __syncthreads();
-    const AtSample s = *s_sample;
-    const int n = s.q1 - s.q0, m = s.k1 - s.k0, t0 = s.tile * tokens;
-    if (s.tile < 0 || t0 >= n) return;
-    if (warp == S::kWarpMma) {
+        __syncwarp();
+    } else if (warp == 0) {
         tmem_alloc(smem_u32(s_tmem), S::kColumns);
         tmem_relinquish();
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    if (warp != S::kWarpLoad) {
+        s = *s_sample;
+        share();
+    }
     const uint32_t tmem = *s_tmem, t_dp = tmem + 2 * W, t_dq = tmem + 3 * W;
-    const int head0 = blockIdx.y << log_p, kh = head0 / (a.H / a.K);
-    const int seen_last = at_seen(a, min(n, t0 + tokens) - 1, n, m);
-    int first, last;
-    at_split(a.splits, blockIdx.z, (seen_last + W - 1) / W, first, last);
-    const int tiles = last - first;
-    const int end_valid = min(W, seen_last - (last - 1) * W);
     auto wait = [&](uint64_t *b, uint32_t parity) { return mbar_wait_suspended(smem_u32(b), parity, s_abort, a.wait_ns); };
     auto next = [](int &i, uint32_t &phase, int stages) {
         if (++i == stages) {
@@ -144,17 +163,8 @@ attention_tc_grad_query_kernel(const __grid_constant__ CUtensorMap map_q, const 
     };
 
     if (warp == S::kWarpLoad) {
-        // ------------------------------------------------------------------ loads: q, grad; then k, v of each tile in turn
+        // ------------------------------------------------------------------ loads: k, v of each tile in turn
         if (tiles > 0) {
-            auto load = [&](uint32_t dst, int rows, const CUtensorMap *map, int head, int row, uint32_t mbar) {
-                for (int c = 0; c < DP / 64; ++c) tma_load_3d(dst + c * rows * 128, map, c * 64, head, row, mbar);
-            };
-            if (elect_one()) {
-                mbar_arrive_expect_tx(smem_u32(qfull), 2 * S::kOwn);
-                load(s_q, kAtRows, &map_q, head0, s.q0 + t0, smem_u32(qfull));
-                load(s_g, kAtRows, &map_g, head0, s.q0 + t0, smem_u32(qfull));
-            }
-            __syncwarp();
             int ks = 0, vs = 0;
             uint32_t kp = 1, vp = 1;
             bool ok = true;
@@ -222,7 +232,7 @@ attention_tc_grad_query_kernel(const __grid_constant__ CUtensorMap map_q, const 
                 if (j + 2 < tiles) scores(j + 2);
             }
         }
-    } else {
+    } else if (tiles >= 0) {
         // ------------------------------------------------------------------ a thread a row and 32 columns
         const int part = warp >> 2, row = tid & 127;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
@@ -287,7 +297,7 @@ attention_tc_grad_query_kernel(const __grid_constant__ CUtensorMap map_q, const 
         __syncthreads();
     }
     tc_fence_after();
-    if (warp == S::kWarpMma) tmem_dealloc(tmem, S::kColumns);
+    if (warp == 0) tmem_dealloc(tmem, S::kColumns);
 }
 
 template <int DP, int W>
@@ -317,41 +327,59 @@ attention_tc_grad_key_kernel(const __grid_constant__ CUtensorMap map_q, const __
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int P = 1 << log_p, tokens = W >> log_p;
 
+    const int kh = blockIdx.y, G = a.H / a.K;
+    auto load = [&](uint32_t dst, int rows, const CUtensorMap *map, int head, int row, uint32_t mbar) {
+        for (int c = 0; c < DP / 64; ++c) tma_load_3d(dst + c * rows * 128, map, c * 64, head, row, mbar);
+    };
+    // what a sample gives the CTA: tiles of queries that see a key of this tile, of each block of P heads of the group
+    AtSample s;
+    int n, m, key0, from, per_head, first, last, tiles;
+    auto share = [&] {
+        n = s.q1 - s.q0;
+        m = s.k1 - s.k0;
+        key0 = s.tile * kAtRows;
+        from = a.causal ? (int)max((int64_t)0, (int64_t)key0 - m + n) / tokens : 0;
+        per_head = max(0, (n + tokens - 1) / tokens - from);
+        at_split(a.splits, blockIdx.z, per_head * (G >> log_p), first, last);
+        tiles = s.tile < 0 || key0 >= m ? -1 : last - first;         // -1: nothing to do at all
+    };
+
     at_check_offsets(a);
-    if (warp == S::kWarpLoad) {
-        const AtSample s = at_find(a.key_offsets, a.N, a, blockIdx.x, kAtRows);
-        if (lane == 0) *s_sample = s;
-    }
-    if (tid == 0) {
-        for (int i = 0; i < S::kStages; ++i) {
-            mbar_init(smem_u32(&full[i]), 2);                        // the copies' bytes, and the rows' numbers
-            mbar_init(smem_u32(&empty[i]), 1);
+    if (warp == S::kWarpLoad) {                                      // up to the first loads by this warp alone
+        if (elect_one()) {
+            for (const CUtensorMap *map : {&map_q, &map_k, &map_v, &map_g}) tma_prefetch_desc(map);
+            for (int i = 0; i < S::kStages; ++i) {
+                mbar_init(smem_u32(&full[i]), 2);                    // the copies' bytes, and the rows' numbers
+                mbar_init(smem_u32(&empty[i]), 1);
+            }
+            for (uint64_t *b : {kvfull, tail, sfull, dpfull, finished}) mbar_init(smem_u32(b), 1);
+            mbar_init(smem_u32(pready), S::kWarps);
+            mbar_init(smem_u32(dsready), S::kWarps);
+            *s_abort = 0;
+            asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
         }
-        for (uint64_t *b : {kvfull, tail, sfull, dpfull, finished}) mbar_init(smem_u32(b), 1);
-        mbar_init(smem_u32(pready), S::kWarps);
-        mbar_init(smem_u32(dsready), S::kWarps);
-        *s_abort = 0;
-        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
-    }
-    __syncthreads();
-    const AtSample s = *s_sample;
-    const int n = s.q1 - s.q0, m = s.k1 - s.k0, key0 = s.tile * kAtRows;
-    if (s.tile < 0 || key0 >= m) return;
-    if (warp == S::kWarpMma) {
+        __syncwarp();
+        s = at_find(a.key_offsets, a.N, a, blockIdx.x, kAtRows);
+        share();
+        if (lane == 0) *s_sample = s;
+        if (tiles > 0 && elect_one()) {
+            mbar_arrive_expect_tx(smem_u32(kvfull), 2 * S::kOwn);
+            load(s_k, kAtRows, &map_k, kh, s.k0 + key0, smem_u32(kvfull));
+            load(s_v, kAtRows, &map_v, kh, s.k0 + key0, smem_u32(kvfull));
+        }
+        __syncwarp();
+    } else if (warp == 0) {
         tmem_alloc(smem_u32(s_tmem), S::kColumns);
         tmem_relinquish();
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    if (warp != S::kWarpLoad) {
+        s = *s_sample;
+        share();
+    }
     const uint32_t tmem = *s_tmem, t_dp = tmem + W, t_dv = tmem + 2 * W, t_dk = t_dv + DP;
-    const int kh = blockIdx.y, G = a.H / a.K;
-    // tiles of queries that see a key of this tile, of each block of P heads of the group
-    const int from = a.causal ? (int)max((int64_t)0, (int64_t)key0 - m + n) / tokens : 0;
-    const int per_head = max(0, (n + tokens - 1) / tokens - from);
-    int first, last;
-    at_split(a.splits, blockIdx.z, per_head * (G >> log_p), first, last);
-    const int tiles = last - first;
     struct Walk {
         int head, t;                                                 // the tile's first head, and its number
     };
@@ -372,17 +400,8 @@ attention_tc_grad_key_kernel(const __grid_constant__ CUtensorMap map_q, const __
     };
 
     if (warp == S::kWarpLoad) {
-        // ------------------------------------------------------------------ loads: k, v; then q, grad and the rows' numbers
+        // ------------------------------------------------------------------ loads: q, grad and the rows' numbers
         if (tiles > 0) {
-            auto load = [&](uint32_t dst, int rows, const CUtensorMap *map, int head, int row, uint32_t mbar) {
-                for (int c = 0; c < DP / 64; ++c) tma_load_3d(dst + c * rows * 128, map, c * 64, head, row, mbar);
-            };
-            if (elect_one()) {
-                mbar_arrive_expect_tx(smem_u32(kvfull), 2 * S::kOwn);
-                load(s_k, kAtRows, &map_k, kh, s.k0 + key0, smem_u32(kvfull));
-                load(s_v, kAtRows, &map_v, kh, s.k0 + key0, smem_u32(kvfull));
-            }
-            __syncwarp();
             int st = 0;
             uint32_t phase = 1, tail_phase = 0;
             bool ok = true;
@@ -465,7 +484,7 @@ attention_tc_grad_key_kernel(const __grid_constant__ CUtensorMap map_q, const __
                 }
             }
         }
-    } else {
+    } else if (tiles >= 0) {
         // ------------------------------------------------------------------ a thread a key and 32 query rows
         const int part = warp >> 2, row = tid & 127, key = key0 + row;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
@@ -561,7 +580,7 @@ attention_tc_grad_key_kernel(const __grid_constant__ CUtensorMap map_q, const __
         __syncthreads();
     }
     tc_fence_after();
-    if (warp == S::kWarpMma) tmem_dealloc(tmem, S::kColumns);
+    if (warp == 0) tmem_dealloc(tmem, S::kColumns);
 }
 
 template <typename T, int DP, int W, bool KEYS>

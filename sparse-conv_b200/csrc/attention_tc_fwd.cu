@@ -98,41 +98,71 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int P = 1 << log_p, tokens = kAtRows >> log_p;             // tokens of a tile
 
+    const int head0 = blockIdx.y << log_p, kh = head0 / (a.H / a.K);
+    auto load = [&](uint32_t dst, const CUtensorMap *map, int head, int row, int bytes, uint64_t *b) {
+        mbar_arrive_expect_tx(smem_u32(b), bytes);
+        for (int c = 0; c < DP / 64; ++c) tma_load_3d(dst + c * (bytes / (DP / 64)), map, c * 64, head, row, smem_u32(b));
+    };
+    // what a sample gives the CTA: its first token, keys, and tiles of them in this split
+    int n, m, t0, first, tiles, end_valid;
+    AtSample s;
+    auto share = [&] {
+        n = s.q1 - s.q0;
+        m = s.k1 - s.k0;
+        t0 = s.tile * tokens;
+        const int seen_last = at_seen(a, min(n, t0 + tokens) - 1, n, m);
+        int last;
+        at_split(a.splits, blockIdx.z, (seen_last + S::kKeys - 1) / S::kKeys, first, last);
+        tiles = s.tile < 0 || t0 >= n ? -1 : last - first;           // -1: nothing to do at all
+        end_valid = min(S::kKeys, seen_last - (last - 1) * S::kKeys);            // keys of the last tile (of this split)
+    };
+    auto load_tile = [&](int j) {
+        const int row = s.k0 + (first + j) * S::kKeys, st = j & 1;
+        load(s_k + st * S::kTile, &map_k, kh, row, S::kTile, &kfull[st]);
+        load(s_v + st * S::kTile, &map_v, kh, row, S::kTile, &vfull[st]);
+    };
+
     at_check_offsets(a);
     if (warp == S::kControl) {
-        // the last tiles of a causal sample see most: they go first
-        const AtSample s = at_find(a.offsets, a.M, a, a.causal ? gridDim.x - 1 - blockIdx.x : blockIdx.x, tokens);
-        if (lane == 0) *s_sample = s;
-    }
-    if (tid == 0) {
-        for (int i = 0; i < S::kStages; ++i) {
-            mbar_init(smem_u32(&kfull[i]), 1);
-            mbar_init(smem_u32(&vfull[i]), 1);
+        // Everything up to the first loads by this warp alone: a short sample's time is mostly this way (TMEM's
+        // allocation, by another warp, and the samples' search go on at the same time).
+        if (elect_one()) {
+            tma_prefetch_desc(&map_q);
+            tma_prefetch_desc(&map_k);
+            tma_prefetch_desc(&map_v);
+            for (int i = 0; i < S::kStages; ++i) {
+                mbar_init(smem_u32(&kfull[i]), 1);
+                mbar_init(smem_u32(&vfull[i]), 1);
+            }
+            mbar_init(smem_u32(qfull), 1);
+            mbar_init(smem_u32(sfull), 1);
+            mbar_init(smem_u32(pready), 4);
+            *s_abort = 0;
+            asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
         }
-        mbar_init(smem_u32(qfull), 1);
-        mbar_init(smem_u32(sfull), 1);
-        mbar_init(smem_u32(pready), 4);
-        *s_abort = 0;
-        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
-    }
-    __syncthreads();
-    const AtSample s = *s_sample;
-    const int n = s.q1 - s.q0, m = s.k1 - s.k0, t0 = s.tile * tokens;            // the CTA's first token in the sample
-    if (s.tile < 0 || t0 >= n) return;                                           // uniform over the CTA
-    if (warp == S::kControl) {
+        __syncwarp();
+        // the last tiles of a causal sample see most: they go first
+        s = at_find(a.offsets, a.M, a, a.causal ? gridDim.x - 1 - blockIdx.x : blockIdx.x, tokens);
+        share();
+        if (lane == 0) *s_sample = s;
+        if (tiles > 0 && elect_one()) {
+            load(s_q, &map_q, head0, s.q0 + t0, S::kOwn, qfull);
+            load_tile(0);
+            if (tiles > 1) load_tile(1);
+        }
+        __syncwarp();
+    } else if (warp == 0) {
         tmem_alloc(smem_u32(s_tmem), S::kColumns);
         tmem_relinquish();
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    if (warp != S::kControl) {
+        s = *s_sample;
+        share();
+    }
     const uint32_t tmem = *s_tmem;
-    const int head0 = blockIdx.y << log_p, kh = head0 / (a.H / a.K);
-    const int seen_last = at_seen(a, min(n, t0 + tokens) - 1, n, m);
-    int first, last;
-    at_split(a.splits, blockIdx.z, (seen_last + S::kKeys - 1) / S::kKeys, first, last);
-    const int tiles = last - first;
-    const int end_valid = min(S::kKeys, seen_last - (last - 1) * S::kKeys);      // keys of the last tile (of this split)
     auto wait = [&](uint64_t *b, uint32_t parity) {
         return __all_sync(0xffffffffu, mbar_wait_suspended(smem_u32(b), parity, s_abort, a.wait_ns)) != 0;
     };
@@ -143,27 +173,13 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             const uint32_t id_s = instr_desc_f16(dtype_traits<T>::mma_format, 128, S::kKeys);
             const uint32_t id_o = instr_desc_f16(dtype_traits<T>::mma_format, 128, (a.D + 15) & ~15) | 1u << 16;
             const int steps = (a.D + 15) >> 4;
-            auto load = [&](uint32_t dst, const CUtensorMap *map, int head, int row, int bytes, uint64_t *b) {
-                mbar_arrive_expect_tx(smem_u32(b), bytes);
-                for (int c = 0; c < DP / 64; ++c) tma_load_3d(dst + c * (bytes / (DP / 64)), map, c * 64, head, row, smem_u32(b));
-            };
-            auto load_tile = [&](int j) {
-                const int row = s.k0 + (first + j) * S::kKeys, st = j & 1;
-                load(s_k + st * S::kTile, &map_k, kh, row, S::kTile, &kfull[st]);
-                load(s_v + st * S::kTile, &map_v, kh, row, S::kTile, &vfull[st]);
-            };
-            if (elect_one()) {
-                load(s_q, &map_q, head0, s.q0 + t0, S::kOwn, qfull);
-                load_tile(0);
-                if (tiles > 1) load_tile(1);
-            }
-            __syncwarp();
             bool ok = wait(qfull, 0);
             for (int j = 0; j <= tiles && ok; ++j) {
-                const int st = j & 1;
-                if (j > 0) {                                         // p v of the tile before
-                    const int v = st ^ 1;
-                    const bool end = j == tiles;
+                const int st = j & 1, v = st ^ 1;
+                const bool end = j == tiles;
+                // what is waited for first is long there when p is
+                if (!end && !(ok = wait(&kfull[st], (j >> 1) & 1))) break;
+                if (j > 0) {
                     if (!(ok = wait(&vfull[v], ((j - 1) >> 1) & 1))) break;
                     if (end && (end_valid & 15)) {
                         at_zero_rows<DP, S::kKeys>(s_v + v * S::kTile, end_valid, (end_valid + 15) & ~15);
@@ -171,30 +187,23 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                         __syncwarp();
                     }
                     if (!(ok = wait(pready, (j - 1) & 1))) break;
-                    tc_fence_after();
-                    if (elect_one()) {
-                        at_mma_rows<S::kKeys, S::kKeys>(tmem + S::kKeys, tmem, s_v + v * S::kTile, id_o, end ? (end_valid + 15) >> 4 : S::kKeys / 16, j > 1);
-                        if (end) tc_commit(smem_u32(sfull));
-                    }
-                    __syncwarp();
                 }
-                if (j < tiles) {
-                    if (!(ok = wait(&kfull[st], (j >> 1) & 1))) break;
-                    tc_fence_after();
-                    if (elect_one()) {
-                        at_mma_head<DP, S::kKeys>(tmem, s_q, s_k + st * S::kTile, id_s, steps);
-                        tc_commit(smem_u32(sfull));
-                    }
+                tc_fence_after();
+                if (elect_one()) {                                   // p v of the tile before, then the next scores over p
+                    if (j > 0)
+                        at_mma_rows<S::kKeys, S::kKeys>(tmem + S::kKeys, tmem, s_v + v * S::kTile, id_o, end ? (end_valid + 15) >> 4 : S::kKeys / 16, j > 1);
+                    if (!end) at_mma_head<DP, S::kKeys>(tmem, s_q, s_k + st * S::kTile, id_s, steps);
+                    tc_commit(smem_u32(sfull));
+                }
+                __syncwarp();
+                if (j > 0 && j + 1 < tiles) {                        // the tile before is done with: its stage takes the next
+                    if (!(ok = wait(sfull, j & 1))) break;
+                    if (elect_one()) load_tile(j + 1);
                     __syncwarp();
-                    if (j > 0 && j + 1 < tiles) {                    // the tile before is done with: its stage takes the next
-                        if (!(ok = wait(sfull, j & 1))) break;
-                        if (elect_one()) load_tile(j + 1);
-                        __syncwarp();
-                    }
                 }
             }
         }
-    } else {
+    } else if (tiles >= 0) {
         // ------------------------------------------------------------------ softmax: a thread a row
         const uint32_t t_s = tmem + ((uint32_t)(warp * 32) << 16), t_o = t_s + S::kKeys;
         const int token = t0 + (tid >> log_p);                       // in the sample
@@ -284,7 +293,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         __syncthreads();
     }
     tc_fence_after();
-    if (warp == S::kControl) tmem_dealloc(tmem, S::kColumns);
+    if (warp == 0) tmem_dealloc(tmem, S::kColumns);
 }
 
 // Heads of more than 64 values: two tiles of queries a CTA, keys 128 at a time.
