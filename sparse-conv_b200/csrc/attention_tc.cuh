@@ -15,6 +15,22 @@ namespace spconv {
 constexpr int kAtRows = 128;                         // rows of a tile, and keys
 constexpr int kAtBlock = kAtRows * 128;              // 16 KB: 128 rows of 64 values, 128-byte swizzle
 
+// Bounded wait, suspended up to 20 us between checks; under a limit of less it polls (these waits are so short that one
+// suspended try, however short its hint, would outlast any such limit).
+__device__ __forceinline__ bool at_wait(uint64_t *bar, uint32_t parity, volatile int *abort_flag, uint64_t limit_ns) {
+    const uint32_t addr = smem_u32(bar);
+    if (mbar_test(addr, parity)) return true;
+    const uint64_t t0 = globaltimer_ns();
+    for (;;) {
+        if (limit_ns < 20000ull ? mbar_test(addr, parity) : mbar_try_wait_suspended(addr, parity, 20000u)) return true;
+        if (*abort_flag) return false;
+        if (globaltimer_ns() - t0 > limit_ns) {
+            *abort_flag = 1;
+            return false;
+        }
+    }
+}
+
 // One box of a 3-D tensor (value, head, row).
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const void *tmap, int x, int y, int z, uint32_t mbar) {
     asm volatile(
@@ -67,35 +83,13 @@ __device__ __forceinline__ void at_load(uint32_t taddr, f32x2 (&x)[N]) {
     }
 }
 
-// 2^x of two values on the FMA pipe: x = n + f, |f| <= 1/2, 2^f by a polynomial (degree 4, exact at 0, the smallest
-// largest relative error on the interval: 2.9e-6, under a rounding of either 16-bit type) and 2^n from n's bits. Exactly
-// 0 from -127 on; NaN stays NaN. The special-function unit gives 16 exponentials a clock and SM, a quarter of
-// what the FMA pipe gives products, and is what a tile waits for: a share of the columns goes here.
-__device__ __forceinline__ f32x2 at_exp2_fma(f32x2 x) {
-    const float2 u = unpack_f32x2(x);
-    float a, b;
-    asm("max.NaN.f32 %0, %1, 0fC2FE0000;" : "=f"(a) : "f"(u.x));
-    asm("max.NaN.f32 %0, %1, 0fC2FE0000;" : "=f"(b) : "f"(u.y));
-    x = pack_f32x2(a, b);
-    const f32x2 magic = pack_f32x2(12582912.f, 12582912.f), unmagic = pack_f32x2(-12582912.f, -12582912.f);
-    const f32x2 t = add2(x, magic);
-    const f32x2 n = add2(t, unmagic), one = pack_f32x2(1.f, 1.f);
-    const f32x2 f = fma2(n, pack_f32x2(-1.f, -1.f), x);
-    f32x2 p = fma2(f, pack_f32x2(0.00958285294f, 0.00958285294f), pack_f32x2(0.0559064262f, 0.0559064262f));
-    p = fma2(p, f, pack_f32x2(0.240240991f, 0.240240991f));
-    p = fma2(p, f, pack_f32x2(0.693124175f, 0.693124175f));
-    p = fma2(p, f, one);
-    const float2 tt = unpack_f32x2(t);
-    return mul2(p, pack_f32x2(__int_as_float((__float_as_int(tt.x) << 23) + 0x3f800000),
-                              __int_as_float((__float_as_int(tt.y) << 23) + 0x3f800000)));
-}
-// 2^x of two values.
+// 2^x of two values, by the special functions: 16 a clock and SM. (A polynomial on the FMA pipe, degree 4, for one to four of
+// eight pairs was 2 % faster at best, in the gradients at one of eight, and slower from three on: a step's time is its
+// chain of waits, not the special functions alone.)
 __device__ __forceinline__ f32x2 at_exp2(f32x2 x) {
     const float2 f = unpack_f32x2(x);
     return pack_f32x2(ex2_approx(f.x), ex2_approx(f.y));
 }
-template <int EMU>
-__device__ __forceinline__ f32x2 at_exp2_mix(f32x2 x, int i) { return i * EMU % 8 < EMU ? at_exp2_fma(x) : at_exp2(x); }
 __device__ __forceinline__ float max3_nan(float a, float b, float c) {
     float r;
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));

@@ -8,13 +8,22 @@
 // a tile where one sweep with atomic sums of grad_query would have five, but every sum has one owner and one order: the
 // same bits every run, no fp32 copy of a gradient in memory.
 //
-// A CTA an SM: sixteen warps compute, a thread a row and a quarter of the 128 columns; one loads (TMA), one issues the
-// products. ds (and p) go back to TMEM in 16 bits, over s and dp, and are the A operand of the second products
-// from there; B is the tile that s or dp was made of, read along its rows (MN-major). While the threads work on one
-// of s and dp, the products that make the other run.
+// The walked side comes W rows at a time. Warps: four for each 32 of the W columns compute, a thread a row and 32 columns; one
+// loads (TMA), one issues the products. ds (and p) go back to TMEM in 16 bits, over s and dp, and are the A operand of
+// the second products from there; B is the tile that s or dp was made of, read along its rows (MN-major). While the threads
+// work on one of s and dp, the products that make the other run.
+//
+// Heads of up to 64: W = 64, two CTAs an SM, whose chains of waits fill one another's gaps (a step waits some 170 clocks
+// for each barrier that another warp completes and 250 for a product's end). One CTA with W = 128 has the better products
+// (128 columns of B to a read of A) but idles in its own chain: 84,000 voxels in 16 scenes, 8 x 64 bf16, 1.69 and 2.41 ms
+// for the two sweeps, against 1.55 and 2.07; voxels to 257 tokens 0.71 and 0.50, against 0.44 and 0.47; many windows of 130,
+// 0.47 and 0.53, against 0.28 and 0.32. Wider heads: W = 128, one CTA (their accumulators take half of TMEM): 4 x 128 there
+// 1.16 and 1.60 ms, 1.25 and 1.21 PFLOP/s. Nothing is full: at 8 x 64 the tensor pipe is 45 and 43 % in use, the special
+// functions 45 and 32 %, the issue slots 58 and 53 %.
 //
 // p of the keys' sweep is scaled by 2^15 in fp16, whose smallest values would else lose bits where a row sees
-// thousands of keys; grad_value is scaled back in fp32. A row that sees a single key has ds = 0 exactly.
+// thousands of keys; grad_value is scaled back in fp32. A row that sees a single key has ds = 0 exactly. delta takes the
+// rounded out: with few keys a row grad_query and grad_key are off by two or three roundings, not one.
 // Rows behind a sample's end are treated as in the forward: zeroed in shared memory where a product sums over rows.
 #include <algorithm>
 
@@ -30,13 +39,6 @@ struct AbShape {
     static constexpr int kPerSm = DP == 64 && W == 64 ? 2 : 1, kColumns = 512 / kPerSm;
     static constexpr int kOwn = DP / 64 * kAtBlock, kTile = DP / 64 * W * 128;      // bytes of an own tile, and of a walked one
 };
-#ifndef AB_EMUQ
-#define AB_EMUQ 0
-#endif
-#ifndef AB_EMUK
-#define AB_EMUK 0
-#endif
-
 // A row of accumulators [from, to) times `factor`, to a row of D values: rounded, or fp32 where `part` is given.
 template <typename T>
 __device__ __forceinline__ void ab_store_row(uint32_t taddr, int from, int to, int D, bool zero, float factor, bool mine, T *out, float *part) {
@@ -103,7 +105,7 @@ attention_tc_grad_query_kernel(const __grid_constant__ CUtensorMap map_q, const 
         for (int c = 0; c < DP / 64; ++c) tma_load_3d(dst + c * rows * 128, map, c * 64, head, row, mbar);
     };
     // what a sample gives the CTA
-    AtSample s;
+    AtSample s = {};
     int n, m, t0, first, last, tiles, end_valid;
     auto share = [&] {
         n = s.q1 - s.q0;
@@ -154,7 +156,7 @@ attention_tc_grad_query_kernel(const __grid_constant__ CUtensorMap map_q, const 
         share();
     }
     const uint32_t tmem = *s_tmem, t_dp = tmem + 2 * W, t_dq = tmem + 3 * W;
-    auto wait = [&](uint64_t *b, uint32_t parity) { return mbar_wait_suspended(smem_u32(b), parity, s_abort, a.wait_ns); };
+    auto wait = [&](uint64_t *b, uint32_t parity) { return at_wait(b, parity, s_abort, a.wait_ns); };
     auto next = [](int &i, uint32_t &phase, int stages) {
         if (++i == stages) {
             i = 0;
@@ -253,7 +255,7 @@ attention_tc_grad_query_kernel(const __grid_constant__ CUtensorMap map_q, const 
             if (some) {
                 lt_load32(t_s, x);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) x[i] = at_exp2_mix<AB_EMUQ>(fma2(x[i], c2, l2), i);
+                for (int i = 0; i < 16; ++i) x[i] = at_exp2(fma2(x[i], c2, l2));
             }
             if (!(ok = __all_sync(0xffffffffu, wait(dpfull, j & 1)) != 0)) break;
             tc_fence_after();
@@ -332,7 +334,7 @@ attention_tc_grad_key_kernel(const __grid_constant__ CUtensorMap map_q, const __
         for (int c = 0; c < DP / 64; ++c) tma_load_3d(dst + c * rows * 128, map, c * 64, head, row, mbar);
     };
     // what a sample gives the CTA: tiles of queries that see a key of this tile, of each block of P heads of the group
-    AtSample s;
+    AtSample s = {};
     int n, m, key0, from, per_head, first, last, tiles;
     auto share = [&] {
         n = s.q1 - s.q0;
@@ -391,7 +393,7 @@ attention_tc_grad_key_kernel(const __grid_constant__ CUtensorMap map_q, const __
         }
     };
     auto rows_of = [&](const Walk &w) { return min(tokens, n - w.t * tokens) << log_p; };
-    auto wait = [&](uint64_t *b, uint32_t parity) { return mbar_wait_suspended(smem_u32(b), parity, s_abort, a.wait_ns); };
+    auto wait = [&](uint64_t *b, uint32_t parity) { return at_wait(b, parity, s_abort, a.wait_ns); };
     auto next = [](int &i, uint32_t &phase) {
         if (++i == S::kStages) {
             i = 0;
@@ -516,8 +518,8 @@ attention_tc_grad_key_kernel(const __grid_constant__ CUtensorMap map_q, const __
             for (int i = 0; i < 16; i += 2) {
                 f32x2 l0, l1;
                 asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];\n" : "=l"(l0.v), "=l"(l1.v) : "r"(s_lse + i * 8));
-                x[i] = at_exp2_mix<AB_EMUK>(fma2(x[i], c2, l0), i);
-                x[i + 1] = at_exp2_mix<AB_EMUK>(fma2(x[i + 1], c2, l1), i + 1);
+                x[i] = at_exp2(fma2(x[i], c2, l0));
+                x[i + 1] = at_exp2(fma2(x[i + 1], c2, l1));
             }
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
@@ -606,15 +608,9 @@ static int ab_run(const AtArgs &a) {
     return check_launch(KEYS ? "attention_tc_grad_key_kernel" : "attention_tc_grad_query_kernel");
 }
 
-#ifndef AB_WQ
-#define AB_WQ 64
-#endif
-#ifndef AB_WK
-#define AB_WK 64
-#endif
 template <typename T, bool KEYS>
 static int ab_size(const AtArgs &a) {
-    return a.D <= 64 ? ab_run<T, 64, KEYS ? AB_WK : AB_WQ, KEYS>(a) : ab_run<T, 128, 128, KEYS>(a);
+    return a.D <= 64 ? ab_run<T, 64, 64, KEYS>(a) : ab_run<T, 128, 128, KEYS>(a);
 }
 
 int launch_at_tc_grad_query(const AtArgs &a) {

@@ -2,12 +2,21 @@
 //
 //   s = q k^T (fp32, TMEM);  p = 2^(s c - m);  out = (p v) / sum p,   c = scale log2(e), m a running maximum of s c
 //
-// A CTA owns NQ tiles of 128 query rows of one key head and walks the sample's keys, 128 at a time. Warps: four a
-// tile for the softmax, a thread a row; one that loads (TMA), one that issues the products. Per tile of keys s
-// arrives in TMEM, its row goes to registers whole, p goes back over it in 16 bits, and is the A operand of p v from there;
-// the rows of v are read along the keys (MN-major), so nothing is transposed. With two tiles (NQ = 2, a CTA an SM) one tile's
-// products run under the other's softmax, and keys and values are read once for both; with one (two CTAs an SM) the two
-// CTAs do that for one another, which wastes less where samples are short.
+// A CTA owns tiles of 128 query rows of one key head and walks the sample's keys; four warps a tile do the softmax, a
+// thread a row. s arrives in TMEM, its row goes to registers whole, p goes back over it in 16 bits, and is the A operand of
+// p v from there; the rows of v are read along the keys (MN-major), so nothing is transposed.
+//
+// A step is a chain: products, softmax, products; each barrier that another warp completes costs about 170 clocks, a
+// product's end 250, and the 64 exponentials a row 520 of the special functions' time. What fills the gaps is other chains:
+//   * attention_tc_kernel: one tile a CTA, 64 keys a step, four CTAs an SM (two for heads over 64): 128 columns of TMEM and
+//     48 KB each. A fifth warp does both loads and products. 84,000 voxels in 16 scenes, 8 x 64 bf16: 1.32 ms, 0.73 PFLOP/s
+//     (three CTAs an SM 1.56; one CTA of two tiles and 128 keys a step, whose two chains fell into step with one another,
+//     1.69; the same with the next scores made ahead of p v 1.48; two threads a row 2.02). The special functions are
+//     64 % in use, the issue slots 46 %, the tensor pipe 32 %. One pooling query a scene over 2.0 M voxels: 120 us and 15 to
+//     join the splits, 4.5 TB/s.
+//   * attention_tc_pair_kernel, for long samples of heads over 64, whose accumulators leave TMEM for two chains only: two
+//     tiles a CTA, which share k and v, 128 keys a step, and registers dealt out anew so that a row of 128 scores fits: 4 x 128
+//     there 0.93 ms, 1.04 PFLOP/s (two CTAs of the kernel above 1.21 ms).
 //
 // The maximum is followed lazily: while a row's new maximum exceeds the one in use by at most 8, the old one
 // stays (p up to 2^8, exact in range), so out and the sum are rescaled a few times a row, not once a tile. p is
@@ -105,7 +114,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     };
     // what a sample gives the CTA: its first token, keys, and tiles of them in this split
     int n, m, t0, first, tiles, end_valid;
-    AtSample s;
+    AtSample s = {};
     auto share = [&] {
         n = s.q1 - s.q0;
         m = s.k1 - s.k0;
@@ -164,7 +173,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     }
     const uint32_t tmem = *s_tmem;
     auto wait = [&](uint64_t *b, uint32_t parity) {
-        return __all_sync(0xffffffffu, mbar_wait_suspended(smem_u32(b), parity, s_abort, a.wait_ns)) != 0;
+        return __all_sync(0xffffffffu, at_wait(b, parity, s_abort, a.wait_ns)) != 0;
     };
 
     if (warp == S::kControl) {
@@ -364,7 +373,7 @@ attention_tc_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     at_split(a.splits, blockIdx.z, (seen_last + kAtRows - 1) / kAtRows, first, last);
     const int tiles = last - first;
     const int end_valid = min(kAtRows, seen_last - (last - 1) * kAtRows);      // keys of the last tile (of this split)
-    auto wait = [&](uint64_t *b, uint32_t parity) { return mbar_wait_suspended(smem_u32(b), parity, s_abort, a.wait_ns); };
+    auto wait = [&](uint64_t *b, uint32_t parity) { return at_wait(b, parity, s_abort, a.wait_ns); };
     auto next = [](int &i, uint32_t &phase) {
         if (++i == S::kStages) {
             i = 0;
@@ -372,75 +381,76 @@ attention_tc_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         }
     };
 
+    // each share of the registers is set inside its roles' branch: behind a join the compiler would keep to the smaller
     if (warp >= S::kWarpLoad) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" :: "n"(S::kRegsOther));
-    if (warp == S::kWarpLoad) {
-        // ------------------------------------------------------------------ loads: q; then k, v of each tile in turn
-        if (tiles > 0) {
-            if (elect_one()) {
-                mbar_arrive_expect_tx(smem_u32(qfull), (uint32_t)(nq * S::kTile));
-                for (int q = 0; q < nq; ++q)
-                    for (int c = 0; c < DP / 64; ++c)
-                        tma_load_3d(s_q + q * S::kTile + c * kAtBlock, &map_q, c * 64, head0, s.q0 + t0 + q * tokens, smem_u32(qfull));
-            }
-            __syncwarp();
-            int st = 0;
-            uint32_t phase = 1;                                      // the first use of a stage passes at once
-            bool ok = true;
-            for (int i = 0; i < 2 * tiles && ok; ++i, next(st, phase)) {
-                const bool is_v = i & 1;
-                const int tile = i >> 1;
-                const bool cut = is_v && tile + 1 == tiles && (end_valid & 15);
-                ok = __all_sync(0xffffffffu, wait(&empty[st], phase)) != 0;
-                if (!ok) break;
-                const uint32_t dst = s_ring + st * S::kTile;
+        if (warp == S::kWarpLoad) {
+            // ------------------------------------------------------------------ loads: q; then k, v of each tile in turn
+            if (tiles > 0) {
                 if (elect_one()) {
-                    const uint32_t mbar = smem_u32(cut ? tail : &full[st]);
-                    mbar_arrive_expect_tx(mbar, S::kTile);
-                    for (int c = 0; c < DP / 64; ++c)
-                        tma_load_3d(dst + c * kAtBlock, is_v ? &map_v : &map_k, c * 64, kh, s.k0 + (first + tile) * kAtRows, mbar);
+                    mbar_arrive_expect_tx(smem_u32(qfull), (uint32_t)(nq * S::kTile));
+                    for (int q = 0; q < nq; ++q)
+                        for (int c = 0; c < DP / 64; ++c)
+                            tma_load_3d(s_q + q * S::kTile + c * kAtBlock, &map_q, c * 64, head0, s.q0 + t0 + q * tokens, smem_u32(qfull));
                 }
                 __syncwarp();
-                if (cut) {
-                    ok = __all_sync(0xffffffffu, wait(tail, 0)) != 0;
-                    at_zero_rows<DP, kAtRows>(dst, end_valid, (end_valid + 15) & ~15);
-                    fence_proxy_async_smem();
+                int st = 0;
+                uint32_t phase = 1;                                      // the first use of a stage passes at once
+                bool ok = true;
+                for (int i = 0; i < 2 * tiles && ok; ++i, next(st, phase)) {
+                    const bool is_v = i & 1;
+                    const int tile = i >> 1;
+                    const bool cut = is_v && tile + 1 == tiles && (end_valid & 15);
+                    ok = __all_sync(0xffffffffu, wait(&empty[st], phase)) != 0;
+                    if (!ok) break;
+                    const uint32_t dst = s_ring + st * S::kTile;
+                    if (elect_one()) {
+                        const uint32_t mbar = smem_u32(cut ? tail : &full[st]);
+                        mbar_arrive_expect_tx(mbar, S::kTile);
+                        for (int c = 0; c < DP / 64; ++c)
+                            tma_load_3d(dst + c * kAtBlock, is_v ? &map_v : &map_k, c * 64, kh, s.k0 + (first + tile) * kAtRows, mbar);
+                    }
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(smem_u32(&full[st]));
+                    if (cut) {
+                        ok = __all_sync(0xffffffffu, wait(tail, 0)) != 0;
+                        at_zero_rows<DP, kAtRows>(dst, end_valid, (end_valid + 15) & ~15);
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(smem_u32(&full[st]));
+                    }
                 }
             }
-        }
-    } else if (warp == S::kWarpMma) {
-        // ------------------------------------------------------------------ products
-        if (tiles > 0 && elect_one()) {
-            const uint32_t id_s = instr_desc_f16(dtype_traits<T>::mma_format, 128, 128);
-            const uint32_t id_o = instr_desc_f16(dtype_traits<T>::mma_format, 128, (a.D + 15) & ~15) | 1u << 16;
-            const int steps = (a.D + 15) >> 4;
-            // the ring holds k0, v0, k1, v1, ..
-            auto landed = [&](int at) { return wait(&full[at % S::kStages], (at / S::kStages) & 1); };
-            auto release = [&](int at) { tc_commit(smem_u32(&empty[at % S::kStages])); };
-            auto stage = [&](int at) { return s_ring + at % S::kStages * S::kTile; };
-            bool ok = wait(qfull, 0);
-            auto scores = [&](int q, int i) {                        // s of tile i
-                if (!(ok = ok && landed(2 * i))) return;
-                tc_fence_after();
-                at_mma_head<DP, kAtRows>(tmem + q * 128, s_q + q * S::kTile, stage(2 * i), id_s, steps);
-                tc_commit(smem_u32(&sfull[q]));
-                if (q + 1 == nq) release(2 * i);
-            };
-            for (int q = 0; q < nq; ++q) scores(q, 0);
-            for (int i = 0; i < tiles && ok; ++i)
-                for (int q = 0; q < nq && ok; ++q) {                 // p v of tile i, then the next scores over p
-                    if (!(ok = wait(&pready[q], i & 1) && landed(2 * i + 1))) break;
+        } else if (warp == S::kWarpMma) {
+            // ------------------------------------------------------------------ products
+            if (tiles > 0 && elect_one()) {
+                const uint32_t id_s = instr_desc_f16(dtype_traits<T>::mma_format, 128, 128);
+                const uint32_t id_o = instr_desc_f16(dtype_traits<T>::mma_format, 128, (a.D + 15) & ~15) | 1u << 16;
+                const int steps = (a.D + 15) >> 4;
+                // the ring holds k0, v0, k1, v1, ..
+                auto landed = [&](int at) { return wait(&full[at % S::kStages], (at / S::kStages) & 1); };
+                auto release = [&](int at) { tc_commit(smem_u32(&empty[at % S::kStages])); };
+                auto stage = [&](int at) { return s_ring + at % S::kStages * S::kTile; };
+                bool ok = wait(qfull, 0);
+                auto scores = [&](int q, int i) {                        // s of tile i
+                    if (!(ok = ok && landed(2 * i))) return;
                     tc_fence_after();
-                    at_mma_rows<128, kAtRows>(tmem + S::kAcc + q * DP, tmem + q * 128, stage(2 * i + 1), id_o,
-                                              i + 1 < tiles ? 8 : (end_valid + 15) >> 4, i > 0);
-                    tc_commit(smem_u32(&odone[q]));
-                    if (q + 1 == nq) release(2 * i + 1);
-                    if (i + 1 < tiles) scores(q, i + 1);
-                }
+                    at_mma_head<DP, kAtRows>(tmem + q * 128, s_q + q * S::kTile, stage(2 * i), id_s, steps);
+                    tc_commit(smem_u32(&sfull[q]));
+                    if (q + 1 == nq) release(2 * i);
+                };
+                for (int q = 0; q < nq; ++q) scores(q, 0);
+                for (int i = 0; i < tiles && ok; ++i)
+                    for (int q = 0; q < nq && ok; ++q) {                 // p v of tile i, then the next scores over p
+                        if (!(ok = wait(&pready[q], i & 1) && landed(2 * i + 1))) break;
+                        tc_fence_after();
+                        at_mma_rows<128, kAtRows>(tmem + S::kAcc + q * DP, tmem + q * 128, stage(2 * i + 1), id_o,
+                                                  i + 1 < tiles ? 8 : (end_valid + 15) >> 4, i > 0);
+                        tc_commit(smem_u32(&odone[q]));
+                        if (q + 1 == nq) release(2 * i + 1);
+                        if (i + 1 < tiles) scores(q, i + 1);
+                    }
+            }
         }
-    }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" :: "n"(S::kRegs));
         // ------------------------------------------------------------------ softmax: a thread a row
