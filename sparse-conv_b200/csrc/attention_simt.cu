@@ -100,22 +100,23 @@ __device__ __forceinline__ void as_rows(const float *p, const float *b, f32x2 (&
     }
 }
 
-// acc[i][j] += sum_q p[q][4 ty + i] b[q][tx + 16 j], q < BM: the even and the odd q apart
+// (acc[i][j]: rows 4 ty + 2 i and 4 ty + 2 i + 1) += sum_q p[q][4 ty + ..] b[q][tx + 16 j], q < BM
 template <int DP>
-__device__ __forceinline__ void as_cols(const float *p, const float *b, f32x2 (&acc)[AsShape<DP>::R][AsShape<DP>::C]) {
+__device__ __forceinline__ void as_cols(const float *p, const float *b, f32x2 (&acc)[AsShape<DP>::R / 2][AsShape<DP>::C]) {
     using S = AsShape<DP>;
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
     const float *pp = p + ty * S::R, *pb = b + tx;
 #pragma unroll 4
-    for (int q = 0; q < S::BM; q += 2) {
-        f32x2 x[S::R];
-#pragma unroll
-        for (int i = 0; i < S::R; ++i) x[i] = pack_f32x2(pp[q * S::LP + i], pp[(q + 1) * S::LP + i]);
+    for (int q = 0; q < S::BM; ++q) {
+        float x[S::R];
+        if constexpr (S::R == 4) *(float4 *)x = *(const float4 *)(pp + q * S::LP);
+        else *(float2 *)x = *(const float2 *)(pp + q * S::LP);
 #pragma unroll
         for (int j = 0; j < S::C; ++j) {
-            const f32x2 y = pack_f32x2(pb[q * S::LD + 16 * j], pb[(q + 1) * S::LD + 16 * j]);
+            const float y = pb[q * S::LD + 16 * j];
+            const f32x2 yy = pack_f32x2(y, y);
 #pragma unroll
-            for (int i = 0; i < S::R; ++i) acc[i][j] = fma2(x[i], y, acc[i][j]);
+            for (int i = 0; i < S::R / 2; ++i) acc[i][j] = fma2(as_pair(x + 2 * i), yy, acc[i][j]);
         }
     }
 }
@@ -321,7 +322,7 @@ attention_simt_grad_key_kernel(const __grid_constant__ AtArgs a) {
     at_split(a.splits, blockIdx.z, tiles * G, first, last);
     as_load<T, DP>(sk, a.k, row0, rows, kh, a.D);
     as_load<T, DP>(sv, a.v, row0, rows, kh, a.D);
-    f32x2 gk[S::R][S::C], gv[S::R][S::C];
+    f32x2 gk[S::R / 2][S::C], gv[S::R / 2][S::C];
     as_clear(gk);
     as_clear(gv);
     for (int it = first; it < last; ++it) {
@@ -349,6 +350,10 @@ attention_simt_grad_key_kernel(const __grid_constant__ AtArgs a) {
         as_cols<DP>(sp, sg, gv);
         as_cols<DP>(sd, sq, gk);
     }
+    auto of = [](f32x2 pair, int i) {
+        const float2 f = unpack_f32x2(pair);
+        return i & 1 ? f.y : f.x;
+    };
 #pragma unroll
     for (int i = 0; i < S::R; ++i) {
         const int r = ty * S::R + i;
@@ -359,11 +364,11 @@ attention_simt_grad_key_kernel(const __grid_constant__ AtArgs a) {
             const int d = tx + 16 * j;
             if (d >= a.D) continue;
             if (a.splits > 1) {
-                a.partial[((2 * blockIdx.z) * all + at) * a.D + d] = as_sum(gk[i][j]) * a.scale;
-                a.partial[((2 * blockIdx.z + 1) * all + at) * a.D + d] = as_sum(gv[i][j]);
+                a.partial[((2 * blockIdx.z) * all + at) * a.D + d] = of(gk[i / 2][j], i) * a.scale;
+                a.partial[((2 * blockIdx.z + 1) * all + at) * a.D + d] = of(gv[i / 2][j], i);
             } else {
-                if (a.gk) ((T *)a.gk)[at * a.D + d] = dtype_traits<T>::from_f(as_sum(gk[i][j]) * a.scale);
-                if (a.gv) ((T *)a.gv)[at * a.D + d] = dtype_traits<T>::from_f(as_sum(gv[i][j]));
+                if (a.gk) ((T *)a.gk)[at * a.D + d] = dtype_traits<T>::from_f(of(gk[i / 2][j], i) * a.scale);
+                if (a.gv) ((T *)a.gv)[at * a.D + d] = dtype_traits<T>::from_f(of(gv[i / 2][j], i));
             }
         }
     }
