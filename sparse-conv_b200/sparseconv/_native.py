@@ -1070,49 +1070,57 @@ def _heads(t: torch.Tensor, what: str) -> torch.Tensor:
     return t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous()
 
 
-@functools.lru_cache(maxsize=256)
-def _rotary_args(dtype: torch.dtype, layout: str, heads: int, key_heads: int, size: int, rotary_dim: int, axes: int,
-                 steps: Tuple[float, ...], amplitude: float, inverse: bool) -> RotaryArgs:
-    """The checked arguments of a call but for its rows and tensors; calls take copies."""
-    if dtype not in DTYPE_CODES:
-        raise TypeError(f"unsupported dtype {dtype}")
-    if layout not in ROTARY_LAYOUTS:
-        raise ValueError(f"unsupported layout {layout}")
-    if not 2 <= size <= 2 * ROTARY_MAX_PAIRS:
-        raise ValueError(f"head size must be in [2, {2 * ROTARY_MAX_PAIRS}], got {size}")
-    a = RotaryArgs(dtype=DTYPE_CODES[dtype], layout=ROTARY_LAYOUTS[layout], heads=heads, key_heads=key_heads, head_size=size,
-                   rotary_dim=rotary_dim, axes=axes, inverse=inverse, amplitude=amplitude)
-    ctypes.memmove(ctypes.addressof(a) + RotaryArgs.steps.offset, _turn_steps(steps), RotaryArgs.steps.size)
-    return a
+class RotaryPlan:
+    """What a configuration of rotary positions needs: an axis's steps as angles, and arguments for each kind of tensors,
+    checked once; calls take copies."""
+
+    def __init__(self, layout: str, rotary_dim: int, axes: int, steps: Tuple[float, ...], amplitude: float):
+        if layout not in ROTARY_LAYOUTS:
+            raise ValueError(f"unsupported layout {layout}")
+        self.layout, self.rotary_dim, self.axes, self.steps, self.amplitude = layout, rotary_dim, axes, steps, amplitude
+        self._args = {}
+
+    def args(self, dtype: torch.dtype, heads: int, key_heads: int, size: int, inverse: bool) -> RotaryArgs:
+        kind = (dtype, heads, key_heads, size, inverse)
+        a = self._args.get(kind)
+        if a is None:
+            if dtype not in DTYPE_CODES:
+                raise TypeError(f"unsupported dtype {dtype}")
+            if not 2 <= size <= 2 * ROTARY_MAX_PAIRS:
+                raise ValueError(f"head size must be in [2, {2 * ROTARY_MAX_PAIRS}], got {size}")
+            a = RotaryArgs(dtype=DTYPE_CODES[dtype], layout=ROTARY_LAYOUTS[self.layout], heads=heads, key_heads=key_heads,
+                           head_size=size, rotary_dim=self.rotary_dim, axes=self.axes, inverse=inverse, amplitude=self.amplitude)
+            ctypes.memmove(ctypes.addressof(a) + RotaryArgs.steps.offset, _turn_steps(self.steps), RotaryArgs.steps.size)
+            if len(self._args) < 256:
+                self._args[kind] = a
+        return RotaryArgs.from_buffer_copy(a)
 
 
 @_on_device
-def _rotary_on(first: torch.Tensor, query, key, positions: torch.Tensor, layout: str, rotary_dim: int,
-               steps: Tuple[float, ...], amplitude: float, inverse: bool) -> tuple:
-    dev = _require_cuda(first, query, key, positions)
+def _rotary_on(first: torch.Tensor, query, key, positions: torch.Tensor, plan: RotaryPlan, inverse: bool) -> tuple:
+    _require_cuda(first, query, key, positions)
     dtype, (rows, _, size) = first.dtype, first.shape
     if positions.dtype != torch.int32:
         raise TypeError(f"positions must be int32, got {positions.dtype}")
     if positions.dim() == 1:
         positions = positions[:, None]
-    if positions.dim() != 2 or positions.shape[0] != rows:
+    if positions.dim() != 2 or positions.shape != (rows, plan.axes):
         raise ValueError(f"positions must have shape [{rows}] or [{rows}, axes], got {list(positions.shape)}")
     heads = key_heads = 0
     query_out = key_out = None
     if query is not None:                    # copies live until the launch
         query = _heads(query, "query")
         heads = query.shape[1]
-        query_out = torch.empty(query.shape, dtype=dtype, device=dev)
+        query_out = query.new_empty(query.shape)
     if key is not None:
         key = _heads(key, "key")
         if key.dtype != dtype:
             raise TypeError(f"key dtype {key.dtype} differs from {dtype}")
-        if key.shape[0] != rows or key.shape[2] != size:
+        key_rows, key_heads, key_size = key.shape
+        if key_rows != rows or key_size != size:
             raise ValueError(f"key must have shape [{rows}, heads, {size}], got {list(key.shape)}")
-        key_heads = key.shape[1]
-        key_out = torch.empty(key.shape, dtype=dtype, device=dev)
-    a = RotaryArgs.from_buffer_copy(_rotary_args(dtype, layout, heads, key_heads, size, rotary_dim, positions.shape[1], steps,
-                                                 amplitude, inverse))
+        key_out = key.new_empty(key.shape)
+    a = plan.args(dtype, heads, key_heads, size, inverse)
     if rows == 0 or heads + key_heads == 0:
         return query_out, key_out
     a.num_rows, a.positions = rows, positions.data_ptr()
@@ -1132,11 +1140,10 @@ def _rotary_on(first: torch.Tensor, query, key, positions: torch.Tensor, layout:
     return query_out, key_out
 
 
-def rotary(query: Optional[torch.Tensor], key: Optional[torch.Tensor], positions: torch.Tensor, layout: str,
-           rotary_dim: int, steps: Tuple[float, ...], amplitude: float, inverse: bool = False) -> tuple:
-    """(query, key) with their pairs turned by positions * steps (an axis's pairs), or backwards; None for None."""
-    return _rotary_on(query if query is not None else key, query, key, positions, layout, rotary_dim, steps,
-                      amplitude, inverse)
+def rotary(query: Optional[torch.Tensor], key: Optional[torch.Tensor], positions: torch.Tensor, plan: RotaryPlan,
+           inverse: bool = False) -> tuple:
+    """(query, key) with their pairs turned by positions * steps, or backwards; None for None."""
+    return _rotary_on(query if query is not None else key, query, key, positions, plan, inverse)
 
 
 def _offsets(t: torch.Tensor, what: str) -> int:
@@ -1195,7 +1202,7 @@ def attention_forward(query: torch.Tensor, key: torch.Tensor, value: torch.Tenso
     (a.query_row, a.query_head, _), (a.key_row, a.key_head, _), (a.value_row, a.value_head, _) = (
         query.stride(), key.stride(), value.stride())
     index = dev.index
-    out = torch.empty((M, H, D), dtype=query.dtype, device=dev)
+    out = query.new_empty((M, H, D))
     a.out = out.data_ptr()
     stats = None
     if keep_stats:
@@ -1226,7 +1233,7 @@ def attention_backward_of(args: AttentionArgs, query, key, value, offsets, key_o
     a.offsets, a.key_offsets = _ptr(offsets), _ptr(key_offsets)
     a.out, a.row_stats = out.data_ptr(), stats.data_ptr()
     a.grad_out, a.grad_row, a.grad_head = grad_out.data_ptr(), grad_out.stride(0), grad_out.stride(1)
-    grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if n else None for t, n in zip((query, key, value), needs)]
+    grads = [t.new_empty(t.shape) if n else None for t, n in zip((query, key, value), needs)]
     a.grad_query, a.grad_key, a.grad_value = map(_ptr, grads)
     ws = _attention_workspace(a, True, query.device)
     a.status = mapped_status(index)

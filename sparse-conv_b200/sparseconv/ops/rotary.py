@@ -68,13 +68,25 @@ def rotary_steps(pairs: int, base: float = 10000.0, scaling: str = RotaryScaling
     return tuple(steps), 0.1 * math.log(factor) + 1.0
 
 
+@functools.lru_cache(maxsize=64)
+def _plan(size: int, rotary_dim: Optional[int], axes: int, layout: str, base: float, scaling: str, factor: float,
+          trained_size: Optional[int]) -> _native.RotaryPlan:
+    if rotary_dim is None:
+        rotary_dim = size // 2 * 2
+    pairs = rotary_dim // 2 // max(axes, 1)
+    if rotary_dim % 2 or not 2 <= rotary_dim <= size or pairs < 1:
+        raise ValueError(f"rotary_dim must be even, at most the head size {size} and at least twice the {axes} axes, "
+                         f"got {rotary_dim}")
+    return _native.RotaryPlan(layout, rotary_dim, axes, *rotary_steps(pairs, float(base), scaling, float(factor), trained_size))
+
+
 class SparseRotaryFunction(Function):
     @staticmethod
-    def forward(ctx, query, key, positions, layout, rotary_dim, steps, amplitude):
+    def forward(ctx, query, key, positions, plan):
         ctx.save_for_backward(positions)
-        ctx.settings = (layout, rotary_dim, steps, amplitude)
+        ctx.plan = plan
         ctx.set_materialize_grads(False)
-        return _native.rotary(query, key, positions, layout, rotary_dim, steps, amplitude)
+        return _native.rotary(query, key, positions, plan)
 
     @staticmethod
     def backward(ctx, grad_query, grad_key):
@@ -84,8 +96,8 @@ class SparseRotaryFunction(Function):
         gq = grad_query if ctx.needs_input_grad[0] else None
         gk = grad_key if ctx.needs_input_grad[1] else None
         if gq is not None or gk is not None:
-            gq, gk = _native.rotary(gq, gk, ctx.saved_tensors[0], *ctx.settings, inverse=True)
-        return gq, gk, None, None, None, None, None
+            gq, gk = _native.rotary(gq, gk, ctx.saved_tensors[0], ctx.plan, inverse=True)
+        return gq, gk, None, None
 
 
 def sparse_rotary(
@@ -123,14 +135,8 @@ def sparse_rotary(
         raise ValueError("query or key is needed")
     if first.dim() != 3:
         raise ValueError(f"query and key must be [N, heads, D], got shape {list(first.shape)}")
-    if rotary_dim is None:
-        rotary_dim = first.shape[2] // 2 * 2
     axes = 1 if positions.dim() == 1 else positions.shape[-1]
-    pairs = rotary_dim // 2 // max(axes, 1)
-    if rotary_dim % 2 or not 2 <= rotary_dim <= first.shape[2] or pairs < 1:
-        raise ValueError(f"rotary_dim must be even, at most the head size {first.shape[2]} and at least twice the "
-                         f"{axes} axes, got {rotary_dim}")
-    steps, amplitude = rotary_steps(pairs, float(base), scaling, float(factor), trained_size)
+    plan = _plan(first.shape[2], rotary_dim, axes, layout, base, scaling, factor, trained_size)
     if torch.is_grad_enabled() and ((query is not None and query.requires_grad) or (key is not None and key.requires_grad)):
-        return SparseRotaryFunction.apply(query, key, positions, layout, rotary_dim, steps, amplitude)
-    return _native.rotary(query, key, positions, layout, rotary_dim, steps, amplitude)
+        return SparseRotaryFunction.apply(query, key, positions, plan)
+    return _native.rotary(query, key, positions, plan)
