@@ -436,6 +436,9 @@ int spconv_rotary(const spconv_rotary_args *args, void *stream);
  *   to the number of rows (anything else sets SPCONV_STATUS_OFFSETS, and rows may be left unwritten); both may be NULL for one
  *   sample of all rows. Samples without queries or keys are allowed.
  *   row_stats [num_queries, heads] fp32: written by the forward unless NULL, read by the backward
+ *   out_rest: NULL, or as out: what rounding took from out, rounded itself, written by the forward and read by the backward, which
+ *   needs grad_out . out. Where rows see many keys, out's rounding is far under the terms' own size; where they see
+ *   few (up to a hundred or so), gradients of queries and keys are off by up to twice as much without it
  *   scale: positive. head_size <= 256. kernel: SPCONV_KERNEL_*; the tensor-core kernels take fp16 and bf16 heads of up
  *   to 128 values and return SPCONV_ERR_UNSUPPORTED for others
  * Products accumulate in fp32, as softmax statistics and row sums; outputs are rounded once. On the tensor cores p and its
@@ -453,7 +456,7 @@ typedef struct {
     const int32_t *offsets, *key_offsets;
     const void *query, *key, *value;
     int64_t query_row, query_head, key_row, key_head, value_row, value_head;
-    void *out;
+    void *out, *out_rest;
     float *row_stats;
     const void *grad_out;
     int64_t grad_row, grad_head;

@@ -24,7 +24,7 @@ attention_pack_kernel(AtTensor t, T *out, int64_t rows, int heads, int D, int to
     }
 }
 
-// delta[row, head] = grad . out, eight lanes each. Bound: HBM.
+// delta[row, head] = grad . (out + what its rounding left out, where that is kept), eight lanes each. Bound: HBM.
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(kAtThreads)
 attention_delta_kernel(const __grid_constant__ AtArgs a) {
@@ -35,7 +35,7 @@ attention_delta_kernel(const __grid_constant__ AtArgs a) {
     if (in) {
         const int64_t r = rh / a.H;
         const T *g = (const T *)a.grad.p + r * a.grad.row + (rh - r * a.H) * a.grad.head;
-        const T *o = (const T *)a.out_in + rh * a.D;
+        const T *o = (const T *)a.out_in + rh * a.D, *rest = a.rest ? (const T *)a.rest + rh * a.D : nullptr;
         if constexpr (WIDE) {
             constexpr int V = 16 / sizeof(T);
             for (int d = lane * V; d < a.D; d += 8 * V) {
@@ -43,9 +43,16 @@ attention_delta_kernel(const __grid_constant__ AtArgs a) {
 #pragma unroll
                 for (int i = 0; i < V; ++i)
                     s = fmaf(dtype_traits<T>::to_f(((const T *)&x)[i]), dtype_traits<T>::to_f(((const T *)&y)[i]), s);
+                if (rest) {
+                    const uint4 z = *(const uint4 *)(rest + d);
+#pragma unroll
+                    for (int i = 0; i < V; ++i)
+                        s = fmaf(dtype_traits<T>::to_f(((const T *)&x)[i]), dtype_traits<T>::to_f(((const T *)&z)[i]), s);
+                }
             }
         } else {
-            for (int d = lane; d < a.D; d += 8) s = fmaf(dtype_traits<T>::to_f(g[d]), dtype_traits<T>::to_f(o[d]), s);
+            for (int d = lane; d < a.D; d += 8)
+                s = fmaf(dtype_traits<T>::to_f(g[d]), dtype_traits<T>::to_f(o[d]) + (rest ? dtype_traits<T>::to_f(rest[d]) : 0.f), s);
         }
     }
 #pragma unroll
@@ -103,7 +110,7 @@ attention_join_kernel(const __grid_constant__ AtArgs a, const int share) {
     const float inv = some ? 1.f / sum : 0.f;
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-        if (lane + 32 * j < a.D) ((T *)a.out)[rh * a.D + lane + 32 * j] = dtype_traits<T>::from_f(acc[j] * inv);
+        if (lane + 32 * j < a.D) at_put<T>(a, rh * a.D + lane + 32 * j, acc[j] * inv);
     if (lane == 0 && a.lse) a.lse[rh] = some ? m + log2f(sum) : INFINITY;
 }
 
@@ -244,6 +251,7 @@ static int at_prepare(const spconv_attention_args *q, const AtPlan &p, bool back
     a.grad = {q->grad_out, q->grad_row, q->grad_head};
     a.out = q->out;
     a.out_in = q->out;
+    a.rest = q->dtype == SPCONV_F32 ? nullptr : q->out_rest;
     a.lse = q->row_stats;
     a.gq = q->grad_query;
     a.gk = q->grad_key;
@@ -317,7 +325,8 @@ extern "C" int spconv_attention_backward(const spconv_attention_args *q, void *s
     AtArgs a;
     if (const int rc = at_prepare(q, p, true, (cudaStream_t)stream, a)) return rc;
     if (a.M > 0) {
-        const bool wide = a.D % 8 == 0 && (((uintptr_t)q->grad_out | (uintptr_t)q->out) & 15) == 0 && q->grad_row % 8 == 0 && q->grad_head % 8 == 0;
+        const bool wide = a.D % 8 == 0 && (((uintptr_t)q->grad_out | (uintptr_t)q->out | (uintptr_t)q->out_rest) & 15) == 0 &&
+                          q->grad_row % 8 == 0 && q->grad_head % 8 == 0;
         AtArgs d = a;
         d.grad = {q->grad_out, q->grad_row, q->grad_head};
         const int rc = at_by_type(a.dtype, [&](auto *t) {

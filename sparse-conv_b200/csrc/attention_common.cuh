@@ -66,4 +66,12 @@ __device__ __forceinline__ void at_split(int splits, int s, int count, int &firs
     last = min(count, first + per);
 }
 
+// Stores a result and, where it is kept, what rounding took from it.
+template <typename T>
+__device__ __forceinline__ void at_put(const AtArgs &a, int64_t i, float x) {
+    const T hi = dtype_traits<T>::from_f(x);
+    ((T *)a.out)[i] = hi;
+    if (a.rest) ((T *)a.rest)[i] = dtype_traits<T>::from_f(x - dtype_traits<T>::to_f(hi));
+}
+
 }  // namespace spconv

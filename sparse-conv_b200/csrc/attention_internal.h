@@ -16,6 +16,7 @@ struct AtArgs {
     AtTensor q, k, v, grad;
     void *out, *gq, *gk, *gv;            // contiguous
     const void *out_in;                  // the backward's: the forward's output, contiguous
+    void *rest;                          // what out's rounding left out, or null
     float *lse;                          // [num_queries, heads]: log2 of the row's sum, + inf where it sees no key
     float *delta;                        // [num_queries, heads]: grad . out
     const int32_t *offsets, *key_offsets;

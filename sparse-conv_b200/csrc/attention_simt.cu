@@ -216,7 +216,7 @@ attention_simt_kernel(const __grid_constant__ AtArgs a) {
         const float inv = 1.f / sum[i];
 #pragma unroll
         for (int j = 0; j < S::C; ++j)
-            if (tx + 16 * j < a.D) ((T *)a.out)[at * a.D + tx + 16 * j] = dtype_traits<T>::from_f(none ? 0.f : as_sum(acc[i][j]) * inv);
+            if (tx + 16 * j < a.D) at_put<T>(a, at * a.D + tx + 16 * j, none ? 0.f : as_sum(acc[i][j]) * inv);
     }
 }
 

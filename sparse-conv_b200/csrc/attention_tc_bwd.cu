@@ -22,8 +22,7 @@
 // functions 45 and 32 %, the issue slots 58 and 53 %.
 //
 // p of the keys' sweep is scaled by 2^15 in fp16, whose smallest values would else lose bits where a row sees
-// thousands of keys; grad_value is scaled back in fp32. A row that sees a single key has ds = 0 exactly. delta takes the
-// rounded out: with few keys a row grad_query and grad_key are off by two or three roundings, not one.
+// thousands of keys; grad_value is scaled back in fp32. A row that sees a single key has ds = 0 exactly.
 // Rows behind a sample's end are treated as in the forward: zeroed in shared memory where a product sums over rows.
 #include <algorithm>
 

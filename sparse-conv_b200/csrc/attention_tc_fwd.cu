@@ -49,7 +49,7 @@ __device__ __forceinline__ void af_store(const AtArgs &a, uint32_t t_o, int size
         else if (a.lse) a.lse[at] = none ? INFINITY : fmaf(top, a.c, log2f(sum));
     }
     T *out = (T *)a.out + at * a.D;
-    const bool wide = (a.D & 7) == 0 && ((uintptr_t)a.out & 15) == 0;
+    const bool wide = (a.D & 7) == 0 && (((uintptr_t)a.out | (uintptr_t)a.rest) & 15) == 0;
 #pragma unroll 1
     for (int c = 0; c < size && c < a.D; c += 16) {
         uint32_t o[16];
@@ -71,11 +71,22 @@ __device__ __forceinline__ void af_store(const AtArgs &a, uint32_t t_o, int size
                 for (int i = 0; i < 8; ++i)
                     if (d + i < a.D) part[d + i] = f[i];
             } else if (wide) {
-                *(uint4 *)(out + d) = make_uint4(lt_pack<T>(f[0], f[1]), lt_pack<T>(f[2], f[3]), lt_pack<T>(f[4], f[5]), lt_pack<T>(f[6], f[7]));
+                uint32_t w[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] = lt_pack<T>(f[2 * i], f[2 * i + 1]);
+                *(uint4 *)(out + d) = make_uint4(w[0], w[1], w[2], w[3]);
+                if (a.rest) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float2 hi = lt_unpack<T>(w[i]);
+                        w[i] = lt_pack<T>(f[2 * i] - hi.x, f[2 * i + 1] - hi.y);
+                    }
+                    *(uint4 *)((T *)a.rest + at * a.D + d) = make_uint4(w[0], w[1], w[2], w[3]);
+                }
             } else {
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
-                    if (d + i < a.D) out[d + i] = dtype_traits<T>::from_f(f[i]);
+                    if (d + i < a.D) at_put<T>(a, at * a.D + d + i, f[i]);
             }
         }
     }

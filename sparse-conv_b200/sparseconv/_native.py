@@ -40,6 +40,7 @@ NOALLOC_MAX_COORDS = 262144   # SPCONV_NOALLOC_MAX_COORDS
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}   # SPCONV_ACT_*
 ROTARY_LAYOUTS = {"half": 0, "interleaved": 1}               # SPCONV_ROTARY_*
 ROTARY_MAX_PAIRS = 128
+ATTENTION_FEW_KEYS = 128      # mean keys a sample up to which the backward takes out before its rounding
 NORMS = {"none": 0, "layer": 1, "rms": 2}                    # SPCONV_NORM_*
 CLIP_P2, CLIP_INF = 0, 1
 
@@ -84,7 +85,7 @@ class AttentionArgs(ctypes.Structure):
                 ("causal", _c_int), ("scale", ctypes.c_float), ("offsets", _c_void_p), ("key_offsets", _c_void_p),
                 ("query", _c_void_p), ("key", _c_void_p), ("value", _c_void_p),
                 ("query_row", _c_i64), ("query_head", _c_i64), ("key_row", _c_i64), ("key_head", _c_i64),
-                ("value_row", _c_i64), ("value_head", _c_i64), ("out", _c_void_p), ("row_stats", _c_void_p),
+                ("value_row", _c_i64), ("value_head", _c_i64), ("out", _c_void_p), ("out_rest", _c_void_p), ("row_stats", _c_void_p),
                 ("grad_out", _c_void_p), ("grad_row", _c_i64), ("grad_head", _c_i64),
                 ("grad_query", _c_void_p), ("grad_key", _c_void_p), ("grad_value", _c_void_p),
                 ("workspace", _c_void_p), ("workspace_bytes", _c_i64), ("status", _c_void_p)]
@@ -1180,7 +1181,8 @@ def _attention_args(dtype: torch.dtype, heads: int, key_heads: int, size: int, c
 def attention_forward(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, offsets: Optional[torch.Tensor],
                       key_offsets: Optional[torch.Tensor], causal: bool, scale: float, keep_stats: bool = False,
                       kernel: int = KERNEL_AUTO) -> tuple:
-    """(out, row statistics if ``keep_stats`` else None, the call's arguments for attention_backward_of)."""
+    """(out, what the backward needs of it if ``keep_stats``: row statistics and, where rows see few keys on average, what
+    out's rounding left out, else None; the call's arguments for attention_backward_of)."""
     dev = _require_cuda(query, key, value, offsets, key_offsets)
     dtype = query.dtype
     if key.dtype != dtype or value.dtype != dtype:
@@ -1208,6 +1210,10 @@ def attention_forward(query: torch.Tensor, key: torch.Tensor, value: torch.Tenso
     if keep_stats:
         stats = torch.empty((M, H), dtype=torch.float32, device=dev)
         a.row_stats = stats.data_ptr()
+        if N <= ATTENTION_FEW_KEYS * a.num_samples and dtype != torch.float32:
+            rest = torch.empty_like(out)
+            a.out_rest = rest.data_ptr()
+            stats = (stats, rest)
     if M == 0:
         return out, stats, a
     ws = _attention_workspace(a, False, dev)
@@ -1231,6 +1237,9 @@ def attention_backward_of(args: AttentionArgs, query, key, value, offsets, key_o
     (a.query_row, a.query_head, _), (a.key_row, a.key_head, _), (a.value_row, a.value_head, _) = (
         query.stride(), key.stride(), value.stride())
     a.offsets, a.key_offsets = _ptr(offsets), _ptr(key_offsets)
+    if isinstance(stats, tuple):
+        stats, rest = stats
+        a.out_rest = rest.data_ptr()
     a.out, a.row_stats = out.data_ptr(), stats.data_ptr()
     a.grad_out, a.grad_row, a.grad_head = grad_out.data_ptr(), grad_out.stride(0), grad_out.stride(1)
     grads = [t.new_empty(t.shape) if n else None for t, n in zip((query, key, value), needs)]

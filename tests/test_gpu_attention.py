@@ -154,6 +154,23 @@ def test_one_key_has_no_score_gradient(dtype):
     assert (gq[0] == 0).all() and (gq[1] != 0).any()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D", [33, 64, 128, 136])
+@pytest.mark.parametrize("m", [2, 3, 16])
+def test_few_keys_keep_their_digits(dtype, D, m):
+    """ds is a difference of grad . v and grad . out: with few keys out's rounding would be as large as any. With it out of the
+    way, p's (in out and in the values' gradient), ds's and the result's roundings are left, 0.42 half steps each in the mean
+    square of a uniform mantissa: at most sqrt(3) of them, under one half step."""
+    lengths = [m] * 200
+    g = torch.Generator(device="cuda").manual_seed(D + m)
+    q, k, v, grad = (torch.randn(200 * m, 2, D, generator=g, device="cuda").to(dtype) for _ in range(4))
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    got = torch.autograd.grad(sparse_attention(*leaves, ends(lengths)), leaves, grad)
+    _, want = reference(*leaves, lengths, lengths, False, D ** -0.5, grad)
+    for name, a, b in zip("qkv", got, want):
+        assert relative(a, b) < torch.finfo(dtype).eps / 2, (name, relative(a, b))
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_peaked_and_growing_scores(dtype):
     """Scores that rise along the keys, so that the running maximum changes in every tile, and large ones."""
