@@ -24,40 +24,74 @@ attention_pack_kernel(AtTensor t, T *out, int64_t rows, int heads, int D, int to
     }
 }
 
-// delta[row, head] = grad . (out + what its rounding left out, where that is kept), eight lanes each. Bound: HBM.
+// The largest of the block's values into *peak, which starts at 0 (NaN above all): the same whatever the order.
+__device__ __forceinline__ void at_peak(float *peak, float square) {
+    __shared__ uint32_t tops[kAtThreads / 32];
+    const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(square));
+    if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        uint32_t most = 0;
+        for (int w = 0; w < kAtThreads / 32; ++w) most = max(most, tops[w]);
+        if (most > *(volatile uint32_t *)peak) atomicMax((uint32_t *)peak, most);
+    }
+}
+
+// Eight lanes a row and head, of which they have x . y (and x . (y + rest)) and x . x. Bound: HBM.
 template <typename T, bool WIDE>
-__global__ void __launch_bounds__(kAtThreads)
-attention_delta_kernel(const __grid_constant__ AtArgs a) {
-    const int64_t rh = ((int64_t)blockIdx.x * kAtThreads + threadIdx.x) >> 3;
+__device__ __forceinline__ void at_dots(const T *x, const T *y, const T *rest, int D, bool in, float &xy, float &xx) {
     const int lane = threadIdx.x & 7;
-    const bool in = rh < (int64_t)a.M * a.H;
-    float s = 0.f;
+    xy = xx = 0.f;
     if (in) {
-        const int64_t r = rh / a.H;
-        const T *g = (const T *)a.grad.p + r * a.grad.row + (rh - r * a.H) * a.grad.head;
-        const T *o = (const T *)a.out_in + rh * a.D, *rest = a.rest ? (const T *)a.rest + rh * a.D : nullptr;
-        if constexpr (WIDE) {
-            constexpr int V = 16 / sizeof(T);
-            for (int d = lane * V; d < a.D; d += 8 * V) {
-                const uint4 x = *(const uint4 *)(g + d), y = *(const uint4 *)(o + d);
-#pragma unroll
-                for (int i = 0; i < V; ++i)
-                    s = fmaf(dtype_traits<T>::to_f(((const T *)&x)[i]), dtype_traits<T>::to_f(((const T *)&y)[i]), s);
-                if (rest) {
-                    const uint4 z = *(const uint4 *)(rest + d);
-#pragma unroll
-                    for (int i = 0; i < V; ++i)
-                        s = fmaf(dtype_traits<T>::to_f(((const T *)&x)[i]), dtype_traits<T>::to_f(((const T *)&z)[i]), s);
-                }
+        constexpr int V = WIDE ? 16 / (int)sizeof(T) : 1;
+        for (int d = lane * V; d < D; d += 8 * V) {
+            T p[V], q[V], r[V];
+            if constexpr (WIDE) {
+                *(uint4 *)p = *(const uint4 *)(x + d);
+                if (y) *(uint4 *)q = *(const uint4 *)(y + d);
+                if (rest) *(uint4 *)r = *(const uint4 *)(rest + d);
+            } else {
+                p[0] = x[d];
+                if (y) q[0] = y[d];
+                if (rest) r[0] = rest[d];
             }
-        } else {
-            for (int d = lane; d < a.D; d += 8)
-                s = fmaf(dtype_traits<T>::to_f(g[d]), dtype_traits<T>::to_f(o[d]) + (rest ? dtype_traits<T>::to_f(rest[d]) : 0.f), s);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const float f = dtype_traits<T>::to_f(p[i]);
+                xx = fmaf(f, f, xx);
+                if (y) xy = fmaf(f, dtype_traits<T>::to_f(q[i]), xy);
+                if (rest) xy = fmaf(f, dtype_traits<T>::to_f(r[i]), xy);
+            }
         }
     }
 #pragma unroll
-    for (int o = 4; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (in && lane == 0) a.delta[rh] = s;
+    for (int o = 4; o; o >>= 1) {
+        xy += __shfl_xor_sync(0xffffffffu, xy, o);
+        xx += __shfl_xor_sync(0xffffffffu, xx, o);
+    }
+}
+
+// delta[row, head] = grad . (out + what its rounding left out, where that is kept), and grad's largest square.
+template <typename T, bool WIDE>
+__global__ void __launch_bounds__(kAtThreads)
+attention_delta_kernel(const __grid_constant__ AtArgs a) {
+    const int64_t rh = ((int64_t)blockIdx.x * kAtThreads + threadIdx.x) >> 3, r = rh / a.H;
+    const bool in = rh < (int64_t)a.M * a.H;
+    float dot, square;
+    at_dots<T, WIDE>((const T *)a.grad.p + r * a.grad.row + (rh - r * a.H) * a.grad.head, (const T *)a.out_in + rh * a.D,
+                     a.rest ? (const T *)a.rest + rh * a.D : nullptr, a.D, in, dot, square);
+    if (in && (threadIdx.x & 7) == 0) a.delta[rh] = dot;
+    if (a.peaks) at_peak(a.peaks, square);
+}
+
+// v's largest square.
+template <typename T, bool WIDE>
+__global__ void __launch_bounds__(kAtThreads)
+attention_peak_kernel(const __grid_constant__ AtArgs a) {
+    const int64_t rh = ((int64_t)blockIdx.x * kAtThreads + threadIdx.x) >> 3, r = rh / a.K;
+    float none, square;
+    at_dots<T, WIDE>((const T *)a.v.p + r * a.v.row + (rh - r * a.K) * a.v.head, nullptr, nullptr, a.D, rh < (int64_t)a.N * a.K, none, square);
+    at_peak(a.peaks + 1, square);
 }
 
 // A row's splits: out = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s. `share` warps take a row's splits in turn and add up in
@@ -147,7 +181,7 @@ struct AtPlan {
     bool pair;                           // forward: two tiles a CTA
     int splits[3];                       // forward (or queries' gradients), and keys' gradients
     bool pack[4];                        // q, k, v, grad
-    int64_t pack_at[4], delta_at, ml_at, partial_at, bytes;
+    int64_t pack_at[4], delta_at, peaks_at, ml_at, partial_at, bytes;
 };
 
 // Splits of `tiles` steps each of `ctas` CTAs, of which `slots` run at a time, none of fewer than `least` steps. The
@@ -206,6 +240,7 @@ static AtPlan at_plan(const spconv_attention_args *q, bool backward) {
     const int64_t rows = M * q->heads, krows = N * q->key_heads;
     if (backward) {
         p.delta_at = take(rows * 4);
+        p.peaks_at = take(8);
         p.partial_at = take(std::max(p.splits[0] > 1 ? p.splits[0] * rows * q->head_size * 4 : 0,
                                      p.splits[1] > 1 ? 2 * p.splits[1] * krows * q->head_size * 4 : 0));
     } else if (p.splits[0] > 1) {
@@ -273,6 +308,7 @@ static int at_prepare(const spconv_attention_args *q, const AtPlan &p, bool back
     a.stream = st;
     uint8_t *ws = (uint8_t *)q->workspace;
     a.delta = (float *)(ws + p.delta_at);
+    a.peaks = backward && p.tc && q->dtype == SPCONV_F16 ? (float *)(ws + p.peaks_at) : nullptr;
     a.part_ml = (float2 *)(ws + p.ml_at);
     a.partial = (float *)(ws + p.partial_at);
     AtTensor *t[4] = {&a.q, &a.k, &a.v, &a.grad};
@@ -289,6 +325,13 @@ static int at_prepare(const spconv_attention_args *q, const AtPlan &p, bool back
         *t[i] = {dst, (int64_t)heads * to, to};
     }
     return SPCONV_OK;
+}
+
+// The arguments with heads as wide as their rows of whole 16 bytes (zeros behind a packed head's end).
+static AtArgs at_whole(const AtArgs &a) {
+    AtArgs w = a;
+    w.D = (a.D + 7) / 8 * 8;
+    return w;
 }
 
 }  // namespace spconv
@@ -327,6 +370,7 @@ extern "C" int spconv_attention_backward(const spconv_attention_args *q, void *s
     if (a.M > 0) {
         const bool wide = a.D % 8 == 0 && (((uintptr_t)q->grad_out | (uintptr_t)q->out | (uintptr_t)q->out_rest) & 15) == 0 &&
                           q->grad_row % 8 == 0 && q->grad_head % 8 == 0;
+        if (a.peaks && cudaMemsetAsync(a.peaks, 0, 8, a.stream) != cudaSuccess) return check_launch("attention: clear");
         AtArgs d = a;
         d.grad = {q->grad_out, q->grad_row, q->grad_head};
         const int rc = at_by_type(a.dtype, [&](auto *t) {
@@ -336,6 +380,10 @@ extern "C" int spconv_attention_backward(const spconv_attention_args *q, void *s
             return check_launch("attention_delta_kernel");
         });
         if (rc) return rc;
+        if (a.peaks) {                       // (a.v as the products read it: packed where its own layout is not aligned)
+            attention_peak_kernel<__half, true><<<at_blocks((int64_t)a.N * a.K * 8), kAtThreads, 0, a.stream>>>(at_whole(a));
+            if (const int rc2 = check_launch("attention_peak_kernel")) return rc2;
+        }
     }
     auto join = [&](const float *from, int64_t stride, void *to, int64_t n) {
         if (!to || n == 0) return (int)SPCONV_OK;

@@ -66,6 +66,17 @@ __device__ __forceinline__ void at_split(int splits, int s, int count, int &firs
     last = min(count, first + per);
 }
 
+// The power of two by which ds is lifted where it has to be rounded to fp16: |ds| <= 2 |grad row| |v row|, so the largest is
+// at most 2^15, and rows of thousands of keys, or gradients of any size, keep their digits above fp16's smallest values.
+__device__ __forceinline__ int at_lift(const AtArgs &a) {
+    if (!a.peaks) return 0;
+    const float x = sqrtf(__ldg(a.peaks)) * sqrtf(__ldg(a.peaks + 1));
+    if (!(x > 0.f && x < INFINITY)) return 0;
+    int e;
+    frexpf(x, &e);                       // x <= 2^e
+    return max(-60, min(60, 14 - e));
+}
+
 // Stores a result and, where it is kept, what rounding took from it.
 template <typename T>
 __device__ __forceinline__ void at_put(const AtArgs &a, int64_t i, float x) {

@@ -21,8 +21,9 @@
 // 1.16 and 1.60 ms, 1.25 and 1.21 PFLOP/s. Nothing is full: at 8 x 64 the tensor pipe is 45 and 43 % in use, the special
 // functions 45 and 32 %, the issue slots 58 and 53 %.
 //
-// p of the keys' sweep is scaled by 2^15 in fp16, whose smallest values would else lose bits where a row sees
-// thousands of keys; grad_value is scaled back in fp32. A row that sees a single key has ds = 0 exactly.
+// In fp16, whose smallest values would else lose bits where a row sees thousands of keys or gradients are small, p of
+// the keys' sweep comes times 2^15, and ds times the power of two that its bound allows (at_lift); the results are
+// scaled back in fp32. A row that sees a single key has ds = 0 exactly.
 // Rows behind a sample's end are treated as in the forward: zeroed in shared memory where a product sums over rows.
 #include <algorithm>
 
@@ -244,7 +245,8 @@ attention_tc_grad_query_kernel(const __grid_constant__ CUtensorMap map_q, const 
         const int seen_all = __reduce_min_sync(0xffffffffu, mine ? seen : m);
         const int64_t at = (int64_t)(s.q0 + token) * a.H + head0 + (row & (P - 1));
         const float lse = mine ? a.lse[at] : INFINITY, delta = mine ? a.delta[at] : 0.f;
-        const f32x2 c2 = pack_f32x2(a.c, a.c), l2 = pack_f32x2(-lse, -lse), d2 = pack_f32x2(-delta, -delta);
+        const int lift = at_lift(a);                                 // p, and so ds, comes times 2^lift
+        const f32x2 c2 = pack_f32x2(a.c, a.c), l2 = pack_f32x2(lift - lse, lift - lse), d2 = pack_f32x2(-delta, -delta);
         bool ok = true;
         for (int j = 0; j < tiles; ++j) {
             const uint32_t t_s = tmem + (j & 1) * W + part * 32 + lanes;
@@ -284,7 +286,7 @@ attention_tc_grad_query_kernel(const __grid_constant__ CUtensorMap map_q, const 
         if (ok && some) {
             constexpr int kCols = DP * 32 / W > 32 ? DP * 32 / W : 32;               // a part's (with more parts than 32s: none)
             float *to = a.splits > 1 ? a.partial + (blockIdx.z * (int64_t)a.M * a.H + at) * a.D : nullptr;
-            ab_store_row<T>(t_dq + lanes, part * kCols, part * kCols + kCols, a.D, tiles == 0, a.scale, mine, (T *)a.gq + at * a.D, to);
+            ab_store_row<T>(t_dq + lanes, part * kCols, part * kCols + kCols, a.D, tiles == 0, ldexpf(a.scale, -lift), mine, (T *)a.gq + at * a.D, to);
         }
     }
 
@@ -315,6 +317,8 @@ attention_tc_grad_key_kernel(const __grid_constant__ CUtensorMap map_q, const __
     using S = AkShape<DP, W>;
     constexpr float kUp = dtype_traits<T>::mma_format == 0 ? 15.f : 0.f;         // powers of two on p
     constexpr float kDown = dtype_traits<T>::mma_format == 0 ? 0x1p-15f : 1.f;
+    const int lift = at_lift(a);                                     // ds comes times 2^lift
+    const float down = ldexpf(kDown, lift);
     extern __shared__ uint8_t smem_raw[];
     uint8_t *base = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     const uint32_t s_k = smem_u32(base), s_v = s_k + S::kOwn, s_q = s_v + S::kOwn;      // stages of q, grad
@@ -416,7 +420,7 @@ attention_tc_grad_key_kernel(const __grid_constant__ CUtensorMap map_q, const __
                     const int r = lane + 32 * i;
                     const int64_t at = (int64_t)(s.q0 + w.t * tokens + (r >> log_p)) * a.H + w.head + (r & (P - 1));
                     lse[i] = r < rows ? kUp - __ldg(a.lse + at) : -INFINITY;
-                    delta[i] = r < rows ? -kDown * __ldg(a.delta + at) : 0.f;
+                    delta[i] = r < rows ? -down * __ldg(a.delta + at) : 0.f;
                 }
                 if (!(ok = __all_sync(0xffffffffu, wait(&empty[st], phase)) != 0)) break;
                 const uint32_t dst = s_q + st * 2 * S::kTile, mbar = smem_u32(cut ? tail : &full[st]);
@@ -491,7 +495,7 @@ attention_tc_grad_key_kernel(const __grid_constant__ CUtensorMap map_q, const __
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t t_s = tmem + part * 32 + lanes, t_d = t_dp + part * 32 + lanes;
         const bool mine = key < m;
-        const f32x2 c2 = pack_f32x2(a.c, a.c), k2 = pack_f32x2(kDown, kDown);
+        const f32x2 c2 = pack_f32x2(a.c, a.c), k2 = pack_f32x2(down, down);
         bool ok = true;
         int st = 0;
         uint32_t phase = 0, t_phase = 0;
@@ -566,7 +570,8 @@ attention_tc_grad_key_kernel(const __grid_constant__ CUtensorMap map_q, const __
             float *to = a.splits > 1 ? a.partial + ((2 * blockIdx.z + !keys) * all + at) * a.D : nullptr;
             T *out = (T *)(keys ? a.gk : a.gv);
             const int c0 = (part & (kParts - 1)) * kCols;
-            ab_store_row<T>((keys ? t_dk : t_dv) + lanes, c0, c0 + kCols, a.D, tiles == 0, keys ? a.scale : kDown, mine && (out || to),
+            ab_store_row<T>((keys ? t_dk : t_dv) + lanes, c0, c0 + kCols, a.D, tiles == 0, keys ? ldexpf(a.scale, -lift) : kDown,
+                            mine && (out || to),
                             out ? out + at * a.D : nullptr, to);
         }
     }

@@ -172,6 +172,24 @@ def test_few_keys_keep_their_digits(dtype, D, m):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("size", [2.0 ** -12, 1.0, 2.0 ** 10])
+@pytest.mark.parametrize("n,D", [(40, 64), (3000, 64), (700, 128), (90, 33)])
+def test_gradients_of_any_size(dtype, size, n, D):
+    """Gradients far from 1 at rows of thousands of keys: ds is p times them, which fp16 could not hold as it is. The values' scale
+    brings the results back to where fp16 holds them."""
+    g = torch.Generator(device="cuda").manual_seed(n + D)
+    q, k, v, grad = (torch.randn(n, 2, D, generator=g, device="cuda") for _ in range(4))
+    leaves = [t.to(dtype).requires_grad_() for t in (q, k, v * (1.0 if size == 1.0 else 2.0 ** -4 if size > 1.0 else 64.0))]
+    grad = (grad * size).to(dtype)
+    got = torch.autograd.grad(sparse_attention(*leaves), leaves, grad)
+    _, want = reference(*leaves, [n], [n], False, D ** -0.5, grad)
+    for name, a, b in zip("qkv", got, want):
+        # the results themselves: half of fp16's smallest step, over a result's root mean square
+        small = 2.0 ** -25 / (b.norm().item() / b.numel() ** 0.5) if dtype == torch.float16 else 0.0
+        assert relative(a, b) < tolerance(dtype) / 2 + small, (name, relative(a, b))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_peaked_and_growing_scores(dtype):
     """Scores that rise along the keys, so that the running maximum changes in every tile, and large ones."""
     n, D = 700, 64
