@@ -84,14 +84,42 @@ attention_delta_kernel(const __grid_constant__ AtArgs a) {
     if (a.peaks) at_peak(a.peaks, square);
 }
 
-// v's largest square.
-template <typename T, bool WIDE>
+// v's largest square: eight lanes take four rows and heads at a time, of whole 16 bytes.
 __global__ void __launch_bounds__(kAtThreads)
 attention_peak_kernel(const __grid_constant__ AtArgs a) {
-    const int64_t rh = ((int64_t)blockIdx.x * kAtThreads + threadIdx.x) >> 3, r = rh / a.K;
-    float none, square;
-    at_dots<T, WIDE>((const T *)a.v.p + r * a.v.row + (rh - r * a.K) * a.v.head, nullptr, nullptr, a.D, rh < (int64_t)a.N * a.K, none, square);
-    at_peak(a.peaks + 1, square);
+    constexpr int B = 4;
+    const int lane = threadIdx.x & 7;
+    const int64_t rows = (int64_t)a.N * a.K, group = ((int64_t)blockIdx.x * kAtThreads + threadIdx.x) >> 3;
+    const int64_t groups = (int64_t)gridDim.x * (kAtThreads / 8);
+    float most = 0.f;
+    bool nan = false;
+    for (int64_t first = group; first < rows; first += groups * B) {
+        float square[B] = {};
+        for (int d = lane * 8; d < a.D; d += 64) {
+            uint4 x[B];
+#pragma unroll
+            for (int k = 0; k < B; ++k) {
+                const int64_t rh = first + k * groups, r = rh / a.K;
+                x[k] = make_uint4(0, 0, 0, 0);
+                if (rh < rows) x[k] = __ldg((const uint4 *)((const __half *)a.v.p + r * a.v.row + (rh - r * a.K) * a.v.head + d));
+            }
+#pragma unroll
+            for (int k = 0; k < B; ++k)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float2 f = __half22float2(reinterpret_cast<const __half2 *>(&x[k])[i]);
+                    square[k] = fmaf(f.x, f.x, fmaf(f.y, f.y, square[k]));
+                }
+        }
+#pragma unroll
+        for (int k = 0; k < B; ++k) {
+#pragma unroll
+            for (int o = 4; o; o >>= 1) square[k] += __shfl_xor_sync(0xffu << (threadIdx.x & 24), square[k], o);
+            most = fmaxf(most, square[k]);
+            nan |= isnan(square[k]);
+        }
+    }
+    at_peak(a.peaks + 1, nan ? NAN : most);
 }
 
 // A row's splits: out = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s. `share` warps take a row's splits in turn and add up in
@@ -184,17 +212,14 @@ struct AtPlan {
     int64_t pack_at[4], delta_at, peaks_at, ml_at, partial_at, bytes;
 };
 
-// Splits of `tiles` steps each of `ctas` CTAs, of which `slots` run at a time, none of fewer than `least` steps. The
-// tensor-core kernels are cut only where CTAs do not fill the slots (a split's rows are written and read once more in fp32:
-// 4,096 tokens x 8 heads in 256 CTAs for 592 slots: 94 us whole, 126 us in two), the CUDA-core kernels, whose steps take as long as
-// a row's joining, also into whole waves.
-static int at_cut(int64_t ctas, int64_t slots, int64_t tiles, int least, bool waves) {
-    if (ctas == 0 || ctas >= (waves ? 4 : 1) * slots) return 1;
-    const int64_t most = std::max<int64_t>(1, std::min<int64_t>({tiles / least, (waves ? 4 : 1) * slots / ctas, 256}));
-    if (!waves) return (int)most;
+// Splits of `tiles` steps each of `ctas` CTAs, of which `slots` run at a time: whole waves, none of fewer than `least` steps. A CTA's
+// start and end count as two steps, and the joining, in the kernels' own time, as six.
+static int at_cut(int64_t ctas, int64_t slots, int64_t tiles, int least) {
+    if (ctas == 0 || ctas >= 4 * slots) return 1;
+    const int64_t most = std::max<int64_t>(1, std::min<int64_t>({tiles / least, 4 * slots / ctas, 256}));
     int64_t best = 1, best_cost = INT64_MAX;
     for (int64_t s = 1; s <= most; ++s) {
-        const int64_t cost = ((ctas * s + slots - 1) / slots) * ((tiles + s - 1) / s + (s > 1 ? 6 : 2));
+        const int64_t cost = ((ctas * s + slots - 1) / slots) * ((tiles + s - 1) / s + 2) + (s > 1 ? 6 : 0);
         if (cost < best_cost) {
             best_cost = cost;
             best = s;
@@ -217,12 +242,12 @@ static AtPlan at_plan(const spconv_attention_args *q, bool backward) {
         p.pair = !backward && q->head_size > 64 && rows > 192 && mean_k > 512 && B * up(rows, 256) * heads >= 148;
         // CTAs that run at a time, and what each has to have for itself: 512 keys (a split's rows are written and read once more)
         const int64_t per_sm = q->head_size > 64 ? 1 : 2;
-        p.splits[0] = at_cut(B * up(rows, 128) * heads, 148 * (backward ? per_sm : 2 * per_sm), up(mean_k, 128), 8, false);
-        p.splits[1] = at_cut(B * up(mean_k, 128) * q->key_heads, 148 * per_sm, up(rows, 128) * (G / P), 8, false);
+        p.splits[0] = at_cut(B * up(rows, 128) * heads, 148 * (backward ? per_sm : 2 * per_sm), up(mean_k, 128), 4);
+        p.splits[1] = at_cut(B * up(mean_k, 128) * q->key_heads, 148 * per_sm, up(rows, 128) * (G / P), 4);
     } else {
         const int64_t R = at_simt_rows(q->head_size);
-        p.splits[0] = at_cut(B * up(mean_q, R) * q->heads, 296, up(mean_k, R), 4, true);
-        p.splits[1] = at_cut(B * up(mean_k, R) * q->key_heads, 296, up(mean_q, R) * G, 4, true);
+        p.splits[0] = at_cut(B * up(mean_q, R) * q->heads, 296, up(mean_k, R), 4);
+        p.splits[1] = at_cut(B * up(mean_k, R) * q->key_heads, 296, up(mean_q, R) * G, 4);
     }
     int64_t at = 0;
     auto take = [&](int64_t bytes) {
@@ -381,7 +406,8 @@ extern "C" int spconv_attention_backward(const spconv_attention_args *q, void *s
         });
         if (rc) return rc;
         if (a.peaks) {                       // (a.v as the products read it: packed where its own layout is not aligned)
-            attention_peak_kernel<__half, true><<<at_blocks((int64_t)a.N * a.K * 8), kAtThreads, 0, a.stream>>>(at_whole(a));
+            const unsigned blocks = (unsigned)std::min<int64_t>(at_blocks((int64_t)a.N * a.K * 8), 148 * 8);
+            attention_peak_kernel<<<blocks, kAtThreads, 0, a.stream>>>(at_whole(a));
             if (const int rc2 = check_launch("attention_peak_kernel")) return rc2;
         }
     }

@@ -61,7 +61,10 @@ __device__ __forceinline__ void ab_store_row(uint32_t taddr, int from, int to, i
                 f[2 * i + 1] = zero ? 0.f : u.y * factor;
                 w[i] = lt_pack<T>(f[2 * i], f[2 * i + 1]);
             }
-            if (part) {
+            if (part && (D & 7) == 0) {                              // (the workspace is aligned, and so are rows of eights)
+                *(float4 *)(part + d) = make_float4(f[0], f[1], f[2], f[3]);
+                *(float4 *)(part + d + 4) = make_float4(f[4], f[5], f[6], f[7]);
+            } else if (part) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
                     if (d + i < D) part[d + i] = f[i];

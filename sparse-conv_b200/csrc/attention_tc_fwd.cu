@@ -66,7 +66,10 @@ __device__ __forceinline__ void af_store(const AtArgs &a, uint32_t t_o, int size
             float f[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) f[i] = none ? 0.f : __uint_as_float(o[v * 8 + i]) * inv;
-            if (part) {
+            if (part && (a.D & 7) == 0) {                            // (the workspace is aligned, and so are rows of eights)
+                *(float4 *)(part + d) = make_float4(f[0], f[1], f[2], f[3]);
+                *(float4 *)(part + d + 4) = make_float4(f[4], f[5], f[6], f[7]);
+            } else if (part) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
                     if (d + i < a.D) part[d + i] = f[i];
