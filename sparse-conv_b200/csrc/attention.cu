@@ -242,7 +242,8 @@ static AtPlan at_plan(const spconv_attention_args *q, bool backward) {
         p.pair = !backward && q->head_size > 64 && rows > 192 && mean_k > 512 && B * up(rows, 256) * heads >= 148;
         // CTAs that run at a time, and what each has to have for itself: 512 keys (a split's rows are written and read once more)
         const int64_t per_sm = q->head_size > 64 ? 1 : 2;
-        p.splits[0] = at_cut(B * up(rows, 128) * heads, 148 * (backward ? per_sm : 2 * per_sm), up(mean_k, 128), 4);
+        p.splits[0] = p.pair ? at_cut(B * up(rows, 256) * heads, 148, up(mean_k, 128), 4)
+                             : at_cut(B * up(rows, 128) * heads, 148 * (backward ? per_sm : 2 * per_sm), up(mean_k, 128), 4);
         p.splits[1] = at_cut(B * up(mean_k, 128) * q->key_heads, 148 * per_sm, up(rows, 128) * (G / P), 4);
     } else {
         const int64_t R = at_simt_rows(q->head_size);

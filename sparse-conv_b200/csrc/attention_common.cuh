@@ -17,8 +17,10 @@ struct AtSample {
 
 // The sample that tile `t` belongs to, where sample b's tiles are numbered from rows(b) / per_tile + b (its rows
 // never need more than the next one's number; a tile past a sample's end has nothing to do). By a converged warp, 32 samples
-// a step; ends inside [0, B) whatever the offsets hold.
-__device__ __forceinline__ AtSample at_find(const int32_t *by, int rows, const AtArgs &a, int t, int per_tile) {
+// a step; ends inside [0, B) whatever the offsets hold, with a tile that begins inside the sample's rows, or -1.
+__device__ __forceinline__ AtSample at_find(const AtArgs &a, bool keys, int t, int per_tile) {
+    const int32_t *by = keys ? a.key_offsets : a.offsets;
+    const int rows = keys ? a.N : a.M;
     const int lane = threadIdx.x & 31;
     int lo = 0, hi = a.B;
     while (hi - lo > 1) {
@@ -35,6 +37,8 @@ __device__ __forceinline__ AtSample at_find(const int32_t *by, int rows, const A
     s.q1 = max(s.q0, at_offset(a.offsets, lo + 1, a.M));
     s.k0 = at_offset(a.key_offsets, lo, a.N);
     s.k1 = max(s.k0, at_offset(a.key_offsets, lo + 1, a.N));
+    const int own = keys ? s.k1 - s.k0 : s.q1 - s.q0;
+    if (s.tile < 0 || s.tile >= own / per_tile + (own % per_tile != 0)) s.tile = -1;
     return s;
 }
 

@@ -130,10 +130,10 @@ __device__ __forceinline__ void as_clear(f32x2 (&acc)[R][C]) {
 }
 
 // This block's sample, found by its first warp.
-__device__ __forceinline__ AtSample as_sample(const AtArgs &a, const int32_t *by, int rows, int per_tile, AtSample *shared) {
+__device__ __forceinline__ AtSample as_sample(const AtArgs &a, bool keys, int per_tile, AtSample *shared) {
     at_check_offsets(a);
     if (threadIdx.x < 32) {
-        const AtSample s = at_find(by, rows, a, blockIdx.x, per_tile);
+        const AtSample s = at_find(a, keys, blockIdx.x, per_tile);
         if (threadIdx.x == 0) *shared = s;
     }
     __syncthreads();
@@ -146,7 +146,7 @@ attention_simt_kernel(const __grid_constant__ AtArgs a) {
     using S = AsShape<DP>;
     extern __shared__ __align__(16) float smem[];
     __shared__ AtSample shared;
-    const AtSample s = as_sample(a, a.offsets, a.M, S::BM, &shared);
+    const AtSample s = as_sample(a, false, S::BM, &shared);
     const int row0 = s.q0 + s.tile * S::BM, rows = min(S::BM, s.q1 - row0);
     if (s.tile < 0 || rows <= 0) return;
     float *sq = smem, *sk = sq + S::kTile, *sv = sk + S::kTile, *sp = sv + S::kTile;
@@ -250,7 +250,7 @@ attention_simt_grad_query_kernel(const __grid_constant__ AtArgs a) {
     using S = AsShape<DP>;
     extern __shared__ __align__(16) float smem[];
     __shared__ AtSample shared;
-    const AtSample s = as_sample(a, a.offsets, a.M, S::BM, &shared);
+    const AtSample s = as_sample(a, false, S::BM, &shared);
     const int row0 = s.q0 + s.tile * S::BM, rows = min(S::BM, s.q1 - row0);
     if (s.tile < 0 || rows <= 0) return;
     float *sq = smem, *sg = sq + S::kTile, *sk = sg + S::kTile, *sv = sk + S::kTile, *sd = sv + S::kTile;
@@ -309,7 +309,7 @@ attention_simt_grad_key_kernel(const __grid_constant__ AtArgs a) {
     using S = AsShape<DP>;
     extern __shared__ __align__(16) float smem[];
     __shared__ AtSample shared;
-    const AtSample s = as_sample(a, a.key_offsets, a.N, S::BM, &shared);
+    const AtSample s = as_sample(a, true, S::BM, &shared);
     const int key0 = s.tile * S::BM, row0 = s.k0 + key0, rows = min(S::BM, s.k1 - row0);
     if (s.tile < 0 || rows <= 0) return;
     float *sk = smem, *sv = sk + S::kTile, *sq = sv + S::kTile, *sg = sq + S::kTile, *sp = sg + S::kTile, *sd = sp + S::kScores;

@@ -138,7 +138,7 @@ attention_tc_grad_query_kernel(const __grid_constant__ CUtensorMap map_q, const 
             asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
         }
         __syncwarp();
-        s = at_find(a.offsets, a.M, a, a.causal ? gridDim.x - 1 - blockIdx.x : blockIdx.x, tokens);
+        s = at_find(a, false, a.causal ? gridDim.x - 1 - blockIdx.x : blockIdx.x, tokens);
         share();
         if (lane == 0) *s_sample = s;
         if (tiles > 0 && elect_one()) {
@@ -367,7 +367,7 @@ attention_tc_grad_key_kernel(const __grid_constant__ CUtensorMap map_q, const __
             asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
         }
         __syncwarp();
-        s = at_find(a.key_offsets, a.N, a, blockIdx.x, kAtRows);
+        s = at_find(a, true, blockIdx.x, kAtRows);
         share();
         if (lane == 0) *s_sample = s;
         if (tiles > 0 && elect_one()) {

@@ -165,7 +165,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         }
         __syncwarp();
         // the last tiles of a causal sample see most: they go first
-        s = at_find(a.offsets, a.M, a, a.causal ? gridDim.x - 1 - blockIdx.x : blockIdx.x, tokens);
+        s = at_find(a, false, a.causal ? gridDim.x - 1 - blockIdx.x : blockIdx.x, tokens);
         share();
         if (lane == 0) *s_sample = s;
         if (tiles > 0 && elect_one()) {
@@ -350,7 +350,7 @@ attention_tc_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     at_check_offsets(a);
     if (warp == S::kWarpLoad) {
         // the last tiles of a causal sample see most: they go first
-        const AtSample s = at_find(a.offsets, a.M, a, a.causal ? gridDim.x - 1 - blockIdx.x : blockIdx.x, 2 * tokens);
+        const AtSample s = at_find(a, false, a.causal ? gridDim.x - 1 - blockIdx.x : blockIdx.x, 2 * tokens);
         if (lane == 0) *s_sample = s;
     }
     if (tid == 0) {

@@ -249,8 +249,8 @@ extern "C" int spconv_rotary(const spconv_rotary_args *q, void *stream) {
     SPCONV_REQUIRE(q->axes >= 1 && q->axes <= q->rotary_dim / 2, SPCONV_ERR_ARG, "axes must be in [1, rotary_dim / 2]");
     SPCONV_REQUIRE(q->layout == SPCONV_ROTARY_HALF || q->layout == SPCONV_ROTARY_INTERLEAVED, SPCONV_ERR_ARG,
                    "unknown layout %d", q->layout);
-    SPCONV_REQUIRE(q->heads >= 0 && q->key_heads >= 0 && q->heads <= 65535 && q->key_heads <= 65535 && q->heads + q->key_heads > 0,
-                   SPCONV_ERR_ARG, "head counts out of range");
+    SPCONV_REQUIRE(q->heads >= 0 && q->key_heads >= 0 && (int64_t)q->heads + q->key_heads > 0 && (int64_t)q->heads + q->key_heads <= 65535,
+                   SPCONV_ERR_ARG, "heads must be in [1, 65535], of queries and keys together");
     if (q->num_rows == 0) return SPCONV_OK;
     SPCONV_REQUIRE(q->positions && (q->heads == 0 || (q->query && q->query_out)) && (q->key_heads == 0 || (q->key && q->key_out)),
                    SPCONV_ERR_ARG, "null pointer argument");
