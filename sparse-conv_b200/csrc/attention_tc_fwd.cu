@@ -11,9 +11,9 @@
 //   * attention_tc_kernel: one tile a CTA, 64 keys a step, four CTAs an SM (two for heads over 64): 128 columns of TMEM and
 //     48 KB each. A fifth warp does both loads and products. 84,000 voxels in 16 scenes, 8 x 64 bf16: 1.32 ms, 0.73 PFLOP/s
 //     (three CTAs an SM 1.56; one CTA of two tiles and 128 keys a step, whose two chains fell into step with one another,
-//     1.69; the same with the next scores made ahead of p v 1.48; two threads a row 2.02). The special functions are
-//     64 % in use, the issue slots 46 %, the tensor pipe 32 %. One pooling query a scene over 2.0 M voxels: 120 us and 15 to
-//     join the splits, 4.5 TB/s.
+//     1.69; the same with the next scores made ahead of p v 1.48; two threads a row 2.02). At 8,192
+//     tokens x 16 x 64 the special functions are 67 % in use, the issue slots 49 %, the tensor pipe 33 %. One pooling query a
+//     scene over 2.0 M voxels: 120 us, 4.3 TB/s, and 15 to join the splits.
 //   * attention_tc_pair_kernel, for long samples of heads over 64, whose accumulators leave TMEM for two chains only: two
 //     tiles a CTA, which share k and v, 128 keys a step, and registers dealt out anew so that a row of 128 scores fits: 4 x 128
 //     there 0.93 ms, 1.04 PFLOP/s (two CTAs of the kernel above 1.21 ms).

