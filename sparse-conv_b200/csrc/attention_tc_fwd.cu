@@ -19,7 +19,7 @@
 //     there 0.93 ms, 1.04 PFLOP/s (two CTAs of the kernel above 1.21 ms).
 //
 // The maximum is followed lazily: while a row's new maximum exceeds the one in use by at most 8, the old one
-// stays (p up to 2^8, exact in range), so out and the sum are rescaled a few times a row, not once a tile. p is
+// stays (p up to 2^8, and 2^15 in fp16, where it comes times 2^7), so out and the sum are rescaled a few times a row, not once a tile. p is
 // rounded to the inputs' type, as the tensor cores' operand; the sum adds p unrounded.
 //
 // Rows and keys behind a sample's end are other samples': s is replaced by -inf there, p v stops at the last 16 keys that
@@ -36,6 +36,11 @@ namespace spconv {
 
 constexpr float kAfSlack = 8.f;                      // by how much the maximum in use may be exceeded, in powers of two
 
+// Powers of two on p: fp16 loses p under 2^-25, of which a row of a hundred thousand keys may have many; with 2^7, the most that the
+// slack leaves below fp16's largest value, under 2^-32. Exact, and out again with the sum.
+template <typename T>
+constexpr float kAfUp = dtype_traits<T>::mma_format == 0 ? 7.f : 0.f;
+
 // A row's result: its accumulators over its sum; or, where keys are split, the accumulators as they
 // are. A warp's lanes together.
 template <typename T>
@@ -45,8 +50,8 @@ __device__ __forceinline__ void af_store(const AtArgs &a, uint32_t t_o, int size
     float *part = a.splits > 1 ? a.partial + (blockIdx.z * all + at) * a.D : nullptr;
     const float inv = part ? 1.f : none ? 0.f : 1.f / sum;
     if (mine) {
-        if (part) a.part_ml[blockIdx.z * all + at] = make_float2(top * a.c, sum);
-        else if (a.lse) a.lse[at] = none ? INFINITY : fmaf(top, a.c, log2f(sum));
+        if (part) a.part_ml[blockIdx.z * all + at] = make_float2(fmaf(top, a.c, -kAfUp<T>), sum);
+        else if (a.lse) a.lse[at] = none ? INFINITY : fmaf(top, a.c, log2f(sum) - kAfUp<T>);
     }
     T *out = (T *)a.out + at * a.D;
     const bool wide = (a.D & 7) == 0 && (((uintptr_t)a.out | (uintptr_t)a.rest) & 15) == 0;
@@ -277,7 +282,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                         }
                     }
                 }
-                const float shift = top == -INFINITY ? 0.f : -top * a.c;
+                const float shift = top == -INFINITY ? 0.f : fmaf(-top, a.c, kAfUp<T>);
                 const f32x2 c2 = pack_f32x2(a.c, a.c), s2 = pack_f32x2(shift, shift);
                 f32x2 add[2] = {pack_f32x2(0.f, 0.f), pack_f32x2(0.f, 0.f)};
 #pragma unroll
@@ -522,7 +527,7 @@ attention_tc_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                             }
                         }
                     }
-                    const float shift = top == -INFINITY ? 0.f : -top * a.c;
+                    const float shift = top == -INFINITY ? 0.f : fmaf(-top, a.c, kAfUp<T>);
                     const f32x2 c2 = pack_f32x2(a.c, a.c), s2 = pack_f32x2(shift, shift);
                     f32x2 add[2] = {pack_f32x2(0.f, 0.f), pack_f32x2(0.f, 0.f)};
 #pragma unroll

@@ -216,6 +216,22 @@ def test_whole_numbers_are_exact(dtype):
     assert torch.equal(gv, (grad.double().sum(0, keepdim=True) / 256).to(dtype).expand_as(gv))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D,M,H", [(64, 4736, 64), (128, 4736, 64)])
+def test_many_far_keys_keep_their_weight(dtype, D, M, H):
+    """One key and 65,535 of e^-18 (2^-26) of its weight: together 1.0e-3 of the whole. There are tiles enough for no
+    split, so all share one maximum. p of the far ones is 2^-19 where fp16 is lifted by 2^7, off by half of fp16's smallest step, 2^-25,
+    and so by 2^-6 relative at most; in bf16, and the result's own rounding, by less than 2^-8 each."""
+    n = 65536
+    q = torch.zeros(M, H, D, device="cuda", dtype=dtype)
+    k = torch.zeros(n, 1, D, device="cuda", dtype=dtype)
+    v = torch.ones(n, 1, D, device="cuda", dtype=dtype)
+    q[:, :, 0], k[1:, 0, 0], v[0] = 1.0, -18.0, 0.0
+    far = (n - 1) * math.exp(-18.0)
+    out = sparse_attention(q, k, v, scale=1.0).double()
+    assert ((out / (far / (1.0 + far)) - 1.0).abs().max().item()) < 2.0 ** -6 + 2.0 ** -8 + 2.0 ** -8
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_other_samples_values_do_not_enter(dtype):
     """Infinities and NaN in the rows before and behind a sample, which its last tiles read."""
