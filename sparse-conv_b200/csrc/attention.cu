@@ -283,8 +283,9 @@ static int at_check(const spconv_attention_args *q, bool backward) {
                    "unsupported dtype code %d", q->dtype);
     SPCONV_REQUIRE(q->kernel >= SPCONV_KERNEL_AUTO && q->kernel <= SPCONV_KERNEL_TCGEN05, SPCONV_ERR_ARG,
                    "unknown kernel choice %d", q->kernel);
-    SPCONV_REQUIRE(q->num_queries >= 0 && q->num_queries < (int64_t)1 << 31 && q->num_keys >= 0 && q->num_keys < (int64_t)1 << 31,
-                   SPCONV_ERR_ARG, "row counts must be in [0, 2^31)");
+    constexpr int64_t most = ((int64_t)1 << 31) - 1024;              // a tile's last row, past the tensor's end, fits 32 bits too
+    SPCONV_REQUIRE(q->num_queries >= 0 && q->num_queries <= most && q->num_keys >= 0 && q->num_keys <= most, SPCONV_ERR_ARG,
+                   "row counts must be in [0, 2^31 - 1024]");
     SPCONV_REQUIRE(q->num_samples >= 1 && q->num_samples < 1 << 24, SPCONV_ERR_ARG, "num_samples must be in [1, 2^24)");
     SPCONV_REQUIRE(q->key_heads >= 1 && q->heads >= q->key_heads && q->heads <= 65535 && q->heads % q->key_heads == 0, SPCONV_ERR_ARG,
                    "heads must be a multiple of key_heads, at most 65535");

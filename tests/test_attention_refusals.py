@@ -57,6 +57,14 @@ def test_attention_more(lib):
             assert need(attention_args(dtype=dtype, **nothing), 0) >= 0 and need(attention_args(dtype=dtype, **nothing), 1) >= 0
 
 
+@pytest.mark.parametrize("field", ["num_queries", "num_keys"])
+def test_rows_whose_tiles_would_pass_32_bits(lib, field):
+    """Numbers of a tile's rows and keys are 32-bit, up to a tile past the last row."""
+    for rows in ((1 << 31) - 1, (1 << 31) - 1023):
+        a = attention_args(**{field: rows})
+        assert lib.spconv_attention_forward(a, None) == 1 and lib.spconv_attention_backward(a, None) == 1
+
+
 def test_attention_python():
     q, k = torch.zeros(10, 4, 64), torch.zeros(12, 2, 64)
     off = torch.tensor([0, 10], dtype=torch.int32)
