@@ -135,6 +135,8 @@ def sparse_rotary(
         raise ValueError("query or key is needed")
     if first.dim() != 3:
         raise ValueError(f"query and key must be [N, heads, D], got shape {list(first.shape)}")
+    if positions.dim() not in (1, 2):
+        raise ValueError(f"positions must be [N] or [N, axes], got shape {list(positions.shape)}")
     axes = 1 if positions.dim() == 1 else positions.shape[-1]
     plan = _plan(first.shape[2], rotary_dim, axes, layout, base, scaling, factor, trained_size)
     if torch.is_grad_enabled() and ((query is not None and query.requires_grad) or (key is not None and key.requires_grad)):

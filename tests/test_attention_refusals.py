@@ -153,6 +153,11 @@ def test_rotary_shapes_on_the_device():
         sparse_rotary(q, None, pos, layout="other")
 
 
+def test_rotary_positions_without_rows():
+    with pytest.raises(ValueError, match="positions"):
+        sparse_rotary(torch.zeros(10, 4, 64), None, torch.zeros((), dtype=torch.int32))
+
+
 def test_steps():
     """Scaled steps at both ends of their ranges, by their formulas."""
     plain, one = rotary_steps(16)
