@@ -23,6 +23,18 @@ __device__ __forceinline__ AtSample at_find(const AtArgs &a, bool keys, int t, i
     const int rows = keys ? a.N : a.M;
     const int lane = threadIdx.x & 31;
     int lo = 0, hi = a.B;
+    // Of many samples first the 32 about where it would be if all were alike, which for windows in their grid's order is mostly the
+    // only step: 1,301 of 65 to 194 rows, 4 x 32 fp16, forward 152 -> 145 us, queries' gradients 298 -> 286 (half of
+    // them empty 201 -> 195; in the order of their sizes, where the guess fails, 249 -> 253).
+    if (hi > 32) {
+        const float part = __fdividef((float)t, (float)(rows / per_tile + a.B));
+        const int first = max(0, min(a.B - 32, (int)(part * (float)a.B) - 16)), at = first + lane;
+        const unsigned in = __ballot_sync(0xffffffffu, at == 0 || at_offset(by, at, rows) / per_tile + at <= t);
+        const int last = 31 - __clz((int)in);                        // -1: before them all
+        if (last < 0) hi = first;
+        else lo = first + last;
+        if (last >= 0 && last < 31) hi = lo + 1;
+    }
     while (hi - lo > 1) {
         const int step = (hi - lo + 31) >> 5, at = lo + lane * step;
         const bool in = lane == 0 || (at < hi && at_offset(by, at, rows) / per_tile + at <= t);

@@ -121,6 +121,16 @@ def test_many_short_samples(dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("order", ["up", "down", "ends", "one"])
+def test_many_samples_of_very_different_lengths(dtype, order):
+    """A tile's sample is not where it would be if all were alike: before it, behind it, among empty ones."""
+    lengths = {"up": [i // 2 for i in range(300)], "down": [i // 2 for i in range(300)][::-1],
+               "ends": [900] + [0] * 200 + [1, 2] * 40 + [700], "one": [0] * 150 + [1000] + [0] * 33}[order]
+    run(lengths, lengths, 4, 2, 32, dtype)
+    run(lengths, lengths[::-1], 2, 2, 32, dtype, causal=True)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("causal", [False, True])
 def test_long_samples(dtype, D, causal):
