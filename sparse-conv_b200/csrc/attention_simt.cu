@@ -9,8 +9,9 @@
 // products of [rows][head] tiles by 16 x 16 threads, 4 x 4 results each (rows 4 ty.., columns tx + 16 j), operands as
 // float4 along the head from rows padded by four floats (no bank conflicts), so that 64 FMAs go with 8 loads of 16 bytes;
 // products along the tile (p v and the like) take single columns tx + 16 j, which spans any head size in sixteens.
-// Bound: the FMA pipe and its operands from shared memory; issue slots 57, 65 and 69 % in use. 6,001 rows in 2 samples, 4 x 35
-// fp32 (heads counted as 48): 0.67, 0.86 and 1.07 ms for the three sweeps, 15 to 19 TFLOP/s of the 35 columns' products.
+// Bound: the FMA pipe and its operands from shared memory; issue slots 57, 65 and 69 % in use (all 48 columns). 6,001 rows
+// in 2 samples, 4 x 35 fp32: 0.62, 0.79 and 1.01 ms for the three sweeps, 17 to 20 TFLOP/s (0.69, 0.85 and 1.06 where products along the head took
+// all 48 columns in place of 36; 4 x 64, where none is left out, 0.81, 1.03 and 1.34 against 0.80, 1.06 and 1.33).
 #include <algorithm>
 
 #include "activation.cuh"
@@ -48,9 +49,9 @@ __device__ __forceinline__ float as_sum(f32x2 x) {
     return f.x + f.y;
 }
 
-// acc[i][j] = a[4 ty + i][.] . b[tx + 16 j][.]
+// acc[i][j] = a[4 ty + i][.] . b[tx + 16 j][.], over whole fours of the head's `size` values (zeros behind its end)
 template <int DP>
-__device__ __forceinline__ void as_dot(const float *a, const float *b, float (&acc)[AsShape<DP>::R][AsShape<DP>::R]) {
+__device__ __forceinline__ void as_dot(const float *a, const float *b, int size, float (&acc)[AsShape<DP>::R][AsShape<DP>::R]) {
     using S = AsShape<DP>;
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
     const float *pa = a + ty * S::R * S::LD, *pb = b + tx * S::LD;
@@ -60,7 +61,7 @@ __device__ __forceinline__ void as_dot(const float *a, const float *b, float (&a
 #pragma unroll
         for (int j = 0; j < S::R; ++j) sum[i][j] = pack_f32x2(0.f, 0.f);
 #pragma unroll 4
-    for (int d = 0; d < DP; d += 4) {
+    for (int d = 0; d < size; d += 4) {
         float4 x[S::R], y[S::R];
 #pragma unroll
         for (int i = 0; i < S::R; ++i) x[i] = *(const float4 *)(pa + i * S::LD + d);
@@ -168,7 +169,7 @@ attention_simt_kernel(const __grid_constant__ AtArgs a) {
         as_load<T, DP>(sv, a.v, s.k0 + key0, valid, kh, a.D);
         __syncthreads();
         float x[S::R][S::R];
-        as_dot<DP>(sq, sk, x);
+        as_dot<DP>(sq, sk, a.D, x);
 #pragma unroll
         for (int i = 0; i < S::R; ++i) {
             const int seen = at_seen(a, i0 + i, n, m) - key0;
@@ -231,8 +232,8 @@ __device__ __forceinline__ void as_grads(const AtArgs &a, const float *sq, const
     using S = AsShape<DP>;
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
     float x[S::R][S::R], y[S::R][S::R];
-    as_dot<DP>(sq, sk, x);
-    as_dot<DP>(sg, sv, y);
+    as_dot<DP>(sq, sk, a.D, x);
+    as_dot<DP>(sg, sv, a.D, y);
 #pragma unroll
     for (int i = 0; i < S::R; ++i)
 #pragma unroll
