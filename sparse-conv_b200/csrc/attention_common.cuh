@@ -68,6 +68,7 @@ __device__ __forceinline__ void at_check_offsets(const AtArgs &a) {
         }
     }
     if (bad) raise_status(a.status, SPCONV_STATUS_OFFSETS);
+    __syncwarp();                        // lanes have walked different numbers of samples
 }
 
 // Keys that query i of a sample of n queries and m keys sees: the last query sees the last key.

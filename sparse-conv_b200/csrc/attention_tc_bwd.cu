@@ -46,6 +46,7 @@ __device__ __forceinline__ void ab_store_row(uint32_t taddr, int from, int to, i
 #pragma unroll 1
     for (int c = from; c < to && c < D; c += 32) {
         f32x2 o[16];
+        __syncwarp();                                                // lanes without a row come here before those that store
         if (!zero) lt_load32(taddr + c, o);
         if (!mine) continue;
 #pragma unroll

@@ -58,6 +58,7 @@ __device__ __forceinline__ void af_store(const AtArgs &a, uint32_t t_o, int size
 #pragma unroll 1
     for (int c = 0; c < size && c < a.D; c += 16) {
         uint32_t o[16];
+        __syncwarp();                                                // lanes without a row come here before those that store
         if (!nothing) {                                              // there were keys, the same for every lane
             tmem_ld16(t_o + c, o);
             tc_wait_ld();
@@ -271,6 +272,7 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
                     if (grown) top = now;
                     sum *= down;
                     if (j > 0) {                                     // the products before are done: s came after them
+                        __syncwarp();
 #pragma unroll 1
                         for (int c = 0; c < DP; c += 16) {
                             uint32_t o[16];
@@ -516,6 +518,7 @@ attention_tc_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                         sum *= down;
                         if (j > 0) {                                 // the products before are done: s came after them
                             const f32x2 d2 = pack_f32x2(down, down);
+                            __syncwarp();
 #pragma unroll 1
                             for (int c = 0; c < DP; c += 32) {
                                 f32x2 o[16];
