@@ -122,7 +122,8 @@ attention_peak_kernel(const __grid_constant__ AtArgs a) {
     at_peak(a.peaks + 1, nan ? NAN : most);
 }
 
-// A row's splits: out = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s. `share` warps take a row's splits in turn and add up in
+// A row's splits: out = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s, over those that saw a key (others have a sum of -1; scores
+// that are all -inf have one of 0, and make the row NaN where no split has another). `share` warps take a row's splits in turn and add up in
 // order: all eight of a block where rows are few (eight rows of 74 splits: 75 us by a warp each), one where they are many.
 template <typename T>
 __global__ void __launch_bounds__(kAtThreads)
@@ -138,7 +139,7 @@ attention_join_kernel(const __grid_constant__ AtArgs a, const int share) {
             const float2 ml = a.part_ml[s * all + rh];
             m = fmaxf(m, ml.x);
             nan |= isnan(ml.x);
-            some |= !(ml.x == -INFINITY && ml.y == 0.f);        // else it saw no key, and nothing may be written there
+            some |= !(ml.y < 0.f);                              // else it saw no key, and nothing may be written there
         }
 #pragma unroll
         for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -147,7 +148,7 @@ attention_join_kernel(const __grid_constant__ AtArgs a, const int share) {
 #pragma unroll 4
         for (int s = w; s < a.splits; s += share) {
             const float2 ml = a.part_ml[s * all + rh];
-            const bool there = !(ml.x == -INFINITY && ml.y == 0.f);
+            const bool there = !(ml.y < 0.f);
             const float weight = there ? exp2f(ml.x - m) : 0.f;
             const float *p = a.partial + (s * all + rh) * a.D;
             sum = fmaf(weight, ml.y, sum);

@@ -28,7 +28,7 @@ struct AtArgs {
     // split s of a sample's keys (or, for the keys' gradients, queries): fp32 results of its own, joined afterwards
     int splits;
     float *partial;                      // [splits, M, H, D]; the keys' gradients [splits, 2, N, K, D]
-    float2 *part_ml;                     // forward: [splits, M, H] (largest score * c, sum)
+    float2 *part_ml;                     // forward: [splits, M, H] (largest score * c, sum; -1: no key seen)
     int32_t *status;
     uint64_t wait_ns;
     int dtype;

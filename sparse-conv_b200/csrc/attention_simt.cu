@@ -205,10 +205,10 @@ attention_simt_kernel(const __grid_constant__ AtArgs a) {
         const int r = ty * S::R + i;
         if (r >= rows) continue;
         const int64_t at = (int64_t)(row0 + r) * a.H + h;
-        const bool none = at_seen(a, i0 + i, n, m) == 0;
+        const bool none = at_seen(a, i0 + i, n, m) <= first * S::BM;        // (of this split's keys)
         if (a.splits > 1) {
             const int64_t all = (int64_t)a.M * a.H;
-            if (tx == 0) a.part_ml[blockIdx.z * all + at] = make_float2(top[i], sum[i]);
+            if (tx == 0) a.part_ml[blockIdx.z * all + at] = make_float2(top[i], none ? -1.f : sum[i]);
 #pragma unroll
             for (int j = 0; j < S::C; ++j)
                 if (tx + 16 * j < a.D) a.partial[(blockIdx.z * all + at) * a.D + tx + 16 * j] = as_sum(acc[i][j]);

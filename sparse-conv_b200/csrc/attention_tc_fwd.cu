@@ -41,8 +41,8 @@ constexpr float kAfSlack = 8.f;                      // by how much the maximum 
 template <typename T>
 constexpr float kAfUp = dtype_traits<T>::mma_format == 0 ? 7.f : 0.f;
 
-// A row's result: its accumulators over its sum; or, where keys are split, the accumulators as they
-// are. A warp's lanes together.
+// A row's result: its accumulators over its sum, zeros if it sees no key (`none`: of this split); or, where keys are split, the
+// accumulators as they are. A warp's lanes together.
 template <typename T>
 __device__ __forceinline__ void af_store(const AtArgs &a, uint32_t t_o, int size, int64_t at, bool mine, bool none, bool nothing, float top,
                                          float sum) {
@@ -50,7 +50,7 @@ __device__ __forceinline__ void af_store(const AtArgs &a, uint32_t t_o, int size
     float *part = a.splits > 1 ? a.partial + (blockIdx.z * all + at) * a.D : nullptr;
     const float inv = part ? 1.f : none ? 0.f : 1.f / sum;
     if (mine) {
-        if (part) a.part_ml[blockIdx.z * all + at] = make_float2(fmaf(top, a.c, -kAfUp<T>), sum);
+        if (part) a.part_ml[blockIdx.z * all + at] = make_float2(fmaf(top, a.c, -kAfUp<T>), none ? -1.f : sum);
         else if (a.lse) a.lse[at] = none ? INFINITY : fmaf(top, a.c, log2f(sum) - kAfUp<T>);
     }
     T *out = (T *)a.out + at * a.D;
@@ -310,7 +310,8 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         if (tiles > 0 && ok) ok = wait(sfull, tiles & 1);            // the last p v
         tc_fence_after();
         if (ok && some)
-            af_store<T>(a, t_o, DP, (int64_t)(s.q0 + token) * a.H + head0 + (tid & (P - 1)), mine, seen == 0, tiles == 0, top, sum);
+            af_store<T>(a, t_o, DP, (int64_t)(s.q0 + token) * a.H + head0 + (tid & (P - 1)), mine, seen <= first * S::kKeys,
+                        tiles == 0, top, sum);
     }
 
     __syncwarp();
@@ -556,7 +557,8 @@ attention_tc_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             if (tiles > 0 && ok) ok = __all_sync(0xffffffffu, wait(&odone[q], (tiles - 1) & 1)) != 0;     // the last p v
             tc_fence_after();
             if (ok && some)
-                af_store<T>(a, t_o, DP, (int64_t)(s.q0 + token) * a.H + head0 + (row & (P - 1)), mine, seen == 0, tiles == 0, top, sum);
+                af_store<T>(a, t_o, DP, (int64_t)(s.q0 + token) * a.H + head0 + (row & (P - 1)), mine, seen <= first * kAtRows,
+                            tiles == 0, top, sum);
         }
     }
 
