@@ -24,19 +24,6 @@ attention_pack_kernel(AtTensor t, T *out, int64_t rows, int heads, int D, int to
     }
 }
 
-// The largest of the block's values into *peak, which starts at 0 (NaN above all): the same whatever the order.
-__device__ __forceinline__ void at_peak(float *peak, float square) {
-    __shared__ uint32_t tops[kAtThreads / 32];
-    const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(square));
-    if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        uint32_t most = 0;
-        for (int w = 0; w < kAtThreads / 32; ++w) most = max(most, tops[w]);
-        if (most > *(volatile uint32_t *)peak) atomicMax((uint32_t *)peak, most);
-    }
-}
-
 // Eight lanes a row and head, of which they have x . y (and x . (y + rest)) and x . x. Bound: HBM.
 template <typename T, bool WIDE>
 __device__ __forceinline__ void at_dots(const T *x, const T *y, const T *rest, int D, bool in, float &xy, float &xx) {
@@ -71,7 +58,11 @@ __device__ __forceinline__ void at_dots(const T *x, const T *y, const T *rest, i
     }
 }
 
-// delta[row, head] = grad . (out + what its rounding left out, where that is kept), and grad's largest square.
+// A row's square as the largest are looked for: none where it is not finite, since the row's products are lost as they are, and others
+// need their digits all the same.
+__device__ __forceinline__ float at_counted(float square) { return square < INFINITY ? square : 0.f; }
+
+// delta[row, head] = grad . (out + what its rounding left out, where that is kept), and grad's square.
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(kAtThreads)
 attention_delta_kernel(const __grid_constant__ AtArgs a) {
@@ -80,28 +71,99 @@ attention_delta_kernel(const __grid_constant__ AtArgs a) {
     float dot, square;
     at_dots<T, WIDE>((const T *)a.grad.p + r * a.grad.row + (rh - r * a.H) * a.grad.head, (const T *)a.out_in + rh * a.D,
                      a.rest ? (const T *)a.rest + rh * a.D : nullptr, a.D, in, dot, square);
-    if (in && (threadIdx.x & 7) == 0) a.delta[rh] = dot;
-    if (a.peaks) at_peak(a.peaks, square);
+    if (!in || (threadIdx.x & 7) != 0) return;
+    a.delta[rh] = dot;
+    if (a.peaks) a.squares[rh] = at_counted(square);
 }
 
-// v's largest square: eight lanes take four rows and heads at a time, of whole 16 bytes.
-__global__ void __launch_bounds__(kAtThreads)
-attention_peak_kernel(const __grid_constant__ AtArgs a) {
+// Each sample's largest square into peaks[sample * 2], which start at 0: the same whatever the order. A converged warp's, whose rows
+// and heads ascend; while they are one sample's that is a comparison.
+struct AtPeaks {
+    const int32_t *offsets;
+    int B, rows, heads;
+    float *peaks;
+    int b;                               // the sample, and the row and head behind it
+    int64_t end;
+    uint32_t most;
+
+    __device__ __forceinline__ void begin(int row) {
+        b = at_sample_of(offsets, B, rows, row);
+        end = b + 1 == B ? INT64_MAX : (int64_t)at_offset(offsets, b + 1, rows) * heads;
+        most = 0;
+    }
+    __device__ __forceinline__ void put(int sample, uint32_t value) const {
+        uint32_t *peak = reinterpret_cast<uint32_t *>(peaks + 2 * (int64_t)sample);
+        if (value > *(volatile uint32_t *)peak) atomicMax(peak, value);
+    }
+    __device__ __forceinline__ void flush() const {
+        const uint32_t top = __reduce_max_sync(0xffffffffu, most);
+        if ((threadIdx.x & 31) == 0) put(b, top);
+        __syncwarp();
+    }
+    // the warp's rows and heads go up to `last`; the lane's own has a square that counts (or 0)
+    __device__ __forceinline__ void add(int64_t last, int64_t own, float square) {
+        const uint32_t value = __float_as_uint(square);
+        if (last < end) {
+            most = max(most, value);
+            return;
+        }
+        flush();
+        const int row = (int)min(own / heads, (int64_t)rows - 1);
+        if (value > 0) {                     // on from the sample before, in steps that double
+            int at = b, step = 1;
+            for (; at + step < B && at_offset(offsets, at + step, rows) <= row; step *= 2) at += step;
+            for (step >>= 1; step > 0; step >>= 1)
+                if (at + step < B && at_offset(offsets, at + step, rows) <= row) at += step;
+            put(at, value);
+        }
+        __syncwarp();
+        begin(__shfl_sync(0xffffffffu, row, 31));
+    }
+};
+
+// grad's largest squares of rows that see a key, from those that the pass before wrote (1/32 of the bytes of 16-bit rows of 64; looking
+// for the samples in that pass took it from 38 to 57 us over 1,301 windows): a warp takes `share` of them, 128 a step.
+__device__ __forceinline__ void at_grad_peaks(const AtArgs &a, int64_t share) {
+    const int lane = threadIdx.x & 31;
+    const int64_t all = (int64_t)a.M * a.H, first = ((int64_t)blockIdx.x * (kAtThreads / 32) + (threadIdx.x >> 5)) * share;
+    if (first >= all) return;
+    AtPeaks peaks{a.offsets, a.B, a.M, a.H, a.peaks};
+    peaks.begin((int)(first / a.H));
+    for (int64_t at = first; at < min(first + share, all); at += 128) {
+        float square[4], lse[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int64_t rh = at + 32 * k + lane;
+            square[k] = rh < all ? __ldg(a.squares + rh) : 0.f;
+            lse[k] = rh < all ? __ldg(a.lse + rh) : 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) peaks.add(at + 32 * k + 31, at + 32 * k + lane, lse[k] == INFINITY ? 0.f : square[k]);
+    }
+    peaks.flush();
+}
+
+// v's: a block takes `parts` times 128 rows and heads, a warp sixteen of them, eight lanes four at a time, of whole 16 bytes.
+__device__ __forceinline__ void at_value_peaks(const AtArgs &a, int64_t parts) {
     constexpr int B = 4;
-    const int lane = threadIdx.x & 7;
-    const int64_t rows = (int64_t)a.N * a.K, group = ((int64_t)blockIdx.x * kAtThreads + threadIdx.x) >> 3;
-    const int64_t groups = (int64_t)gridDim.x * (kAtThreads / 8);
-    float most = 0.f;
-    bool nan = false;
-    for (int64_t first = group; first < rows; first += groups * B) {
+    const int lane = threadIdx.x & 7, group = (threadIdx.x & 31) >> 3;
+    constexpr int kBlock = kAtThreads / 32 * 4 * B;
+    const int64_t all = (int64_t)a.N * a.K, begin = blockIdx.x * parts * kBlock, first = begin + (threadIdx.x >> 5) * 4 * B;
+    if (first >= all) return;
+    AtPeaks peaks{a.key_offsets, a.B, a.N, a.K, a.peaks + 1};
+    peaks.begin((int)(first / a.K));
+    for (int64_t part = first; part < min(begin + parts * kBlock, all); part += kBlock) {
         float square[B] = {};
+        const int64_t row = part / a.K;
+        const int head = (int)(part - row * a.K) + group;
         for (int d = lane * 8; d < a.D; d += 64) {
             uint4 x[B];
 #pragma unroll
             for (int k = 0; k < B; ++k) {
-                const int64_t rh = first + k * groups, r = rh / a.K;
+                const unsigned past = (unsigned)(head + 4 * k) / (unsigned)a.K;          // 64-bit quotients cost four times as much
                 x[k] = make_uint4(0, 0, 0, 0);
-                if (rh < rows) x[k] = __ldg((const uint4 *)((const __half *)a.v.p + r * a.v.row + (rh - r * a.K) * a.v.head + d));
+                if (part + 4 * k + group < all)
+                    x[k] = __ldg((const uint4 *)((const __half *)a.v.p + (row + past) * a.v.row + (head + 4 * k - (int64_t)past * a.K) * a.v.head + d));
             }
 #pragma unroll
             for (int k = 0; k < B; ++k)
@@ -111,15 +173,23 @@ attention_peak_kernel(const __grid_constant__ AtArgs a) {
                     square[k] = fmaf(f.x, f.x, fmaf(f.y, f.y, square[k]));
                 }
         }
+        __syncwarp();                        // (lanes past the head's end have read less)
 #pragma unroll
         for (int k = 0; k < B; ++k) {
 #pragma unroll
-            for (int o = 4; o; o >>= 1) square[k] += __shfl_xor_sync(0xffu << (threadIdx.x & 24), square[k], o);
-            most = fmaxf(most, square[k]);
-            nan |= isnan(square[k]);
+            for (int o = 4; o; o >>= 1) square[k] += __shfl_xor_sync(0xffffffffu, square[k], o);
+            peaks.add(part + 4 * k + 3, part + 4 * k + group, at_counted(square[k]));
         }
     }
-    at_peak(a.peaks + 1, nan ? NAN : most);
+    peaks.flush();
+}
+
+// Both in one launch, in each other's latency (1,301 windows, 4 x 32: 34 us, 42 one after the other; one largest for the whole call, which
+// one sample's rows would set for all others, 23).
+__global__ void __launch_bounds__(kAtThreads)
+attention_peaks_kernel(const __grid_constant__ AtArgs a, const int64_t parts, const int64_t share) {
+    if (blockIdx.y == 0) at_value_peaks(a, parts);
+    else at_grad_peaks(a, share);
 }
 
 // A row's splits: out = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s, over those that saw a key (others have a sum of -1; scores
@@ -210,7 +280,7 @@ struct AtPlan {
     bool pair;                           // forward: two tiles a CTA
     int splits[3];                       // forward (or queries' gradients), and keys' gradients
     bool pack[4];                        // q, k, v, grad
-    int64_t pack_at[4], delta_at, peaks_at, ml_at, partial_at, bytes;
+    int64_t pack_at[4], delta_at, peaks_at, squares_at, ml_at, partial_at, bytes;
 };
 
 // Splits of `tiles` steps each of `ctas` CTAs, of which `slots` run at a time: whole waves, none of fewer than `least` steps. A CTA's
@@ -267,7 +337,9 @@ static AtPlan at_plan(const spconv_attention_args *q, bool backward) {
     const int64_t rows = M * q->heads, krows = N * q->key_heads;
     if (backward) {
         p.delta_at = take(rows * 4);
-        p.peaks_at = take(8);
+        const bool lift = p.tc && q->dtype == SPCONV_F16;
+        p.peaks_at = take(lift ? B * 8 : 0);
+        p.squares_at = take(lift ? rows * 4 : 0);
         p.partial_at = take(std::max(p.splits[0] > 1 ? p.splits[0] * rows * q->head_size * 4 : 0,
                                      p.splits[1] > 1 ? 2 * p.splits[1] * krows * q->head_size * 4 : 0));
     } else if (p.splits[0] > 1) {
@@ -337,6 +409,7 @@ static int at_prepare(const spconv_attention_args *q, const AtPlan &p, bool back
     uint8_t *ws = (uint8_t *)q->workspace;
     a.delta = (float *)(ws + p.delta_at);
     a.peaks = backward && p.tc && q->dtype == SPCONV_F16 ? (float *)(ws + p.peaks_at) : nullptr;
+    a.squares = (float *)(ws + p.squares_at);
     a.part_ml = (float2 *)(ws + p.ml_at);
     a.partial = (float *)(ws + p.partial_at);
     AtTensor *t[4] = {&a.q, &a.k, &a.v, &a.grad};
@@ -398,7 +471,7 @@ extern "C" int spconv_attention_backward(const spconv_attention_args *q, void *s
     if (a.M > 0) {
         const bool wide = a.D % 8 == 0 && (((uintptr_t)q->grad_out | (uintptr_t)q->out | (uintptr_t)q->out_rest) & 15) == 0 &&
                           q->grad_row % 8 == 0 && q->grad_head % 8 == 0;
-        if (a.peaks && cudaMemsetAsync(a.peaks, 0, 8, a.stream) != cudaSuccess) return check_launch("attention: clear");
+        if (a.peaks && cudaMemsetAsync(a.peaks, 0, (size_t)a.B * 8, a.stream) != cudaSuccess) return check_launch("attention: clear");
         AtArgs d = a;
         d.grad = {q->grad_out, q->grad_row, q->grad_head};
         const int rc = at_by_type(a.dtype, [&](auto *t) {
@@ -409,9 +482,12 @@ extern "C" int spconv_attention_backward(const spconv_attention_args *q, void *s
         });
         if (rc) return rc;
         if (a.peaks) {                       // (a.v as the products read it: packed where its own layout is not aligned)
-            const unsigned blocks = (unsigned)std::min<int64_t>(at_blocks((int64_t)a.N * a.K * 8), 148 * 8);
-            attention_peak_kernel<<<blocks, kAtThreads, 0, a.stream>>>(at_whole(a));
-            if (const int rc2 = check_launch("attention_peak_kernel")) return rc2;
+            const int64_t rows = (int64_t)a.M * a.H, values = (int64_t)a.N * a.K;
+            auto share = [](int64_t n, int each, int many) { return std::max<int64_t>(1, (n + (int64_t)each * many - 1) / ((int64_t)each * many)); };
+            const int64_t parts = share(values, 128, 148 * 8), steps = share(rows, 128, 148 * 32);
+            const int64_t blocks = std::max((values + parts * 128 - 1) / (parts * 128), (rows + steps * 1024 - 1) / (steps * 1024));
+            attention_peaks_kernel<<<dim3((unsigned)blocks, 2), kAtThreads, 0, a.stream>>>(at_whole(a), parts, steps * 128);
+            if (const int rc2 = check_launch("attention_peaks_kernel")) return rc2;
         }
     }
     auto join = [&](const float *from, int64_t stride, void *to, int64_t n) {

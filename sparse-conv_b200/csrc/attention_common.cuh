@@ -10,6 +10,21 @@ __device__ __forceinline__ int at_offset(const int32_t *offsets, int b, int rows
     return offsets ? max(0, min(rows, __ldg(offsets + b))) : (b ? rows : 0);
 }
 
+// The sample that a row lies in: the last that begins at or before it. By a converged warp, 32 samples a step; inside [0, B)
+// whatever the offsets hold.
+__device__ __forceinline__ int at_sample_of(const int32_t *offsets, int B, int rows, int row) {
+    const int lane = threadIdx.x & 31;
+    int lo = 0, hi = B;
+    while (hi - lo > 1) {
+        const int step = (hi - lo + 31) >> 5, at = lo + lane * step;
+        const bool in = lane == 0 || (at < hi && at_offset(offsets, at, rows) <= row);
+        const int last = 31 - __clz((int)__ballot_sync(0xffffffffu, in));
+        lo += last * step;
+        hi = min(hi, lo + step);
+    }
+    return lo;
+}
+
 struct AtSample {
     int b, tile;                         // the sample and the tile's number in it
     int q0, q1, k0, k1;                  // its query and key rows
@@ -83,11 +98,12 @@ __device__ __forceinline__ void at_split(int splits, int s, int count, int &firs
     last = min(count, first + per);
 }
 
-// The power of two by which ds is lifted where it has to be rounded to fp16: |ds| <= 2 |grad row| |v row|, so the largest is
-// at most 2^15, and rows of thousands of keys, or gradients of any size, keep their digits above fp16's smallest values.
-__device__ __forceinline__ int at_lift(const AtArgs &a) {
+// The power of two by which a sample's ds is lifted where it has to be rounded to fp16: |ds| <= 2 |grad row| |v row|, so the largest
+// is at most 2^15, and rows of thousands of keys, or gradients of any size, keep their digits above fp16's smallest values.
+__device__ __forceinline__ int at_lift(const AtArgs &a, int b) {
     if (!a.peaks) return 0;
-    const float x = sqrtf(__ldg(a.peaks)) * sqrtf(__ldg(a.peaks + 1));
+    const float2 squares = __ldg(reinterpret_cast<const float2 *>(a.peaks) + b);
+    const float x = sqrtf(squares.x) * sqrtf(squares.y);
     if (!(x > 0.f && x < INFINITY)) return 0;
     int e;
     frexpf(x, &e);                       // x <= 2^e

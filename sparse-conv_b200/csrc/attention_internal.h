@@ -19,7 +19,8 @@ struct AtArgs {
     void *rest;                          // what out's rounding left out, or null
     float *lse;                          // [num_queries, heads]: log2 of the row's sum, + inf where it sees no key
     float *delta;                        // [num_queries, heads]: grad . out
-    float *peaks;                        // fp16 gradients: largest square of a row of grad, and of v; else null
+    float *peaks;                        // fp16 gradients: [samples, 2] largest squares of a row of grad, and of v; else null
+    float *squares;                      // [num_queries, heads], of grad's rows
     const int32_t *offsets, *key_offsets;
     int B, M, N;                         // samples, query rows, key rows
     int H, K, D;                         // heads, key heads, head size

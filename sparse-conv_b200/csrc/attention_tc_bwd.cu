@@ -249,7 +249,7 @@ attention_tc_grad_query_kernel(const __grid_constant__ CUtensorMap map_q, const 
         const int seen_all = __reduce_min_sync(0xffffffffu, mine ? seen : m);
         const int64_t at = (int64_t)(s.q0 + token) * a.H + head0 + (row & (P - 1));
         const float lse = mine ? a.lse[at] : INFINITY, delta = mine ? a.delta[at] : 0.f;
-        const int lift = at_lift(a);                                 // p, and so ds, comes times 2^lift
+        const int lift = at_lift(a, s.b);                                 // p, and so ds, comes times 2^lift
         const f32x2 c2 = pack_f32x2(a.c, a.c), l2 = pack_f32x2(lift - lse, lift - lse), d2 = pack_f32x2(-delta, -delta);
         bool ok = true;
         for (int j = 0; j < tiles; ++j) {
@@ -321,8 +321,6 @@ attention_tc_grad_key_kernel(const __grid_constant__ CUtensorMap map_q, const __
     using S = AkShape<DP, W>;
     constexpr float kUp = dtype_traits<T>::mma_format == 0 ? 15.f : 0.f;         // powers of two on p
     constexpr float kDown = dtype_traits<T>::mma_format == 0 ? 0x1p-15f : 1.f;
-    const int lift = at_lift(a);                                     // ds comes times 2^lift
-    const float down = ldexpf(kDown, lift);
     extern __shared__ uint8_t smem_raw[];
     uint8_t *base = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     const uint32_t s_k = smem_u32(base), s_v = s_k + S::kOwn, s_q = s_v + S::kOwn;      // stages of q, grad
@@ -415,6 +413,7 @@ attention_tc_grad_key_kernel(const __grid_constant__ CUtensorMap map_q, const __
             uint32_t phase = 1, tail_phase = 0;
             bool ok = true;
             Walk w = begin();
+            float down = 0.f;
             for (int j = 0; j < tiles; ++j, advance(w), next(st, phase)) {
                 const int rows = rows_of(w);
                 const bool cut = rows & 15;
@@ -424,7 +423,7 @@ attention_tc_grad_key_kernel(const __grid_constant__ CUtensorMap map_q, const __
                     const int r = lane + 32 * i;
                     const int64_t at = (int64_t)(s.q0 + w.t * tokens + (r >> log_p)) * a.H + w.head + (r & (P - 1));
                     lse[i] = r < rows ? kUp - __ldg(a.lse + at) : -INFINITY;
-                    delta[i] = r < rows ? -down * __ldg(a.delta + at) : 0.f;
+                    delta[i] = r < rows ? -__ldg(a.delta + at) : 0.f;
                 }
                 if (!(ok = __all_sync(0xffffffffu, wait(&empty[st], phase)) != 0)) break;
                 const uint32_t dst = s_q + st * 2 * S::kTile, mbar = smem_u32(cut ? tail : &full[st]);
@@ -433,10 +432,11 @@ attention_tc_grad_key_kernel(const __grid_constant__ CUtensorMap map_q, const __
                     load(dst, W, &map_q, w.head, s.q0 + w.t * tokens, mbar);
                     load(dst + S::kTile, W, &map_g, w.head, s.q0 + w.t * tokens, mbar);
                 }
+                if (j == 0) down = ldexpf(kDown, at_lift(a, s.b));   // not before the first copies are on their way
 #pragma unroll
                 for (int i = 0; i < W / 32; ++i) {
                     s_rows[st * 2 * W + lane + 32 * i] = lse[i];
-                    s_rows[st * 2 * W + W + lane + 32 * i] = delta[i];
+                    s_rows[st * 2 * W + W + lane + 32 * i] = delta[i] * down;
                 }
                 __syncwarp();
                 if (cut) {
@@ -499,6 +499,8 @@ attention_tc_grad_key_kernel(const __grid_constant__ CUtensorMap map_q, const __
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t t_s = tmem + part * 32 + lanes, t_d = t_dp + part * 32 + lanes;
         const bool mine = key < m;
+        const int lift = at_lift(a, s.b);                            // ds comes times 2^lift
+        const float down = ldexpf(kDown, lift);
         const f32x2 c2 = pack_f32x2(a.c, a.c), k2 = pack_f32x2(down, down);
         bool ok = true;
         int st = 0;
