@@ -437,8 +437,8 @@ int spconv_rotary(const spconv_rotary_args *args, void *stream);
  *   sample of all rows. Samples without queries or keys are allowed.
  *   row_stats [num_queries, heads] fp32: written by the forward unless NULL, read by the backward
  *   out_rest: NULL, or as out: what rounding took from out, rounded itself, written by the forward and read by the backward, which
- *   needs grad_out . out. Where rows see many keys, out's rounding is far under the terms' own size; where they see
- *   few (up to a hundred or so), gradients of queries and keys are off by up to twice as much without it
+ *   needs grad_out . out. Without it the gradients of queries and keys of rows whose weight is on a few keys, however many they
+ *   see, are off by up to twice as much
  *   num_queries, num_keys: up to 2^31 - 1024
  *   scale: positive. head_size <= 256. kernel: SPCONV_KERNEL_*; the tensor-core kernels take fp16 and bf16 heads of up
  *   to 128 values and return SPCONV_ERR_UNSUPPORTED for others

@@ -83,6 +83,12 @@ __device__ __forceinline__ void at_load(uint32_t taddr, f32x2 (&x)[N]) {
     }
 }
 
+// 32 aligned bytes at once: a sector, which two stores of 16 would write in halves.
+__device__ __forceinline__ void at_store32(void *p, const uint32_t (&w)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n"
+                 :: "l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
+}
+
 // 2^x of two values, by the special functions: 16 a clock and SM. (A polynomial on the FMA pipe, degree 4, for one to four of
 // eight pairs was 2 % faster at best, in the gradients at one of eight, and slower from three on: a step's time is its
 // chain of waits, not the special functions alone.)

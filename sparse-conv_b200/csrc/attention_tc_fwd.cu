@@ -55,6 +55,7 @@ __device__ __forceinline__ void af_store(const AtArgs &a, uint32_t t_o, int size
     }
     T *out = (T *)a.out + at * a.D;
     const bool wide = (a.D & 7) == 0 && (((uintptr_t)a.out | (uintptr_t)a.rest) & 15) == 0;
+    const bool whole = (a.D & 15) == 0 && (((uintptr_t)a.out | (uintptr_t)a.rest) & 31) == 0;
 #pragma unroll 1
     for (int c = 0; c < size && c < a.D; c += 16) {
         uint32_t o[16];
@@ -65,6 +66,23 @@ __device__ __forceinline__ void af_store(const AtArgs &a, uint32_t t_o, int size
         }
         if (!mine || (part && nothing)) continue;
         none |= nothing;
+        if (!part && whole) {
+            // a lane's 16 values are a sector: out and rest of voxels to 257 tokens 334 -> 252 us (out alone 240 -> 236)
+            uint32_t w[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                w[i] = none ? 0u : lt_pack<T>(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
+            at_store32(out + c, w);
+            if (a.rest) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float2 hi = lt_unpack<T>(w[i]);
+                    w[i] = none ? 0u : lt_pack<T>(fmaf(__uint_as_float(o[2 * i]), inv, -hi.x), fmaf(__uint_as_float(o[2 * i + 1]), inv, -hi.y));
+                }
+                at_store32((T *)a.rest + at * a.D + c, w);
+            }
+            continue;
+        }
 #pragma unroll
         for (int v = 0; v < 2; ++v) {
             const int d = c + v * 8;

@@ -40,7 +40,6 @@ NOALLOC_MAX_COORDS = 262144   # SPCONV_NOALLOC_MAX_COORDS
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}   # SPCONV_ACT_*
 ROTARY_LAYOUTS = {"half": 0, "interleaved": 1}               # SPCONV_ROTARY_*
 ROTARY_MAX_PAIRS = 128
-ATTENTION_FEW_KEYS = 128      # mean keys a sample up to which the backward takes out before its rounding
 NORMS = {"none": 0, "layer": 1, "rms": 2}                    # SPCONV_NORM_*
 CLIP_P2, CLIP_INF = 0, 1
 
@@ -1177,12 +1176,23 @@ def _attention_args(dtype: torch.dtype, heads: int, key_heads: int, size: int, c
                          causal=causal, scale=scale)
 
 
+def _rest_bytes(out: torch.Tensor) -> int:
+    """Of what out's rounding left out, in whole fours; fp32 out leaves none."""
+    return 0 if out.dtype == torch.float32 else (out.numel() * 2 + 3) // 4 * 4
+
+
+def _kept(a: AttentionArgs, stats: torch.Tensor, out: torch.Tensor) -> None:
+    rest = _rest_bytes(out)
+    a.out_rest = stats.data_ptr() if rest else None
+    a.row_stats = stats.data_ptr() + rest
+
+
 @_on_device
 def attention_forward(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, offsets: Optional[torch.Tensor],
                       key_offsets: Optional[torch.Tensor], causal: bool, scale: float, keep_stats: bool = False,
                       kernel: int = KERNEL_AUTO) -> tuple:
-    """(out, what the backward needs of it if ``keep_stats``: row statistics and, where rows see few keys on average, what
-    out's rounding left out, else None; the call's arguments for attention_backward_of)."""
+    """(out, what the backward needs of it if ``keep_stats``, in one tensor: what out's rounding left out, in 16 bits, and
+    row statistics, else None; the call's arguments for attention_backward_of)."""
     dev = _require_cuda(query, key, value, offsets, key_offsets)
     dtype = query.dtype
     if key.dtype != dtype or value.dtype != dtype:
@@ -1208,12 +1218,8 @@ def attention_forward(query: torch.Tensor, key: torch.Tensor, value: torch.Tenso
     a.out = out.data_ptr()
     stats = None
     if keep_stats:
-        stats = torch.empty((M, H), dtype=torch.float32, device=dev)
-        a.row_stats = stats.data_ptr()
-        if N <= ATTENTION_FEW_KEYS * a.num_samples and dtype != torch.float32:
-            rest = torch.empty_like(out)
-            a.out_rest = rest.data_ptr()
-            stats = (stats, rest)
+        stats = torch.empty(_rest_bytes(out) + M * H * 4, dtype=torch.uint8, device=dev)
+        _kept(a, stats, out)
     if M == 0:
         return out, stats, a
     ws = _attention_workspace(a, False, dev)
@@ -1237,10 +1243,8 @@ def attention_backward_of(args: AttentionArgs, query, key, value, offsets, key_o
     (a.query_row, a.query_head, _), (a.key_row, a.key_head, _), (a.value_row, a.value_head, _) = (
         query.stride(), key.stride(), value.stride())
     a.offsets, a.key_offsets = _ptr(offsets), _ptr(key_offsets)
-    if isinstance(stats, tuple):
-        stats, rest = stats
-        a.out_rest = rest.data_ptr()
-    a.out, a.row_stats = out.data_ptr(), stats.data_ptr()
+    a.out = out.data_ptr()
+    _kept(a, stats, out)
     a.grad_out, a.grad_row, a.grad_head = grad_out.data_ptr(), grad_out.stride(0), grad_out.stride(1)
     grads = [t.new_empty(t.shape) if n else None for t, n in zip((query, key, value), needs)]
     a.grad_query, a.grad_key, a.grad_value = map(_ptr, grads)

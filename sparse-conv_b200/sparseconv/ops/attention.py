@@ -17,16 +17,15 @@ class SparseAttentionFunction(Function):
     @staticmethod
     def forward(ctx, query, key, value, offsets, key_offsets, causal, scale):
         out, stats, ctx.args = _native.attention_forward(query, key, value, offsets, key_offsets, causal, scale, keep_stats=True)
-        ctx.save_for_backward(query, key, value, offsets, key_offsets, out, *(stats if isinstance(stats, tuple) else (stats, None)))
+        ctx.save_for_backward(query, key, value, offsets, key_offsets, out, stats)
         return out
 
     @staticmethod
     def backward(ctx, grad_out):
-        """The probabilities again, from the inputs and a number a row that the forward kept."""
+        """The probabilities again, from the inputs and what the forward kept."""
         if torch.is_grad_enabled():              # create_graph=True: these gradients would be constants
             raise NotImplementedError("sparse_attention has no second derivative")
-        *saved, stats, rest = ctx.saved_tensors
-        grads = _native.attention_backward_of(ctx.args, *saved, stats if rest is None else (stats, rest), grad_out, ctx.needs_input_grad)
+        grads = _native.attention_backward_of(ctx.args, *ctx.saved_tensors, grad_out, ctx.needs_input_grad)
         return (*grads, None, None, None, None)
 
 
@@ -59,8 +58,8 @@ def sparse_attention(
         [N, heads, D] in the query's dtype; zeros for a query that sees no key. Scores, softmax and sums are fp32.
         fp16 and bf16 heads of up to 128 values run on the tensor cores, where the probabilities (and in the backward
         their gradients) enter the second product rounded to the dtype; fp32 and wider heads run in fp32 on the CUDA
-        cores. For the backward a number a row is kept, and in 16 bits, for samples of at most 128 keys on average, what out's
-        rounding left out. The gradients add in a fixed order: the same bits every run.
+        cores. For the backward a number a row is kept, and in 16 bits what out's rounding left out, as large as out. The
+        gradients add in a fixed order: the same bits every run.
     """
     _native.refuse_forward_mode("sparse_attention", query, key, value)
     if batch_offsets is None and key_offsets is not None:

@@ -70,3 +70,52 @@ def test_small_fp16_gradients_beside_others(mate, D, first):
     for name, a, b, whole in zip("qkv", got, want, (q2, k2, v2)):
         at = whole.shape[0] if order(0, 1)[0] == 1 else 0
         assert relative(a[at:at + n], b) < eps + small_step(b), (name, relative(a[at:at + n], b))
+
+
+TYPES16 = [torch.bfloat16, torch.float16]
+
+
+def apart(rows, D, dtype, seed, heads=2):
+    """Queries, keys, values and gradients whose scores are far apart, as a trained network's: a row's weight is on a few keys, and
+    out's rounding then of ds's size, however many keys there are. What is left without it is four roundings (p's in out and in
+    the values' gradient, ds's, the result's) of 0.42 half steps each in the mean square of a uniform mantissa: under one."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    q, k, v, grad = (torch.randn(r, heads, D, generator=g, device="cuda") for r in rows)
+    return [t.to(dtype).requires_grad_() for t in (q * 4.0, k, v)], grad.to(dtype)
+
+
+def check(got, want, dtype):
+    for name, a, b in zip("qkv", got, want):
+        assert relative(a, b) < torch.finfo(dtype).eps / 2, (name, relative(a, b) / (torch.finfo(dtype).eps / 2))
+
+
+@pytest.mark.parametrize("dtype", TYPES16)
+@pytest.mark.parametrize("D", [64, 128, 136])
+def test_short_samples_beside_a_long_one(dtype, D):
+    """Windows of two keys beside a scene of 20,000: as near to 64 bits, and to the bit, as without it."""
+    m, windows, long = 2, 100, 20000
+    leaves, grad = apart([windows * m + long] * 4, D, dtype, D)
+    got = torch.autograd.grad(sparse_attention(*leaves, ends([m] * windows + [long])), leaves, grad)
+    each = [gradients64(*(t.detach()[i:i + m] for t in leaves), grad[i:i + m]) for i in range(0, windows * m, m)]
+    check([t[:windows * m] for t in got], [torch.cat(t) for t in zip(*each)], dtype)
+    alone = [t.detach()[:windows * m].clone().requires_grad_() for t in leaves]
+    want = torch.autograd.grad(sparse_attention(*alone, ends([m] * windows)), alone, grad[:windows * m])
+    assert all(torch.equal(a[:windows * m], b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", TYPES16)
+@pytest.mark.parametrize("D", [64, 128, 136])
+def test_first_rows_of_a_long_causal_sample(dtype, D):
+    """They see 1 to 16 keys."""
+    leaves, grad = apart([2000] * 4, D, dtype, D)
+    (gq,) = torch.autograd.grad(sparse_attention(*leaves, causal=True), leaves[:1], grad)
+    check([gq[:16]], [gradients64(*leaves, grad, causal=True)[0][:16]], dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES16)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("n,m", [(300, 129), (300, 257), (700, 2000)])
+def test_few_keys_that_count_among_many(dtype, D, n, m):
+    leaves, grad = apart([n, m, m, n], D, dtype, m)
+    got = torch.autograd.grad(sparse_attention(*leaves, ends([n]), ends([m])), leaves, grad)
+    check(got, gradients64(*leaves, grad), dtype)
