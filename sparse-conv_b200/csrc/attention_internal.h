@@ -45,7 +45,7 @@ int launch_at_simt_grad_query(const AtArgs &a);
 int launch_at_simt_grad_key(const AtArgs &a);
 int at_simt_rows(int D);                 // rows (and keys) of a tile
 
-// Tensor cores (fp16, bf16; sizes that are multiples of 8 up to 128).
+// Tensor cores (fp16, bf16; sizes up to 128, whose rows and heads lie whole multiples of 16 bytes apart: the size itself is any).
 int launch_at_tc_forward(const AtArgs &a, bool pair);        // pair: of tiles of 128 rows a CTA, not one (sizes over 64)
 int launch_at_tc_grad_query(const AtArgs &a);
 int launch_at_tc_grad_key(const AtArgs &a);
