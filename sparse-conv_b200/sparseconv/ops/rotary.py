@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import functools
 import math
+import operator
 from typing import Optional, Tuple
 
 import torch
@@ -31,7 +32,11 @@ class RotaryScaling:
 YARN_TURNS = (1.0, 32.0)
 
 
-@functools.lru_cache(maxsize=64)
+def _number(x, what: str) -> float:
+    """A setting's value now, by which plans are kept (a tensor of it may be another one at the next call)."""
+    return float(x)
+
+
 def rotary_steps(pairs: int, base: float = 10000.0, scaling: str = RotaryScaling.NONE, factor: float = 1.0,
                  trained_size: Optional[int] = None) -> Tuple[Tuple[float, ...], float]:
     """(angle of one unit of position for each of an axis's pairs, amplitude of the rotation).
@@ -42,6 +47,16 @@ def rotary_steps(pairs: int, base: float = 10000.0, scaling: str = RotaryScaling
     one full turn within ``trained_size``, leaves those of more than 32, and goes linearly between them, with an
     amplitude of ``0.1 log(factor) + 1`` (on queries and keys, so scores grow by its square).
     """
+    return _steps(operator.index(pairs), *_settings(base, scaling, factor, trained_size))
+
+
+def _settings(base, scaling: str, factor, trained_size) -> tuple:
+    return (_number(base, "base"), scaling, _number(factor, "factor"),
+            None if trained_size is None else _number(trained_size, "trained_size"))
+
+
+@functools.lru_cache(maxsize=64)
+def _steps(pairs: int, base: float, scaling: str, factor: float, trained_size: Optional[float]) -> Tuple[Tuple[float, ...], float]:
     if scaling not in (RotaryScaling.NONE, RotaryScaling.LINEAR, RotaryScaling.NTK, RotaryScaling.YARN):
         raise ValueError(f"unsupported scaling {scaling}")
     if not (base > 0.0 and math.isfinite(base)):
@@ -70,14 +85,14 @@ def rotary_steps(pairs: int, base: float = 10000.0, scaling: str = RotaryScaling
 
 @functools.lru_cache(maxsize=64)
 def _plan(size: int, rotary_dim: Optional[int], axes: int, layout: str, base: float, scaling: str, factor: float,
-          trained_size: Optional[int]) -> _native.RotaryPlan:
+          trained_size: Optional[float]) -> _native.RotaryPlan:
     if rotary_dim is None:
         rotary_dim = size // 2 * 2
     pairs = rotary_dim // 2 // max(axes, 1)
     if rotary_dim % 2 or not 2 <= rotary_dim <= size or pairs < 1:
         raise ValueError(f"rotary_dim must be even, at most the head size {size} and at least twice the {axes} axes, "
                          f"got {rotary_dim}")
-    return _native.RotaryPlan(layout, rotary_dim, axes, *rotary_steps(pairs, float(base), scaling, float(factor), trained_size))
+    return _native.RotaryPlan(layout, rotary_dim, axes, *_steps(pairs, base, scaling, factor, trained_size))
 
 
 class SparseRotaryFunction(Function):
@@ -138,7 +153,8 @@ def sparse_rotary(
     if positions.dim() not in (1, 2):
         raise ValueError(f"positions must be [N] or [N, axes], got shape {list(positions.shape)}")
     axes = 1 if positions.dim() == 1 else positions.shape[-1]
-    plan = _plan(first.shape[2], rotary_dim, axes, layout, base, scaling, factor, trained_size)
+    plan = _plan(first.shape[2], None if rotary_dim is None else operator.index(rotary_dim), axes, layout,
+                 *_settings(base, scaling, factor, trained_size))
     if torch.is_grad_enabled() and ((query is not None and query.requires_grad) or (key is not None and key.requires_grad)):
         return SparseRotaryFunction.apply(query, key, positions, plan)
     return _native.rotary(query, key, positions, plan)

@@ -1,0 +1,34 @@
+"""Numbers given to rotary positions and attention count by their value at the call: tensors of them too, which may have changed since
+the last one."""
+import pytest
+import torch
+
+from sparseconv.ops.attention import sparse_attention
+from sparseconv.ops.rotary import rotary_steps, sparse_rotary
+
+
+def test_steps_of_a_base_that_changes():
+    base, factor = torch.tensor(100.0), torch.tensor(2.0)
+    assert rotary_steps(4, base, "linear", factor) == rotary_steps(4, 100.0, "linear", 2.0)
+    base.fill_(10000.0)
+    factor.fill_(4.0)
+    steps, _ = rotary_steps(4, base, "linear", factor)
+    assert steps == rotary_steps(4, 10000.0, "linear", 4.0)[0] and all(isinstance(s, float) for s in steps)
+    size = torch.tensor(1000)
+    first = rotary_steps(4, 1e4, "yarn", 4.0, size)
+    size.fill_(50)
+    assert first == rotary_steps(4, 1e4, "yarn", 4.0, 1000) and rotary_steps(4, 1e4, "yarn", 4.0, size) == rotary_steps(4, 1e4, "yarn", 4.0, 50)
+
+
+@pytest.mark.gpu
+def test_rotary_by_a_base_that_changes():
+    q = torch.randn(5, 2, 16, device="cuda")
+    pos = torch.arange(5, device="cuda", dtype=torch.int32)
+    base = torch.tensor(100.0)
+    assert torch.equal(sparse_rotary(q, None, pos, base=base)[0], sparse_rotary(q, None, pos, base=100.0)[0])
+    base.fill_(10000.0)
+    assert torch.equal(sparse_rotary(q, None, pos, base=base)[0], sparse_rotary(q, None, pos, base=10000.0)[0])
+    scale = torch.tensor(0.5)
+    first = sparse_attention(q, q, q, scale=scale)
+    scale.fill_(0.25)
+    assert torch.equal(first, sparse_attention(q, q, q, scale=0.5)) and torch.equal(sparse_attention(q, q, q, scale=scale), sparse_attention(q, q, q, scale=0.25))
