@@ -52,7 +52,7 @@ def sparse_attention(
             library's other device-side checks do. Samples may have no queries, or no keys.
         causal: each query sees the keys up to its own place, counted from the sample's end (the last query sees the
             last key), so one new query a sample sees everything.
-        scale: factor of the scores, positive; None: D ** -0.5.
+        scale: factor of the scores, a positive number; None: D ** -0.5. It has no gradient.
 
     Returns:
         [N, heads, D] in the query's dtype; zeros for a query that sees no key. Scores, softmax and sums are fp32.
@@ -68,8 +68,7 @@ def sparse_attention(
         if batch_offsets is not None and key.shape[0] != query.shape[0]:
             raise ValueError("as many keys as queries are needed where key_offsets is not given")
         key_offsets = batch_offsets
-    if scale is None:
-        scale = max(query.shape[-1], 1) ** -0.5
+    scale = max(query.shape[-1], 1) ** -0.5 if scale is None else _native.constant("sparse_attention", "scale", scale)
     if torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad):
-        return SparseAttentionFunction.apply(query, key, value, batch_offsets, key_offsets, bool(causal), float(scale))
+        return SparseAttentionFunction.apply(query, key, value, batch_offsets, key_offsets, bool(causal), scale)
     return _native.attention_forward(query, key, value, batch_offsets, key_offsets, causal, scale)[0]

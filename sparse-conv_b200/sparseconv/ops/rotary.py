@@ -32,11 +32,6 @@ class RotaryScaling:
 YARN_TURNS = (1.0, 32.0)
 
 
-def _number(x, what: str) -> float:
-    """A setting's value now, by which plans are kept (a tensor of it may be another one at the next call)."""
-    return float(x)
-
-
 def rotary_steps(pairs: int, base: float = 10000.0, scaling: str = RotaryScaling.NONE, factor: float = 1.0,
                  trained_size: Optional[int] = None) -> Tuple[Tuple[float, ...], float]:
     """(angle of one unit of position for each of an axis's pairs, amplitude of the rotation).
@@ -51,8 +46,9 @@ def rotary_steps(pairs: int, base: float = 10000.0, scaling: str = RotaryScaling
 
 
 def _settings(base, scaling: str, factor, trained_size) -> tuple:
-    return (_number(base, "base"), scaling, _number(factor, "factor"),
-            None if trained_size is None else _number(trained_size, "trained_size"))
+    """Their values now, by which plans are kept (a tensor of one may hold another at the next call)."""
+    return (_native.constant("rotary positions", "base", base), scaling, _native.constant("rotary positions", "factor", factor),
+            None if trained_size is None else _native.constant("rotary positions", "trained_size", trained_size))
 
 
 @functools.lru_cache(maxsize=64)

@@ -1,5 +1,7 @@
 """Numbers given to rotary positions and attention count by their value at the call: tensors of them too, which may have changed since
-the last one."""
+the last one, and whose gradients there are not."""
+import warnings
+
 import pytest
 import torch
 
@@ -32,3 +34,17 @@ def test_rotary_by_a_base_that_changes():
     first = sparse_attention(q, q, q, scale=scale)
     scale.fill_(0.25)
     assert torch.equal(first, sparse_attention(q, q, q, scale=0.5)) and torch.equal(sparse_attention(q, q, q, scale=scale), sparse_attention(q, q, q, scale=0.25))
+
+
+def test_learned_settings_are_refused():
+    """Their gradients would be lost without a word. Where none are asked for, they are numbers."""
+    q, pos = torch.zeros(10, 4, 64), torch.zeros(10, dtype=torch.int32)
+    learned = torch.tensor(2.0, requires_grad=True)
+    for call in (lambda: sparse_attention(q, q, q, scale=learned), lambda: sparse_rotary(q, q, pos, base=learned),
+                 lambda: sparse_rotary(q, q, pos, scaling="linear", factor=learned),
+                 lambda: sparse_rotary(q, q, pos, scaling="yarn", factor=2.0, trained_size=learned)):
+        with pytest.raises(NotImplementedError, match="gradient"):
+            call()
+        with torch.no_grad(), warnings.catch_warnings(), pytest.raises(RuntimeError, match="CUDA"):
+            warnings.simplefilter("error")
+            call()
