@@ -440,7 +440,7 @@ int spconv_rotary(const spconv_rotary_args *args, void *stream);
  *   needs grad_out . out. Without it the gradients of queries and keys of rows whose weight is on a few keys, however many they
  *   see, are off by up to twice as much
  *   num_queries, num_keys: up to 2^31 - 1024
- *   scale: positive. head_size <= 256. kernel: SPCONV_KERNEL_*; the tensor-core kernels take fp16 and bf16 heads of up
+ *   scale: positive, up to 2.35e38 (1.44 times it is finite). head_size <= 256. kernel: SPCONV_KERNEL_*; the tensor-core kernels take fp16 and bf16 heads of up
  *   to 128 values and return SPCONV_ERR_UNSUPPORTED for others
  * Products accumulate in fp32, as softmax statistics and row sums; outputs are rounded once. On the tensor cores p and its
  * gradient are rounded to dtype, as their operands.

@@ -350,6 +350,9 @@ static AtPlan at_plan(const spconv_attention_args *q, bool backward) {
     return p;
 }
 
+// A score's factor in powers of two.
+static float at_exponent(float scale) { return (float)((double)scale * 1.4426950408889634); }
+
 static int at_check(const spconv_attention_args *q, bool backward) {
     SPCONV_REQUIRE(q != nullptr, SPCONV_ERR_ARG, "null pointer argument");
     SPCONV_REQUIRE(q->dtype == SPCONV_F32 || q->dtype == SPCONV_F16 || q->dtype == SPCONV_BF16, SPCONV_ERR_ARG,
@@ -364,7 +367,7 @@ static int at_check(const spconv_attention_args *q, bool backward) {
                    "heads must be a multiple of key_heads, at most 65535");
     SPCONV_REQUIRE(q->head_size >= 1 && q->head_size <= SPCONV_ATTENTION_MAX_SIZE, SPCONV_ERR_ARG, "head size must be in [1, %d]",
                    SPCONV_ATTENTION_MAX_SIZE);
-    SPCONV_REQUIRE(q->scale > 0.f && q->scale < INFINITY, SPCONV_ERR_ARG, "scale must be positive and finite");
+    SPCONV_REQUIRE(q->scale > 0.f && at_exponent(q->scale) < INFINITY, SPCONV_ERR_ARG, "scale must be positive and finite, its 1.44-fold too");
     SPCONV_REQUIRE((q->offsets && q->key_offsets) || q->num_samples == 1, SPCONV_ERR_ARG, "several samples need the row offsets of both sides");
     SPCONV_REQUIRE(q->kernel != SPCONV_KERNEL_TCGEN05 || (q->dtype != SPCONV_F32 && q->head_size <= 128), SPCONV_ERR_UNSUPPORTED,
                    "the tensor-core kernels take fp16 and bf16 heads of at most 128 values");
@@ -401,7 +404,7 @@ static int at_prepare(const spconv_attention_args *q, const AtPlan &p, bool back
     a.D = q->head_size;
     a.causal = q->causal != 0;
     a.scale = q->scale;
-    a.c = (float)((double)q->scale * 1.4426950408889634);
+    a.c = at_exponent(q->scale);
     a.status = q->status;
     a.wait_ns = wait_limit_ns();
     a.dtype = q->dtype;

@@ -1,5 +1,6 @@
 """Numbers given to rotary positions and attention count by their value at the call: tensors of them too, which may have changed since
 the last one, and whose gradients there are not."""
+import math
 import warnings
 
 import pytest
@@ -48,3 +49,13 @@ def test_learned_settings_are_refused():
         with torch.no_grad(), warnings.catch_warnings(), pytest.raises(RuntimeError, match="CUDA"):
             warnings.simplefilter("error")
             call()
+
+
+@pytest.mark.gpu
+def test_scales_past_the_range_are_refused():
+    """A score's factor to base 2 is 1.44 times the scale."""
+    q = torch.zeros(10, 2, 64, device="cuda")
+    for scale in (3e38, 1e39, 1e-50):
+        with pytest.raises(ValueError, match="scale"):
+            sparse_attention(q, q, q, scale=scale)
+    assert math.isfinite(sparse_attention(q, q, q, scale=2.3e38).sum().item())
