@@ -27,6 +27,7 @@
 // Rows behind a sample's end are treated as in the forward: zeroed in shared memory where a product sums over rows.
 #include <algorithm>
 
+#include "attention_hidden.cuh"
 #include "attention_tc.cuh"
 
 namespace spconv {
@@ -39,9 +40,11 @@ struct AbShape {
     static constexpr int kPerSm = DP == 64 && W == 64 ? 2 : 1, kColumns = 512 / kPerSm;
     static constexpr int kOwn = DP / 64 * kAtBlock, kTile = DP / 64 * W * 128;      // bytes of an own tile, and of a walked one
 };
-// A row of accumulators [from, to) times `factor`, to a row of D values: rounded, or fp32 where `part` is given.
-template <typename T>
-__device__ __forceinline__ void ab_store_row(uint32_t taddr, int from, int to, int D, bool zero, float factor, bool mine, T *out, float *part) {
+// A row of accumulators [from, to) times `factor`, to a row of D values: rounded, or fp32 where `part` is given; zeros if `none`, and
+// without a look at them if `zero`, which holds for the warp. Whether one is not finite, if that is asked for.
+template <typename T, bool ASK>
+__device__ __forceinline__ bool ab_store_row(uint32_t taddr, int from, int to, int D, bool zero, bool none, float factor, bool mine, T *out, float *part) {
+    f32x2 lost = pack_f32x2(0.f, 0.f);                               // NaN once a value was not finite
     const bool wide = (D & 7) == 0 && ((uintptr_t)out & 15) == 0;
 #pragma unroll 1
     for (int c = from; c < to && c < D; c += 32) {
@@ -49,6 +52,10 @@ __device__ __forceinline__ void ab_store_row(uint32_t taddr, int from, int to, i
         __syncwarp();                                                // lanes without a row come here before those that store
         if (!zero) lt_load32(taddr + c, o);
         if (!mine) continue;
+        if (ASK && !zero) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) lost = fma2(o[i], pack_f32x2(0.f, 0.f), lost);
+        }
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
             const int d = c + v * 8;
@@ -58,8 +65,8 @@ __device__ __forceinline__ void ab_store_row(uint32_t taddr, int from, int to, i
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const float2 u = unpack_f32x2(o[v * 4 + i]);
-                f[2 * i] = zero ? 0.f : u.x * factor;
-                f[2 * i + 1] = zero ? 0.f : u.y * factor;
+                f[2 * i] = zero || none ? 0.f : u.x * factor;
+                f[2 * i + 1] = zero || none ? 0.f : u.y * factor;
                 w[i] = lt_pack<T>(f[2 * i], f[2 * i + 1]);
             }
             if (part && (D & 7) == 0) {                              // (the workspace is aligned, and so are rows of eights)
@@ -78,6 +85,8 @@ __device__ __forceinline__ void ab_store_row(uint32_t taddr, int from, int to, i
             }
         }
     }
+    const float2 z = unpack_f32x2(lost);
+    return !(z.x + z.y == 0.f);
 }
 
 template <int DP, int W>
@@ -86,7 +95,7 @@ struct AqShape : AbShape<DP, W> {
     static constexpr int kSmem = 1024 + 2 * AbShape<DP, W>::kOwn + (kK + kV) * AbShape<DP, W>::kTile + 512;
 };
 
-template <typename T, int DP, int W>
+template <typename T, int DP, int W, bool CAUSAL>
 __global__ void __launch_bounds__(AbShape<DP, W>::kThreads, AbShape<DP, W>::kPerSm)
 attention_tc_grad_query_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                                const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_g,
@@ -290,7 +299,12 @@ attention_tc_grad_query_kernel(const __grid_constant__ CUtensorMap map_q, const 
         if (ok && some) {
             constexpr int kCols = DP * 32 / W > 32 ? DP * 32 / W : 32;               // a part's (with more parts than 32s: none)
             float *to = a.splits > 1 ? a.partial + (blockIdx.z * (int64_t)a.M * a.H + at) * a.D : nullptr;
-            ab_store_row<T>(t_dq + lanes, part * kCols, part * kCols + kCols, a.D, tiles == 0, ldexpf(a.scale, -lift), mine, (T *)a.gq + at * a.D, to);
+            const AtHidden hidden{s.q0 + token, head0 + (row & (P - 1)), kh, s.k0, first * W, seen, min(m, (first + tiles) * W)};
+            const int c0 = part * kCols;
+            const bool lost = ab_store_row<T, CAUSAL>(t_dq + lanes, c0, c0 + kCols, a.D, tiles == 0, seen == 0, ldexpf(a.scale, -lift), mine,
+                                              (T *)a.gq + at * a.D, to);
+            if (CAUSAL && lost && seen > 0 && seen < hidden.hi && lse == lse && delta == delta)
+                at_keys_again<T>(a, hidden, -lse, delta, c0, c0 + kCols, a.scale, {to, (T *)a.gq + at * a.D});
         }
     }
 
@@ -313,7 +327,7 @@ struct AkShape : AbShape<DP, W> {
     static constexpr int kSmem = 1024 + 2 * AbShape<DP, W>::kOwn + 2 * kStages * AbShape<DP, W>::kTile + kStages * W * 8 + 512;
 };
 
-template <typename T, int DP, int W>
+template <typename T, int DP, int W, bool CAUSAL>
 __global__ void __launch_bounds__(AbShape<DP, W>::kThreads, AbShape<DP, W>::kPerSm)
 attention_tc_grad_key_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                              const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_g,
@@ -576,9 +590,10 @@ attention_tc_grad_key_kernel(const __grid_constant__ CUtensorMap map_q, const __
             float *to = a.splits > 1 ? a.partial + ((2 * blockIdx.z + !keys) * all + at) * a.D : nullptr;
             T *out = (T *)(keys ? a.gk : a.gv);
             const int c0 = (part & (kParts - 1)) * kCols;
-            ab_store_row<T>((keys ? t_dk : t_dv) + lanes, c0, c0 + kCols, a.D, tiles == 0, keys ? ldexpf(a.scale, -lift) : kDown,
-                            mine && (out || to),
-                            out ? out + at * a.D : nullptr, to);
+            if (out) out += at * a.D;
+            const bool lost = ab_store_row<T, CAUSAL>((keys ? t_dk : t_dv) + lanes, c0, c0 + kCols, a.D, tiles == 0, false,
+                                              keys ? ldexpf(a.scale, -lift) : kDown, mine && (out || to), out, to);
+            if (CAUSAL && lost) at_rows_again<T>(a, *s_sample, kAtRows, W, log_p, !keys, c0, c0 + kCols, {to, out});
         }
     }
 
@@ -595,7 +610,7 @@ attention_tc_grad_key_kernel(const __grid_constant__ CUtensorMap map_q, const __
     if (warp == 0) tmem_dealloc(tmem, S::kColumns);
 }
 
-template <typename T, int DP, int W, bool KEYS>
+template <typename T, int DP, int W, bool KEYS, bool CAUSAL>
 static int ab_run(const AtArgs &a) {
     using S = AbShape<DP, W>;
     const int G = a.H / a.K;
@@ -608,7 +623,7 @@ static int ab_run(const AtArgs &a) {
         !at_map(&mv, a.v, a.N, a.K, a.D, 1, keys) || !at_map(&mg, a.grad, a.M, a.H, a.D, P, tokens))
         return SPCONV_ERR_CUDA;
     static std::atomic<uint64_t> done;
-    auto kern = KEYS ? attention_tc_grad_key_kernel<T, DP, W> : attention_tc_grad_query_kernel<T, DP, W>;
+    auto kern = KEYS ? attention_tc_grad_key_kernel<T, DP, W, CAUSAL> : attention_tc_grad_query_kernel<T, DP, W, CAUSAL>;
     // padded so that no more CTAs share an SM than its TMEM columns serve
     constexpr int need = KEYS ? AkShape<DP, W>::kSmem : AqShape<DP, W>::kSmem, least = S::kPerSm == 2 ? 80 * 1024 : 120 * 1024;
     constexpr int smem = need > least ? need : least;
@@ -620,7 +635,8 @@ static int ab_run(const AtArgs &a) {
 
 template <typename T, bool KEYS>
 static int ab_size(const AtArgs &a) {
-    return a.D <= 64 ? ab_run<T, 64, 64, KEYS>(a) : ab_run<T, 128, 128, KEYS>(a);
+    if (a.causal) return a.D <= 64 ? ab_run<T, 64, 64, KEYS, true>(a) : ab_run<T, 128, 128, KEYS, true>(a);
+    return a.D <= 64 ? ab_run<T, 64, 64, KEYS, false>(a) : ab_run<T, 128, 128, KEYS, false>(a);
 }
 
 int launch_at_tc_grad_query(const AtArgs &a) {

@@ -30,6 +30,7 @@
 // before it frees TMEM and exits.
 #include <algorithm>
 
+#include "attention_hidden.cuh"
 #include "attention_tc.cuh"
 
 namespace spconv {
@@ -41,12 +42,14 @@ constexpr float kAfSlack = 8.f;                      // by how much the maximum 
 template <typename T>
 constexpr float kAfUp = dtype_traits<T>::mma_format == 0 ? 7.f : 0.f;
 
-// A row's result: its accumulators over its sum, zeros if it sees no key (`none`: of this split); or, where keys are split, the
+// A row's result: its accumulators over its sum, zeros if it sees no key (of this split); or, where keys are split, the
 // accumulators as they are. A warp's lanes together.
-template <typename T>
-__device__ __forceinline__ void af_store(const AtArgs &a, uint32_t t_o, int size, int64_t at, bool mine, bool none, bool nothing, float top,
+template <typename T, bool CAUSAL>
+__device__ __forceinline__ void af_store(const AtArgs &a, uint32_t t_o, int size, const AtHidden &row, bool mine, bool nothing, float top,
                                          float sum) {
-    const int64_t all = (int64_t)a.M * a.H;
+    const int64_t all = (int64_t)a.M * a.H, at = row.row * a.H + row.head;
+    bool none = row.seen <= row.lo;
+    f32x2 lost = pack_f32x2(0.f, 0.f);                               // NaN once a value was not finite
     float *part = a.splits > 1 ? a.partial + (blockIdx.z * all + at) * a.D : nullptr;
     const float inv = part ? 1.f : none ? 0.f : 1.f / sum;
     if (mine) {
@@ -66,6 +69,10 @@ __device__ __forceinline__ void af_store(const AtArgs &a, uint32_t t_o, int size
         }
         if (!mine || (part && nothing)) continue;
         none |= nothing;
+        if constexpr (CAUSAL) {
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) lost = fma2(pack_f32x2(__uint_as_float(o[i]), __uint_as_float(o[i + 1])), pack_f32x2(0.f, 0.f), lost);
+        }
         if (!part && whole) {
             // a lane's 16 values are a sector: out and rest of voxels to 257 tokens 334 -> 252 us (out alone 240 -> 236)
             uint32_t w[8];
@@ -117,6 +124,9 @@ __device__ __forceinline__ void af_store(const AtArgs &a, uint32_t t_o, int size
             }
         }
     }
+    const float2 z = unpack_f32x2(lost);
+    if (CAUSAL && !(z.x + z.y == 0.f) && !none && row.seen < row.hi && sum == sum)
+        at_values_again<T>(a, row, fmaf(-top, a.c, kAfUp<T>), inv, part);
 }
 
 // A CTA a tile of queries.
@@ -129,7 +139,7 @@ struct AfShape {
     static constexpr int kThreads = 160, kControl = 4;
 };
 
-template <typename T, int DP>
+template <typename T, int DP, bool CAUSAL>
 __global__ void __launch_bounds__(AfShape<DP>::kThreads, AfShape<DP>::kPerSm)
 attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                       const __grid_constant__ CUtensorMap map_v, const __grid_constant__ AtArgs a, const int log_p) {
@@ -328,8 +338,8 @@ attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         if (tiles > 0 && ok) ok = wait(sfull, tiles & 1);            // the last p v
         tc_fence_after();
         if (ok && some)
-            af_store<T>(a, t_o, DP, (int64_t)(s.q0 + token) * a.H + head0 + (tid & (P - 1)), mine, seen <= first * S::kKeys,
-                        tiles == 0, top, sum);
+            af_store<T, CAUSAL>(a, t_o, DP, AtHidden{s.q0 + token, head0 + (tid & (P - 1)), kh, s.k0, first * S::kKeys, seen,
+                                             min(m, (first + tiles) * S::kKeys)}, mine, tiles == 0, top, sum);
     }
 
     __syncwarp();
@@ -355,7 +365,7 @@ struct ApShape {
     static constexpr int kAcc = 256;                 // first column of the accumulators, behind two tiles' scores
 };
 
-template <typename T>
+template <typename T, bool CAUSAL>
 __global__ void __launch_bounds__(ApShape::kThreads, 1)
 attention_tc_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                     const __grid_constant__ CUtensorMap map_v, const __grid_constant__ AtArgs a, const int log_p) {
@@ -575,8 +585,8 @@ attention_tc_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             if (tiles > 0 && ok) ok = __all_sync(0xffffffffu, wait(&odone[q], (tiles - 1) & 1)) != 0;     // the last p v
             tc_fence_after();
             if (ok && some)
-                af_store<T>(a, t_o, DP, (int64_t)(s.q0 + token) * a.H + head0 + (row & (P - 1)), mine, seen <= first * kAtRows,
-                            tiles == 0, top, sum);
+                af_store<T, CAUSAL>(a, t_o, DP, AtHidden{s.q0 + token, head0 + (row & (P - 1)), kh, s.k0, first * kAtRows, seen,
+                                                 min(m, (first + tiles) * kAtRows)}, mine, tiles == 0, top, sum);
         }
     }
 
@@ -611,16 +621,18 @@ static int af_run(const AtArgs &a, K kern, int keys, std::atomic<uint64_t> &done
     return check_launch("attention_tc_kernel");
 }
 
-template <typename T>
+template <typename T, bool CAUSAL>
 static int af_type(const AtArgs &a, bool pair) {
     static std::atomic<uint64_t> done[3];
-    if (a.D <= 64) return af_run<T, AfShape<64>, false>(a, attention_tc_kernel<T, 64>, AfShape<64>::kKeys, done[0]);
-    if (!pair) return af_run<T, AfShape<128>, false>(a, attention_tc_kernel<T, 128>, AfShape<128>::kKeys, done[1]);
-    return af_run<T, ApShape, true>(a, attention_tc_pair_kernel<T>, kAtRows, done[2]);
+    if (a.D <= 64) return af_run<T, AfShape<64>, false>(a, attention_tc_kernel<T, 64, CAUSAL>, AfShape<64>::kKeys, done[0]);
+    if (!pair) return af_run<T, AfShape<128>, false>(a, attention_tc_kernel<T, 128, CAUSAL>, AfShape<128>::kKeys, done[1]);
+    return af_run<T, ApShape, true>(a, attention_tc_pair_kernel<T, CAUSAL>, kAtRows, done[2]);
+}
+template <bool CAUSAL>
+static int af_causal(const AtArgs &a, bool pair) {
+    return a.dtype == SPCONV_F16 ? af_type<__half, CAUSAL>(a, pair) : af_type<__nv_bfloat16, CAUSAL>(a, pair);
 }
 
-int launch_at_tc_forward(const AtArgs &a, bool pair) {
-    return a.dtype == SPCONV_F16 ? af_type<__half>(a, pair) : af_type<__nv_bfloat16>(a, pair);
-}
+int launch_at_tc_forward(const AtArgs &a, bool pair) { return a.causal ? af_causal<true>(a, pair) : af_causal<false>(a, pair); }
 
 }  // namespace spconv

@@ -51,7 +51,8 @@ def sparse_attention(
             queries. Offsets that do not ascend from 0 to the number of rows raise ``RuntimeError`` as the
             library's other device-side checks do. Samples may have no queries, or no keys.
         causal: each query sees the keys up to its own place, counted from the sample's end (the last query sees the
-            last key), so one new query a sample sees everything.
+            last key), so one new query a sample sees everything. Keys that a query does not see leave its row and its
+            gradient as they are, and it theirs, whatever they hold (NaN too).
         scale: factor of the scores, a positive number; None: D ** -0.5. It has no gradient.
 
     Returns:

@@ -32,7 +32,7 @@ def small_step(want):
     return 2.0 ** -25 / (want.norm().item() / want.numel() ** 0.5)
 
 
-@pytest.mark.parametrize("mate", ["nan", "inf", "large", "no keys", "no queries"])
+@pytest.mark.parametrize("mate", ["nan", "inf", "large", "no keys", "no queries", "unseen"])
 @pytest.mark.parametrize("D", [64, 128, 33])
 @pytest.mark.parametrize("first", [False, True])
 def test_small_fp16_gradients_beside_others(mate, D, first):
