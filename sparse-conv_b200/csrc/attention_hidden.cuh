@@ -101,10 +101,11 @@ __device__ __noinline__ void at_keys_again(const AtArgs &a, const AtHidden r, fl
             for (int j = r.seen; j < r.hi && !lost; ++j) lost = at_any_lost(at_row<T>(a.k, r.k0 + j, r.key_head), c, a.D);
         if (!lost) continue;
         float sums[kAtSums] = {};
-        for (int j = r.lo; j < r.seen && r.seen > 1; ++j) {          // (a single key's probability is 1)
+        for (int j = r.lo; j < r.seen; ++j) {
             const T *k = at_row<T>(a.k, r.k0 + j, r.key_head);
             const float p = exp2f(fmaf(at_dot(q, k, a.D), a.c, shift));
-            at_add(sums, p * (at_dot(g, at_row<T>(a.v, r.k0 + j, r.key_head), a.D) - delta), k, c, a.D);
+            const float ds = p * (at_dot(g, at_row<T>(a.v, r.k0 + j, r.key_head), a.D) - delta);
+            at_add(sums, r.seen > 1 ? ds : 0.f, k, c, a.D);          // (a single key's probability is 1)
             if (j % kAtAgain == 0 && at_all_lost(sums, c, a.D)) break;
         }
         to.put(c, a.D, sums, factor);

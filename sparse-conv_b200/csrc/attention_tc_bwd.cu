@@ -303,7 +303,7 @@ attention_tc_grad_query_kernel(const __grid_constant__ CUtensorMap map_q, const 
             const int c0 = part * kCols;
             const bool lost = ab_store_row<T, CAUSAL>(t_dq + lanes, c0, c0 + kCols, a.D, tiles == 0, seen == 0, ldexpf(a.scale, -lift), mine,
                                               (T *)a.gq + at * a.D, to);
-            if (CAUSAL && lost && seen > 0 && seen < hidden.hi && lse == lse && delta == delta)
+            if (CAUSAL && lost && seen > 0 && seen < hidden.hi && (seen == 1 || (lse == lse && delta == delta)))
                 at_keys_again<T>(a, hidden, -lse, delta, c0, c0 + kCols, a.scale, {to, (T *)a.gq + at * a.D});
         }
     }

@@ -123,6 +123,16 @@ def test_queries_before_the_first_key(dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D", [33, 64, 128, 136])
+def test_a_row_that_sees_one_key_and_is_lost(dtype, D):
+    """Its score has no gradient, so its query has none but of what it sees."""
+    q, k, v, grad = setup(200, 200, 2, 2, D, dtype)
+    q[0], k[1:] = math.nan, math.nan
+    _, gq, _, _ = run(q, k, v, grad)
+    assert (gq[0] == 0).all() and gq[1:].isnan().all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("n,D", [(700, 64), (700, 128), (130, 136)])
 def test_all_values_lost(dtype, n, D):
     """NaN everywhere, as after a step that overflowed: every row that sees one is NaN."""
