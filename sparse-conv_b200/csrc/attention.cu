@@ -194,7 +194,8 @@ attention_peaks_kernel(const __grid_constant__ AtArgs a, const int64_t parts, co
 
 // A row's splits: out = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s, over those that saw a key (others have a sum of -1; scores
 // that are all -inf have one of 0, and make the row NaN where no split has another). `share` warps take a row's splits in turn and add up in
-// order: all eight of a block where rows are few (eight rows of 74 splits: 75 us by a warp each), one where they are many.
+// order: all eight of a block where rows are few, one where they are many. Forward by eight warps a row and by one, in us: 8 rows and heads
+// over 200,000 keys 55 and 174, 512 over 20,000 35 and 55, 2,048 over 8,000 41 and 41, 4,096 over 4,096 43 and 35, 8,192 61 and 47.
 template <typename T>
 __global__ void __launch_bounds__(kAtThreads)
 attention_join_kernel(const __grid_constant__ AtArgs a, const int share) {
@@ -284,7 +285,11 @@ struct AtPlan {
 };
 
 // Splits of `tiles` steps each of `ctas` CTAs, of which `slots` run at a time: whole waves, none of fewer than `least` steps. A CTA's
-// start and end count as two steps, and the joining, in the kernels' own time, as six.
+// start and end count as two steps, and the joining, in the kernels' own time, as six. What that chooses against the best of every count
+// up to 256, in us: one query of 8 heads over 10,000 keys 26.6 and 20.4 (64 splits), over 100,000 41.0 and 41.0, eight over 1.0 M 77.8
+// and 77.8; 512 tokens x 16 heads 18.4 and 18.4 (one; two 26.6), 2,048 x 8 47.1 and 45.1, 4,096 x 8 92 and 92 (gradients 82 and 82,
+// 100 and 98); keys' gradients of 257 tokens, 10,534 queries 55.3 and 55.3 (one 185), 16 such samples 436 and 436 (one 510); fp32,
+// 2,000 x 4, 213 and 211, keys' gradients 342 and 315.
 static int at_cut(int64_t ctas, int64_t slots, int64_t tiles, int least) {
     if (ctas == 0 || ctas >= 4 * slots) return 1;
     const int64_t most = std::max<int64_t>(1, std::min<int64_t>({tiles / least, 4 * slots / ctas, 256}));
@@ -310,6 +315,9 @@ static AtPlan at_plan(const spconv_attention_args *q, bool backward) {
     auto up = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
     if (p.tc) {
         const int64_t rows = mean_q * P, heads = q->heads / P;
+        // One tile a CTA and two, 4 heads of 128, samples of n rows and keys, in us: 64 of 320 47 and 59, 16 of 512 24.6 and 24.6, 64 of
+        // 512 78 and 74, 16 of 768 53 and 47, 16 of 2,048 221 and 166. (Two are faster with fewer of them than SMs as well, from 768 keys
+        // on: one sample of 1,024 33 and 27. They are not taken there yet.)
         p.pair = !backward && q->head_size > 64 && rows > 192 && mean_k > 512 && B * up(rows, 256) * heads >= 148;
         // CTAs that run at a time, and what each has to have for itself: 512 keys (a split's rows are written and read once more)
         const int64_t per_sm = q->head_size > 64 ? 1 : 2;

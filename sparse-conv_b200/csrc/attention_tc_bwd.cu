@@ -17,7 +17,8 @@
 // for each barrier that another warp completes and 250 for a product's end). One CTA with W = 128 has the better products
 // (128 columns of B to a read of A) but idles in its own chain: 84,000 voxels in 16 scenes, 8 x 64 bf16, 1.69 and 2.41 ms
 // for the two sweeps, against 1.55 and 2.07; voxels to 257 tokens 0.71 and 0.50, against 0.44 and 0.47; many windows of 130,
-// 0.47 and 0.53, against 0.28 and 0.32. Wider heads: W = 128, one CTA (their accumulators take half of TMEM): 4 x 128 there
+// 0.47 and 0.53, against 0.28 and 0.32 (launches apart from one another; back to back, at the clocks that the power limit leaves, the
+// scenes' forward and sweeps are 5.7 ms where these add up to 5.0). Wider heads: W = 128, one CTA (their accumulators take half of TMEM): 4 x 128 there
 // 1.16 and 1.60 ms, 1.25 and 1.21 PFLOP/s. Nothing is full: at 8,192 tokens x 16 x 64 the tensor pipe is 44 and 43 % in use,
 // the special functions 58 and 43 %, the issue slots 50 and 48 %.
 //

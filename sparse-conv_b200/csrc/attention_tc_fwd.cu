@@ -9,7 +9,8 @@
 // A step is a chain: products, softmax, products; each barrier that another warp completes costs about 170 clocks, a
 // product's end 250, and the 64 exponentials a row 520 of the special functions' time. What fills the gaps is other chains:
 //   * attention_tc_kernel: one tile a CTA, 64 keys a step, four CTAs an SM (two for heads over 64): 128 columns of TMEM and
-//     48 KB each. A fifth warp does both loads and products. 84,000 voxels in 16 scenes, 8 x 64 bf16: 1.32 ms, 0.73 PFLOP/s
+//     48 KB each. A fifth warp does both loads and products. 84,000 voxels in 16 scenes, 8 x 64 bf16: 1.32 ms, 0.73 PFLOP/s, in
+//     launches apart from one another (as all times here; back to back, at the clocks that the power limit leaves, 1.45 ms)
 //     (three CTAs an SM 1.56; one CTA of two tiles and 128 keys a step, whose two chains fell into step with one another,
 //     1.69; the same with the next scores made ahead of p v 1.48; two threads a row 2.02). At 8,192
 //     tokens x 16 x 64 the special functions are 67 % in use, the issue slots 49 %, the tensor pipe 33 %. One pooling query a
