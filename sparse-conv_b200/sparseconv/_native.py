@@ -243,6 +243,8 @@ def refuse_forward_mode(what: str, *tensors: Optional[torch.Tensor]) -> None:
 
 def constant(what: str, name: str, value) -> float:
     """A setting that an operator takes as a number. Raises for a tensor whose gradient is asked for, which would be lost."""
+    if type(value) is float:
+        return value
     if isinstance(value, torch.Tensor):
         if value.requires_grad and torch.is_grad_enabled():
             raise NotImplementedError(f"{what}: no gradient of {name}")

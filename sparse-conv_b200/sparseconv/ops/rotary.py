@@ -97,7 +97,11 @@ class SparseRotaryFunction(Function):
         ctx.save_for_backward(positions)
         ctx.plan = plan
         ctx.set_materialize_grads(False)
-        return _native.rotary(query, key, positions, plan)
+        turned = _native.rotary(query, key, positions, plan)
+        constant = [t for t, needed in zip(turned, ctx.needs_input_grad) if t is not None and not needed]
+        if constant:
+            ctx.mark_non_differentiable(*constant)
+        return turned
 
     @staticmethod
     def backward(ctx, grad_query, grad_key):
