@@ -25,6 +25,11 @@
 // In fp16, whose smallest values would else lose bits where a row sees thousands of keys or gradients are small, p of
 // the keys' sweep comes times 2^15, and ds times the power of two that its bound allows (at_lift); the results are
 // scaled back in fp32. A row that sees a single key has ds = 0 exactly.
+// Heads of up to 32: the queries' sweep takes ds in two parts, rounded and what that leaves, a product each. The roundings' errors
+// add up along what a row's keys have in common (sum p k), which in narrow heads is much of them: over 257 keys, scores of deviation
+// 1.5, the gradients are off by 1.79, 1.62 and 1.52 times their own rounding at 8, 16 and 32 values with one part, by 1.25, 1.13 and
+// 1.07 with two, for 12 % of the sweep's time (windows of 130, 4 x 32: 301 and 338 us). From 48 on it is 1.49 and less, and at 64
+// over long samples two parts would cost 26 %.
 // Rows behind a sample's end are treated as in the forward: zeroed in shared memory where a product sums over rows.
 #include <algorithm>
 
@@ -96,7 +101,7 @@ struct AqShape : AbShape<DP, W> {
     static constexpr int kSmem = 1024 + 2 * AbShape<DP, W>::kOwn + (kK + kV) * AbShape<DP, W>::kTile + 512;
 };
 
-template <typename T, int DP, int W, bool CAUSAL>
+template <typename T, int DP, int W, bool CAUSAL, bool TWO>
 __global__ void __launch_bounds__(AbShape<DP, W>::kThreads, AbShape<DP, W>::kPerSm)
 attention_tc_grad_query_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                                const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_g,
@@ -241,7 +246,9 @@ attention_tc_grad_query_kernel(const __grid_constant__ CUtensorMap map_q, const 
             for (int j = 0; j < tiles && ok; ++j, ds_phase ^= 1u) {
                 if (!(ok = wait(dsready, ds_phase))) break;
                 tc_fence_after();
-                at_mma_rows<32, W>(t_dq, tmem + (j & 1) * W, s_k + done * S::kTile, id_o, j + 1 < tiles ? W / 16 : (end_valid + 15) >> 4, j > 0);
+                const int sum_steps = j + 1 < tiles ? W / 16 : (end_valid + 15) >> 4;
+                at_mma_rows<32, W>(t_dq, tmem + (j & 1) * W, s_k + done * S::kTile, id_o, sum_steps, j > 0);
+                if constexpr (TWO) at_mma_rows<32, W>(t_dq, tmem + (j & 1) * W + 16, s_k + done * S::kTile, id_o, sum_steps, true);
                 tc_commit(smem_u32(j + 1 < tiles ? &kempty[done] : finished));
                 if (++done == S::kK) done = 0;
                 if (j + 1 < tiles) products();
@@ -275,20 +282,29 @@ attention_tc_grad_query_kernel(const __grid_constant__ CUtensorMap map_q, const 
             if (!(ok = __all_sync(0xffffffffu, wait(dpfull, j & 1)) != 0)) break;
             tc_fence_after();
             if (some) {
-                uint32_t w[16];
+                uint32_t w[16], rest[16];
                 f32x2 y[16];
                 lt_load32(t_dp + part * 32 + lanes, y);
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     const float2 f = unpack_f32x2(mul2(x[i], add2(y[i], d2)));
                     w[i] = lt_pack<T>(f.x, f.y);
+                    if constexpr (TWO) {
+                        const float2 hi = lt_unpack<T>(w[i]);
+                        rest[i] = lt_pack<T>(f.x - hi.x, f.y - hi.y);
+                    }
                 }
                 if ((first + j + 1) * W > seen_all) {          // behind the row's keys; all of a single one
                     const int keep = seen == 1 ? 0 : seen - (first + j) * W - part * 32;
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) w[i] &= (2 * i < keep ? 0xffffu : 0u) | (2 * i + 1 < keep ? 0xffff0000u : 0u);
+                    for (int i = 0; i < 16; ++i) {
+                        const uint32_t mask = (2 * i < keep ? 0xffffu : 0u) | (2 * i + 1 < keep ? 0xffff0000u : 0u);
+                        w[i] &= mask;
+                        if constexpr (TWO) rest[i] &= mask;
+                    }
                 }
                 tmem_st16(t_s, w);
+                if constexpr (TWO) tmem_st16(t_s + 16, rest);
                 tc_wait_st();
             }
             tc_fence_before();
@@ -611,7 +627,7 @@ attention_tc_grad_key_kernel(const __grid_constant__ CUtensorMap map_q, const __
     if (warp == 0) tmem_dealloc(tmem, S::kColumns);
 }
 
-template <typename T, int DP, int W, bool KEYS, bool CAUSAL>
+template <typename T, int DP, int W, bool KEYS, bool CAUSAL, bool TWO>
 static int ab_run(const AtArgs &a) {
     using S = AbShape<DP, W>;
     const int G = a.H / a.K;
@@ -624,7 +640,7 @@ static int ab_run(const AtArgs &a) {
         !at_map(&mv, a.v, a.N, a.K, a.D, 1, keys) || !at_map(&mg, a.grad, a.M, a.H, a.D, P, tokens))
         return SPCONV_ERR_CUDA;
     static std::atomic<uint64_t> done;
-    auto kern = KEYS ? attention_tc_grad_key_kernel<T, DP, W, CAUSAL> : attention_tc_grad_query_kernel<T, DP, W, CAUSAL>;
+    auto kern = KEYS ? attention_tc_grad_key_kernel<T, DP, W, CAUSAL> : attention_tc_grad_query_kernel<T, DP, W, CAUSAL, TWO>;
     // padded so that no more CTAs share an SM than its TMEM columns serve
     constexpr int need = KEYS ? AkShape<DP, W>::kSmem : AqShape<DP, W>::kSmem, least = S::kPerSm == 2 ? 80 * 1024 : 120 * 1024;
     constexpr int smem = need > least ? need : least;
@@ -634,17 +650,21 @@ static int ab_run(const AtArgs &a) {
     return check_launch(KEYS ? "attention_tc_grad_key_kernel" : "attention_tc_grad_query_kernel");
 }
 
-template <typename T, bool KEYS>
+template <typename T, bool KEYS, bool CAUSAL>
 static int ab_size(const AtArgs &a) {
-    if (a.causal) return a.D <= 64 ? ab_run<T, 64, 64, KEYS, true>(a) : ab_run<T, 128, 128, KEYS, true>(a);
-    return a.D <= 64 ? ab_run<T, 64, 64, KEYS, false>(a) : ab_run<T, 128, 128, KEYS, false>(a);
+    if (!KEYS && a.D <= 32) return ab_run<T, 64, 64, KEYS, CAUSAL, !KEYS>(a);
+    return a.D <= 64 ? ab_run<T, 64, 64, KEYS, CAUSAL, false>(a) : ab_run<T, 128, 128, KEYS, CAUSAL, false>(a);
+}
+template <typename T, bool KEYS>
+static int ab_causal(const AtArgs &a) {
+    return a.causal ? ab_size<T, KEYS, true>(a) : ab_size<T, KEYS, false>(a);
 }
 
 int launch_at_tc_grad_query(const AtArgs &a) {
-    return a.dtype == SPCONV_F16 ? ab_size<__half, false>(a) : ab_size<__nv_bfloat16, false>(a);
+    return a.dtype == SPCONV_F16 ? ab_causal<__half, false>(a) : ab_causal<__nv_bfloat16, false>(a);
 }
 int launch_at_tc_grad_key(const AtArgs &a) {
-    return a.dtype == SPCONV_F16 ? ab_size<__half, true>(a) : ab_size<__nv_bfloat16, true>(a);
+    return a.dtype == SPCONV_F16 ? ab_causal<__half, true>(a) : ab_causal<__nv_bfloat16, true>(a);
 }
 
 }  // namespace spconv
