@@ -160,7 +160,7 @@ __device__ __forceinline__ void at_value_peaks(const AtArgs &a, int64_t parts) {
             uint4 x[B];
 #pragma unroll
             for (int k = 0; k < B; ++k) {
-                const unsigned past = (unsigned)(head + 4 * k) / (unsigned)a.K;          // 64-bit quotients cost four times as much
+                const unsigned past = (unsigned)(head + 4 * k) / (unsigned)a.K;          // (32 bits are enough)
                 x[k] = make_uint4(0, 0, 0, 0);
                 if (part + 4 * k + group < all)
                     x[k] = __ldg((const uint4 *)((const __half *)a.v.p + (row + past) * a.v.row + (head + 4 * k - (int64_t)past * a.K) * a.v.head + d));

@@ -266,7 +266,7 @@ attention_tc_grad_query_kernel(const __grid_constant__ CUtensorMap map_q, const 
         const int seen_all = __reduce_min_sync(0xffffffffu, mine ? seen : m);
         const int64_t at = (int64_t)(s.q0 + token) * a.H + head0 + (row & (P - 1));
         const float lse = mine ? a.lse[at] : INFINITY, delta = mine ? a.delta[at] : 0.f;
-        const int lift = at_lift(a, s.b);                                 // p, and so ds, comes times 2^lift
+        const int lift = at_lift(a, s.b);                            // p, and so ds, comes times 2^lift
         const f32x2 c2 = pack_f32x2(a.c, a.c), l2 = pack_f32x2(lift - lse, lift - lse), d2 = pack_f32x2(-delta, -delta);
         bool ok = true;
         for (int j = 0; j < tiles; ++j) {
